@@ -177,7 +177,7 @@ def run(st):
     total = e.sum(dim=1, keepdim=True)
     valid = y != _IGNORE
     col = torch.where(valid, y, torch.zeros_like(y))[:, None]
-    loss = torch.where(valid, (top + torch.log(total) - logits.gather(1, col))[:, 0], torch.zeros_like(top[:, 0]))
+    loss = torch.where(valid, (torch.log(total) + (top - logits.gather(1, col)))[:, 0], torch.zeros_like(top[:, 0]))
     if op == "ce":
         return loss
     coef = valid.float()[:, None] / valid.sum().clamp(min=1).float()
