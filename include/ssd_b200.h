@@ -338,6 +338,102 @@ typedef struct ssd_sp_fixup_params {
  * src/mamba2_jax/kernels/chunk_scan_fwd.py:108-232 across a segment boundary. */
 int ssd_sp_state_fixup(const ssd_sp_fixup_params_t* p, ssd_stream_t stream);
 
+/* Token embedding, the first step of a language model around the mixer layers:
+ *   out[t,:] = scale * weight[tokens[t],:]
+ * A token outside [0, vocab), or equal to padding_idx, gives a zero row and reads nothing.
+ * Arithmetic is f32; out is rounded once. */
+typedef struct ssd_embedding_params {
+  int64_t num_tokens, vocab, dim;
+  int64_t weight_stride_row;  /* element stride between rows of weight, >= dim */
+  int64_t padding_idx;        /* a token that is dropped; -1 for none */
+  int32_t tokens_int64;       /* nonzero: tokens are int64, else int32 */
+  int32_t weight_dtype, out_dtype; /* ssd_dtype_t */
+  float scale;
+  const void* tokens;         /* (num_tokens,) contiguous */
+  const void* weight;         /* (vocab, dim) */
+  void* out;                  /* (num_tokens, dim) contiguous */
+} ssd_embedding_params_t;
+
+int ssd_embedding(const ssd_embedding_params_t* p, ssd_stream_t stream);
+
+/* Gradient of the embedding with respect to its table, dense:
+ *   out[v,:] (+)= scale * sum over t with tokens[t] = v of grad[t,:]
+ * summed in f32 in an order that the tokens alone decide, so equal calls give equal bits.
+ * accumulate = 0 writes every row of out (zeros where no token names it); accumulate = 1 adds
+ * to out and touches only the rows that are named.  num_tokens may be 0. */
+typedef struct ssd_embedding_grad_params {
+  int64_t num_tokens, vocab, dim;
+  int64_t grad_stride_row, out_stride_row; /* element strides between rows, >= dim */
+  int64_t padding_idx;        /* a token that is dropped; -1 for none */
+  int32_t tokens_int64;
+  int32_t grad_dtype, out_dtype; /* ssd_dtype_t */
+  int32_t accumulate;
+  float scale;
+  const void* tokens;         /* (num_tokens,) contiguous */
+  const void* grad;           /* (num_tokens, dim) */
+  void* out;                  /* (vocab, dim) */
+} ssd_embedding_grad_params_t;
+
+size_t ssd_embedding_grad_workspace_bytes(const ssd_embedding_grad_params_t* p);
+int ssd_embedding_grad(const ssd_embedding_grad_params_t* p, void* workspace, size_t workspace_bytes,
+                       ssd_stream_t stream);
+
+/* How the losses of the tokens are put together. */
+typedef enum ssd_reduction {
+  SSD_REDUCE_NONE = 0,   /* one loss per token */
+  SSD_REDUCE_SUM = 1,
+  SSD_REDUCE_MEAN = 2    /* over the targets that are not ignore_index; 0 if there are none */
+} ssd_reduction_t;
+
+/* Output projection and softmax cross entropy without the logits of the whole batch:
+ *   s = hidden . weight^T;  loss_t = log(sum_v exp(s_tv)) - s_{t,target_t}
+ * and, where grad_hidden or grad_weight is given, the gradients of the reduced loss (of
+ * sum_t grad_loss_t loss_t for SSD_REDUCE_NONE) with respect to hidden and weight.
+ * A target equal to ignore_index has loss 0 and no gradient; any other target outside
+ * [0, vocab) makes its loss NaN (and the gradients it takes part in).
+ * bf16 inputs: products on the tensor cores with f32 accumulation; the gradient of the logits
+ * is rounded once to bf16 as an operand of the products behind it.  f32 inputs: every operand
+ * as two bf16 terms, three products per pair. */
+typedef struct ssd_linear_ce_params {
+  int64_t tokens, vocab, dim;
+  int64_t hidden_stride_row, weight_stride_row; /* element strides between rows, >= dim */
+  int64_t ignore_index;
+  int32_t dtype;              /* ssd_dtype_t of hidden, weight and grad_hidden */
+  int32_t targets_int64;
+  int32_t reduction;          /* ssd_reduction_t */
+  int32_t grad_weight_dtype;  /* ssd_dtype_t */
+  const void* hidden;         /* (tokens, dim) */
+  const void* weight;         /* (vocab, dim) */
+  const void* targets;        /* (tokens,) contiguous, int32 or int64 */
+  const float* grad_loss;     /* (tokens,) for SSD_REDUCE_NONE, else one value; NULL: ones */
+  float* loss;                /* (tokens,) for SSD_REDUCE_NONE, else one value */
+  float* lse;                 /* (tokens,) log(sum exp) of each row (0 where ignored), or NULL */
+  void* grad_hidden;          /* (tokens, dim) contiguous, or NULL */
+  void* grad_weight;          /* (vocab, dim) contiguous, or NULL */
+} ssd_linear_ce_params_t;
+
+/* The workspace starts with the device status word (see ssd_status_copy_async). */
+size_t ssd_linear_cross_entropy_workspace_bytes(const ssd_linear_ce_params_t* p);
+int ssd_linear_cross_entropy(const ssd_linear_ce_params_t* p, void* workspace, size_t workspace_bytes,
+                             ssd_stream_t stream);
+
+/* One tensor of a gradient list. */
+typedef struct ssd_grad_tensor {
+  const void* grad;           /* numel contiguous values */
+  void* out;                  /* where the scaled values go (== grad: in place); unused for the norm alone */
+  int64_t numel;              /* 0 is allowed */
+  int32_t grad_dtype, out_dtype; /* ssd_dtype_t */
+} ssd_grad_tensor_t;
+
+/* Norm over all tensors of a list and the clipped gradients:
+ *   norm = sqrt(sum of all squares);  out = min(1, max_norm / (norm + eps)) * grad
+ * The list is in host memory and read during the call only.  Sums are f64, in a fixed order.
+ * scale = 0: the norm alone.  A NaN norm gives NaN gradients, an infinite one zero (and NaN
+ * where the gradient itself is infinite). */
+size_t ssd_clip_grad_norm_workspace_bytes(const ssd_grad_tensor_t* tensors, int64_t count);
+int ssd_clip_grad_norm(const ssd_grad_tensor_t* tensors, int64_t count, float max_norm, float eps, int32_t scale,
+                       float* norm, void* workspace, size_t workspace_bytes, ssd_stream_t stream);
+
 /* Thread-local description of the last failure on this host thread ("" if none). */
 const char* ssd_last_error(void);
 

@@ -498,4 +498,120 @@ int ssd_sp_state_fixup(const ssd_sp_fixup_params_t* p, ssd_stream_t stream) {
   return cuda_status(ssd::launch_sp_fixup(p, (cudaStream_t)stream), "sp_state_fixup");
 }
 
+int ssd_embedding(const ssd_embedding_params_t* p, ssd_stream_t stream) {
+  g_err[0] = 0;
+  if (!p) return fail(SSD_ERR_INVALID_ARG, "params is NULL");
+  if (p->num_tokens <= 0 || p->vocab <= 0 || p->dim <= 0) return fail(SSD_ERR_INVALID_ARG, "dims must be positive");
+  if (p->num_tokens > INT32_MAX || p->vocab > INT32_MAX || p->dim > INT32_MAX)
+    return fail(SSD_ERR_UNSUPPORTED, "dims must be below 2^31");
+  if (p->weight_stride_row < p->dim) return fail(SSD_ERR_INVALID_ARG, "row strides must be at least dim");
+  if (!dtype_ok(p->weight_dtype) || !dtype_ok(p->out_dtype)) return fail(SSD_ERR_INVALID_ARG, "bad dtype enum");
+  if (!p->tokens || !p->weight || !p->out) return fail(SSD_ERR_INVALID_ARG, "tokens, weight and out are required");
+  return cuda_status(ssd::launch_embedding(p, (cudaStream_t)stream), "embedding");
+}
+
+namespace {
+int check_embedding_grad(const ssd_embedding_grad_params_t* p) {
+  if (!p) return fail(SSD_ERR_INVALID_ARG, "params is NULL");
+  if (p->num_tokens < 0 || p->vocab <= 0 || p->dim <= 0) return fail(SSD_ERR_INVALID_ARG, "dims must be positive");
+  if (p->num_tokens > INT32_MAX || p->vocab > INT32_MAX || p->dim > INT32_MAX)
+    return fail(SSD_ERR_UNSUPPORTED, "dims must be below 2^31");
+  return SSD_OK;
+}
+
+int check_linear_ce(const ssd_linear_ce_params_t* p) {
+  if (!p) return fail(SSD_ERR_INVALID_ARG, "params is NULL");
+  if (p->tokens <= 0 || p->vocab <= 0 || p->dim <= 0) return fail(SSD_ERR_INVALID_ARG, "dims must be positive");
+  // tile coordinates are 32-bit, and a tile may reach 256 past the end
+  if (p->tokens > INT32_MAX - 256 || p->vocab > INT32_MAX - 256 || p->dim > INT32_MAX - 256)
+    return fail(SSD_ERR_UNSUPPORTED, "dims must be below 2^31 - 256");
+  if (p->hidden_stride_row < p->dim || p->weight_stride_row < p->dim)
+    return fail(SSD_ERR_INVALID_ARG, "row strides must be at least dim");
+  if (!dtype_ok(p->dtype) || !dtype_ok(p->grad_weight_dtype)) return fail(SSD_ERR_INVALID_ARG, "bad dtype enum");
+  if (p->reduction < SSD_REDUCE_NONE || p->reduction > SSD_REDUCE_MEAN) return fail(SSD_ERR_INVALID_ARG, "bad reduction");
+  return SSD_OK;
+}
+}  // namespace
+
+size_t ssd_embedding_grad_workspace_bytes(const ssd_embedding_grad_params_t* p) {
+  g_err[0] = 0;
+  if (check_embedding_grad(p)) return 0;
+  return ssd::embedding_grad_workspace(p->num_tokens, p->dim);
+}
+
+int ssd_embedding_grad(const ssd_embedding_grad_params_t* p, void* workspace, size_t workspace_bytes,
+                       ssd_stream_t stream) {
+  g_err[0] = 0;
+  if (int s = check_embedding_grad(p)) return s;
+  if (p->grad_stride_row < p->dim || p->out_stride_row < p->dim)
+    return fail(SSD_ERR_INVALID_ARG, "row strides must be at least dim");
+  if (!dtype_ok(p->grad_dtype) || !dtype_ok(p->out_dtype)) return fail(SSD_ERR_INVALID_ARG, "bad dtype enum");
+  if (!p->out || (p->num_tokens && (!p->tokens || !p->grad)))
+    return fail(SSD_ERR_INVALID_ARG, "tokens, grad and out are required");
+  const size_t need = ssd::embedding_grad_workspace(p->num_tokens, p->dim);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(SSD_ERR_WORKSPACE, "workspace too small: %zu bytes, need %zu", workspace_bytes, need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(SSD_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
+  return cuda_status(ssd::launch_embedding_grad(p, workspace, (cudaStream_t)stream), "embedding_grad");
+}
+
+size_t ssd_linear_cross_entropy_workspace_bytes(const ssd_linear_ce_params_t* p) {
+  g_err[0] = 0;
+  if (check_linear_ce(p)) return 0;
+  return ssd::linear_ce_workspace(p);
+}
+
+int ssd_linear_cross_entropy(const ssd_linear_ce_params_t* p, void* workspace, size_t workspace_bytes,
+                             ssd_stream_t stream) {
+  g_err[0] = 0;
+  if (int s = check_linear_ce(p)) return s;
+  if (!p->hidden || !p->weight || !p->targets || !p->loss)
+    return fail(SSD_ERR_INVALID_ARG, "hidden, weight, targets and loss are required");
+  const size_t need = ssd::linear_ce_workspace(p);
+  if (!workspace || workspace_bytes < need)
+    return fail(SSD_ERR_WORKSPACE, "workspace too small: %zu bytes, need %zu", workspace_bytes, need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(SSD_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
+  const char* at = "linear_cross_entropy";
+  return cuda_status(ssd::launch_linear_ce(p, workspace, (cudaStream_t)stream, &at), at);
+}
+
+namespace {
+int check_grad_list(const ssd_grad_tensor_t* tensors, int64_t count) {
+  if (count < 0 || (count && !tensors)) return fail(SSD_ERR_INVALID_ARG, "bad tensor list");
+  for (int64_t i = 0; i < count; ++i) {
+    const ssd_grad_tensor_t& t = tensors[i];
+    if (t.numel < 0 || (t.numel && !t.grad)) return fail(SSD_ERR_INVALID_ARG, "tensor %lld: null or negative size", (long long)i);
+    if (t.numel > ((int64_t)1 << 42)) return fail(SSD_ERR_UNSUPPORTED, "tensor %lld: too large", (long long)i);
+    if (!dtype_ok(t.grad_dtype) || !dtype_ok(t.out_dtype)) return fail(SSD_ERR_INVALID_ARG, "tensor %lld: bad dtype enum", (long long)i);
+  }
+  return SSD_OK;
+}
+}  // namespace
+
+size_t ssd_clip_grad_norm_workspace_bytes(const ssd_grad_tensor_t* tensors, int64_t count) {
+  g_err[0] = 0;
+  if (check_grad_list(tensors, count)) return 0;
+  return std::max<size_t>(8, (size_t)ssd::grad_clip_partials(tensors, count) * 8);
+}
+
+int ssd_clip_grad_norm(const ssd_grad_tensor_t* tensors, int64_t count, float max_norm, float eps, int32_t scale,
+                       float* norm, void* workspace, size_t workspace_bytes, ssd_stream_t stream) {
+  g_err[0] = 0;
+  if (int s = check_grad_list(tensors, count)) return s;
+  if (!norm) return fail(SSD_ERR_INVALID_ARG, "norm is required");
+  if (!(max_norm >= 0.f) || !(eps >= 0.f)) return fail(SSD_ERR_INVALID_ARG, "max_norm and eps must be non-negative");
+  if (scale)
+    for (int64_t i = 0; i < count; ++i) {
+      if (tensors[i].numel && !tensors[i].out) return fail(SSD_ERR_INVALID_ARG, "tensor %lld: out is required", (long long)i);
+      if (tensors[i].out == tensors[i].grad && tensors[i].grad_dtype != tensors[i].out_dtype && tensors[i].numel)
+        return fail(SSD_ERR_INVALID_ARG, "tensor %lld: in place needs one dtype", (long long)i);
+    }
+  const size_t need = (size_t)ssd::grad_clip_partials(tensors, count) * 8;
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(SSD_ERR_WORKSPACE, "workspace too small: %zu bytes, need %zu", workspace_bytes, need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 8) return fail(SSD_ERR_ALIGNMENT, "workspace must be 8-byte aligned");
+  return cuda_status(ssd::launch_grad_clip(tensors, count, max_norm, eps, scale != 0, norm, workspace, (cudaStream_t)stream),
+                     "clip_grad_norm");
+}
+
 }  // extern "C"

@@ -38,6 +38,16 @@ cudaError_t launch_rms_norm_gated(const ssd_rms_norm_params_t* p, cudaStream_t s
 cudaError_t launch_sp_fixup(const ssd_sp_fixup_params_t* p, cudaStream_t st);
 size_t sp_fixup_smem_bytes(int64_t P, int64_t N);
 
+cudaError_t launch_embedding(const ssd_embedding_params_t* p, cudaStream_t st);
+size_t embedding_grad_workspace(int64_t num_tokens, int64_t dim);
+cudaError_t launch_embedding_grad(const ssd_embedding_grad_params_t* p, void* workspace, cudaStream_t st);
+size_t linear_ce_workspace(const ssd_linear_ce_params_t* p);
+// `at` names the step that failed.
+cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, cudaStream_t st, const char** at);
+int64_t grad_clip_partials(const ssd_grad_tensor_t* list, int64_t count);
+cudaError_t launch_grad_clip(const ssd_grad_tensor_t* list, int64_t count, float max_norm, float eps, bool scale,
+                             float* norm, void* workspace, cudaStream_t st);
+
 // Set the thread-local message ssd_last_error() returns.
 void set_last_error(const char* msg);
 

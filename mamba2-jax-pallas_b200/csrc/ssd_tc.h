@@ -1,5 +1,6 @@
 // Tensor-core (tcgen05) pipeline for bf16 inputs: host-side interface.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 
@@ -20,5 +21,9 @@ int tc_combined_fwd(const ssd_fwd_params_t* p, unsigned* status, void* workspace
 // The sequence-parallel fix-up on the tensor cores (bf16 C, P = 64, N = 128 or 256).
 bool tc_sp_fixup_supported(const ssd_sp_fixup_params_t* p);
 int tc_sp_fixup(const ssd_sp_fixup_params_t* p, cudaStream_t st);
+
+// 2-D tensor map over rows of `inner` bf16 values, `stride` bytes apart (a multiple of 16),
+// with a 64-value (128-byte, swizzled) x box_rows box.  False if the driver refuses it.
+bool tc_map_2d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows, uint64_t stride, uint32_t box_rows);
 
 }  // namespace ssd

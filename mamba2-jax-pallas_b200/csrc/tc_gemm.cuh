@@ -1,0 +1,332 @@
+// Tensor-core GEMM core for the language-model head: D = A B^T (+ epilogue), bf16 operands,
+// f32 accumulators in TMEM.
+//
+// One persistent CTA per SM, or a pair of CTAs per two SMs (CG = 2: tcgen05 cta_group::2, one
+// 256 x 256 tile per pair).  The pair halves what each SM fetches of B, in shared memory and
+// from L2: a 128 x 256 tile per SM needs 48 KB per 64-wide K block, which at the tensor
+// pipe's rate is 16 TB/s over the GPU; a pair needs 32 KB per SM.  Warps:
+//   0     TMA producer: A and B boxes into a ring of shared-memory stages
+//   1     MMA issuer (the pair's first CTA only issues): four K = 16 MMAs per stage
+//   2..9  epilogue: warp w reads the TMEM lanes of quadrant w % 4, column half (w - 2) / 4
+// Two accumulators (2 x 256 TMEM columns) let the epilogue of a tile overlap the next tile's
+// MMAs.  Operands are K-major (the reduced dimension contiguous in memory) or MN-major (the
+// other one contiguous), so no operand is ever transposed in memory.
+//
+// f32 operands come as two bf16 planes, v = hi + lo, and the K loop runs over the plane pairs
+// hi*lo, lo*hi, hi*hi (the split of Henry, Tang and Heinecke, ARITH 2019, as in ssd_x3.cu).
+//
+// Every wait is bounded; one that gives up sets the status word and the CTA drains and ends.
+#pragma once
+#include <cuda.h>
+
+#include "common.cuh"
+#include "ptx_sm100.cuh"
+
+namespace ssd {
+namespace gemm {
+
+constexpr int BK = 64;                    // one 128-byte swizzled row
+constexpr int BN = 256;                   // columns of a tile
+constexpr int BM = 128;                   // rows of a CTA's part of a tile
+constexpr int EPI_WARPS = 8;
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr long long WAIT_CYCLES = 4000000000LL;   // about 2 s at the boost clock
+
+template <int CG>
+struct Shape {
+  static constexpr int STAGES = CG == 2 ? 6 : 4;
+  static constexpr int A_BYTES = BM * BK * 2;
+  static constexpr int B_BYTES = BN / CG * BK * 2;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024;   // + alignment
+};
+
+struct Ctl {
+  uint64_t full[6], empty[6], acc_full[2], acc_empty[2], drain;
+  uint32_t tmem;
+  volatile uint32_t abort;
+};
+
+// What the kernel runs over.  Tiles are numbered m fastest or n fastest; a tile's K range is
+// split into `splits` parts, each its own unit of work.
+// A dimension whose size only the device knows (rows that count) is `limit`: rows from
+// `limit_from` on, at most `rows`; it bounds the m tiles, or the K blocks with limit_k.
+struct Problem {
+  CUtensorMap a[2], b[2];                 // planes hi and lo (lo unused for bf16 operands)
+  const int* limit;
+  int limit_from, rows, limit_k;
+  int m_tiles, n_tiles, splits;           // m tiles of CG * 128 rows
+  int k_blocks;                           // of 64
+  int passes;                             // 1, or 3 for split f32 operands
+  int m_fastest;
+  unsigned* status;
+};
+
+struct Tile {
+  int m, n, split, k0, k1;                // k0 == k1: nothing to add, the accumulator is not written
+};
+
+// Rows that count, of those that the launch was made for.
+__device__ __forceinline__ int live_rows(const Problem& p) { return min(max(*p.limit - p.limit_from, 0), p.rows); }
+
+__device__ __forceinline__ Tile tile_at(const Problem& p, int m_tiles, int k_blocks, int64_t u) {
+  Tile t;
+  const int64_t per = (int64_t)m_tiles * p.n_tiles;
+  t.split = (int)(u / per);
+  const int64_t r = u - t.split * per;
+  if (p.m_fastest) {
+    t.n = (int)(r / m_tiles);
+    t.m = (int)(r - (int64_t)t.n * m_tiles);
+  } else {
+    t.m = (int)(r / p.n_tiles);
+    t.n = (int)(r - (int64_t)t.m * p.n_tiles);
+  }
+  t.k0 = (int)((int64_t)k_blocks * t.split / p.splits);
+  t.k1 = (int)((int64_t)k_blocks * (t.split + 1) / p.splits);
+  return t;
+}
+
+__device__ __forceinline__ bool wait(Ctl* c, uint64_t* bar, uint32_t parity, unsigned* status, int id) {
+  if (ptx::mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!ptx::mbar_try_wait(bar, parity)) {
+    if (c->abort) return false;
+    if (clock64() - t0 > WAIT_CYCLES) {
+      atomicCAS(status, 0u, (unsigned)(0x100 | id));
+      c->abort = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
+// ---- the pair's forms of the PTX wrappers ------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// shared::cluster address of the same variable in CTA `rank` of the cluster
+__device__ __forceinline__ uint32_t map_rank(uint32_t saddr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+  else
+    ptx::mma_f16(d, a, b, idesc, acc);
+}
+
+// Arrive on `bar` (of both CTAs of a pair) once this thread's MMAs have completed.
+template <int CG>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            ptx::smem_u32(bar)), "h"((uint16_t)3) : "memory");
+  else
+    ptx::mma_commit(bar);
+}
+
+template <int CG>
+__device__ __forceinline__ void tmem_alloc_all(uint32_t* dst) {
+  if constexpr (CG == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ptx::smem_u32(dst)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    ptx::tmem_alloc(dst, 512);
+    ptx::tmem_relinquish();
+  }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_free_all(uint32_t t) {
+  if constexpr (CG == 2)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(512) : "memory");
+  else
+    ptx::tmem_dealloc(t, 512);
+}
+
+// The kernel's body.  epi(tile, tmem address of the accumulator's first column for this warp's
+// quadrant, quadrant, column half, first row of this CTA's part, rows that count) runs on each
+// epilogue warp; it ends with its TMEM reads complete.
+template <int CG, bool A_MN, bool B_MN, typename Epi>
+__device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c, Epi&& epi) {
+  using S = Shape<CG>;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cluster_rank() : 0;
+  const int live = live_rows(p);
+  const int m_tiles = p.limit_k ? p.m_tiles : (live + BM * CG - 1) / (BM * CG);
+  const int k_blocks = p.limit_k ? (live + BK - 1) / BK : p.k_blocks;
+  const int64_t unit0 = blockIdx.x / CG, units = (int64_t)m_tiles * p.n_tiles * p.splits, step = gridDim.x / CG;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::STAGES; ++i) {
+      ptx::mbar_init(&c->full[i], 1);
+      ptx::mbar_init(&c->empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(&c->acc_full[i], 1);
+      ptx::mbar_init(&c->acc_empty[i], EPI_WARPS * CG);
+    }
+    ptx::mbar_init(&c->drain, 1);
+    c->abort = 0;
+    ptx::fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc_all<CG>(&c->tmem);
+  ptx::tc_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync_all();
+  ptx::tc_fence_after();
+  const uint32_t tmem = c->tmem;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int i = 0; i < (p.passes == 3 ? 2 : 1); ++i) {
+        ptx::prefetch_tmap(&p.a[i]);
+        ptx::prefetch_tmap(&p.b[i]);
+      }
+      uint32_t it = 0;
+      bool ok = true;
+      for (int64_t u = unit0; ok && u < units; u += step) {
+        const Tile t = tile_at(p, m_tiles, k_blocks, u);
+        const int m0 = (t.m * CG + (int)rank) * BM, n0 = t.n * BN + (int)rank * (BN / CG);
+        for (int ps = 0; ok && ps < p.passes; ++ps) {
+          // pass order hi*lo, lo*hi, hi*hi: the small products first
+          const CUtensorMap* ma = &p.a[p.passes == 3 && ps == 1];
+          const CUtensorMap* mb = &p.b[p.passes == 3 && ps == 0];
+          for (int kb = t.k0; kb < t.k1; ++kb, ++it) {
+            const int s = it % S::STAGES;
+            if (it >= S::STAGES && !wait(c, &c->empty[s], ((it / S::STAGES) - 1) & 1, p.status, 1)) {
+              ok = false;
+              break;
+            }
+            const uint32_t sa = ptx::smem_u32(smem + s * S::STAGE_BYTES), sb = sa + S::A_BYTES;
+            uint32_t bar = ptx::smem_u32(&c->full[s]);
+            // the pair's first CTA counts the bytes of both
+            if (rank == 0) ptx::mbar_arrive_expect_tx(&c->full[s], CG * S::STAGE_BYTES);
+            if constexpr (CG == 2) bar = map_rank(bar, 0);
+            const int k = kb * BK;
+            if constexpr (A_MN) {
+              for (int i = 0; i < BM / 64; ++i) tma_load_2d<CG>(sa + i * 8192, ma, bar, m0 + 64 * i, k);
+            } else {
+              tma_load_2d<CG>(sa, ma, bar, k, m0);
+            }
+            if constexpr (B_MN) {
+              for (int i = 0; i < BN / CG / 64; ++i) tma_load_2d<CG>(sb + i * 8192, mb, bar, n0 + 64 * i, k);
+            } else {
+              tma_load_2d<CG>(sb, mb, bar, k, n0);
+            }
+          }
+        }
+      }
+      // a wait gave up: let the loads that are still in flight land before the CTA ends
+      if (!ok) {
+        const long long t0 = clock64();
+        for (uint32_t j = it > S::STAGES ? it - S::STAGES : 0; rank == 0 && j < it; ++j)
+          while (!ptx::mbar_try_wait(&c->full[j % S::STAGES], (j / S::STAGES) & 1) && clock64() - t0 < WAIT_CYCLES) {
+          }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t ID = ptx::idesc_bf16_f32(BM * CG, BN, A_MN, B_MN);
+      uint32_t it = 0, n = 0;
+      bool ok = true;
+      for (int64_t u = unit0; ok && u < units; u += step, ++n) {
+        const Tile t = tile_at(p, m_tiles, k_blocks, u);
+        const int acc = n & 1;
+        if (n >= 2 && !wait(c, &c->acc_empty[acc], ((n >> 1) - 1) & 1, p.status, 2)) break;
+        ptx::tc_fence_after();
+        const uint32_t d = tmem + acc * BN;
+        const int steps = p.passes * (t.k1 - t.k0);
+        for (int j = 0; j < steps; ++j, ++it) {
+          const int s = it % S::STAGES;
+          if (!wait(c, &c->full[s], (it / S::STAGES) & 1, p.status, 3)) {
+            ok = false;
+            break;
+          }
+          ptx::tc_fence_after();
+          const uint32_t sa = ptx::smem_u32(smem + s * S::STAGE_BYTES), sb = sa + S::A_BYTES;
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k) {
+            const uint64_t da = A_MN ? ptx::sdesc_sw128(sa + k * 2048, 8192, 1024) : ptx::sdesc_sw128(sa + k * 32, 16, 1024);
+            const uint64_t db = B_MN ? ptx::sdesc_sw128(sb + k * 2048, 8192, 1024) : ptx::sdesc_sw128(sb + k * 32, 16, 1024);
+            mma<CG>(d, da, db, ID, (j > 0 || k > 0) ? 1u : 0u);
+          }
+          commit<CG>(&c->empty[s]);
+        }
+        if (!ok) break;
+        commit<CG>(&c->acc_full[acc]);
+      }
+      if (!ok) {   // let the MMAs in flight finish
+        ptx::tc_fence_before();
+        if constexpr (CG == 2)
+          asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(ptx::smem_u32(&c->drain)) : "memory");
+        else
+          ptx::mma_commit(&c->drain);
+        const long long t0 = clock64();
+        while (!ptx::mbar_try_wait(&c->drain, 0) && clock64() - t0 < WAIT_CYCLES) {
+        }
+      }
+    }
+  } else {
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    uint32_t n = 0;
+    for (int64_t u = unit0; u < units; u += step, ++n) {
+      const Tile t = tile_at(p, m_tiles, k_blocks, u);
+      const int acc = n & 1;
+      // one lane waits for the warp, so that the warp stays converged for its TMEM loads
+      int ok = 0;
+      if (lane == 0) ok = wait(c, &c->acc_full[acc], (n >> 1) & 1, p.status, 4);
+      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+      ptx::tc_fence_after();
+      epi(t, tmem + acc * BN + ((uint32_t)(32 * quad) << 16), quad, half, (t.m * CG + (int)rank) * BM, live);
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CG == 2)
+          arrive_remote(map_rank(ptx::smem_u32(&c->acc_empty[acc]), 0));
+        else
+          ptx::mbar_arrive(&c->acc_empty[acc]);
+      }
+    }
+  }
+  __syncwarp();
+  ptx::tc_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync_all();   // no CTA leaves while its peer may still signal it
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    tmem_free_all<CG>(tmem);
+  }
+  if constexpr (CG == 2) cluster_sync_all();
+}
+
+}  // namespace gemm
+}  // namespace ssd

@@ -37,7 +37,10 @@ EXPORTED = ["ssd_combined_workspace_bytes", "ssd_combined_uses_tensor_cores",
             "ssd_chunk_state_fwd", "ssd_state_passing_fwd", "ssd_bmm_chunk_fwd",
             "ssd_chunk_scan_fwd", "ssd_chunk_state_varlen_fwd", "ssd_selective_state_update",
             "ssd_causal_conv1d_fwd", "ssd_causal_conv1d_update", "ssd_rms_norm_gated", "ssd_sp_state_fixup", "ssd_status_copy_async", "ssd_status_decode",
-            "ssd_last_error", "ssd_abi_version", "ssd_set_fp32_stage_path"]
+            "ssd_last_error", "ssd_abi_version", "ssd_set_fp32_stage_path",
+            "ssd_embedding", "ssd_embedding_grad", "ssd_embedding_grad_workspace_bytes",
+            "ssd_linear_cross_entropy", "ssd_linear_cross_entropy_workspace_bytes",
+            "ssd_clip_grad_norm", "ssd_clip_grad_norm_workspace_bytes"]
 
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -99,6 +102,34 @@ class SpFixupParams(ctypes.Structure):
                 ("out", _vp), ("final_states", _vp)]
 
 
+class EmbeddingParams(ctypes.Structure):
+    _fields_ = [("num_tokens", _i64), ("vocab", _i64), ("dim", _i64), ("weight_stride_row", _i64),
+                ("padding_idx", _i64), ("tokens_int64", _i32), ("weight_dtype", _i32), ("out_dtype", _i32),
+                ("scale", _f32), ("tokens", _vp), ("weight", _vp), ("out", _vp)]
+
+
+class EmbeddingGradParams(ctypes.Structure):
+    _fields_ = [("num_tokens", _i64), ("vocab", _i64), ("dim", _i64), ("grad_stride_row", _i64),
+                ("out_stride_row", _i64), ("padding_idx", _i64), ("tokens_int64", _i32), ("grad_dtype", _i32),
+                ("out_dtype", _i32), ("accumulate", _i32), ("scale", _f32),
+                ("tokens", _vp), ("grad", _vp), ("out", _vp)]
+
+
+class LinearCeParams(ctypes.Structure):
+    _fields_ = [("tokens", _i64), ("vocab", _i64), ("dim", _i64), ("hidden_stride_row", _i64),
+                ("weight_stride_row", _i64), ("ignore_index", _i64), ("dtype", _i32), ("targets_int64", _i32),
+                ("reduction", _i32), ("grad_weight_dtype", _i32),
+                ("hidden", _vp), ("weight", _vp), ("targets", _vp), ("grad_loss", _vp),
+                ("loss", _vp), ("lse", _vp), ("grad_hidden", _vp), ("grad_weight", _vp)]
+
+
+class GradTensor(ctypes.Structure):
+    _fields_ = [("grad", _vp), ("out", _vp), ("numel", _i64), ("grad_dtype", _i32), ("out_dtype", _i32)]
+
+
+REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+
+
 class SsdError(RuntimeError):
     """A non-zero ssd_status_t from the library."""
 
@@ -149,8 +180,17 @@ def load() -> ctypes.CDLL:
     lib.ssd_status_copy_async.argtypes = [_vp, _vp, _vp]
     lib.ssd_status_decode.argtypes = [ctypes.c_uint32]
     lib.ssd_set_fp32_stage_path.argtypes = [_i32]
+    lib.ssd_embedding.argtypes = [P(EmbeddingParams), _vp]
+    lib.ssd_embedding_grad.argtypes = [P(EmbeddingGradParams), _vp, ctypes.c_size_t, _vp]
+    lib.ssd_linear_cross_entropy.argtypes = [P(LinearCeParams), _vp, ctypes.c_size_t, _vp]
+    lib.ssd_clip_grad_norm.argtypes = [_vp, _i64, _f32, _f32, _i32, _vp, _vp, ctypes.c_size_t, _vp]
+    lib.ssd_clip_grad_norm_workspace_bytes.argtypes = [_vp, _i64]
+    lib.ssd_embedding_grad_workspace_bytes.argtypes = [P(EmbeddingGradParams)]
+    lib.ssd_linear_cross_entropy_workspace_bytes.argtypes = [P(LinearCeParams)]
     for name in EXPORTED:
-        if name not in ("ssd_last_error", "ssd_abi_version", "ssd_combined_workspace_bytes"):
+        if name.endswith("_workspace_bytes"):
+            getattr(lib, name).restype = ctypes.c_size_t
+        elif name not in ("ssd_last_error", "ssd_abi_version"):
             getattr(lib, name).restype = ctypes.c_int
     if lib.ssd_abi_version() != ABI_VERSION:
         raise RuntimeError(f"libssd_b200.so has ABI version {lib.ssd_abi_version()}, these bindings "
@@ -233,6 +273,28 @@ def dev(t, name: str, dtype=None):
 
 def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+def index_list(t, name: str) -> torch.Tensor:
+    """Token ids or targets: a contiguous CUDA tensor of int32 or int64."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{name} must be int32 or int64, not {t.dtype}")
+    return dev(t, name)
+
+
+def rows2d(t: torch.Tensor, width: int) -> torch.Tensor:
+    """(rows, width) view with a contiguous last axis and one row stride, else a copy."""
+    t2 = t.reshape(-1, width)
+    if (width > 1 and t2.stride(1) != 1) or (t2.shape[0] > 1 and t2.stride(0) < width):
+        t2 = t2.contiguous()
+    return t2
+
+
+def row_stride(t2: torch.Tensor) -> int:
+    """Element stride between rows of a rows2d tensor (its width where there is one row)."""
+    return t2.stride(0) if t2.shape[0] > 1 else t2.shape[1]
 
 
 def stream_of(t: torch.Tensor) -> int:

@@ -1,0 +1,107 @@
+"""Token embedding and its gradient: the first step of a language model around the mixer layers."""
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+
+_DTYPES = (torch.float32, torch.bfloat16)
+
+
+def _pad(padding_idx, vocab: int) -> int:
+    if padding_idx is None:
+        return -1
+    padding_idx = int(padding_idx)
+    if not 0 <= padding_idx < vocab:
+        raise ValueError(f"padding_idx {padding_idx} is outside [0, {vocab})")
+    return padding_idx
+
+
+def embedding(tokens, weight, scale: float = 1.0, *, padding_idx=None, out_dtype=None):
+    """``scale * weight[tokens]``, computed in float32 and rounded once.
+
+    tokens (...) int32 or int64; weight (vocab, dim) float32 or bfloat16.  Returns (..., dim)
+    in ``out_dtype`` (default: weight's dtype).  A token outside [0, vocab) or equal to
+    ``padding_idx`` gives a zero row.
+    """
+    ids = _lib.index_list(tokens, "tokens")
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        raise ValueError("weight must be a (vocab, dim) tensor")
+    if not weight.is_cuda:
+        raise ValueError("weight must be a CUDA tensor (no CPU path)")
+    if ids.device != weight.device:
+        raise ValueError("tokens and weight must be on one device")
+    vocab, dim = weight.shape
+    if vocab == 0 or dim == 0:
+        raise ValueError("weight must not be empty")
+    _lib.dtype_code(weight)
+    out_dtype = weight.dtype if out_dtype is None else out_dtype
+    if out_dtype not in _DTYPES:
+        raise ValueError("out_dtype must be torch.float32 or torch.bfloat16")
+    w = _lib.rows2d(weight, dim)
+    p = _lib.EmbeddingParams(num_tokens=ids.numel(), vocab=vocab, dim=dim, weight_stride_row=_lib.row_stride(w),
+                             padding_idx=_pad(padding_idx, vocab), tokens_int64=int(ids.dtype == torch.int64),
+                             weight_dtype=_lib.dtype_code(w), scale=float(scale))
+    out = torch.empty((*tokens.shape, dim), device=w.device, dtype=out_dtype)
+    if ids.numel() == 0:
+        return out
+    p.out_dtype = _lib.dtype_code(out)
+    p.tokens, p.weight, p.out = ids.data_ptr(), w.data_ptr(), out.data_ptr()
+    with torch.cuda.device(w.device):
+        _lib.check(_lib.load().ssd_embedding(p, _lib.stream_of(out)))
+    return out
+
+
+def embedding_grad(tokens, grad_out, num_embeddings: int, scale: float = 1.0, *, padding_idx=None, out_dtype=None,
+                   accumulate_into=None):
+    """Gradient of ``embedding`` with respect to its weight: (num_embeddings, dim), dense.
+
+    tokens (...) int32 or int64 and grad_out (..., dim) float32 or bfloat16.  Row v is
+    ``scale`` times the sum of grad_out over the tokens equal to v, summed in float32 by sorted
+    tokens (the same bits in every run) and rounded once to ``out_dtype`` (default: grad_out's
+    dtype).  With ``accumulate_into`` (a float32 or bfloat16 (num_embeddings, dim) tensor, rows
+    contiguous) the sums are added to that tensor, only the named rows are touched, and it is
+    returned: the tied output projection's gradient, or that of an earlier micro-batch.
+    """
+    ids = _lib.index_list(tokens, "tokens")
+    vocab = int(num_embeddings)
+    if vocab <= 0:
+        raise ValueError("num_embeddings must be positive")
+    if not isinstance(grad_out, torch.Tensor) or not grad_out.is_cuda:
+        raise ValueError("grad_out must be a CUDA tensor (no CPU path)")
+    if grad_out.dim() < 1 or tuple(grad_out.shape[:-1]) != tuple(tokens.shape):
+        raise ValueError(f"grad_out {tuple(grad_out.shape)} must be tokens' shape {tuple(tokens.shape)} and one axis more")
+    if ids.device != grad_out.device:
+        raise ValueError("tokens and grad_out must be on one device")
+    dim = grad_out.shape[-1]
+    if dim == 0:
+        raise ValueError("grad_out must not have an empty last axis")
+    _lib.dtype_code(grad_out)
+    g = _lib.rows2d(grad_out, dim)
+    if accumulate_into is not None:
+        out = accumulate_into
+        if out_dtype is not None and out_dtype != out.dtype:
+            raise ValueError("out_dtype is accumulate_into's dtype")
+        if not out.is_cuda or out.device != g.device:
+            raise ValueError("accumulate_into must be on grad_out's device")
+        if tuple(out.shape) != (vocab, dim) or (dim > 1 and out.stride(1) != 1) or (vocab > 1 and out.stride(0) < dim):
+            raise ValueError(f"accumulate_into must be ({vocab}, {dim}) with contiguous rows")
+    else:
+        out_dtype = grad_out.dtype if out_dtype is None else out_dtype
+        if out_dtype not in _DTYPES:
+            raise ValueError("out_dtype must be torch.float32 or torch.bfloat16")
+        out = torch.empty((vocab, dim), device=g.device, dtype=out_dtype)
+    p = _lib.EmbeddingGradParams(num_tokens=ids.numel(), vocab=vocab, dim=dim, grad_stride_row=_lib.row_stride(g),
+                                 out_stride_row=_lib.row_stride(out), padding_idx=_pad(padding_idx, vocab),
+                                 tokens_int64=int(ids.dtype == torch.int64), grad_dtype=_lib.dtype_code(g),
+                                 out_dtype=_lib.dtype_code(out), accumulate=int(accumulate_into is not None),
+                                 scale=float(scale))
+    if accumulate_into is not None and ids.numel() == 0:
+        return out
+    p.tokens, p.grad, p.out = ids.data_ptr(), g.data_ptr(), out.data_ptr()
+    lib = _lib.load()
+    n = lib.ssd_embedding_grad_workspace_bytes(p)
+    ws = torch.empty(max(n, 1), device=g.device, dtype=torch.uint8)
+    with torch.cuda.device(g.device):
+        _lib.check(lib.ssd_embedding_grad(p, ws.data_ptr(), ws.numel(), _lib.stream_of(out)))
+    return out
