@@ -12,11 +12,13 @@
 //              confidence keeps the digits of 1 - p, which a sum with p in it would lose.
 //   gradients  tokens go in chunks whose logits fit a bounded workspace.  The same epilogue also
 //              stores the f32 logits; a row pass forms lse and dl (rounded once, to bf16, for
-//              the tensor pipe); two GEMMs follow.  Keeping f32 logits for the chunk costs 10
+//              the tensor pipe; f32 inputs: two f16); two GEMMs follow.  Keeping f32 logits for the chunk costs 10
 //              bytes of HBM per logit; computing them again would cost 2 D operations, more
 //              from D = 512 on.
-// f32 inputs are split into two bf16 planes, three products per pair (tc_gemm.cuh).
+// f32 inputs are split into two f16 planes, three products per pair (tc_gemm.cuh).
 #include <algorithm>
+
+#include <cuda_fp16.h>
 
 #include "common.cuh"
 #include "ssd_kernels.h"
@@ -29,11 +31,12 @@ namespace {
 using gemm::BM;
 using gemm::BN;
 
-#ifndef CE_PAIR
-#define CE_PAIR 1
-#endif
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr double LN2 = 0.6931471805599453;
+// K blocks summed in TMEM before the sum goes to registers (tc_gemm.cuh), measured over K = 4096:
+// one segment 3.3e-6 off in the loss, 16 blocks 7.7e-7 (2 % slower), 8 blocks 3.6e-7 (4 % slower).
+// bf16 logits take 16; f32 products 8, which leaves 9e-7 in the gradients (16: 1.2e-6).
+constexpr int SEGMENT_BF16 = 16, SEGMENT_F32 = 8;
 constexpr int64_t LOSS_CHUNK = 16384;              // tokens whose statistics are kept at a time
 constexpr int64_t GRAD_BYTES = int64_t(3) << 30;   // logits and dl of a chunk of tokens
 
@@ -46,6 +49,22 @@ __device__ __forceinline__ int64_t target_at(const void* y, int is64, int64_t t)
   return is64 ? __ldg(static_cast<const long long*>(y) + t) : (int64_t)__ldg(static_cast<const int*>(y) + t);
 }
 
+// f32 inputs: the largest finite magnitudes (as the bits of a float, which order like it), and
+// from them the powers of two that bring the planes' largest value to [2^14, 2^15): f16 ends at
+// 65504 below, and two planes keep 22 bits down to 2^-1.
+struct Scales {
+  unsigned x, w, dl;
+};
+
+__device__ __forceinline__ float scale_of(unsigned largest) {
+  const int e = (int)(largest >> 23);                       // biased exponent; 0 also for subnormals
+  return e == 0 ? 1.f : __uint_as_float((unsigned)min(max(127 + 14 + 127 - e, 1), 254) << 23);
+}
+__device__ __forceinline__ unsigned finite_bits(float v) {
+  const unsigned u = __float_as_uint(v) & 0x7fffffffu;
+  return u < 0x7f800000u ? u : 0u;
+}
+
 // Tokens whose target is not ignore_index, in order.  Everything behind works on these rows
 // alone: an ignored token costs no products, and what its row of hidden holds (padding, NaN)
 // cannot reach the others' gradients through a product with zero.
@@ -54,17 +73,27 @@ struct Selected {
   int* index;              // (tokens): row r is token index[r]
   int* target;             // (tokens): its target, or -1 where that is outside [0, vocab)
   float* alpha;            // the factor common to all rows: 1 or 1 / count, times a scalar grad_loss
+  Scales* scales;
 };
 
 // One CTA; each thread owns a run of tokens: count, one scan over the threads, write.
 __global__ void __launch_bounds__(1024) select_kernel(const void* targets, int is64, int64_t n, int64_t vocab,
-                                                      int64_t ignore, int mean, const float* grad_loss, Selected s,
-                                                      float* loss, float* lse) {
+                                                      int64_t ignore, int mean, const float* grad_loss,
+                                                      const float* weights, Selected s, float* loss, float* lse) {
   __shared__ int sh[32];
+  __shared__ unsigned sh_largest;
+  if (threadIdx.x == 0) sh_largest = weights ? 0u : __float_as_uint(1.f);
+  __syncthreads();
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int64_t per = (n + 1023) / 1024, lo = min(tid * per, n), hi = min(lo + per, n);
   int mine = 0;
-  for (int64_t t = lo; t < hi; ++t) mine += target_at(targets, is64, t) != ignore;
+  unsigned largest = 0;
+  for (int64_t t = lo; t < hi; ++t) {
+    const bool counts = target_at(targets, is64, t) != ignore;
+    mine += counts;
+    if (weights && counts) largest = max(largest, finite_bits(weights[t]));
+  }
+  if (weights) atomicMax(&sh_largest, largest);
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -90,28 +119,50 @@ __global__ void __launch_bounds__(1024) select_kernel(const void* targets, int i
   }
   if (tid == 0) {
     *s.count = total;
+    s.scales->x = s.scales->w = 0;
+    s.scales->dl = sh_largest;
     *s.alpha = (mean ? (float)(1.0 / (double)max(total, 1)) : 1.f) * (grad_loss ? *grad_loss : 1.f);
   }
 }
 
 // ---------------------------------------------------------------------------
-// operands: bf16 rows whose stride is a multiple of 16 bytes
+// operands: 16-bit rows whose stride is a multiple of 16 bytes
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ void split_store(float v, bf16* hi, bf16* lo, int64_t i) {
-  const bf16 h = __float2bfloat16_rn(v);
-  hi[i] = h;
-  // an infinite value has no rest; v - hi would make it NaN
-  if (lo) lo[i] = isinf(v) ? __float2bfloat16_rn(0.f) : __float2bfloat16_rn(v - __bfloat162float(h));
+// bf16 values go as they are; f32 values times the scale, as two f16.
+__device__ __forceinline__ void put_planes(bf16 v, float, void* hi, void*, int64_t i) { static_cast<bf16*>(hi)[i] = v; }
+__device__ __forceinline__ void put_planes(float v, float scale, void* hi, void* lo, int64_t i) {
+  const float s = v * scale;
+  const __half h = __float2half_rn(s);
+  static_cast<__half*>(hi)[i] = h;
+  // an infinite value has no rest; s - hi would make it NaN
+  static_cast<__half*>(lo)[i] = isinf(s) ? __float2half_rn(0.f) : __float2half_rn(s - __half2float(h));
+}
+template <typename T>
+__device__ __forceinline__ T zero_of() { return T(0.f); }
+
+// Largest finite magnitude of a matrix's rows (of those whose target counts, where given).
+__global__ void __launch_bounds__(256) largest_kernel(const float* src, int64_t stride, int64_t rows, int64_t dim,
+                                                      const void* targets, int is64, int64_t ignore, unsigned* out) {
+  unsigned m = 0;
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
+    if (targets && target_at(targets, is64, r) == ignore) continue;
+    const float* x = src + r * stride;
+#pragma unroll 8
+    for (int64_t c = threadIdx.x & 31; c < dim; c += 32) m = max(m, finite_bits(x[c]));
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if ((threadIdx.x & 31) == 0 && m) atomicMax(out, m);
 }
 
 // Planes of a whole matrix (the weight, where the tensor maps cannot read it as it is).
 template <typename T>
 __global__ void __launch_bounds__(256) planes_kernel(const T* src, int64_t stride, int64_t rows, int64_t dim,
-                                                     int64_t ld, bf16* hi, bf16* lo) {
+                                                     int64_t ld, void* hi, void* lo, const unsigned* largest) {
   const int64_t n = rows * ld;
+  const float scale = scale_of(*largest);
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / ld, c = i - r * ld;
-    split_store(c < dim ? ldg(src + r * stride + c) : 0.f, hi, lo, i);
+    put_planes(c < dim ? src[r * stride + c] : zero_of<T>(), scale, hi, lo, i);
   }
 }
 
@@ -119,20 +170,21 @@ __global__ void __launch_bounds__(256) planes_kernel(const T* src, int64_t strid
 // weight's gradient).  blockIdx.y = 1: zero rows of grad_hidden for the ignored tokens.
 template <typename T>
 __global__ void __launch_bounds__(256) gather_kernel(const T* src, int64_t stride, int64_t tokens, int64_t dim, int64_t ld,
-                                                     Selected s, const void* targets, int is64, int64_t ignore, bf16* hi,
-                                                     bf16* lo, T* grad_hidden) {
+                                                     Selected s, const void* targets, int is64, int64_t ignore, void* hi,
+                                                     void* lo, T* grad_hidden) {
   const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (r >= tokens) return;
   if (blockIdx.y == 1) {
     if (target_at(targets, is64, r) == ignore)
-      for (int64_t c = lane; c < dim; c += 32) st(grad_hidden + r * dim + c, 0.f);
+      for (int64_t c = lane; c < dim; c += 32) grad_hidden[r * dim + c] = zero_of<T>();
     return;
   }
   const int64_t count = *s.count;
   if (r >= (count + 63) / 64 * 64) return;
   const T* x = src + (r < count ? s.index[r] : 0) * stride;
-  for (int64_t c = lane; c < ld; c += 32) split_store(r < count && c < dim ? ldg(x + c) : 0.f, hi, lo, r * ld + c);
+  const float scale = scale_of(s.scales->x);
+  for (int64_t c = lane; c < ld; c += 32) put_planes(r < count && c < dim ? x[c] : zero_of<T>(), scale, hi, lo, r * ld + c);
 }
 
 // A matrix as the GEMMs read it.
@@ -152,19 +204,6 @@ void place_planes(Operand* o, int dtype, uint8_t* mem) {
   o->plane[1] = dtype == SSD_DTYPE_F32 ? mem + up256((size_t)o->rows * o->ld * 2) : nullptr;
 }
 
-cudaError_t make_planes(const void* src, int dtype, int64_t stride, Operand* o, uint8_t* mem, cudaStream_t st) {
-  place_planes(o, dtype, mem);
-  bf16* hi = static_cast<bf16*>(const_cast<void*>(o->plane[0]));
-  bf16* lo = static_cast<bf16*>(const_cast<void*>(o->plane[1]));
-  const int64_t n = o->rows * o->ld;
-  const unsigned grid = (unsigned)std::min<int64_t>((n + 255) / 256, 148 * 8 * 4);
-  if (dtype == SSD_DTYPE_F32)
-    planes_kernel<float><<<grid, 256, 0, st>>>(static_cast<const float*>(src), stride, o->rows, o->dim, o->ld, hi, lo);
-  else
-    planes_kernel<bf16><<<grid, 256, 0, st>>>(static_cast<const bf16*>(src), stride, o->rows, o->dim, o->ld, hi, lo);
-  return cudaGetLastError();
-}
-
 size_t planes_bytes(int64_t rows, int64_t dim, int dtype) {
   return (dtype == SSD_DTYPE_F32 ? 2 : 1) * up256((size_t)rows * ((dim + 7) / 8 * 8) * 2);
 }
@@ -180,6 +219,7 @@ struct LogitArgs {
   float* picked;           // (rows): the target's logit
   float* logits;           // (rows, ld) or NULL
   int64_t ld;
+  const Scales* scales;
 };
 
 template <int CG>
@@ -187,49 +227,41 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) logits_kernel(const __grid_c
                                                                   const __grid_constant__ LogitArgs a) {
   extern __shared__ uint8_t smem[];
   __shared__ gemm::Ctl ctl;
-  const int lane = threadIdx.x & 31;
-  gemm::run<CG, false, false>(p, smem, &ctl, [&](const gemm::Tile& t, uint32_t acc, int quad, int half, int m0, int live) {
-    const int64_t row = m0 + 32 * quad + lane;
-    const int64_t n0 = (int64_t)t.n * BN + half * 128;
-    const int64_t y = row < live ? a.target[row] : -1;
-    float m2 = -INFINITY, l = 0.f;
-#pragma unroll 1
-    for (int ch = 0; ch < 4; ++ch) {
-      const int64_t c0 = n0 + 32 * ch;
-      if (c0 >= a.vocab) break;
-      float v[32];
-      ptx::tmem_ld32(acc + half * 128 + 32 * ch, v);
-      ptx::tmem_ld_wait();
-      if (c0 + 32 > a.vocab) {
+  const float unscale = p.passes == 3 ? 1.f / (scale_of(a.scales->x) * scale_of(a.scales->w)) : 1.f;
+  gemm::run<CG, false, false>(p, smem, &ctl, [&](const gemm::Tile& t, float (&v)[BN / 2], int row, int n0, int live) {
+    const int y = row < live ? a.target[row] : -1;
+    if (p.passes == 3) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = c0 + i < a.vocab ? v[i] : -INFINITY;
-      }
-      if (a.logits && row < live) {
-        float4* o = reinterpret_cast<float4*>(a.logits + row * a.ld + c0);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-      }
-      if (y >= c0 && y < c0 + 32) {   // the target's logit is kept out of the sum
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          s = y == c0 + i ? v[i] : s;
-          v[i] = y == c0 + i ? -INFINITY : v[i];
-        }
-        a.picked[row] = s;
-      }
-      float top = v[0];
-#pragma unroll
-      for (int i = 1; i < 32; ++i) top = fmaxf(top, v[i]);
-      // the anchor is the rounded product itself, so that what is stored says what was summed
-      const float n2 = fmaxf(m2, top * LOG2E), at = n2 == -INFINITY ? 0.f : n2;
-      float e[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < 32; ++i) e[i & 3] += exp2f(fmaf(v[i], LOG2E, -at));
-      l = l * exp2f(m2 - at) + ((e[0] + e[1]) + (e[2] + e[3]));
-      m2 = n2;
+      for (int i = 0; i < BN / 2; ++i) v[i] *= unscale;
     }
-    if (row < live) a.stats[row * a.ns + 2 * t.n + half] = make_float2(m2, l);
+    if (a.logits && row < live) {
+      float4* o = reinterpret_cast<float4*>(a.logits + row * a.ld + n0);
+#pragma unroll
+      for (int i = 0; i < BN / 8; ++i)
+        if (n0 + 4 * i < a.vocab) o[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    }
+    if (n0 + BN / 2 > a.vocab) {
+#pragma unroll
+      for (int i = 0; i < BN / 2; ++i) v[i] = n0 + i < a.vocab ? v[i] : -INFINITY;
+    }
+    if (y >= n0 && y < n0 + BN / 2) {   // the target's logit is kept out of the sum
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < BN / 2; ++i) {
+        s = y == n0 + i ? v[i] : s;
+        v[i] = y == n0 + i ? -INFINITY : v[i];
+      }
+      a.picked[row] = s;
+    }
+    float m[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int i = 4; i < BN / 2; ++i) m[i & 3] = fmaxf(m[i & 3], v[i]);
+    // the anchor is the rounded product itself, so that what is stored says what was summed
+    const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * LOG2E, at = top == -INFINITY ? 0.f : top;
+    float e[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < BN / 2; ++i) e[i & 3] += exp2f(fmaf(v[i], LOG2E, -at));
+    if (row < live) a.stats[(int64_t)row * a.ns + n0 / (BN / 2)] = make_float2(top, (e[0] + e[1]) + (e[2] + e[3]));
   });
 }
 
@@ -314,7 +346,7 @@ struct RowArgs {
   const float* picked;
   const float* logits;
   const float* weight;     // per-token factor or NULL
-  bf16* dl[2];             // (rows, ld); [1] for f32 inputs only
+  void* dl[2];             // (rows, ld): bf16, or two f16 planes of dl times its scale
   float* loss;             // (tokens)
   float* lse;              // (tokens) or NULL
 };
@@ -336,8 +368,9 @@ __global__ void __launch_bounds__(ROW_THREADS) row_kernel(const RowArgs a) {
       const int token = a.sel.index[a.from + row];
       const float w = a.weight ? a.weight[token] : 1.f;
       sh_at = r.top;
-      sh_inv = w * r.inv;
-      sh_y = w * r.pm1;
+      const float scale = SPLIT ? scale_of(a.sel.scales->dl) : 1.f;
+      sh_inv = w * scale * r.inv;
+      sh_y = w * scale * r.pm1;
       a.loss[token] = r.loss;
       if (a.lse) a.lse[token] = r.lse;
     }
@@ -345,8 +378,8 @@ __global__ void __launch_bounds__(ROW_THREADS) row_kernel(const RowArgs a) {
   __syncthreads();
   const float at = counted ? sh_at : 0.f, f = counted ? sh_inv : 0.f, at_y = counted ? sh_y : 0.f;
   const float* s = a.logits + row * a.ld;
-  bf16* hi = a.dl[0] + row * a.ld;
-  bf16* lo = SPLIT ? a.dl[1] + row * a.ld : nullptr;
+  uint2* hi = reinterpret_cast<uint2*>(static_cast<bf16*>(a.dl[0]) + row * a.ld);
+  uint2* lo = SPLIT ? reinterpret_cast<uint2*>(static_cast<__half*>(a.dl[1]) + row * a.ld) : nullptr;
   for (int64_t c = threadIdx.x * 4; c < a.vocab; c += ROW_THREADS * 4) {
     float d[4] = {0.f, 0.f, 0.f, 0.f};
     if (counted) {
@@ -359,12 +392,15 @@ __global__ void __launch_bounds__(ROW_THREADS) row_kernel(const RowArgs a) {
       for (int k = 0; k < 4; ++k)
         if (c + k == y) d[k] = at_y;
     }
-    __nv_bfloat162 h[2] = {__floats2bfloat162_rn(d[0], d[1]), __floats2bfloat162_rn(d[2], d[3])};
-    *reinterpret_cast<uint2*>(hi + c) = *reinterpret_cast<uint2*>(h);
     if constexpr (SPLIT) {
-      const float2 g0 = __bfloat1622float2(h[0]), g1 = __bfloat1622float2(h[1]);
-      __nv_bfloat162 l[2] = {__floats2bfloat162_rn(d[0] - g0.x, d[1] - g0.y), __floats2bfloat162_rn(d[2] - g1.x, d[3] - g1.y)};
-      *reinterpret_cast<uint2*>(lo + c) = *reinterpret_cast<uint2*>(l);
+      __half2 h[2] = {__floats2half2_rn(d[0], d[1]), __floats2half2_rn(d[2], d[3])};
+      const float2 g0 = __half22float2(h[0]), g1 = __half22float2(h[1]);
+      __half2 l[2] = {__floats2half2_rn(d[0] - g0.x, d[1] - g0.y), __floats2half2_rn(d[2] - g1.x, d[3] - g1.y)};
+      hi[c / 4] = *reinterpret_cast<uint2*>(h);
+      lo[c / 4] = *reinterpret_cast<uint2*>(l);
+    } else {
+      __nv_bfloat162 h[2] = {__floats2bfloat162_rn(d[0], d[1]), __floats2bfloat162_rn(d[2], d[3])};
+      hi[c / 4] = *reinterpret_cast<uint2*>(h);
     }
   }
 }
@@ -378,77 +414,68 @@ struct OutArgs {
   const float* alpha;
   float* part;             // f32: parts of a split K range (splits, rows, cols), or the running sum
   int add_part;            // add what `part` holds (the running sum over token chunks)
+  const unsigned* largest[2];   // f32 inputs: what the operands' scales come from
 };
-
-__device__ __forceinline__ void put32(const OutArgs& a, int64_t row, int64_t c0, float (&v)[32], float alpha) {
-  const int64_t at = row * a.cols + c0;
-  if (a.out_bf16) {
-    bf16* o = static_cast<bf16*>(a.out) + at;
-    if (c0 + 32 <= a.cols && reinterpret_cast<uintptr_t>(o) % 16 == 0) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t u[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * i + 2 * k] * alpha, v[8 * i + 2 * k + 1] * alpha);
-          u[k] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-        reinterpret_cast<uint4*>(o)[i] = make_uint4(u[0], u[1], u[2], u[3]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (c0 + i < a.cols) o[i] = __float2bfloat16_rn(v[i] * alpha);
-    }
-  } else {
-    float* o = static_cast<float*>(a.out) + at;
-    if (c0 + 32 <= a.cols && reinterpret_cast<uintptr_t>(o) % 16 == 0) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        reinterpret_cast<float4*>(o)[i] = make_float4(v[4 * i] * alpha, v[4 * i + 1] * alpha, v[4 * i + 2] * alpha, v[4 * i + 3] * alpha);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (c0 + i < a.cols) o[i] = v[i] * alpha;
-    }
-  }
-}
 
 template <int CG, bool A_MN>
 __global__ void __launch_bounds__(gemm::THREADS, 1) grad_gemm_kernel(const __grid_constant__ gemm::Problem p,
                                                                      const __grid_constant__ OutArgs a) {
   extern __shared__ uint8_t smem[];
   __shared__ gemm::Ctl ctl;
-  const int lane = threadIdx.x & 31;
+  const float unscale = p.passes == 3 ? 1.f / scale_of(*a.largest[0]) / scale_of(*a.largest[1]) : 1.f;
   const float alpha = a.out ? *a.alpha : 1.f;
-  gemm::run<CG, A_MN, true>(p, smem, &ctl, [&](const gemm::Tile& t, uint32_t acc, int quad, int half, int m0, int live) {
-    const int64_t row = m0 + 32 * quad + lane;
-    const int64_t n0 = (int64_t)t.n * BN + half * 128;
-    const int64_t rows = p.limit_k ? a.rows : live;
-    const int64_t to = a.index && row < rows ? a.index[row] : row;
-#pragma unroll 1
-    for (int ch = 0; ch < 4; ++ch) {
-      const int64_t c0 = n0 + 32 * ch;
-      if (c0 >= a.cols) break;
-      float v[32];
-      ptx::tmem_ld32(acc + half * 128 + 32 * ch, v);
-      ptx::tmem_ld_wait();
-      if (row >= rows) continue;
-      if (t.k0 == t.k1) {
+  gemm::run<CG, A_MN, true>(p, smem, &ctl, [&](const gemm::Tile& t, float (&v)[BN / 2], int row, int n0, int live) {
+    if (row >= (p.limit_k ? a.rows : live)) return;
+    if (p.passes == 3) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = 0.f;
-      }
-      if (a.part) {
-        float* q = a.part + ((int64_t)t.split * a.rows + row) * a.cols + c0;
+      for (int i = 0; i < BN / 2; ++i) v[i] *= unscale;
+    }
+    if (a.part) {
+      float* q = a.part + ((int64_t)t.split * a.rows + row) * a.cols + n0;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          if (c0 + i < a.cols) {
-            if (a.add_part) v[i] += q[i];
-            if (!a.out) q[i] = v[i];
-          }
+      for (int i = 0; i < BN / 2; ++i) {
+        if (n0 + i < a.cols) {
+          if (a.add_part) v[i] += q[i];
+          if (!a.out) q[i] = v[i];
         }
       }
-      if (a.out) put32(a, to, c0, v, alpha);
+    }
+    if (!a.out) return;
+    const int64_t at = (a.index ? a.index[row] : row) * a.cols + n0;
+#pragma unroll
+    for (int i = 0; i < BN / 2; ++i) v[i] *= alpha;
+    if (a.out_bf16) {
+      bf16* o = static_cast<bf16*>(a.out) + at;
+      const bool al = reinterpret_cast<uintptr_t>(o) % 16 == 0;
+#pragma unroll
+      for (int i = 0; i < BN / 2; i += 8) {
+        if (al && n0 + i + 8 <= a.cols) {
+          uint32_t u[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[i + 2 * k], v[i + 2 * k + 1]);
+            u[k] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+          *reinterpret_cast<uint4*>(o + i) = make_uint4(u[0], u[1], u[2], u[3]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (n0 + i + k < a.cols) o[i + k] = __float2bfloat16_rn(v[i + k]);
+        }
+      }
+    } else {
+      float* o = static_cast<float*>(a.out) + at;
+      const bool al = reinterpret_cast<uintptr_t>(o) % 16 == 0;
+#pragma unroll
+      for (int i = 0; i < BN / 2; i += 4) {
+        if (al && n0 + i + 4 <= a.cols) {
+          *reinterpret_cast<float4*>(o + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (n0 + i + k < a.cols) o[i + k] = v[i + k];
+        }
+      }
     }
   });
 }
@@ -560,7 +587,7 @@ Plan plan_of(const ssd_linear_ce_params_t* p) {
     at += up256(bytes);
     return o;
   };
-  q.one = take(8);
+  q.one = take(64);
   q.index = take((size_t)p->tokens * 4);
   q.target = take((size_t)p->tokens * 4);
   q.rows = take(p->reduction == SSD_REDUCE_NONE ? 0 : (size_t)p->tokens * 4);
@@ -601,6 +628,7 @@ cudaError_t logits_gemm(const Operand& x, const Operand& w, int planes, const Lo
   g.k_blocks = cdiv(x.dim, gemm::BK);
   g.passes = planes == 2 ? 3 : 1;
   g.m_fastest = 1;
+  g.segment = planes == 2 ? SEGMENT_F32 : SEGMENT_BF16;
   g.status = status;
   return launch_gemm<CG>(logits_kernel<CG>, g, a, st);
 }
@@ -620,6 +648,8 @@ cudaError_t grad_gemm(const Operand& a, const Operand& b, int64_t k, int planes,
   g.k_blocks = cdiv(k, gemm::BK);
   g.passes = planes == 2 ? 3 : 1;
   g.m_fastest = 0;
+  // bf16: the operands' own rounding is a hundred times what the adds lose
+  g.segment = planes == 2 ? SEGMENT_F32 : 1 << 20;
   g.status = status;
   return launch_gemm<CG>(grad_gemm_kernel<CG, A_MN>, g, o, st);
 }
@@ -636,20 +666,29 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
   Selected sel;
   sel.count = reinterpret_cast<int*>(ws + q.one);
   sel.alpha = reinterpret_cast<float*>(ws + q.one) + 1;
+  sel.scales = reinterpret_cast<Scales*>(ws + q.one + 16);
   sel.index = reinterpret_cast<int*>(ws + q.index);
   sel.target = reinterpret_cast<int*>(ws + q.target);
   float* rows = p->reduction == SSD_REDUCE_NONE ? p->loss : reinterpret_cast<float*>(ws + q.rows);
   const bool bf = p->dtype == SSD_DTYPE_BF16, mean = p->reduction == SSD_REDUCE_MEAN;
   const bool per_row = p->reduction == SSD_REDUCE_NONE && p->grad_loss;
   select_kernel<<<1, 1024, 0, st>>>(p->targets, p->targets_int64, p->tokens, p->vocab, p->ignore_index, mean,
-                                    per_row ? nullptr : p->grad_loss, sel, rows, p->lse);
+                                    per_row ? nullptr : p->grad_loss, per_row ? p->grad_loss : nullptr, sel, rows, p->lse);
   CE_CHECK(cudaGetLastError(), "select");
   Operand x{}, w{};
   x.rows = p->tokens; x.dim = p->dim;
   place_planes(&x, p->dtype, ws + q.x);
   const dim3 grid((unsigned)cdiv(p->tokens, 8), p->grad_hidden ? 2 : 1);
-  bf16* hi = static_cast<bf16*>(const_cast<void*>(x.plane[0]));
-  bf16* lo = static_cast<bf16*>(const_cast<void*>(x.plane[1]));
+  void* hi = const_cast<void*>(x.plane[0]);
+  void* lo = const_cast<void*>(x.plane[1]);
+  const unsigned wide = 148 * 8;
+  if (!bf) {
+    largest_kernel<<<std::min<unsigned>(grid.x, wide), 256, 0, st>>>(static_cast<const float*>(p->hidden), p->hidden_stride_row,
+        p->tokens, p->dim, p->targets, p->targets_int64, p->ignore_index, &sel.scales->x);
+    largest_kernel<<<std::min<unsigned>((unsigned)cdiv(p->vocab, 8), wide), 256, 0, st>>>(static_cast<const float*>(p->weight),
+        p->weight_stride_row, p->vocab, p->dim, nullptr, 0, 0, &sel.scales->w);
+    CE_CHECK(cudaGetLastError(), "largest");
+  }
   if (bf)
     gather_kernel<bf16><<<grid, 256, 0, st>>>(static_cast<const bf16*>(p->hidden), p->hidden_stride_row, p->tokens, p->dim,
                                               x.ld, sel, p->targets, p->targets_int64, p->ignore_index, hi, lo,
@@ -660,7 +699,19 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
                                                static_cast<float*>(p->grad_hidden));
   CE_CHECK(cudaGetLastError(), "gather");
   w.rows = p->vocab; w.dim = p->dim; w.ld = p->weight_stride_row; w.plane[0] = p->weight;
-  if (q.pack_w) CE_CHECK(make_planes(p->weight, p->dtype, p->weight_stride_row, &w, ws + q.w, st), "weight planes");
+  if (q.pack_w) {
+    place_planes(&w, p->dtype, ws + q.w);
+    void* whi = const_cast<void*>(w.plane[0]);
+    void* wlo = const_cast<void*>(w.plane[1]);
+    const unsigned g = (unsigned)std::min<int64_t>((w.rows * w.ld + 255) / 256, wide * 4);
+    if (bf)
+      planes_kernel<bf16><<<g, 256, 0, st>>>(static_cast<const bf16*>(p->weight), p->weight_stride_row, p->vocab, p->dim,
+                                             w.ld, whi, wlo, &sel.scales->w);
+    else
+      planes_kernel<float><<<g, 256, 0, st>>>(static_cast<const float*>(p->weight), p->weight_stride_row, p->vocab, p->dim,
+                                              w.ld, whi, wlo, &sel.scales->w);
+    CE_CHECK(cudaGetLastError(), "weight planes");
+  }
   for (int64_t c = 0; c < q.nchunks; ++c) {
     const int64_t t0 = c * q.chunk, n = std::min(q.chunk, p->tokens - t0);
     const int from = (int)t0;
@@ -674,7 +725,8 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
     a.picked = reinterpret_cast<float*>(ws + q.picked);
     a.logits = q.grad ? reinterpret_cast<float*>(ws + q.logits) : nullptr;
     a.ld = q.ld;
-    if (n > BM) CE_CHECK(logits_gemm<CE_PAIR>(xc, w, q.planes, a, sel.count, from, status, st), "logits");
+    a.scales = sel.scales;
+    if (n > BM) CE_CHECK(logits_gemm<2>(xc, w, q.planes, a, sel.count, from, status, st), "logits");
     else CE_CHECK(logits_gemm<1>(xc, w, q.planes, a, sel.count, from, status, st), "logits");
     if (!q.grad) {
       loss_kernel<<<(unsigned)cdiv(n, 8), 256, 0, st>>>(a.stats, a.ns, a.picked, sel, from, (int)n, rows, p->lse);
@@ -685,7 +737,7 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
     r.vocab = p->vocab; r.ld = q.ld; r.sel = sel; r.from = from;
     r.ns = a.ns; r.stats = a.stats; r.picked = a.picked; r.logits = a.logits;
     r.weight = per_row ? p->grad_loss : nullptr;
-    for (int i = 0; i < q.planes; ++i) r.dl[i] = reinterpret_cast<bf16*>(ws + q.dl[i]);
+    for (int i = 0; i < q.planes; ++i) r.dl[i] = ws + q.dl[i];
     r.loss = rows; r.lse = p->lse;
     if (q.planes == 2) row_kernel<true><<<(unsigned)n, ROW_THREADS, 0, st>>>(r);
     else row_kernel<false><<<(unsigned)n, ROW_THREADS, 0, st>>>(r);
@@ -696,9 +748,10 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
     if (p->grad_hidden) {
       OutArgs o{};
       o.rows = n; o.cols = p->dim; o.alpha = sel.alpha; o.out_bf16 = bf; o.index = sel.index + t0;
+      o.largest[0] = &sel.scales->dl; o.largest[1] = &sel.scales->w;
       if (q.splits > 1) o.part = reinterpret_cast<float*>(ws + q.part);
       else o.out = p->grad_hidden;
-      if (n > BM) CE_CHECK((grad_gemm<CE_PAIR, false>(dl, w, p->vocab, q.planes, q.splits, o, sel.count, from, status, st)), "grad_hidden");
+      if (n > BM) CE_CHECK((grad_gemm<2, false>(dl, w, p->vocab, q.planes, q.splits, o, sel.count, from, status, st)), "grad_hidden");
       else CE_CHECK((grad_gemm<1, false>(dl, w, p->vocab, q.planes, q.splits, o, sel.count, from, status, st)), "grad_hidden");
       if (q.splits > 1) {
         if (bf)
@@ -711,10 +764,11 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
     if (p->grad_weight) {
       OutArgs o{};
       o.rows = p->vocab; o.cols = p->dim; o.alpha = sel.alpha; o.out_bf16 = p->grad_weight_dtype == SSD_DTYPE_BF16;
+      o.largest[0] = &sel.scales->dl; o.largest[1] = &sel.scales->x;
       if (q.sum_w) o.part = reinterpret_cast<float*>(ws + q.wsum);
       o.add_part = c > 0;
       o.out = c == q.nchunks - 1 ? p->grad_weight : nullptr;
-      if (p->vocab > BM) CE_CHECK((grad_gemm<CE_PAIR, true>(dl, xc, n, q.planes, 1, o, sel.count, from, status, st)), "grad_weight");
+      if (p->vocab > BM) CE_CHECK((grad_gemm<2, true>(dl, xc, n, q.planes, 1, o, sel.count, from, status, st)), "grad_weight");
       else CE_CHECK((grad_gemm<1, true>(dl, xc, n, q.planes, 1, o, sel.count, from, status, st)), "grad_weight");
     }
   }

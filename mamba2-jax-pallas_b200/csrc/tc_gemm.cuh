@@ -1,5 +1,5 @@
-// Tensor-core GEMM core for the language-model head: D = A B^T (+ epilogue), bf16 operands,
-// f32 accumulators in TMEM.
+// Tensor-core GEMM core for the language-model head: D = A B^T (+ epilogue), 16-bit operands,
+// f32 accumulation.
 //
 // One persistent CTA per SM, or a pair of CTAs per two SMs (CG = 2: tcgen05 cta_group::2, one
 // 256 x 256 tile per pair).  The pair halves what each SM fetches of B, in shared memory and
@@ -8,12 +8,18 @@
 //   0     TMA producer: A and B boxes into a ring of shared-memory stages
 //   1     MMA issuer (the pair's first CTA only issues): four K = 16 MMAs per stage
 //   2..9  epilogue: warp w reads the TMEM lanes of quadrant w % 4, column half (w - 2) / 4
-// Two accumulators (2 x 256 TMEM columns) let the epilogue of a tile overlap the next tile's
-// MMAs.  Operands are K-major (the reduced dimension contiguous in memory) or MN-major (the
+// Two accumulators (2 x 256 TMEM columns) let the reading of one overlap the MMAs into the
+// other.  Operands are K-major (the reduced dimension contiguous in memory) or MN-major (the
 // other one contiguous), so no operand is ever transposed in memory.
 //
-// f32 operands come as two bf16 planes, v = hi + lo, and the K loop runs over the plane pairs
-// hi*lo, lo*hi, hi*hi (the split of Henry, Tang and Heinecke, ARITH 2019, as in ssd_x3.cu).
+// The tensor core's f32 adds truncate: over K = 4096 a dot product loses about 1e-5 of its
+// value, always towards zero.  So a tile's K range runs in segments, each from zero in its own
+// TMEM accumulator, and the epilogue warps add the segments in registers, rounding to nearest:
+// 128 values per thread.
+//
+// f32 operands come as two f16 planes of the values times a power of two, v = hi + lo, and the
+// K loop runs over the plane pairs hi*lo, lo*hi, hi*hi.  Two f16 hold 22 bits of a value down
+// to 2^-16 of the largest, so three products carry what f32 carries; two bf16 hold 16.
 //
 // Every wait is bounded; one that gives up sets the status word and the CTA drains and ends.
 #pragma once
@@ -57,13 +63,14 @@ struct Problem {
   int limit_from, rows, limit_k;
   int m_tiles, n_tiles, splits;           // m tiles of CG * 128 rows
   int k_blocks;                           // of 64
-  int passes;                             // 1, or 3 for split f32 operands
+  int passes;                             // 1 (bf16), or 3 (f32 as two f16 planes)
+  int segment;                            // K blocks that are summed in TMEM
   int m_fastest;
   unsigned* status;
 };
 
 struct Tile {
-  int m, n, split, k0, k1;                // k0 == k1: nothing to add, the accumulator is not written
+  int m, n, split, k0, k1;
 };
 
 // Rows that count, of those that the launch was made for.
@@ -172,9 +179,15 @@ __device__ __forceinline__ void tmem_free_all(uint32_t t) {
     ptx::tmem_dealloc(t, 512);
 }
 
-// The kernel's body.  epi(tile, tmem address of the accumulator's first column for this warp's
-// quadrant, quadrant, column half, first row of this CTA's part, rows that count) runs on each
-// epilogue warp; it ends with its TMEM reads complete.
+// Instruction descriptor: f16 operands have format 0, bf16 format 1.
+template <int CG, bool A_MN, bool B_MN>
+__device__ __forceinline__ uint32_t idesc(const Problem& p) {
+  constexpr uint32_t ID = ptx::idesc_bf16_f32(BM * CG, BN, A_MN, B_MN);
+  return p.passes == 3 ? ID & ~((1u << 7) | (1u << 10)) : ID;
+}
+
+// The kernel's body.  epi(tile, v, row, first column, rows that count) runs on each epilogue
+// thread with 128 values of one row.
 template <int CG, bool A_MN, bool B_MN, typename Epi>
 __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c, Epi&& epi) {
   using S = Shape<CG>;
@@ -255,17 +268,24 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      constexpr uint32_t ID = ptx::idesc_bf16_f32(BM * CG, BN, A_MN, B_MN);
+      const uint32_t ID = idesc<CG, A_MN, B_MN>(p);
       uint32_t it = 0, n = 0;
       bool ok = true;
-      for (int64_t u = unit0; ok && u < units; u += step, ++n) {
+      for (int64_t u = unit0; ok && u < units; u += step) {
         const Tile t = tile_at(p, m_tiles, k_blocks, u);
-        const int acc = n & 1;
-        if (n >= 2 && !wait(c, &c->acc_empty[acc], ((n >> 1) - 1) & 1, p.status, 2)) break;
-        ptx::tc_fence_after();
-        const uint32_t d = tmem + acc * BN;
         const int steps = p.passes * (t.k1 - t.k0);
-        for (int j = 0; j < steps; ++j, ++it) {
+        uint32_t d = 0;
+        for (int j = 0, left = 0; j < steps; ++j, ++it, --left) {
+          const bool first = left == 0;
+          if (first) {
+            left = min(p.segment, steps - j);
+            if (n >= 2 && !wait(c, &c->acc_empty[n & 1], ((n >> 1) - 1) & 1, p.status, 2)) {
+              ok = false;
+              break;
+            }
+            ptx::tc_fence_after();
+            d = tmem + (n & 1) * BN;
+          }
           const int s = it % S::STAGES;
           if (!wait(c, &c->full[s], (it / S::STAGES) & 1, p.status, 3)) {
             ok = false;
@@ -277,12 +297,14 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
           for (int k = 0; k < BK / 16; ++k) {
             const uint64_t da = A_MN ? ptx::sdesc_sw128(sa + k * 2048, 8192, 1024) : ptx::sdesc_sw128(sa + k * 32, 16, 1024);
             const uint64_t db = B_MN ? ptx::sdesc_sw128(sb + k * 2048, 8192, 1024) : ptx::sdesc_sw128(sb + k * 32, 16, 1024);
-            mma<CG>(d, da, db, ID, (j > 0 || k > 0) ? 1u : 0u);
+            mma<CG>(d, da, db, ID, (!first || k > 0) ? 1u : 0u);
           }
           commit<CG>(&c->empty[s]);
+          if (left == 1) {
+            commit<CG>(&c->acc_full[n & 1]);
+            ++n;
+          }
         }
-        if (!ok) break;
-        commit<CG>(&c->acc_full[acc]);
       }
       if (!ok) {   // let the MMAs in flight finish
         ptx::tc_fence_before();
@@ -298,23 +320,40 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
   } else {
     const int quad = warp & 3, half = (warp - 2) >> 2;
     uint32_t n = 0;
-    for (int64_t u = unit0; u < units; u += step, ++n) {
+    bool ok = true;
+    for (int64_t u = unit0; ok && u < units; u += step) {
       const Tile t = tile_at(p, m_tiles, k_blocks, u);
-      const int acc = n & 1;
-      // one lane waits for the warp, so that the warp stays converged for its TMEM loads
-      int ok = 0;
-      if (lane == 0) ok = wait(c, &c->acc_full[acc], (n >> 1) & 1, p.status, 4);
-      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-      ptx::tc_fence_after();
-      epi(t, tmem + acc * BN + ((uint32_t)(32 * quad) << 16), quad, half, (t.m * CG + (int)rank) * BM, live);
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (CG == 2)
-          arrive_remote(map_rank(ptx::smem_u32(&c->acc_empty[acc]), 0));
-        else
-          ptx::mbar_arrive(&c->acc_empty[acc]);
+      float v[BN / 2];
+#pragma unroll
+      for (int i = 0; i < BN / 2; ++i) v[i] = 0.f;
+      for (int left = p.passes * (t.k1 - t.k0); left > 0; left -= p.segment, ++n) {
+        // one lane waits for the warp, so that the warp stays converged for its TMEM loads
+        int there = 0;
+        if (lane == 0) there = wait(c, &c->acc_full[n & 1], (n >> 1) & 1, p.status, 4);
+        if (!__shfl_sync(0xffffffffu, there, 0)) {
+          ok = false;
+          break;
+        }
+        ptx::tc_fence_after();
+        const uint32_t from = tmem + (n & 1) * BN + half * (BN / 2) + ((uint32_t)(32 * quad) << 16);
+#pragma unroll
+        for (int ch = 0; ch < BN / 64; ++ch) {
+          float x[32];
+          ptx::tmem_ld32(from + 32 * ch, x);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[32 * ch + i] += x[i];
+        }
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (CG == 2)
+            arrive_remote(map_rank(ptx::smem_u32(&c->acc_empty[n & 1]), 0));
+          else
+            ptx::mbar_arrive(&c->acc_empty[n & 1]);
+        }
       }
+      if (ok) epi(t, v, (t.m * CG + (int)rank) * BM + 32 * quad + lane, t.n * BN + half * (BN / 2), live);
     }
   }
   __syncwarp();
