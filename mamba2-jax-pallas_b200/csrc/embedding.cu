@@ -10,20 +10,23 @@
 // gradient has V rows, most of them zero).
 //
 // The gradient is a sum by sorted ids, so that it is the same in every run: no atomics on
-// floats.  Three launches:
-//   1. one cluster sorts (id, position) pairs by a stable radix sort whose histograms live in
-//      distributed shared memory, while every other CTA of the grid writes the zero rows of
-//      the ids that do not occur (it marks the ids of its own rows in a shared bitmap);
-//   2. the sorted order is cut into pieces of equal length, whatever the ids, so that one
-//      frequent id cannot hold up a CTA; a warp sums a piece's rows over 256 columns in f32
-//      and writes each id's row where the id begins and ends inside the piece; an id that
-//      crosses into another piece leaves its part in the workspace;
-//   3. the piece in which such an id begins adds its parts up, again in order.
+// floats.  Launches:
+//   1. one cluster of 8 CTAs sorts (id, position) pairs by a stable radix sort whose histograms
+//      live in distributed shared memory;
+//   2. meanwhile (a programmatic dependent launch that does not wait) the other SMs write the
+//      zero rows of the ids that do not occur, most of a dense gradient: a CTA marks the ids of
+//      its own rows in a shared bitmap;
+//   3. the sorted order is cut into pieces of equal length, whatever the ids, so that one
+//      frequent id cannot hold up a CTA.  A warp sums a piece's rows over 256 columns in f32 and
+//      writes each id's row.  An id that goes on for at most EXTEND rows into the next piece is
+//      finished by the piece it began in; a longer one leaves its parts in the workspace;
+//   4. the parts of such ids are added up, again in order.
 #include <algorithm>
 
 #include <cooperative_groups.h>
 
 #include "common.cuh"
+#include "ptx_sm100.cuh"
 #include "ssd_kernels.h"
 
 namespace cg = cooperative_groups;
@@ -31,39 +34,79 @@ namespace cg = cooperative_groups;
 namespace ssd {
 namespace {
 
-constexpr int VEC = 8;            // values per lane and load: 16 bytes of bf16, 32 of f32
+constexpr int VEC = 8;            // columns per lane
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[VEC]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p));
-    const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-    const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+// Which columns of a run of 256 a lane holds.
+//   EIGHT  8 lane .. + 7: one 16-byte access of bf16
+//   FOURS  4 lane .. + 3, and the same 128 further on: two 16-byte accesses of f32, each of
+//          them 512 contiguous bytes per warp (8 f32 side by side would leave half sectors)
+//   ONES   lane, lane + 32, ...: any width and alignment
+enum Cols { EIGHT, FOURS, ONES };
+
+template <Cols M>
+__device__ __forceinline__ int col_of(int lane, int k) {
+  return M == EIGHT ? lane * 8 + k : M == FOURS ? lane * 4 + (k & 3) + 128 * (k >> 2) : lane + 32 * k;
+}
+
+__device__ __forceinline__ void unpack2(uint32_t u, float& a, float& b) {
+  a = __uint_as_float(u << 16);
+  b = __uint_as_float(u & 0xffff0000u);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The lane's columns of `row` (the start of a run of 256; `left` columns to the row's end).
+template <typename T, Cols M>
+__device__ __forceinline__ void load_cols(const T* row, int64_t left, float (&v)[VEC]) {
+  const int lane = threadIdx.x & 31;
+  if constexpr (M == EIGHT && sizeof(T) == 2) {
+    uint4 q = make_uint4(0, 0, 0, 0);
+    if (lane * 8 < left) q = *reinterpret_cast<const uint4*>(row + lane * 8);
+    unpack2(q.x, v[0], v[1]); unpack2(q.y, v[2], v[3]); unpack2(q.z, v[4], v[5]); unpack2(q.w, v[6], v[7]);
+  } else if constexpr (M != ONES) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      v[2 * k] = __uint_as_float(u[k] << 16);
-      v[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+    for (int g = 0; g < 2; ++g) {
+      const int c = col_of<M>(lane, 4 * g);
+      if constexpr (sizeof(T) == 4) {
+        float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c < left) q = *reinterpret_cast<const float4*>(row + c);
+        v[4 * g] = q.x; v[4 * g + 1] = q.y; v[4 * g + 2] = q.z; v[4 * g + 3] = q.w;
+      } else {
+        uint2 q = make_uint2(0, 0);
+        if (c < left) q = *reinterpret_cast<const uint2*>(row + c);
+        unpack2(q.x, v[4 * g], v[4 * g + 1]); unpack2(q.y, v[4 * g + 2], v[4 * g + 3]);
+      }
     }
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = lane + 32 * k < left ? ld(row + lane + 32 * k) : 0.f;
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&v)[VEC]) {
-  if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-    uint32_t u[4];
+template <typename T, Cols M>
+__device__ __forceinline__ void store_cols(T* row, int64_t left, const float (&v)[VEC]) {
+  const int lane = threadIdx.x & 31;
+  if constexpr (M == EIGHT && sizeof(T) == 2) {
+    if (lane * 8 < left)
+      *reinterpret_cast<uint4*>(row + lane * 8) =
+          make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
+  } else if constexpr (M != ONES) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-      u[i] = *reinterpret_cast<uint32_t*>(&h);
+    for (int g = 0; g < 2; ++g) {
+      const int c = col_of<M>(lane, 4 * g);
+      if (c < left) {
+        if constexpr (sizeof(T) == 4)
+          *reinterpret_cast<float4*>(row + c) = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+        else
+          *reinterpret_cast<uint2*>(row + c) = make_uint2(pack2(v[4 * g], v[4 * g + 1]), pack2(v[4 * g + 2], v[4 * g + 3]));
+      }
     }
-    *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k)
+      if (lane + 32 * k < left) st(row + lane + 32 * k, v[k]);
   }
 }
 
@@ -86,48 +129,31 @@ struct LookupArgs {
 };
 
 constexpr int LK_THREADS = 256;
-constexpr int LK_UNROLL = 4;      // 16-byte loads in flight per lane
+constexpr int LK_UNROLL = 4;      // runs of 256 columns in flight per warp
 
-// One warp per (token, run of 32 * LK_UNROLL vectors of 8).
-template <typename TW, typename TO>
-__global__ void __launch_bounds__(LK_THREADS) lookup_vec_kernel(const LookupArgs a, int runs) {
+// One warp per (token, LK_UNROLL runs of 256 columns).
+template <typename TW, typename TO, Cols M>
+__global__ void __launch_bounds__(LK_THREADS) lookup_kernel(const LookupArgs a, int runs) {
   const int64_t unit = (int64_t)blockIdx.x * (LK_THREADS / 32) + threadIdx.x / 32;
   const int64_t t = unit / runs;
   if (t >= a.n) return;
-  const int lane = threadIdx.x & 31;
-  const int64_t c0 = (unit - t * runs) * (32 * LK_UNROLL * VEC);
+  const int64_t c0 = (unit - t * runs) * (256 * LK_UNROLL);
   const int64_t row = row_of(a.ids, a.is64, t, a.vocab, a.pad);
   TO* o = static_cast<TO*>(a.out) + t * a.os;
   const TW* w = static_cast<const TW*>(a.w) + (row < 0 ? 0 : row) * a.ws;
   float v[LK_UNROLL][VEC];
 #pragma unroll
   for (int i = 0; i < LK_UNROLL; ++i) {
-    const int64_t c = c0 + (int64_t)(i * 32 + lane) * VEC;
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) v[i][k] = 0.f;
-    if (row >= 0 && c < a.dim) load8(w + c, v[i]);
+    const int64_t c = c0 + 256 * i;
+    load_cols<TW, M>(w + c, row < 0 ? 0 : a.dim - c, v[i]);   // a dropped token reads nothing
   }
 #pragma unroll
   for (int i = 0; i < LK_UNROLL; ++i) {
-    const int64_t c = c0 + (int64_t)(i * 32 + lane) * VEC;
-    if (c >= a.dim) continue;
-    if (row >= 0) {
+    const int64_t c = c0 + 256 * i;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) v[i][k] *= a.scale;
-    }
-    store8(o + c, v[i]);
+    for (int k = 0; k < VEC; ++k) v[i][k] = row < 0 ? 0.f : v[i][k] * a.scale;
+    store_cols<TO, M>(o + c, a.dim - c, v[i]);
   }
-}
-
-// Any width and alignment: one warp per token, one value per lane and step.
-template <typename TW, typename TO>
-__global__ void __launch_bounds__(LK_THREADS) lookup_any_kernel(const LookupArgs a) {
-  const int64_t t = (int64_t)blockIdx.x * (LK_THREADS / 32) + threadIdx.x / 32;
-  if (t >= a.n) return;
-  const int64_t row = row_of(a.ids, a.is64, t, a.vocab, a.pad);
-  TO* o = static_cast<TO*>(a.out) + t * a.os;
-  const TW* w = static_cast<const TW*>(a.w) + (row < 0 ? 0 : row) * a.ws;
-  for (int64_t c = threadIdx.x & 31; c < a.dim; c += 32) st(o + c, row < 0 ? 0.f : ldg(w + c) * a.scale);
 }
 
 bool rows16(const void* p, int64_t stride, int64_t dim, int dtype) {
@@ -138,17 +164,16 @@ bool rows16(const void* p, int64_t stride, int64_t dim, int dtype) {
 template <typename TW, typename TO>
 cudaError_t lookup(const LookupArgs& a, bool vec, cudaStream_t stream) {
   constexpr int W = LK_THREADS / 32;
-  if (vec) {
-    const int64_t runs = (a.dim + 32 * LK_UNROLL * VEC - 1) / (32 * LK_UNROLL * VEC);
-    lookup_vec_kernel<TW, TO><<<(unsigned)((a.n * runs + W - 1) / W), LK_THREADS, 0, stream>>>(a, (int)runs);
-  } else {
-    lookup_any_kernel<TW, TO><<<(unsigned)((a.n + W - 1) / W), LK_THREADS, 0, stream>>>(a);
-  }
+  constexpr Cols M = sizeof(TW) == 2 && sizeof(TO) == 2 ? EIGHT : FOURS;
+  const int64_t runs = (a.dim + 256 * LK_UNROLL - 1) / (256 * LK_UNROLL);
+  const unsigned grid = (unsigned)((a.n * runs + W - 1) / W);
+  if (vec) lookup_kernel<TW, TO, M><<<grid, LK_THREADS, 0, stream>>>(a, (int)runs);
+  else lookup_kernel<TW, TO, ONES><<<grid, LK_THREADS, 0, stream>>>(a, (int)runs);
   return cudaGetLastError();
 }
 
 // ---------------------------------------------------------------------------
-// gradient, launch 1: sort and zero rows
+// gradient, launches 1 and 2: sort, zero rows
 // ---------------------------------------------------------------------------
 constexpr int SORT_CTAS = 8;      // the sorting cluster
 constexpr int SORT_THREADS = 1024;
@@ -159,7 +184,7 @@ constexpr int ZERO_ROWS = 8192;   // rows whose bits the bitmap holds at a time
 
 struct GradArgs {
   int64_t n, vocab, dim, gs, os, pad, piece, npieces;
-  int is64, passes, accumulate, zero_ctas;
+  int is64, passes, accumulate;
   float scale;
   const void* ids;
   const void* g;
@@ -167,6 +192,7 @@ struct GradArgs {
   uint32_t* key[2];               // sorted ids (V = dropped, last); result in key[0], pos[0]
   uint32_t* pos[2];
   float* part;                    // (npieces, 2, dim)
+  int* heavy;                     // count, then the pieces in which an id with parts begins
 };
 
 struct SortShared {
@@ -259,18 +285,34 @@ __device__ void sort_pass(const GradArgs& a, SortShared* s, int shift, const uin
   cluster.sync();   // the cluster's keys are in place; every CTA has read the others' counts
 }
 
+__global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_THREADS, 1) sort_kernel(const GradArgs a) {
+  extern __shared__ uint8_t smem[];
+  ptx::griddep_launch_dependents();   // the zero rows need nothing from here
+  SortShared* s = reinterpret_cast<SortShared*>(smem);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.heavy = 0;
+  // the passes end in key[0] / pos[0]
+  int to = (a.passes - 1) & 1;
+  sort_pass<true>(a, s, 0, nullptr, nullptr, a.key[to], a.pos[to]);
+  for (int p = 1; p < a.passes; ++p) {
+    sort_pass<false>(a, s, p * SORT_BITS, a.key[to], a.pos[to], a.key[to ^ 1], a.pos[to ^ 1]);
+    to ^= 1;
+  }
+}
+
 // Zero rows of the ids that do not occur.  A CTA owns rows [r0, r1) and marks those that
 // occur in a shared bitmap, ZERO_ROWS at a time, reading all ids (L2) once for each.
 template <typename TO>
-__device__ void zero_rows(const GradArgs& a, uint32_t* bits, int cta) {
+__global__ void __launch_bounds__(SORT_THREADS, 1) zero_rows_kernel(const GradArgs a) {
+  __shared__ uint32_t bits[ZERO_ROWS / 32];
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
-  const int64_t per = (a.vocab + a.zero_ctas - 1) / a.zero_ctas;
-  const int64_t r0 = cta * per, r1 = min(r0 + per, a.vocab);
+  const int64_t per = (a.vocab + gridDim.x - 1) / gridDim.x;
+  const int64_t r0 = blockIdx.x * per, r1 = min(r0 + per, a.vocab);
   const bool vec = (reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.os * sizeof(TO))) % 16 == 0;
   for (int64_t b0 = r0; b0 < r1; b0 += ZERO_ROWS) {
     const int64_t b1 = min(b0 + ZERO_ROWS, r1);
     for (int i = tid; i < ZERO_ROWS / 32; i += SORT_THREADS) bits[i] = 0;
     __syncthreads();
+#pragma unroll 8
     for (int64_t t = tid; t < a.n; t += SORT_THREADS) {
       const int64_t v = row_of(a.ids, a.is64, t, a.vocab, a.pad);
       if (v >= b0 && v < b1) atomicOr(&bits[(v - b0) >> 5], 1u << ((v - b0) & 31));
@@ -289,101 +331,72 @@ __device__ void zero_rows(const GradArgs& a, uint32_t* bits, int cta) {
     }
     __syncthreads();
   }
-}
-
-template <typename TO>
-__global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_THREADS, 1)
-    grad_sort_kernel(const GradArgs a) {
-  extern __shared__ uint8_t smem[];
-  if (blockIdx.x >= SORT_CTAS) {
-    zero_rows<TO>(a, reinterpret_cast<uint32_t*>(smem), (int)blockIdx.x - SORT_CTAS);
-    return;
-  }
-  SortShared* s = reinterpret_cast<SortShared*>(smem);
-  // the passes end in key[0] / pos[0]
-  int to = (a.passes - 1) & 1;
-  sort_pass<true>(a, s, 0, nullptr, nullptr, a.key[to], a.pos[to]);
-  for (int p = 1; p < a.passes; ++p) {
-    sort_pass<false>(a, s, p * SORT_BITS, a.key[to], a.pos[to], a.key[to ^ 1], a.pos[to ^ 1]);
-    to ^= 1;
-  }
+  // what is launched behind this kernel may take the sort as done, too
+  ptx::griddep_wait();
 }
 
 // ---------------------------------------------------------------------------
-// gradient, launches 2 and 3: sums
+// gradient, launches 3 and 4: sums
 // ---------------------------------------------------------------------------
 constexpr int SUM_THREADS = 256;
 constexpr int SUM_COLS = 32 * VEC;   // columns of a warp
 constexpr int SUM_UNROLL = 8;        // rows in flight
+constexpr int EXTEND = 32;           // rows that a piece may take from the next one
 
-template <typename T, bool V>
-__device__ __forceinline__ void load_cols(const T* row, int64_t c, int64_t dim, float (&v)[VEC]) {
-  if constexpr (V) {
-    if (c < dim) {
-      load8(row + c, v);
-    } else {
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) v[k] = 0.f;
-    }
-  } else {   // columns c + 32 k: neighbouring lanes read neighbouring values
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) v[k] = c + 32 * k < dim ? ldg(row + c + 32 * k) : 0.f;
-  }
-}
-
-template <typename T, bool V>
-__device__ __forceinline__ void store_cols(T* row, int64_t c, int64_t dim, const float (&v)[VEC]) {
-  if constexpr (V) {
-    if (c < dim) store8(row + c, v);
-  } else {
-#pragma unroll
-    for (int k = 0; k < VEC; ++k)
-      if (c + 32 * k < dim) st(row + c + 32 * k, v[k]);
-  }
-}
-
-template <typename TO, bool V>
-__device__ __forceinline__ void put_row(const GradArgs& a, uint32_t id, int64_t c, float (&acc)[VEC]) {
-  TO* o = static_cast<TO*>(a.out) + (int64_t)id * a.os;
+template <typename TO, Cols M>
+__device__ __forceinline__ void put_row(const GradArgs& a, uint32_t id, int64_t c0, float (&acc)[VEC]) {
+  TO* o = static_cast<TO*>(a.out) + (int64_t)id * a.os + c0;
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] *= a.scale;
   if (a.accumulate) {
     float old[VEC];
-    if constexpr (V) {
-      if (c < a.dim) {
-        load8(o + c, old);
+    load_cols<TO, M>(o, a.dim - c0, old);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[k] += old[k];
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < VEC; ++k)
-        if (c + 32 * k < a.dim) acc[k] += ld(o + c + 32 * k);
-    }
+    for (int k = 0; k < VEC; ++k) acc[k] += old[k];
   }
-  store_cols<TO, V>(o, c, a.dim, acc);
+  store_cols<TO, M>(o, a.dim - c0, acc);
 }
 
-// Warp (piece p, columns): rows of the sorted positions [p * piece, + piece).
-template <typename TG, typename TO, bool V>
+// Warp (piece p, 256 columns): rows of the sorted positions [p * piece, + piece).
+template <typename TG, typename TO, Cols M>
 __global__ void __launch_bounds__(SUM_THREADS) grad_sum_kernel(const GradArgs a, int col_warps) {
+  ptx::griddep_wait();
   const int64_t unit = (int64_t)blockIdx.x * (SUM_THREADS / 32) + threadIdx.x / 32;
   const int64_t p = unit / col_warps;
   if (p >= a.npieces) return;
   const int lane = threadIdx.x & 31;
-  const int64_t c = (unit - p * col_warps) * SUM_COLS + (V ? lane * VEC : lane);
+  const int64_t c0 = (unit - p * col_warps) * SUM_COLS;
   const int64_t lo = p * a.piece, hi = min(lo + a.piece, a.n);
+  const uint32_t none = (uint32_t)a.vocab;
   const uint32_t* key = a.key[0];
   const uint32_t* pos = a.pos[0];
-  const TG* g = static_cast<const TG*>(a.g);
+  const TG* g = static_cast<const TG*>(a.g) + c0;
   uint32_t cur = key[lo];
-  bool open = lo > 0 && key[lo - 1] == cur;   // the id began in an earlier piece
+  if (cur == none) return;
+  // the first id: it may have begun in an earlier piece, and then either the piece before
+  // finishes it (skip) or this piece's share of it is a part (open)
+  bool open = lo > 0 && key[lo - 1] == cur, skip = false;
+  if (open) {
+    const int64_t before = lo - a.piece;
+    skip = (before == 0 || key[before - 1] != cur) && (lo + EXTEND >= a.n || key[lo + EXTEND] != cur);
+  }
+  // the last id: rows of the next piece that this one takes, or the id goes on too long
+  int64_t end = hi;
+  bool goes_on = false;
+  const uint32_t last = key[hi - 1];
+  if (hi < a.n && last != none && key[hi] == last) {
+    const bool starts_here = lo == 0 || key[lo - 1] != last;
+    if (starts_here && (hi + EXTEND >= a.n || key[hi + EXTEND] != last))
+      end += __popc(__ballot_sync(0xffffffffu, hi + lane < a.n && key[min(hi + lane, a.n - 1)] == last));
+    else
+      goes_on = true;
+  }
   float acc[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
-  for (int64_t i0 = lo; i0 < hi && cur != (uint32_t)a.vocab; i0 += 32) {
-    const int m = (int)min((int64_t)32, hi - i0);
-    const uint32_t mk = lane < m ? key[i0 + lane] : (uint32_t)a.vocab;
+  for (int64_t i0 = lo; i0 < end && cur != none; i0 += 32) {
+    const int m = (int)min((int64_t)32, end - i0);
+    const uint32_t mk = lane < m ? key[i0 + lane] : none;
     const uint32_t mp = lane < m ? pos[i0 + lane] : 0;
     for (int j0 = 0; j0 < m; j0 += SUM_UNROLL) {
       float v[SUM_UNROLL][VEC];
@@ -391,23 +404,24 @@ __global__ void __launch_bounds__(SUM_THREADS) grad_sum_kernel(const GradArgs a,
       for (int j = 0; j < SUM_UNROLL; ++j) {
         const uint32_t kj = __shfl_sync(0xffffffffu, mk, j0 + j);
         const int64_t t = __shfl_sync(0xffffffffu, mp, j0 + j);
-        if (kj != (uint32_t)a.vocab) load_cols<TG, V>(g + t * a.gs, c, a.dim, v[j]);
+        if (kj != none) load_cols<TG, M>(g + t * a.gs, a.dim - c0, v[j]);
       }
 #pragma unroll
       for (int j = 0; j < SUM_UNROLL; ++j) {
         const uint32_t kj = __shfl_sync(0xffffffffu, mk, j0 + j);
-        if (j0 + j < m && cur != (uint32_t)a.vocab) {
+        if (j0 + j < m && cur != none) {
           if (kj != cur) {
-            if (open)
-              store_cols<float, V>(a.part + (p * 2) * a.dim, c, a.dim, acc);
-            else
-              put_row<TO, V>(a, cur, c, acc);
-            open = false;
+            if (open) {
+              if (!skip) store_cols<float, M>(a.part + (p * 2) * a.dim + c0, a.dim - c0, acc);
+            } else {
+              put_row<TO, M>(a, cur, c0, acc);
+            }
+            open = skip = false;
             cur = kj;
 #pragma unroll
             for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
           }
-          if (kj != (uint32_t)a.vocab) {
+          if (kj != none) {
 #pragma unroll
             for (int k = 0; k < VEC; ++k) acc[k] += v[j][k];
           }
@@ -415,72 +429,99 @@ __global__ void __launch_bounds__(SUM_THREADS) grad_sum_kernel(const GradArgs a,
       }
     }
   }
-  if (cur == (uint32_t)a.vocab) return;
-  const bool goes_on = hi < a.n && key[hi] == cur;
-  if (open)
-    store_cols<float, V>(a.part + (p * 2) * a.dim, c, a.dim, acc);
-  else if (goes_on)
-    store_cols<float, V>(a.part + (p * 2 + 1) * a.dim, c, a.dim, acc);
-  else
-    put_row<TO, V>(a, cur, c, acc);
+  if (cur == none) return;
+  if (open) {
+    if (!skip) store_cols<float, M>(a.part + (p * 2) * a.dim + c0, a.dim - c0, acc);
+  } else if (goes_on) {
+    store_cols<float, M>(a.part + (p * 2 + 1) * a.dim + c0, a.dim - c0, acc);
+    if (c0 == 0 && lane == 0) a.heavy[1 + atomicAdd(a.heavy, 1)] = (int)p;
+  } else {
+    put_row<TO, M>(a, cur, c0, acc);
+  }
 }
 
-// CTA (piece p, 256 columns): where an id begins in piece p and goes on, the sum of its parts.
-// The parts of the following pieces are shared out over the CTA's warps in runs, each summed
-// in order, and the runs are added in order.
-template <typename TO, bool V>
+// CTA (256 columns, every gridDim.y-th listed piece p): the id that begins in piece p, the sum
+// of its parts.  The parts of the following pieces are shared out over the CTA's warps in
+// runs, each summed in order, and the runs are added in order; which CTA does it, and when,
+// changes nothing.
+template <typename TO, Cols M>
 __global__ void __launch_bounds__(SUM_THREADS) grad_join_kernel(const GradArgs a) {
   __shared__ float sums[SUM_THREADS / 32][SUM_COLS];
-  const int64_t p = blockIdx.y;
+  ptx::griddep_wait();
   const uint32_t* key = a.key[0];
-  const int64_t lo = p * a.piece, hi = lo + a.piece;
-  if (hi >= a.n) return;
-  const uint32_t id = key[hi - 1];
-  if (id == (uint32_t)a.vocab || key[hi] != id || (lo > 0 && key[lo - 1] == id && key[lo] == id)) return;
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // last piece that holds the id: pieces p+1, p+2, ... whose first key is the id
-  int64_t last = p + 1;
-  while (true) {
-    const int64_t q = last + 1 + lane;
-    const bool same = q < a.npieces && key[q * a.piece] == id;
-    const unsigned b = __ballot_sync(0xffffffffu, same);
-    const int more = b == 0xffffffffu ? 32 : __ffs(~b) - 1;
-    last += more;
-    if (more < 32) break;
-  }
-  const int64_t count = last - p, per = (count + SUM_THREADS / 32 - 1) / (SUM_THREADS / 32);
-  const int64_t q0 = p + 1 + w * per, q1 = min(q0 + per, last + 1);
-  const int64_t c = (int64_t)blockIdx.x * SUM_COLS + (V ? lane * VEC : lane);
-  float acc[VEC];
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, listed = *a.heavy;
+  for (int h = blockIdx.y; h < listed; h += gridDim.y) {
+    const int64_t p = a.heavy[1 + h];
+    const uint32_t id = key[(p + 1) * a.piece - 1];
+    // last piece that holds the id: pieces p+1, p+2, ... whose first key is the id
+    int64_t last = p + 1;
+    while (true) {
+      const int64_t q = last + 1 + lane;
+      const unsigned b = __ballot_sync(0xffffffffu, q < a.npieces && key[min(q, a.npieces - 1) * a.piece] == id);
+      const int more = b == 0xffffffffu ? 32 : __ffs(~b) - 1;
+      last += more;
+      if (more < 32) break;
+    }
+    const int64_t count = last - p, per = (count + SUM_THREADS / 32 - 1) / (SUM_THREADS / 32);
+    const int64_t q0 = p + 1 + w * per, q1 = min(q0 + per, last + 1);
+    const int64_t c0 = (int64_t)blockIdx.x * SUM_COLS;
+    const float* part = a.part + c0;
+    float acc[VEC];
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
-  if (w == 0) load_cols<float, V>(a.part + (p * 2 + 1) * a.dim, c, a.dim, acc);
+    for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+    if (w == 0) load_cols<float, M>(part + (p * 2 + 1) * a.dim, a.dim - c0, acc);
 #pragma unroll 4
-  for (int64_t q = q0; q < q1; ++q) {
-    float v[VEC];
-    load_cols<float, V>(a.part + (q * 2) * a.dim, c, a.dim, v);
+    for (int64_t q = q0; q < q1; ++q) {
+      float v[VEC];
+      load_cols<float, M>(part + (q * 2) * a.dim, a.dim - c0, v);
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) acc[k] += v[k];
+      for (int k = 0; k < VEC; ++k) acc[k] += v[k];
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) sums[w][k * 32 + lane] = acc[k];
+    __syncthreads();
+    if (w == 0) {
+      for (int i = 1; i < SUM_THREADS / 32; ++i) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] += sums[i][k * 32 + lane];
+      }
+      put_row<TO, M>(a, id, c0, acc);
+    }
+    __syncthreads();
   }
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) sums[w][k * 32 + lane] = acc[k];
-  __syncthreads();
-  if (w != 0) return;
-  for (int i = 1; i < SUM_THREADS / 32; ++i) {
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) acc[k] += sums[i][k * 32 + lane];
-  }
-  put_row<TO, V>(a, id, c, acc);
 }
 
-template <typename TG, typename TO, bool V>
+// Launch that may start while the one before it ends (the kernels wait where they must).
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
+template <typename TG, typename TO, Cols M>
 cudaError_t grad_sums(const GradArgs& a, cudaStream_t stream) {
   const int64_t col_warps = (a.dim + SUM_COLS - 1) / SUM_COLS;
   constexpr int W = SUM_THREADS / 32;
-  grad_sum_kernel<TG, TO, V><<<(unsigned)((a.npieces * col_warps + W - 1) / W), SUM_THREADS, 0, stream>>>(a, (int)col_warps);
-  if (a.npieces > 1)
-    grad_join_kernel<TO, V><<<dim3((unsigned)col_warps, (unsigned)a.npieces), SUM_THREADS, 0, stream>>>(a);
-  return cudaGetLastError();
+  cudaError_t e = launch_dependent(grad_sum_kernel<TG, TO, M>, dim3((unsigned)((a.npieces * col_warps + W - 1) / W)),
+                                   SUM_THREADS, stream, a, (int)col_warps);
+  if (e == cudaSuccess && a.n > a.piece + EXTEND)   // shorter lists have no id with parts
+    e = launch_dependent(grad_join_kernel<TO, M>, dim3((unsigned)col_warps, (unsigned)std::min<int64_t>(a.npieces, 32)),
+                         SUM_THREADS, stream, a);
+  return e;
+}
+
+template <typename TG, typename TO>
+cudaError_t grad_sums(const GradArgs& a, bool vec, cudaStream_t stream) {
+  constexpr Cols M = sizeof(TG) == 2 && sizeof(TO) == 2 ? EIGHT : FOURS;
+  return vec ? grad_sums<TG, TO, M>(a, stream) : grad_sums<TG, TO, ONES>(a, stream);
 }
 
 int64_t piece_len(int64_t n) {
@@ -509,7 +550,7 @@ cudaError_t launch_embedding(const ssd_embedding_params_t* p, cudaStream_t strea
 
 size_t embedding_grad_workspace(int64_t n, int64_t dim) {
   const int64_t pieces = (n + piece_len(n) - 1) / piece_len(n);
-  return 4 * up256((size_t)n * 4) + (size_t)pieces * 2 * dim * 4;
+  return 4 * up256((size_t)n * 4) + up256((size_t)(pieces + 1) * 4) + (size_t)pieces * 2 * dim * 4;
 }
 
 cudaError_t launch_embedding_grad(const ssd_embedding_grad_params_t* p, void* workspace, cudaStream_t stream) {
@@ -526,27 +567,26 @@ cudaError_t launch_embedding_grad(const ssd_embedding_grad_params_t* p, void* wo
     a.key[i] = reinterpret_cast<uint32_t*>(ws + (2 * i) * list);
     a.pos[i] = reinterpret_cast<uint32_t*>(ws + (2 * i + 1) * list);
   }
-  a.part = reinterpret_cast<float*>(ws + 4 * list);
+  a.heavy = reinterpret_cast<int*>(ws + 4 * list);
+  a.part = reinterpret_cast<float*>(ws + 4 * list + up256((size_t)(a.npieces + 1) * 4));
   int bits = 1;
   while (((int64_t)1 << bits) <= a.vocab) ++bits;   // the largest key is V itself (dropped)
   a.passes = (bits + SORT_BITS - 1) / SORT_BITS;
   const bool gb = p->grad_dtype == SSD_DTYPE_BF16, ob = p->out_dtype == SSD_DTYPE_BF16;
-  // one CTA per SM next to the sorting cluster, in whole clusters: 8 + 17 * 8 = 144 of 148 SMs
-  a.zero_ctas = a.accumulate ? 0 : 17 * SORT_CTAS;
   const size_t smem = sizeof(SortShared);
-  const void* fn = ob ? (const void*)grad_sort_kernel<bf16> : (const void*)grad_sort_kernel<float>;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
-  void* args[] = {&a};
-  e = cudaLaunchKernel(fn, dim3((unsigned)(SORT_CTAS + a.zero_ctas)), dim3(SORT_THREADS), args, smem, stream);
-  if (e != cudaSuccess || a.n == 0) return e;
-  const bool vec = rows16(p->grad, a.gs, a.dim, p->grad_dtype) && rows16(p->out, a.os, a.dim, p->out_dtype);
-  if (gb) {
-    if (ob) return vec ? grad_sums<bf16, bf16, true>(a, stream) : grad_sums<bf16, bf16, false>(a, stream);
-    return vec ? grad_sums<bf16, float, true>(a, stream) : grad_sums<bf16, float, false>(a, stream);
+  sort_kernel<<<SORT_CTAS, SORT_THREADS, smem, stream>>>(a);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  if (!a.accumulate) {   // one CTA per SM that does not sort
+    e = launch_dependent(ob ? zero_rows_kernel<bf16> : zero_rows_kernel<float>, dim3(148 - SORT_CTAS), SORT_THREADS, stream, a);
+    if (e != cudaSuccess) return e;
   }
-  if (ob) return vec ? grad_sums<float, bf16, true>(a, stream) : grad_sums<float, bf16, false>(a, stream);
-  return vec ? grad_sums<float, float, true>(a, stream) : grad_sums<float, float, false>(a, stream);
+  if (a.n == 0) return e;
+  const bool vec = rows16(p->grad, a.gs, a.dim, p->grad_dtype) && rows16(p->out, a.os, a.dim, p->out_dtype);
+  if (gb) return ob ? grad_sums<bf16, bf16>(a, vec, stream) : grad_sums<bf16, float>(a, vec, stream);
+  return ob ? grad_sums<float, bf16>(a, vec, stream) : grad_sums<float, float>(a, vec, stream);
 }
 
 }  // namespace ssd

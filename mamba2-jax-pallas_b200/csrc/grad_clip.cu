@@ -12,7 +12,7 @@
 // sum and the second kernel adds the partial sums in a fixed order in each CTA: no atomics,
 // the same norm in every run, and two launches.
 //
-// Squares are summed in f64: squares of f32 gradients leave the range of f32 on both sides
+// Sums are f64: squares of f32 gradients leave the range of f32 on both sides
 // (1e-23 and 1e19), and a sum over 1e9 values in f32 loses its last digits.
 #include <algorithm>
 
@@ -23,8 +23,7 @@ namespace ssd {
 namespace {
 
 constexpr int GC_THREADS = 256;
-constexpr int VEC = 8;
-constexpr int CHUNK = 8192;             // 256 threads x 4 vectors of 8
+constexpr int CHUNK = 8192;             // values; 32 per thread
 constexpr int MAX_TENSORS = 1000;       // 1000 x 28 bytes: inside the 32764 bytes of parameters
 constexpr int MAX_PARTIALS = 148 * 8;
 
@@ -49,53 +48,52 @@ __device__ __forceinline__ int tensor_of(const Table<N>& t, int chunk) {
   return lo;
 }
 
-template <typename T>
-__device__ __forceinline__ bool load_vec(const T* p, int64_t i, int64_t n, bool al, float (&v)[VEC]) {
-  if (al && i + VEC <= n) {
+// V values from i on (zeros past the end); one access of V * sizeof(T) bytes where `al`.
+template <int V, typename T>
+__device__ __forceinline__ void load_vec(const T* p, int64_t i, int64_t n, bool al, float (&v)[V]) {
+  if (al && i + V <= n) {
     if constexpr (sizeof(T) == 4) {
       const float4 a = *reinterpret_cast<const float4*>(p + i);
-      const float4 b = reinterpret_cast<const float4*>(p + i)[1];
       v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
     } else {
-      const uint4 q = *reinterpret_cast<const uint4*>(p + i);
-      const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+      uint32_t u[V / 2];
+      if constexpr (V == 8) *reinterpret_cast<uint4*>(u) = *reinterpret_cast<const uint4*>(p + i);
+      else *reinterpret_cast<uint2*>(u) = *reinterpret_cast<const uint2*>(p + i);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < V / 2; ++k) {
         v[2 * k] = __uint_as_float(u[k] << 16);
         v[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
       }
     }
-    return true;
+    return;
   }
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) v[k] = i + k < n ? ld(p + i + k) : 0.f;
-  return false;
+  for (int k = 0; k < V; ++k) v[k] = i + k < n ? ld(p + i + k) : 0.f;
 }
 
-template <typename T>
-__device__ __forceinline__ void store_vec(T* p, int64_t i, int64_t n, int align, const float (&v)[VEC]) {
-  if (i + VEC > n || align < 4) {
+// `align`: the output's alignment in bytes, 16, 8, 4 or 2 (pieces of one flat buffer start anywhere).
+template <int V, typename T>
+__device__ __forceinline__ void store_vec(T* p, int64_t i, int64_t n, int align, const float (&v)[V]) {
+  if (i + V > n || align < 4) {
 #pragma unroll
-    for (int k = 0; k < VEC; ++k)
+    for (int k = 0; k < V; ++k)
       if (i + k < n) st(p + i + k, v[k]);
     return;
   }
-  uint32_t u[VEC];
-  constexpr int W = sizeof(T) == 4 ? 8 : 4;    // 32-bit words
+  constexpr int W = V * sizeof(T) / 4;         // 32-bit words
+  uint32_t u[W];
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) u[k] = __float_as_uint(v[k]);
+    for (int k = 0; k < W; ++k) u[k] = __float_as_uint(v[k]);
   } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < W; ++k) {
       __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
       u[k] = *reinterpret_cast<uint32_t*>(&h);
     }
   }
-  if (align >= 16) {
-#pragma unroll
-    for (int k = 0; k < W; k += 4) reinterpret_cast<uint4*>(p + i)[k / 4] = make_uint4(u[k], u[k + 1], u[k + 2], u[k + 3]);
+  if (W == 4 && align >= 16) {
+    *reinterpret_cast<uint4*>(p + i) = make_uint4(u[0], u[1], u[W - 2], u[W - 1]);
   } else if (align >= 8) {
 #pragma unroll
     for (int k = 0; k < W; k += 2) reinterpret_cast<uint2*>(p + i)[k / 2] = make_uint2(u[k], u[k + 1]);
@@ -120,8 +118,27 @@ __device__ __forceinline__ double block_sum(double v, double* sh) {
   return s;
 }
 
+// Sum of V squares.  Four are added in f32 before they go to f64: a conversion per value would
+// bound the kernel (16 per clock and SM).  Sums that may have left f32's range are taken again in f64.
+template <int V>
+__device__ __forceinline__ double squares(const float (&v)[V]) {
+  double s = 0;
+#pragma unroll
+  for (int k = 0; k < V; k += 4) {
+    const float q = fmaf(v[k], v[k], v[k + 1] * v[k + 1]) + fmaf(v[k + 2], v[k + 2], v[k + 3] * v[k + 3]);
+    if (q > 1e-25f && q < 1e38f) {
+      s += (double)q;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s = fma((double)v[k + j], (double)v[k + j], s);
+    }
+  }
+  return s;
+}
+
 template <typename T, int N>
 __global__ void __launch_bounds__(GC_THREADS) norm_kernel(const __grid_constant__ Table<N> t, double* partial) {
+  constexpr int V = 16 / sizeof(T), U = CHUNK / GC_THREADS / V;
   __shared__ double sh[GC_THREADS / 32];
   const int c0 = (int)((int64_t)t.chunks * blockIdx.x / gridDim.x), c1 = (int)((int64_t)t.chunks * (blockIdx.x + 1) / gridDim.x);
   double sum = 0;
@@ -131,16 +148,11 @@ __global__ void __launch_bounds__(GC_THREADS) norm_kernel(const __grid_constant_
     const T* g = static_cast<const T*>(t.g[i]);
     const int64_t n = t.numel[i], base = (int64_t)(c - t.first[i]) * CHUNK;
     const bool al = reinterpret_cast<uintptr_t>(g) % 16 == 0;
-    float v[CHUNK / GC_THREADS / VEC][VEC];
+    float v[U][V];
 #pragma unroll
-    for (int j = 0; j < CHUNK / GC_THREADS / VEC; ++j) {
-      const int64_t e = base + (int64_t)(j * GC_THREADS + threadIdx.x) * VEC;
-      load_vec(g, e, n, al, v[j]);
-    }
+    for (int j = 0; j < U; ++j) load_vec<V>(g, base + (int64_t)(j * GC_THREADS + threadIdx.x) * V, n, al, v[j]);
 #pragma unroll
-    for (int j = 0; j < CHUNK / GC_THREADS / VEC; ++j)
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) sum = fma((double)v[j][k], (double)v[j][k], sum);
+    for (int j = 0; j < U; ++j) sum += squares<V>(v[j]);
   }
   sum = block_sum(sum, sh);
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;
@@ -159,6 +171,8 @@ __device__ __forceinline__ float2 norm_and_factor(const double* partial, int npa
 template <typename T, typename TO, int N>
 __global__ void __launch_bounds__(GC_THREADS) scale_kernel(const __grid_constant__ Table<N> t, const double* partial,
                                                            int npartial, float max_norm, float eps, float* norm) {
+  // 16 bytes of the wider type per access: neighbouring lanes write neighbouring 16 bytes
+  constexpr int V = 16 / (sizeof(T) > sizeof(TO) ? sizeof(T) : sizeof(TO)), U = CHUNK / GC_THREADS / V;
   __shared__ double sh[GC_THREADS / 32];
   const float2 nf = norm_and_factor(partial, npartial, max_norm, eps, sh);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = nf.x;
@@ -173,18 +187,15 @@ __global__ void __launch_bounds__(GC_THREADS) scale_kernel(const __grid_constant
     const int64_t n = t.numel[i], base = (int64_t)(c - t.first[i]) * CHUNK;
     const bool al = reinterpret_cast<uintptr_t>(g) % 16 == 0;
     const int oal = align_of(o);
-    float v[CHUNK / GC_THREADS / VEC][VEC];
+    float v[U][V];
 #pragma unroll
-    for (int j = 0; j < CHUNK / GC_THREADS / VEC; ++j) {
-      const int64_t e = base + (int64_t)(j * GC_THREADS + threadIdx.x) * VEC;
-      load_vec(g, e, n, al, v[j]);
-    }
+    for (int j = 0; j < U; ++j) load_vec<V>(g, base + (int64_t)(j * GC_THREADS + threadIdx.x) * V, n, al, v[j]);
 #pragma unroll
-    for (int j = 0; j < CHUNK / GC_THREADS / VEC; ++j) {
-      const int64_t e = base + (int64_t)(j * GC_THREADS + threadIdx.x) * VEC;
+    for (int j = 0; j < U; ++j) {
+      const int64_t e = base + (int64_t)(j * GC_THREADS + threadIdx.x) * V;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) v[j][k] *= f;
-      if (e < n) store_vec(o, e, n, oal, v[j]);
+      for (int k = 0; k < V; ++k) v[j][k] *= f;
+      if (e < n) store_vec<V>(o, e, n, oal, v[j]);
     }
   }
 }

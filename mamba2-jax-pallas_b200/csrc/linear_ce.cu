@@ -76,46 +76,48 @@ struct Selected {
   Scales* scales;
 };
 
-// One CTA; each thread owns a run of tokens: count, one scan over the threads, write.
+// One CTA; each warp owns a run of tokens and reads 32 at a time: count, one scan over the warps,
+// then the same again to write.
 __global__ void __launch_bounds__(1024) select_kernel(const void* targets, int is64, int64_t n, int64_t vocab,
                                                       int64_t ignore, int mean, const float* grad_loss,
                                                       const float* weights, Selected s, float* loss, float* lse) {
   __shared__ int sh[32];
   __shared__ unsigned sh_largest;
-  if (threadIdx.x == 0) sh_largest = weights ? 0u : __float_as_uint(1.f);
-  __syncthreads();
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  const int64_t per = (n + 1023) / 1024, lo = min(tid * per, n), hi = min(lo + per, n);
+  if (tid == 0) sh_largest = weights ? 0u : __float_as_uint(1.f);
+  __syncthreads();
+  const int64_t per = (n + 1023) / 1024 * 32, lo = min(w * per, n), hi = min(lo + per, n);
   int mine = 0;
   unsigned largest = 0;
-  for (int64_t t = lo; t < hi; ++t) {
+#pragma unroll 8
+  for (int64_t t = lo + lane; t < hi; t += 32) {
     const bool counts = target_at(targets, is64, t) != ignore;
     mine += counts;
     if (weights && counts) largest = max(largest, finite_bits(weights[t]));
   }
   if (weights) atomicMax(&sh_largest, largest);
-  int incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) sh[w] = incl;
+  mine = __reduce_add_sync(0xffffffffu, mine);
+  if (lane == 0) sh[w] = mine;
   __syncthreads();
-  int at = incl - mine, total = 0;
+  int at = 0, total = 0;
   for (int i = 0; i < 32; ++i) {
     at += i < w ? sh[i] : 0;
     total += sh[i];
   }
-  for (int64_t t = lo; t < hi; ++t) {
-    const int64_t y = target_at(targets, is64, t);
-    if (y == ignore) {
+#pragma unroll 4
+  for (int64_t t0 = lo; t0 < hi; t0 += 32) {
+    const int64_t t = t0 + lane;
+    const int64_t y = t < hi ? target_at(targets, is64, t) : ignore;
+    const unsigned b = __ballot_sync(0xffffffffu, t < hi && y != ignore);
+    if (t < hi && y == ignore) {
       loss[t] = 0.f;
       if (lse) lse[t] = 0.f;
-      continue;
+    } else if (t < hi) {
+      const int r = at + __popc(b & ((1u << lane) - 1));
+      s.index[r] = (int)t;
+      s.target[r] = y >= 0 && y < vocab ? (int)y : -1;
     }
-    s.index[at] = (int)t;
-    s.target[at++] = y >= 0 && y < vocab ? (int)y : -1;
+    at += __popc(b);
   }
   if (tid == 0) {
     *s.count = total;
@@ -128,63 +130,114 @@ __global__ void __launch_bounds__(1024) select_kernel(const void* targets, int i
 // ---------------------------------------------------------------------------
 // operands: 16-bit rows whose stride is a multiple of 16 bytes
 // ---------------------------------------------------------------------------
-// bf16 values go as they are; f32 values times the scale, as two f16.
-__device__ __forceinline__ void put_planes(bf16 v, float, void* hi, void*, int64_t i) { static_cast<bf16*>(hi)[i] = v; }
-__device__ __forceinline__ void put_planes(float v, float scale, void* hi, void* lo, int64_t i) {
-  const float s = v * scale;
-  const __half h = __float2half_rn(s);
-  static_cast<__half*>(hi)[i] = h;
-  // an infinite value has no rest; s - hi would make it NaN
-  static_cast<__half*>(lo)[i] = isinf(s) ? __float2half_rn(0.f) : __float2half_rn(s - __half2float(h));
+// 8 values of a row from column c on (zeros past the end); one 16-byte load per 4 or 8 values
+// where the row allows it.
+__device__ __forceinline__ void load8(const float* row, int64_t c, int64_t dim, bool vec, float (&v)[8]) {
+  if (vec && c + 8 <= dim) {
+    const float4 a = *reinterpret_cast<const float4*>(row + c), b = *reinterpret_cast<const float4*>(row + c + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c + k < dim ? row[c + k] : 0.f;
+  }
 }
+
+// 8 values into the planes: bf16 values as they are; f32 values times the scale, as two f16.
+__device__ __forceinline__ void planes8(const bf16* row, int64_t c, int64_t dim, bool vec, float, void* hi, void*, int64_t i) {
+  uint4 q;
+  if (vec && c + 8 <= dim) {
+    q = *reinterpret_cast<const uint4*>(row + c);
+  } else {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(row);
+    uint32_t u[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t a = c + 2 * k < dim ? h[c + 2 * k] : 0, b = c + 2 * k + 1 < dim ? h[c + 2 * k + 1] : 0;
+      u[k] = a | b << 16;
+    }
+    q = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+  *reinterpret_cast<uint4*>(static_cast<bf16*>(hi) + i) = q;
+}
+__device__ __forceinline__ void planes8(const float* row, int64_t c, int64_t dim, bool vec, float scale, void* hi, void* lo,
+                                        int64_t i) {
+  float v[8];
+  load8(row, c, dim, vec, v);
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float a = v[2 * k] * scale, b = v[2 * k + 1] * scale;
+    const __half2 p = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(p);
+    // an infinite value has no rest; v - hi would make it NaN
+    const __half2 r = __floats2half2_rn(isinf(a) ? 0.f : a - f.x, isinf(b) ? 0.f : b - f.y);
+    h[k] = *reinterpret_cast<const uint32_t*>(&p);
+    l[k] = *reinterpret_cast<const uint32_t*>(&r);
+  }
+  *reinterpret_cast<uint4*>(static_cast<__half*>(hi) + i) = make_uint4(h[0], h[1], h[2], h[3]);
+  *reinterpret_cast<uint4*>(static_cast<__half*>(lo) + i) = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
 template <typename T>
-__device__ __forceinline__ T zero_of() { return T(0.f); }
+__device__ __forceinline__ bool vec_rows(const T* p, int64_t stride) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * sizeof(T) % 16 == 0;
+}
 
 // Largest finite magnitude of a matrix's rows (of those whose target counts, where given).
 __global__ void __launch_bounds__(256) largest_kernel(const float* src, int64_t stride, int64_t rows, int64_t dim,
                                                       const void* targets, int is64, int64_t ignore, unsigned* out) {
   unsigned m = 0;
+  const bool vec = vec_rows(src, stride);
   for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
     if (targets && target_at(targets, is64, r) == ignore) continue;
-    const float* x = src + r * stride;
-#pragma unroll 8
-    for (int64_t c = threadIdx.x & 31; c < dim; c += 32) m = max(m, finite_bits(x[c]));
+#pragma unroll 4
+    for (int64_t c = (threadIdx.x & 31) * 8; c < dim; c += 256) {
+      float v[8];
+      load8(src + r * stride, c, dim, vec, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) m = max(m, finite_bits(v[k]));
+    }
   }
   m = __reduce_max_sync(0xffffffffu, m);
   if ((threadIdx.x & 31) == 0 && m) atomicMax(out, m);
 }
 
-// Planes of a whole matrix (the weight, where the tensor maps cannot read it as it is).
+// Planes of a whole matrix (the weight, where the tensor maps cannot read it as it is), a warp
+// per row and 256 columns.
 template <typename T>
 __global__ void __launch_bounds__(256) planes_kernel(const T* src, int64_t stride, int64_t rows, int64_t dim,
                                                      int64_t ld, void* hi, void* lo, const unsigned* largest) {
-  const int64_t n = rows * ld;
   const float scale = scale_of(*largest);
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / ld, c = i - r * ld;
-    put_planes(c < dim ? src[r * stride + c] : zero_of<T>(), scale, hi, lo, i);
+  const bool vec = vec_rows(src, stride);
+  const int64_t runs = (ld + 255) / 256, n = rows * runs;
+#pragma unroll 2
+  for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < n; u += (int64_t)gridDim.x * 8) {
+    const int64_t r = u / runs, c = (u - r * runs) * 256 + (threadIdx.x & 31) * 8;
+    if (c < ld) planes8(src + r * stride, c, dim, vec, scale, hi, lo, r * ld + c);
   }
 }
 
 // Rows of hidden that count, side by side; zero rows up to the next 64 (a K block of the
 // weight's gradient).  blockIdx.y = 1: zero rows of grad_hidden for the ignored tokens.
 template <typename T>
-__global__ void __launch_bounds__(256) gather_kernel(const T* src, int64_t stride, int64_t tokens, int64_t dim, int64_t ld,
-                                                     Selected s, const void* targets, int is64, int64_t ignore, void* hi,
-                                                     void* lo, T* grad_hidden) {
-  const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (r >= tokens) return;
+__global__ void __launch_bounds__(128) gather_kernel(const T* src, int64_t stride, int64_t dim, int64_t ld, Selected s,
+                                                     const void* targets, int is64, int64_t ignore, void* hi, void* lo,
+                                                     T* grad_hidden) {
+  const int64_t r = blockIdx.x;
   if (blockIdx.y == 1) {
     if (target_at(targets, is64, r) == ignore)
-      for (int64_t c = lane; c < dim; c += 32) grad_hidden[r * dim + c] = zero_of<T>();
+      for (int64_t c = threadIdx.x; c < dim; c += 128) grad_hidden[r * dim + c] = T(0.f);
     return;
   }
   const int64_t count = *s.count;
   if (r >= (count + 63) / 64 * 64) return;
   const T* x = src + (r < count ? s.index[r] : 0) * stride;
   const float scale = scale_of(s.scales->x);
-  for (int64_t c = lane; c < ld; c += 32) put_planes(r < count && c < dim ? x[c] : zero_of<T>(), scale, hi, lo, r * ld + c);
+  const bool vec = vec_rows(src, stride);
+#pragma unroll 2
+  for (int64_t c = threadIdx.x * 8; c < ld; c += 128 * 8)
+    planes8(x, r < count ? c : dim, dim, vec, scale, hi, lo, r * ld + c);
 }
 
 // A matrix as the GEMMs read it.
@@ -228,18 +281,18 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) logits_kernel(const __grid_c
   extern __shared__ uint8_t smem[];
   __shared__ gemm::Ctl ctl;
   const float unscale = p.passes == 3 ? 1.f / (scale_of(a.scales->x) * scale_of(a.scales->w)) : 1.f;
-  gemm::run<CG, false, false>(p, smem, &ctl, [&](const gemm::Tile& t, float (&v)[BN / 2], int row, int n0, int live) {
+  gemm::run<CG, false, false>(p, smem, &ctl, [&](const gemm::Tile& t, float (&v)[BN / 2], int row0, int n0, int live,
+                                                 float* stage) {
+    const int row = row0 + (threadIdx.x & 31);
     const int y = row < live ? a.target[row] : -1;
     if (p.passes == 3) {
 #pragma unroll
       for (int i = 0; i < BN / 2; ++i) v[i] *= unscale;
     }
-    if (a.logits && row < live) {
-      float4* o = reinterpret_cast<float4*>(a.logits + row * a.ld + n0);
-#pragma unroll
-      for (int i = 0; i < BN / 8; ++i)
-        if (n0 + 4 * i < a.vocab) o[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    }
+    if (a.logits)
+      gemm::by_rows4(stage, v, [&](int i, int c, float4 x) {
+        if (row0 + i < live && n0 + c < a.vocab) *reinterpret_cast<float4*>(a.logits + (row0 + i) * a.ld + n0 + c) = x;
+      });
     if (n0 + BN / 2 > a.vocab) {
 #pragma unroll
       for (int i = 0; i < BN / 2; ++i) v[i] = n0 + i < a.vocab ? v[i] : -INFINITY;
@@ -380,6 +433,7 @@ __global__ void __launch_bounds__(ROW_THREADS) row_kernel(const RowArgs a) {
   const float* s = a.logits + row * a.ld;
   uint2* hi = reinterpret_cast<uint2*>(static_cast<bf16*>(a.dl[0]) + row * a.ld);
   uint2* lo = SPLIT ? reinterpret_cast<uint2*>(static_cast<__half*>(a.dl[1]) + row * a.ld) : nullptr;
+#pragma unroll 4
   for (int64_t c = threadIdx.x * 4; c < a.vocab; c += ROW_THREADS * 4) {
     float d[4] = {0.f, 0.f, 0.f, 0.f};
     if (counted) {
@@ -424,63 +478,84 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) grad_gemm_kernel(const __gri
   __shared__ gemm::Ctl ctl;
   const float unscale = p.passes == 3 ? 1.f / scale_of(*a.largest[0]) / scale_of(*a.largest[1]) : 1.f;
   const float alpha = a.out ? *a.alpha : 1.f;
-  gemm::run<CG, A_MN, true>(p, smem, &ctl, [&](const gemm::Tile& t, float (&v)[BN / 2], int row, int n0, int live) {
-    if (row >= (p.limit_k ? a.rows : live)) return;
-    if (p.passes == 3) {
+  gemm::run<CG, A_MN, true>(p, smem, &ctl, [&](const gemm::Tile& t, float (&v)[BN / 2], int row0, int n0, int live,
+                                               float* stage) {
+    const int64_t rows = p.limit_k ? a.rows : live;
+    if (row0 >= rows || n0 >= a.cols) return;
+    const float f = unscale * (a.part ? 1.f : alpha);
 #pragma unroll
-      for (int i = 0; i < BN / 2; ++i) v[i] *= unscale;
-    }
+    for (int i = 0; i < BN / 2; ++i) v[i] *= f;
     if (a.part) {
-      float* q = a.part + ((int64_t)t.split * a.rows + row) * a.cols + n0;
-#pragma unroll
-      for (int i = 0; i < BN / 2; ++i) {
-        if (n0 + i < a.cols) {
-          if (a.add_part) v[i] += q[i];
-          if (!a.out) q[i] = v[i];
-        }
-      }
-    }
-    if (!a.out) return;
-    const int64_t at = (a.index ? a.index[row] : row) * a.cols + n0;
-#pragma unroll
-    for (int i = 0; i < BN / 2; ++i) v[i] *= alpha;
-    if (a.out_bf16) {
-      bf16* o = static_cast<bf16*>(a.out) + at;
-      const bool al = reinterpret_cast<uintptr_t>(o) % 16 == 0;
-#pragma unroll
-      for (int i = 0; i < BN / 2; i += 8) {
-        if (al && n0 + i + 8 <= a.cols) {
-          uint32_t u[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(v[i + 2 * k], v[i + 2 * k + 1]);
-            u[k] = *reinterpret_cast<const uint32_t*>(&h);
+      // parts stay as they are; the running sum takes alpha when it is complete
+      float* part = a.part + ((int64_t)t.split * a.rows + row0) * a.cols + n0;
+      const bool vec = vec_rows(part, a.cols);
+      gemm::by_rows4(stage, v, [&](int i, int c, float4 x) {
+        if (row0 + i >= rows || n0 + c >= a.cols) return;
+        float* q = part + i * a.cols + c;
+        float y[4] = {x.x, x.y, x.z, x.w};
+        const bool whole = vec && n0 + c + 4 <= a.cols;
+        if (a.add_part) {
+          if (whole) {
+            const float4 o = *reinterpret_cast<const float4*>(q);
+            y[0] += o.x; y[1] += o.y; y[2] += o.z; y[3] += o.w;
+          } else {
+            for (int k = 0; k < 4; ++k)
+              if (n0 + c + k < a.cols) y[k] += q[k];
           }
-          *reinterpret_cast<uint4*>(o + i) = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+        if (!a.out) {
+          if (whole) {
+            *reinterpret_cast<float4*>(q) = make_float4(y[0], y[1], y[2], y[3]);
+          } else {
+            for (int k = 0; k < 4; ++k)
+              if (n0 + c + k < a.cols) q[k] = y[k];
+          }
+          return;
+        }
+        const int64_t at = (row0 + i) * a.cols + n0 + c;
+        for (int k = 0; k < 4; ++k)
+          if (n0 + c + k < a.cols) {
+            if (a.out_bf16) static_cast<bf16*>(a.out)[at + k] = __float2bfloat16_rn(y[k] * alpha);
+            else static_cast<float*>(a.out)[at + k] = y[k] * alpha;
+          }
+      });
+      return;
+    }
+    if (a.out_bf16) {
+      bf16* out = static_cast<bf16*>(a.out) + n0;
+      const bool vec = vec_rows(out, a.cols);
+      gemm::by_rows8(stage, v, [&](int i, int c, float4 x, float4 y) {
+        if (row0 + i >= rows || n0 + c >= a.cols) return;
+        bf16* o = out + (a.index ? a.index[row0 + i] : row0 + i) * a.cols + c;
+        __nv_bfloat162 h[4] = {__floats2bfloat162_rn(x.x, x.y), __floats2bfloat162_rn(x.z, x.w),
+                               __floats2bfloat162_rn(y.x, y.y), __floats2bfloat162_rn(y.z, y.w)};
+        if (vec && n0 + c + 8 <= a.cols) {
+          *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(h);
         } else {
-#pragma unroll
+          const bf16* e = reinterpret_cast<const bf16*>(h);
           for (int k = 0; k < 8; ++k)
-            if (n0 + i + k < a.cols) o[i + k] = __float2bfloat16_rn(v[i + k]);
+            if (n0 + c + k < a.cols) o[k] = e[k];
         }
-      }
+      });
     } else {
-      float* o = static_cast<float*>(a.out) + at;
-      const bool al = reinterpret_cast<uintptr_t>(o) % 16 == 0;
-#pragma unroll
-      for (int i = 0; i < BN / 2; i += 4) {
-        if (al && n0 + i + 4 <= a.cols) {
-          *reinterpret_cast<float4*>(o + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+      float* out = static_cast<float*>(a.out) + n0;
+      const bool vec = vec_rows(out, a.cols);
+      gemm::by_rows4(stage, v, [&](int i, int c, float4 x) {
+        if (row0 + i >= rows || n0 + c >= a.cols) return;
+        float* o = out + (a.index ? a.index[row0 + i] : row0 + i) * a.cols + c;
+        if (vec && n0 + c + 4 <= a.cols) {
+          *reinterpret_cast<float4*>(o) = x;
         } else {
-#pragma unroll
+          const float e[4] = {x.x, x.y, x.z, x.w};
           for (int k = 0; k < 4; ++k)
-            if (n0 + i + k < a.cols) o[i + k] = v[i + k];
+            if (n0 + c + k < a.cols) o[k] = e[k];
         }
-      }
+      });
     }
   });
 }
 
-// Sum of the parts of a split K range, in order, times alpha.  One CTA row per row that counts.
+// Sum of the parts of a split K range, in order, times alpha.  One CTA per row that counts.
 template <typename TO>
 __global__ void __launch_bounds__(256) join_kernel(const float* part, int splits, int64_t rows, int64_t cols, Selected s,
                                                    int from, TO* out) {
@@ -488,9 +563,28 @@ __global__ void __launch_bounds__(256) join_kernel(const float* part, int splits
   if (from + row >= *s.count) return;
   const float f = *s.alpha;
   TO* o = out + (int64_t)s.index[from + row] * cols;
+  const float* q = part + row * cols;
+  const int64_t step = rows * cols;
+  if (cols % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0) {   // the parts start at 256 bytes
+    for (int64_t c = threadIdx.x * 4; c < cols; c += 1024) {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int j = 0; j < splits; ++j) {
+        const float4 x = *reinterpret_cast<const float4*>(q + j * step + c);
+        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+      }
+      if constexpr (sizeof(TO) == 4) {
+        *reinterpret_cast<float4*>(o + c) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+      } else {
+        __nv_bfloat162 h[2] = {__floats2bfloat162_rn(v.x * f, v.y * f), __floats2bfloat162_rn(v.z * f, v.w * f)};
+        *reinterpret_cast<uint2*>(o + c) = *reinterpret_cast<uint2*>(h);
+      }
+    }
+    return;
+  }
   for (int64_t c = threadIdx.x; c < cols; c += 256) {
     float v = 0.f;
-    for (int j = 0; j < splits; ++j) v += part[(j * rows + row) * cols + c];
+    for (int j = 0; j < splits; ++j) v += q[j * step + c];
     st(o + c, v * f);
   }
 }
@@ -678,24 +772,24 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
   Operand x{}, w{};
   x.rows = p->tokens; x.dim = p->dim;
   place_planes(&x, p->dtype, ws + q.x);
-  const dim3 grid((unsigned)cdiv(p->tokens, 8), p->grad_hidden ? 2 : 1);
+  const dim3 grid((unsigned)p->tokens, p->grad_hidden ? 2 : 1);
   void* hi = const_cast<void*>(x.plane[0]);
   void* lo = const_cast<void*>(x.plane[1]);
   const unsigned wide = 148 * 8;
   if (!bf) {
-    largest_kernel<<<std::min<unsigned>(grid.x, wide), 256, 0, st>>>(static_cast<const float*>(p->hidden), p->hidden_stride_row,
+    largest_kernel<<<std::min<unsigned>((unsigned)cdiv(p->tokens, 8), wide), 256, 0, st>>>(static_cast<const float*>(p->hidden), p->hidden_stride_row,
         p->tokens, p->dim, p->targets, p->targets_int64, p->ignore_index, &sel.scales->x);
     largest_kernel<<<std::min<unsigned>((unsigned)cdiv(p->vocab, 8), wide), 256, 0, st>>>(static_cast<const float*>(p->weight),
         p->weight_stride_row, p->vocab, p->dim, nullptr, 0, 0, &sel.scales->w);
     CE_CHECK(cudaGetLastError(), "largest");
   }
   if (bf)
-    gather_kernel<bf16><<<grid, 256, 0, st>>>(static_cast<const bf16*>(p->hidden), p->hidden_stride_row, p->tokens, p->dim,
+    gather_kernel<bf16><<<grid, 128, 0, st>>>(static_cast<const bf16*>(p->hidden), p->hidden_stride_row, p->dim,
                                               x.ld, sel, p->targets, p->targets_int64, p->ignore_index, hi, lo,
                                               static_cast<bf16*>(p->grad_hidden));
   else
-    gather_kernel<float><<<grid, 256, 0, st>>>(static_cast<const float*>(p->hidden), p->hidden_stride_row, p->tokens,
-                                               p->dim, x.ld, sel, p->targets, p->targets_int64, p->ignore_index, hi, lo,
+    gather_kernel<float><<<grid, 128, 0, st>>>(static_cast<const float*>(p->hidden), p->hidden_stride_row, p->dim,
+                                               x.ld, sel, p->targets, p->targets_int64, p->ignore_index, hi, lo,
                                                static_cast<float*>(p->grad_hidden));
   CE_CHECK(cudaGetLastError(), "gather");
   w.rows = p->vocab; w.dim = p->dim; w.ld = p->weight_stride_row; w.plane[0] = p->weight;
@@ -703,7 +797,7 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
     place_planes(&w, p->dtype, ws + q.w);
     void* whi = const_cast<void*>(w.plane[0]);
     void* wlo = const_cast<void*>(w.plane[1]);
-    const unsigned g = (unsigned)std::min<int64_t>((w.rows * w.ld + 255) / 256, wide * 4);
+    const unsigned g = (unsigned)std::min<int64_t>((w.rows * ((w.ld + 255) / 256) + 7) / 8, wide * 2);
     if (bf)
       planes_kernel<bf16><<<g, 256, 0, st>>>(static_cast<const bf16*>(p->weight), p->weight_stride_row, p->vocab, p->dim,
                                              w.ld, whi, wlo, &sel.scales->w);

@@ -38,17 +38,23 @@ constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr long long WAIT_CYCLES = 4000000000LL;   // about 2 s at the boost clock
 
+// Each epilogue warp turns its rows through shared memory, 32 columns at a time, so that what it
+// writes to global memory are runs of one row and not one value of 32 rows.  Rows 36 floats
+// apart: 16-byte accesses of a quarter-warp fall into different banks, by rows and by columns.
+constexpr int EPI_ROW = 36;
+constexpr int EPI_WARP_BYTES = 32 * EPI_ROW * 4;
+
 template <int CG>
 struct Shape {
-  static constexpr int STAGES = CG == 2 ? 6 : 4;
+  static constexpr int STAGES = CG == 2 ? 5 : 3;
   static constexpr int A_BYTES = BM * BK * 2;
   static constexpr int B_BYTES = BN / CG * BK * 2;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024;   // + alignment
+  static constexpr int SMEM = STAGES * STAGE_BYTES + EPI_WARPS * EPI_WARP_BYTES + 1024;   // + alignment
 };
 
 struct Ctl {
-  uint64_t full[6], empty[6], acc_full[2], acc_empty[2], drain;
+  uint64_t full[5], empty[5], acc_full[2], acc_empty[2], drain;
   uint32_t tmem;
   volatile uint32_t abort;
 };
@@ -186,8 +192,51 @@ __device__ __forceinline__ uint32_t idesc(const Problem& p) {
   return p.passes == 3 ? ID & ~((1u << 7) | (1u << 10)) : ID;
 }
 
-// The kernel's body.  epi(tile, v, row, first column, rows that count) runs on each epilogue
-// thread with 128 values of one row.
+// Calls put(i, c, x) for every 16 bytes x of the warp's 32 x 128 block: row i, columns c .. c+3.
+// Lanes 8k .. 8k+7 hold 128 bytes of one row.
+template <typename Put>
+__device__ __forceinline__ void by_rows4(float* stage, const float (&v)[BN / 2], Put&& put) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int ch = 0; ch < BN / 64; ++ch) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      *reinterpret_cast<float4*>(stage + lane * EPI_ROW + 4 * i) =
+          make_float4(v[32 * ch + 4 * i], v[32 * ch + 4 * i + 1], v[32 * ch + 4 * i + 2], v[32 * ch + 4 * i + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = 4 * j + (lane >> 3), c = 4 * (lane & 7);
+      put(i, 32 * ch + c, *reinterpret_cast<const float4*>(stage + i * EPI_ROW + c));
+    }
+  }
+}
+
+// The same with 8 columns per call, for 16-bit results: lanes 4k .. 4k+3 hold 64 bytes of a row.
+template <typename Put>
+__device__ __forceinline__ void by_rows8(float* stage, const float (&v)[BN / 2], Put&& put) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int ch = 0; ch < BN / 64; ++ch) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      *reinterpret_cast<float4*>(stage + lane * EPI_ROW + 4 * i) =
+          make_float4(v[32 * ch + 4 * i], v[32 * ch + 4 * i + 1], v[32 * ch + 4 * i + 2], v[32 * ch + 4 * i + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = 8 * j + (lane >> 2), c = 8 * (lane & 3);
+      const float4 a = *reinterpret_cast<const float4*>(stage + i * EPI_ROW + c);
+      const float4 b = *reinterpret_cast<const float4*>(stage + i * EPI_ROW + c + 4);
+      put(i, 32 * ch + c, a, b);
+    }
+  }
+}
+
+// The kernel's body.  epi(tile, v, row0, first column, rows that count, stage) runs on each
+// epilogue thread; v holds 128 values of row row0 + lane.
 template <int CG, bool A_MN, bool B_MN, typename Epi>
 __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c, Epi&& epi) {
   using S = Shape<CG>;
@@ -319,6 +368,7 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
     }
   } else {
     const int quad = warp & 3, half = (warp - 2) >> 2;
+    float* stage = reinterpret_cast<float*>(smem + S::STAGES * S::STAGE_BYTES + (warp - 2) * EPI_WARP_BYTES);
     uint32_t n = 0;
     bool ok = true;
     for (int64_t u = unit0; ok && u < units; u += step) {
@@ -353,7 +403,7 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
             ptx::mbar_arrive(&c->acc_empty[n & 1]);
         }
       }
-      if (ok) epi(t, v, (t.m * CG + (int)rank) * BM + 32 * quad + lane, t.n * BN + half * (BN / 2), live);
+      if (ok) epi(t, v, (t.m * CG + (int)rank) * BM + 32 * quad, t.n * BN + half * (BN / 2), live, stage);
     }
   }
   __syncwarp();

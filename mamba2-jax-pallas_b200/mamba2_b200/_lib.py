@@ -7,6 +7,7 @@ be loaded, or a tensor is not on a CUDA device, the call raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import os
@@ -295,6 +296,14 @@ def rows2d(t: torch.Tensor, width: int) -> torch.Tensor:
 def row_stride(t2: torch.Tensor) -> int:
     """Element stride between rows of a rows2d tensor (its width where there is one row)."""
     return t2.stride(0) if t2.shape[0] > 1 else t2.shape[1]
+
+
+_HERE_ALREADY = contextlib.nullcontext()
+
+
+def on_device(dev: torch.device):
+    """Context in which ``dev`` is the current device (launches go to the current one)."""
+    return _HERE_ALREADY if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def stream_of(t: torch.Tensor) -> int:

@@ -54,7 +54,7 @@ def _call(hidden, weight, targets, ignore_index, reduction, grad_loss, want_lse,
     p.hidden, p.weight, p.targets, p.loss = x.data_ptr(), w.data_ptr(), y.data_ptr(), loss.data_ptr()
     p.grad_loss, p.lse, p.grad_hidden, p.grad_weight = _lib.ptr(g), _lib.ptr(lse), _lib.ptr(gx), _lib.ptr(gw)
     lib = _lib.load()
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         ws = torch.empty(lib.ssd_linear_cross_entropy_workspace_bytes(p), device=dev, dtype=torch.uint8)
         _lib.check(lib.ssd_linear_cross_entropy(p, ws.data_ptr(), ws.numel(), _lib.stream_of(x)))
         if check_status:

@@ -47,7 +47,7 @@ def embedding(tokens, weight, scale: float = 1.0, *, padding_idx=None, out_dtype
         return out
     p.out_dtype = _lib.dtype_code(out)
     p.tokens, p.weight, p.out = ids.data_ptr(), w.data_ptr(), out.data_ptr()
-    with torch.cuda.device(w.device):
+    with _lib.on_device(w.device):
         _lib.check(_lib.load().ssd_embedding(p, _lib.stream_of(out)))
     return out
 
@@ -102,6 +102,6 @@ def embedding_grad(tokens, grad_out, num_embeddings: int, scale: float = 1.0, *,
     lib = _lib.load()
     n = lib.ssd_embedding_grad_workspace_bytes(p)
     ws = torch.empty(max(n, 1), device=g.device, dtype=torch.uint8)
-    with torch.cuda.device(g.device):
+    with _lib.on_device(g.device):
         _lib.check(lib.ssd_embedding_grad(p, ws.data_ptr(), ws.numel(), _lib.stream_of(out)))
     return out

@@ -8,35 +8,50 @@ import torch
 from .. import _lib
 
 _DTYPE = {torch.float32: _lib.SSD_DTYPE_F32, torch.bfloat16: _lib.SSD_DTYPE_BF16}
+_T = torch.Tensor
 
 
+# A model has hundreds of tensors, and the kernels take a few microseconds where they are
+# small: what is asked of each tensor goes through map() over the method itself.
 def _checked(ts, name):
+    """(list of tensors, their dtype codes, their device index), or an error."""
     ts = list(ts)
-    for t in ts:
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a list of torch.Tensor")
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be CUDA tensors (no CPU path)")
-        if t.dtype not in _DTYPE:
-            raise TypeError(f"unsupported dtype {t.dtype} (float32 or bfloat16)")
-        if t.device != ts[0].device:
-            raise ValueError(f"{name} must be on one device")
-    return ts
+    if not ts:
+        raise ValueError(f"{name} must not be empty")
+    try:
+        devices = set(map(_T.get_device, ts))
+    except TypeError:
+        raise TypeError(f"{name} must be a list of torch.Tensor") from None
+    if -1 in devices:
+        raise ValueError(f"{name} must be CUDA tensors (no CPU path)")
+    if len(devices) != 1:
+        raise ValueError(f"{name} must be on one device")
+    codes = [_DTYPE.get(t.dtype) for t in ts]
+    if None in codes:
+        raise TypeError(f"unsupported dtype {ts[codes.index(None)].dtype} (float32 or bfloat16)")
+    return ts, codes, devices.pop()
 
 
-def _run(grads, outs, max_norm, eps, scale):
+def _contiguous(ts):
+    return ts if all(map(_T.is_contiguous, ts)) else [t.contiguous() for t in ts]
+
+
+def _run(grads, codes, outs, out_codes, max_norm, eps, scale):
     dev = grads[0].device
     norm = torch.empty((), device=dev, dtype=torch.float32)
     # ssd_grad_tensor_t: two addresses, the size, two 32-bit dtypes
-    rec = array("q")
-    for g, o in zip(grads, outs):
-        rec.extend((g.data_ptr(), o.data_ptr(), g.numel(), _DTYPE[g.dtype] | _DTYPE[o.dtype] << 32))
+    n = len(grads)
+    rec = array("q", bytes(32 * n))
+    rec[0::4] = array("q", map(_T.data_ptr, grads))
+    rec[1::4] = rec[0::4] if outs is grads else array("q", map(_T.data_ptr, outs))
+    rec[2::4] = array("q", map(_T.numel, grads))
+    rec[3::4] = array("q", [g | o << 32 for g, o in zip(codes, out_codes)])
     lib = _lib.load()
     addr = rec.buffer_info()[0]
-    with torch.cuda.device(dev):
-        n = lib.ssd_clip_grad_norm_workspace_bytes(addr, len(grads))
-        ws = torch.empty(max(n, 8), device=dev, dtype=torch.uint8)
-        _lib.check(lib.ssd_clip_grad_norm(addr, len(grads), float(max_norm), float(eps), int(scale), norm.data_ptr(),
+    with _lib.on_device(dev):
+        size = lib.ssd_clip_grad_norm_workspace_bytes(addr, n)
+        ws = torch.empty(max(size, 8), device=dev, dtype=torch.uint8)
+        _lib.check(lib.ssd_clip_grad_norm(addr, n, float(max_norm), float(eps), int(scale), norm.data_ptr(),
                                           ws.data_ptr(), ws.numel(), _lib.stream_of(norm)))
     return norm
 
@@ -44,10 +59,9 @@ def _run(grads, outs, max_norm, eps, scale):
 def grad_norm(grads):
     """2-norm over all tensors of ``grads`` (float32 or bfloat16, any mix and shapes): a float32
     scalar tensor.  Squares are summed in float64."""
-    ts = [g.contiguous() for g in _checked(grads, "grads")]
-    if not ts:
-        raise ValueError("grads must not be empty")
-    return _run(ts, ts, 0.0, 0.0, False)
+    ts, codes, _ = _checked(grads, "grads")
+    ts = _contiguous(ts)
+    return _run(ts, codes, ts, codes, 0.0, 0.0, False)
 
 
 def clip_grad_norm(grads, max_norm: float, *, eps: float = 1e-6, out=None, inplace: bool = False):
@@ -59,29 +73,25 @@ def clip_grad_norm(grads, max_norm: float, *, eps: float = 1e-6, out=None, inpla
     gives tensors of the same shapes to write to, float32 or bfloat16 (bfloat16 gradients into
     the float32 buffers of an optimizer).  A NaN norm makes every gradient NaN.
     """
-    ts = _checked(grads, "grads")
-    if not ts:
-        raise ValueError("grads must not be empty")
+    ts, codes, device = _checked(grads, "grads")
     if not float(max_norm) >= 0.0 or not float(eps) >= 0.0:
         raise ValueError("max_norm and eps must be non-negative")
     if inplace:
         if out is not None:
             raise ValueError("give either out or inplace=True")
-        for g in ts:
-            if not g.is_contiguous():
-                raise ValueError("inplace=True needs contiguous gradients")
-        outs = ts
+        if not all(map(_T.is_contiguous, ts)):
+            raise ValueError("inplace=True needs contiguous gradients")
+        outs, out_codes = ts, codes
     else:
-        ts = [g.contiguous() for g in ts]
+        ts = _contiguous(ts)
         if out is None:
-            outs = [torch.empty_like(g) for g in ts]
+            outs, out_codes = [torch.empty_like(g) for g in ts], codes
         else:
-            outs = _checked(out, "out")
+            outs, out_codes, out_device = _checked(out, "out") if len(out) else ([], [], device)
             if len(outs) != len(ts):
                 raise ValueError(f"out has {len(outs)} tensors, grads {len(ts)}")
-            for g, o in zip(ts, outs):
-                if o.shape != g.shape or not o.is_contiguous():
-                    raise ValueError("out must hold contiguous tensors of grads' shapes")
-                if o.device != g.device:
-                    raise ValueError("out and grads must be on one device")
-    return outs, _run(ts, outs, max_norm, eps, True)
+            if list(map(_T.size, outs)) != list(map(_T.size, ts)) or not all(map(_T.is_contiguous, outs)):
+                raise ValueError("out must hold contiguous tensors of grads' shapes")
+            if out_device != device:
+                raise ValueError("out and grads must be on one device")
+    return outs, _run(ts, codes, outs, out_codes, max_norm, eps, True)
