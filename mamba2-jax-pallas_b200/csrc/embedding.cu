@@ -340,8 +340,53 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) zero_rows_kernel(const GradAr
 // ---------------------------------------------------------------------------
 constexpr int SUM_THREADS = 256;
 constexpr int SUM_COLS = 32 * VEC;   // columns of a warp
-constexpr int SUM_UNROLL = 8;        // rows in flight
 constexpr int EXTEND = 32;           // rows that a piece may take from the next one
+
+// A row's columns as they were loaded, unpacked when they are added: bf16 in flight takes half
+// the registers of f32, so twice the rows fit.
+template <typename T, Cols M>
+struct Raw {
+  static constexpr int ROWS = sizeof(T) == 2 && M != ONES ? 16 : 8;   // in flight
+  float v[VEC];
+  __device__ __forceinline__ void load(const T* row, int64_t left) { load_cols<T, M>(row, left, v); }
+  __device__ __forceinline__ void add(float (&acc)[VEC]) const {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] += v[k];
+  }
+};
+template <Cols M>
+struct RawPacked {
+  static constexpr int ROWS = 16;
+  uint32_t u[4];
+  __device__ __forceinline__ void load(const bf16* row, int64_t left) {
+    const int lane = threadIdx.x & 31;
+    if constexpr (M == EIGHT) {
+      uint4 q = make_uint4(0, 0, 0, 0);
+      if (lane * 8 < left) q = *reinterpret_cast<const uint4*>(row + lane * 8);
+      u[0] = q.x; u[1] = q.y; u[2] = q.z; u[3] = q.w;
+    } else {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        uint2 q = make_uint2(0, 0);
+        if (col_of<FOURS>(lane, 4 * g) < left) q = *reinterpret_cast<const uint2*>(row + col_of<FOURS>(lane, 4 * g));
+        u[2 * g] = q.x; u[2 * g + 1] = q.y;
+      }
+    }
+  }
+  __device__ __forceinline__ void add(float (&acc)[VEC]) const {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float a, b;
+      unpack2(u[k], a, b);
+      acc[2 * k] += a;
+      acc[2 * k + 1] += b;
+    }
+  }
+};
+template <>
+struct Raw<bf16, EIGHT> : RawPacked<EIGHT> {};
+template <>
+struct Raw<bf16, FOURS> : RawPacked<FOURS> {};
 
 template <typename TO, Cols M>
 __device__ __forceinline__ void put_row(const GradArgs& a, uint32_t id, int64_t c0, float (&acc)[VEC]) {
@@ -359,84 +404,87 @@ __device__ __forceinline__ void put_row(const GradArgs& a, uint32_t id, int64_t 
 
 // Warp (piece p, 256 columns): rows of the sorted positions [p * piece, + piece).
 template <typename TG, typename TO, Cols M>
-__global__ void __launch_bounds__(SUM_THREADS) grad_sum_kernel(const GradArgs a, int col_warps) {
+__global__ void __launch_bounds__(SUM_THREADS, 3) grad_sum_kernel(const GradArgs a, int col_warps) {
+  using R = Raw<TG, M>;
   ptx::griddep_wait();
   const int64_t unit = (int64_t)blockIdx.x * (SUM_THREADS / 32) + threadIdx.x / 32;
   const int64_t p = unit / col_warps;
   if (p >= a.npieces) return;
   const int lane = threadIdx.x & 31;
-  const int64_t c0 = (unit - p * col_warps) * SUM_COLS;
-  const int64_t lo = p * a.piece, hi = min(lo + a.piece, a.n);
+  const int64_t c0 = (unit - p * col_warps) * SUM_COLS, left = a.dim - c0;
+  const int64_t lo = p * a.piece, hi = min(lo + a.piece, a.n), top = a.n - 1;
   const uint32_t none = (uint32_t)a.vocab;
   const uint32_t* key = a.key[0];
   const uint32_t* pos = a.pos[0];
   const TG* g = static_cast<const TG*>(a.g) + c0;
-  uint32_t cur = key[lo];
+  // every key that decides about the piece's ends, in one round trip
+  const uint32_t first = key[lo], last = key[hi - 1];
+  const uint32_t k_prev = key[max(lo - 1, (int64_t)0)], k_before = key[max(lo - a.piece - 1, (int64_t)0)];
+  const uint32_t k_far = key[min(lo + EXTEND, top)], k_next = key[min(hi, top)], k_next_far = key[min(hi + EXTEND, top)];
+  const uint32_t k_ext = key[min(hi + lane, top)];
+  uint32_t mk = key[min(lo + lane, top)], mp = pos[min(lo + lane, top)];
+  uint32_t cur = first;
   if (cur == none) return;
   // the first id: it may have begun in an earlier piece, and then either the piece before
   // finishes it (skip) or this piece's share of it is a part (open)
-  bool open = lo > 0 && key[lo - 1] == cur, skip = false;
-  if (open) {
-    const int64_t before = lo - a.piece;
-    skip = (before == 0 || key[before - 1] != cur) && (lo + EXTEND >= a.n || key[lo + EXTEND] != cur);
-  }
+  bool open = lo > 0 && k_prev == first;
+  bool skip = open && (lo == a.piece || k_before != first) && (lo + EXTEND >= a.n || k_far != first);
   // the last id: rows of the next piece that this one takes, or the id goes on too long
   int64_t end = hi;
   bool goes_on = false;
-  const uint32_t last = key[hi - 1];
-  if (hi < a.n && last != none && key[hi] == last) {
-    const bool starts_here = lo == 0 || key[lo - 1] != last;
-    if (starts_here && (hi + EXTEND >= a.n || key[hi + EXTEND] != last))
-      end += __popc(__ballot_sync(0xffffffffu, hi + lane < a.n && key[min(hi + lane, a.n - 1)] == last));
+  if (hi < a.n && last != none && k_next == last) {
+    const bool starts_here = lo == 0 || k_prev != last;
+    if (starts_here && (hi + EXTEND >= a.n || k_next_far != last))
+      end += __popc(__ballot_sync(0xffffffffu, hi + lane < a.n && k_ext == last));
     else
       goes_on = true;
   }
   float acc[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+  auto close = [&]() {   // the id's rows of this piece are added up
+    if (open) {
+      if (!skip) store_cols<float, M>(a.part + (p * 2) * a.dim + c0, left, acc);
+    } else {
+      put_row<TO, M>(a, cur, c0, acc);
+    }
+  };
   for (int64_t i0 = lo; i0 < end && cur != none; i0 += 32) {
     const int m = (int)min((int64_t)32, end - i0);
-    const uint32_t mk = lane < m ? key[i0 + lane] : none;
-    const uint32_t mp = lane < m ? pos[i0 + lane] : 0;
-    for (int j0 = 0; j0 < m; j0 += SUM_UNROLL) {
-      float v[SUM_UNROLL][VEC];
+    if (i0 > lo) {
+      mk = key[min(i0 + lane, top)];
+      mp = pos[min(i0 + lane, top)];
+    }
+    if (lane >= m) mk = none;
+#pragma unroll 1
+    for (int j0 = 0; j0 < m; j0 += R::ROWS) {
+      R v[R::ROWS];
 #pragma unroll
-      for (int j = 0; j < SUM_UNROLL; ++j) {
+      for (int j = 0; j < R::ROWS; ++j) {
         const uint32_t kj = __shfl_sync(0xffffffffu, mk, j0 + j);
         const int64_t t = __shfl_sync(0xffffffffu, mp, j0 + j);
-        if (kj != none) load_cols<TG, M>(g + t * a.gs, a.dim - c0, v[j]);
+        v[j].load(g + t * a.gs, kj != none ? left : 0);
       }
 #pragma unroll
-      for (int j = 0; j < SUM_UNROLL; ++j) {
+      for (int j = 0; j < R::ROWS; ++j) {
         const uint32_t kj = __shfl_sync(0xffffffffu, mk, j0 + j);
-        if (j0 + j < m && cur != none) {
-          if (kj != cur) {
-            if (open) {
-              if (!skip) store_cols<float, M>(a.part + (p * 2) * a.dim + c0, a.dim - c0, acc);
-            } else {
-              put_row<TO, M>(a, cur, c0, acc);
-            }
-            open = skip = false;
-            cur = kj;
+        if (j0 + j < m && kj != cur && cur != none) {
+          close();
+          open = skip = false;
+          cur = kj;
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
-          }
-          if (kj != none) {
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) acc[k] += v[j][k];
-          }
+          for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
         }
+        v[j].add(acc);   // zeros past the end
       }
     }
   }
   if (cur == none) return;
-  if (open) {
-    if (!skip) store_cols<float, M>(a.part + (p * 2) * a.dim + c0, a.dim - c0, acc);
-  } else if (goes_on) {
-    store_cols<float, M>(a.part + (p * 2 + 1) * a.dim + c0, a.dim - c0, acc);
-    if (c0 == 0 && lane == 0) a.heavy[1 + atomicAdd(a.heavy, 1)] = (int)p;
+  if (open || !goes_on) {
+    close();
   } else {
-    put_row<TO, M>(a, cur, c0, acc);
+    store_cols<float, M>(a.part + (p * 2 + 1) * a.dim + c0, left, acc);
+    if (c0 == 0 && lane == 0) a.heavy[1 + atomicAdd(a.heavy, 1)] = (int)p;
   }
 }
 

@@ -25,7 +25,8 @@ namespace {
 constexpr int GC_THREADS = 256;
 constexpr int CHUNK = 8192;             // values; 32 per thread
 constexpr int MAX_TENSORS = 1000;       // 1000 x 28 bytes: inside the 32764 bytes of parameters
-constexpr int MAX_PARTIALS = 148 * 8;
+constexpr int CTAS_PER_SM = 4;          // resident (64 registers); a CTA's run of chunks is its share of all
+constexpr int MAX_PARTIALS = 148 * CTAS_PER_SM;
 
 template <int N>
 struct Table {
@@ -137,7 +138,7 @@ __device__ __forceinline__ double squares(const float (&v)[V]) {
 }
 
 template <typename T, int N>
-__global__ void __launch_bounds__(GC_THREADS) norm_kernel(const __grid_constant__ Table<N> t, double* partial) {
+__global__ void __launch_bounds__(GC_THREADS, CTAS_PER_SM) norm_kernel(const __grid_constant__ Table<N> t, double* partial) {
   constexpr int V = 16 / sizeof(T), U = CHUNK / GC_THREADS / V;
   __shared__ double sh[GC_THREADS / 32];
   const int c0 = (int)((int64_t)t.chunks * blockIdx.x / gridDim.x), c1 = (int)((int64_t)t.chunks * (blockIdx.x + 1) / gridDim.x);
@@ -169,7 +170,7 @@ __device__ __forceinline__ float2 norm_and_factor(const double* partial, int npa
 }
 
 template <typename T, typename TO, int N>
-__global__ void __launch_bounds__(GC_THREADS) scale_kernel(const __grid_constant__ Table<N> t, const double* partial,
+__global__ void __launch_bounds__(GC_THREADS, CTAS_PER_SM) scale_kernel(const __grid_constant__ Table<N> t, const double* partial,
                                                            int npartial, float max_norm, float eps, float* norm) {
   // 16 bytes of the wider type per access: neighbouring lanes write neighbouring 16 bytes
   constexpr int V = 16 / (sizeof(T) > sizeof(TO) ? sizeof(T) : sizeof(TO)), U = CHUNK / GC_THREADS / V;

@@ -6,7 +6,7 @@
 //
 // The work is three products of 2 T V D operations, so it is bound by the tensor pipe; what
 // lies between them is made small:
-//   loss       the GEMM's epilogue keeps, per row and 128 columns, the running maximum and the
+//   loss       the GEMM's epilogue keeps, per row and 64 columns, the running maximum and the
 //              sum of exponentials of the accumulator in TMEM: no logit leaves the SM but the
 //              target's.  The sums leave the target out, so that a token predicted with
 //              confidence keeps the digits of 1 - p, which a sum with p in it would lose.
@@ -30,6 +30,7 @@ namespace {
 
 using gemm::BM;
 using gemm::BN;
+constexpr int EC = gemm::EPI_COLS;
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr double LN2 = 0.6931471805599453;
@@ -267,7 +268,7 @@ size_t planes_bytes(int64_t rows, int64_t dim, int dtype) {
 struct LogitArgs {
   int64_t vocab;
   const int* target;       // of this chunk's rows
-  int ns;                  // statistics per row: one for each 128 columns
+  int ns;                  // statistics per row: one for each 64 columns
   float2* stats;           // (rows, ns), target left out: maximum * log2(e), sum of 2^(s log2(e) - that)
   float* picked;           // (rows): the target's logit
   float* logits;           // (rows, ld) or NULL
@@ -281,26 +282,29 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) logits_kernel(const __grid_c
   extern __shared__ uint8_t smem[];
   __shared__ gemm::Ctl ctl;
   const float unscale = p.passes == 3 ? 1.f / (scale_of(a.scales->x) * scale_of(a.scales->w)) : 1.f;
-  gemm::run<CG, false, false>(p, smem, &ctl, [&](const gemm::Tile& t, float (&v)[BN / 2], int row0, int n0, int live,
-                                                 float* stage) {
+  gemm::run<CG, false, false>(p, smem, &ctl, [&](const gemm::Tile& t, float (&v)[EC], int row0, int n0, int live,
+                                                 float4* stage) {
     const int row = row0 + (threadIdx.x & 31);
     const int y = row < live ? a.target[row] : -1;
     if (p.passes == 3) {
 #pragma unroll
-      for (int i = 0; i < BN / 2; ++i) v[i] *= unscale;
+      for (int i = 0; i < EC; ++i) v[i] *= unscale;
     }
-    if (a.logits)
+    if (a.logits) {
+      float* o = a.logits + row0 * a.ld + n0;
+      const int rows = live - row0, cols = (int)min((int64_t)EC, a.vocab - n0);
       gemm::by_rows4(stage, v, [&](int i, int c, float4 x) {
-        if (row0 + i < live && n0 + c < a.vocab) *reinterpret_cast<float4*>(a.logits + (row0 + i) * a.ld + n0 + c) = x;
+        if (i < rows && c < cols) *reinterpret_cast<float4*>(o + i * a.ld + c) = x;
       });
-    if (n0 + BN / 2 > a.vocab) {
-#pragma unroll
-      for (int i = 0; i < BN / 2; ++i) v[i] = n0 + i < a.vocab ? v[i] : -INFINITY;
     }
-    if (y >= n0 && y < n0 + BN / 2) {   // the target's logit is kept out of the sum
+    if (n0 + EC > a.vocab) {
+#pragma unroll
+      for (int i = 0; i < EC; ++i) v[i] = n0 + i < a.vocab ? v[i] : -INFINITY;
+    }
+    if (y >= n0 && y < n0 + EC) {   // the target's logit is kept out of the sum
       float s = 0.f;
 #pragma unroll
-      for (int i = 0; i < BN / 2; ++i) {
+      for (int i = 0; i < EC; ++i) {
         s = y == n0 + i ? v[i] : s;
         v[i] = y == n0 + i ? -INFINITY : v[i];
       }
@@ -308,13 +312,13 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) logits_kernel(const __grid_c
     }
     float m[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-    for (int i = 4; i < BN / 2; ++i) m[i & 3] = fmaxf(m[i & 3], v[i]);
+    for (int i = 4; i < EC; ++i) m[i & 3] = fmaxf(m[i & 3], v[i]);
     // the anchor is the rounded product itself, so that what is stored says what was summed
     const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * LOG2E, at = top == -INFINITY ? 0.f : top;
     float e[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < BN / 2; ++i) e[i & 3] += exp2f(fmaf(v[i], LOG2E, -at));
-    if (row < live) a.stats[(int64_t)row * a.ns + n0 / (BN / 2)] = make_float2(top, (e[0] + e[1]) + (e[2] + e[3]));
+    for (int i = 0; i < EC; ++i) e[i & 3] += exp2f(fmaf(v[i], LOG2E, -at));
+    if (row < live) a.stats[(int64_t)row * a.ns + n0 / (EC)] = make_float2(top, (e[0] + e[1]) + (e[2] + e[3]));
   });
 }
 
@@ -360,8 +364,15 @@ __device__ __forceinline__ RowResult warp_row(const float2* stats, int ns, const
   return r;
 }
 
+// What the row pass needs of a row: p of a column other than the target's is f 2^(s log2(e) - top).
+struct RowFactors {
+  float top, f, at_y;
+};
+
+// A warp per row that counts: its loss, and with `factors` what the gradients need.
 __global__ void __launch_bounds__(256) loss_kernel(const float2* stats, int ns, const float* picked, Selected s, int from,
-                                                   int rows, float* loss, float* lse) {
+                                                   int rows, float* loss, float* lse, const float* weight, int split,
+                                                   RowFactors* factors) {
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row >= rows || from + row >= *s.count) return;
   const RowResult r = warp_row(stats + row * ns, ns, picked + row, s.target[from + row]);
@@ -369,6 +380,10 @@ __global__ void __launch_bounds__(256) loss_kernel(const float2* stats, int ns, 
     const int t = s.index[from + row];
     loss[t] = r.loss;
     if (lse) lse[t] = r.lse;
+    if (factors) {
+      const float w = (weight ? weight[t] : 1.f) * (split ? scale_of(s.scales->dl) : 1.f);
+      factors[row] = {r.top, w * r.inv, w * r.pm1};
+    }
   }
 }
 
@@ -394,57 +409,48 @@ __global__ void __launch_bounds__(1024) reduce_kernel(const float* rows, int64_t
 struct RowArgs {
   int64_t vocab, ld;
   Selected sel;
-  int from, ns;            // first of the rows that count, of this chunk
-  const float2* stats;
-  const float* picked;
+  int from;                // first of the rows that count, of this chunk
+  const RowFactors* factors;
   const float* logits;
-  const float* weight;     // per-token factor or NULL
   void* dl[2];             // (rows, ld): bf16, or two f16 planes of dl times its scale
-  float* loss;             // (tokens)
-  float* lse;              // (tokens) or NULL
 };
 
-constexpr int ROW_THREADS = 512;
+constexpr int ROW_THREADS = 256, ROW_UNROLL = 8, ROW_COLS = ROW_THREADS * 4 * ROW_UNROLL;
 
-// One CTA per row that counts: lse and loss, then dl over the row.  Zero rows up to the next 64.
+// dl from the logits, ROW_COLS columns of a row per CTA, every load issued before the first use.
+// Zero rows up to the next 64.  HBM-bound: 6 bytes per logit (f32 inputs: 8).
 template <bool SPLIT>
 __global__ void __launch_bounds__(ROW_THREADS) row_kernel(const RowArgs a) {
-  __shared__ float sh_at, sh_inv, sh_y;
   const int64_t row = blockIdx.x;
   const int64_t live = (int64_t)*a.sel.count - a.from;
   if (live <= 0 || row >= (live + 63) / 64 * 64) return;
   const bool counted = row < live;
-  const int y = counted ? a.sel.target[a.from + row] : -1;
-  if (threadIdx.x < 32 && counted) {
-    const RowResult r = warp_row(a.stats + row * a.ns, a.ns, a.picked + row, y);
-    if (threadIdx.x == 0) {
-      const int token = a.sel.index[a.from + row];
-      const float w = a.weight ? a.weight[token] : 1.f;
-      sh_at = r.top;
-      const float scale = SPLIT ? scale_of(a.sel.scales->dl) : 1.f;
-      sh_inv = w * scale * r.inv;
-      sh_y = w * scale * r.pm1;
-      a.loss[token] = r.loss;
-      if (a.lse) a.lse[token] = r.lse;
-    }
-  }
-  __syncthreads();
-  const float at = counted ? sh_at : 0.f, f = counted ? sh_inv : 0.f, at_y = counted ? sh_y : 0.f;
+  const int64_t c0 = (int64_t)blockIdx.y * ROW_COLS + threadIdx.x * 4;
   const float* s = a.logits + row * a.ld;
+  float4 x[ROW_UNROLL];
+#pragma unroll
+  for (int u = 0; u < ROW_UNROLL; ++u) {
+    const int64_t c = c0 + u * ROW_THREADS * 4;
+    x[u] = counted && c < a.vocab ? *reinterpret_cast<const float4*>(s + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  const int y = counted ? a.sel.target[a.from + row] : -1;
+  RowFactors r = {0.f, 0.f, 0.f};
+  if (counted) r = a.factors[row];
   uint2* hi = reinterpret_cast<uint2*>(static_cast<bf16*>(a.dl[0]) + row * a.ld);
   uint2* lo = SPLIT ? reinterpret_cast<uint2*>(static_cast<__half*>(a.dl[1]) + row * a.ld) : nullptr;
-#pragma unroll 4
-  for (int64_t c = threadIdx.x * 4; c < a.vocab; c += ROW_THREADS * 4) {
+#pragma unroll
+  for (int u = 0; u < ROW_UNROLL; ++u) {
+    const int64_t c = c0 + u * ROW_THREADS * 4;
+    if (c >= a.vocab) break;
     float d[4] = {0.f, 0.f, 0.f, 0.f};
     if (counted) {
-      const float4 v = *reinterpret_cast<const float4*>(s + c);
-      d[0] = f * exp2f(fmaf(v.x, LOG2E, -at));
-      d[1] = f * exp2f(fmaf(v.y, LOG2E, -at));
-      d[2] = f * exp2f(fmaf(v.z, LOG2E, -at));
-      d[3] = f * exp2f(fmaf(v.w, LOG2E, -at));
+      d[0] = r.f * exp2f(fmaf(x[u].x, LOG2E, -r.top));
+      d[1] = r.f * exp2f(fmaf(x[u].y, LOG2E, -r.top));
+      d[2] = r.f * exp2f(fmaf(x[u].z, LOG2E, -r.top));
+      d[3] = r.f * exp2f(fmaf(x[u].w, LOG2E, -r.top));
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (c + k == y) d[k] = at_y;
+        if (c + k == y) d[k] = r.at_y;
     }
     if constexpr (SPLIT) {
       __half2 h[2] = {__floats2half2_rn(d[0], d[1]), __floats2half2_rn(d[2], d[3])};
@@ -471,84 +477,85 @@ struct OutArgs {
   const unsigned* largest[2];   // f32 inputs: what the operands' scales come from
 };
 
-template <int CG, bool A_MN>
+// Where a gradient's tile goes: to the output, times alpha, or through `part`.
+enum Out { OUT_BF16, OUT_F32, OUT_PART };
+
+template <int CG, bool A_MN, Out MODE>
 __global__ void __launch_bounds__(gemm::THREADS, 1) grad_gemm_kernel(const __grid_constant__ gemm::Problem p,
                                                                      const __grid_constant__ OutArgs a) {
   extern __shared__ uint8_t smem[];
   __shared__ gemm::Ctl ctl;
-  const float unscale = p.passes == 3 ? 1.f / scale_of(*a.largest[0]) / scale_of(*a.largest[1]) : 1.f;
-  const float alpha = a.out ? *a.alpha : 1.f;
-  gemm::run<CG, A_MN, true>(p, smem, &ctl, [&](const gemm::Tile& t, float (&v)[BN / 2], int row0, int n0, int live,
-                                               float* stage) {
-    const int64_t rows = p.limit_k ? a.rows : live;
-    if (row0 >= rows || n0 >= a.cols) return;
-    const float f = unscale * (a.part ? 1.f : alpha);
+  float f = p.passes == 3 ? 1.f / scale_of(*a.largest[0]) / scale_of(*a.largest[1]) : 1.f;
+  const float alpha = *a.alpha;
+  if (MODE != OUT_PART) f *= alpha;
+  gemm::run<CG, A_MN, true>(p, smem, &ctl, [&](const gemm::Tile& t, float (&v)[EC], int row0, int n0, int live,
+                                               float4* stage) {
+    const int rows = (int)min((int64_t)32, (p.limit_k ? a.rows : live) - row0);
+    const int cols = (int)min((int64_t)EC, a.cols - n0);
+    if (rows <= 0 || cols <= 0) return;
 #pragma unroll
-    for (int i = 0; i < BN / 2; ++i) v[i] *= f;
-    if (a.part) {
-      // parts stay as they are; the running sum takes alpha when it is complete
-      float* part = a.part + ((int64_t)t.split * a.rows + row0) * a.cols + n0;
-      const bool vec = vec_rows(part, a.cols);
-      gemm::by_rows4(stage, v, [&](int i, int c, float4 x) {
-        if (row0 + i >= rows || n0 + c >= a.cols) return;
-        float* q = part + i * a.cols + c;
-        float y[4] = {x.x, x.y, x.z, x.w};
-        const bool whole = vec && n0 + c + 4 <= a.cols;
-        if (a.add_part) {
-          if (whole) {
-            const float4 o = *reinterpret_cast<const float4*>(q);
-            y[0] += o.x; y[1] += o.y; y[2] += o.z; y[3] += o.w;
-          } else {
-            for (int k = 0; k < 4; ++k)
-              if (n0 + c + k < a.cols) y[k] += q[k];
-          }
-        }
-        if (!a.out) {
-          if (whole) {
-            *reinterpret_cast<float4*>(q) = make_float4(y[0], y[1], y[2], y[3]);
-          } else {
-            for (int k = 0; k < 4; ++k)
-              if (n0 + c + k < a.cols) q[k] = y[k];
-          }
-          return;
-        }
-        const int64_t at = (row0 + i) * a.cols + n0 + c;
-        for (int k = 0; k < 4; ++k)
-          if (n0 + c + k < a.cols) {
-            if (a.out_bf16) static_cast<bf16*>(a.out)[at + k] = __float2bfloat16_rn(y[k] * alpha);
-            else static_cast<float*>(a.out)[at + k] = y[k] * alpha;
-          }
-      });
-      return;
-    }
-    if (a.out_bf16) {
+    for (int i = 0; i < EC; ++i) v[i] *= f;
+    if constexpr (MODE == OUT_BF16) {
       bf16* out = static_cast<bf16*>(a.out) + n0;
       const bool vec = vec_rows(out, a.cols);
       gemm::by_rows8(stage, v, [&](int i, int c, float4 x, float4 y) {
-        if (row0 + i >= rows || n0 + c >= a.cols) return;
+        if (i >= rows || c >= cols) return;
         bf16* o = out + (a.index ? a.index[row0 + i] : row0 + i) * a.cols + c;
         __nv_bfloat162 h[4] = {__floats2bfloat162_rn(x.x, x.y), __floats2bfloat162_rn(x.z, x.w),
                                __floats2bfloat162_rn(y.x, y.y), __floats2bfloat162_rn(y.z, y.w)};
-        if (vec && n0 + c + 8 <= a.cols) {
+        if (vec && c + 8 <= cols) {
           *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(h);
         } else {
           const bf16* e = reinterpret_cast<const bf16*>(h);
+#pragma unroll
           for (int k = 0; k < 8; ++k)
-            if (n0 + c + k < a.cols) o[k] = e[k];
+            if (c + k < cols) o[k] = e[k];
         }
       });
     } else {
-      float* out = static_cast<float*>(a.out) + n0;
+      // parts and running sums stay without alpha until they are complete
+      float* out = MODE == OUT_F32 ? static_cast<float*>(a.out) + n0
+                                   : a.part + ((int64_t)t.split * a.rows + row0) * a.cols + n0;
       const bool vec = vec_rows(out, a.cols);
       gemm::by_rows4(stage, v, [&](int i, int c, float4 x) {
-        if (row0 + i >= rows || n0 + c >= a.cols) return;
-        float* o = out + (a.index ? a.index[row0 + i] : row0 + i) * a.cols + c;
-        if (vec && n0 + c + 4 <= a.cols) {
-          *reinterpret_cast<float4*>(o) = x;
+        if (i >= rows || c >= cols) return;
+        float e[4] = {x.x, x.y, x.z, x.w};
+        const bool whole = vec && c + 4 <= cols;
+        float* o = out + (MODE == OUT_F32 ? (a.index ? a.index[row0 + i] : row0 + i) : i) * a.cols + c;
+        if (MODE == OUT_PART && a.add_part) {
+          if (whole) {
+            const float4 q = *reinterpret_cast<const float4*>(o);
+            e[0] += q.x; e[1] += q.y; e[2] += q.z; e[3] += q.w;
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (c + k < cols) e[k] += o[k];
+          }
+        }
+        if (MODE == OUT_PART && a.out) {
+          const int64_t at = (row0 + i) * a.cols + n0 + c;
+          if (a.out_bf16) {
+            bf16* w = static_cast<bf16*>(a.out) + at;
+            if (whole && reinterpret_cast<uintptr_t>(w) % 8 == 0) {
+              __nv_bfloat162 h[2] = {__floats2bfloat162_rn(e[0] * alpha, e[1] * alpha), __floats2bfloat162_rn(e[2] * alpha, e[3] * alpha)};
+              *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(h);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (c + k < cols) w[k] = __float2bfloat16_rn(e[k] * alpha);
+            }
+          } else {
+            float* w = static_cast<float*>(a.out) + at;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (c + k < cols) w[k] = e[k] * alpha;
+          }
+        } else if (whole) {
+          *reinterpret_cast<float4*>(o) = make_float4(e[0], e[1], e[2], e[3]);
         } else {
-          const float e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (n0 + c + k < a.cols) o[k] = e[k];
+            if (c + k < cols) o[k] = e[k];
         }
       });
     }
@@ -637,7 +644,7 @@ struct Plan {
   int64_t chunk, nchunks, ns, ld;   // tokens of a chunk; statistics per row; logits' row length
   int splits;                       // of the reduction over the vocabulary (dX)
   bool pack_w, sum_w;       // sum_w: dW's running sum over chunks needs its own f32 buffer
-  size_t one, index, target, rows, picked, stats, x, w, logits, dl[2], part, wsum, total;
+  size_t one, index, target, rows, picked, factors, stats, x, w, logits, dl[2], part, wsum, total;
 };
 
 int split_k(int64_t rows, int64_t dim, int64_t vocab) {
@@ -661,7 +668,7 @@ Plan plan_of(const ssd_linear_ce_params_t* p) {
   Plan q{};
   q.grad = p->grad_hidden || p->grad_weight;
   q.planes = p->dtype == SSD_DTYPE_F32 ? 2 : 1;
-  q.ns = 2 * (int64_t)cdiv(p->vocab, BN);
+  q.ns = BN / EC * (int64_t)cdiv(p->vocab, BN);
   q.ld = (p->vocab + 63) / 64 * 64;
   if (q.grad) {
     const int64_t per = q.ld * (4 + 2 * q.planes);
@@ -686,6 +693,7 @@ Plan plan_of(const ssd_linear_ce_params_t* p) {
   q.target = take((size_t)p->tokens * 4);
   q.rows = take(p->reduction == SSD_REDUCE_NONE ? 0 : (size_t)p->tokens * 4);
   q.picked = take((size_t)q.chunk * 4);
+  q.factors = take(q.grad ? (size_t)q.chunk * sizeof(RowFactors) : 0);
   q.stats = take((size_t)q.chunk * q.ns * 8);
   q.x = take(planes_bytes(p->tokens, p->dim, p->dtype));
   q.w = take(q.pack_w ? planes_bytes(p->vocab, p->dim, p->dtype) : 0);
@@ -745,7 +753,9 @@ cudaError_t grad_gemm(const Operand& a, const Operand& b, int64_t k, int planes,
   // bf16: the operands' own rounding is a hundred times what the adds lose
   g.segment = planes == 2 ? SEGMENT_F32 : 1 << 20;
   g.status = status;
-  return launch_gemm<CG>(grad_gemm_kernel<CG, A_MN>, g, o, st);
+  if (o.part) return launch_gemm<CG>(grad_gemm_kernel<CG, A_MN, OUT_PART>, g, o, st);
+  if (o.out_bf16) return launch_gemm<CG>(grad_gemm_kernel<CG, A_MN, OUT_BF16>, g, o, st);
+  return launch_gemm<CG>(grad_gemm_kernel<CG, A_MN, OUT_F32>, g, o, st);
 }
 
 }  // namespace
@@ -822,19 +832,17 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
     a.scales = sel.scales;
     if (n > BM) CE_CHECK(logits_gemm<2>(xc, w, q.planes, a, sel.count, from, status, st), "logits");
     else CE_CHECK(logits_gemm<1>(xc, w, q.planes, a, sel.count, from, status, st), "logits");
-    if (!q.grad) {
-      loss_kernel<<<(unsigned)cdiv(n, 8), 256, 0, st>>>(a.stats, a.ns, a.picked, sel, from, (int)n, rows, p->lse);
-      CE_CHECK(cudaGetLastError(), "loss");
-      continue;
-    }
+    RowFactors* factors = q.grad ? reinterpret_cast<RowFactors*>(ws + q.factors) : nullptr;
+    loss_kernel<<<(unsigned)cdiv(n, 8), 256, 0, st>>>(a.stats, a.ns, a.picked, sel, from, (int)n, rows, p->lse,
+                                                     per_row ? p->grad_loss : nullptr, q.planes == 2, factors);
+    CE_CHECK(cudaGetLastError(), "loss");
+    if (!q.grad) continue;
     RowArgs r{};
-    r.vocab = p->vocab; r.ld = q.ld; r.sel = sel; r.from = from;
-    r.ns = a.ns; r.stats = a.stats; r.picked = a.picked; r.logits = a.logits;
-    r.weight = per_row ? p->grad_loss : nullptr;
+    r.vocab = p->vocab; r.ld = q.ld; r.sel = sel; r.from = from; r.factors = factors; r.logits = a.logits;
     for (int i = 0; i < q.planes; ++i) r.dl[i] = ws + q.dl[i];
-    r.loss = rows; r.lse = p->lse;
-    if (q.planes == 2) row_kernel<true><<<(unsigned)n, ROW_THREADS, 0, st>>>(r);
-    else row_kernel<false><<<(unsigned)n, ROW_THREADS, 0, st>>>(r);
+    const dim3 row_grid((unsigned)n, (unsigned)cdiv(p->vocab, ROW_COLS));
+    if (q.planes == 2) row_kernel<true><<<row_grid, ROW_THREADS, 0, st>>>(r);
+    else row_kernel<false><<<row_grid, ROW_THREADS, 0, st>>>(r);
     CE_CHECK(cudaGetLastError(), "rows");
     Operand dl{};
     dl.rows = n; dl.dim = p->vocab; dl.ld = q.ld;

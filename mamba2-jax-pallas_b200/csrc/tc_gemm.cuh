@@ -7,7 +7,9 @@
 // pipe's rate is 16 TB/s over the GPU; a pair needs 32 KB per SM.  Warps:
 //   0     TMA producer: A and B boxes into a ring of shared-memory stages
 //   1     MMA issuer (the pair's first CTA only issues): four K = 16 MMAs per stage
-//   2..9  epilogue: warp w reads the TMEM lanes of quadrant w % 4, column half (w - 2) / 4
+//   2..17 epilogue: warp w reads the TMEM lanes of quadrant w % 4, 64 columns at (w - 2) / 4 * 64
+// (16 epilogue warps: with 8 of 128 columns each, two per scheduler, the epilogue of a K = 1000
+// tile took longer than its MMAs.)
 // Two accumulators (2 x 256 TMEM columns) let the reading of one overlap the MMAs into the
 // other.  Operands are K-major (the reduced dimension contiguous in memory) or MN-major (the
 // other one contiguous), so no operand is ever transposed in memory.
@@ -15,7 +17,7 @@
 // The tensor core's f32 adds truncate: over K = 4096 a dot product loses about 1e-5 of its
 // value, always towards zero.  So a tile's K range runs in segments, each from zero in its own
 // TMEM accumulator, and the epilogue warps add the segments in registers, rounding to nearest:
-// 128 values per thread.
+// 64 values per thread.
 //
 // f32 operands come as two f16 planes of the values times a power of two, v = hi + lo, and the
 // K loop runs over the plane pairs hi*lo, lo*hi, hi*hi.  Two f16 hold 22 bits of a value down
@@ -34,19 +36,20 @@ namespace gemm {
 constexpr int BK = 64;                    // one 128-byte swizzled row
 constexpr int BN = 256;                   // columns of a tile
 constexpr int BM = 128;                   // rows of a CTA's part of a tile
-constexpr int EPI_WARPS = 8;
+constexpr int EPI_WARPS = 16;
+constexpr int EPI_COLS = 64;               // columns of an epilogue warp
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr long long WAIT_CYCLES = 4000000000LL;   // about 2 s at the boost clock
 
-// Each epilogue warp turns its rows through shared memory, 32 columns at a time, so that what it
-// writes to global memory are runs of one row and not one value of 32 rows.  Rows 36 floats
-// apart: 16-byte accesses of a quarter-warp fall into different banks, by rows and by columns.
-constexpr int EPI_ROW = 36;
-constexpr int EPI_WARP_BYTES = 32 * EPI_ROW * 4;
+// Each epilogue warp turns its rows through shared memory, 16 columns at a time, so that what it
+// writes to global memory are runs of one row and not one value of 32 rows.  A row's four
+// 16-byte chunks are permuted by its number, which keeps the accesses of a quarter-warp in
+// different banks, by rows and by columns.
+constexpr int EPI_WARP_BYTES = 32 * 64;
 
 template <int CG>
 struct Shape {
-  static constexpr int STAGES = CG == 2 ? 5 : 3;
+  static constexpr int STAGES = CG == 2 ? 6 : 4;
   static constexpr int A_BYTES = BM * BK * 2;
   static constexpr int B_BYTES = BN / CG * BK * 2;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
@@ -54,7 +57,7 @@ struct Shape {
 };
 
 struct Ctl {
-  uint64_t full[5], empty[5], acc_full[2], acc_empty[2], drain;
+  uint64_t full[6], empty[6], acc_full[2], acc_empty[2], drain;
   uint32_t tmem;
   volatile uint32_t abort;
 };
@@ -99,10 +102,24 @@ __device__ __forceinline__ Tile tile_at(const Problem& p, int m_tiles, int k_blo
   return t;
 }
 
+// A probe that lets the hardware suspend the thread for up to a millisecond: 16 waiting
+// epilogue warps that poll cost 10 % of a power-bound GEMM.
+__device__ __forceinline__ bool probe(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(ptx::smem_u32(bar)), "r"(parity), "r"(1000000)
+      : "memory");
+  return ok != 0;
+}
+
 __device__ __forceinline__ bool wait(Ctl* c, uint64_t* bar, uint32_t parity, unsigned* status, int id) {
-  if (ptx::mbar_try_wait(bar, parity)) return true;
+  if (probe(bar, parity)) return true;
   const long long t0 = clock64();
-  while (!ptx::mbar_try_wait(bar, parity)) {
+  while (!probe(bar, parity)) {
     if (c->abort) return false;
     if (clock64() - t0 > WAIT_CYCLES) {
       atomicCAS(status, 0u, (unsigned)(0x100 | id));
@@ -192,51 +209,51 @@ __device__ __forceinline__ uint32_t idesc(const Problem& p) {
   return p.passes == 3 ? ID & ~((1u << 7) | (1u << 10)) : ID;
 }
 
-// Calls put(i, c, x) for every 16 bytes x of the warp's 32 x 128 block: row i, columns c .. c+3.
-// Lanes 8k .. 8k+7 hold 128 bytes of one row.
+__device__ __forceinline__ void epi_put(float4* stage, const float* v) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    stage[lane * 4 + (i ^ ((lane >> 1) & 3))] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  __syncwarp();
+}
+__device__ __forceinline__ float4 epi_get(const float4* stage, int row, int chunk) {
+  return stage[row * 4 + (chunk ^ ((row >> 1) & 3))];
+}
+
+// Calls put(i, c, x) for every 16 bytes x of the warp's 32 x 64 block: row i, columns c .. c+3.
+// Lanes 4k .. 4k+3 hold 64 bytes of one row.
 template <typename Put>
-__device__ __forceinline__ void by_rows4(float* stage, const float (&v)[BN / 2], Put&& put) {
+__device__ __forceinline__ void by_rows4(float4* stage, const float (&v)[EPI_COLS], Put&& put) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int ch = 0; ch < BN / 64; ++ch) {
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      *reinterpret_cast<float4*>(stage + lane * EPI_ROW + 4 * i) =
-          make_float4(v[32 * ch + 4 * i], v[32 * ch + 4 * i + 1], v[32 * ch + 4 * i + 2], v[32 * ch + 4 * i + 3]);
-    __syncwarp();
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int i = 4 * j + (lane >> 3), c = 4 * (lane & 7);
-      put(i, 32 * ch + c, *reinterpret_cast<const float4*>(stage + i * EPI_ROW + c));
+  for (int ch = 0; ch < EPI_COLS / 16; ++ch) {
+    epi_put(stage, v + 16 * ch);
+#pragma unroll 2
+    for (int j = 0; j < 4; ++j) {
+      const int i = 8 * j + (lane >> 2);
+      put(i, 16 * ch + 4 * (lane & 3), epi_get(stage, i, lane & 3));
     }
   }
 }
 
-// The same with 8 columns per call, for 16-bit results: lanes 4k .. 4k+3 hold 64 bytes of a row.
+// The same with 8 columns per call, for 16-bit results: lanes 2k and 2k+1 hold 32 bytes of a row.
 template <typename Put>
-__device__ __forceinline__ void by_rows8(float* stage, const float (&v)[BN / 2], Put&& put) {
+__device__ __forceinline__ void by_rows8(float4* stage, const float (&v)[EPI_COLS], Put&& put) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int ch = 0; ch < BN / 64; ++ch) {
-    __syncwarp();
+  for (int ch = 0; ch < EPI_COLS / 16; ++ch) {
+    epi_put(stage, v + 16 * ch);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      *reinterpret_cast<float4*>(stage + lane * EPI_ROW + 4 * i) =
-          make_float4(v[32 * ch + 4 * i], v[32 * ch + 4 * i + 1], v[32 * ch + 4 * i + 2], v[32 * ch + 4 * i + 3]);
-    __syncwarp();
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = 8 * j + (lane >> 2), c = 8 * (lane & 3);
-      const float4 a = *reinterpret_cast<const float4*>(stage + i * EPI_ROW + c);
-      const float4 b = *reinterpret_cast<const float4*>(stage + i * EPI_ROW + c + 4);
-      put(i, 32 * ch + c, a, b);
+    for (int j = 0; j < 2; ++j) {
+      const int i = 16 * j + (lane >> 1), c = 2 * (lane & 1);
+      put(i, 16 * ch + 4 * c, epi_get(stage, i, c), epi_get(stage, i, c + 1));
     }
   }
 }
 
 // The kernel's body.  epi(tile, v, row0, first column, rows that count, stage) runs on each
-// epilogue thread; v holds 128 values of row row0 + lane.
+// epilogue thread; v holds 64 values of row row0 + lane.
 template <int CG, bool A_MN, bool B_MN, typename Epi>
 __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c, Epi&& epi) {
   using S = Shape<CG>;
@@ -367,15 +384,15 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
       }
     }
   } else {
-    const int quad = warp & 3, half = (warp - 2) >> 2;
-    float* stage = reinterpret_cast<float*>(smem + S::STAGES * S::STAGE_BYTES + (warp - 2) * EPI_WARP_BYTES);
+    const int quad = warp & 3, col = (warp - 2) / 4 * EPI_COLS;
+    float4* stage = reinterpret_cast<float4*>(smem + S::STAGES * S::STAGE_BYTES + (warp - 2) * EPI_WARP_BYTES);
     uint32_t n = 0;
     bool ok = true;
     for (int64_t u = unit0; ok && u < units; u += step) {
       const Tile t = tile_at(p, m_tiles, k_blocks, u);
-      float v[BN / 2];
+      float v[EPI_COLS];
 #pragma unroll
-      for (int i = 0; i < BN / 2; ++i) v[i] = 0.f;
+      for (int i = 0; i < EPI_COLS; ++i) v[i] = 0.f;
       for (int left = p.passes * (t.k1 - t.k0); left > 0; left -= p.segment, ++n) {
         // one lane waits for the warp, so that the warp stays converged for its TMEM loads
         int there = 0;
@@ -385,14 +402,14 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
           break;
         }
         ptx::tc_fence_after();
-        const uint32_t from = tmem + (n & 1) * BN + half * (BN / 2) + ((uint32_t)(32 * quad) << 16);
+        const uint32_t from = tmem + (n & 1) * BN + col + ((uint32_t)(32 * quad) << 16);
 #pragma unroll
-        for (int ch = 0; ch < BN / 64; ++ch) {
-          float x[32];
-          ptx::tmem_ld32(from + 32 * ch, x);
+        for (int ch = 0; ch < EPI_COLS / 16; ++ch) {
+          float x[16];
+          ptx::tmem_ld16(from + 16 * ch, x);
           ptx::tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[32 * ch + i] += x[i];
+          for (int i = 0; i < 16; ++i) v[16 * ch + i] += x[i];
         }
         ptx::tc_fence_before();
         __syncwarp();
@@ -403,7 +420,7 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
             ptx::mbar_arrive(&c->acc_empty[n & 1]);
         }
       }
-      if (ok) epi(t, v, (t.m * CG + (int)rank) * BM + 32 * quad, t.n * BN + half * (BN / 2), live, stage);
+      if (ok) epi(t, v, (t.m * CG + (int)rank) * BM + 32 * quad, t.n * BN + col, live, stage);
     }
   }
   __syncwarp();
