@@ -514,8 +514,9 @@ namespace {
 int check_embedding_grad(const ssd_embedding_grad_params_t* p) {
   if (!p) return fail(SSD_ERR_INVALID_ARG, "params is NULL");
   if (p->num_tokens < 0 || p->vocab <= 0 || p->dim <= 0) return fail(SSD_ERR_INVALID_ARG, "dims must be positive");
-  if (p->num_tokens > INT32_MAX || p->vocab > INT32_MAX || p->dim > INT32_MAX)
-    return fail(SSD_ERR_UNSUPPORTED, "dims must be below 2^31");
+  // positions, pieces and columns are 32-bit in the kernels
+  if (p->num_tokens > ((int64_t)1 << 30) || p->vocab > INT32_MAX || p->dim > (1 << 24))
+    return fail(SSD_ERR_UNSUPPORTED, "num_tokens must be at most 2^30, vocab below 2^31 and dim at most 2^24");
   return SSD_OK;
 }
 

@@ -346,7 +346,7 @@ constexpr int EXTEND = 32;           // rows that a piece may take from the next
 // the registers of f32, so twice the rows fit.
 template <typename T, Cols M>
 struct Raw {
-  static constexpr int ROWS = sizeof(T) == 2 && M != ONES ? 16 : 8;   // in flight
+  static constexpr int ROWS = 4;    // in flight
   float v[VEC];
   __device__ __forceinline__ void load(const T* row, int64_t left) { load_cols<T, M>(row, left, v); }
   __device__ __forceinline__ void add(float (&acc)[VEC]) const {
@@ -356,7 +356,7 @@ struct Raw {
 };
 template <Cols M>
 struct RawPacked {
-  static constexpr int ROWS = 16;
+  static constexpr int ROWS = 8;
   uint32_t u[4];
   __device__ __forceinline__ void load(const bf16* row, int64_t left) {
     const int lane = threadIdx.x & 31;
@@ -404,87 +404,87 @@ __device__ __forceinline__ void put_row(const GradArgs& a, uint32_t id, int64_t 
 
 // Warp (piece p, 256 columns): rows of the sorted positions [p * piece, + piece).
 template <typename TG, typename TO, Cols M>
-__global__ void __launch_bounds__(SUM_THREADS, 3) grad_sum_kernel(const GradArgs a, int col_warps) {
+__global__ void __launch_bounds__(SUM_THREADS, 4) grad_sum_kernel(const __grid_constant__ GradArgs a, int col_warps) {
   using R = Raw<TG, M>;
   ptx::griddep_wait();
-  const int64_t unit = (int64_t)blockIdx.x * (SUM_THREADS / 32) + threadIdx.x / 32;
-  const int64_t p = unit / col_warps;
-  if (p >= a.npieces) return;
-  const int lane = threadIdx.x & 31;
-  const int64_t c0 = (unit - p * col_warps) * SUM_COLS, left = a.dim - c0;
-  const int64_t lo = p * a.piece, hi = min(lo + a.piece, a.n), top = a.n - 1;
+  const int unit = blockIdx.x * (SUM_THREADS / 32) + threadIdx.x / 32;
+  const int p = unit / col_warps;
+  if (p >= (int)a.npieces) return;
+  const int lane = threadIdx.x & 31, n = (int)a.n, top = n - 1, piece = (int)a.piece;
+  const int c0 = (unit - p * col_warps) * SUM_COLS, left = (int)a.dim - c0;
+  const int lo = p * piece, hi = min(lo + piece, n);
   const uint32_t none = (uint32_t)a.vocab;
   const uint32_t* key = a.key[0];
   const uint32_t* pos = a.pos[0];
-  const TG* g = static_cast<const TG*>(a.g) + c0;
   // every key that decides about the piece's ends, in one round trip
   const uint32_t first = key[lo], last = key[hi - 1];
-  const uint32_t k_prev = key[max(lo - 1, (int64_t)0)], k_before = key[max(lo - a.piece - 1, (int64_t)0)];
+  const uint32_t k_prev = key[max(lo - 1, 0)], k_before = key[max(lo - piece - 1, 0)];
   const uint32_t k_far = key[min(lo + EXTEND, top)], k_next = key[min(hi, top)], k_next_far = key[min(hi + EXTEND, top)];
   const uint32_t k_ext = key[min(hi + lane, top)];
-  uint32_t mk = key[min(lo + lane, top)], mp = pos[min(lo + lane, top)];
-  uint32_t cur = first;
-  if (cur == none) return;
+  uint32_t mk = key[min(lo + lane, top)];
+  int mp = (int)pos[min(lo + lane, top)];
+  if (first == none) return;
   // the first id: it may have begun in an earlier piece, and then either the piece before
   // finishes it (skip) or this piece's share of it is a part (open)
   bool open = lo > 0 && k_prev == first;
-  bool skip = open && (lo == a.piece || k_before != first) && (lo + EXTEND >= a.n || k_far != first);
+  const bool skip = open && (lo == piece || k_before != first) && (lo + EXTEND >= n || k_far != first);
   // the last id: rows of the next piece that this one takes, or the id goes on too long
-  int64_t end = hi;
+  int end = hi;
   bool goes_on = false;
-  if (hi < a.n && last != none && k_next == last) {
-    const bool starts_here = lo == 0 || k_prev != last;
-    if (starts_here && (hi + EXTEND >= a.n || k_next_far != last))
-      end += __popc(__ballot_sync(0xffffffffu, hi + lane < a.n && k_ext == last));
+  if (hi < n && last != none && k_next == last) {
+    if ((lo == 0 || k_prev != last) && (hi + EXTEND >= n || k_next_far != last))
+      end += __popc(__ballot_sync(0xffffffffu, hi + lane < n && k_ext == last));
     else
       goes_on = true;
   }
   float acc[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
-  auto close = [&]() {   // the id's rows of this piece are added up
+  uint32_t cur = first;
+  auto close = [&]() {   // the rows of `cur` in this piece are added up
     if (open) {
-      if (!skip) store_cols<float, M>(a.part + (p * 2) * a.dim + c0, left, acc);
-    } else {
+      if (!skip) store_cols<float, M>(a.part + (int64_t)(p * 2) * a.dim + c0, left, acc);
+    } else if (cur != none) {
       put_row<TO, M>(a, cur, c0, acc);
     }
+    open = false;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
   };
-  for (int64_t i0 = lo; i0 < end && cur != none; i0 += 32) {
-    const int m = (int)min((int64_t)32, end - i0);
+  for (int i0 = lo; i0 < end; i0 += 32) {
     if (i0 > lo) {
       mk = key[min(i0 + lane, top)];
-      mp = pos[min(i0 + lane, top)];
+      mp = (int)pos[min(i0 + lane, top)];
     }
-    if (lane >= m) mk = none;
+    const int m = min(32, end - i0);
+    // rows that add something, and rows at which another id begins
+    const unsigned live = __ballot_sync(0xffffffffu, lane < m && mk != none);
+    uint32_t before = __shfl_up_sync(0xffffffffu, mk, 1);
+    if (lane == 0) before = cur;
+    unsigned turns = __ballot_sync(0xffffffffu, lane < m && mk != before);
 #pragma unroll 1
     for (int j0 = 0; j0 < m; j0 += R::ROWS) {
       R v[R::ROWS];
 #pragma unroll
       for (int j = 0; j < R::ROWS; ++j) {
-        const uint32_t kj = __shfl_sync(0xffffffffu, mk, j0 + j);
         const int64_t t = __shfl_sync(0xffffffffu, mp, j0 + j);
-        v[j].load(g + t * a.gs, kj != none ? left : 0);
+        v[j].load(static_cast<const TG*>(a.g) + t * a.gs + c0, (live >> (j0 + j)) & 1 ? left : 0);
       }
 #pragma unroll
       for (int j = 0; j < R::ROWS; ++j) {
-        const uint32_t kj = __shfl_sync(0xffffffffu, mk, j0 + j);
-        if (j0 + j < m && kj != cur && cur != none) {
+        if ((turns >> (j0 + j)) & 1) {
           close();
-          open = skip = false;
-          cur = kj;
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+          cur = __shfl_sync(0xffffffffu, mk, j0 + j);
         }
         v[j].add(acc);   // zeros past the end
       }
     }
   }
-  if (cur == none) return;
   if (open || !goes_on) {
     close();
   } else {
-    store_cols<float, M>(a.part + (p * 2 + 1) * a.dim + c0, left, acc);
-    if (c0 == 0 && lane == 0) a.heavy[1 + atomicAdd(a.heavy, 1)] = (int)p;
+    store_cols<float, M>(a.part + (int64_t)(p * 2 + 1) * a.dim + c0, left, acc);
+    if (c0 == 0 && lane == 0) a.heavy[1 + atomicAdd(a.heavy, 1)] = p;
   }
 }
 
@@ -601,6 +601,7 @@ size_t embedding_grad_workspace(int64_t n, int64_t dim) {
   return 4 * up256((size_t)n * 4) + up256((size_t)(pieces + 1) * 4) + (size_t)pieces * 2 * dim * 4;
 }
 
+// (positions, pieces and columns are ints in the kernels: checked by the caller)
 cudaError_t launch_embedding_grad(const ssd_embedding_grad_params_t* p, void* workspace, cudaStream_t stream) {
   GradArgs a;
   a.n = p->num_tokens; a.vocab = p->vocab; a.dim = p->dim;

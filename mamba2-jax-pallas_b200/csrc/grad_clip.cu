@@ -137,6 +137,32 @@ __device__ __forceinline__ double squares(const float (&v)[V]) {
   return s;
 }
 
+// A whole chunk of an aligned tensor: U accesses per thread with no condition between them, so
+// that all of them are in flight.  (A load under a condition is merged with its other value at
+// once, and waits there.)
+template <int V, int U, typename T>
+__device__ __forceinline__ void load_chunk(const T* p, float (&v)[U][V]) {
+  constexpr int W = V * sizeof(T) / 4;
+  uint32_t u[U][W];
+#pragma unroll
+  for (int j = 0; j < U; ++j) {
+    const T* q = p + (j * GC_THREADS + threadIdx.x) * V;
+    if constexpr (W == 4) *reinterpret_cast<uint4*>(u[j]) = *reinterpret_cast<const uint4*>(q);
+    else *reinterpret_cast<uint2*>(u[j]) = *reinterpret_cast<const uint2*>(q);
+  }
+#pragma unroll
+  for (int j = 0; j < U; ++j)
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      if constexpr (sizeof(T) == 4) {
+        v[j][k] = __uint_as_float(u[j][k]);
+      } else {
+        v[j][2 * k] = __uint_as_float(u[j][k] << 16);
+        v[j][2 * k + 1] = __uint_as_float(u[j][k] & 0xffff0000u);
+      }
+    }
+}
+
 template <typename T, int N>
 __global__ void __launch_bounds__(GC_THREADS, CTAS_PER_SM) norm_kernel(const __grid_constant__ Table<N> t, double* partial) {
   constexpr int V = 16 / sizeof(T), U = CHUNK / GC_THREADS / V;
@@ -149,11 +175,19 @@ __global__ void __launch_bounds__(GC_THREADS, CTAS_PER_SM) norm_kernel(const __g
     const T* g = static_cast<const T*>(t.g[i]);
     const int64_t n = t.numel[i], base = (int64_t)(c - t.first[i]) * CHUNK;
     const bool al = reinterpret_cast<uintptr_t>(g) % 16 == 0;
-    float v[U][V];
+    if (al && base + CHUNK <= n) {
+      float v[U][V];
+      load_chunk<V, U>(g + base, v);
 #pragma unroll
-    for (int j = 0; j < U; ++j) load_vec<V>(g, base + (int64_t)(j * GC_THREADS + threadIdx.x) * V, n, al, v[j]);
-#pragma unroll
-    for (int j = 0; j < U; ++j) sum += squares<V>(v[j]);
+      for (int j = 0; j < U; ++j) sum += squares<V>(v[j]);
+    } else {
+      for (int64_t e = base + threadIdx.x * V; e < n; e += GC_THREADS * V) {
+        if (e >= base + CHUNK) break;
+        float v[V];
+        load_vec<V>(g, e, n, al, v);
+        sum += squares<V>(v);
+      }
+    }
   }
   sum = block_sum(sum, sh);
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;
@@ -188,15 +222,24 @@ __global__ void __launch_bounds__(GC_THREADS, CTAS_PER_SM) scale_kernel(const __
     const int64_t n = t.numel[i], base = (int64_t)(c - t.first[i]) * CHUNK;
     const bool al = reinterpret_cast<uintptr_t>(g) % 16 == 0;
     const int oal = align_of(o);
-    float v[U][V];
+    if (al && oal == 16 && base + CHUNK <= n) {
+      float v[U][V];
+      load_chunk<V, U>(g + base, v);
 #pragma unroll
-    for (int j = 0; j < U; ++j) load_vec<V>(g, base + (int64_t)(j * GC_THREADS + threadIdx.x) * V, n, al, v[j]);
+      for (int j = 0; j < U; ++j) {
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int64_t e = base + (int64_t)(j * GC_THREADS + threadIdx.x) * V;
+        for (int k = 0; k < V; ++k) v[j][k] *= f;
+        store_vec<V>(o, base + (j * GC_THREADS + threadIdx.x) * V, n, 16, v[j]);
+      }
+    } else {
+      for (int64_t e = base + threadIdx.x * V; e < n; e += GC_THREADS * V) {
+        if (e >= base + CHUNK) break;
+        float v[V];
+        load_vec<V>(g, e, n, al, v);
 #pragma unroll
-      for (int k = 0; k < V; ++k) v[j][k] *= f;
-      if (e < n) store_vec<V>(o, e, n, oal, v[j]);
+        for (int k = 0; k < V; ++k) v[k] *= f;
+        store_vec<V>(o, e, n, oal, v);
+      }
     }
   }
 }
