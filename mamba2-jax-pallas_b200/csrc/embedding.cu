@@ -18,7 +18,7 @@
 //      its own rows in a shared bitmap;
 //   3. the sorted order is cut into pieces of equal length, whatever the ids, so that one
 //      frequent id cannot hold up a CTA.  A warp sums a piece's rows over 256 columns in f32 and
-//      writes each id's row.  An id that goes on for at most EXTEND rows into the next piece is
+//      writes each id's row.  An id that goes on for at most `extend` rows into the next piece is
 //      finished by the piece it began in; a longer one leaves its parts in the workspace;
 //   4. the parts of such ids are added up, again in order.
 #include <algorithm>
@@ -185,6 +185,7 @@ constexpr int ZERO_ROWS = 8192;   // rows whose bits the bitmap holds at a time
 struct GradArgs {
   int64_t n, vocab, dim, gs, os, pad, piece, npieces;
   int is64, passes, accumulate;
+  int extend;                     // rows that a piece may take from the next one, at most a piece and 32
   float scale;
   const void* ids;
   const void* g;
@@ -340,7 +341,6 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) zero_rows_kernel(const GradAr
 // ---------------------------------------------------------------------------
 constexpr int SUM_THREADS = 256;
 constexpr int SUM_COLS = 32 * VEC;   // columns of a warp
-constexpr int EXTEND = 32;           // rows that a piece may take from the next one
 
 // A row's columns as they were loaded, unpacked when they are added: bf16 in flight takes half
 // the registers of f32, so twice the rows fit.
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(SUM_THREADS, 4) grad_sum_kernel(const __grid_c
   const int unit = blockIdx.x * (SUM_THREADS / 32) + threadIdx.x / 32;
   const int p = unit / col_warps;
   if (p >= (int)a.npieces) return;
-  const int lane = threadIdx.x & 31, n = (int)a.n, top = n - 1, piece = (int)a.piece;
+  const int lane = threadIdx.x & 31, n = (int)a.n, top = n - 1, piece = (int)a.piece, extend = a.extend;
   const int c0 = (unit - p * col_warps) * SUM_COLS, left = (int)a.dim - c0;
   const int lo = p * piece, hi = min(lo + piece, n);
   const uint32_t none = (uint32_t)a.vocab;
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(SUM_THREADS, 4) grad_sum_kernel(const __grid_c
   // every key that decides about the piece's ends, in one round trip
   const uint32_t first = key[lo], last = key[hi - 1];
   const uint32_t k_prev = key[max(lo - 1, 0)], k_before = key[max(lo - piece - 1, 0)];
-  const uint32_t k_far = key[min(lo + EXTEND, top)], k_next = key[min(hi, top)], k_next_far = key[min(hi + EXTEND, top)];
+  const uint32_t k_far = key[min(lo + extend, top)], k_next = key[min(hi, top)], k_next_far = key[min(hi + extend, top)];
   const uint32_t k_ext = key[min(hi + lane, top)];
   uint32_t mk = key[min(lo + lane, top)];
   int mp = (int)pos[min(lo + lane, top)];
@@ -427,13 +427,13 @@ __global__ void __launch_bounds__(SUM_THREADS, 4) grad_sum_kernel(const __grid_c
   // the first id: it may have begun in an earlier piece, and then either the piece before
   // finishes it (skip) or this piece's share of it is a part (open)
   bool open = lo > 0 && k_prev == first;
-  const bool skip = open && (lo == piece || k_before != first) && (lo + EXTEND >= n || k_far != first);
+  const bool skip = open && (lo == piece || k_before != first) && (lo + extend >= n || k_far != first);
   // the last id: rows of the next piece that this one takes, or the id goes on too long
   int end = hi;
   bool goes_on = false;
   if (hi < n && last != none && k_next == last) {
-    if ((lo == 0 || k_prev != last) && (hi + EXTEND >= n || k_next_far != last))
-      end += __popc(__ballot_sync(0xffffffffu, hi + lane < n && k_ext == last));
+    if ((lo == 0 || k_prev != last) && (hi + extend >= n || k_next_far != last))
+      end += __popc(__ballot_sync(0xffffffffu, lane < extend && hi + lane < n && k_ext == last));
     else
       goes_on = true;
   }
@@ -560,7 +560,7 @@ cudaError_t grad_sums(const GradArgs& a, cudaStream_t stream) {
   constexpr int W = SUM_THREADS / 32;
   cudaError_t e = launch_dependent(grad_sum_kernel<TG, TO, M>, dim3((unsigned)((a.npieces * col_warps + W - 1) / W)),
                                    SUM_THREADS, stream, a, (int)col_warps);
-  if (e == cudaSuccess && a.n > a.piece + EXTEND)   // shorter lists have no id with parts
+  if (e == cudaSuccess && a.n > a.piece + a.extend)   // shorter lists have no id with parts
     e = launch_dependent(grad_join_kernel<TO, M>, dim3((unsigned)col_warps, (unsigned)std::min<int64_t>(a.npieces, 32)),
                          SUM_THREADS, stream, a);
   return e;
@@ -572,11 +572,14 @@ cudaError_t grad_sums(const GradArgs& a, bool vec, cudaStream_t stream) {
   return vec ? grad_sums<TG, TO, M>(a, stream) : grad_sums<TG, TO, ONES>(a, stream);
 }
 
-int64_t piece_len(int64_t n) {
-  // at least 32 rows, so that a warp's loads are worth its start, and at most 2048 pieces,
-  // which bounds the parts' workspace and the join's grid
+int64_t piece_len(int64_t n, int64_t dim) {
+  // at most 2048 pieces, which bounds the parts' workspace; 32 rows, which a warp reads in a few
+  // microseconds, unless that leaves most of the GPU without a warp: 777 x 768 f32 takes 20 us in
+  // pieces of 32 and 5 us in pieces of 4
+  const int64_t col_warps = (dim + SUM_COLS - 1) / SUM_COLS;
   int64_t len = 32;
   while ((n + len - 1) / len > 2048) len *= 2;
+  while (len > 4 && len <= 32 && n / len * col_warps < 148 * 16 && (2 * n + len - 1) / len <= 2048) len /= 2;
   return len;
 }
 
@@ -597,7 +600,7 @@ cudaError_t launch_embedding(const ssd_embedding_params_t* p, cudaStream_t strea
 }
 
 size_t embedding_grad_workspace(int64_t n, int64_t dim) {
-  const int64_t pieces = (n + piece_len(n) - 1) / piece_len(n);
+  const int64_t len = piece_len(n, dim), pieces = (n + len - 1) / len;
   return 4 * up256((size_t)n * 4) + up256((size_t)(pieces + 1) * 4) + (size_t)pieces * 2 * dim * 4;
 }
 
@@ -608,7 +611,8 @@ cudaError_t launch_embedding_grad(const ssd_embedding_grad_params_t* p, void* wo
   a.gs = p->grad_stride_row; a.os = p->out_stride_row; a.pad = p->padding_idx;
   a.is64 = p->tokens_int64; a.accumulate = p->accumulate; a.scale = p->scale;
   a.ids = p->tokens; a.g = p->grad; a.out = p->out;
-  a.piece = piece_len(a.n);
+  a.piece = piece_len(a.n, a.dim);
+  a.extend = (int)std::min<int64_t>(a.piece, 32);
   a.npieces = (a.n + a.piece - 1) / a.piece;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const size_t list = up256((size_t)a.n * 4);

@@ -21,6 +21,7 @@
 #include <cuda_fp16.h>
 
 #include "common.cuh"
+#include "linear_ce.cuh"
 #include "ssd_kernels.h"
 #include "ssd_tc.h"
 #include "tc_gemm.cuh"
@@ -28,12 +29,11 @@
 namespace ssd {
 namespace {
 
+using namespace ce;
 using gemm::BM;
 using gemm::BN;
 constexpr int EC = gemm::EPI_COLS;
 
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr double LN2 = 0.6931471805599453;
 // K blocks summed in TMEM before the sum goes to registers (tc_gemm.cuh), measured over K = 4096:
 // one segment 3.3e-6 off in the loss, 16 blocks 7.7e-7 (2 % slower), 8 blocks 3.6e-7 (4 % slower).
 // bf16 logits take 16; f32 products 8, which leaves 9e-7 in the gradients (16: 1.2e-6).
@@ -46,10 +46,6 @@ size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 // ---------------------------------------------------------------------------
 // the tokens that count
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ int64_t target_at(const void* y, int is64, int64_t t) {
-  return is64 ? __ldg(static_cast<const long long*>(y) + t) : (int64_t)__ldg(static_cast<const int*>(y) + t);
-}
-
 // f32 inputs: the largest finite magnitudes (as the bits of a float, which order like it), and
 // from them the powers of two that bring the planes' largest value to [2^14, 2^15): f16 ends at
 // 65504 below, and two planes keep 22 bits down to 2^-1.
@@ -321,53 +317,6 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) logits_kernel(const __grid_c
     if (row < live) a.stats[(int64_t)row * a.ns + n0 / (EC)] = make_float2(top, (e[0] + e[1]) + (e[2] + e[3]));
   });
 }
-
-// A row's results from its statistics, by one warp; the few values behind the sum in f64.
-struct RowResult {
-  float loss, lse;
-  float pm1;               // p - 1 of the target
-  float top, inv;          // p of another column: inv * 2^(s log2(e) - top)
-};
-
-__device__ __forceinline__ RowResult warp_row(const float2* stats, int ns, const float* picked, int target) {
-  const int lane = threadIdx.x & 31;
-  float top = -INFINITY;
-  for (int i = lane; i < ns; i += 32) top = fmaxf(top, stats[i].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (top == -INFINITY) top = 0.f;
-  double others = 0;
-  for (int i = lane; i < ns; i += 32) {
-    const float2 s = stats[i];
-    others += (double)(s.y * exp2f(s.x - top));
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) others += __shfl_xor_sync(0xffffffffu, others, o);
-  const double anchor = LN2 * (double)top;
-  RowResult r;
-  r.top = top;
-  if (target < 0) {        // an invalid target: its loss is NaN, and so is its gradient
-    r.loss = r.pm1 = r.inv = NAN;
-    r.lse = (float)(anchor + log(others));
-    return r;
-  }
-  const double s = (double)*picked, d = anchor - s;
-  // others / e^s: the odds against the target
-  const double odds = others == 0.0 ? 0.0 : others * exp(d);
-  const bool far = d > 600.0;
-  double loss = far ? log(others) + d : log1p(odds);
-  if (!(s < INFINITY)) loss = NAN;   // an infinite or NaN logit, as the formula has it
-  r.loss = (float)loss;
-  r.lse = (float)(loss + s);
-  r.pm1 = (float)(!(s < INFINITY) ? NAN : far ? -1.0 : -odds / (1.0 + odds));
-  r.inv = (float)(1.0 / (others + exp(-d)));
-  return r;
-}
-
-// What the row pass needs of a row: p of a column other than the target's is f 2^(s log2(e) - top).
-struct RowFactors {
-  float top, f, at_y;
-};
 
 // A warp per row that counts: its loss, and with `factors` what the gradients need.
 __global__ void __launch_bounds__(256) loss_kernel(const float2* stats, int ns, const float* picked, Selected s, int from,
@@ -760,9 +709,12 @@ cudaError_t grad_gemm(const Operand& a, const Operand& b, int64_t k, int planes,
 
 }  // namespace
 
-size_t linear_ce_workspace(const ssd_linear_ce_params_t* p) { return plan_of(p).total; }
+size_t linear_ce_workspace(const ssd_linear_ce_params_t* p) {
+  return linear_ce_is_small(p) ? linear_ce_small_workspace(p) : plan_of(p).total;
+}
 
 cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, cudaStream_t st, const char** at) {
+  if (linear_ce_is_small(p)) return launch_linear_ce_small(p, workspace, st, at);
   const Plan q = plan_of(p);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   unsigned* status = reinterpret_cast<unsigned*>(ws);

@@ -1,0 +1,456 @@
+// Linear cross entropy of a few tokens (scoring a drafted continuation, a small fine-tuning
+// step): the same operator as linear_ce.cu where the weight is read for so few rows that
+// nothing but its bytes counts.
+//
+// The products run in f32 on the CUDA cores, straight from the weight as it lies in memory: a
+// tensor-core tile would be mostly padding, and f32 weights would first have to be split into
+// planes (three times their bytes).  Bound by HBM: the loss reads the weight once, the gradients
+// read it once more and write as much.
+//   1. a warp takes four words at a time, all rows of hidden in shared memory: logits, and per row
+//      the running maximum and sum over the words that the warp saw;
+//   2. one CTA: losses, their sum or mean, the factors of the gradients;
+//   3. gradients: a CTA takes a range of words and 1024 columns; every value of the weight that it
+//      loads goes into grad_hidden's sums in registers, and the same dl times hidden is
+//      grad_weight's row;
+//   4. the ranges' sums of grad_hidden are added, in order.
+#include <algorithm>
+
+#include "common.cuh"
+#include "linear_ce.cuh"
+#include "ptx_sm100.cuh"
+#include "ssd_kernels.h"
+
+namespace ssd {
+namespace {
+using namespace ce;
+
+constexpr int SM_THREADS = 512, SM_WARPS = SM_THREADS / 32, SM_CTAS = 148;
+constexpr int WORDS = 4;                     // words of a warp at a time
+constexpr int MAX_ROWS = 8;                  // rows of one pass over the weight
+constexpr size_t MAX_SMEM = 200 * 1024;
+constexpr int G_THREADS = 256, G_COLS = 4 * G_THREADS, G_TILE = 64;
+
+size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
+int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+struct SmallArgs {
+  int tokens, vocab, dim, is64, ns;
+  int64_t xs, ws, ignore, ld;
+  const void* x;
+  const void* w;
+  const void* targets;
+  float2* stats;            // (tokens, ns)
+  float* picked;            // (tokens)
+  float* logits;            // (tokens, ld) or NULL
+  // finish
+  int reduction;
+  const float* grad_loss;
+  float* loss;
+  float* lse;
+  RowFactors* factors;      // (tokens) or NULL
+  // gradients
+  float* part;              // (ranges, rows, dim): grad_hidden's sums
+  int ranges;
+  void* gx;
+  void* gw;
+  int gw_bf16;
+};
+
+template <typename T>
+__device__ __forceinline__ float value(const T* p, int64_t i) { return ld(p + i); }
+
+// K consecutive values: 16 bytes of T.
+template <typename T>
+struct Vec {
+  static constexpr int K = 16 / sizeof(T);
+  uint4 q;
+  __device__ __forceinline__ float at(int k) const {
+    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+    if constexpr (sizeof(T) == 4) return __uint_as_float(u[k]);
+    return __uint_as_float(k & 1 ? u[k / 2] & 0xffff0000u : u[k / 2] << 16);
+  }
+};
+
+// Values v[0..N) summed over the warp; lane l ends with the sum of value l % N.
+template <int N>
+__device__ __forceinline__ float warp_sums(float (&v)[N]) {
+  const int lane = threadIdx.x & 31;
+  int bit = 1;
+#pragma unroll
+  for (int n = N / 2; n >= 1; n /= 2, bit *= 2) {
+    // lanes that differ in `bit` keep the values with that bit of the index clear and set
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float keep = lane & bit ? v[2 * i + 1] : v[2 * i], give = lane & bit ? v[2 * i] : v[2 * i + 1];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, bit);
+    }
+  }
+  float s = v[0];
+#pragma unroll
+  for (int o = N; o < 32; o *= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
+// blockIdx.y: rows 8 y ..; R of them are computed (those past the last token on zeros).
+template <typename T, int R, bool VECTOR>
+__global__ void __launch_bounds__(SM_THREADS, 1) small_logits_kernel(const __grid_constant__ SmallArgs a) {
+  extern __shared__ float xs[];   // (R, dim rounded up to 8)
+  __shared__ float2 red[SM_WARPS][R * WORDS];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int row0 = blockIdx.y * MAX_ROWS, rows = min(R, a.tokens - row0), pitch = (a.dim + 7) / 8 * 8;
+  const T* x = static_cast<const T*>(a.x) + row0 * a.xs;
+  for (int i = tid; i < R * pitch; i += SM_THREADS) {
+    const int r = i / pitch, c = i - r * pitch;
+    xs[i] = r < rows && c < a.dim ? value(x + r * a.xs, c) : 0.f;
+  }
+  // lane l: row l / WORDS (if below R), word l % WORDS of the warp's four
+  const int my_row = (lane / WORDS) % R, my_word = lane % WORDS;
+  const int64_t y = my_row < rows ? target_at(a.targets, a.is64, row0 + my_row) : -1;
+  __syncthreads();
+  float top = -INFINITY, sum = 0.f;
+  const int step = SM_CTAS * SM_WARPS * WORDS;
+  for (int v0 = (blockIdx.x * SM_WARPS + warp) * WORDS; v0 < a.vocab; v0 += step) {
+    const T* w[WORDS];
+#pragma unroll
+    for (int j = 0; j < WORDS; ++j) w[j] = static_cast<const T*>(a.w) + (int64_t)min(v0 + j, a.vocab - 1) * a.ws;
+    float acc[WORDS * R];
+#pragma unroll
+    for (int i = 0; i < WORDS * R; ++i) acc[i] = 0.f;
+    if constexpr (VECTOR) {
+      constexpr int K = Vec<T>::K;
+#pragma unroll 2
+      for (int c = lane * K; c < a.dim; c += 32 * K) {
+        Vec<T> q[WORDS];
+#pragma unroll
+        for (int j = 0; j < WORDS; ++j) q[j].q = *reinterpret_cast<const uint4*>(w[j] + c);
+#pragma unroll
+        for (int k0 = 0; k0 < K; k0 += 4) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const float4 xv = *reinterpret_cast<const float4*>(xs + r * pitch + c + k0);
+#pragma unroll
+            for (int j = 0; j < WORDS; ++j) {
+              float& s = acc[r * WORDS + j];
+              s = fmaf(q[j].at(k0), xv.x, s);
+              s = fmaf(q[j].at(k0 + 1), xv.y, s);
+              s = fmaf(q[j].at(k0 + 2), xv.z, s);
+              s = fmaf(q[j].at(k0 + 3), xv.w, s);
+            }
+          }
+        }
+      }
+    } else {
+#pragma unroll 4
+      for (int c = lane; c < a.dim; c += 32) {
+        float q[WORDS];
+#pragma unroll
+        for (int j = 0; j < WORDS; ++j) q[j] = value(w[j], c);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float xv = xs[r * pitch + c];
+#pragma unroll
+          for (int j = 0; j < WORDS; ++j) acc[r * WORDS + j] = fmaf(q[j], xv, acc[r * WORDS + j]);
+        }
+      }
+    }
+    const float s = warp_sums(acc);
+    const int v = v0 + my_word;
+    if (v < a.vocab && lane < WORDS * R && my_row < rows) {
+      if (a.logits) a.logits[(row0 + my_row) * a.ld + v] = s;
+      if (v == y) {
+        a.picked[row0 + my_row] = s;     // kept out of the sum
+      } else {
+        const float n = fmaxf(top, s * LOG2E), at = n == -INFINITY ? 0.f : n;
+        sum = sum * exp2f(top - at) + exp2f(fmaf(s, LOG2E, -at));
+        top = n;
+      }
+    }
+  }
+  if (lane < WORDS * R) red[warp][lane] = make_float2(top, sum);
+  __syncthreads();
+  if (tid < rows) {
+    float t = -INFINITY;
+    for (int i = 0; i < SM_WARPS * WORDS; ++i) t = fmaxf(t, red[i / WORDS][tid * WORDS + i % WORDS].x);
+    const float at = t == -INFINITY ? 0.f : t;
+    float l = 0.f;
+    for (int i = 0; i < SM_WARPS * WORDS; ++i) {
+      const float2 e = red[i / WORDS][tid * WORDS + i % WORDS];
+      l += e.y * exp2f(e.x - at);
+    }
+    a.stats[(row0 + tid) * a.ns + blockIdx.x] = make_float2(t, l);
+  }
+}
+
+// One CTA, a warp per token (in turns).
+__global__ void __launch_bounds__(256) small_finish_kernel(const __grid_constant__ SmallArgs a) {
+  __shared__ float losses[32];
+  ptx::griddep_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int count = 0;
+  for (int t = 0; t < a.tokens; ++t) count += target_at(a.targets, a.is64, t) != a.ignore;
+  const bool none = a.reduction == SSD_REDUCE_NONE, mean = a.reduction == SSD_REDUCE_MEAN;
+  const float scale = mean ? (float)(1.0 / (double)max(count, 1)) : 1.f;
+  for (int t = warp; t < a.tokens; t += 8) {
+    const int64_t y64 = target_at(a.targets, a.is64, t);
+    const bool counts = y64 != a.ignore;
+    const RowResult r = warp_row(a.stats + t * a.ns, a.ns, a.picked + t, y64 >= 0 && y64 < a.vocab ? (int)y64 : -1);
+    if (lane) continue;
+    const float loss = counts ? r.loss : 0.f;
+    losses[t] = loss;
+    if (none) a.loss[t] = loss;
+    if (a.lse) a.lse[t] = counts ? r.lse : 0.f;
+    if (a.factors) {
+      const float w = scale * (a.grad_loss ? a.grad_loss[none ? t : 0] : 1.f);
+      RowFactors f = {0.f, 0.f, 0.f};
+      if (counts) f = {r.top, w * r.inv, w * r.pm1};
+      a.factors[t] = f;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && !none) {
+    double s = 0;
+    for (int t = 0; t < a.tokens; ++t) s += (double)losses[t];
+    *a.loss = (float)(mean ? s / (double)max(count, 1) : s);
+  }
+}
+
+template <typename T, bool VECTOR>
+__device__ __forceinline__ void load4(const T* row, int c, int dim, float (&v)[4]) {
+  if constexpr (VECTOR) {
+    // 4 columns side by side
+    if constexpr (sizeof(T) == 4) {
+      float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c < dim) q = *reinterpret_cast<const float4*>(row + c);
+      v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+    } else {
+      uint2 q = make_uint2(0, 0);
+      if (c < dim) q = *reinterpret_cast<const uint2*>(row + c);
+      v[0] = __uint_as_float(q.x << 16); v[1] = __uint_as_float(q.x & 0xffff0000u);
+      v[2] = __uint_as_float(q.y << 16); v[3] = __uint_as_float(q.y & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = c + k * G_THREADS < dim ? value(row, c + k * G_THREADS) : 0.f;
+  }
+}
+template <typename T, bool VECTOR>
+__device__ __forceinline__ void store4(T* row, int c, int dim, const float (&v)[4]) {
+  if constexpr (VECTOR) {
+    if (c >= dim) return;
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(row + c) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      const __nv_bfloat162 h[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
+      *reinterpret_cast<uint2*>(row + c) = *reinterpret_cast<const uint2*>(h);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (c + k * G_THREADS < dim) st(row + c + k * G_THREADS, v[k]);
+  }
+}
+
+// CTA (range of words, 1024 columns); a thread holds 4 columns of every row of hidden and of
+// grad_hidden's sums.
+template <typename T, typename TW, int R, bool VECTOR>
+__global__ void __launch_bounds__(G_THREADS) small_grad_kernel(const __grid_constant__ SmallArgs a) {
+  __shared__ float dl[G_TILE][R];
+  ptx::griddep_wait();
+  const int tid = threadIdx.x;
+  const int c0 = blockIdx.y * G_COLS, c = c0 + (VECTOR ? 4 * tid : tid);
+  const int per = (a.vocab + a.ranges - 1) / a.ranges, lo = blockIdx.x * per, hi = min(lo + per, a.vocab);
+  float x[R][4], acc[R][4];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[r][k] = acc[r][k] = 0.f;
+    // an ignored row may hold anything
+    if (r < a.tokens && target_at(a.targets, a.is64, r) != a.ignore)
+      load4<T, VECTOR>(static_cast<const T*>(a.x) + r * a.xs, c, a.dim, x[r]);
+  }
+  for (int v0 = lo; v0 < hi; v0 += G_TILE) {
+    const int n = min(G_TILE, hi - v0);
+    __syncthreads();
+    for (int i = tid; i < G_TILE * R; i += G_THREADS) {
+      const int r = i / G_TILE, j = i - r * G_TILE, v = v0 + j;
+      float d = 0.f;
+      if (r < a.tokens && j < n) {
+        const RowFactors f = a.factors[r];
+        d = target_at(a.targets, a.is64, r) == v ? f.at_y : f.f * exp2f(fmaf(a.logits[r * a.ld + v], LOG2E, -f.top));
+        if (f.f == 0.f && f.at_y == 0.f) d = 0.f;   // ignored: its logits may be NaN
+      }
+      dl[j][r] = d;
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      float w[4] = {0.f, 0.f, 0.f, 0.f}, g[4] = {0.f, 0.f, 0.f, 0.f};
+      if (a.gx) load4<T, VECTOR>(static_cast<const T*>(a.w) + (int64_t)(v0 + j) * a.ws, c, a.dim, w);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float d = dl[j][r];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          acc[r][k] = fmaf(d, w[k], acc[r][k]);
+          g[k] = fmaf(d, x[r][k], g[k]);
+        }
+      }
+      if (a.gw) store4<TW, VECTOR>(static_cast<TW*>(a.gw) + (int64_t)(v0 + j) * a.dim, c, a.dim, g);
+    }
+  }
+  if (a.gx) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (r < a.tokens) store4<float, VECTOR>(a.part + ((int64_t)blockIdx.x * a.tokens + r) * a.dim, c, a.dim, acc[r]);
+  }
+}
+
+// grad_hidden: the ranges' sums, in order; a warp per 32 values, its lanes' loads coalesced.
+template <typename T>
+__global__ void __launch_bounds__(256) small_join_kernel(const __grid_constant__ SmallArgs a) {
+  ptx::griddep_wait();
+  const int64_t n = (int64_t)a.tokens * a.dim, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float s = 0.f;
+#pragma unroll 8
+  for (int j = 0; j < a.ranges; ++j) s += a.part[j * n + i];
+  st(static_cast<T*>(a.gx) + i, s);
+}
+
+template <typename... Params, typename... Args>
+cudaError_t launch(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, bool dependent, cudaStream_t stream,
+                   Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
+int row_width(int64_t tokens) { return tokens == 1 ? 1 : tokens == 2 ? 2 : tokens <= 4 ? 4 : 8; }
+
+size_t logits_smem(const ssd_linear_ce_params_t* p) {
+  return (size_t)row_width(p->tokens) * ((p->dim + 7) / 8 * 8) * 4;
+}
+
+template <typename T, int R>
+cudaError_t run_logits(const SmallArgs& a, bool vec, size_t smem, cudaStream_t st) {
+  auto kernel = vec ? small_logits_kernel<T, R, true> : small_logits_kernel<T, R, false>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  return launch(kernel, dim3(SM_CTAS, (unsigned)cdiv(a.tokens, MAX_ROWS)), SM_THREADS, smem, false, st, a);
+}
+template <typename T>
+cudaError_t run_logits(const SmallArgs& a, bool vec, size_t smem, cudaStream_t st) {
+  switch (row_width(a.tokens)) {
+    case 1: return run_logits<T, 1>(a, vec, smem, st);
+    case 2: return run_logits<T, 2>(a, vec, smem, st);
+    case 4: return run_logits<T, 4>(a, vec, smem, st);
+    default: return run_logits<T, 8>(a, vec, smem, st);
+  }
+}
+
+template <typename T, typename TW, int R>
+cudaError_t run_grad(const SmallArgs& a, bool vec, cudaStream_t st) {
+  return launch(vec ? small_grad_kernel<T, TW, R, true> : small_grad_kernel<T, TW, R, false>,
+                dim3((unsigned)a.ranges, (unsigned)cdiv(a.dim, G_COLS)), G_THREADS, 0, true, st, a);
+}
+template <typename T, typename TW>
+cudaError_t run_grad(const SmallArgs& a, bool vec, cudaStream_t st) {
+  switch (row_width(a.tokens)) {
+    case 1: return run_grad<T, TW, 1>(a, vec, st);
+    case 2: return run_grad<T, TW, 2>(a, vec, st);
+    case 4: return run_grad<T, TW, 4>(a, vec, st);
+    default: return run_grad<T, TW, 8>(a, vec, st);
+  }
+}
+
+bool aligned(const void* p, int64_t stride, int64_t dim, int dtype) {
+  const int64_t es = dtype == SSD_DTYPE_BF16 ? 2 : 4;
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * es % 16 == 0 && dim * es % 16 == 0;
+}
+
+struct SmallPlan {
+  size_t picked, factors, stats, logits, part, total;
+  int ranges;
+  int64_t ld;
+};
+
+SmallPlan plan_of(const ssd_linear_ce_params_t* p) {
+  SmallPlan q{};
+  const bool grad = p->grad_hidden || p->grad_weight;
+  q.ld = (p->vocab + 63) / 64 * 64;
+  // about eight CTAs per SM over the ranges and column blocks
+  q.ranges = (int)std::max<int64_t>(1, std::min<int64_t>(cdiv(SM_CTAS * 8, cdiv(p->dim, G_COLS)), cdiv(p->vocab, 16)));
+  size_t at = 256;   // the status word, as in every workspace
+  auto take = [&](size_t bytes) {
+    const size_t o = at;
+    at += up256(bytes);
+    return o;
+  };
+  q.picked = take((size_t)p->tokens * 4);
+  q.factors = take((size_t)p->tokens * sizeof(RowFactors));
+  q.stats = take((size_t)p->tokens * SM_CTAS * sizeof(float2));
+  q.logits = take(grad ? (size_t)p->tokens * q.ld * 4 : 0);
+  q.part = take(p->grad_hidden ? (size_t)q.ranges * p->tokens * p->dim * 4 : 0);
+  q.total = at;
+  return q;
+}
+
+}  // namespace
+
+bool linear_ce_is_small(const ssd_linear_ce_params_t* p) {
+  const bool grad = p->grad_hidden || p->grad_weight;
+  const int64_t most = grad ? MAX_ROWS : p->dtype == SSD_DTYPE_F32 ? 4 * MAX_ROWS : MAX_ROWS;
+  return p->tokens <= most && logits_smem(p) <= MAX_SMEM && p->vocab < (1 << 30);
+}
+
+size_t linear_ce_small_workspace(const ssd_linear_ce_params_t* p) { return plan_of(p).total; }
+
+#define CE_CHECK(call, where)     \
+  do {                            \
+    const cudaError_t e_ = (call); \
+    if (e_ != cudaSuccess) {      \
+      *at = where;                \
+      return e_;                  \
+    }                             \
+  } while (0)
+
+cudaError_t launch_linear_ce_small(const ssd_linear_ce_params_t* p, void* workspace, cudaStream_t st, const char** at) {
+  const SmallPlan q = plan_of(p);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  CE_CHECK(cudaMemsetAsync(ws, 0, 4, st), "status");
+  const bool bf = p->dtype == SSD_DTYPE_BF16, grad = p->grad_hidden || p->grad_weight;
+  SmallArgs a{};
+  a.tokens = (int)p->tokens; a.vocab = (int)p->vocab; a.dim = (int)p->dim; a.is64 = p->targets_int64; a.ns = SM_CTAS;
+  a.xs = p->hidden_stride_row; a.ws = p->weight_stride_row; a.ignore = p->ignore_index; a.ld = q.ld;
+  a.x = p->hidden; a.w = p->weight; a.targets = p->targets;
+  a.stats = reinterpret_cast<float2*>(ws + q.stats);
+  a.picked = reinterpret_cast<float*>(ws + q.picked);
+  a.logits = grad ? reinterpret_cast<float*>(ws + q.logits) : nullptr;
+  a.reduction = p->reduction; a.grad_loss = p->grad_loss; a.loss = p->loss; a.lse = p->lse;
+  a.factors = grad ? reinterpret_cast<RowFactors*>(ws + q.factors) : nullptr;
+  a.part = reinterpret_cast<float*>(ws + q.part);
+  a.ranges = q.ranges;
+  a.gx = p->grad_hidden; a.gw = p->grad_weight; a.gw_bf16 = p->grad_weight_dtype == SSD_DTYPE_BF16;
+  const bool vec = aligned(p->weight, p->weight_stride_row, p->dim, p->dtype);
+  CE_CHECK(bf ? run_logits<bf16>(a, vec, logits_smem(p), st) : run_logits<float>(a, vec, logits_smem(p), st), "logits");
+  CE_CHECK(launch(small_finish_kernel, dim3(1), 256, 0, true, st, a), "loss");
+  if (!grad) return cudaSuccess;
+  const bool gvec = vec && aligned(p->hidden, p->hidden_stride_row, p->dim, p->dtype) &&
+                    (!p->grad_weight || aligned(p->grad_weight, p->dim, p->dim, p->grad_weight_dtype));
+  if (bf) CE_CHECK((a.gw_bf16 ? run_grad<bf16, bf16>(a, gvec, st) : run_grad<bf16, float>(a, gvec, st)), "gradients");
+  else CE_CHECK((a.gw_bf16 ? run_grad<float, bf16>(a, gvec, st) : run_grad<float, float>(a, gvec, st)), "gradients");
+  if (p->grad_hidden)
+    CE_CHECK(launch(bf ? small_join_kernel<bf16> : small_join_kernel<float>, dim3((unsigned)cdiv(p->tokens * p->dim, 256)), 256, 0,
+                    true, st, a), "grad_hidden");
+  return cudaSuccess;
+}
+
+}  // namespace ssd

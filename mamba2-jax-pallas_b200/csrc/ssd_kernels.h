@@ -44,6 +44,10 @@ cudaError_t launch_embedding_grad(const ssd_embedding_grad_params_t* p, void* wo
 size_t linear_ce_workspace(const ssd_linear_ce_params_t* p);
 // `at` names the step that failed.
 cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, cudaStream_t st, const char** at);
+// The form for a few tokens (linear_ce_small.cu).
+bool linear_ce_is_small(const ssd_linear_ce_params_t* p);
+size_t linear_ce_small_workspace(const ssd_linear_ce_params_t* p);
+cudaError_t launch_linear_ce_small(const ssd_linear_ce_params_t* p, void* workspace, cudaStream_t st, const char** at);
 int64_t grad_clip_partials(const ssd_grad_tensor_t* list, int64_t count);
 cudaError_t launch_grad_clip(const ssd_grad_tensor_t* list, int64_t count, float max_norm, float eps, bool scale,
                              float* norm, void* workspace, cudaStream_t st);

@@ -243,7 +243,10 @@ def grad_bound(r, dim, dtype):
 
 
 SIZES = [(1, 1, 1), (1, 2, 8), (1, 3001, 64), (3, 255, 72), (7, 257, 100), (64, 513, 65), (127, 1000, 40),
-         (128, 256, 64), (129, 2049, 128), (200, 1023, 200), (257, 4096, 264), (300, 131, 1000)]
+         (128, 256, 64), (129, 2049, 128), (200, 1023, 200), (257, 4096, 264), (300, 131, 1000),
+         # the forms for a few tokens: every row width, widths past one column block, past one pass
+         (2, 500, 96), (2, 37, 1025), (4, 777, 260), (4, 9, 2056), (5, 60, 1031), (8, 3000, 72), (8, 300, 33),
+         (9, 400, 128), (20, 300, 64), (32, 700, 48), (33, 700, 48)]
 
 
 @gpu
