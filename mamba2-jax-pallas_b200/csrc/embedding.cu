@@ -26,6 +26,7 @@
 #include <cooperative_groups.h>
 
 #include "common.cuh"
+#include "launch.cuh"
 #include "ptx_sm100.cuh"
 #include "ssd_kernels.h"
 
@@ -539,30 +540,15 @@ __global__ void __launch_bounds__(SUM_THREADS) grad_join_kernel(const GradArgs a
   }
 }
 
-// Launch that may start while the one before it ends (the kernels wait where they must).
-template <typename... Params, typename... Args>
-cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t stream, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
-}
-
 template <typename TG, typename TO, Cols M>
 cudaError_t grad_sums(const GradArgs& a, cudaStream_t stream) {
   const int64_t col_warps = (a.dim + SUM_COLS - 1) / SUM_COLS;
   constexpr int W = SUM_THREADS / 32;
   cudaError_t e = launch_dependent(grad_sum_kernel<TG, TO, M>, dim3((unsigned)((a.npieces * col_warps + W - 1) / W)),
-                                   SUM_THREADS, stream, a, (int)col_warps);
+                                   SUM_THREADS, 0, 1, stream, a, (int)col_warps);
   if (e == cudaSuccess && a.n > a.piece + a.extend)   // shorter lists have no id with parts
     e = launch_dependent(grad_join_kernel<TO, M>, dim3((unsigned)col_warps, (unsigned)std::min<int64_t>(a.npieces, 32)),
-                         SUM_THREADS, stream, a);
+                         SUM_THREADS, 0, 1, stream, a);
   return e;
 }
 
@@ -627,13 +613,15 @@ cudaError_t launch_embedding_grad(const ssd_embedding_grad_params_t* p, void* wo
   a.passes = (bits + SORT_BITS - 1) / SORT_BITS;
   const bool gb = p->grad_dtype == SSD_DTYPE_BF16, ob = p->out_dtype == SSD_DTYPE_BF16;
   const size_t smem = sizeof(SortShared);
-  cudaError_t e = cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = allow_smem((const void*)sort_kernel, smem, &allowed);
   if (e != cudaSuccess) return e;
   sort_kernel<<<SORT_CTAS, SORT_THREADS, smem, stream>>>(a);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   if (!a.accumulate) {   // one CTA per SM that does not sort
-    e = launch_dependent(ob ? zero_rows_kernel<bf16> : zero_rows_kernel<float>, dim3(148 - SORT_CTAS), SORT_THREADS, stream, a);
+    e = launch_dependent(ob ? zero_rows_kernel<bf16> : zero_rows_kernel<float>, dim3(148 - SORT_CTAS), SORT_THREADS,
+                         0, 1, stream, a);
     if (e != cudaSuccess) return e;
   }
   if (a.n == 0) return e;

@@ -343,7 +343,10 @@ cudaError_t launch_grad_clip(const ssd_grad_tensor_t* list, int64_t count, float
   cudaError_t e = for_batches(list, count, false, [&](const Batch& b, const int* index) {
     double* p = partial + npartial;
     npartial += grid_of(b.chunks);
-    return b.count <= 64 ? norm_batch<64>(list, index, b, p, stream) : norm_batch<MAX_TENSORS>(list, index, b, p, stream);
+    // the table is copied at the launch: a short list takes a short one
+    return b.count <= 64    ? norm_batch<64>(list, index, b, p, stream)
+           : b.count <= 256 ? norm_batch<256>(list, index, b, p, stream)
+                            : norm_batch<MAX_TENSORS>(list, index, b, p, stream);
   });
   if (e != cudaSuccess) return e;
   if (!scale || npartial == 0) {
@@ -354,8 +357,9 @@ cudaError_t launch_grad_clip(const ssd_grad_tensor_t* list, int64_t count, float
   return for_batches(list, count, true, [&](const Batch& b, const int* index) {
     float* n = out;
     out = nullptr;
-    return b.count <= 64 ? scale_batch<64>(list, index, b, partial, npartial, max_norm, eps, n, stream)
-                         : scale_batch<MAX_TENSORS>(list, index, b, partial, npartial, max_norm, eps, n, stream);
+    return b.count <= 64    ? scale_batch<64>(list, index, b, partial, npartial, max_norm, eps, n, stream)
+           : b.count <= 256 ? scale_batch<256>(list, index, b, partial, npartial, max_norm, eps, n, stream)
+                            : scale_batch<MAX_TENSORS>(list, index, b, partial, npartial, max_norm, eps, n, stream);
   });
 }
 

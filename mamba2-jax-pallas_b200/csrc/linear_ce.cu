@@ -21,6 +21,7 @@
 #include <cuda_fp16.h>
 
 #include "common.cuh"
+#include "launch.cuh"
 #include "linear_ce.cuh"
 #include "ssd_kernels.h"
 #include "ssd_tc.h"
@@ -70,6 +71,7 @@ struct Selected {
   int* index;              // (tokens): row r is token index[r]
   int* target;             // (tokens): its target, or -1 where that is outside [0, vocab)
   float* alpha;            // the factor common to all rows: 1 or 1 / count, times a scalar grad_loss
+  unsigned* status;        // the workspace's status word
   Scales* scales;
 };
 
@@ -117,6 +119,7 @@ __global__ void __launch_bounds__(1024) select_kernel(const void* targets, int i
     at += __popc(b);
   }
   if (tid == 0) {
+    *s.status = 0;
     *s.count = total;
     s.scales->x = s.scales->w = 0;
     s.scales->dl = sh_largest;
@@ -184,6 +187,7 @@ __device__ __forceinline__ bool vec_rows(const T* p, int64_t stride) {
 // Largest finite magnitude of a matrix's rows (of those whose target counts, where given).
 __global__ void __launch_bounds__(256) largest_kernel(const float* src, int64_t stride, int64_t rows, int64_t dim,
                                                       const void* targets, int is64, int64_t ignore, unsigned* out) {
+  ptx::griddep_wait();
   unsigned m = 0;
   const bool vec = vec_rows(src, stride);
   for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
@@ -205,6 +209,7 @@ __global__ void __launch_bounds__(256) largest_kernel(const float* src, int64_t 
 template <typename T>
 __global__ void __launch_bounds__(256) planes_kernel(const T* src, int64_t stride, int64_t rows, int64_t dim,
                                                      int64_t ld, void* hi, void* lo, const unsigned* largest) {
+  ptx::griddep_wait();
   const float scale = scale_of(*largest);
   const bool vec = vec_rows(src, stride);
   const int64_t runs = (ld + 255) / 256, n = rows * runs;
@@ -221,6 +226,7 @@ template <typename T>
 __global__ void __launch_bounds__(128) gather_kernel(const T* src, int64_t stride, int64_t dim, int64_t ld, Selected s,
                                                      const void* targets, int is64, int64_t ignore, void* hi, void* lo,
                                                      T* grad_hidden) {
+  ptx::griddep_wait();
   const int64_t r = blockIdx.x;
   if (blockIdx.y == 1) {
     if (target_at(targets, is64, r) == ignore)
@@ -277,8 +283,11 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) logits_kernel(const __grid_c
                                                                   const __grid_constant__ LogitArgs a) {
   extern __shared__ uint8_t smem[];
   __shared__ gemm::Ctl ctl;
-  const float unscale = p.passes == 3 ? 1.f / (scale_of(a.scales->x) * scale_of(a.scales->w)) : 1.f;
-  gemm::run<CG, false, false>(p, smem, &ctl, [&](const gemm::Tile& t, float (&v)[EC], int row0, int n0, int live,
+  float unscale = 1.f;
+  auto prep = [&]() {
+    if (p.passes == 3) unscale = 1.f / scale_of(a.scales->x) / scale_of(a.scales->w);
+  };
+  gemm::run<CG, false, false>(p, smem, &ctl, prep, [&](const gemm::Tile& t, float (&v)[EC], int row0, int n0, int live,
                                                  float4* stage) {
     const int row = row0 + (threadIdx.x & 31);
     const int y = row < live ? a.target[row] : -1;
@@ -322,6 +331,7 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) logits_kernel(const __grid_c
 __global__ void __launch_bounds__(256) loss_kernel(const float2* stats, int ns, const float* picked, Selected s, int from,
                                                    int rows, float* loss, float* lse, const float* weight, int split,
                                                    RowFactors* factors) {
+  ptx::griddep_wait();
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row >= rows || from + row >= *s.count) return;
   const RowResult r = warp_row(stats + row * ns, ns, picked + row, s.target[from + row]);
@@ -338,6 +348,7 @@ __global__ void __launch_bounds__(256) loss_kernel(const float2* stats, int ns, 
 
 // One CTA: sum (or mean over the tokens that count) of the tokens' losses, in a fixed order.
 __global__ void __launch_bounds__(1024) reduce_kernel(const float* rows, int64_t n, const int* count, int mean, float* out) {
+  ptx::griddep_wait();
   __shared__ double sh[32];
   double s = 0;
   for (int64_t i = threadIdx.x; i < n; i += 1024) s += (double)rows[i];
@@ -370,6 +381,7 @@ constexpr int ROW_THREADS = 256, ROW_UNROLL = 8, ROW_COLS = ROW_THREADS * 4 * RO
 // Zero rows up to the next 64.  HBM-bound: 6 bytes per logit (f32 inputs: 8).
 template <bool SPLIT>
 __global__ void __launch_bounds__(ROW_THREADS) row_kernel(const RowArgs a) {
+  ptx::griddep_wait();
   const int64_t row = blockIdx.x;
   const int64_t live = (int64_t)*a.sel.count - a.from;
   if (live <= 0 || row >= (live + 63) / 64 * 64) return;
@@ -434,10 +446,13 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) grad_gemm_kernel(const __gri
                                                                      const __grid_constant__ OutArgs a) {
   extern __shared__ uint8_t smem[];
   __shared__ gemm::Ctl ctl;
-  float f = p.passes == 3 ? 1.f / scale_of(*a.largest[0]) / scale_of(*a.largest[1]) : 1.f;
-  const float alpha = *a.alpha;
-  if (MODE != OUT_PART) f *= alpha;
-  gemm::run<CG, A_MN, true>(p, smem, &ctl, [&](const gemm::Tile& t, float (&v)[EC], int row0, int n0, int live,
+  float f = 1.f, alpha = 1.f;
+  auto prep = [&]() {
+    if (p.passes == 3) f = 1.f / scale_of(*a.largest[0]) / scale_of(*a.largest[1]);
+    alpha = *a.alpha;
+    if (MODE != OUT_PART) f *= alpha;
+  };
+  gemm::run<CG, A_MN, true>(p, smem, &ctl, prep, [&](const gemm::Tile& t, float (&v)[EC], int row0, int n0, int live,
                                                float4* stage) {
     const int rows = (int)min((int64_t)32, (p.limit_k ? a.rows : live) - row0);
     const int cols = (int)min((int64_t)EC, a.cols - n0);
@@ -515,6 +530,7 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) grad_gemm_kernel(const __gri
 template <typename TO>
 __global__ void __launch_bounds__(256) join_kernel(const float* part, int splits, int64_t rows, int64_t cols, Selected s,
                                                    int from, TO* out) {
+  ptx::griddep_wait();
   const int64_t row = blockIdx.x;
   if (from + row >= *s.count) return;
   const float f = *s.alpha;
@@ -548,33 +564,15 @@ __global__ void __launch_bounds__(256) join_kernel(const float* part, int splits
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-int sm_count() {
-  int dev = 0, n = 0;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n > 0 ? n : 148;
-}
+constexpr int SMS = 148;   // of a B200
 
 template <int CG, typename Kernel, typename Args>
-cudaError_t launch_gemm(Kernel kernel, const gemm::Problem& p, const Args& a, cudaStream_t st) {
+cudaError_t launch_gemm(Kernel kernel, const gemm::Problem& p, const Args& a, std::atomic<uint64_t>* allowed, cudaStream_t st) {
   constexpr int smem = gemm::Shape<CG>::SMEM;
-  cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const cudaError_t e = allow_smem((const void*)kernel, smem, allowed);
   if (e != cudaSuccess) return e;
   const int64_t units = (int64_t)p.m_tiles * p.n_tiles * p.splits;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3((unsigned)(CG * std::min<int64_t>(units, sm_count() / CG)));
-  cfg.blockDim = dim3(gemm::THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  if (CG > 1) {
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CG;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-  }
-  return cudaLaunchKernelEx(&cfg, kernel, p, a);
+  return launch_dependent(kernel, dim3((unsigned)(CG * std::min<int64_t>(units, SMS / CG))), gemm::THREADS, smem, CG, st, p, a);
 }
 
 // Maps of an operand's planes.  K-major: 64 values of the reduced dimension x `box` rows.
@@ -681,7 +679,8 @@ cudaError_t logits_gemm(const Operand& x, const Operand& w, int planes, const Lo
   g.m_fastest = 1;
   g.segment = planes == 2 ? SEGMENT_F32 : SEGMENT_BF16;
   g.status = status;
-  return launch_gemm<CG>(logits_kernel<CG>, g, a, st);
+  static std::atomic<uint64_t> allowed{0};
+  return launch_gemm<CG>(logits_kernel<CG>, g, a, &allowed, st);
 }
 
 template <int CG, bool A_MN>
@@ -702,9 +701,10 @@ cudaError_t grad_gemm(const Operand& a, const Operand& b, int64_t k, int planes,
   // bf16: the operands' own rounding is a hundred times what the adds lose
   g.segment = planes == 2 ? SEGMENT_F32 : 1 << 20;
   g.status = status;
-  if (o.part) return launch_gemm<CG>(grad_gemm_kernel<CG, A_MN, OUT_PART>, g, o, st);
-  if (o.out_bf16) return launch_gemm<CG>(grad_gemm_kernel<CG, A_MN, OUT_BF16>, g, o, st);
-  return launch_gemm<CG>(grad_gemm_kernel<CG, A_MN, OUT_F32>, g, o, st);
+  static std::atomic<uint64_t> allowed[3] = {};
+  if (o.part) return launch_gemm<CG>(grad_gemm_kernel<CG, A_MN, OUT_PART>, g, o, &allowed[0], st);
+  if (o.out_bf16) return launch_gemm<CG>(grad_gemm_kernel<CG, A_MN, OUT_BF16>, g, o, &allowed[1], st);
+  return launch_gemm<CG>(grad_gemm_kernel<CG, A_MN, OUT_F32>, g, o, &allowed[2], st);
 }
 
 }  // namespace
@@ -718,8 +718,8 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
   const Plan q = plan_of(p);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   unsigned* status = reinterpret_cast<unsigned*>(ws);
-  CE_CHECK(cudaMemsetAsync(status, 0, 4, st), "status");
   Selected sel;
+  sel.status = status;
   sel.count = reinterpret_cast<int*>(ws + q.one);
   sel.alpha = reinterpret_cast<float*>(ws + q.one) + 1;
   sel.scales = reinterpret_cast<Scales*>(ws + q.one + 16);
@@ -730,7 +730,8 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
   const bool per_row = p->reduction == SSD_REDUCE_NONE && p->grad_loss;
   select_kernel<<<1, 1024, 0, st>>>(p->targets, p->targets_int64, p->tokens, p->vocab, p->ignore_index, mean,
                                     per_row ? nullptr : p->grad_loss, per_row ? p->grad_loss : nullptr, sel, rows, p->lse);
-  CE_CHECK(cudaGetLastError(), "select");
+  cudaError_t err = cudaGetLastError();
+  CE_CHECK(err, "select");
   Operand x{}, w{};
   x.rows = p->tokens; x.dim = p->dim;
   place_planes(&x, p->dtype, ws + q.x);
@@ -739,21 +740,22 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
   void* lo = const_cast<void*>(x.plane[1]);
   const unsigned wide = 148 * 8;
   if (!bf) {
-    largest_kernel<<<std::min<unsigned>((unsigned)cdiv(p->tokens, 8), wide), 256, 0, st>>>(static_cast<const float*>(p->hidden), p->hidden_stride_row,
+    err = launch_dependent(largest_kernel, std::min<unsigned>((unsigned)cdiv(p->tokens, 8), wide), 256, 0, 1, st, static_cast<const float*>(p->hidden), p->hidden_stride_row,
         p->tokens, p->dim, p->targets, p->targets_int64, p->ignore_index, &sel.scales->x);
-    largest_kernel<<<std::min<unsigned>((unsigned)cdiv(p->vocab, 8), wide), 256, 0, st>>>(static_cast<const float*>(p->weight),
+    CE_CHECK(err, "largest");
+    err = launch_dependent(largest_kernel, std::min<unsigned>((unsigned)cdiv(p->vocab, 8), wide), 256, 0, 1, st, static_cast<const float*>(p->weight),
         p->weight_stride_row, p->vocab, p->dim, nullptr, 0, 0, &sel.scales->w);
-    CE_CHECK(cudaGetLastError(), "largest");
+    CE_CHECK(err, "largest");
   }
   if (bf)
-    gather_kernel<bf16><<<grid, 128, 0, st>>>(static_cast<const bf16*>(p->hidden), p->hidden_stride_row, p->dim,
+    err = launch_dependent(gather_kernel<bf16>, grid, 128, 0, 1, st, static_cast<const bf16*>(p->hidden), p->hidden_stride_row, p->dim,
                                               x.ld, sel, p->targets, p->targets_int64, p->ignore_index, hi, lo,
                                               static_cast<bf16*>(p->grad_hidden));
   else
-    gather_kernel<float><<<grid, 128, 0, st>>>(static_cast<const float*>(p->hidden), p->hidden_stride_row, p->dim,
+    err = launch_dependent(gather_kernel<float>, grid, 128, 0, 1, st, static_cast<const float*>(p->hidden), p->hidden_stride_row, p->dim,
                                                x.ld, sel, p->targets, p->targets_int64, p->ignore_index, hi, lo,
                                                static_cast<float*>(p->grad_hidden));
-  CE_CHECK(cudaGetLastError(), "gather");
+  CE_CHECK(err, "gather");
   w.rows = p->vocab; w.dim = p->dim; w.ld = p->weight_stride_row; w.plane[0] = p->weight;
   if (q.pack_w) {
     place_planes(&w, p->dtype, ws + q.w);
@@ -761,12 +763,12 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
     void* wlo = const_cast<void*>(w.plane[1]);
     const unsigned g = (unsigned)std::min<int64_t>((w.rows * ((w.ld + 255) / 256) + 7) / 8, wide * 2);
     if (bf)
-      planes_kernel<bf16><<<g, 256, 0, st>>>(static_cast<const bf16*>(p->weight), p->weight_stride_row, p->vocab, p->dim,
+      err = launch_dependent(planes_kernel<bf16>, g, 256, 0, 1, st, static_cast<const bf16*>(p->weight), p->weight_stride_row, p->vocab, p->dim,
                                              w.ld, whi, wlo, &sel.scales->w);
     else
-      planes_kernel<float><<<g, 256, 0, st>>>(static_cast<const float*>(p->weight), p->weight_stride_row, p->vocab, p->dim,
+      err = launch_dependent(planes_kernel<float>, g, 256, 0, 1, st, static_cast<const float*>(p->weight), p->weight_stride_row, p->vocab, p->dim,
                                               w.ld, whi, wlo, &sel.scales->w);
-    CE_CHECK(cudaGetLastError(), "weight planes");
+    CE_CHECK(err, "weight planes");
   }
   for (int64_t c = 0; c < q.nchunks; ++c) {
     const int64_t t0 = c * q.chunk, n = std::min(q.chunk, p->tokens - t0);
@@ -785,17 +787,17 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
     if (n > BM) CE_CHECK(logits_gemm<2>(xc, w, q.planes, a, sel.count, from, status, st), "logits");
     else CE_CHECK(logits_gemm<1>(xc, w, q.planes, a, sel.count, from, status, st), "logits");
     RowFactors* factors = q.grad ? reinterpret_cast<RowFactors*>(ws + q.factors) : nullptr;
-    loss_kernel<<<(unsigned)cdiv(n, 8), 256, 0, st>>>(a.stats, a.ns, a.picked, sel, from, (int)n, rows, p->lse,
+    err = launch_dependent(loss_kernel, (unsigned)cdiv(n, 8), 256, 0, 1, st, a.stats, a.ns, a.picked, sel, from, (int)n, rows, p->lse,
                                                      per_row ? p->grad_loss : nullptr, q.planes == 2, factors);
-    CE_CHECK(cudaGetLastError(), "loss");
+    CE_CHECK(err, "loss");
     if (!q.grad) continue;
     RowArgs r{};
     r.vocab = p->vocab; r.ld = q.ld; r.sel = sel; r.from = from; r.factors = factors; r.logits = a.logits;
     for (int i = 0; i < q.planes; ++i) r.dl[i] = ws + q.dl[i];
     const dim3 row_grid((unsigned)n, (unsigned)cdiv(p->vocab, ROW_COLS));
-    if (q.planes == 2) row_kernel<true><<<row_grid, ROW_THREADS, 0, st>>>(r);
-    else row_kernel<false><<<row_grid, ROW_THREADS, 0, st>>>(r);
-    CE_CHECK(cudaGetLastError(), "rows");
+    if (q.planes == 2) err = launch_dependent(row_kernel<true>, row_grid, ROW_THREADS, 0, 1, st, r);
+    else err = launch_dependent(row_kernel<false>, row_grid, ROW_THREADS, 0, 1, st, r);
+    CE_CHECK(err, "rows");
     Operand dl{};
     dl.rows = n; dl.dim = p->vocab; dl.ld = q.ld;
     for (int i = 0; i < q.planes; ++i) dl.plane[i] = r.dl[i];
@@ -809,10 +811,10 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
       else CE_CHECK((grad_gemm<1, false>(dl, w, p->vocab, q.planes, q.splits, o, sel.count, from, status, st)), "grad_hidden");
       if (q.splits > 1) {
         if (bf)
-          join_kernel<bf16><<<(unsigned)n, 256, 0, st>>>(o.part, q.splits, n, p->dim, sel, from, static_cast<bf16*>(p->grad_hidden));
+          err = launch_dependent(join_kernel<bf16>, (unsigned)n, 256, 0, 1, st, o.part, q.splits, n, p->dim, sel, from, static_cast<bf16*>(p->grad_hidden));
         else
-          join_kernel<float><<<(unsigned)n, 256, 0, st>>>(o.part, q.splits, n, p->dim, sel, from, static_cast<float*>(p->grad_hidden));
-        CE_CHECK(cudaGetLastError(), "grad_hidden join");
+          err = launch_dependent(join_kernel<float>, (unsigned)n, 256, 0, 1, st, o.part, q.splits, n, p->dim, sel, from, static_cast<float*>(p->grad_hidden));
+        CE_CHECK(err, "grad_hidden join");
       }
     }
     if (p->grad_weight) {
@@ -827,8 +829,8 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
     }
   }
   if (p->reduction != SSD_REDUCE_NONE) {
-    reduce_kernel<<<1, 1024, 0, st>>>(rows, p->tokens, sel.count, mean, p->loss);
-    CE_CHECK(cudaGetLastError(), "reduce");
+    err = launch_dependent(reduce_kernel, 1, 1024, 0, 1, st, rows, p->tokens, sel.count, mean, p->loss);
+    CE_CHECK(err, "reduce");
   }
   return cudaSuccess;
 }

@@ -16,6 +16,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "launch.cuh"
 #include "linear_ce.cuh"
 #include "ptx_sm100.cuh"
 #include "ssd_kernels.h"
@@ -39,6 +40,7 @@ struct SmallArgs {
   const void* x;
   const void* w;
   const void* targets;
+  unsigned* status;         // the workspace's status word: cleared (nothing here waits)
   float2* stats;            // (tokens, ns)
   float* picked;            // (tokens)
   float* logits;            // (tokens, ld) or NULL
@@ -99,6 +101,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) small_logits_kernel(const __gri
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int row0 = blockIdx.y * MAX_ROWS, rows = min(R, a.tokens - row0), pitch = (a.dim + 7) / 8 * 8;
   const T* x = static_cast<const T*>(a.x) + row0 * a.xs;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) *a.status = 0;
   for (int i = tid; i < R * pitch; i += SM_THREADS) {
     const int r = i / pitch, c = i - r * pitch;
     xs[i] = r < rows && c < a.dim ? value(x + r * a.xs, c) : 0.f;
@@ -317,22 +320,6 @@ __global__ void __launch_bounds__(256) small_join_kernel(const __grid_constant__
   st(static_cast<T*>(a.gx) + i, s);
 }
 
-template <typename... Params, typename... Args>
-cudaError_t launch(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, bool dependent, cudaStream_t stream,
-                   Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = dependent ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
-}
-
 int row_width(int64_t tokens) { return tokens == 1 ? 1 : tokens == 2 ? 2 : tokens <= 4 ? 4 : 8; }
 
 size_t logits_smem(const ssd_linear_ce_params_t* p) {
@@ -342,9 +329,11 @@ size_t logits_smem(const ssd_linear_ce_params_t* p) {
 template <typename T, int R>
 cudaError_t run_logits(const SmallArgs& a, bool vec, size_t smem, cudaStream_t st) {
   auto kernel = vec ? small_logits_kernel<T, R, true> : small_logits_kernel<T, R, false>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> allowed[2] = {};
+  const cudaError_t e = allow_smem((const void*)kernel, MAX_SMEM, &allowed[vec]);
   if (e != cudaSuccess) return e;
-  return launch(kernel, dim3(SM_CTAS, (unsigned)cdiv(a.tokens, MAX_ROWS)), SM_THREADS, smem, false, st, a);
+  kernel<<<dim3(SM_CTAS, (unsigned)cdiv(a.tokens, MAX_ROWS)), SM_THREADS, smem, st>>>(a);
+  return cudaGetLastError();
 }
 template <typename T>
 cudaError_t run_logits(const SmallArgs& a, bool vec, size_t smem, cudaStream_t st) {
@@ -358,8 +347,8 @@ cudaError_t run_logits(const SmallArgs& a, bool vec, size_t smem, cudaStream_t s
 
 template <typename T, typename TW, int R>
 cudaError_t run_grad(const SmallArgs& a, bool vec, cudaStream_t st) {
-  return launch(vec ? small_grad_kernel<T, TW, R, true> : small_grad_kernel<T, TW, R, false>,
-                dim3((unsigned)a.ranges, (unsigned)cdiv(a.dim, G_COLS)), G_THREADS, 0, true, st, a);
+  return launch_dependent(vec ? small_grad_kernel<T, TW, R, true> : small_grad_kernel<T, TW, R, false>,
+                          dim3((unsigned)a.ranges, (unsigned)cdiv(a.dim, G_COLS)), G_THREADS, 0, 1, st, a);
 }
 template <typename T, typename TW>
 cudaError_t run_grad(const SmallArgs& a, bool vec, cudaStream_t st) {
@@ -425,12 +414,12 @@ size_t linear_ce_small_workspace(const ssd_linear_ce_params_t* p) { return plan_
 cudaError_t launch_linear_ce_small(const ssd_linear_ce_params_t* p, void* workspace, cudaStream_t st, const char** at) {
   const SmallPlan q = plan_of(p);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  CE_CHECK(cudaMemsetAsync(ws, 0, 4, st), "status");
   const bool bf = p->dtype == SSD_DTYPE_BF16, grad = p->grad_hidden || p->grad_weight;
   SmallArgs a{};
   a.tokens = (int)p->tokens; a.vocab = (int)p->vocab; a.dim = (int)p->dim; a.is64 = p->targets_int64; a.ns = SM_CTAS;
   a.xs = p->hidden_stride_row; a.ws = p->weight_stride_row; a.ignore = p->ignore_index; a.ld = q.ld;
   a.x = p->hidden; a.w = p->weight; a.targets = p->targets;
+  a.status = reinterpret_cast<unsigned*>(ws);
   a.stats = reinterpret_cast<float2*>(ws + q.stats);
   a.picked = reinterpret_cast<float*>(ws + q.picked);
   a.logits = grad ? reinterpret_cast<float*>(ws + q.logits) : nullptr;
@@ -441,15 +430,15 @@ cudaError_t launch_linear_ce_small(const ssd_linear_ce_params_t* p, void* worksp
   a.gx = p->grad_hidden; a.gw = p->grad_weight; a.gw_bf16 = p->grad_weight_dtype == SSD_DTYPE_BF16;
   const bool vec = aligned(p->weight, p->weight_stride_row, p->dim, p->dtype);
   CE_CHECK(bf ? run_logits<bf16>(a, vec, logits_smem(p), st) : run_logits<float>(a, vec, logits_smem(p), st), "logits");
-  CE_CHECK(launch(small_finish_kernel, dim3(1), 256, 0, true, st, a), "loss");
+  CE_CHECK(launch_dependent(small_finish_kernel, dim3(1), 256, 0, 1, st, a), "loss");
   if (!grad) return cudaSuccess;
   const bool gvec = vec && aligned(p->hidden, p->hidden_stride_row, p->dim, p->dtype) &&
                     (!p->grad_weight || aligned(p->grad_weight, p->dim, p->dim, p->grad_weight_dtype));
   if (bf) CE_CHECK((a.gw_bf16 ? run_grad<bf16, bf16>(a, gvec, st) : run_grad<bf16, float>(a, gvec, st)), "gradients");
   else CE_CHECK((a.gw_bf16 ? run_grad<float, bf16>(a, gvec, st) : run_grad<float, float>(a, gvec, st)), "gradients");
   if (p->grad_hidden)
-    CE_CHECK(launch(bf ? small_join_kernel<bf16> : small_join_kernel<float>, dim3((unsigned)cdiv(p->tokens * p->dim, 256)), 256, 0,
-                    true, st, a), "grad_hidden");
+    CE_CHECK(launch_dependent(bf ? small_join_kernel<bf16> : small_join_kernel<float>,
+                              dim3((unsigned)cdiv(p->tokens * p->dim, 256)), 256, 0, 1, st, a), "grad_hidden");
   return cudaSuccess;
 }
 

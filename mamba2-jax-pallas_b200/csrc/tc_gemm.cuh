@@ -252,17 +252,13 @@ __device__ __forceinline__ void by_rows8(float4* stage, const float (&v)[EPI_COL
   }
 }
 
-// The kernel's body.  epi(tile, v, row0, first column, rows that count, stage) runs on each
+// The kernel's body.  prep() runs on every thread once the launches before are complete.  epi(tile, v, row0, first column, rows that count, stage) runs on each
 // epilogue thread; v holds 64 values of row row0 + lane.
-template <int CG, bool A_MN, bool B_MN, typename Epi>
-__device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c, Epi&& epi) {
+template <int CG, bool A_MN, bool B_MN, typename Prep, typename Epi>
+__device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c, Prep&& prep, Epi&& epi) {
   using S = Shape<CG>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0;
-  const int live = live_rows(p);
-  const int m_tiles = p.limit_k ? p.m_tiles : (live + BM * CG - 1) / (BM * CG);
-  const int k_blocks = p.limit_k ? (live + BK - 1) / BK : p.k_blocks;
-  const int64_t unit0 = blockIdx.x / CG, units = (int64_t)m_tiles * p.n_tiles * p.splits, step = gridDim.x / CG;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::STAGES; ++i) {
@@ -283,7 +279,12 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
   if constexpr (CG == 2) cluster_sync_all();
   ptx::tc_fence_after();
   const uint32_t tmem = c->tmem;
-
+  ptx::griddep_wait();   // all above needs nothing from the launches before
+  prep();
+  const int live = live_rows(p);
+  const int m_tiles = p.limit_k ? p.m_tiles : (live + BM * CG - 1) / (BM * CG);
+  const int k_blocks = p.limit_k ? (live + BK - 1) / BK : p.k_blocks;
+  const int64_t unit0 = blockIdx.x / CG, units = (int64_t)m_tiles * p.n_tiles * p.splits, step = gridDim.x / CG;
   if (warp == 0) {
     if (lane == 0) {
       for (int i = 0; i < (p.passes == 3 ? 2 : 1); ++i) {

@@ -276,17 +276,22 @@ def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+_INDEX_DTYPES = (torch.int32, torch.int64)
+
+
 def index_list(t, name: str) -> torch.Tensor:
     """Token ids or targets: a contiguous CUDA tensor of int32 or int64."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if t.dtype not in (torch.int32, torch.int64):
+    if t.dtype not in _INDEX_DTYPES:
         raise TypeError(f"{name} must be int32 or int64, not {t.dtype}")
-    return dev(t, name)
+    return t if t.is_cuda and t.is_contiguous() else dev(t, name)
 
 
 def rows2d(t: torch.Tensor, width: int) -> torch.Tensor:
     """(rows, width) view with a contiguous last axis and one row stride, else a copy."""
+    if t.dim() == 2 and t.is_contiguous():
+        return t
     t2 = t.reshape(-1, width)
     if (width > 1 and t2.stride(1) != 1) or (t2.shape[0] > 1 and t2.stride(0) < width):
         t2 = t2.contiguous()
@@ -306,7 +311,14 @@ def on_device(dev: torch.device):
     return _HERE_ALREADY if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
+# the address of the current stream alone; the public call also builds a Stream object, which
+# takes as long as a small kernel's launch
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_of(t: torch.Tensor) -> int:
+    if _raw_stream is not None:
+        return _raw_stream(t.device.index)
     return torch.cuda.current_stream(t.device).cuda_stream
 
 

@@ -29,25 +29,26 @@ def embedding(tokens, weight, scale: float = 1.0, *, padding_idx=None, out_dtype
         raise ValueError("weight must be a (vocab, dim) tensor")
     if not weight.is_cuda:
         raise ValueError("weight must be a CUDA tensor (no CPU path)")
-    if ids.device != weight.device:
+    dev = weight.device
+    if ids.device != dev:
         raise ValueError("tokens and weight must be on one device")
     vocab, dim = weight.shape
     if vocab == 0 or dim == 0:
         raise ValueError("weight must not be empty")
-    _lib.dtype_code(weight)
-    out_dtype = weight.dtype if out_dtype is None else out_dtype
-    if out_dtype not in _DTYPES:
+    w_code = _lib.dtype_code(weight)
+    if out_dtype is None:
+        out_dtype = weight.dtype
+    elif out_dtype not in _DTYPES:
         raise ValueError("out_dtype must be torch.float32 or torch.bfloat16")
     w = _lib.rows2d(weight, dim)
-    p = _lib.EmbeddingParams(num_tokens=ids.numel(), vocab=vocab, dim=dim, weight_stride_row=_lib.row_stride(w),
-                             padding_idx=_pad(padding_idx, vocab), tokens_int64=int(ids.dtype == torch.int64),
-                             weight_dtype=_lib.dtype_code(w), scale=float(scale))
-    out = torch.empty((*tokens.shape, dim), device=w.device, dtype=out_dtype)
-    if ids.numel() == 0:
+    pad = -1 if padding_idx is None else _pad(padding_idx, vocab)
+    out = torch.empty((*ids.shape, dim), device=dev, dtype=out_dtype)
+    n = ids.numel()
+    if n == 0:
         return out
-    p.out_dtype = _lib.dtype_code(out)
-    p.tokens, p.weight, p.out = ids.data_ptr(), w.data_ptr(), out.data_ptr()
-    with _lib.on_device(w.device):
+    p = _lib.EmbeddingParams(n, vocab, dim, _lib.row_stride(w), pad, ids.dtype is torch.int64, w_code,
+                             _lib.dtype_code(out), scale, ids.data_ptr(), w.data_ptr(), out.data_ptr())
+    with _lib.on_device(dev):
         _lib.check(_lib.load().ssd_embedding(p, _lib.stream_of(out)))
     return out
 

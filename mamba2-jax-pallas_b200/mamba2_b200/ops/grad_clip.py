@@ -1,6 +1,7 @@
 """Global gradient norm over many tensors, and clipping by it."""
 from __future__ import annotations
 
+import operator
 from array import array
 
 import torch
@@ -9,12 +10,13 @@ from .. import _lib
 
 _DTYPE = {torch.float32: _lib.SSD_DTYPE_F32, torch.bfloat16: _lib.SSD_DTYPE_BF16}
 _T = torch.Tensor
+_dtype = operator.attrgetter("dtype")
 
 
 # A model has hundreds of tensors, and the kernels take a few microseconds where they are
 # small: what is asked of each tensor goes through map() over the method itself.
 def _checked(ts, name):
-    """(list of tensors, their dtype codes, their device index), or an error."""
+    """(list of tensors, their dtypes, their device index), or an error."""
     ts = list(ts)
     if not ts:
         raise ValueError(f"{name} must not be empty")
@@ -26,17 +28,18 @@ def _checked(ts, name):
         raise ValueError(f"{name} must be CUDA tensors (no CPU path)")
     if len(devices) != 1:
         raise ValueError(f"{name} must be on one device")
-    codes = [_DTYPE.get(t.dtype) for t in ts]
-    if None in codes:
-        raise TypeError(f"unsupported dtype {ts[codes.index(None)].dtype} (float32 or bfloat16)")
-    return ts, codes, devices.pop()
+    dtypes = list(map(_dtype, ts))
+    for d in set(dtypes):
+        if d not in _DTYPE:
+            raise TypeError(f"unsupported dtype {d} (float32 or bfloat16)")
+    return ts, dtypes, devices.pop()
 
 
 def _contiguous(ts):
     return ts if all(map(_T.is_contiguous, ts)) else [t.contiguous() for t in ts]
 
 
-def _run(grads, codes, outs, out_codes, max_norm, eps, scale):
+def _run(grads, dtypes, outs, out_dtypes, max_norm, eps, scale):
     dev = grads[0].device
     norm = torch.empty((), device=dev, dtype=torch.float32)
     # ssd_grad_tensor_t: two addresses, the size, two 32-bit dtypes
@@ -45,7 +48,8 @@ def _run(grads, codes, outs, out_codes, max_norm, eps, scale):
     rec[0::4] = array("q", map(_T.data_ptr, grads))
     rec[1::4] = rec[0::4] if outs is grads else array("q", map(_T.data_ptr, outs))
     rec[2::4] = array("q", map(_T.numel, grads))
-    rec[3::4] = array("q", [g | o << 32 for g, o in zip(codes, out_codes)])
+    pairs = {(g, o): _DTYPE[g] | _DTYPE[o] << 32 for g, o in set(zip(dtypes, out_dtypes))}
+    rec[3::4] = array("q", map(pairs.__getitem__, zip(dtypes, out_dtypes)))
     lib = _lib.load()
     addr = rec.buffer_info()[0]
     with _lib.on_device(dev):
@@ -59,9 +63,9 @@ def _run(grads, codes, outs, out_codes, max_norm, eps, scale):
 def grad_norm(grads):
     """2-norm over all tensors of ``grads`` (float32 or bfloat16, any mix and shapes): a float32
     scalar tensor.  Squares are summed in float64."""
-    ts, codes, _ = _checked(grads, "grads")
+    ts, dtypes, _ = _checked(grads, "grads")
     ts = _contiguous(ts)
-    return _run(ts, codes, ts, codes, 0.0, 0.0, False)
+    return _run(ts, dtypes, ts, dtypes, 0.0, 0.0, False)
 
 
 def clip_grad_norm(grads, max_norm: float, *, eps: float = 1e-6, out=None, inplace: bool = False):
@@ -73,7 +77,7 @@ def clip_grad_norm(grads, max_norm: float, *, eps: float = 1e-6, out=None, inpla
     gives tensors of the same shapes to write to, float32 or bfloat16 (bfloat16 gradients into
     the float32 buffers of an optimizer).  A NaN norm makes every gradient NaN.
     """
-    ts, codes, device = _checked(grads, "grads")
+    ts, dtypes, device = _checked(grads, "grads")
     if not float(max_norm) >= 0.0 or not float(eps) >= 0.0:
         raise ValueError("max_norm and eps must be non-negative")
     if inplace:
@@ -81,17 +85,17 @@ def clip_grad_norm(grads, max_norm: float, *, eps: float = 1e-6, out=None, inpla
             raise ValueError("give either out or inplace=True")
         if not all(map(_T.is_contiguous, ts)):
             raise ValueError("inplace=True needs contiguous gradients")
-        outs, out_codes = ts, codes
+        outs, out_dtypes = ts, dtypes
     else:
         ts = _contiguous(ts)
         if out is None:
-            outs, out_codes = [torch.empty_like(g) for g in ts], codes
+            outs, out_dtypes = [torch.empty_like(g) for g in ts], dtypes
         else:
-            outs, out_codes, out_device = _checked(out, "out") if len(out) else ([], [], device)
+            outs, out_dtypes, out_device = _checked(out, "out") if len(out) else ([], [], device)
             if len(outs) != len(ts):
                 raise ValueError(f"out has {len(outs)} tensors, grads {len(ts)}")
             if list(map(_T.size, outs)) != list(map(_T.size, ts)) or not all(map(_T.is_contiguous, outs)):
                 raise ValueError("out must hold contiguous tensors of grads' shapes")
             if out_device != device:
                 raise ValueError("out and grads must be on one device")
-    return outs, _run(ts, codes, outs, out_codes, max_norm, eps, True)
+    return outs, _run(ts, dtypes, outs, out_dtypes, max_norm, eps, True)
