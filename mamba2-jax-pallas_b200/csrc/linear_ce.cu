@@ -288,19 +288,19 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) logits_kernel(const __grid_c
     if (p.passes == 3) unscale = 1.f / scale_of(a.scales->x) / scale_of(a.scales->w);
   };
   gemm::run<CG, false, false>(p, smem, &ctl, prep, [&](const gemm::Tile& t, float (&v)[EC], int row0, int n0, int live,
-                                                 float4* stage) {
+                                                       int, uint4* stage) {
     const int row = row0 + (threadIdx.x & 31);
     const int y = row < live ? a.target[row] : -1;
     if (p.passes == 3) {
 #pragma unroll
       for (int i = 0; i < EC; ++i) v[i] *= unscale;
     }
-    if (a.logits) {
+    if (a.logits) {   // their rows are a multiple of 64 long
       float* o = a.logits + row0 * a.ld + n0;
-      const int rows = live - row0, cols = (int)min((int64_t)EC, a.vocab - n0);
-      gemm::by_rows4(stage, v, [&](int i, int c, float4 x) {
-        if (i < rows && c < cols) *reinterpret_cast<float4*>(o + i * a.ld + c) = x;
-      });
+      const int cols = (int)min((int64_t)EC, a.vocab - n0);
+      gemm::by_rows<CG, float>(stage, v, true, live - row0, [&](int i, int c, uint4 q) {
+        if (c < cols) *reinterpret_cast<uint4*>(o + i * a.ld + c) = q;
+      }, [](int, int, float) {});
     }
     if (n0 + EC > a.vocab) {
 #pragma unroll
@@ -431,131 +431,104 @@ struct OutArgs {
   int64_t rows, cols;
   const int* index;        // row r of the result goes to row index[r] of out (NULL: to row r)
   void* out;               // (rows, cols), the result times alpha; NULL: into `part` only
-  int out_bf16;
   const float* alpha;
   float* part;             // f32: parts of a split K range (splits, rows, cols), or the running sum
-  int add_part;            // add what `part` holds (the running sum over token chunks)
+  int sum, add_part;       // `part` is the running sum over chunks of tokens; add what it holds
   const unsigned* largest[2];   // f32 inputs: what the operands' scales come from
 };
 
-// Where a gradient's tile goes: to the output, times alpha, or through `part`.
-enum Out { OUT_BF16, OUT_F32, OUT_PART };
+// OUT: tiles go to the output, times alpha.  PART: to f32 parts where the K range is split, or to
+// the running sum over chunks of tokens; the last chunk, and a range that the device did not
+// split, go to the output.
+enum Mode { OUT, PART };
 
-template <int CG, bool A_MN, Out MODE>
+template <int CG, bool A_MN, typename TO, Mode MODE>
 __global__ void __launch_bounds__(gemm::THREADS, 1) grad_gemm_kernel(const __grid_constant__ gemm::Problem p,
                                                                      const __grid_constant__ OutArgs a) {
   extern __shared__ uint8_t smem[];
   __shared__ gemm::Ctl ctl;
-  float f = 1.f, alpha = 1.f;
+  float unscale = 1.f, alpha = 1.f;
   auto prep = [&]() {
-    if (p.passes == 3) f = 1.f / scale_of(*a.largest[0]) / scale_of(*a.largest[1]);
+    if (p.passes == 3) unscale = 1.f / scale_of(*a.largest[0]) / scale_of(*a.largest[1]);
     alpha = *a.alpha;
-    if (MODE != OUT_PART) f *= alpha;
   };
   gemm::run<CG, A_MN, true>(p, smem, &ctl, prep, [&](const gemm::Tile& t, float (&v)[EC], int row0, int n0, int live,
-                                               float4* stage) {
-    const int rows = (int)min((int64_t)32, (p.limit_k ? a.rows : live) - row0);
-    const int cols = (int)min((int64_t)EC, a.cols - n0);
+                                                     int splits, uint4* stage) {
+    const int64_t all = p.limit_k ? a.rows : live;
+    const int rows = (int)min((int64_t)32, all - row0), cols = (int)min((int64_t)EC, a.cols - n0);
     if (rows <= 0 || cols <= 0) return;
+    const float f = MODE == OUT ? unscale * alpha : unscale;
 #pragma unroll
     for (int i = 0; i < EC; ++i) v[i] *= f;
-    if constexpr (MODE == OUT_BF16) {
-      bf16* out = static_cast<bf16*>(a.out) + n0;
-      const bool vec = vec_rows(out, a.cols);
-      gemm::by_rows8(stage, v, [&](int i, int c, float4 x, float4 y) {
-        if (i >= rows || c >= cols) return;
-        bf16* o = out + (a.index ? a.index[row0 + i] : row0 + i) * a.cols + c;
-        __nv_bfloat162 h[4] = {__floats2bfloat162_rn(x.x, x.y), __floats2bfloat162_rn(x.z, x.w),
-                               __floats2bfloat162_rn(y.x, y.y), __floats2bfloat162_rn(y.z, y.w)};
-        if (vec && c + 8 <= cols) {
-          *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(h);
-        } else {
-          const bf16* e = reinterpret_cast<const bf16*>(h);
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (c + k < cols) o[k] = e[k];
-        }
+    TO* out = static_cast<TO*>(a.out) + n0;
+    auto row_at = [&](int i) { return out + (int64_t)(a.index ? a.index[row0 + i] : row0 + i) * a.cols; };
+    bool vec = vec_rows(out, a.cols) && cols % (16 / (int)sizeof(TO)) == 0;
+    if constexpr (MODE == OUT) {
+      gemm::by_rows<CG, TO>(stage, v, vec, rows, [&](int i, int c, uint4 q) {
+        if (c < cols) *reinterpret_cast<uint4*>(row_at(i) + c) = q;
+      }, [&](int i, int c, TO x) {
+        if (c < cols) row_at(i)[c] = x;
       });
     } else {
-      // parts and running sums stay without alpha until they are complete
-      float* out = MODE == OUT_F32 ? static_cast<float*>(a.out) + n0
-                                   : a.part + ((int64_t)t.split * a.rows + row0) * a.cols + n0;
-      const bool vec = vec_rows(out, a.cols);
-      gemm::by_rows4(stage, v, [&](int i, int c, float4 x) {
-        if (i >= rows || c >= cols) return;
-        float e[4] = {x.x, x.y, x.z, x.w};
-        const bool whole = vec && c + 4 <= cols;
-        float* o = out + (MODE == OUT_F32 ? (a.index ? a.index[row0 + i] : row0 + i) : i) * a.cols + c;
-        if (MODE == OUT_PART && a.add_part) {
-          if (whole) {
-            const float4 q = *reinterpret_cast<const float4*>(o);
-            e[0] += q.x; e[1] += q.y; e[2] += q.z; e[3] += q.w;
-          } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (c + k < cols) e[k] += o[k];
-          }
+      const bool done = a.sum ? a.out != nullptr : splits == 1, add = a.sum && a.add_part;
+      float* part = a.part + ((int64_t)t.split * all + row0) * a.cols + n0;
+      vec = vec_rows(part, a.cols) && cols % 4 == 0 && (!done || vec);
+      gemm::by_rows<CG, float>(stage, v, vec, rows, [&](int i, int c, uint4 q) {
+        if (c >= cols) return;
+        float4 x = make_float4(__uint_as_float(q.x), __uint_as_float(q.y), __uint_as_float(q.z), __uint_as_float(q.w));
+        float4* at = reinterpret_cast<float4*>(part + i * a.cols + c);
+        if (add) {
+          const float4 y = *at;
+          x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
         }
-        if (MODE == OUT_PART && a.out) {
-          const int64_t at = (row0 + i) * a.cols + n0 + c;
-          if (a.out_bf16) {
-            bf16* w = static_cast<bf16*>(a.out) + at;
-            if (whole && reinterpret_cast<uintptr_t>(w) % 8 == 0) {
-              __nv_bfloat162 h[2] = {__floats2bfloat162_rn(e[0] * alpha, e[1] * alpha), __floats2bfloat162_rn(e[2] * alpha, e[3] * alpha)};
-              *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(h);
-            } else {
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                if (c + k < cols) w[k] = __float2bfloat16_rn(e[k] * alpha);
-            }
-          } else {
-            float* w = static_cast<float*>(a.out) + at;
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (c + k < cols) w[k] = e[k] * alpha;
-          }
-        } else if (whole) {
-          *reinterpret_cast<float4*>(o) = make_float4(e[0], e[1], e[2], e[3]);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (c + k < cols) o[k] = e[k];
-        }
+        if (!done)
+          *at = x;
+        else if constexpr (sizeof(TO) == 4)
+          *reinterpret_cast<float4*>(row_at(i) + c) = make_float4(x.x * alpha, x.y * alpha, x.z * alpha, x.w * alpha);
+        else
+          *reinterpret_cast<uint2*>(row_at(i) + c) =
+              make_uint2(gemm::pack_bf16(x.x * alpha, x.y * alpha), gemm::pack_bf16(x.z * alpha, x.w * alpha));
+      }, [&](int i, int c, float x) {
+        if (c >= cols) return;
+        float* at = part + i * a.cols + c;
+        if (add) x += *at;
+        if (done) st(row_at(i) + c, x * alpha);
+        else *at = x;
       });
     }
   });
 }
 
-// Sum of the parts of a split K range, in order, times alpha.  One CTA per row that counts.
-template <typename TO>
-__global__ void __launch_bounds__(256) join_kernel(const float* part, int splits, int64_t rows, int64_t cols, Selected s,
-                                                   int from, TO* out) {
+// Sum of the parts of a split K range, in order, times alpha; nothing where it was not split.
+// One CTA per row of the result (and per 1024 columns).
+template <int CG, typename TO>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ gemm::Problem p, const __grid_constant__ OutArgs a) {
   ptx::griddep_wait();
-  const int64_t row = blockIdx.x;
-  if (from + row >= *s.count) return;
-  const float f = *s.alpha;
-  TO* o = out + (int64_t)s.index[from + row] * cols;
-  const float* q = part + row * cols;
-  const int64_t step = rows * cols;
-  if (cols % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0) {   // the parts start at 256 bytes
-    for (int64_t c = threadIdx.x * 4; c < cols; c += 1024) {
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int j = 0; j < splits; ++j) {
-        const float4 x = *reinterpret_cast<const float4*>(q + j * step + c);
-        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
-      }
-      if constexpr (sizeof(TO) == 4) {
-        *reinterpret_cast<float4*>(o + c) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
-      } else {
-        __nv_bfloat162 h[2] = {__floats2bfloat162_rn(v.x * f, v.y * f), __floats2bfloat162_rn(v.z * f, v.w * f)};
-        *reinterpret_cast<uint2*>(o + c) = *reinterpret_cast<uint2*>(h);
-      }
+  const int live = gemm::live_rows(p), splits = gemm::splits_of<CG>(p, live);
+  const int64_t row = blockIdx.x, rows = p.limit_k ? a.rows : live;
+  if (splits == 1 || row >= rows) return;
+  const float f = *a.alpha;
+  TO* o = static_cast<TO*>(a.out) + (int64_t)(a.index ? a.index[row] : row) * a.cols;
+  const float* q = a.part + row * a.cols;
+  const int64_t step = rows * a.cols, c1 = min(a.cols, (int64_t)(blockIdx.y + 1) * 1024);
+  if (a.cols % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0) {   // the parts start at 256 bytes
+    const int64_t c = (int64_t)blockIdx.y * 1024 + threadIdx.x * 4;
+    if (c >= c1) return;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int j = 0; j < splits; ++j) {
+      const float4 x = *reinterpret_cast<const float4*>(q + j * step + c);
+      v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
     }
+    if constexpr (sizeof(TO) == 4)
+      *reinterpret_cast<float4*>(o + c) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+    else
+      *reinterpret_cast<uint2*>(o + c) = make_uint2(gemm::pack_bf16(v.x * f, v.y * f), gemm::pack_bf16(v.z * f, v.w * f));
     return;
   }
-  for (int64_t c = threadIdx.x; c < cols; c += 256) {
+  for (int64_t c = (int64_t)blockIdx.y * 1024 + threadIdx.x; c < c1; c += 256) {
     float v = 0.f;
+#pragma unroll 8
     for (int j = 0; j < splits; ++j) v += q[j * step + c];
     st(o + c, v * f);
   }
@@ -565,13 +538,14 @@ __global__ void __launch_bounds__(256) join_kernel(const float* part, int splits
 // host side
 // ---------------------------------------------------------------------------
 constexpr int SMS = 148;   // of a B200
+constexpr int MAX_SPLITS = 32;
 
 template <int CG, typename Kernel, typename Args>
 cudaError_t launch_gemm(Kernel kernel, const gemm::Problem& p, const Args& a, std::atomic<uint64_t>* allowed, cudaStream_t st) {
   constexpr int smem = gemm::Shape<CG>::SMEM;
   const cudaError_t e = allow_smem((const void*)kernel, smem, allowed);
   if (e != cudaSuccess) return e;
-  const int64_t units = (int64_t)p.m_tiles * p.n_tiles * p.splits;
+  const int64_t units = (int64_t)p.m_tiles * p.n_tiles * std::max(1, p.max_splits);
   return launch_dependent(kernel, dim3((unsigned)(CG * std::min<int64_t>(units, SMS / CG))), gemm::THREADS, smem, CG, st, p, a);
 }
 
@@ -589,27 +563,10 @@ struct Plan {
   bool grad;
   int planes;
   int64_t chunk, nchunks, ns, ld;   // tokens of a chunk; statistics per row; logits' row length
-  int splits;                       // of the reduction over the vocabulary (dX)
+  int64_t part_x, part_w;           // values that the parts of split K ranges may take (0: no split)
   bool pack_w, sum_w;       // sum_w: dW's running sum over chunks needs its own f32 buffer
   size_t one, index, target, rows, picked, factors, stats, x, w, logits, dl[2], part, wsum, total;
 };
-
-int split_k(int64_t rows, int64_t dim, int64_t vocab) {
-  // enough units of work to fill the GPU: the split whose last wave wastes least, no part
-  // shorter than 32 K blocks
-  const int64_t tiles = (int64_t)cdiv(rows, 2 * BM) * cdiv(dim, BN), sms = 74;
-  const int most = (int)std::min<int64_t>(16, std::max<int64_t>(1, vocab / (32 * 64)));
-  int best = 1;
-  double cost = 1e30;
-  for (int s = 1; s <= most; ++s) {
-    const double c = (double)cdiv(tiles * s, sms) / s * (1.0 + 0.01 * s);
-    if (c < cost) {
-      cost = c;
-      best = s;
-    }
-  }
-  return best;
-}
 
 Plan plan_of(const ssd_linear_ce_params_t* p) {
   Plan q{};
@@ -627,8 +584,12 @@ Plan plan_of(const ssd_linear_ce_params_t* p) {
   }
   q.nchunks = cdiv(p->tokens, q.chunk);
   q.pack_w = !direct(p->weight, p->weight_stride_row, p->dtype);
-  q.splits = p->grad_hidden ? split_k(q.chunk, p->dim, p->vocab) : 1;
   q.sum_w = p->grad_weight && q.nchunks > 1;
+  // the reduction over the vocabulary may be split in up to 32 parts (how many, the device decides:
+  // it knows how many rows count); that over tokens only where the weight is a few tiles
+  const int64_t x_values = q.chunk * p->dim, w_values = p->vocab * p->dim;
+  q.part_x = p->grad_hidden ? std::min<int64_t>(MAX_SPLITS * x_values, std::max<int64_t>(4 * x_values, 1 << 25)) : 0;
+  q.part_w = p->grad_weight && !q.sum_w && w_values <= (1 << 24) ? std::min<int64_t>(MAX_SPLITS * w_values, 1 << 25) : 0;
   size_t at = 256;   // the status word
   auto take = [&](size_t bytes) {
     const size_t o = at;
@@ -647,7 +608,7 @@ Plan plan_of(const ssd_linear_ce_params_t* p) {
   if (q.grad) {
     q.logits = take((size_t)q.chunk * q.ld * 4);
     for (int i = 0; i < q.planes; ++i) q.dl[i] = take((size_t)q.chunk * q.ld * 2);
-    q.part = take(q.splits > 1 ? (size_t)q.splits * q.chunk * p->dim * 4 : 0);
+    q.part = take((size_t)std::max(q.part_x, q.part_w) * 4);   // one after the other
     q.wsum = take(q.sum_w ? (size_t)p->vocab * p->dim * 4 : 0);
   }
   q.total = at;
@@ -673,7 +634,6 @@ cudaError_t logits_gemm(const Operand& x, const Operand& w, int planes, const Lo
   if (!maps(g.a, x, planes, BM) || !maps(g.b, w, planes, BN / CG)) return cudaErrorInvalidValue;
   g.m_tiles = cdiv(x.rows, BM * CG);
   g.n_tiles = cdiv(a.vocab, BN);
-  g.splits = 1;
   g.k_blocks = cdiv(x.dim, gemm::BK);
   g.passes = planes == 2 ? 3 : 1;
   g.m_fastest = 1;
@@ -683,9 +643,10 @@ cudaError_t logits_gemm(const Operand& x, const Operand& w, int planes, const Lo
   return launch_gemm<CG>(logits_kernel<CG>, g, a, &allowed, st);
 }
 
-template <int CG, bool A_MN>
-cudaError_t grad_gemm(const Operand& a, const Operand& b, int64_t k, int planes, int splits, const OutArgs& o,
-                      const int* count, int from, unsigned* status, cudaStream_t st) {
+// One gradient: the GEMM, and where its K range may be split the sum of the parts.
+template <int CG, bool A_MN, typename TO>
+cudaError_t grad_gemm(const Operand& a, const Operand& b, int64_t k, int planes, int64_t part_values,
+                      const OutArgs& o, const int* count, int from, unsigned* status, cudaStream_t st) {
   gemm::Problem g{};
   g.limit = count;
   g.limit_from = from;
@@ -694,17 +655,27 @@ cudaError_t grad_gemm(const Operand& a, const Operand& b, int64_t k, int planes,
   if (!maps(g.a, a, planes, A_MN ? 64 : BM) || !maps(g.b, b, planes, 64)) return cudaErrorInvalidValue;
   g.m_tiles = cdiv(o.rows, BM * CG);
   g.n_tiles = cdiv(o.cols, BN);
-  g.splits = splits;
+  g.rows_out = (int)o.rows;
+  g.cols = (int)o.cols;
+  g.max_splits = part_values > 0 ? MAX_SPLITS : 1;
+  g.part_values = part_values;
   g.k_blocks = cdiv(k, gemm::BK);
   g.passes = planes == 2 ? 3 : 1;
   g.m_fastest = 0;
   // bf16: the operands' own rounding is a hundred times what the adds lose
   g.segment = planes == 2 ? SEGMENT_F32 : 1 << 20;
   g.status = status;
-  static std::atomic<uint64_t> allowed[3] = {};
-  if (o.part) return launch_gemm<CG>(grad_gemm_kernel<CG, A_MN, OUT_PART>, g, o, &allowed[0], st);
-  if (o.out_bf16) return launch_gemm<CG>(grad_gemm_kernel<CG, A_MN, OUT_BF16>, g, o, &allowed[1], st);
-  return launch_gemm<CG>(grad_gemm_kernel<CG, A_MN, OUT_F32>, g, o, &allowed[2], st);
+  static std::atomic<uint64_t> allowed[2] = {};
+  if (!o.sum && g.max_splits == 1) return launch_gemm<CG>(grad_gemm_kernel<CG, A_MN, TO, OUT>, g, o, &allowed[0], st);
+  const cudaError_t e = launch_gemm<CG>(grad_gemm_kernel<CG, A_MN, TO, PART>, g, o, &allowed[1], st);
+  if (e != cudaSuccess || g.max_splits == 1) return e;
+  return launch_dependent(join_kernel<CG, TO>, dim3((unsigned)o.rows, (unsigned)cdiv(o.cols, 1024)), 256, 0, 1, st, g, o);
+}
+
+template <bool A_MN, typename... Args>
+cudaError_t grad_gemm_as(bool pair, bool bf16_out, Args&&... args) {
+  if (pair) return bf16_out ? grad_gemm<2, A_MN, bf16>(args...) : grad_gemm<2, A_MN, float>(args...);
+  return bf16_out ? grad_gemm<1, A_MN, bf16>(args...) : grad_gemm<1, A_MN, float>(args...);
 }
 
 }  // namespace
@@ -801,31 +772,27 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
     Operand dl{};
     dl.rows = n; dl.dim = p->vocab; dl.ld = q.ld;
     for (int i = 0; i < q.planes; ++i) dl.plane[i] = r.dl[i];
+    OutArgs o{};
+    o.alpha = sel.alpha;
+    o.largest[0] = &sel.scales->dl;
+    o.part = reinterpret_cast<float*>(ws + q.part);
     if (p->grad_hidden) {
-      OutArgs o{};
-      o.rows = n; o.cols = p->dim; o.alpha = sel.alpha; o.out_bf16 = bf; o.index = sel.index + t0;
-      o.largest[0] = &sel.scales->dl; o.largest[1] = &sel.scales->w;
-      if (q.splits > 1) o.part = reinterpret_cast<float*>(ws + q.part);
-      else o.out = p->grad_hidden;
-      if (n > BM) CE_CHECK((grad_gemm<2, false>(dl, w, p->vocab, q.planes, q.splits, o, sel.count, from, status, st)), "grad_hidden");
-      else CE_CHECK((grad_gemm<1, false>(dl, w, p->vocab, q.planes, q.splits, o, sel.count, from, status, st)), "grad_hidden");
-      if (q.splits > 1) {
-        if (bf)
-          err = launch_dependent(join_kernel<bf16>, (unsigned)n, 256, 0, 1, st, o.part, q.splits, n, p->dim, sel, from, static_cast<bf16*>(p->grad_hidden));
-        else
-          err = launch_dependent(join_kernel<float>, (unsigned)n, 256, 0, 1, st, o.part, q.splits, n, p->dim, sel, from, static_cast<float*>(p->grad_hidden));
-        CE_CHECK(err, "grad_hidden join");
-      }
+      OutArgs ox = o;
+      ox.rows = n; ox.cols = p->dim; ox.index = sel.index + t0; ox.out = p->grad_hidden;
+      ox.largest[1] = &sel.scales->w;
+      CE_CHECK(grad_gemm_as<false>(n > BM, bf, dl, w, p->vocab, q.planes, q.part_x, ox, sel.count, from, status, st),
+               "grad_hidden");
     }
     if (p->grad_weight) {
-      OutArgs o{};
-      o.rows = p->vocab; o.cols = p->dim; o.alpha = sel.alpha; o.out_bf16 = p->grad_weight_dtype == SSD_DTYPE_BF16;
-      o.largest[0] = &sel.scales->dl; o.largest[1] = &sel.scales->x;
-      if (q.sum_w) o.part = reinterpret_cast<float*>(ws + q.wsum);
-      o.add_part = c > 0;
-      o.out = c == q.nchunks - 1 ? p->grad_weight : nullptr;
-      if (p->vocab > BM) CE_CHECK((grad_gemm<2, true>(dl, xc, n, q.planes, 1, o, sel.count, from, status, st)), "grad_weight");
-      else CE_CHECK((grad_gemm<1, true>(dl, xc, n, q.planes, 1, o, sel.count, from, status, st)), "grad_weight");
+      OutArgs ow = o;
+      ow.rows = p->vocab; ow.cols = p->dim;
+      ow.largest[1] = &sel.scales->x;
+      if (q.sum_w) ow.part = reinterpret_cast<float*>(ws + q.wsum);
+      ow.sum = q.sum_w;
+      ow.add_part = c > 0;
+      ow.out = c == q.nchunks - 1 ? p->grad_weight : nullptr;
+      CE_CHECK(grad_gemm_as<true>(p->vocab > BM, p->grad_weight_dtype == SSD_DTYPE_BF16, dl, xc, n, q.planes, q.part_w, ow,
+                                  sel.count, from, status, st), "grad_weight");
     }
   }
   if (p->reduction != SSD_REDUCE_NONE) {

@@ -52,7 +52,7 @@ struct SmallArgs {
   RowFactors* factors;      // (tokens) or NULL
   // gradients
   float* part;              // (ranges, rows, dim): grad_hidden's sums
-  int ranges;
+  int ranges, group;        // ranges of words; threads that share one
   void* gx;
   void* gw;
   int gw_bf16;
@@ -61,16 +61,41 @@ struct SmallArgs {
 template <typename T>
 __device__ __forceinline__ float value(const T* p, int64_t i) { return ld(p + i); }
 
-// K consecutive values: 16 bytes of T.
-template <typename T>
-struct Vec {
-  static constexpr int K = 16 / sizeof(T);
-  uint4 q;
-  __device__ __forceinline__ float at(int k) const {
-    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
-    if constexpr (sizeof(T) == 4) return __uint_as_float(u[k]);
-    return __uint_as_float(k & 1 ? u[k / 2] & 0xffff0000u : u[k / 2] << 16);
+// 16 bytes of one word's row, as a lane holds them: U accesses of K values each.  U = 1 where rows
+// are aligned to 16 bytes; else the widest access that every row allows.
+template <typename T, int U>
+struct Piece {
+  static constexpr int K = 16 / sizeof(T) / U, COLS = 32 * K * U;   // columns of a warp's piece
+  uint32_t u[4];
+  __device__ __forceinline__ void load(const T* row, int c0, int dim) {
+    const int lane = threadIdx.x & 31;
+    if constexpr (U == 1) {
+      const int c = c0 + lane * K;
+      uint4 q = make_uint4(0, 0, 0, 0);
+      if (c < dim) q = *reinterpret_cast<const uint4*>(row + c);
+      u[0] = q.x; u[1] = q.y; u[2] = q.z; u[3] = q.w;
+    } else if constexpr (U == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = c0 + (i * 32 + lane) * K;
+        u[i] = c < dim ? *reinterpret_cast<const uint32_t*>(row + c) : 0u;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = c0 + 2 * i * 32 + lane;
+        const uint32_t a = c < dim ? *reinterpret_cast<const uint16_t*>(row + c) : 0u;
+        const uint32_t b = c + 32 < dim ? *reinterpret_cast<const uint16_t*>(row + c + 32) : 0u;
+        u[i] = a | b << 16;
+      }
+    }
   }
+  // value i of the 16 / sizeof(T), and its column (from c0)
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(u[i]);
+    return __uint_as_float(i & 1 ? u[i / 2] & 0xffff0000u : u[i / 2] << 16);
+  }
+  static __device__ __forceinline__ int col(int i) { return (i / K * 32 + (threadIdx.x & 31)) * K + i % K; }
 };
 
 // Values v[0..N) summed over the warp; lane l ends with the sum of value l % N.
@@ -93,13 +118,18 @@ __device__ __forceinline__ float warp_sums(float (&v)[N]) {
   return s;
 }
 
-// blockIdx.y: rows 8 y ..; R of them are computed (those past the last token on zeros).
-template <typename T, int R, bool VECTOR>
+// blockIdx.y: rows 8 y ..; R of them are computed (those past the last token on zeros).  The
+// pieces of the weight are loaded two steps ahead, across the ends of the words, so that a
+// warp's reductions do not leave the memory idle.
+template <typename T, int R, int U>
 __global__ void __launch_bounds__(SM_THREADS, 1) small_logits_kernel(const __grid_constant__ SmallArgs a) {
-  extern __shared__ float xs[];   // (R, dim rounded up to 8)
+  using P = Piece<T, U>;
+  constexpr int V = 16 / sizeof(T);
+  extern __shared__ float xs[];   // (R, dim rounded up to whole pieces)
   __shared__ float2 red[SM_WARPS][R * WORDS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int row0 = blockIdx.y * MAX_ROWS, rows = min(R, a.tokens - row0), pitch = (a.dim + 7) / 8 * 8;
+  const int row0 = blockIdx.y * MAX_ROWS, rows = min(R, a.tokens - row0);
+  const int steps = (a.dim + P::COLS - 1) / P::COLS, pitch = steps * P::COLS;
   const T* x = static_cast<const T*>(a.x) + row0 * a.xs;
   if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) *a.status = 0;
   for (int i = tid; i < R * pitch; i += SM_THREADS) {
@@ -110,50 +140,51 @@ __global__ void __launch_bounds__(SM_THREADS, 1) small_logits_kernel(const __gri
   const int my_row = (lane / WORDS) % R, my_word = lane % WORDS;
   const int64_t y = my_row < rows ? target_at(a.targets, a.is64, row0 + my_row) : -1;
   __syncthreads();
-  float top = -INFINITY, sum = 0.f;
-  const int step = SM_CTAS * SM_WARPS * WORDS;
-  for (int v0 = (blockIdx.x * SM_WARPS + warp) * WORDS; v0 < a.vocab; v0 += step) {
-    const T* w[WORDS];
+  const int stride = SM_CTAS * SM_WARPS * WORDS;
+  int next_v = (blockIdx.x * SM_WARPS + warp) * WORDS, next_s = 0;
+  auto fetch = [&](P (&q)[WORDS]) {   // the next piece of the next words, in the order of their use
+    if (next_v < a.vocab) {
 #pragma unroll
-    for (int j = 0; j < WORDS; ++j) w[j] = static_cast<const T*>(a.w) + (int64_t)min(v0 + j, a.vocab - 1) * a.ws;
+      for (int j = 0; j < WORDS; ++j)
+        q[j].load(static_cast<const T*>(a.w) + (int64_t)min(next_v + j, a.vocab - 1) * a.ws, next_s * P::COLS, a.dim);
+    }
+    if (++next_s == steps) {
+      next_s = 0;
+      next_v += stride;
+    }
+  };
+  float top = -INFINITY, sum = 0.f;
+  P q0[WORDS], q1[WORDS], q2[WORDS];
+  fetch(q0);
+  fetch(q1);
+  for (int v0 = (blockIdx.x * SM_WARPS + warp) * WORDS; v0 < a.vocab; v0 += stride) {
     float acc[WORDS * R];
 #pragma unroll
     for (int i = 0; i < WORDS * R; ++i) acc[i] = 0.f;
-    if constexpr (VECTOR) {
-      constexpr int K = Vec<T>::K;
-#pragma unroll 2
-      for (int c = lane * K; c < a.dim; c += 32 * K) {
-        Vec<T> q[WORDS];
+#pragma unroll 1
+    for (int s = 0; s < steps; ++s) {
+      fetch(q2);
+      const float* xc = xs + s * P::COLS;
 #pragma unroll
-        for (int j = 0; j < WORDS; ++j) q[j].q = *reinterpret_cast<const uint4*>(w[j] + c);
+      for (int r = 0; r < R; ++r) {
+        constexpr int G = P::K >= 4 ? 4 : P::K;    // columns side by side in shared memory
 #pragma unroll
-        for (int k0 = 0; k0 < K; k0 += 4) {
+        for (int i = 0; i < V; i += G) {
+          float xv[G];
+          const float* at = xc + r * pitch + P::col(i);
+          if constexpr (G == 4) *reinterpret_cast<float4*>(xv) = *reinterpret_cast<const float4*>(at);
+          else if constexpr (G == 2) *reinterpret_cast<float2*>(xv) = *reinterpret_cast<const float2*>(at);
+          else xv[0] = *at;
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const float4 xv = *reinterpret_cast<const float4*>(xs + r * pitch + c + k0);
+          for (int k = 0; k < G; ++k)
 #pragma unroll
-            for (int j = 0; j < WORDS; ++j) {
-              float& s = acc[r * WORDS + j];
-              s = fmaf(q[j].at(k0), xv.x, s);
-              s = fmaf(q[j].at(k0 + 1), xv.y, s);
-              s = fmaf(q[j].at(k0 + 2), xv.z, s);
-              s = fmaf(q[j].at(k0 + 3), xv.w, s);
-            }
-          }
+            for (int j = 0; j < WORDS; ++j) acc[r * WORDS + j] = fmaf(q0[j].at(i + k), xv[k], acc[r * WORDS + j]);
         }
       }
-    } else {
-#pragma unroll 4
-      for (int c = lane; c < a.dim; c += 32) {
-        float q[WORDS];
 #pragma unroll
-        for (int j = 0; j < WORDS; ++j) q[j] = value(w[j], c);
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const float xv = xs[r * pitch + c];
-#pragma unroll
-          for (int j = 0; j < WORDS; ++j) acc[r * WORDS + j] = fmaf(q[j], xv, acc[r * WORDS + j]);
-        }
+      for (int j = 0; j < WORDS; ++j) {
+        q0[j] = q1[j];
+        q1[j] = q2[j];
       }
     }
     const float s = warp_sums(acc);
@@ -218,7 +249,7 @@ __global__ void __launch_bounds__(256) small_finish_kernel(const __grid_constant
 }
 
 template <typename T, bool VECTOR>
-__device__ __forceinline__ void load4(const T* row, int c, int dim, float (&v)[4]) {
+__device__ __forceinline__ void load4(const T* row, int c, int dim, int step, float (&v)[4]) {
   if constexpr (VECTOR) {
     // 4 columns side by side
     if constexpr (sizeof(T) == 4) {
@@ -233,11 +264,11 @@ __device__ __forceinline__ void load4(const T* row, int c, int dim, float (&v)[4
     }
   } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = c + k * G_THREADS < dim ? value(row, c + k * G_THREADS) : 0.f;
+    for (int k = 0; k < 4; ++k) v[k] = c + k * step < dim ? value(row, c + k * step) : 0.f;
   }
 }
 template <typename T, bool VECTOR>
-__device__ __forceinline__ void store4(T* row, int c, int dim, const float (&v)[4]) {
+__device__ __forceinline__ void store4(T* row, int c, int dim, int step, const float (&v)[4]) {
   if constexpr (VECTOR) {
     if (c >= dim) return;
     if constexpr (sizeof(T) == 4) {
@@ -249,19 +280,19 @@ __device__ __forceinline__ void store4(T* row, int c, int dim, const float (&v)[
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (c + k * G_THREADS < dim) st(row + c + k * G_THREADS, v[k]);
+      if (c + k * step < dim) st(row + c + k * step, v[k]);
   }
 }
 
-// CTA (range of words, 1024 columns); a thread holds 4 columns of every row of hidden and of
-// grad_hidden's sums.
+// CTA (ranges of words, 1024 columns); a thread holds 4 columns of every row of hidden and of
+// grad_hidden's sums.  Where hidden is narrow, groups of `a.group` threads take ranges of their own.
 template <typename T, typename TW, int R, bool VECTOR>
 __global__ void __launch_bounds__(G_THREADS) small_grad_kernel(const __grid_constant__ SmallArgs a) {
-  __shared__ float dl[G_TILE][R];
+  extern __shared__ float dl[];   // (groups * G_TILE, R)
   ptx::griddep_wait();
-  const int tid = threadIdx.x;
-  const int c0 = blockIdx.y * G_COLS, c = c0 + (VECTOR ? 4 * tid : tid);
-  const int per = (a.vocab + a.ranges - 1) / a.ranges, lo = blockIdx.x * per, hi = min(lo + per, a.vocab);
+  const int tid = threadIdx.x, groups = G_THREADS / a.group, g = tid / a.group, t = tid - g * a.group;
+  const int c = blockIdx.y * G_COLS + (VECTOR ? 4 * t : t), step = a.group;
+  const int per = (a.vocab + a.ranges - 1) / a.ranges, range = blockIdx.x * groups + g;
   float x[R][4], acc[R][4];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -269,86 +300,111 @@ __global__ void __launch_bounds__(G_THREADS) small_grad_kernel(const __grid_cons
     for (int k = 0; k < 4; ++k) x[r][k] = acc[r][k] = 0.f;
     // an ignored row may hold anything
     if (r < a.tokens && target_at(a.targets, a.is64, r) != a.ignore)
-      load4<T, VECTOR>(static_cast<const T*>(a.x) + r * a.xs, c, a.dim, x[r]);
+      load4<T, VECTOR>(static_cast<const T*>(a.x) + r * a.xs, c, a.dim, step, x[r]);
   }
-  for (int v0 = lo; v0 < hi; v0 += G_TILE) {
-    const int n = min(G_TILE, hi - v0);
+  for (int off = 0; off < per; off += G_TILE) {
     __syncthreads();
-    for (int i = tid; i < G_TILE * R; i += G_THREADS) {
-      const int r = i / G_TILE, j = i - r * G_TILE, v = v0 + j;
+    for (int i = tid; i < groups * G_TILE * R; i += G_THREADS) {
+      const int r = i / (groups * G_TILE), e = i - r * (groups * G_TILE);
+      const int rg = blockIdx.x * groups + e / G_TILE, j = off + e % G_TILE;
+      const int64_t v = (int64_t)rg * per + j;
       float d = 0.f;
-      if (r < a.tokens && j < n) {
+      if (r < a.tokens && j < per && v < a.vocab) {
         const RowFactors f = a.factors[r];
         d = target_at(a.targets, a.is64, r) == v ? f.at_y : f.f * exp2f(fmaf(a.logits[r * a.ld + v], LOG2E, -f.top));
         if (f.f == 0.f && f.at_y == 0.f) d = 0.f;   // ignored: its logits may be NaN
       }
-      dl[j][r] = d;
+      dl[e * R + r] = d;
     }
     __syncthreads();
+    const int64_t v0 = (int64_t)range * per + off;
+    const int n = (int)min((int64_t)min(G_TILE, per - off), a.vocab - v0);
 #pragma unroll 4
     for (int j = 0; j < n; ++j) {
-      float w[4] = {0.f, 0.f, 0.f, 0.f}, g[4] = {0.f, 0.f, 0.f, 0.f};
-      if (a.gx) load4<T, VECTOR>(static_cast<const T*>(a.w) + (int64_t)(v0 + j) * a.ws, c, a.dim, w);
+      float w[4] = {0.f, 0.f, 0.f, 0.f}, gw[4] = {0.f, 0.f, 0.f, 0.f};
+      if (a.gx) load4<T, VECTOR>(static_cast<const T*>(a.w) + (v0 + j) * a.ws, c, a.dim, step, w);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const float d = dl[j][r];
+        const float d = dl[(g * G_TILE + j) * R + r];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           acc[r][k] = fmaf(d, w[k], acc[r][k]);
-          g[k] = fmaf(d, x[r][k], g[k]);
+          gw[k] = fmaf(d, x[r][k], gw[k]);
         }
       }
-      if (a.gw) store4<TW, VECTOR>(static_cast<TW*>(a.gw) + (int64_t)(v0 + j) * a.dim, c, a.dim, g);
+      if (a.gw) store4<TW, VECTOR>(static_cast<TW*>(a.gw) + (v0 + j) * a.dim, c, a.dim, step, gw);
     }
   }
   if (a.gx) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      if (r < a.tokens) store4<float, VECTOR>(a.part + ((int64_t)blockIdx.x * a.tokens + r) * a.dim, c, a.dim, acc[r]);
+      if (r < a.tokens) store4<float, VECTOR>(a.part + ((int64_t)range * a.tokens + r) * a.dim, c, a.dim, step, acc[r]);
   }
 }
 
-// grad_hidden: the ranges' sums, in order; a warp per 32 values, its lanes' loads coalesced.
+// grad_hidden: the ranges' sums.  A CTA takes 32 values: each of its warps adds a run of ranges,
+// and the runs are added in order.
+constexpr int J_WARPS = 16;
 template <typename T>
-__global__ void __launch_bounds__(256) small_join_kernel(const __grid_constant__ SmallArgs a) {
+__global__ void __launch_bounds__(32 * J_WARPS) small_join_kernel(const __grid_constant__ SmallArgs a) {
+  __shared__ float sums[J_WARPS][32];
   ptx::griddep_wait();
-  const int64_t n = (int64_t)a.tokens * a.dim, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t n = (int64_t)a.tokens * a.dim, i = (int64_t)blockIdx.x * 32 + lane;
+  const int per = (a.ranges + J_WARPS - 1) / J_WARPS, lo = warp * per, hi = min(lo + per, a.ranges);
   float s = 0.f;
+  if (i < n) {
 #pragma unroll 8
-  for (int j = 0; j < a.ranges; ++j) s += a.part[j * n + i];
+    for (int j = lo; j < hi; ++j) s += a.part[j * n + i];
+  }
+  sums[warp][lane] = s;
+  __syncthreads();
+  if (warp || i >= n) return;
+  for (int w = 1; w < J_WARPS; ++w) s += sums[w][lane];
   st(static_cast<T*>(a.gx) + i, s);
 }
 
 int row_width(int64_t tokens) { return tokens == 1 ? 1 : tokens == 2 ? 2 : tokens <= 4 ? 4 : 8; }
 
+// hidden's rows in f32, padded to whole pieces (at most 256 columns)
 size_t logits_smem(const ssd_linear_ce_params_t* p) {
-  return (size_t)row_width(p->tokens) * ((p->dim + 7) / 8 * 8) * 4;
+  return (size_t)row_width(p->tokens) * ((p->dim + 255) / 256 * 256) * 4;
 }
 
-template <typename T, int R>
-cudaError_t run_logits(const SmallArgs& a, bool vec, size_t smem, cudaStream_t st) {
-  auto kernel = vec ? small_logits_kernel<T, R, true> : small_logits_kernel<T, R, false>;
-  static std::atomic<uint64_t> allowed[2] = {};
-  const cudaError_t e = allow_smem((const void*)kernel, MAX_SMEM, &allowed[vec]);
+template <typename T, int R, int U>
+cudaError_t run_logits(const SmallArgs& a, size_t smem, cudaStream_t st) {
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e = allow_smem((const void*)small_logits_kernel<T, R, U>, MAX_SMEM, &allowed);
   if (e != cudaSuccess) return e;
-  kernel<<<dim3(SM_CTAS, (unsigned)cdiv(a.tokens, MAX_ROWS)), SM_THREADS, smem, st>>>(a);
+  small_logits_kernel<T, R, U><<<dim3(SM_CTAS, (unsigned)cdiv(a.tokens, MAX_ROWS)), SM_THREADS, smem, st>>>(a);
   return cudaGetLastError();
 }
-template <typename T>
-cudaError_t run_logits(const SmallArgs& a, bool vec, size_t smem, cudaStream_t st) {
+template <typename T, int U>
+cudaError_t run_logits(const SmallArgs& a, size_t smem, cudaStream_t st) {
   switch (row_width(a.tokens)) {
-    case 1: return run_logits<T, 1>(a, vec, smem, st);
-    case 2: return run_logits<T, 2>(a, vec, smem, st);
-    case 4: return run_logits<T, 4>(a, vec, smem, st);
-    default: return run_logits<T, 8>(a, vec, smem, st);
+    case 1: return run_logits<T, 1, U>(a, smem, st);
+    case 2: return run_logits<T, 2, U>(a, smem, st);
+    case 4: return run_logits<T, 4, U>(a, smem, st);
+    default: return run_logits<T, 8, U>(a, smem, st);
   }
+}
+// Every row of the weight can be read in accesses of `bytes`.
+bool reads_by(const ssd_linear_ce_params_t* p, int bytes) {
+  const int64_t es = p->dtype == SSD_DTYPE_BF16 ? 2 : 4;
+  return reinterpret_cast<uintptr_t>(p->weight) % bytes == 0 && p->weight_stride_row * es % bytes == 0 && p->dim * es % bytes == 0;
+}
+cudaError_t run_logits(const ssd_linear_ce_params_t* p, const SmallArgs& a, cudaStream_t st) {
+  const size_t smem = logits_smem(p);
+  if (p->dtype == SSD_DTYPE_F32) return reads_by(p, 16) ? run_logits<float, 1>(a, smem, st) : run_logits<float, 4>(a, smem, st);
+  if (reads_by(p, 16)) return run_logits<bf16, 1>(a, smem, st);
+  return reads_by(p, 4) ? run_logits<bf16, 4>(a, smem, st) : run_logits<bf16, 8>(a, smem, st);
 }
 
 template <typename T, typename TW, int R>
 cudaError_t run_grad(const SmallArgs& a, bool vec, cudaStream_t st) {
   return launch_dependent(vec ? small_grad_kernel<T, TW, R, true> : small_grad_kernel<T, TW, R, false>,
-                          dim3((unsigned)a.ranges, (unsigned)cdiv(a.dim, G_COLS)), G_THREADS, 0, 1, st, a);
+                          dim3((unsigned)(a.ranges / (G_THREADS / a.group)), (unsigned)cdiv(a.dim, G_COLS)), G_THREADS,
+                          (size_t)(G_THREADS / a.group) * G_TILE * R * sizeof(float), 1, st, a);
 }
 template <typename T, typename TW>
 cudaError_t run_grad(const SmallArgs& a, bool vec, cudaStream_t st) {
@@ -367,7 +423,7 @@ bool aligned(const void* p, int64_t stride, int64_t dim, int dtype) {
 
 struct SmallPlan {
   size_t picked, factors, stats, logits, part, total;
-  int ranges;
+  int ranges, group;
   int64_t ld;
 };
 
@@ -375,8 +431,11 @@ SmallPlan plan_of(const ssd_linear_ce_params_t* p) {
   SmallPlan q{};
   const bool grad = p->grad_hidden || p->grad_weight;
   q.ld = (p->vocab + 63) / 64 * 64;
-  // about eight CTAs per SM over the ranges and column blocks
-  q.ranges = (int)std::max<int64_t>(1, std::min<int64_t>(cdiv(SM_CTAS * 8, cdiv(p->dim, G_COLS)), cdiv(p->vocab, 16)));
+  q.group = 32;
+  while (q.group < G_THREADS && q.group * 4 < p->dim) q.group *= 2;
+  // about eight CTAs per SM over the ranges and column blocks, and 16 words or more in a range
+  const int groups = G_THREADS / q.group;
+  q.ranges = groups * (int)std::max<int64_t>(1, std::min<int64_t>(cdiv(SM_CTAS * 8, cdiv(p->dim, G_COLS)), cdiv(p->vocab, 16 * groups)));
   size_t at = 256;   // the status word, as in every workspace
   auto take = [&](size_t bytes) {
     const size_t o = at;
@@ -427,18 +486,18 @@ cudaError_t launch_linear_ce_small(const ssd_linear_ce_params_t* p, void* worksp
   a.factors = grad ? reinterpret_cast<RowFactors*>(ws + q.factors) : nullptr;
   a.part = reinterpret_cast<float*>(ws + q.part);
   a.ranges = q.ranges;
+  a.group = q.group;
   a.gx = p->grad_hidden; a.gw = p->grad_weight; a.gw_bf16 = p->grad_weight_dtype == SSD_DTYPE_BF16;
-  const bool vec = aligned(p->weight, p->weight_stride_row, p->dim, p->dtype);
-  CE_CHECK(bf ? run_logits<bf16>(a, vec, logits_smem(p), st) : run_logits<float>(a, vec, logits_smem(p), st), "logits");
+  CE_CHECK(run_logits(p, a, st), "logits");
   CE_CHECK(launch_dependent(small_finish_kernel, dim3(1), 256, 0, 1, st, a), "loss");
   if (!grad) return cudaSuccess;
-  const bool gvec = vec && aligned(p->hidden, p->hidden_stride_row, p->dim, p->dtype) &&
+  const bool gvec = aligned(p->weight, p->weight_stride_row, p->dim, p->dtype) && aligned(p->hidden, p->hidden_stride_row, p->dim, p->dtype) &&
                     (!p->grad_weight || aligned(p->grad_weight, p->dim, p->dim, p->grad_weight_dtype));
   if (bf) CE_CHECK((a.gw_bf16 ? run_grad<bf16, bf16>(a, gvec, st) : run_grad<bf16, float>(a, gvec, st)), "gradients");
   else CE_CHECK((a.gw_bf16 ? run_grad<float, bf16>(a, gvec, st) : run_grad<float, float>(a, gvec, st)), "gradients");
   if (p->grad_hidden)
     CE_CHECK(launch_dependent(bf ? small_join_kernel<bf16> : small_join_kernel<float>,
-                              dim3((unsigned)cdiv(p->tokens * p->dim, 256)), 256, 0, 1, st, a), "grad_hidden");
+                              dim3((unsigned)cdiv(p->tokens * p->dim, 32)), 32 * J_WARPS, 0, 1, st, a), "grad_hidden");
   return cudaSuccess;
 }
 

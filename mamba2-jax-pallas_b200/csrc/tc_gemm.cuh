@@ -41,15 +41,16 @@ constexpr int EPI_COLS = 64;               // columns of an epilogue warp
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr long long WAIT_CYCLES = 4000000000LL;   // about 2 s at the boost clock
 
-// Each epilogue warp turns its rows through shared memory, 16 columns at a time, so that what it
-// writes to global memory are runs of one row and not one value of 32 rows.  A row's four
-// 16-byte chunks are permuted by its number, which keeps the accesses of a quarter-warp in
-// different banks, by rows and by columns.
-constexpr int EPI_WARP_BYTES = 32 * 64;
-
+// Each epilogue warp turns its 32 rows through shared memory, so that what it writes to global
+// memory are runs of one row and not one value of 32 rows: whole 128-byte lines in a pair's
+// tiles (with runs of 32 bytes, K = 64 products wrote 1.7 TB/s), 64 bytes where shared memory
+// is shorter.  A row's 16-byte chunks are permuted by its number, which keeps the accesses of a
+// quarter-warp in different banks, by rows and by columns.
 template <int CG>
 struct Shape {
-  static constexpr int STAGES = CG == 2 ? 6 : 4;
+  static constexpr int STAGES = CG == 2 ? 5 : 4;
+  static constexpr int EPI_ROW = CG == 2 ? 128 : 64;         // bytes of a staged row
+  static constexpr int EPI_WARP_BYTES = 32 * EPI_ROW;
   static constexpr int A_BYTES = BM * BK * 2;
   static constexpr int B_BYTES = BN / CG * BK * 2;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
@@ -70,7 +71,10 @@ struct Problem {
   CUtensorMap a[2], b[2];                 // planes hi and lo (lo unused for bf16 operands)
   const int* limit;
   int limit_from, rows, limit_k;
-  int m_tiles, n_tiles, splits;           // m tiles of CG * 128 rows
+  int m_tiles, n_tiles;                   // m tiles of CG * 128 rows
+  int max_splits;                         // of the K range, decided on the device (pick_splits)
+  int64_t part_values;                    // room for the parts
+  int rows_out, cols;                     // of the result (limit_k; else its rows are the live ones)
   int k_blocks;                           // of 64
   int passes;                             // 1 (bf16), or 3 (f32 as two f16 planes)
   int segment;                            // K blocks that are summed in TMEM
@@ -85,7 +89,23 @@ struct Tile {
 // Rows that count, of those that the launch was made for.
 __device__ __forceinline__ int live_rows(const Problem& p) { return min(max(*p.limit - p.limit_from, 0), p.rows); }
 
-__device__ __forceinline__ Tile tile_at(const Problem& p, int m_tiles, int k_blocks, int64_t u) {
+// Parts of the K range: enough units of work to fill the GPU where there are few tiles.  Cost in
+// K blocks of one wave of units (a unit's start and epilogue count as 12), plus 8 bytes per
+// value and part written and read again (at 6 TB/s; a K block takes 0.37 us).  A warp tries 32.
+template <int CG>
+__device__ __forceinline__ int pick_splits(int tiles, int blocks, int64_t values, int max_splits, int64_t part_values) {
+  if (max_splits <= 1 || tiles <= 0) return 1;
+  const int s = (threadIdx.x & 31) + 1, ctas = 148 / CG;
+  float cost = (float)((tiles * s + ctas - 1) / ctas) * (float)((blocks + s - 1) / s + 12);
+  if (s > 1) cost += (float)s * (float)values * 3.6e-6f + 8.f;
+  if (s > max_splits || s * values > part_values || s > blocks) cost = 3e38f;
+  if (s == 1) cost = fminf(cost, 1e38f);
+  // positive floats order like their bits; the lowest lane of the least cost
+  const unsigned bits = __float_as_uint(cost), least = __reduce_min_sync(0xffffffffu, bits);
+  return __ffs(__ballot_sync(0xffffffffu, bits == least));
+}
+
+__device__ __forceinline__ Tile tile_at(const Problem& p, int m_tiles, int k_blocks, int splits, int64_t u) {
   Tile t;
   const int64_t per = (int64_t)m_tiles * p.n_tiles;
   t.split = (int)(u / per);
@@ -97,13 +117,13 @@ __device__ __forceinline__ Tile tile_at(const Problem& p, int m_tiles, int k_blo
     t.m = (int)(r / p.n_tiles);
     t.n = (int)(r - (int64_t)t.m * p.n_tiles);
   }
-  t.k0 = (int)((int64_t)k_blocks * t.split / p.splits);
-  t.k1 = (int)((int64_t)k_blocks * (t.split + 1) / p.splits);
+  t.k0 = (int)((int64_t)k_blocks * t.split / splits);
+  t.k1 = (int)((int64_t)k_blocks * (t.split + 1) / splits);
   return t;
 }
 
-// A probe that lets the hardware suspend the thread for up to a millisecond: 16 waiting
-// epilogue warps that poll cost 10 % of a power-bound GEMM.
+// A probe that lets the hardware suspend the thread for up to 20 us (20 ns to 1 ms measured
+// alike): 16 waiting epilogue warps that poll cost 10 % of a power-bound GEMM.
 __device__ __forceinline__ bool probe(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -111,7 +131,7 @@ __device__ __forceinline__ bool probe(uint64_t* bar, uint32_t parity) {
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
-      : "r"(ptx::smem_u32(bar)), "r"(parity), "r"(1000000)
+      : "r"(ptx::smem_u32(bar)), "r"(parity), "r"(20000)
       : "memory");
   return ok != 0;
 }
@@ -130,6 +150,15 @@ __device__ __forceinline__ bool wait(Ctl* c, uint64_t* bar, uint32_t parity, uns
   return true;
 }
 
+// The parts of a launch, given its live rows: the GEMM and what adds the parts agree on it.
+template <int CG>
+__device__ __forceinline__ int splits_of(const Problem& p, int live) {
+  const int m_tiles = p.limit_k ? p.m_tiles : (live + BM * CG - 1) / (BM * CG);
+  const int k_blocks = p.limit_k ? (live + BK - 1) / BK : p.k_blocks;
+  return pick_splits<CG>(m_tiles * p.n_tiles, k_blocks, (int64_t)(p.limit_k ? p.rows_out : live) * p.cols,
+                         p.max_splits, p.part_values);
+}
+
 // ---- the pair's forms of the PTX wrappers ------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -145,8 +174,10 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t saddr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
   return r;
 }
+// What the arrival orders are TMEM reads, by tcgen05 fences on both sides; a release at cluster
+// scope would also wait for the thread's global stores (half of a short tile's epilogue).
 __device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 template <int CG>
@@ -209,51 +240,58 @@ __device__ __forceinline__ uint32_t idesc(const Problem& p) {
   return p.passes == 3 ? ID & ~((1u << 7) | (1u << 10)) : ID;
 }
 
-__device__ __forceinline__ void epi_put(float4* stage, const float* v) {
-  const int lane = threadIdx.x & 31;
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    stage[lane * 4 + (i ^ ((lane >> 1) & 3))] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-  __syncwarp();
-}
-__device__ __forceinline__ float4 epi_get(const float4* stage, int row, int chunk) {
-  return stage[row * 4 + (chunk ^ ((row >> 1) & 3))];
+// Where chunk `c` of a staged row lies, in 16-byte units.
+template <int CG>
+__device__ __forceinline__ int epi_at(int row, int c) {
+  return CG == 2 ? row * 8 + (c ^ (row & 7)) : row * 4 + (c ^ ((row >> 1) & 3));
 }
 
-// Calls put(i, c, x) for every 16 bytes x of the warp's 32 x 64 block: row i, columns c .. c+3.
-// Lanes 4k .. 4k+3 hold 64 bytes of one row.
-template <typename Put>
-__device__ __forceinline__ void by_rows4(float4* stage, const float (&v)[EPI_COLS], Put&& put) {
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The warp's 32 x 64 block as values of T, by rows.  With `wide`, put(i, c, q) for every 16 bytes q
+// (row i, columns from c on); else put1(i, c, x) for every value, neighbouring lanes at
+// neighbouring columns.
+template <int CG, typename T, typename Put, typename Put1>
+__device__ __forceinline__ void by_rows(uint4* stage, const float (&v)[EPI_COLS], bool wide, int rows, Put&& put,
+                                        Put1&& put1) {
+  constexpr int CHUNKS = Shape<CG>::EPI_ROW / 16, PER = 16 / sizeof(T), COLS = CHUNKS * PER;
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int ch = 0; ch < EPI_COLS / 16; ++ch) {
-    epi_put(stage, v + 16 * ch);
+  for (int at = 0; at < EPI_COLS; at += COLS) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      const float* x = v + at + i * PER;
+      if constexpr (sizeof(T) == 4)
+        stage[epi_at<CG>(lane, i)] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+      else
+        stage[epi_at<CG>(lane, i)] = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+    }
+    __syncwarp();
+    if (wide) {
 #pragma unroll 2
-    for (int j = 0; j < 4; ++j) {
-      const int i = 8 * j + (lane >> 2);
-      put(i, 16 * ch + 4 * (lane & 3), epi_get(stage, i, lane & 3));
+      for (int j = 0; j < CHUNKS; ++j) {
+        const int i = j * (32 / CHUNKS) + lane / CHUNKS, c = lane % CHUNKS;
+        if (i < rows) put(i, at + c * PER, stage[epi_at<CG>(i, c)]);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < rows; ++i) {
+#pragma unroll 1
+        for (int c0 = 0; c0 < COLS; c0 += 32) {
+          const int c = c0 + lane;
+          if (c < COLS) put1(i, at + c, reinterpret_cast<const T*>(stage + epi_at<CG>(i, c / PER))[c % PER]);
+        }
+      }
     }
   }
 }
 
-// The same with 8 columns per call, for 16-bit results: lanes 2k and 2k+1 hold 32 bytes of a row.
-template <typename Put>
-__device__ __forceinline__ void by_rows8(float4* stage, const float (&v)[EPI_COLS], Put&& put) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int ch = 0; ch < EPI_COLS / 16; ++ch) {
-    epi_put(stage, v + 16 * ch);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int i = 16 * j + (lane >> 1), c = 2 * (lane & 1);
-      put(i, 16 * ch + 4 * c, epi_get(stage, i, c), epi_get(stage, i, c + 1));
-    }
-  }
-}
-
-// The kernel's body.  prep() runs on every thread once the launches before are complete.  epi(tile, v, row0, first column, rows that count, stage) runs on each
-// epilogue thread; v holds 64 values of row row0 + lane.
+// The kernel's body.  prep() runs on every thread once the launches before are complete.  epi(tile, v, row0, first column, rows that count, splits, stage) runs on each
+// epilogue thread; v holds 64 values of row row0 + lane; `splits` parts of the K range.
 template <int CG, bool A_MN, bool B_MN, typename Prep, typename Epi>
 __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c, Prep&& prep, Epi&& epi) {
   using S = Shape<CG>;
@@ -284,7 +322,8 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
   const int live = live_rows(p);
   const int m_tiles = p.limit_k ? p.m_tiles : (live + BM * CG - 1) / (BM * CG);
   const int k_blocks = p.limit_k ? (live + BK - 1) / BK : p.k_blocks;
-  const int64_t unit0 = blockIdx.x / CG, units = (int64_t)m_tiles * p.n_tiles * p.splits, step = gridDim.x / CG;
+  const int splits = splits_of<CG>(p, live);
+  const int64_t unit0 = blockIdx.x / CG, units = (int64_t)m_tiles * p.n_tiles * splits, step = gridDim.x / CG;
   if (warp == 0) {
     if (lane == 0) {
       for (int i = 0; i < (p.passes == 3 ? 2 : 1); ++i) {
@@ -294,7 +333,7 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
       uint32_t it = 0;
       bool ok = true;
       for (int64_t u = unit0; ok && u < units; u += step) {
-        const Tile t = tile_at(p, m_tiles, k_blocks, u);
+        const Tile t = tile_at(p, m_tiles, k_blocks, splits, u);
         const int m0 = (t.m * CG + (int)rank) * BM, n0 = t.n * BN + (int)rank * (BN / CG);
         for (int ps = 0; ok && ps < p.passes; ++ps) {
           // pass order hi*lo, lo*hi, hi*hi: the small products first
@@ -339,7 +378,7 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
       uint32_t it = 0, n = 0;
       bool ok = true;
       for (int64_t u = unit0; ok && u < units; u += step) {
-        const Tile t = tile_at(p, m_tiles, k_blocks, u);
+        const Tile t = tile_at(p, m_tiles, k_blocks, splits, u);
         const int steps = p.passes * (t.k1 - t.k0);
         uint32_t d = 0;
         for (int j = 0, left = 0; j < steps; ++j, ++it, --left) {
@@ -386,11 +425,11 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
     }
   } else {
     const int quad = warp & 3, col = (warp - 2) / 4 * EPI_COLS;
-    float4* stage = reinterpret_cast<float4*>(smem + S::STAGES * S::STAGE_BYTES + (warp - 2) * EPI_WARP_BYTES);
+    uint4* stage = reinterpret_cast<uint4*>(smem + S::STAGES * S::STAGE_BYTES + (warp - 2) * S::EPI_WARP_BYTES);
     uint32_t n = 0;
     bool ok = true;
     for (int64_t u = unit0; ok && u < units; u += step) {
-      const Tile t = tile_at(p, m_tiles, k_blocks, u);
+      const Tile t = tile_at(p, m_tiles, k_blocks, splits, u);
       float v[EPI_COLS];
 #pragma unroll
       for (int i = 0; i < EPI_COLS; ++i) v[i] = 0.f;
@@ -421,7 +460,7 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
             ptx::mbar_arrive(&c->acc_empty[n & 1]);
         }
       }
-      if (ok) epi(t, v, (t.m * CG + (int)rank) * BM + 32 * quad, t.n * BN + col, live, stage);
+      if (ok) epi(t, v, (t.m * CG + (int)rank) * BM + 32 * quad, t.n * BN + col, live, splits, stage);
     }
   }
   __syncwarp();
