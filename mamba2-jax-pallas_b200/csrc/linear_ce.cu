@@ -72,6 +72,7 @@ struct Selected {
   int* target;             // (tokens): its target, or -1 where that is outside [0, vocab)
   float* alpha;            // the factor common to all rows: 1 or 1 / count, times a scalar grad_loss
   unsigned* status;        // the workspace's status word
+  int* ticket;
   Scales* scales;
 };
 
@@ -120,6 +121,7 @@ __global__ void __launch_bounds__(1024) select_kernel(const void* targets, int i
   }
   if (tid == 0) {
     *s.status = 0;
+    *s.ticket = 0;
     *s.count = total;
     s.scales->x = s.scales->w = 0;
     s.scales->dl = sh_largest;
@@ -184,14 +186,18 @@ __device__ __forceinline__ bool vec_rows(const T* p, int64_t stride) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * sizeof(T) % 16 == 0;
 }
 
-// Largest finite magnitude of a matrix's rows (of those whose target counts, where given).
-__global__ void __launch_bounds__(256) largest_kernel(const float* src, int64_t stride, int64_t rows, int64_t dim,
-                                                      const void* targets, int is64, int64_t ignore, unsigned* out) {
+// Largest finite magnitude of hidden's rows that count (blockIdx.y = 0) and of the weight (1).
+__global__ void __launch_bounds__(256) largest_kernel(const float* x, int64_t x_stride, int64_t tokens, const float* w,
+                                                      int64_t w_stride, int64_t vocab, int64_t dim, const void* targets,
+                                                      int is64, int64_t ignore, Scales* out) {
   ptx::griddep_wait();
+  const bool of_w = blockIdx.y == 1;
+  const float* src = of_w ? w : x;
+  const int64_t stride = of_w ? w_stride : x_stride, rows = of_w ? vocab : tokens;
   unsigned m = 0;
   const bool vec = vec_rows(src, stride);
   for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
-    if (targets && target_at(targets, is64, r) == ignore) continue;
+    if (!of_w && target_at(targets, is64, r) == ignore) continue;
 #pragma unroll 4
     for (int64_t c = (threadIdx.x & 31) * 8; c < dim; c += 256) {
       float v[8];
@@ -201,7 +207,7 @@ __global__ void __launch_bounds__(256) largest_kernel(const float* src, int64_t 
     }
   }
   m = __reduce_max_sync(0xffffffffu, m);
-  if ((threadIdx.x & 31) == 0 && m) atomicMax(out, m);
+  if ((threadIdx.x & 31) == 0 && m) atomicMax(of_w ? &out->w : &out->x, m);
 }
 
 // Planes of a whole matrix (the weight, where the tensor maps cannot read it as it is), a warp
@@ -327,38 +333,53 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) logits_kernel(const __grid_c
   });
 }
 
-// A warp per row that counts: its loss, and with `factors` what the gradients need.
+// The sum (or mean over the tokens that count) of the tokens' losses.
+struct Reduced {
+  float* out;              // one value, or NULL: the tokens' losses are the result
+  int64_t tokens;
+  int mean;
+  int* ticket;
+  int ctas;                // of loss_kernel, over all chunks
+};
+
+// A warp per row that counts: its loss, and with `factors` what the gradients need.  The last CTA
+// of the last chunk reduces the losses, in a fixed order.
 __global__ void __launch_bounds__(256) loss_kernel(const float2* stats, int ns, const float* picked, Selected s, int from,
                                                    int rows, float* loss, float* lse, const float* weight, int split,
-                                                   RowFactors* factors) {
+                                                   RowFactors* factors, const Reduced red) {
   ptx::griddep_wait();
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= rows || from + row >= *s.count) return;
-  const RowResult r = warp_row(stats + row * ns, ns, picked + row, s.target[from + row]);
-  if ((threadIdx.x & 31) == 0) {
-    const int t = s.index[from + row];
-    loss[t] = r.loss;
-    if (lse) lse[t] = r.lse;
-    if (factors) {
-      const float w = (weight ? weight[t] : 1.f) * (split ? scale_of(s.scales->dl) : 1.f);
-      factors[row] = {r.top, w * r.inv, w * r.pm1};
+  if (row < rows && from + row < *s.count) {
+    const RowResult r = warp_row(stats + row * ns, ns, picked + row, s.target[from + row]);
+    if ((threadIdx.x & 31) == 0) {
+      const int t = s.index[from + row];
+      loss[t] = r.loss;
+      if (lse) lse[t] = r.lse;
+      if (factors) {
+        const float w = (weight ? weight[t] : 1.f) * (split ? scale_of(s.scales->dl) : 1.f);
+        factors[row] = {r.top, w * r.inv, w * r.pm1};
+      }
     }
   }
-}
-
-// One CTA: sum (or mean over the tokens that count) of the tokens' losses, in a fixed order.
-__global__ void __launch_bounds__(1024) reduce_kernel(const float* rows, int64_t n, const int* count, int mean, float* out) {
-  ptx::griddep_wait();
-  __shared__ double sh[32];
-  double s = 0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) s += (double)rows[i];
+  if (!red.out) return;
+  __shared__ int last;
+  __shared__ double sh[8];
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(red.ticket, 1) == red.ctas - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double sum = 0;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < red.tokens; i += 256) sum += (double)__ldcg(loss + i);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = s;
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = sum;
   __syncthreads();
   if (threadIdx.x) return;
-  for (int i = 1; i < 32; ++i) s += sh[i];
-  *out = (float)(mean ? s / (double)max(*count, 1) : s);
+  for (int i = 1; i < 8; ++i) sum += sh[i];
+  *red.out = (float)(red.mean ? sum / (double)max(*s.count, 1) : sum);
 }
 
 // ---------------------------------------------------------------------------
@@ -500,37 +521,40 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) grad_gemm_kernel(const __gri
 }
 
 // Sum of the parts of a split K range, in order, times alpha; nothing where it was not split.
-// One CTA per row of the result (and per 1024 columns).
+// CTAs take rows of the result in turns.
 template <int CG, typename TO>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ gemm::Problem p, const __grid_constant__ OutArgs a) {
   ptx::griddep_wait();
   const int live = gemm::live_rows(p), splits = gemm::splits_of<CG>(p, live);
-  const int64_t row = blockIdx.x, rows = p.limit_k ? a.rows : live;
-  if (splits == 1 || row >= rows) return;
+  if (splits == 1) return;
+  const int64_t rows = p.limit_k ? a.rows : live, step = rows * a.cols;
   const float f = *a.alpha;
-  TO* o = static_cast<TO*>(a.out) + (int64_t)(a.index ? a.index[row] : row) * a.cols;
-  const float* q = a.part + row * a.cols;
-  const int64_t step = rows * a.cols, c1 = min(a.cols, (int64_t)(blockIdx.y + 1) * 1024);
-  if (a.cols % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0) {   // the parts start at 256 bytes
-    const int64_t c = (int64_t)blockIdx.y * 1024 + threadIdx.x * 4;
-    if (c >= c1) return;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int j = 0; j < splits; ++j) {
-      const float4 x = *reinterpret_cast<const float4*>(q + j * step + c);
-      v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+  const bool vec = a.cols % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;   // the parts start at 256 bytes
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    TO* o = static_cast<TO*>(a.out) + (int64_t)(a.index ? a.index[row] : row) * a.cols;
+    const float* q = a.part + row * a.cols;
+    if (vec) {
+#pragma unroll 2
+      for (int64_t c = threadIdx.x * 4; c < a.cols; c += 1024) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int j = 0; j < splits; ++j) {
+          const float4 x = *reinterpret_cast<const float4*>(q + j * step + c);
+          v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+        }
+        if constexpr (sizeof(TO) == 4)
+          *reinterpret_cast<float4*>(o + c) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+        else
+          *reinterpret_cast<uint2*>(o + c) = make_uint2(gemm::pack_bf16(v.x * f, v.y * f), gemm::pack_bf16(v.z * f, v.w * f));
+      }
+    } else {
+      for (int64_t c = threadIdx.x; c < a.cols; c += 256) {
+        float v = 0.f;
+#pragma unroll 4
+        for (int j = 0; j < splits; ++j) v += q[j * step + c];
+        st(o + c, v * f);
+      }
     }
-    if constexpr (sizeof(TO) == 4)
-      *reinterpret_cast<float4*>(o + c) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
-    else
-      *reinterpret_cast<uint2*>(o + c) = make_uint2(gemm::pack_bf16(v.x * f, v.y * f), gemm::pack_bf16(v.z * f, v.w * f));
-    return;
-  }
-  for (int64_t c = (int64_t)blockIdx.y * 1024 + threadIdx.x; c < c1; c += 256) {
-    float v = 0.f;
-#pragma unroll 8
-    for (int j = 0; j < splits; ++j) v += q[j * step + c];
-    st(o + c, v * f);
   }
 }
 
@@ -669,7 +693,7 @@ cudaError_t grad_gemm(const Operand& a, const Operand& b, int64_t k, int planes,
   if (!o.sum && g.max_splits == 1) return launch_gemm<CG>(grad_gemm_kernel<CG, A_MN, TO, OUT>, g, o, &allowed[0], st);
   const cudaError_t e = launch_gemm<CG>(grad_gemm_kernel<CG, A_MN, TO, PART>, g, o, &allowed[1], st);
   if (e != cudaSuccess || g.max_splits == 1) return e;
-  return launch_dependent(join_kernel<CG, TO>, dim3((unsigned)o.rows, (unsigned)cdiv(o.cols, 1024)), 256, 0, 1, st, g, o);
+  return launch_dependent(join_kernel<CG, TO>, dim3((unsigned)std::min<int64_t>(o.rows, SMS * 8)), 256, 0, 1, st, g, o);
 }
 
 template <bool A_MN, typename... Args>
@@ -694,6 +718,7 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
   sel.count = reinterpret_cast<int*>(ws + q.one);
   sel.alpha = reinterpret_cast<float*>(ws + q.one) + 1;
   sel.scales = reinterpret_cast<Scales*>(ws + q.one + 16);
+  sel.ticket = reinterpret_cast<int*>(ws + q.one + 32);
   sel.index = reinterpret_cast<int*>(ws + q.index);
   sel.target = reinterpret_cast<int*>(ws + q.target);
   float* rows = p->reduction == SSD_REDUCE_NONE ? p->loss : reinterpret_cast<float*>(ws + q.rows);
@@ -711,11 +736,10 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
   void* lo = const_cast<void*>(x.plane[1]);
   const unsigned wide = 148 * 8;
   if (!bf) {
-    err = launch_dependent(largest_kernel, std::min<unsigned>((unsigned)cdiv(p->tokens, 8), wide), 256, 0, 1, st, static_cast<const float*>(p->hidden), p->hidden_stride_row,
-        p->tokens, p->dim, p->targets, p->targets_int64, p->ignore_index, &sel.scales->x);
-    CE_CHECK(err, "largest");
-    err = launch_dependent(largest_kernel, std::min<unsigned>((unsigned)cdiv(p->vocab, 8), wide), 256, 0, 1, st, static_cast<const float*>(p->weight),
-        p->weight_stride_row, p->vocab, p->dim, nullptr, 0, 0, &sel.scales->w);
+    err = launch_dependent(largest_kernel, dim3((unsigned)std::min<int64_t>(cdiv(std::max(p->vocab, p->tokens), 8), wide), 2), 256, 0, 1,
+                           st, static_cast<const float*>(p->hidden), p->hidden_stride_row, p->tokens,
+                           static_cast<const float*>(p->weight), p->weight_stride_row, p->vocab, p->dim, p->targets,
+                           p->targets_int64, p->ignore_index, sel.scales);
     CE_CHECK(err, "largest");
   }
   if (bf)
@@ -741,6 +765,14 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
                                               w.ld, whi, wlo, &sel.scales->w);
     CE_CHECK(err, "weight planes");
   }
+  Reduced red{};
+  if (p->reduction != SSD_REDUCE_NONE) {
+    red.out = p->loss;
+    red.tokens = p->tokens;
+    red.mean = mean;
+    red.ticket = sel.ticket;
+    for (int64_t c = 0; c < q.nchunks; ++c) red.ctas += cdiv(std::min(q.chunk, p->tokens - c * q.chunk), 8);
+  }
   for (int64_t c = 0; c < q.nchunks; ++c) {
     const int64_t t0 = c * q.chunk, n = std::min(q.chunk, p->tokens - t0);
     const int from = (int)t0;
@@ -759,7 +791,7 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
     else CE_CHECK(logits_gemm<1>(xc, w, q.planes, a, sel.count, from, status, st), "logits");
     RowFactors* factors = q.grad ? reinterpret_cast<RowFactors*>(ws + q.factors) : nullptr;
     err = launch_dependent(loss_kernel, (unsigned)cdiv(n, 8), 256, 0, 1, st, a.stats, a.ns, a.picked, sel, from, (int)n, rows, p->lse,
-                                                     per_row ? p->grad_loss : nullptr, q.planes == 2, factors);
+                                                     per_row ? p->grad_loss : nullptr, q.planes == 2, factors, red);
     CE_CHECK(err, "loss");
     if (!q.grad) continue;
     RowArgs r{};
@@ -794,10 +826,6 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
       CE_CHECK(grad_gemm_as<true>(p->vocab > BM, p->grad_weight_dtype == SSD_DTYPE_BF16, dl, xc, n, q.planes, q.part_w, ow,
                                   sel.count, from, status, st), "grad_weight");
     }
-  }
-  if (p->reduction != SSD_REDUCE_NONE) {
-    err = launch_dependent(reduce_kernel, 1, 1024, 0, 1, st, rows, p->tokens, sel.count, mean, p->loss);
-    CE_CHECK(err, "reduce");
   }
   return cudaSuccess;
 }

@@ -28,7 +28,7 @@ using namespace ce;
 constexpr int SM_THREADS = 512, SM_WARPS = SM_THREADS / 32, SM_CTAS = 148;
 constexpr int WORDS = 4;                     // words of a warp at a time
 constexpr int MAX_ROWS = 8;                  // rows of one pass over the weight
-constexpr size_t MAX_SMEM = 200 * 1024;
+constexpr size_t MAX_SMEM = 222 * 1024;      // besides the static part
 constexpr int G_THREADS = 256, G_COLS = 4 * G_THREADS, G_TILE = 64;
 
 size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
@@ -66,29 +66,40 @@ __device__ __forceinline__ float value(const T* p, int64_t i) { return ld(p + i)
 template <typename T, int U>
 struct Piece {
   static constexpr int K = 16 / sizeof(T) / U, COLS = 32 * K * U;   // columns of a warp's piece
+  // asynchronous copies of 4 bytes were slower than loads (77 against 51 us for 6 x 56640 x 1106)
+  static constexpr bool ASYNC = U == 1;
   uint32_t u[4];
+
+  // Into the lane's own 16 bytes of shared memory, asynchronously.  Columns past the end are
+  // read at the last ones and cleared by cut().
+  static __device__ __forceinline__ void copy(void* slot, const T* row, int c0, int dim) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t to = ptx::smem_u32(slot);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(row + min(c0 + lane * K, dim - K)) : "memory");
+  }
+  __device__ __forceinline__ void take(const void* slot) {
+    const uint4 q = *static_cast<const uint4*>(slot);
+    u[0] = q.x; u[1] = q.y; u[2] = q.z; u[3] = q.w;
+  }
+  // The same straight into registers, for U = 4 and 8.
   __device__ __forceinline__ void load(const T* row, int c0, int dim) {
     const int lane = threadIdx.x & 31;
-    if constexpr (U == 1) {
-      const int c = c0 + lane * K;
-      uint4 q = make_uint4(0, 0, 0, 0);
-      if (c < dim) q = *reinterpret_cast<const uint4*>(row + c);
-      u[0] = q.x; u[1] = q.y; u[2] = q.z; u[3] = q.w;
-    } else if constexpr (U == 4) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int c = c0 + (i * 32 + lane) * K;
-        u[i] = c < dim ? *reinterpret_cast<const uint32_t*>(row + c) : 0u;
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (U == 4) {
+        u[i] = *reinterpret_cast<const uint32_t*>(row + min(c0 + (i * 32 + lane) * K, dim - K));
+        continue;
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int c = c0 + 2 * i * 32 + lane;
-        const uint32_t a = c < dim ? *reinterpret_cast<const uint16_t*>(row + c) : 0u;
-        const uint32_t b = c + 32 < dim ? *reinterpret_cast<const uint16_t*>(row + c + 32) : 0u;
-        u[i] = a | b << 16;
-      }
+      const int c = c0 + 2 * i * 32 + lane;
+      u[i] = *reinterpret_cast<const uint16_t*>(row + min(c, dim - 1)) |
+             (uint32_t)*reinterpret_cast<const uint16_t*>(row + min(c + 32, dim - 1)) << 16;
     }
+  }
+  __device__ __forceinline__ void cut(int c0, int dim) {
+    constexpr int V = 16 / sizeof(T), W = 4 / sizeof(T);   // values of a piece, of a 32-bit word
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (c0 + col(i) >= dim) u[i / W] &= W == 1 ? 0u : i & 1 ? 0xffffu : 0xffff0000u;
   }
   // value i of the 16 / sizeof(T), and its column (from c0)
   __device__ __forceinline__ float at(int i) const {
@@ -118,20 +129,40 @@ __device__ __forceinline__ float warp_sums(float (&v)[N]) {
   return s;
 }
 
-// blockIdx.y: rows 8 y ..; R of them are computed (those past the last token on zeros).  The
-// pieces of the weight are loaded two steps ahead, across the ends of the words, so that a
-// warp's reductions do not leave the memory idle.
-template <typename T, int R, int U>
+// blockIdx.y: rows 8 y ..; R of them are computed (those past the last token on zeros).  A lane
+// copies its pieces of the weight STAGES - 1 steps ahead, across the ends of the words, into
+// slots of its own: 96 KB in flight per SM, which registers could not hold.
+template <typename T, int R, int U, int STAGES>
 __global__ void __launch_bounds__(SM_THREADS, 1) small_logits_kernel(const __grid_constant__ SmallArgs a) {
   using P = Piece<T, U>;
   constexpr int V = 16 / sizeof(T);
-  extern __shared__ float xs[];   // (R, dim rounded up to whole pieces)
+  extern __shared__ __align__(16) uint8_t smem[];   // ring, then hidden (R, dim rounded up to whole pieces)
   __shared__ float2 red[SM_WARPS][R * WORDS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint4* ring = reinterpret_cast<uint4*>(smem) + warp * (STAGES * WORDS * 32) + lane;   // [stage][word][lane]
+  float* xs = reinterpret_cast<float*>(smem + SM_WARPS * STAGES * WORDS * 512);
   const int row0 = blockIdx.y * MAX_ROWS, rows = min(R, a.tokens - row0);
   const int steps = (a.dim + P::COLS - 1) / P::COLS, pitch = steps * P::COLS;
   const T* x = static_cast<const T*>(a.x) + row0 * a.xs;
   if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) *a.status = 0;
+  const int stride = SM_CTAS * SM_WARPS * WORDS, v_first = (blockIdx.x * SM_WARPS + warp) * WORDS;
+  int next_v = v_first, next_s = 0, next_slot = 0;
+  auto fetch = [&]() {   // the next piece of the next words, in the order of their use
+    if (next_v < a.vocab) {
+#pragma unroll
+      for (int j = 0; j < WORDS; ++j)
+        P::copy(ring + (next_slot * WORDS + j) * 32, static_cast<const T*>(a.w) + (int64_t)min(next_v + j, a.vocab - 1) * a.ws,
+                next_s * P::COLS, a.dim);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    next_slot = next_slot + 1 == STAGES ? 0 : next_slot + 1;
+    if (++next_s == steps) {
+      next_s = 0;
+      next_v += stride;
+    }
+  };
+  if constexpr (P::ASYNC)
+    for (int i = 0; i < STAGES - 1; ++i) fetch();
   for (int i = tid; i < R * pitch; i += SM_THREADS) {
     const int r = i / pitch, c = i - r * pitch;
     xs[i] = r < rows && c < a.dim ? value(x + r * a.xs, c) : 0.f;
@@ -140,30 +171,30 @@ __global__ void __launch_bounds__(SM_THREADS, 1) small_logits_kernel(const __gri
   const int my_row = (lane / WORDS) % R, my_word = lane % WORDS;
   const int64_t y = my_row < rows ? target_at(a.targets, a.is64, row0 + my_row) : -1;
   __syncthreads();
-  const int stride = SM_CTAS * SM_WARPS * WORDS;
-  int next_v = (blockIdx.x * SM_WARPS + warp) * WORDS, next_s = 0;
-  auto fetch = [&](P (&q)[WORDS]) {   // the next piece of the next words, in the order of their use
-    if (next_v < a.vocab) {
-#pragma unroll
-      for (int j = 0; j < WORDS; ++j)
-        q[j].load(static_cast<const T*>(a.w) + (int64_t)min(next_v + j, a.vocab - 1) * a.ws, next_s * P::COLS, a.dim);
-    }
-    if (++next_s == steps) {
-      next_s = 0;
-      next_v += stride;
-    }
-  };
   float top = -INFINITY, sum = 0.f;
-  P q0[WORDS], q1[WORDS], q2[WORDS];
-  fetch(q0);
-  fetch(q1);
-  for (int v0 = (blockIdx.x * SM_WARPS + warp) * WORDS; v0 < a.vocab; v0 += stride) {
+  int slot = 0;
+  for (int v0 = v_first; v0 < a.vocab; v0 += stride) {
     float acc[WORDS * R];
 #pragma unroll
     for (int i = 0; i < WORDS * R; ++i) acc[i] = 0.f;
-#pragma unroll 1
+#pragma unroll (P::ASYNC ? 1 : 2)
     for (int s = 0; s < steps; ++s) {
-      fetch(q2);
+      P q[WORDS];
+      if constexpr (P::ASYNC) {
+        fetch();   // into the slot that the last step emptied
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+#pragma unroll
+        for (int j = 0; j < WORDS; ++j) q[j].take(ring + (slot * WORDS + j) * 32);
+        slot = slot + 1 == STAGES ? 0 : slot + 1;
+      } else {
+#pragma unroll
+        for (int j = 0; j < WORDS; ++j)
+          q[j].load(static_cast<const T*>(a.w) + (int64_t)min(v0 + j, a.vocab - 1) * a.ws, s * P::COLS, a.dim);
+      }
+      if (s == steps - 1 && pitch > a.dim) {
+#pragma unroll
+        for (int j = 0; j < WORDS; ++j) q[j].cut(s * P::COLS, a.dim);
+      }
       const float* xc = xs + s * P::COLS;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -178,13 +209,8 @@ __global__ void __launch_bounds__(SM_THREADS, 1) small_logits_kernel(const __gri
 #pragma unroll
           for (int k = 0; k < G; ++k)
 #pragma unroll
-            for (int j = 0; j < WORDS; ++j) acc[r * WORDS + j] = fmaf(q0[j].at(i + k), xv[k], acc[r * WORDS + j]);
+            for (int j = 0; j < WORDS; ++j) acc[r * WORDS + j] = fmaf(q[j].at(i + k), xv[k], acc[r * WORDS + j]);
         }
-      }
-#pragma unroll
-      for (int j = 0; j < WORDS; ++j) {
-        q0[j] = q1[j];
-        q1[j] = q2[j];
       }
     }
     const float s = warp_sums(acc);
@@ -371,13 +397,22 @@ size_t logits_smem(const ssd_linear_ce_params_t* p) {
   return (size_t)row_width(p->tokens) * ((p->dim + 255) / 256 * 256) * 4;
 }
 
-template <typename T, int R, int U>
+size_t ring_bytes(int stages) { return (size_t)SM_WARPS * stages * WORDS * 512; }
+
+template <typename T, int R, int U, int STAGES>
 cudaError_t run_logits(const SmallArgs& a, size_t smem, cudaStream_t st) {
   static std::atomic<uint64_t> allowed{0};
-  const cudaError_t e = allow_smem((const void*)small_logits_kernel<T, R, U>, MAX_SMEM, &allowed);
+  const auto kernel = small_logits_kernel<T, R, U, STAGES>;
+  const cudaError_t e = allow_smem((const void*)kernel, MAX_SMEM, &allowed);
   if (e != cudaSuccess) return e;
-  small_logits_kernel<T, R, U><<<dim3(SM_CTAS, (unsigned)cdiv(a.tokens, MAX_ROWS)), SM_THREADS, smem, st>>>(a);
+  kernel<<<dim3(SM_CTAS, (unsigned)cdiv(a.tokens, MAX_ROWS)), SM_THREADS, smem + ring_bytes(STAGES), st>>>(a);
   return cudaGetLastError();
+}
+template <typename T, int R, int U>
+cudaError_t run_logits(const SmallArgs& a, size_t smem, cudaStream_t st) {
+  // four stages where hidden leaves the room, else two
+  if (smem + ring_bytes(4) <= MAX_SMEM) return run_logits<T, R, U, 4>(a, smem, st);
+  return run_logits<T, R, U, 2>(a, smem, st);
 }
 template <typename T, int U>
 cudaError_t run_logits(const SmallArgs& a, size_t smem, cudaStream_t st) {
@@ -456,7 +491,7 @@ SmallPlan plan_of(const ssd_linear_ce_params_t* p) {
 bool linear_ce_is_small(const ssd_linear_ce_params_t* p) {
   const bool grad = p->grad_hidden || p->grad_weight;
   const int64_t most = grad ? MAX_ROWS : p->dtype == SSD_DTYPE_F32 ? 4 * MAX_ROWS : MAX_ROWS;
-  return p->tokens <= most && logits_smem(p) <= MAX_SMEM && p->vocab < (1 << 30);
+  return p->tokens <= most && logits_smem(p) + ring_bytes(2) <= MAX_SMEM && p->vocab < (1 << 30);
 }
 
 size_t linear_ce_small_workspace(const ssd_linear_ce_params_t* p) { return plan_of(p).total; }
