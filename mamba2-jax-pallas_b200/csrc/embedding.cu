@@ -13,14 +13,14 @@
 // floats.  Launches:
 //   1. one cluster of 8 CTAs sorts (id, position) pairs by a stable radix sort whose histograms
 //      live in distributed shared memory;
-//   2. meanwhile (a programmatic dependent launch that does not wait) the other SMs write the
-//      zero rows of the ids that do not occur, most of a dense gradient: a CTA marks the ids of
-//      its own rows in a shared bitmap;
-//   3. the sorted order is cut into pieces of equal length, whatever the ids, so that one
-//      frequent id cannot hold up a CTA.  A warp sums a piece's rows over 256 columns in f32 and
-//      writes each id's row.  An id that goes on for at most `extend` rows into the next piece is
-//      finished by the piece it began in; a longer one leaves its parts in the workspace;
-//   4. the parts of such ids are added up, again in order.
+//   2. a programmatic dependent launch that begins at once.  Its first CTAs write the zero rows of
+//      the ids that do not occur, most of a dense gradient: a CTA marks the ids of its own rows
+//      in a shared bitmap.  The others wait for the sort; they cut the sorted order into pieces
+//      of equal length, whatever the ids, so that one frequent id cannot hold up a CTA.  A warp
+//      sums a piece's rows over 256 columns in f32 and writes each id's row.  An id that goes on
+//      for at most `extend` rows into the next piece is finished by the piece it began in; a
+//      longer one leaves its parts in the workspace;
+//   3. the parts of such ids are added up, again in order.
 #include <algorithm>
 
 #include <cooperative_groups.h>
@@ -174,25 +174,25 @@ cudaError_t lookup(const LookupArgs& a, bool vec, cudaStream_t stream) {
 }
 
 // ---------------------------------------------------------------------------
-// gradient, launches 1 and 2: sort, zero rows
+// gradient: sort
 // ---------------------------------------------------------------------------
 constexpr int SORT_CTAS = 8;      // the sorting cluster
 constexpr int SORT_THREADS = 1024;
 constexpr int SORT_WARPS = SORT_THREADS / 32;
+constexpr int SORT_AHEAD = 4;
 constexpr int SORT_BITS = 9;
 constexpr int SORT_BINS = 1 << SORT_BITS;
 constexpr int ZERO_ROWS = 8192;   // rows whose bits the bitmap holds at a time
 
 struct GradArgs {
   int64_t n, vocab, dim, gs, os, pad, piece, npieces;
-  int is64, passes, accumulate;
+  int is64, passes, accumulate, zero_ctas;
   int extend;                     // rows that a piece may take from the next one, at most a piece and 32
   float scale;
   const void* ids;
   const void* g;
   void* out;
-  uint32_t* key[2];               // sorted ids (V = dropped, last); result in key[0], pos[0]
-  uint32_t* pos[2];
+  uint2* list[2];                 // (id, position), sorted by id (V = dropped, last); result in list[0]
   float* part;                    // (npieces, 2, dim)
   int* heavy;                     // count, then the pieces in which an id with parts begins
 };
@@ -203,12 +203,12 @@ struct SortShared {
   uint32_t scan[SORT_WARPS];
 };
 
-// One stable pass of the radix sort over the cluster.  CTA c and its warp w own consecutive
-// tokens; a warp takes 32 of them at a time and lanes with equal digits find each other by
-// match_any, so equal digits keep their order.
+// One stable pass of the radix sort over the cluster.  What bounds it are the scattered stores, a
+// line for every lane: id and position go in one 8-byte store (32768 ids: 34 -> 28 us).  CTA c and its warp w own consecutive
+// tokens; a warp takes 32 of them at a time and lanes with equal digits find each other, so
+// equal digits keep their order.
 template <bool FIRST>
-__device__ void sort_pass(const GradArgs& a, SortShared* s, int shift, const uint32_t* ki, const uint32_t* pi,
-                          uint32_t* ko, uint32_t* po) {
+__device__ void sort_pass(const GradArgs& a, SortShared* s, int shift, const uint2* from, uint2* to) {
   cg::cluster_group cluster = cg::this_cluster();
   const int cta = (int)cluster.block_rank(), tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
   for (int i = tid; i < SORT_WARPS * SORT_BINS; i += SORT_THREADS) (&s->warp_bin[0][0])[i] = 0;
@@ -220,19 +220,25 @@ __device__ void sort_pass(const GradArgs& a, SortShared* s, int shift, const uin
       const int64_t v = row_of(a.ids, a.is64, t, a.vocab, a.pad);
       return v < 0 ? (uint32_t)a.vocab : (uint32_t)v;
     } else {
-      return ki[t];
+      return from[t].x;
     }
   };
-  for (int64_t t0 = lo; t0 < hi; t0 += 32) {
-    const int64_t t = t0 + lane;
-    const bool in = t < hi;
-    const unsigned live = __ballot_sync(0xffffffffu, in);
-    if (in) {
-      const uint32_t d = (key_at(t) >> shift) & (SORT_BINS - 1);
-      const unsigned same = __match_any_sync(live, d);
-      if (lane == __ffs(same) - 1) s->warp_bin[w][d] += __popc(same);
+  // SORT_AHEAD groups of 32 tokens are loaded at a time
+  for (int64_t t0 = lo; t0 < hi; t0 += 32 * SORT_AHEAD) {
+    uint32_t k[SORT_AHEAD];
+#pragma unroll
+    for (int j = 0; j < SORT_AHEAD; ++j) k[j] = key_at(min(t0 + 32 * j + lane, hi - 1));
+#pragma unroll
+    for (int j = 0; j < SORT_AHEAD; ++j) {
+      const bool in = t0 + 32 * j + lane < hi;
+      const unsigned live = __ballot_sync(0xffffffffu, in);
+      if (in) {
+        const uint32_t d = (k[j] >> shift) & (SORT_BINS - 1);
+        const unsigned same = __match_any_sync(live, d);
+        if (lane == __ffs(same) - 1) s->warp_bin[w][d] += __popc(same);
+      }
+      __syncwarp();
     }
-    __syncwarp();
   }
   __syncthreads();
   // counts of each digit: exclusive over this CTA's warps, total over the CTA
@@ -269,20 +275,28 @@ __device__ void sort_pass(const GradArgs& a, SortShared* s, int shift, const uin
     for (int i = 0; i < SORT_WARPS; ++i) s->warp_bin[i][tid] += base;
   }
   __syncthreads();
-  for (int64_t t0 = lo; t0 < hi; t0 += 32) {
-    const int64_t t = t0 + lane;
-    const bool in = t < hi;
-    const unsigned live = __ballot_sync(0xffffffffu, in);
-    if (in) {
-      const uint32_t k = key_at(t), d = (k >> shift) & (SORT_BINS - 1);
-      const unsigned same = __match_any_sync(live, d);
-      const uint32_t slot = s->warp_bin[w][d] + __popc(same & ((1u << lane) - 1));
-      __syncwarp(live);
-      if (lane == __ffs(same) - 1) s->warp_bin[w][d] += __popc(same);
-      ko[slot] = k;
-      po[slot] = FIRST ? (uint32_t)t : pi[t];
+  for (int64_t t0 = lo; t0 < hi; t0 += 32 * SORT_AHEAD) {
+    uint2 e[SORT_AHEAD];
+#pragma unroll
+    for (int j = 0; j < SORT_AHEAD; ++j) {
+      const int64_t t = min(t0 + 32 * j + lane, hi - 1);
+      if constexpr (FIRST) e[j] = make_uint2(key_at(t), (uint32_t)t);
+      else e[j] = from[t];
     }
-    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < SORT_AHEAD; ++j) {
+      const bool in = t0 + 32 * j + lane < hi;
+      const unsigned live = __ballot_sync(0xffffffffu, in);
+      if (in) {
+        const uint32_t d = (e[j].x >> shift) & (SORT_BINS - 1);
+        const unsigned same = __match_any_sync(live, d);
+        const uint32_t slot = s->warp_bin[w][d] + __popc(same & ((1u << lane) - 1));
+        __syncwarp(live);
+        if (lane == __ffs(same) - 1) s->warp_bin[w][d] += __popc(same);
+        to[slot] = e[j];
+      }
+      __syncwarp();
+    }
   }
   cluster.sync();   // the cluster's keys are in place; every CTA has read the others' counts
 }
@@ -292,53 +306,17 @@ __global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_THREADS
   ptx::griddep_launch_dependents();   // the zero rows need nothing from here
   SortShared* s = reinterpret_cast<SortShared*>(smem);
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.heavy = 0;
-  // the passes end in key[0] / pos[0]
+  // the passes end in list[0]
   int to = (a.passes - 1) & 1;
-  sort_pass<true>(a, s, 0, nullptr, nullptr, a.key[to], a.pos[to]);
+  sort_pass<true>(a, s, 0, nullptr, a.list[to]);
   for (int p = 1; p < a.passes; ++p) {
-    sort_pass<false>(a, s, p * SORT_BITS, a.key[to], a.pos[to], a.key[to ^ 1], a.pos[to ^ 1]);
+    sort_pass<false>(a, s, p * SORT_BITS, a.list[to], a.list[to ^ 1]);
     to ^= 1;
   }
 }
 
-// Zero rows of the ids that do not occur.  A CTA owns rows [r0, r1) and marks those that
-// occur in a shared bitmap, ZERO_ROWS at a time, reading all ids (L2) once for each.
-template <typename TO>
-__global__ void __launch_bounds__(SORT_THREADS, 1) zero_rows_kernel(const GradArgs a) {
-  __shared__ uint32_t bits[ZERO_ROWS / 32];
-  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
-  const int64_t per = (a.vocab + gridDim.x - 1) / gridDim.x;
-  const int64_t r0 = blockIdx.x * per, r1 = min(r0 + per, a.vocab);
-  const bool vec = (reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.os * sizeof(TO))) % 16 == 0;
-  for (int64_t b0 = r0; b0 < r1; b0 += ZERO_ROWS) {
-    const int64_t b1 = min(b0 + ZERO_ROWS, r1);
-    for (int i = tid; i < ZERO_ROWS / 32; i += SORT_THREADS) bits[i] = 0;
-    __syncthreads();
-#pragma unroll 8
-    for (int64_t t = tid; t < a.n; t += SORT_THREADS) {
-      const int64_t v = row_of(a.ids, a.is64, t, a.vocab, a.pad);
-      if (v >= b0 && v < b1) atomicOr(&bits[(v - b0) >> 5], 1u << ((v - b0) & 31));
-    }
-    __syncthreads();
-    for (int64_t r = b0 + w; r < b1; r += SORT_WARPS) {
-      if ((bits[(r - b0) >> 5] >> ((r - b0) & 31)) & 1) continue;
-      TO* o = static_cast<TO*>(a.out) + r * a.os;
-      int64_t c = 0;
-      if (vec) {
-        constexpr int PER = 16 / sizeof(TO);
-        for (c = lane * PER; c + PER <= a.dim; c += 32 * PER) *reinterpret_cast<uint4*>(o + c) = make_uint4(0, 0, 0, 0);
-        c = a.dim / PER * PER;
-      }
-      for (c += lane; c < a.dim; c += 32) st(o + c, 0.f);
-    }
-    __syncthreads();
-  }
-  // what is launched behind this kernel may take the sort as done, too
-  ptx::griddep_wait();
-}
-
 // ---------------------------------------------------------------------------
-// gradient, launches 3 and 4: sums
+// gradient: zero rows and sums
 // ---------------------------------------------------------------------------
 constexpr int SUM_THREADS = 256;
 constexpr int SUM_COLS = 32 * VEC;   // columns of a warp
@@ -403,27 +381,73 @@ __device__ __forceinline__ void put_row(const GradArgs& a, uint32_t id, int64_t 
   store_cols<TO, M>(o, a.dim - c0, acc);
 }
 
-// Warp (piece p, 256 columns): rows of the sorted positions [p * piece, + piece).
+// Zero rows of the ids that do not occur.  A CTA owns rows [r0, r1) and marks those that
+// occur in a shared bitmap, ZERO_ROWS at a time, reading all ids (L2) once for each.
+template <typename TO>
+__device__ void zero_rows(const GradArgs& a, uint32_t* bits) {
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
+  const int64_t per = (a.vocab + a.zero_ctas - 1) / a.zero_ctas;
+  const int64_t r0 = blockIdx.x * per, r1 = min(r0 + per, a.vocab);
+  const bool vec = (reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.os * sizeof(TO))) % 16 == 0;
+  // two 64-bit ids at a time where they lie so
+  const int64_t pairs = a.is64 && reinterpret_cast<uintptr_t>(a.ids) % 16 == 0 ? a.n / 2 : 0;
+  for (int64_t b0 = r0; b0 < r1; b0 += ZERO_ROWS) {
+    const int64_t b1 = min(b0 + ZERO_ROWS, r1);
+    for (int i = tid; i < ZERO_ROWS / 32; i += SUM_THREADS) bits[i] = 0;
+    __syncthreads();
+    auto mark = [&](int64_t v) {
+      if (v >= b0 && v < b1 && v != a.pad) atomicOr(&bits[(v - b0) >> 5], 1u << ((v - b0) & 31));
+    };
+#pragma unroll 8
+    for (int64_t t = tid; t < pairs; t += SUM_THREADS) {
+      const longlong2 q = __ldg(static_cast<const longlong2*>(a.ids) + t);
+      mark(q.x);
+      mark(q.y);
+    }
+#pragma unroll 8
+    for (int64_t t = 2 * pairs + tid; t < a.n; t += SUM_THREADS) mark(row_of(a.ids, a.is64, t, a.vocab, a.pad));
+    __syncthreads();
+    for (int64_t r = b0 + w; r < b1; r += SUM_THREADS / 32) {
+      if ((bits[(r - b0) >> 5] >> ((r - b0) & 31)) & 1) continue;
+      TO* o = static_cast<TO*>(a.out) + r * a.os;
+      int64_t c = 0;
+      if (vec) {
+        constexpr int PER = 16 / sizeof(TO);
+        for (c = lane * PER; c + PER <= a.dim; c += 32 * PER) *reinterpret_cast<uint4*>(o + c) = make_uint4(0, 0, 0, 0);
+        c = a.dim / PER * PER;
+      }
+      for (c += lane; c < a.dim; c += 32) st(o + c, 0.f);
+    }
+    __syncthreads();
+  }
+}
+
+// The first a.zero_ctas CTAs: zero rows.  Then a warp for each (piece p, 256 columns): rows of the
+// sorted positions [p * piece, + piece).
 template <typename TG, typename TO, Cols M>
-__global__ void __launch_bounds__(SUM_THREADS, 4) grad_sum_kernel(const __grid_constant__ GradArgs a, int col_warps) {
+__global__ void __launch_bounds__(SUM_THREADS, 4) grad_rows_kernel(const __grid_constant__ GradArgs a, int col_warps) {
+  __shared__ uint32_t bits[ZERO_ROWS / 32];
+  if (blockIdx.x < a.zero_ctas) {
+    zero_rows<TO>(a, bits);
+    ptx::griddep_wait();   // what is launched behind may take the sort as done, too
+    return;
+  }
   using R = Raw<TG, M>;
   ptx::griddep_wait();
-  const int unit = blockIdx.x * (SUM_THREADS / 32) + threadIdx.x / 32;
+  const int unit = (blockIdx.x - a.zero_ctas) * (SUM_THREADS / 32) + threadIdx.x / 32;
   const int p = unit / col_warps;
   if (p >= (int)a.npieces) return;
   const int lane = threadIdx.x & 31, n = (int)a.n, top = n - 1, piece = (int)a.piece, extend = a.extend;
   const int c0 = (unit - p * col_warps) * SUM_COLS, left = (int)a.dim - c0;
   const int lo = p * piece, hi = min(lo + piece, n);
   const uint32_t none = (uint32_t)a.vocab;
-  const uint32_t* key = a.key[0];
-  const uint32_t* pos = a.pos[0];
+  const uint2* list = a.list[0];
   // every key that decides about the piece's ends, in one round trip
-  const uint32_t first = key[lo], last = key[hi - 1];
-  const uint32_t k_prev = key[max(lo - 1, 0)], k_before = key[max(lo - piece - 1, 0)];
-  const uint32_t k_far = key[min(lo + extend, top)], k_next = key[min(hi, top)], k_next_far = key[min(hi + extend, top)];
-  const uint32_t k_ext = key[min(hi + lane, top)];
-  uint32_t mk = key[min(lo + lane, top)];
-  int mp = (int)pos[min(lo + lane, top)];
+  const uint32_t first = list[lo].x, last = list[hi - 1].x;
+  const uint32_t k_prev = list[max(lo - 1, 0)].x, k_before = list[max(lo - piece - 1, 0)].x;
+  const uint32_t k_far = list[min(lo + extend, top)].x, k_next = list[min(hi, top)].x, k_next_far = list[min(hi + extend, top)].x;
+  const uint32_t k_ext = list[min(hi + lane, top)].x;
+  uint2 mine = list[min(lo + lane, top)];
   if (first == none) return;
   // the first id: it may have begun in an earlier piece, and then either the piece before
   // finishes it (skip) or this piece's share of it is a part (open)
@@ -453,10 +477,9 @@ __global__ void __launch_bounds__(SUM_THREADS, 4) grad_sum_kernel(const __grid_c
     for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
   };
   for (int i0 = lo; i0 < end; i0 += 32) {
-    if (i0 > lo) {
-      mk = key[min(i0 + lane, top)];
-      mp = (int)pos[min(i0 + lane, top)];
-    }
+    if (i0 > lo) mine = list[min(i0 + lane, top)];
+    const uint32_t mk = mine.x;
+    const int mp = (int)mine.y;
     const int m = min(32, end - i0);
     // rows that add something, and rows at which another id begins
     const unsigned live = __ballot_sync(0xffffffffu, lane < m && mk != none);
@@ -489,73 +512,77 @@ __global__ void __launch_bounds__(SUM_THREADS, 4) grad_sum_kernel(const __grid_c
   }
 }
 
-// CTA (256 columns, every gridDim.y-th listed piece p): the id that begins in piece p, the sum
-// of its parts.  The parts of the following pieces are shared out over the CTA's warps in
-// runs, each summed in order, and the runs are added in order; which CTA does it, and when,
-// changes nothing.
-template <typename TO, Cols M>
-__global__ void __launch_bounds__(SUM_THREADS) grad_join_kernel(const GradArgs a) {
-  __shared__ float sums[SUM_THREADS / 32][SUM_COLS];
+// CTA (64 columns, every gridDim.y-th listed piece p): the id that begins in piece p, the sum of
+// its parts.  The parts of the following pieces are shared out over the CTA's warps in runs,
+// each summed in order, and the runs are added in order; which CTA does it, and when, changes
+// nothing.
+constexpr int JOIN_COLS = 64;
+template <typename TO>
+__global__ void __launch_bounds__(SUM_THREADS) grad_join_kernel(const __grid_constant__ GradArgs a) {
+  constexpr int W = SUM_THREADS / 32;
+  __shared__ float2 sums[W][32];
+  __shared__ int pieces;
   ptx::griddep_wait();
-  const uint32_t* key = a.key[0];
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, listed = *a.heavy;
+  const uint2* list = a.list[0];
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, listed = *a.heavy, npieces = (int)a.npieces;
+  const int64_t c = (int64_t)blockIdx.x * JOIN_COLS + 2 * lane;
+  const bool one = c < a.dim, two = c + 1 < a.dim;
   for (int h = blockIdx.y; h < listed; h += gridDim.y) {
-    const int64_t p = a.heavy[1 + h];
-    const uint32_t id = key[(p + 1) * a.piece - 1];
-    // last piece that holds the id: pieces p+1, p+2, ... whose first key is the id
-    int64_t last = p + 1;
-    while (true) {
-      const int64_t q = last + 1 + lane;
-      const unsigned b = __ballot_sync(0xffffffffu, q < a.npieces && key[min(q, a.npieces - 1) * a.piece] == id);
-      const int more = b == 0xffffffffu ? 32 : __ffs(~b) - 1;
-      last += more;
-      if (more < 32) break;
-    }
-    const int64_t count = last - p, per = (count + SUM_THREADS / 32 - 1) / (SUM_THREADS / 32);
-    const int64_t q0 = p + 1 + w * per, q1 = min(q0 + per, last + 1);
-    const int64_t c0 = (int64_t)blockIdx.x * SUM_COLS;
-    const float* part = a.part + c0;
-    float acc[VEC];
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
-    if (w == 0) load_cols<float, M>(part + (p * 2 + 1) * a.dim, a.dim - c0, acc);
-#pragma unroll 4
-    for (int64_t q = q0; q < q1; ++q) {
-      float v[VEC];
-      load_cols<float, M>(part + (q * 2) * a.dim, a.dim - c0, v);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) acc[k] += v[k];
-    }
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) sums[w][k * 32 + lane] = acc[k];
+    const int p = a.heavy[1 + h];
+    const uint32_t id = list[(int64_t)(p + 1) * a.piece - 1].x;
+    if (threadIdx.x == 0) pieces = 0;
     __syncthreads();
+    // pieces p+1, p+2, ... whose first key is the id: they follow one another
+    int mine = 0;
+#pragma unroll 8
+    for (int q = p + 1 + threadIdx.x; q < npieces; q += SUM_THREADS) mine += list[(int64_t)q * a.piece].x == id;
+    if (mine) atomicAdd(&pieces, mine);
+    __syncthreads();
+    const int count = pieces, per = (count + W - 1) / W;
+    const int q0 = p + 1 + w * per, q1 = min(q0 + per, p + 1 + count);
+    float2 acc = make_float2(0.f, 0.f);
     if (w == 0) {
-      for (int i = 1; i < SUM_THREADS / 32; ++i) {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[k] += sums[i][k * 32 + lane];
+      const float* row = a.part + (int64_t)(p * 2 + 1) * a.dim + c;
+      if (one) acc.x = row[0];
+      if (two) acc.y = row[1];
+    }
+#pragma unroll 8
+    for (int q = q0; q < q1; ++q) {
+      const float* row = a.part + (int64_t)q * 2 * a.dim + c;
+      acc.x += one ? row[0] : 0.f;
+      acc.y += two ? row[1] : 0.f;
+    }
+    sums[w][lane] = acc;
+    __syncthreads();
+    if (w == 0 && one) {
+      for (int i = 1; i < W; ++i) {
+        acc.x += sums[i][lane].x;
+        acc.y += sums[i][lane].y;
       }
-      put_row<TO, M>(a, id, c0, acc);
+      TO* o = static_cast<TO*>(a.out) + (int64_t)id * a.os + c;
+      st(o, acc.x * a.scale + (a.accumulate ? ld(o) : 0.f));
+      if (two) st(o + 1, acc.y * a.scale + (a.accumulate ? ld(o + 1) : 0.f));
     }
     __syncthreads();
   }
 }
 
 template <typename TG, typename TO, Cols M>
-cudaError_t grad_sums(const GradArgs& a, cudaStream_t stream) {
+cudaError_t grad_rows(const GradArgs& a, cudaStream_t stream) {
   const int64_t col_warps = (a.dim + SUM_COLS - 1) / SUM_COLS;
   constexpr int W = SUM_THREADS / 32;
-  cudaError_t e = launch_dependent(grad_sum_kernel<TG, TO, M>, dim3((unsigned)((a.npieces * col_warps + W - 1) / W)),
-                                   SUM_THREADS, 0, 1, stream, a, (int)col_warps);
+  cudaError_t e = launch_dependent(grad_rows_kernel<TG, TO, M>,
+                                   dim3((unsigned)(a.zero_ctas + (a.npieces * col_warps + W - 1) / W)), SUM_THREADS, 0, 1, stream, a, (int)col_warps);
   if (e == cudaSuccess && a.n > a.piece + a.extend)   // shorter lists have no id with parts
-    e = launch_dependent(grad_join_kernel<TO, M>, dim3((unsigned)col_warps, (unsigned)std::min<int64_t>(a.npieces, 32)),
-                         SUM_THREADS, 0, 1, stream, a);
+    e = launch_dependent(grad_join_kernel<TO>,
+                         dim3((unsigned)((a.dim + JOIN_COLS - 1) / JOIN_COLS), (unsigned)std::min<int64_t>(a.npieces, 64)), SUM_THREADS, 0, 1, stream, a);
   return e;
 }
 
 template <typename TG, typename TO>
-cudaError_t grad_sums(const GradArgs& a, bool vec, cudaStream_t stream) {
+cudaError_t grad_rows(const GradArgs& a, bool vec, cudaStream_t stream) {
   constexpr Cols M = sizeof(TG) == 2 && sizeof(TO) == 2 ? EIGHT : FOURS;
-  return vec ? grad_sums<TG, TO, M>(a, stream) : grad_sums<TG, TO, ONES>(a, stream);
+  return vec ? grad_rows<TG, TO, M>(a, stream) : grad_rows<TG, TO, ONES>(a, stream);
 }
 
 int64_t piece_len(int64_t n, int64_t dim) {
@@ -587,7 +614,7 @@ cudaError_t launch_embedding(const ssd_embedding_params_t* p, cudaStream_t strea
 
 size_t embedding_grad_workspace(int64_t n, int64_t dim) {
   const int64_t len = piece_len(n, dim), pieces = (n + len - 1) / len;
-  return 4 * up256((size_t)n * 4) + up256((size_t)(pieces + 1) * 4) + (size_t)pieces * 2 * dim * 4;
+  return 2 * up256((size_t)n * 8) + up256((size_t)(pieces + 1) * 4) + (size_t)pieces * 2 * dim * 4;
 }
 
 // (positions, pieces and columns are ints in the kernels: checked by the caller)
@@ -601,13 +628,10 @@ cudaError_t launch_embedding_grad(const ssd_embedding_grad_params_t* p, void* wo
   a.extend = (int)std::min<int64_t>(a.piece, 32);
   a.npieces = (a.n + a.piece - 1) / a.piece;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  const size_t list = up256((size_t)a.n * 4);
-  for (int i = 0; i < 2; ++i) {
-    a.key[i] = reinterpret_cast<uint32_t*>(ws + (2 * i) * list);
-    a.pos[i] = reinterpret_cast<uint32_t*>(ws + (2 * i + 1) * list);
-  }
-  a.heavy = reinterpret_cast<int*>(ws + 4 * list);
-  a.part = reinterpret_cast<float*>(ws + 4 * list + up256((size_t)(a.npieces + 1) * 4));
+  const size_t list = up256((size_t)a.n * 8);
+  for (int i = 0; i < 2; ++i) a.list[i] = reinterpret_cast<uint2*>(ws + i * list);
+  a.heavy = reinterpret_cast<int*>(ws + 2 * list);
+  a.part = reinterpret_cast<float*>(ws + 2 * list + up256((size_t)(a.npieces + 1) * 4));
   int bits = 1;
   while (((int64_t)1 << bits) <= a.vocab) ++bits;   // the largest key is V itself (dropped)
   a.passes = (bits + SORT_BITS - 1) / SORT_BITS;
@@ -616,18 +640,18 @@ cudaError_t launch_embedding_grad(const ssd_embedding_grad_params_t* p, void* wo
   static std::atomic<uint64_t> allowed{0};
   cudaError_t e = allow_smem((const void*)sort_kernel, smem, &allowed);
   if (e != cudaSuccess) return e;
+  a.zero_ctas = 0;
   sort_kernel<<<SORT_CTAS, SORT_THREADS, smem, stream>>>(a);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  if (!a.accumulate) {   // one CTA per SM that does not sort
-    e = launch_dependent(ob ? zero_rows_kernel<bf16> : zero_rows_kernel<float>, dim3(148 - SORT_CTAS), SORT_THREADS,
-                         0, 1, stream, a);
-    if (e != cudaSuccess) return e;
-  }
-  if (a.n == 0) return e;
+  // two of the four resident CTAs of an SM write zeros while the sort runs, the others wait for it;
+  // all four where there are few sums
+  const int64_t sum_ctas = (a.npieces * ((a.dim + SUM_COLS - 1) / SUM_COLS) + SUM_THREADS / 32 - 1) / (SUM_THREADS / 32);
+  a.zero_ctas = a.accumulate ? 0 : 148 * 4 - (int)std::min<int64_t>(148 * 2, sum_ctas);
+  if (a.accumulate && a.n == 0) return e;
   const bool vec = rows16(p->grad, a.gs, a.dim, p->grad_dtype) && rows16(p->out, a.os, a.dim, p->out_dtype);
-  if (gb) return ob ? grad_sums<bf16, bf16>(a, vec, stream) : grad_sums<bf16, float>(a, vec, stream);
-  return ob ? grad_sums<float, bf16>(a, vec, stream) : grad_sums<float, float>(a, vec, stream);
+  if (gb) return ob ? grad_rows<bf16, bf16>(a, vec, stream) : grad_rows<bf16, float>(a, vec, stream);
+  return ob ? grad_rows<float, bf16>(a, vec, stream) : grad_rows<float, float>(a, vec, stream);
 }
 
 }  // namespace ssd

@@ -104,6 +104,23 @@ __device__ __forceinline__ void store_vec(T* p, int64_t i, int64_t n, int align,
   }
 }
 
+// V values to an aligned address, not to be kept in L2 (the gradients are).
+template <int V, typename T>
+__device__ __forceinline__ void store_stream(T* p, const float (&v)[V]) {
+  if constexpr (sizeof(T) == 4) {
+    __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
+  } else {
+    uint32_t u[V / 2];
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+      u[k] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    if constexpr (V == 8) __stcs(reinterpret_cast<uint4*>(p), make_uint4(u[0], u[1], u[2], u[3]));
+    else __stcs(reinterpret_cast<uint2*>(p), make_uint2(u[0], u[1]));
+  }
+}
+
 __device__ __forceinline__ int align_of(const void* p) {
   const uintptr_t a = reinterpret_cast<uintptr_t>(p);
   return a % 16 == 0 ? 16 : a % 8 == 0 ? 8 : a % 4 == 0 ? 4 : 2;
@@ -213,9 +230,10 @@ __global__ void __launch_bounds__(GC_THREADS, CTAS_PER_SM) scale_kernel(const __
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = nf.x;
   const float f = nf.y;
   const int c0 = (int)((int64_t)t.chunks * blockIdx.x / gridDim.x), c1 = (int)((int64_t)t.chunks * (blockIdx.x + 1) / gridDim.x);
-  int i = c0 < c1 ? tensor_of(t, c0) : 0;
-  for (int c = c0; c < c1; ++c) {
-    if (i + 1 < t.count && t.first[i + 1] <= c) ++i;
+  // backwards: the norm read the run's end last, and L2 may still hold it
+  int i = c0 < c1 ? tensor_of(t, c1 - 1) : 0;
+  for (int c = c1 - 1; c >= c0; --c) {
+    if (t.first[i] > c) --i;
     const T* g = static_cast<const T*>(t.g[i]);
     TO* o = static_cast<TO*>(t.out[i]);
     if (f == 1.f && static_cast<const void*>(o) == static_cast<const void*>(g)) continue;   // times one, in place
@@ -229,7 +247,7 @@ __global__ void __launch_bounds__(GC_THREADS, CTAS_PER_SM) scale_kernel(const __
       for (int j = 0; j < U; ++j) {
 #pragma unroll
         for (int k = 0; k < V; ++k) v[j][k] *= f;
-        store_vec<V>(o, base + (j * GC_THREADS + threadIdx.x) * V, n, 16, v[j]);
+        store_stream<V>(o + base + (j * GC_THREADS + threadIdx.x) * V, v[j]);
       }
     } else {
       for (int64_t e = base + threadIdx.x * V; e < n; e += GC_THREADS * V) {
