@@ -11,8 +11,8 @@
 //
 // The gradient is a sum by sorted ids, so that it is the same in every run: no atomics on
 // floats.  Launches:
-//   1. one cluster of 8 CTAs sorts (id, position) pairs by a stable radix sort whose histograms
-//      live in distributed shared memory;
+//   1. one cluster of 8 CTAs (one CTA for a few ids) sorts (id, position) pairs by a stable radix
+//      sort whose histograms live in distributed shared memory;
 //   2. a programmatic dependent launch that begins at once.  Its first CTAs write the zero rows of
 //      the ids that do not occur, most of a dense gradient: a CTA marks the ids of its own rows
 //      in a shared bitmap.  The others wait for the sort; they cut the sorted order into pieces
@@ -186,7 +186,7 @@ constexpr int ZERO_ROWS = 8192;   // rows whose bits the bitmap holds at a time
 
 struct GradArgs {
   int64_t n, vocab, dim, gs, os, pad, piece, npieces;
-  int is64, passes, accumulate, zero_ctas;
+  int is64, passes, bits, accumulate, zero_ctas;   // `bits` of an id per pass
   int extend;                     // rows that a piece may take from the next one, at most a piece and 32
   float scale;
   const void* ids;
@@ -198,22 +198,26 @@ struct GradArgs {
 };
 
 struct SortShared {
-  uint32_t warp_bin[SORT_WARPS][SORT_BINS];   // this CTA's counts, then each warp's next slot
+  // this CTA's counts, then each warp's next slot among the CTA's; a column lies in 32 banks
+  uint32_t warp_bin[SORT_WARPS][SORT_BINS + 1];
   uint32_t cta_bin[SORT_BINS];                // this CTA's count of each digit, read by the cluster
+  uint32_t base[SORT_BINS];                   // first slot of each digit for this CTA
   uint32_t scan[SORT_WARPS];
 };
 
-// One stable pass of the radix sort over the cluster.  What bounds it are the scattered stores, a
-// line for every lane: id and position go in one 8-byte store (32768 ids: 34 -> 28 us).  CTA c and its warp w own consecutive
-// tokens; a warp takes 32 of them at a time and lanes with equal digits find each other, so
-// equal digits keep their order.
+// One stable pass of the radix sort over the cluster, by the `bits` from `shift` on.  What bounds
+// it are the scattered stores, a line for every lane: id and position go in one 8-byte store
+// (32768 ids: 34 -> 28 us).  CTA c and its warp w own consecutive tokens; a warp takes 32 of them
+// at a time and lanes with equal digits find each other by match_any, so equal digits keep
+// their order.
 template <bool FIRST>
-__device__ void sort_pass(const GradArgs& a, SortShared* s, int shift, const uint2* from, uint2* to) {
+__device__ void sort_pass(const GradArgs& a, SortShared* s, int shift, int bits, const uint2* from, uint2* to) {
   cg::cluster_group cluster = cg::this_cluster();
-  const int cta = (int)cluster.block_rank(), tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
-  for (int i = tid; i < SORT_WARPS * SORT_BINS; i += SORT_THREADS) (&s->warp_bin[0][0])[i] = 0;
+  const int ctas = (int)cluster.num_blocks(), cta = (int)cluster.block_rank();
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, bins = 1 << bits;
+  for (int i = tid; i < SORT_WARPS * bins; i += SORT_THREADS) s->warp_bin[i >> bits][i & (bins - 1)] = 0;
   __syncthreads();
-  const int64_t per = (a.n + SORT_CTAS * SORT_WARPS - 1) / (SORT_CTAS * SORT_WARPS);
+  const int64_t per = (a.n + ctas * SORT_WARPS - 1) / (ctas * SORT_WARPS);
   const int64_t lo = (int64_t)(cta * SORT_WARPS + w) * per, hi = min(lo + per, a.n);
   auto key_at = [&](int64_t t) -> uint32_t {
     if constexpr (FIRST) {
@@ -233,7 +237,7 @@ __device__ void sort_pass(const GradArgs& a, SortShared* s, int shift, const uin
       const bool in = t0 + 32 * j + lane < hi;
       const unsigned live = __ballot_sync(0xffffffffu, in);
       if (in) {
-        const uint32_t d = (k[j] >> shift) & (SORT_BINS - 1);
+        const uint32_t d = (k[j] >> shift) & (bins - 1);
         const unsigned same = __match_any_sync(live, d);
         if (lane == __ffs(same) - 1) s->warp_bin[w][d] += __popc(same);
       }
@@ -241,21 +245,23 @@ __device__ void sort_pass(const GradArgs& a, SortShared* s, int shift, const uin
     }
   }
   __syncthreads();
-  // counts of each digit: exclusive over this CTA's warps, total over the CTA
-  if (tid < SORT_BINS) {
-    uint32_t sum = 0;
-    for (int i = 0; i < SORT_WARPS; ++i) {
-      const uint32_t c = s->warp_bin[i][tid];
-      s->warp_bin[i][tid] = sum;
-      sum += c;
+  // a warp per digit: exclusive over this CTA's warps, total over the CTA
+  for (int d = w; d < bins; d += SORT_WARPS) {
+    const uint32_t c = s->warp_bin[lane][d];
+    uint32_t incl = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
     }
-    s->cta_bin[tid] = sum;
+    s->warp_bin[lane][d] = incl - c;
+    if (lane == 31) s->cta_bin[d] = incl;
   }
   cluster.sync();
   // first slot of digit d for this CTA: all smaller digits, then digit d in the CTAs before
   uint32_t before = 0, total = 0;
-  if (tid < SORT_BINS) {
-    for (int c = 0; c < SORT_CTAS; ++c) {
+  if (tid < bins) {
+    for (int c = 0; c < ctas; ++c) {
       const uint32_t v = cluster.map_shared_rank(s->cta_bin, c)[tid];
       before += c < cta ? v : 0;
       total += v;
@@ -269,10 +275,10 @@ __device__ void sort_pass(const GradArgs& a, SortShared* s, int shift, const uin
   }
   if (lane == 31) s->scan[w] = incl;
   __syncthreads();
-  if (tid < SORT_BINS) {
+  if (tid < bins) {
     uint32_t base = incl - total + before;
     for (int i = 0; i < w; ++i) base += s->scan[i];
-    for (int i = 0; i < SORT_WARPS; ++i) s->warp_bin[i][tid] += base;
+    s->base[tid] = base;
   }
   __syncthreads();
   for (int64_t t0 = lo; t0 < hi; t0 += 32 * SORT_AHEAD) {
@@ -288,9 +294,9 @@ __device__ void sort_pass(const GradArgs& a, SortShared* s, int shift, const uin
       const bool in = t0 + 32 * j + lane < hi;
       const unsigned live = __ballot_sync(0xffffffffu, in);
       if (in) {
-        const uint32_t d = (e[j].x >> shift) & (SORT_BINS - 1);
+        const uint32_t d = (e[j].x >> shift) & (bins - 1);
         const unsigned same = __match_any_sync(live, d);
-        const uint32_t slot = s->warp_bin[w][d] + __popc(same & ((1u << lane) - 1));
+        const uint32_t slot = s->base[d] + s->warp_bin[w][d] + __popc(same & ((1u << lane) - 1));
         __syncwarp(live);
         if (lane == __ffs(same) - 1) s->warp_bin[w][d] += __popc(same);
         to[slot] = e[j];
@@ -301,16 +307,16 @@ __device__ void sort_pass(const GradArgs& a, SortShared* s, int shift, const uin
   cluster.sync();   // the cluster's keys are in place; every CTA has read the others' counts
 }
 
-__global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_THREADS, 1) sort_kernel(const GradArgs a) {
+__global__ void __launch_bounds__(SORT_THREADS, 1) sort_kernel(const GradArgs a) {
   extern __shared__ uint8_t smem[];
   ptx::griddep_launch_dependents();   // the zero rows need nothing from here
   SortShared* s = reinterpret_cast<SortShared*>(smem);
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.heavy = 0;
   // the passes end in list[0]
   int to = (a.passes - 1) & 1;
-  sort_pass<true>(a, s, 0, nullptr, a.list[to]);
+  sort_pass<true>(a, s, 0, a.bits, nullptr, a.list[to]);
   for (int p = 1; p < a.passes; ++p) {
-    sort_pass<false>(a, s, p * SORT_BITS, a.list[to], a.list[to ^ 1]);
+    sort_pass<false>(a, s, p * a.bits, a.bits, a.list[to], a.list[to ^ 1]);
     to ^= 1;
   }
 }
@@ -635,14 +641,27 @@ cudaError_t launch_embedding_grad(const ssd_embedding_grad_params_t* p, void* wo
   int bits = 1;
   while (((int64_t)1 << bits) <= a.vocab) ++bits;   // the largest key is V itself (dropped)
   a.passes = (bits + SORT_BITS - 1) / SORT_BITS;
+  a.bits = (bits + a.passes - 1) / a.passes;
   const bool gb = p->grad_dtype == SSD_DTYPE_BF16, ob = p->out_dtype == SSD_DTYPE_BF16;
   const size_t smem = sizeof(SortShared);
   static std::atomic<uint64_t> allowed{0};
   cudaError_t e = allow_smem((const void*)sort_kernel, smem, &allowed);
   if (e != cudaSuccess) return e;
   a.zero_ctas = 0;
-  sort_kernel<<<SORT_CTAS, SORT_THREADS, smem, stream>>>(a);
-  e = cudaGetLastError();
+  // one CTA where each warp has 32 ids at most (4 ids: 14 -> 12 us; 3237 ids took 6 us more in one)
+  const int ctas = a.n <= 32 * SORT_WARPS ? 1 : SORT_CTAS;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(SORT_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, sort_kernel, a);
   if (e != cudaSuccess) return e;
   // two of the four resident CTAs of an SM write zeros while the sort runs, the others wait for it;
   // all four where there are few sums

@@ -42,7 +42,7 @@ def embedding(tokens, weight, scale: float = 1.0, *, padding_idx=None, out_dtype
         raise ValueError("out_dtype must be torch.float32 or torch.bfloat16")
     w = _lib.rows2d(weight, dim)
     pad = -1 if padding_idx is None else _pad(padding_idx, vocab)
-    out = torch.empty((*ids.shape, dim), device=dev, dtype=out_dtype)
+    out = weight.new_empty((*ids.shape, dim), dtype=out_dtype)
     n = ids.numel()
     if n == 0:
         return out

@@ -74,8 +74,8 @@ def clip_grad_norm(grads, max_norm: float, *, eps: float = 1e-6, out=None, inpla
     Returns ``(clipped, norm)``: ``grads`` times ``min(1, max_norm / (norm + eps))`` and the norm
     before clipping (a float32 scalar tensor on the device; nothing waits for it).  By default
     the clipped gradients are new tensors; ``inplace=True`` scales ``grads`` themselves, ``out``
-    gives tensors of the same shapes to write to, float32 or bfloat16 (bfloat16 gradients into
-    the float32 buffers of an optimizer).  A NaN norm makes every gradient NaN.
+    gives contiguous tensors of as many elements to write to, float32 or bfloat16 (bfloat16
+    gradients into the float32 buffers of an optimizer).  A NaN norm makes every gradient NaN.
     """
     ts, dtypes, device = _checked(grads, "grads")
     if not float(max_norm) >= 0.0 or not float(eps) >= 0.0:
@@ -94,8 +94,8 @@ def clip_grad_norm(grads, max_norm: float, *, eps: float = 1e-6, out=None, inpla
             outs, out_dtypes, out_device = _checked(out, "out") if len(out) else ([], [], device)
             if len(outs) != len(ts):
                 raise ValueError(f"out has {len(outs)} tensors, grads {len(ts)}")
-            if list(map(_T.size, outs)) != list(map(_T.size, ts)) or not all(map(_T.is_contiguous, outs)):
-                raise ValueError("out must hold contiguous tensors of grads' shapes")
+            if list(map(_T.numel, outs)) != list(map(_T.numel, ts)) or not all(map(_T.is_contiguous, outs)):
+                raise ValueError("out must hold contiguous tensors of grads' sizes")
             if out_device != device:
                 raise ValueError("out and grads must be on one device")
     return outs, _run(ts, dtypes, outs, out_dtypes, max_norm, eps, True)
