@@ -37,8 +37,9 @@ constexpr int EC = gemm::EPI_COLS;
 
 // K blocks summed in TMEM before the sum goes to registers (tc_gemm.cuh), measured over K = 4096:
 // one segment 3.3e-6 off in the loss, 16 blocks 7.7e-7 (2 % slower), 8 blocks 3.6e-7 (4 % slower).
-// bf16 logits take 16; f32 products 8, which leaves 9e-7 in the gradients (16: 1.2e-6).
-constexpr int SEGMENT_BF16 = 16, SEGMENT_F32 = 8;
+// bf16 logits take 16.  f32 operands, with three products a block, take 2: gradients 7.6e-7 off (3
+// blocks 1.0e-6 and 3 % faster, 4 blocks 1.3e-6).
+constexpr int SEGMENT_BF16 = 16, SEGMENT_F32 = 2;
 constexpr int64_t LOSS_CHUNK = 16384;              // tokens whose statistics are kept at a time
 constexpr int64_t GRAD_BYTES = int64_t(3) << 30;   // logits and dl of a chunk of tokens
 
@@ -284,20 +285,20 @@ struct LogitArgs {
   const Scales* scales;
 };
 
-template <int CG>
+template <int CG, int PLANES>
 __global__ void __launch_bounds__(gemm::THREADS, 1) logits_kernel(const __grid_constant__ gemm::Problem p,
                                                                   const __grid_constant__ LogitArgs a) {
   extern __shared__ uint8_t smem[];
   __shared__ gemm::Ctl ctl;
   float unscale = 1.f;
   auto prep = [&]() {
-    if (p.passes == 3) unscale = 1.f / scale_of(a.scales->x) / scale_of(a.scales->w);
+    if (PLANES == 2) unscale = 1.f / scale_of(a.scales->x) / scale_of(a.scales->w);
   };
-  gemm::run<CG, false, false>(p, smem, &ctl, prep, [&](const gemm::Tile& t, float (&v)[EC], int row0, int n0, int live,
+  gemm::run<CG, PLANES, false, false>(p, smem, &ctl, prep, [&](const gemm::Tile& t, float (&v)[EC], int row0, int n0, int live,
                                                        int, uint4* stage) {
     const int row = row0 + (threadIdx.x & 31);
     const int y = row < live ? a.target[row] : -1;
-    if (p.passes == 3) {
+    if (PLANES == 2) {
 #pragma unroll
       for (int i = 0; i < EC; ++i) v[i] *= unscale;
     }
@@ -463,17 +464,17 @@ struct OutArgs {
 // split, go to the output.
 enum Mode { OUT, PART };
 
-template <int CG, bool A_MN, typename TO, Mode MODE>
+template <int CG, int PLANES, bool A_MN, typename TO, Mode MODE>
 __global__ void __launch_bounds__(gemm::THREADS, 1) grad_gemm_kernel(const __grid_constant__ gemm::Problem p,
                                                                      const __grid_constant__ OutArgs a) {
   extern __shared__ uint8_t smem[];
   __shared__ gemm::Ctl ctl;
   float unscale = 1.f, alpha = 1.f;
   auto prep = [&]() {
-    if (p.passes == 3) unscale = 1.f / scale_of(*a.largest[0]) / scale_of(*a.largest[1]);
+    if (PLANES == 2) unscale = 1.f / scale_of(*a.largest[0]) / scale_of(*a.largest[1]);
     alpha = *a.alpha;
   };
-  gemm::run<CG, A_MN, true>(p, smem, &ctl, prep, [&](const gemm::Tile& t, float (&v)[EC], int row0, int n0, int live,
+  gemm::run<CG, PLANES, A_MN, true>(p, smem, &ctl, prep, [&](const gemm::Tile& t, float (&v)[EC], int row0, int n0, int live,
                                                      int splits, uint4* stage) {
     const int64_t all = p.limit_k ? a.rows : live;
     const int rows = (int)min((int64_t)32, all - row0), cols = (int)min((int64_t)EC, a.cols - n0);
@@ -659,12 +660,13 @@ cudaError_t logits_gemm(const Operand& x, const Operand& w, int planes, const Lo
   g.m_tiles = cdiv(x.rows, BM * CG);
   g.n_tiles = cdiv(a.vocab, BN);
   g.k_blocks = cdiv(x.dim, gemm::BK);
-  g.passes = planes == 2 ? 3 : 1;
+  g.planes = planes;
   g.m_fastest = 1;
   g.segment = planes == 2 ? SEGMENT_F32 : SEGMENT_BF16;
   g.status = status;
-  static std::atomic<uint64_t> allowed{0};
-  return launch_gemm<CG>(logits_kernel<CG>, g, a, &allowed, st);
+  static std::atomic<uint64_t> allowed[2] = {};
+  if (planes == 2) return launch_gemm<CG>(logits_kernel<CG, 2>, g, a, &allowed[1], st);
+  return launch_gemm<CG>(logits_kernel<CG, 1>, g, a, &allowed[0], st);
 }
 
 // One gradient: the GEMM, and where its K range may be split the sum of the parts.
@@ -684,14 +686,20 @@ cudaError_t grad_gemm(const Operand& a, const Operand& b, int64_t k, int planes,
   g.max_splits = part_values > 0 ? MAX_SPLITS : 1;
   g.part_values = part_values;
   g.k_blocks = cdiv(k, gemm::BK);
-  g.passes = planes == 2 ? 3 : 1;
+  g.planes = planes;
   g.m_fastest = 0;
   // bf16: the operands' own rounding is a hundred times what the adds lose
   g.segment = planes == 2 ? SEGMENT_F32 : 1 << 20;
   g.status = status;
-  static std::atomic<uint64_t> allowed[2] = {};
-  if (!o.sum && g.max_splits == 1) return launch_gemm<CG>(grad_gemm_kernel<CG, A_MN, TO, OUT>, g, o, &allowed[0], st);
-  const cudaError_t e = launch_gemm<CG>(grad_gemm_kernel<CG, A_MN, TO, PART>, g, o, &allowed[1], st);
+  static std::atomic<uint64_t> allowed[4] = {};
+  const bool out = !o.sum && g.max_splits == 1;
+  cudaError_t e;
+  if (planes == 2)
+    e = out ? launch_gemm<CG>(grad_gemm_kernel<CG, 2, A_MN, TO, OUT>, g, o, &allowed[0], st)
+            : launch_gemm<CG>(grad_gemm_kernel<CG, 2, A_MN, TO, PART>, g, o, &allowed[1], st);
+  else
+    e = out ? launch_gemm<CG>(grad_gemm_kernel<CG, 1, A_MN, TO, OUT>, g, o, &allowed[2], st)
+            : launch_gemm<CG>(grad_gemm_kernel<CG, 1, A_MN, TO, PART>, g, o, &allowed[3], st);
   if (e != cudaSuccess || g.max_splits == 1) return e;
   return launch_dependent(join_kernel<CG, TO>, dim3((unsigned)std::min<int64_t>(o.rows, SMS * 8)), 256, 0, 1, st, g, o);
 }

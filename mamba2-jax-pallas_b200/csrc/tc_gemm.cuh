@@ -19,8 +19,8 @@
 // TMEM accumulator, and the epilogue warps add the segments in registers, rounding to nearest:
 // 64 values per thread.
 //
-// f32 operands come as two f16 planes of the values times a power of two, v = hi + lo, and the
-// K loop runs over the plane pairs hi*lo, lo*hi, hi*hi.  Two f16 hold 22 bits of a value down
+// f32 operands come as two f16 planes of the values times a power of two, v = hi + lo, and a K
+// block takes the products hi*hi, hi*lo, lo*hi from two stages.  Two f16 hold 22 bits of a value down
 // to 2^-16 of the largest, so three products carry what f32 carries; two bf16 hold 16.
 //
 // Every wait is bounded; one that gives up sets the status word and the CTA drains and ends.
@@ -76,7 +76,7 @@ struct Problem {
   int64_t part_values;                    // room for the parts
   int rows_out, cols;                     // of the result (limit_k; else its rows are the live ones)
   int k_blocks;                           // of 64
-  int passes;                             // 1 (bf16), or 3 (f32 as two f16 planes)
+  int planes;                             // 1 (bf16), or 2 (f32 as two f16 planes, three products)
   int segment;                            // K blocks that are summed in TMEM
   int m_fastest;
   unsigned* status;
@@ -95,7 +95,7 @@ __device__ __forceinline__ int live_rows(const Problem& p) { return min(max(*p.l
 template <int CG>
 __device__ __forceinline__ int pick_splits(int tiles, int blocks, int64_t values, int max_splits, int64_t part_values) {
   if (max_splits <= 1 || tiles <= 0) return 1;
-  const int s = (threadIdx.x & 31) + 1, ctas = 148 / CG;
+  const int s = (threadIdx.x & 31) + 1, ctas = 148 / CG;   // `blocks`: as many MMAs as a bf16 K block
   float cost = (float)((tiles * s + ctas - 1) / ctas) * (float)((blocks + s - 1) / s + 12);
   if (s > 1) cost += (float)s * (float)values * 3.6e-6f + 8.f;
   if (s > max_splits || s * values > part_values || s > blocks) cost = 3e38f;
@@ -155,7 +155,7 @@ template <int CG>
 __device__ __forceinline__ int splits_of(const Problem& p, int live) {
   const int m_tiles = p.limit_k ? p.m_tiles : (live + BM * CG - 1) / (BM * CG);
   const int k_blocks = p.limit_k ? (live + BK - 1) / BK : p.k_blocks;
-  return pick_splits<CG>(m_tiles * p.n_tiles, k_blocks, (int64_t)(p.limit_k ? p.rows_out : live) * p.cols,
+  return pick_splits<CG>(m_tiles * p.n_tiles, k_blocks * (2 * p.planes - 1), (int64_t)(p.limit_k ? p.rows_out : live) * p.cols,
                          p.max_splits, p.part_values);
 }
 
@@ -234,10 +234,10 @@ __device__ __forceinline__ void tmem_free_all(uint32_t t) {
 }
 
 // Instruction descriptor: f16 operands have format 0, bf16 format 1.
-template <int CG, bool A_MN, bool B_MN>
-__device__ __forceinline__ uint32_t idesc(const Problem& p) {
+template <int CG, int PLANES, bool A_MN, bool B_MN>
+__device__ __forceinline__ constexpr uint32_t idesc() {
   constexpr uint32_t ID = ptx::idesc_bf16_f32(BM * CG, BN, A_MN, B_MN);
-  return p.passes == 3 ? ID & ~((1u << 7) | (1u << 10)) : ID;
+  return PLANES == 2 ? ID & ~((1u << 7) | (1u << 10)) : ID;
 }
 
 // Where chunk `c` of a staged row lies, in 16-byte units.
@@ -290,9 +290,20 @@ __device__ __forceinline__ void by_rows(uint4* stage, const float (&v)[EPI_COLS]
   }
 }
 
+// One K block: A at sa and B at sb in shared memory.
+template <int CG, bool A_MN, bool B_MN>
+__device__ __forceinline__ void mma_block(uint32_t d, uint32_t sa, uint32_t sb, uint32_t id, bool accumulate) {
+#pragma unroll
+  for (int k = 0; k < BK / 16; ++k) {
+    const uint64_t da = A_MN ? ptx::sdesc_sw128(sa + k * 2048, 8192, 1024) : ptx::sdesc_sw128(sa + k * 32, 16, 1024);
+    const uint64_t db = B_MN ? ptx::sdesc_sw128(sb + k * 2048, 8192, 1024) : ptx::sdesc_sw128(sb + k * 32, 16, 1024);
+    mma<CG>(d, da, db, id, (accumulate || k > 0) ? 1u : 0u);
+  }
+}
+
 // The kernel's body.  prep() runs on every thread once the launches before are complete.  epi(tile, v, row0, first column, rows that count, splits, stage) runs on each
 // epilogue thread; v holds 64 values of row row0 + lane; `splits` parts of the K range.
-template <int CG, bool A_MN, bool B_MN, typename Prep, typename Epi>
+template <int CG, int PLANES, bool A_MN, bool B_MN, typename Prep, typename Epi>
 __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c, Prep&& prep, Epi&& epi) {
   using S = Shape<CG>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -326,7 +337,7 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
   const int64_t unit0 = blockIdx.x / CG, units = (int64_t)m_tiles * p.n_tiles * splits, step = gridDim.x / CG;
   if (warp == 0) {
     if (lane == 0) {
-      for (int i = 0; i < (p.passes == 3 ? 2 : 1); ++i) {
+      for (int i = 0; i < PLANES; ++i) {
         ptx::prefetch_tmap(&p.a[i]);
         ptx::prefetch_tmap(&p.b[i]);
       }
@@ -335,11 +346,9 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
       for (int64_t u = unit0; ok && u < units; u += step) {
         const Tile t = tile_at(p, m_tiles, k_blocks, splits, u);
         const int m0 = (t.m * CG + (int)rank) * BM, n0 = t.n * BN + (int)rank * (BN / CG);
-        for (int ps = 0; ok && ps < p.passes; ++ps) {
-          // pass order hi*lo, lo*hi, hi*hi: the small products first
-          const CUtensorMap* ma = &p.a[p.passes == 3 && ps == 1];
-          const CUtensorMap* mb = &p.b[p.passes == 3 && ps == 0];
-          for (int kb = t.k0; kb < t.k1; ++kb, ++it) {
+        for (int kb = t.k0; ok && kb < t.k1; ++kb) {
+#pragma unroll
+          for (int pl = 0; pl < PLANES; ++pl, ++it) {
             const int s = it % S::STAGES;
             if (it >= S::STAGES && !wait(c, &c->empty[s], ((it / S::STAGES) - 1) & 1, p.status, 1)) {
               ok = false;
@@ -352,14 +361,14 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
             if constexpr (CG == 2) bar = map_rank(bar, 0);
             const int k = kb * BK;
             if constexpr (A_MN) {
-              for (int i = 0; i < BM / 64; ++i) tma_load_2d<CG>(sa + i * 8192, ma, bar, m0 + 64 * i, k);
+              for (int i = 0; i < BM / 64; ++i) tma_load_2d<CG>(sa + i * 8192, &p.a[pl], bar, m0 + 64 * i, k);
             } else {
-              tma_load_2d<CG>(sa, ma, bar, k, m0);
+              tma_load_2d<CG>(sa, &p.a[pl], bar, k, m0);
             }
             if constexpr (B_MN) {
-              for (int i = 0; i < BN / CG / 64; ++i) tma_load_2d<CG>(sb + i * 8192, mb, bar, n0 + 64 * i, k);
+              for (int i = 0; i < BN / CG / 64; ++i) tma_load_2d<CG>(sb + i * 8192, &p.b[pl], bar, n0 + 64 * i, k);
             } else {
-              tma_load_2d<CG>(sb, mb, bar, k, n0);
+              tma_load_2d<CG>(sb, &p.b[pl], bar, k, n0);
             }
           }
         }
@@ -374,17 +383,16 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      const uint32_t ID = idesc<CG, A_MN, B_MN>(p);
+      const uint32_t ID = idesc<CG, PLANES, A_MN, B_MN>(), smem0 = ptx::smem_u32(smem);
       uint32_t it = 0, n = 0;
       bool ok = true;
       for (int64_t u = unit0; ok && u < units; u += step) {
         const Tile t = tile_at(p, m_tiles, k_blocks, splits, u);
-        const int steps = p.passes * (t.k1 - t.k0);
         uint32_t d = 0;
-        for (int j = 0, left = 0; j < steps; ++j, ++it, --left) {
+        for (int kb = t.k0, left = 0; kb < t.k1; ++kb, --left) {
           const bool first = left == 0;
           if (first) {
-            left = min(p.segment, steps - j);
+            left = min(p.segment, t.k1 - kb);
             if (n >= 2 && !wait(c, &c->acc_empty[n & 1], ((n >> 1) - 1) & 1, p.status, 2)) {
               ok = false;
               break;
@@ -398,12 +406,21 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
             break;
           }
           ptx::tc_fence_after();
-          const uint32_t sa = ptx::smem_u32(smem + s * S::STAGE_BYTES), sb = sa + S::A_BYTES;
-#pragma unroll
-          for (int k = 0; k < BK / 16; ++k) {
-            const uint64_t da = A_MN ? ptx::sdesc_sw128(sa + k * 2048, 8192, 1024) : ptx::sdesc_sw128(sa + k * 32, 16, 1024);
-            const uint64_t db = B_MN ? ptx::sdesc_sw128(sb + k * 2048, 8192, 1024) : ptx::sdesc_sw128(sb + k * 32, 16, 1024);
-            mma<CG>(d, da, db, ID, (!first || k > 0) ? 1u : 0u);
+          const uint32_t sa = smem0 + s * S::STAGE_BYTES;
+          mma_block<CG, A_MN, B_MN>(d, sa, sa + S::A_BYTES, ID, !first);
+          ++it;
+          if constexpr (PLANES == 2) {   // the low planes lie in the next stage
+            const int s1 = it % S::STAGES;
+            if (!wait(c, &c->full[s1], (it / S::STAGES) & 1, p.status, 3)) {
+              ok = false;
+              break;
+            }
+            ptx::tc_fence_after();
+            const uint32_t sl = smem0 + s1 * S::STAGE_BYTES;
+            mma_block<CG, A_MN, B_MN>(d, sa, sl + S::A_BYTES, ID, true);
+            mma_block<CG, A_MN, B_MN>(d, sl, sa + S::A_BYTES, ID, true);
+            commit<CG>(&c->empty[s1]);
+            ++it;
           }
           commit<CG>(&c->empty[s]);
           if (left == 1) {
@@ -433,7 +450,7 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
       float v[EPI_COLS];
 #pragma unroll
       for (int i = 0; i < EPI_COLS; ++i) v[i] = 0.f;
-      for (int left = p.passes * (t.k1 - t.k0); left > 0; left -= p.segment, ++n) {
+      for (int left = t.k1 - t.k0; left > 0; left -= p.segment, ++n) {
         // one lane waits for the warp, so that the warp stays converged for its TMEM loads
         int there = 0;
         if (lane == 0) there = wait(c, &c->acc_full[n & 1], (n >> 1) & 1, p.status, 4);
