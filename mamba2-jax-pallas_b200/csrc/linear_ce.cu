@@ -571,6 +571,7 @@ cudaError_t launch_gemm(Kernel kernel, const gemm::Problem& p, const Args& a, st
   const cudaError_t e = allow_smem((const void*)kernel, smem, allowed);
   if (e != cudaSuccess) return e;
   const int64_t units = (int64_t)p.m_tiles * p.n_tiles * std::max(1, p.max_splits);
+  if (units >= (int64_t(1) << 31) || (int64_t)p.k_blocks * MAX_SPLITS >= (int64_t(1) << 31)) return cudaErrorInvalidValue;
   return launch_dependent(kernel, dim3((unsigned)(CG * std::min<int64_t>(units, SMS / CG))), gemm::THREADS, smem, CG, st, p, a);
 }
 

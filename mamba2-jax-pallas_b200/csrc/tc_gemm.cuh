@@ -105,20 +105,16 @@ __device__ __forceinline__ int pick_splits(int tiles, int blocks, int64_t values
   return __ffs(__ballot_sync(0xffffffffu, bits == least));
 }
 
-__device__ __forceinline__ Tile tile_at(const Problem& p, int m_tiles, int k_blocks, int splits, int64_t u) {
+__device__ __forceinline__ Tile tile_at(const Problem& p, unsigned m_tiles, int k_blocks, unsigned splits, unsigned u) {
   Tile t;
-  const int64_t per = (int64_t)m_tiles * p.n_tiles;
-  t.split = (int)(u / per);
-  const int64_t r = u - t.split * per;
-  if (p.m_fastest) {
-    t.n = (int)(r / m_tiles);
-    t.m = (int)(r - (int64_t)t.n * m_tiles);
-  } else {
-    t.m = (int)(r / p.n_tiles);
-    t.n = (int)(r - (int64_t)t.m * p.n_tiles);
-  }
-  t.k0 = (int)((int64_t)k_blocks * t.split / splits);
-  t.k1 = (int)((int64_t)k_blocks * (t.split + 1) / splits);
+  const unsigned n_tiles = (unsigned)p.n_tiles, per = m_tiles * n_tiles;
+  const unsigned split = splits == 1 ? 0 : u / per, r = u - split * per;
+  const unsigned a = p.m_fastest ? m_tiles : n_tiles, q = r / a, rest = r - q * a;
+  t.split = (int)split;
+  t.n = (int)(p.m_fastest ? q : rest);
+  t.m = (int)(p.m_fastest ? rest : q);
+  t.k0 = splits == 1 ? 0 : (int)((unsigned)k_blocks * split / splits);   // splits <= 32
+  t.k1 = splits == 1 ? k_blocks : (int)((unsigned)k_blocks * (split + 1) / splits);
   return t;
 }
 
@@ -334,27 +330,29 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
   const int m_tiles = p.limit_k ? p.m_tiles : (live + BM * CG - 1) / (BM * CG);
   const int k_blocks = p.limit_k ? (live + BK - 1) / BK : p.k_blocks;
   const int splits = splits_of<CG>(p, live);
-  const int64_t unit0 = blockIdx.x / CG, units = (int64_t)m_tiles * p.n_tiles * splits, step = gridDim.x / CG;
+  const unsigned unit0 = blockIdx.x / CG, units = (unsigned)m_tiles * p.n_tiles * splits, step = gridDim.x / CG;   // below 2^31
+  const uint32_t smem0 = ptx::smem_u32(smem);
+
   if (warp == 0) {
     if (lane == 0) {
       for (int i = 0; i < PLANES; ++i) {
         ptx::prefetch_tmap(&p.a[i]);
         ptx::prefetch_tmap(&p.b[i]);
       }
-      uint32_t it = 0;
+      uint32_t it = 0, s = 0, phase = 1;   // stage, and the parity of its last release
       bool ok = true;
-      for (int64_t u = unit0; ok && u < units; u += step) {
+      for (unsigned u = unit0; ok && u < units; u += step) {
         const Tile t = tile_at(p, m_tiles, k_blocks, splits, u);
         const int m0 = (t.m * CG + (int)rank) * BM, n0 = t.n * BN + (int)rank * (BN / CG);
         for (int kb = t.k0; ok && kb < t.k1; ++kb) {
 #pragma unroll
           for (int pl = 0; pl < PLANES; ++pl, ++it) {
-            const int s = it % S::STAGES;
-            if (it >= S::STAGES && !wait(c, &c->empty[s], ((it / S::STAGES) - 1) & 1, p.status, 1)) {
+            // (a barrier's phase before its first counts as complete)
+            if (!wait(c, &c->empty[s], phase, p.status, 1)) {
               ok = false;
               break;
             }
-            const uint32_t sa = ptx::smem_u32(smem + s * S::STAGE_BYTES), sb = sa + S::A_BYTES;
+            const uint32_t sa = smem0 + s * S::STAGE_BYTES, sb = sa + S::A_BYTES;
             uint32_t bar = ptx::smem_u32(&c->full[s]);
             // the pair's first CTA counts the bytes of both
             if (rank == 0) ptx::mbar_arrive_expect_tx(&c->full[s], CG * S::STAGE_BYTES);
@@ -370,6 +368,10 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
             } else {
               tma_load_2d<CG>(sb, &p.b[pl], bar, k, n0);
             }
+            if (++s == S::STAGES) {
+              s = 0;
+              phase ^= 1;
+            }
           }
         }
       }
@@ -383,10 +385,10 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      const uint32_t ID = idesc<CG, PLANES, A_MN, B_MN>(), smem0 = ptx::smem_u32(smem);
-      uint32_t it = 0, n = 0;
+      const uint32_t ID = idesc<CG, PLANES, A_MN, B_MN>();
+      uint32_t s = 0, phase = 0, n = 0;
       bool ok = true;
-      for (int64_t u = unit0; ok && u < units; u += step) {
+      for (unsigned u = unit0; ok && u < units; u += step) {
         const Tile t = tile_at(p, m_tiles, k_blocks, splits, u);
         uint32_t d = 0;
         for (int kb = t.k0, left = 0; kb < t.k1; ++kb, --left) {
@@ -400,29 +402,34 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
             ptx::tc_fence_after();
             d = tmem + (n & 1) * BN;
           }
-          const int s = it % S::STAGES;
-          if (!wait(c, &c->full[s], (it / S::STAGES) & 1, p.status, 3)) {
+          if (!wait(c, &c->full[s], phase, p.status, 3)) {
             ok = false;
             break;
           }
           ptx::tc_fence_after();
           const uint32_t sa = smem0 + s * S::STAGE_BYTES;
+          uint64_t* const done = &c->empty[s];
           mma_block<CG, A_MN, B_MN>(d, sa, sa + S::A_BYTES, ID, !first);
-          ++it;
+          if (++s == S::STAGES) {
+            s = 0;
+            phase ^= 1;
+          }
           if constexpr (PLANES == 2) {   // the low planes lie in the next stage
-            const int s1 = it % S::STAGES;
-            if (!wait(c, &c->full[s1], (it / S::STAGES) & 1, p.status, 3)) {
+            if (!wait(c, &c->full[s], phase, p.status, 3)) {
               ok = false;
               break;
             }
             ptx::tc_fence_after();
-            const uint32_t sl = smem0 + s1 * S::STAGE_BYTES;
+            const uint32_t sl = smem0 + s * S::STAGE_BYTES;
             mma_block<CG, A_MN, B_MN>(d, sa, sl + S::A_BYTES, ID, true);
             mma_block<CG, A_MN, B_MN>(d, sl, sa + S::A_BYTES, ID, true);
-            commit<CG>(&c->empty[s1]);
-            ++it;
+            commit<CG>(&c->empty[s]);
+            if (++s == S::STAGES) {
+              s = 0;
+              phase ^= 1;
+            }
           }
-          commit<CG>(&c->empty[s]);
+          commit<CG>(done);
           if (left == 1) {
             commit<CG>(&c->acc_full[n & 1]);
             ++n;
@@ -445,7 +452,7 @@ __device__ __forceinline__ void run(const Problem& p, uint8_t* smem_raw, Ctl* c,
     uint4* stage = reinterpret_cast<uint4*>(smem + S::STAGES * S::STAGE_BYTES + (warp - 2) * S::EPI_WARP_BYTES);
     uint32_t n = 0;
     bool ok = true;
-    for (int64_t u = unit0; ok && u < units; u += step) {
+    for (unsigned u = unit0; ok && u < units; u += step) {
       const Tile t = tile_at(p, m_tiles, k_blocks, splits, u);
       float v[EPI_COLS];
 #pragma unroll
