@@ -561,6 +561,69 @@ def test_clip_grad_norm_nonfinite_zero_and_strides():
 
 
 # ---------------------------------------------------------------------------------------------
+# offsets past 32 bits
+# ---------------------------------------------------------------------------------------------
+BIG_V, BIG_D = 540_001, 4096          # 2.2e9 values
+
+
+@gpu
+def test_offsets_past_32_bits_embedding():
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    w = torch.empty((BIG_V, BIG_D), dtype=torch.bfloat16, device="cuda")
+    w[-300:] = torch.randn((300, BIG_D), generator=gen, device="cuda").bfloat16()
+    w[:300] = 1.0
+    ids = torch.cat([torch.arange(BIG_V - 300, BIG_V), torch.arange(300)]).cuda()
+    out = embedding(ids, w, scale=1.5)
+    assert same_bits(out, (w[ids].float() * 1.5).bfloat16())
+    g = torch.randn((600, BIG_D), generator=gen, device="cuda").bfloat16()
+    dw = embedding_grad(ids, g, BIG_V)
+    assert same_bits(dw[ids], g) and not bool(dw[300:-300].any())
+
+
+@gpu
+@pytest.mark.parametrize("t", [3, 40])
+def test_offsets_past_32_bits_linear_cross_entropy(t):
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    w = torch.randn((BIG_V, BIG_D), generator=gen, device="cuda", dtype=torch.bfloat16) / 64
+    y = torch.randint(0, BIG_V, (t,), generator=gen, device="cuda")
+    y[0], y[-1] = BIG_V - 1, 0
+    x = (torch.randn((t, BIG_D), generator=gen, device="cuda") + 8 * w[y].float()).bfloat16()
+    loss, dx, dw = linear_cross_entropy_grad(x, w, y, reduction="sum", check_status=True)
+    # float64, in pieces of the vocabulary
+    xs = x.double()
+    lse = torch.full((t,), -float("inf"), dtype=torch.float64, device="cuda")
+    for lo in range(0, BIG_V, 60000):
+        lse = torch.logaddexp(lse, torch.logsumexp(xs @ w[lo:lo + 60000].double().t(), 1))
+    rows = lse - (xs * w[y].double()).sum(1)
+    assert abs(float(loss) - float(rows.sum())) <= 1e-5 * float(rows.sum())
+    dxs = torch.zeros_like(xs)
+    err = norm = 0.0
+    for lo in range(0, BIG_V, 60000):
+        p = torch.exp(xs @ w[lo:lo + 60000].double().t() - lse[:, None])
+        for i, v in enumerate(y.tolist()):
+            if lo <= v < lo + 60000:
+                p[i, v - lo] -= 1.0
+        dxs += p @ w[lo:lo + 60000].double()
+        ref = p.t() @ xs
+        err += float((dw[lo:lo + 60000].double() - ref).norm() ** 2)
+        norm += float(ref.norm() ** 2)
+    assert rel(dx, dxs.cpu()) <= 2 * V + 1e-3 and math.sqrt(err / norm) <= 2 * V + 1e-3
+
+
+@gpu
+def test_offsets_past_32_bits_clip():
+    n = 2 ** 31 + 4099
+    g = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    g[-5:] = 3.0
+    got, norm = clip_grad_norm([g], 1.0, inplace=True)
+    want = math.sqrt(n - 5 + 45)
+    assert abs(float(norm) - want) <= 2 * U * want
+    c = 1.0 / (want + 1e-6)
+    assert abs(float(got[0][-1]) - 3 * c) <= V * 3 * c and abs(float(got[0][2 ** 31]) - c) <= V * c
+    assert abs(float(got[0][0]) - c) <= V * c
+
+
+# ---------------------------------------------------------------------------------------------
 # refusals (no GPU needed unless a CUDA tensor is)
 # ---------------------------------------------------------------------------------------------
 def test_refuse_cpu_tensors():
