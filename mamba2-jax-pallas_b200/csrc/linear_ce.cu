@@ -36,10 +36,10 @@ using gemm::BN;
 constexpr int EC = gemm::EPI_COLS;
 
 // K blocks summed in TMEM before the sum goes to registers (tc_gemm.cuh), measured over K = 4096:
-// one segment 3.3e-6 off in the loss, 16 blocks 7.7e-7 (2 % slower), 8 blocks 3.6e-7 (4 % slower).
-// bf16 logits take 16.  f32 operands, with three products a block, take 2: gradients 7.6e-7 off (3
-// blocks 1.0e-6 and 3 % faster, 4 blocks 1.3e-6).
-constexpr int SEGMENT_BF16 = 16, SEGMENT_F32 = 2;
+// one segment 3.3e-6 off in the loss, 16 blocks 7.7e-7, 8 blocks 3.6e-7 at the same speed (4096 x
+// 131072 in 2.67 and 2.69 ms).  f32 operands, with three products a block, take 2: gradients
+// 7.6e-7 off (3 blocks 1.0e-6 and 3 % faster, 1 block 5.8e-7 and 3 % slower).
+constexpr int SEGMENT_BF16 = 8, SEGMENT_F32 = 2;
 constexpr int64_t LOSS_CHUNK = 16384;              // tokens whose statistics are kept at a time
 constexpr int64_t GRAD_BYTES = int64_t(3) << 30;   // logits and dl of a chunk of tokens
 
