@@ -283,7 +283,29 @@ struct LogitArgs {
   float* logits;           // (rows, ld) or NULL
   int64_t ld;
   const Scales* scales;
+  CUtensorMap map;         // of the logits, 32 x 32 values a box (pairs)
 };
+
+// Half a warp's 32 x 64 block to global memory: through its 4 KB of shared memory, in the layout
+// of a swizzled box, by one bulk store (f32, 2048 x 50257 x 768: the kernel takes 370 us where
+// the warp stores values itself, 354 us so and 297 us without any store).
+template <int HALF>
+__device__ __forceinline__ void store_half(const CUtensorMap* map, uint4* stage, const float (&v)[EC], int n0, int row0) {
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) ptx::bulk_wait_read();   // the store before has left the shared memory
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float* x = v + 32 * HALF + 4 * i;
+    stage[gemm::epi_at<2>(lane, i)] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+  }
+  ptx::fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    ptx::tma_store_2d(map, stage, n0 + 32 * HALF, row0);
+    ptx::bulk_commit();
+  }
+}
 
 template <int CG, int PLANES>
 __global__ void __launch_bounds__(gemm::THREADS, 1) logits_kernel(const __grid_constant__ gemm::Problem p,
@@ -302,7 +324,13 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) logits_kernel(const __grid_c
 #pragma unroll
       for (int i = 0; i < EC; ++i) v[i] *= unscale;
     }
-    if (a.logits) {   // their rows are a multiple of 64 long
+    // the logits' rows are a multiple of 64 long
+    if (CG == 2) {
+      if (a.logits && row0 < live && n0 < a.vocab) {
+        store_half<0>(&a.map, stage, v, n0, row0);
+        store_half<1>(&a.map, stage, v, n0, row0);
+      }
+    } else if (a.logits) {
       float* o = a.logits + row0 * a.ld + n0;
       const int cols = (int)min((int64_t)EC, a.vocab - n0);
       gemm::by_rows<CG, float>(stage, v, true, live - row0, [&](int i, int c, uint4 q) {
@@ -332,6 +360,7 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) logits_kernel(const __grid_c
     for (int i = 0; i < EC; ++i) e[i & 3] += exp2f(fmaf(v[i], LOG2E, -at));
     if (row < live) a.stats[(int64_t)row * a.ns + n0 / (EC)] = make_float2(top, (e[0] + e[1]) + (e[2] + e[3]));
   });
+  if (CG == 2) ptx::bulk_wait_all();
 }
 
 // The sum (or mean over the tokens that count) of the tokens' losses.
@@ -651,7 +680,7 @@ Plan plan_of(const ssd_linear_ce_params_t* p) {
   } while (0)
 
 template <int CG>
-cudaError_t logits_gemm(const Operand& x, const Operand& w, int planes, const LogitArgs& a, const int* count, int from,
+cudaError_t logits_gemm(const Operand& x, const Operand& w, int planes, LogitArgs a, const int* count, int from,
                         unsigned* status, cudaStream_t st) {
   gemm::Problem g{};
   g.limit = count;
@@ -665,6 +694,8 @@ cudaError_t logits_gemm(const Operand& x, const Operand& w, int planes, const Lo
   g.m_fastest = 1;
   g.segment = planes == 2 ? SEGMENT_F32 : SEGMENT_BF16;
   g.status = status;
+  if (CG == 2 && a.logits && !tc_map_2d(&a.map, a.logits, (uint64_t)a.ld, (uint64_t)x.rows, (uint64_t)a.ld * 4, 32, true))
+    return cudaErrorInvalidValue;
   static std::atomic<uint64_t> allowed[2] = {};
   if (planes == 2) return launch_gemm<CG>(logits_kernel<CG, 2>, g, a, &allowed[1], st);
   return launch_gemm<CG>(logits_kernel<CG, 1>, g, a, &allowed[0], st);

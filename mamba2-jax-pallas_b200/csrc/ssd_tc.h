@@ -23,7 +23,9 @@ bool tc_sp_fixup_supported(const ssd_sp_fixup_params_t* p);
 int tc_sp_fixup(const ssd_sp_fixup_params_t* p, cudaStream_t st);
 
 // 2-D tensor map over rows of `inner` bf16 values, `stride` bytes apart (a multiple of 16),
-// with a 64-value (128-byte, swizzled) x box_rows box.  False if the driver refuses it.
-bool tc_map_2d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows, uint64_t stride, uint32_t box_rows);
+// with a 64-value (128-byte, swizzled) x box_rows box; f32 values with `f32`, 32 to a box's row.
+// False if the driver refuses it.
+bool tc_map_2d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows, uint64_t stride, uint32_t box_rows,
+               bool f32 = false);
 
 }  // namespace ssd
