@@ -827,6 +827,8 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
     a.logits = q.grad ? reinterpret_cast<float*>(ws + q.logits) : nullptr;
     a.ld = q.ld;
     a.scales = sel.scales;
+    // one SM's tiles where a pair's second half would be empty (loss of 128 x 50000 x 2560: 68 us, by pairs 70;
+    // of 200 tokens, in two rows of tiles: 78, by pairs 71)
     if (n > BM) CE_CHECK(logits_gemm<2>(xc, w, q.planes, a, sel.count, from, status, st), "logits");
     else CE_CHECK(logits_gemm<1>(xc, w, q.planes, a, sel.count, from, status, st), "logits");
     RowFactors* factors = q.grad ? reinterpret_cast<RowFactors*>(ws + q.factors) : nullptr;

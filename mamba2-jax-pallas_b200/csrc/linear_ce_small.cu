@@ -28,6 +28,7 @@ using namespace ce;
 constexpr int SM_THREADS = 512, SM_WARPS = SM_THREADS / 32, SM_CTAS = 148;
 constexpr int WORDS = 4;                     // words of a warp at a time
 constexpr int MAX_ROWS = 8;                  // rows of one pass over the weight
+constexpr int MAX_TOKENS = 4 * MAX_ROWS;     // of a call
 constexpr size_t MAX_SMEM = 222 * 1024;      // besides the static part
 constexpr int G_THREADS = 256, G_COLS = 4 * G_THREADS, G_TILE = 64;
 
@@ -243,7 +244,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) small_logits_kernel(const __gri
 
 // One CTA, a warp per token (in turns).
 __global__ void __launch_bounds__(256) small_finish_kernel(const __grid_constant__ SmallArgs a) {
-  __shared__ float losses[32];
+  __shared__ float losses[MAX_TOKENS];
   ptx::griddep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int count = 0;
@@ -420,7 +421,9 @@ cudaError_t run_logits(const SmallArgs& a, size_t smem, cudaStream_t st) {
     case 1: return run_logits<T, 1, U>(a, smem, st);
     case 2: return run_logits<T, 2, U>(a, smem, st);
     case 4: return run_logits<T, 4, U>(a, smem, st);
-    default: return run_logits<T, 8, U>(a, smem, st);
+    default:   // (most_tokens)
+      if constexpr (sizeof(T) == 4 || U > 1) return run_logits<T, 8, U>(a, smem, st);
+      return cudaErrorInvalidValue;
   }
 }
 // Every row of the weight can be read in accesses of `bytes`.
@@ -446,8 +449,9 @@ cudaError_t run_grad(const SmallArgs& a, bool vec, cudaStream_t st) {
   switch (row_width(a.tokens)) {
     case 1: return run_grad<T, TW, 1>(a, vec, st);
     case 2: return run_grad<T, TW, 2>(a, vec, st);
-    case 4: return run_grad<T, TW, 4>(a, vec, st);
-    default: return run_grad<T, TW, 8>(a, vec, st);
+    default:   // (most_tokens)
+      if constexpr (sizeof(T) == 4) return a.tokens <= 4 ? run_grad<T, TW, 4>(a, vec, st) : run_grad<T, TW, 8>(a, vec, st);
+      return cudaErrorInvalidValue;
   }
 }
 
@@ -486,12 +490,23 @@ SmallPlan plan_of(const ssd_linear_ce_params_t* p) {
   return q;
 }
 
+// The most tokens of this form, from both forms' times (us, this one against tensor cores):
+//   bf16 loss       4 x 131072 x 4096 180 / 207, 5: 301 / 205; 4 x 50257 x 768 25 / 31, 6: 37 / 31; where the
+//                   weight would have to be copied for the tensor maps: 8 x 50000 x 1001 59 / 81, 16: 105 / 82
+//   bf16 gradients  2 x 50257 x 768 76 / 91, 4: 119 / 91; 2 x 50000 x 2560 190 / 193, 3: 313 / 195
+//   f32 loss        32 x 50257 x 768 123 / 132, 32 x 50000 x 2560 331 / 384
+//   f32 gradients   8 x 50257 x 768 150 / 223, 8 x 50000 x 2560 385 / 595 (rows of one pass)
+int64_t most_tokens(const ssd_linear_ce_params_t* p) {
+  const bool grad = p->grad_hidden || p->grad_weight;
+  if (p->dtype == SSD_DTYPE_F32) return grad ? MAX_ROWS : MAX_TOKENS;
+  if (grad) return 2;
+  return reinterpret_cast<uintptr_t>(p->weight) % 16 == 0 && p->weight_stride_row % 8 == 0 ? 4 : MAX_ROWS;
+}
+
 }  // namespace
 
 bool linear_ce_is_small(const ssd_linear_ce_params_t* p) {
-  const bool grad = p->grad_hidden || p->grad_weight;
-  const int64_t most = grad ? MAX_ROWS : p->dtype == SSD_DTYPE_F32 ? 4 * MAX_ROWS : MAX_ROWS;
-  return p->tokens <= most && logits_smem(p) + ring_bytes(2) <= MAX_SMEM && p->vocab < (1 << 30);
+  return p->tokens <= most_tokens(p) && logits_smem(p) + ring_bytes(2) <= MAX_SMEM && p->vocab < (1 << 30);
 }
 
 size_t linear_ce_small_workspace(const ssd_linear_ce_params_t* p) { return plan_of(p).total; }

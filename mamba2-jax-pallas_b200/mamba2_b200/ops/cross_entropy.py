@@ -40,22 +40,20 @@ def _call(hidden, weight, targets, ignore_index, reduction, grad_loss, want_lse,
         if not isinstance(grad_loss, torch.Tensor) or tuple(grad_loss.shape) != want or grad_loss.device != dev:
             raise ValueError(f"grad_loss must be a {want} tensor on hidden's device")
         g = _lib.dev(grad_loss, "grad_loss", torch.float32)
-    new = torch.zeros if n == 0 else torch.empty
-    loss = new(targets.shape if reduction == "none" else (), device=dev, dtype=torch.float32)
-    lse = new(targets.shape, device=dev, dtype=torch.float32) if want_lse else None
-    gx = new(hidden.shape, device=dev, dtype=x.dtype) if want_hidden else None
-    gw = new((vocab, dim), device=dev, dtype=wd) if want_weight else None
+    new = x.new_zeros if n == 0 else x.new_empty
+    loss = new(targets.shape if reduction == "none" else (), dtype=torch.float32)
+    lse = new(targets.shape, dtype=torch.float32) if want_lse else None
+    gx = new(hidden.shape) if want_hidden else None
+    gw = new((vocab, dim), dtype=wd) if want_weight else None
     if n == 0:
         return loss, lse, gx, gw
-    p = _lib.LinearCeParams(tokens=n, vocab=vocab, dim=dim, hidden_stride_row=_lib.row_stride(x),
-                            weight_stride_row=_lib.row_stride(w), ignore_index=int(ignore_index), dtype=dtype,
-                            targets_int64=int(y.dtype == torch.int64), reduction=_lib.REDUCTIONS[reduction],
-                            grad_weight_dtype=_lib.SSD_DTYPE_BF16 if wd == torch.bfloat16 else _lib.SSD_DTYPE_F32)
-    p.hidden, p.weight, p.targets, p.loss = x.data_ptr(), w.data_ptr(), y.data_ptr(), loss.data_ptr()
-    p.grad_loss, p.lse, p.grad_hidden, p.grad_weight = _lib.ptr(g), _lib.ptr(lse), _lib.ptr(gx), _lib.ptr(gw)
+    p = _lib.LinearCeParams(n, vocab, dim, _lib.row_stride(x), _lib.row_stride(w), int(ignore_index), dtype,
+                            y.dtype is torch.int64, _lib.REDUCTIONS[reduction], wd is torch.bfloat16, x.data_ptr(),
+                            w.data_ptr(), y.data_ptr(), _lib.ptr(g), loss.data_ptr(), _lib.ptr(lse), _lib.ptr(gx),
+                            _lib.ptr(gw))
     lib = _lib.load()
     with _lib.on_device(dev):
-        ws = torch.empty(lib.ssd_linear_cross_entropy_workspace_bytes(p), device=dev, dtype=torch.uint8)
+        ws = x.new_empty(lib.ssd_linear_cross_entropy_workspace_bytes(p), dtype=torch.uint8)
         _lib.check(lib.ssd_linear_cross_entropy(p, ws.data_ptr(), ws.numel(), _lib.stream_of(x)))
         if check_status:
             _lib.check_device_status(ws)

@@ -70,39 +70,42 @@ def embedding_grad(tokens, grad_out, num_embeddings: int, scale: float = 1.0, *,
         raise ValueError("num_embeddings must be positive")
     if not isinstance(grad_out, torch.Tensor) or not grad_out.is_cuda:
         raise ValueError("grad_out must be a CUDA tensor (no CPU path)")
-    if grad_out.dim() < 1 or tuple(grad_out.shape[:-1]) != tuple(tokens.shape):
-        raise ValueError(f"grad_out {tuple(grad_out.shape)} must be tokens' shape {tuple(tokens.shape)} and one axis more")
-    if ids.device != grad_out.device:
+    shape = grad_out.shape
+    if len(shape) < 1 or shape[:-1] != tokens.shape:
+        raise ValueError(f"grad_out {tuple(shape)} must be tokens' shape {tuple(tokens.shape)} and one axis more")
+    dev = grad_out.device
+    if ids.device != dev:
         raise ValueError("tokens and grad_out must be on one device")
-    dim = grad_out.shape[-1]
+    dim = shape[-1]
     if dim == 0:
         raise ValueError("grad_out must not have an empty last axis")
-    _lib.dtype_code(grad_out)
+    g_code = _lib.dtype_code(grad_out)
     g = _lib.rows2d(grad_out, dim)
     if accumulate_into is not None:
         out = accumulate_into
         if out_dtype is not None and out_dtype != out.dtype:
             raise ValueError("out_dtype is accumulate_into's dtype")
-        if not out.is_cuda or out.device != g.device:
+        if not out.is_cuda or out.device != dev:
             raise ValueError("accumulate_into must be on grad_out's device")
         if tuple(out.shape) != (vocab, dim) or (dim > 1 and out.stride(1) != 1) or (vocab > 1 and out.stride(0) < dim):
             raise ValueError(f"accumulate_into must be ({vocab}, {dim}) with contiguous rows")
+        out_stride = _lib.row_stride(out)
     else:
         out_dtype = grad_out.dtype if out_dtype is None else out_dtype
         if out_dtype not in _DTYPES:
             raise ValueError("out_dtype must be torch.float32 or torch.bfloat16")
-        out = torch.empty((vocab, dim), device=g.device, dtype=out_dtype)
-    p = _lib.EmbeddingGradParams(num_tokens=ids.numel(), vocab=vocab, dim=dim, grad_stride_row=_lib.row_stride(g),
-                                 out_stride_row=_lib.row_stride(out), padding_idx=_pad(padding_idx, vocab),
-                                 tokens_int64=int(ids.dtype == torch.int64), grad_dtype=_lib.dtype_code(g),
-                                 out_dtype=_lib.dtype_code(out), accumulate=int(accumulate_into is not None),
-                                 scale=float(scale))
-    if accumulate_into is not None and ids.numel() == 0:
+        out = g.new_empty((vocab, dim), dtype=out_dtype)
+        out_stride = dim
+    pad = -1 if padding_idx is None else _pad(padding_idx, vocab)
+    n = ids.numel()
+    p = _lib.EmbeddingGradParams(n, vocab, dim, _lib.row_stride(g), out_stride, pad, ids.dtype is torch.int64, g_code,
+                                 _lib.dtype_code(out), accumulate_into is not None, scale, ids.data_ptr(), g.data_ptr(),
+                                 out.data_ptr())
+    if accumulate_into is not None and n == 0:
         return out
-    p.tokens, p.grad, p.out = ids.data_ptr(), g.data_ptr(), out.data_ptr()
     lib = _lib.load()
-    n = lib.ssd_embedding_grad_workspace_bytes(p)
-    ws = torch.empty(max(n, 1), device=g.device, dtype=torch.uint8)
-    with _lib.on_device(g.device):
-        _lib.check(lib.ssd_embedding_grad(p, ws.data_ptr(), ws.numel(), _lib.stream_of(out)))
+    size = lib.ssd_embedding_grad_workspace_bytes(p)
+    ws = g.new_empty(max(size, 1), dtype=torch.uint8)
+    with _lib.on_device(dev):
+        _lib.check(lib.ssd_embedding_grad(p, ws.data_ptr(), size, _lib.stream_of(out)))
     return out
