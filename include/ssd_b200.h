@@ -393,7 +393,9 @@ typedef enum ssd_reduction {
  * [0, vocab) makes its loss NaN (and the gradients it takes part in).
  * bf16 inputs: products on the tensor cores with f32 accumulation; the gradient of the logits
  * is rounded once to bf16 as an operand of the products behind it.  f32 inputs: every operand
- * as two bf16 terms, three products per pair. */
+ * as two f16 terms of its values times a power of two (22 bits down to 2^-16 of the operand's
+ * largest value), three products per pair.  For a few tokens (f32: 32, with gradients 8; bf16: 4
+ * or 8, with gradients 2) the products run in f32 on the CUDA cores. */
 typedef struct ssd_linear_ce_params {
   int64_t tokens, vocab, dim;
   int64_t hidden_stride_row, weight_stride_row; /* element strides between rows, >= dim */

@@ -11,8 +11,8 @@
 //
 // The gradient is a sum by sorted ids, so that it is the same in every run: no atomics on
 // floats.  Launches:
-//   1. one cluster of 8 CTAs (one CTA for a few ids) sorts (id, position) pairs by a stable radix
-//      sort whose histograms live in distributed shared memory;
+//   1. one cluster of 8 CTAs sorts (id, position) pairs by a stable radix sort whose histograms
+//      live in distributed shared memory; few ids are placed by counting instead;
 //   2. a programmatic dependent launch that begins at once.  Its first CTAs write the zero rows of
 //      the ids that do not occur, most of a dense gradient: a CTA marks the ids of its own rows
 //      in a shared bitmap.  The others wait for the sort; they cut the sorted order into pieces
@@ -187,6 +187,7 @@ constexpr int ZERO_ROWS = 8192;   // rows whose bits the bitmap holds at a time
 struct GradArgs {
   int64_t n, vocab, dim, gs, os, pad, piece, npieces;
   int is64, passes, bits, accumulate, zero_ctas;   // `bits` of an id per pass
+  int zero_lanes;                 // lanes of a zero row, as a power of two
   int extend;                     // rows that a piece may take from the next one, at most a piece and 32
   float scale;
   const void* ids;
@@ -321,6 +322,49 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) sort_kernel(const GradArgs a)
   }
 }
 
+// Few ids: a warp finds a token's place by counting the ids before it, four tokens at a time, all
+// ids in the shared memory of every CTA.  An id and its position make one 32-bit number, so each pair
+// takes one comparison: n^2 of them, spread over the GPU, against the radix sort's passes, which
+// wait for one another.  777 ids 3.4 us, 4000 ids 9 us.
+constexpr int RANK_THREADS = 512, RANK_WARPS = RANK_THREADS / 32, RANK_KEYS = 4;
+constexpr int64_t RANK_MAX = 4096;
+constexpr int64_t RANK_TABLE = 64 << 20;
+
+__global__ void __launch_bounds__(RANK_THREADS) rank_kernel(const GradArgs a, int shift) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint32_t* code = reinterpret_cast<uint32_t*>(smem);
+  ptx::griddep_launch_dependents();   // the zero rows need nothing from here
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, n = (int)a.n, padded = (n + 127) / 128 * 128;
+  if (blockIdx.x == 0 && tid == 0) *a.heavy = 0;
+#pragma unroll 4
+  for (int t = tid; t < padded; t += RANK_THREADS) {
+    const int64_t v = row_of(a.ids, a.is64, min(t, n - 1), a.vocab, a.pad);
+    code[t] = t < n ? (uint32_t)(v < 0 ? a.vocab : v) << shift | (uint32_t)t : ~0u;
+  }
+  __syncthreads();
+  const int warps = gridDim.x * RANK_WARPS;
+  for (int t0 = blockIdx.x * RANK_WARPS + w; t0 < n; t0 += warps * RANK_KEYS) {
+    uint32_t mine[RANK_KEYS], before[RANK_KEYS];
+#pragma unroll
+    for (int k = 0; k < RANK_KEYS; ++k) {
+      mine[k] = t0 + k * warps < n ? code[t0 + k * warps] : 0;
+      before[k] = 0;
+    }
+#pragma unroll 2
+    for (int j = lane * 4; j < padded; j += 128) {
+      const uint4 q = *reinterpret_cast<const uint4*>(code + j);
+#pragma unroll
+      for (int k = 0; k < RANK_KEYS; ++k)
+        before[k] += (q.x < mine[k]) + (q.y < mine[k]) + (q.z < mine[k]) + (q.w < mine[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < RANK_KEYS; ++k) {
+      const uint32_t at = __reduce_add_sync(0xffffffffu, before[k]);
+      if (lane == 0 && t0 + k * warps < n) a.list[0][at] = make_uint2(mine[k] >> shift, (uint32_t)(t0 + k * warps));
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // gradient: zero rows and sums
 // ---------------------------------------------------------------------------
@@ -388,21 +432,22 @@ __device__ __forceinline__ void put_row(const GradArgs& a, uint32_t id, int64_t 
 }
 
 // Zero rows of the ids that do not occur.  A CTA owns rows [r0, r1) and marks those that
-// occur in a shared bitmap, ZERO_ROWS at a time, reading all ids (L2) once for each.
+// occur in a shared bitmap, ZERO_ROWS at a time, reading all ids (L2) once for each.  2^zero_lanes
+// lanes write a row.
 template <typename TO>
 __device__ void zero_rows(const GradArgs& a, uint32_t* bits) {
-  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int rows_at_once = 32 >> a.zero_lanes, sub = lane & ((1 << a.zero_lanes) - 1), step = 1 << a.zero_lanes;
   const int64_t per = (a.vocab + a.zero_ctas - 1) / a.zero_ctas;
   const int64_t r0 = blockIdx.x * per, r1 = min(r0 + per, a.vocab);
-  const bool vec = (reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.os * sizeof(TO))) % 16 == 0;
   // two 64-bit ids at a time where they lie so
   const int64_t pairs = a.is64 && reinterpret_cast<uintptr_t>(a.ids) % 16 == 0 ? a.n / 2 : 0;
   for (int64_t b0 = r0; b0 < r1; b0 += ZERO_ROWS) {
-    const int64_t b1 = min(b0 + ZERO_ROWS, r1);
+    const int count = (int)min((int64_t)ZERO_ROWS, r1 - b0);
     for (int i = tid; i < ZERO_ROWS / 32; i += SUM_THREADS) bits[i] = 0;
     __syncthreads();
     auto mark = [&](int64_t v) {
-      if (v >= b0 && v < b1 && v != a.pad) atomicOr(&bits[(v - b0) >> 5], 1u << ((v - b0) & 31));
+      if (v >= b0 && v < b0 + count && v != a.pad) atomicOr(&bits[(v - b0) >> 5], 1u << ((v - b0) & 31));
     };
 #pragma unroll 8
     for (int64_t t = tid; t < pairs; t += SUM_THREADS) {
@@ -413,16 +458,17 @@ __device__ void zero_rows(const GradArgs& a, uint32_t* bits) {
 #pragma unroll 8
     for (int64_t t = 2 * pairs + tid; t < a.n; t += SUM_THREADS) mark(row_of(a.ids, a.is64, t, a.vocab, a.pad));
     __syncthreads();
-    for (int64_t r = b0 + w; r < b1; r += SUM_THREADS / 32) {
-      if ((bits[(r - b0) >> 5] >> ((r - b0) & 31)) & 1) continue;
-      TO* o = static_cast<TO*>(a.out) + r * a.os;
-      int64_t c = 0;
-      if (vec) {
-        constexpr int PER = 16 / sizeof(TO);
-        for (c = lane * PER; c + PER <= a.dim; c += 32 * PER) *reinterpret_cast<uint4*>(o + c) = make_uint4(0, 0, 0, 0);
-        c = a.dim / PER * PER;
-      }
-      for (c += lane; c < a.dim; c += 32) st(o + c, 0.f);
+    for (int i = (tid >> 5) * rows_at_once + (lane >> a.zero_lanes); i < count; i += SUM_THREADS / 32 * rows_at_once) {
+      if ((bits[i >> 5] >> (i & 31)) & 1) continue;
+      TO* o = static_cast<TO*>(a.out) + (b0 + i) * a.os;
+      // values before the first 16-byte boundary, whole 16 bytes, and what is left
+      constexpr int PER = 16 / sizeof(TO);
+      const int dim = (int)a.dim, head = min((int)((0 - reinterpret_cast<uintptr_t>(o)) % 16 / sizeof(TO)), dim);
+      const int body = (dim - head) / PER;
+      uint4* q = reinterpret_cast<uint4*>(o + head);
+      for (int c = sub; c < body; c += step) q[c] = make_uint4(0, 0, 0, 0);
+      for (int c = sub; c < head; c += step) st(o + c, 0.f);
+      for (int c = head + body * PER + sub; c < dim; c += step) st(o + c, 0.f);
     }
     __syncthreads();
   }
@@ -594,7 +640,7 @@ cudaError_t grad_rows(const GradArgs& a, bool vec, cudaStream_t stream) {
 int64_t piece_len(int64_t n, int64_t dim) {
   // at most 2048 pieces, which bounds the parts' workspace; 32 rows, which a warp reads in a few
   // microseconds, unless that leaves most of the GPU without a warp: 777 x 768 f32 takes 20 us in
-  // pieces of 32 and 5 us in pieces of 4
+  // pieces of 32 and 6 us in pieces of 4
   const int64_t col_warps = (dim + SUM_COLS - 1) / SUM_COLS;
   int64_t len = 32;
   while ((n + len - 1) / len > 2048) len *= 2;
@@ -625,7 +671,7 @@ size_t embedding_grad_workspace(int64_t n, int64_t dim) {
 
 // (positions, pieces and columns are ints in the kernels: checked by the caller)
 cudaError_t launch_embedding_grad(const ssd_embedding_grad_params_t* p, void* workspace, cudaStream_t stream) {
-  GradArgs a;
+  GradArgs a{};
   a.n = p->num_tokens; a.vocab = p->vocab; a.dim = p->dim;
   a.gs = p->grad_stride_row; a.os = p->out_stride_row; a.pad = p->padding_idx;
   a.is64 = p->tokens_int64; a.accumulate = p->accumulate; a.scale = p->scale;
@@ -638,35 +684,47 @@ cudaError_t launch_embedding_grad(const ssd_embedding_grad_params_t* p, void* wo
   for (int i = 0; i < 2; ++i) a.list[i] = reinterpret_cast<uint2*>(ws + i * list);
   a.heavy = reinterpret_cast<int*>(ws + 2 * list);
   a.part = reinterpret_cast<float*>(ws + 2 * list + up256((size_t)(a.npieces + 1) * 4));
-  int bits = 1;
+  int bits = 1, shift = 1;
   while (((int64_t)1 << bits) <= a.vocab) ++bits;   // the largest key is V itself (dropped)
+  while (((int64_t)1 << shift) < a.n) ++shift;
   a.passes = (bits + SORT_BITS - 1) / SORT_BITS;
   a.bits = (bits + a.passes - 1) / a.passes;
   const bool gb = p->grad_dtype == SSD_DTYPE_BF16, ob = p->out_dtype == SSD_DTYPE_BF16;
-  const size_t smem = sizeof(SortShared);
-  static std::atomic<uint64_t> allowed{0};
-  cudaError_t e = allow_smem((const void*)sort_kernel, smem, &allowed);
-  if (e != cudaSuccess) return e;
-  a.zero_ctas = 0;
-  // one CTA where each warp has 32 ids at most (4 ids: 14 -> 12 us; 3237 ids took 6 us more in one)
-  const int ctas = a.n <= 32 * SORT_WARPS ? 1 : SORT_CTAS;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)ctas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(SORT_THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, sort_kernel, a);
+  cudaError_t e;
+  // (us by counting / by the cluster) 4 x 1395 x 71 6 / 12, 875 x 6111 x 128 12 / 21, 4096 x 2000 x 128 19 / 23,
+  // 8192 x 2000 x 128 29 / 28.  Where zero rows take longer than the sort, the counting's CTAs on every
+  // SM only hold them up: 2274 x 64120 x 223 f32 (57 MB) 24 / 27, 6000 x 50000 x 768 bf16 (77 MB) 35 / 31,
+  // 777 x 50257 x 768 f32 (154 MB) 35 / 34.
+  const int out_size = p->out_dtype == SSD_DTYPE_BF16 ? 2 : 4;
+  if (a.n <= RANK_MAX && bits + shift <= 32 && (a.accumulate || a.vocab * a.dim <= RANK_TABLE / out_size)) {
+    const int64_t ctas = std::min<int64_t>(148, std::max<int64_t>(1, (a.n + RANK_WARPS - 1) / RANK_WARPS));
+    rank_kernel<<<(unsigned)ctas, RANK_THREADS, (size_t)(a.n + 127) / 128 * 512, stream>>>(a, shift);
+    e = cudaGetLastError();
+  } else {
+    const size_t smem = sizeof(SortShared);
+    static std::atomic<uint64_t> allowed{0};
+    e = allow_smem((const void*)sort_kernel, smem, &allowed);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = SORT_CTAS;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(SORT_CTAS);
+    cfg.blockDim = dim3(SORT_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, sort_kernel, a);
+  }
   if (e != cudaSuccess) return e;
   // two of the four resident CTAs of an SM write zeros while the sort runs, the others wait for it;
   // all four where there are few sums
   const int64_t sum_ctas = (a.npieces * ((a.dim + SUM_COLS - 1) / SUM_COLS) + SUM_THREADS / 32 - 1) / (SUM_THREADS / 32);
   a.zero_ctas = a.accumulate ? 0 : 148 * 4 - (int)std::min<int64_t>(148 * 2, sum_ctas);
+  // a lane for every 16 bytes of a row (8192 ids, a table of 400000 x 64 bf16: 41 -> 29 us)
+  while (a.zero_lanes < 5 && ((int64_t)16 << a.zero_lanes) < a.dim * out_size) ++a.zero_lanes;
   if (a.accumulate && a.n == 0) return e;
   const bool vec = rows16(p->grad, a.gs, a.dim, p->grad_dtype) && rows16(p->out, a.os, a.dim, p->out_dtype);
   if (gb) return ob ? grad_rows<bf16, bf16>(a, vec, stream) : grad_rows<bf16, float>(a, vec, stream);

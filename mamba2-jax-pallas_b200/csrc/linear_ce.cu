@@ -16,6 +16,10 @@
 //              bytes of HBM per logit; computing them again would cost 2 D operations, more
 //              from D = 512 on.
 // f32 inputs are split into two f16 planes, three products per pair (tc_gemm.cuh).
+//
+// Measured: loss of 4096 x 131072 x 4096, bf16, 2.72 ms (1.62 PFLOP/s); gradients of 16384 x 50000 x 2560,
+// bf16, 9.5 ms of kernels (1.32 PFLOP/s): logits 3.04, dX 2.67, dW 2.81, rows 0.73, parts 0.14, the
+// rest 0.1; gradients of 2048 x 50257 x 768, f32, 1.2 ms (1.2 PFLOP/s of f16 products).
 #include <algorithm>
 
 #include <cuda_fp16.h>
@@ -41,7 +45,8 @@ constexpr int EC = gemm::EPI_COLS;
 // 7.6e-7 off (3 blocks 1.0e-6 and 3 % faster, 1 block 5.8e-7 and 3 % slower).
 constexpr int SEGMENT_BF16 = 8, SEGMENT_F32 = 2;
 constexpr int64_t LOSS_CHUNK = 16384;              // tokens whose statistics are kept at a time
-constexpr int64_t GRAD_BYTES = int64_t(3) << 30;   // logits and dl of a chunk of tokens
+// logits and dl of a chunk of tokens (16384 x 50000 x 2560: chunks of 1 GiB 9.6 ms, 3 GiB 9.5, 6 GiB 9.6)
+constexpr int64_t GRAD_BYTES = int64_t(3) << 30;
 
 size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 
@@ -78,7 +83,7 @@ struct Selected {
 };
 
 // One CTA; each warp owns a run of tokens and reads 32 at a time: count, one scan over the warps,
-// then the same again to write.
+// then the same again to write.  Latency-bound: 6 us for 2048 tokens, 13 us for 16384.
 __global__ void __launch_bounds__(1024) select_kernel(const void* targets, int is64, int64_t n, int64_t vocab,
                                                       int64_t ignore, int mean, const float* grad_loss,
                                                       const float* weights, Selected s, float* loss, float* lse) {
@@ -188,6 +193,7 @@ __device__ __forceinline__ bool vec_rows(const T* p, int64_t stride) {
 }
 
 // Largest finite magnitude of hidden's rows that count (blockIdx.y = 0) and of the weight (1).
+// Reads both once: 37 us for 50257 x 768 (4.3 TB/s).
 __global__ void __launch_bounds__(256) largest_kernel(const float* x, int64_t x_stride, int64_t tokens, const float* w,
                                                       int64_t w_stride, int64_t vocab, int64_t dim, const void* targets,
                                                       int is64, int64_t ignore, Scales* out) {
@@ -212,7 +218,7 @@ __global__ void __launch_bounds__(256) largest_kernel(const float* x, int64_t x_
 }
 
 // Planes of a whole matrix (the weight, where the tensor maps cannot read it as it is), a warp
-// per row and 256 columns.
+// per row and 256 columns.  HBM-bound: f32 50257 x 768 46 us (6.7 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256) planes_kernel(const T* src, int64_t stride, int64_t rows, int64_t dim,
                                                      int64_t ld, void* hi, void* lo, const unsigned* largest) {
@@ -228,7 +234,8 @@ __global__ void __launch_bounds__(256) planes_kernel(const T* src, int64_t strid
 }
 
 // Rows of hidden that count, side by side; zero rows up to the next 64 (a K block of the
-// weight's gradient).  blockIdx.y = 1: zero rows of grad_hidden for the ignored tokens.
+// weight's gradient).  blockIdx.y = 1: zero rows of grad_hidden for the ignored tokens.  HBM-bound:
+// bf16 16384 x 2560 35 us (4.8 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(128) gather_kernel(const T* src, int64_t stride, int64_t dim, int64_t ld, Selected s,
                                                      const void* targets, int is64, int64_t ignore, void* hi, void* lo,
@@ -373,7 +380,8 @@ struct Reduced {
 };
 
 // A warp per row that counts: its loss, and with `factors` what the gradients need.  The last CTA
-// of the last chunk reduces the losses, in a fixed order.
+// of the last chunk reduces the losses, in a fixed order.  Bound by the statistics' bytes: 8192 rows of
+// 784 statistics 26 us (2 TB/s, from L2), f64 sums included.
 __global__ void __launch_bounds__(256) loss_kernel(const float2* stats, int ns, const float* picked, Selected s, int from,
                                                    int rows, float* loss, float* lse, const float* weight, int split,
                                                    RowFactors* factors, const Reduced red) {
@@ -429,7 +437,8 @@ struct RowArgs {
 constexpr int ROW_THREADS = 256, ROW_UNROLL = 8, ROW_COLS = ROW_THREADS * 4 * ROW_UNROLL;
 
 // dl from the logits, ROW_COLS columns of a row per CTA, every load issued before the first use.
-// Zero rows up to the next 64.  HBM-bound: 6 bytes per logit (f32 inputs: 8).
+// Zero rows up to the next 64.  HBM-bound: 6 bytes per logit (f32 inputs: 8); 8192 x 50000 in 367 us
+// (6.7 TB/s).
 template <bool SPLIT>
 __global__ void __launch_bounds__(ROW_THREADS) row_kernel(const RowArgs a) {
   ptx::griddep_wait();
@@ -551,7 +560,7 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) grad_gemm_kernel(const __gri
 }
 
 // Sum of the parts of a split K range, in order, times alpha; nothing where it was not split.
-// CTAs take rows of the result in turns.
+// CTAs take rows of the result in turns.  HBM-bound: 70 us for the parts of 8192 x 2560.
 template <int CG, typename TO>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ gemm::Problem p, const __grid_constant__ OutArgs a) {
   ptx::griddep_wait();
