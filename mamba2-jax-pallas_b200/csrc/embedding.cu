@@ -187,7 +187,8 @@ constexpr int ZERO_ROWS = 8192;   // rows whose bits the bitmap holds at a time
 
 struct GradArgs {
   int64_t n, vocab, dim, gs, os, pad, piece, npieces;
-  int is64, passes, bits, accumulate, zero_ctas;   // `bits` of an id per pass
+  int is64, passes, bits, accumulate;   // `bits` of an id per pass
+  int zero_ctas, zero_first;      // CTAs that write zero rows; so many of them come before the sums' CTAs
   int zero_lanes;                 // lanes of a zero row, as a power of two
   int extend;                     // rows that a piece may take from the next one, at most a piece and 32
   float scale;
@@ -436,11 +437,11 @@ __device__ __forceinline__ void put_row(const GradArgs& a, uint32_t id, int64_t 
 // occur in a shared bitmap, ZERO_ROWS at a time, reading all ids (L2) once for each.  2^zero_lanes
 // lanes write a row.
 template <typename TO>
-__device__ void zero_rows(const GradArgs& a, uint32_t* bits) {
+__device__ void zero_rows(const GradArgs& a, int cta, uint32_t* bits) {
   const int tid = threadIdx.x, lane = tid & 31;
   const int rows_at_once = 32 >> a.zero_lanes, sub = lane & ((1 << a.zero_lanes) - 1), step = 1 << a.zero_lanes;
   const int64_t per = (a.vocab + a.zero_ctas - 1) / a.zero_ctas;
-  const int64_t r0 = blockIdx.x * per, r1 = min(r0 + per, a.vocab);
+  const int64_t r0 = cta * per, r1 = min(r0 + per, a.vocab);
   // two 64-bit ids at a time where they lie so
   const int64_t pairs = a.is64 && reinterpret_cast<uintptr_t>(a.ids) % 16 == 0 ? a.n / 2 : 0;
   for (int64_t b0 = r0; b0 < r1; b0 += ZERO_ROWS) {
@@ -477,19 +478,20 @@ __device__ void zero_rows(const GradArgs& a, uint32_t* bits) {
 }
 
 // HBM-bound: 32768 tokens into 131072 x 4096 bf16 232 us (5.8 TB/s), 777 into 50257 x 768 f32 27 us.
-// The first a.zero_ctas CTAs: zero rows.  Then a warp for each (piece p, 256 columns): rows of the
-// sorted positions [p * piece, + piece).
+// The first a.zero_first CTAs: zero rows.  Then a warp for each (piece p, 256 columns): rows of the
+// sorted positions [p * piece, + piece).  Then the other CTAs of zero rows.
 template <typename TG, typename TO, Cols M>
 __global__ void __launch_bounds__(SUM_THREADS, 4) grad_rows_kernel(const __grid_constant__ GradArgs a, int col_warps) {
   __shared__ uint32_t bits[ZERO_ROWS / 32];
-  if (blockIdx.x < a.zero_ctas) {
-    zero_rows<TO>(a, bits);
+  const int sum_ctas = (int)gridDim.x - a.zero_ctas, at = (int)blockIdx.x - a.zero_first;
+  if (at < 0 || at >= sum_ctas) {
+    zero_rows<TO>(a, at < 0 ? (int)blockIdx.x : (int)blockIdx.x - sum_ctas, bits);
     ptx::griddep_wait();   // what is launched behind may take the sort as done, too
     return;
   }
   using R = Raw<TG, M>;
   ptx::griddep_wait();
-  const int unit = (blockIdx.x - a.zero_ctas) * (SUM_THREADS / 32) + threadIdx.x / 32;
+  const int unit = at * (SUM_THREADS / 32) + threadIdx.x / 32;
   const int p = unit / col_warps;
   if (p >= (int)a.npieces) return;
   const int lane = threadIdx.x & 31, n = (int)a.n, top = n - 1, piece = (int)a.piece, extend = a.extend;
@@ -722,10 +724,18 @@ cudaError_t launch_embedding_grad(const ssd_embedding_grad_params_t* p, void* wo
     e = cudaLaunchKernelEx(&cfg, sort_kernel, a);
   }
   if (e != cudaSuccess) return e;
-  // two of the four resident CTAs of an SM write zeros while the sort runs, the others wait for it;
-  // all four where there are few sums
+  // Two of the four resident CTAs of an SM write zeros while the sort runs, the others wait for it;
+  // all four where there are few sums.  Where the table is large against the ids (which every CTA of
+  // zero rows reads), half of the zero rows or more come behind the sums, which would else leave their
+  // slots empty (us without / with): 5000 ids, 100000 x 1600 f32 132 / 118; 3000 ids, 131072 x 4096 bf16 201 /
+  // 185; 4000 ids, 60000 x 1216 f32 (292 MB) 61 / 58; but 777 ids, 50257 x 768 f32 (154 MB) 33 / 37; 32768 ids,
+  // 131072 x 4096 bf16 251 / 263.
   const int64_t sum_ctas = (a.npieces * ((a.dim + SUM_COLS - 1) / SUM_COLS) + SUM_THREADS / 32 - 1) / (SUM_THREADS / 32);
-  a.zero_ctas = a.accumulate ? 0 : 148 * 4 - (int)std::min<int64_t>(148 * 2, sum_ctas);
+  if (!a.accumulate) {
+    a.zero_first = 148 * 4 - (int)std::min<int64_t>(148 * 2, sum_ctas);
+    const bool large = a.vocab * a.dim * out_size / (148 * 8) >= std::max<int64_t>(4 * 8 * a.n, (256 << 20) / (148 * 8));
+    a.zero_ctas = large ? 148 * 8 : a.zero_first;
+  }
   // a lane for every 16 bytes of a row (8192 ids, a table of 400000 x 64 bf16: 41 -> 29 us)
   while (a.zero_lanes < 5 && ((int64_t)16 << a.zero_lanes) < a.dim * out_size) ++a.zero_lanes;
   if (a.accumulate && a.n == 0) return e;
