@@ -142,6 +142,39 @@ def test_embedding_grad_radix_edges(vocab):
 
 
 @gpu
+@pytest.mark.parametrize("n,vocab", [(5001, v) for v in (1, 2, 511, 512, 513, 1 << 18, (1 << 18) + 1)] +
+                         [(4096, 777), (4097, 777), (4096, (1 << 20) - 1), (4096, 1 << 20), (129, 5), (128, 1), (1, 3)])
+def test_embedding_grad_both_sorts(n, vocab):
+    """Few ids are placed by counting, more by digits: sizes on both sides of the change."""
+    g = torch.Generator().manual_seed(n)
+    ids = torch.randint(-1, vocab + 1, (n,), generator=g)
+    ids[0] = vocab - 1
+    x = rnd(n, 4, seed=8)
+    for t in (ids, ids.int()):
+        out = embedding_grad(t.cuda(), x.cuda(), vocab)
+        s, a, cnt = ref_embedding_grad(ids, x, vocab, 1.0)
+        assert ((f64(out) - s).abs() <= (cnt + 2) * U * a).all()
+
+
+@gpu
+@pytest.mark.parametrize("vocab,dim,od", [(1 << 19, 130, "f32"), (100001, 1367, "bf16"), (3000, 1, "bf16"), (3000, 7, "bf16"),
+                                          (3000, 9, "f32"), (3000, 33, "bf16"), (3000, 127, "f32")])
+def test_embedding_grad_zero_rows(vocab, dim, od):
+    """Every other row is written with zeros: wide and narrow rows, aligned or not, large tables."""
+    ids, x = ids_for("uniform", 300, vocab), rnd(300, dim, dtype=od, seed=9)
+    ic, xc = ids.cuda(), x.cuda()
+    torch.full((vocab, dim), float("nan"), device="cuda", dtype=DT[od])   # what the allocator hands out next
+    out = embedding_grad(ic, xc, vocab)
+    named = torch.zeros(vocab, dtype=torch.bool, device="cuda")
+    named[ic] = True
+    assert not out[~named].any() and not torch.isnan(out[~named]).any()
+    s, a, cnt = ref_embedding_grad(ids, x, vocab, 1.0)
+    bound = (cnt + 2) * U * a + (V * s.abs() if od == "bf16" else 0)
+    rows = ids.unique()
+    assert ((f64(out[rows.cuda()]) - s[rows]).abs() <= bound[rows]).all()
+
+
+@gpu
 def test_embedding_grad_large_sort_and_repeatable():
     """Several tokens per sorting lane, runs over many pieces; equal bits in every run."""
     ids, g = ids_for("zipf", 200001, 50000), rnd(200001, 24, dtype="bf16", seed=3)
