@@ -10,7 +10,8 @@
 //   2..17 epilogue: warp w reads the TMEM lanes of quadrant w % 4, 64 columns at (w - 2) / 4 * 64
 // (16 epilogue warps of 64 columns: with 8 of 128 the logits of 900 x 32003 x 1000 took 84 us, so 81.)
 // Bound by the tensor pipe where K is long: 4096 x 131072 x 4096 without a store takes 2.68 ms, 1.64
-// PFLOP/s, the pipe active 98 % of the cycles; by what an epilogue writes where K is short.
+// PFLOP/s (8192 x 50000 x 2560: the pipe active 98 % of the cycles); by what an epilogue writes where
+// K is short.
 // Two accumulators (2 x 256 TMEM columns) let the reading of one overlap the MMAs into the
 // other.  Operands are K-major (the reduced dimension contiguous in memory) or MN-major (the
 // other one contiguous), so no operand is ever transposed in memory.
@@ -158,7 +159,7 @@ __device__ __forceinline__ int splits_of(const Problem& p, int live) {
 // One thread of a converged warp.  The compiler knows that what this guards runs on one thread and
 // keeps descriptors and barrier addresses in uniform registers; under `lane == 0` four MMAs and
 // their commit took 335 + 66 cycles to issue, of the 512 that they take to run, and the tensor pipe
-// was busy 70 % of the time (85 % so: 8192 x 50000 x 2560, 1.55 -> 1.28 ms).
+// was busy 70 % of the time (85 % so: 8192 x 50000 x 2560, 1.52 -> 1.34 ms).
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
