@@ -16,7 +16,7 @@ _dtype = operator.attrgetter("dtype")
 # A model has hundreds of tensors, and the kernels take a few microseconds where they are
 # small: what is asked of each tensor goes through map() over the method itself.
 def _checked(ts, name):
-    """(list of tensors, their dtypes, their device index), or an error."""
+    """(list of tensors, the set of their dtypes, their device index), or an error."""
     ts = list(ts)
     if not ts:
         raise ValueError(f"{name} must not be empty")
@@ -28,8 +28,8 @@ def _checked(ts, name):
         raise ValueError(f"{name} must be CUDA tensors (no CPU path)")
     if len(devices) != 1:
         raise ValueError(f"{name} must be on one device")
-    dtypes = list(map(_dtype, ts))
-    for d in set(dtypes):
+    dtypes = set(map(_dtype, ts))
+    for d in dtypes:
         if d not in _DTYPE:
             raise TypeError(f"unsupported dtype {d} (float32 or bfloat16)")
     return ts, dtypes, devices.pop()
@@ -39,7 +39,11 @@ def _contiguous(ts):
     return ts if all(map(_T.is_contiguous, ts)) else [t.contiguous() for t in ts]
 
 
-def _run(grads, dtypes, outs, out_dtypes, max_norm, eps, scale):
+def _sizes(ts):
+    return array("q", map(_T.numel, ts))
+
+
+def _run(grads, dtypes, outs, out_dtypes, sizes, max_norm, eps, scale):
     dev = grads[0].device
     norm = torch.empty((), device=dev, dtype=torch.float32)
     # ssd_grad_tensor_t: two addresses, the size, two 32-bit dtypes
@@ -47,9 +51,12 @@ def _run(grads, dtypes, outs, out_dtypes, max_norm, eps, scale):
     rec = array("q", bytes(32 * n))
     rec[0::4] = array("q", map(_T.data_ptr, grads))
     rec[1::4] = rec[0::4] if outs is grads else array("q", map(_T.data_ptr, outs))
-    rec[2::4] = array("q", map(_T.numel, grads))
-    pairs = {(g, o): _DTYPE[g] | _DTYPE[o] << 32 for g, o in set(zip(dtypes, out_dtypes))}
-    rec[3::4] = array("q", map(pairs.__getitem__, zip(dtypes, out_dtypes)))
+    rec[2::4] = sizes
+    pairs = {(g, o): _DTYPE[g] | _DTYPE[o] << 32 for g in dtypes for o in out_dtypes}
+    if len(pairs) == 1:
+        rec[3::4] = array("q", pairs.values()) * n
+    else:
+        rec[3::4] = array("q", map(pairs.__getitem__, zip(map(_dtype, grads), map(_dtype, outs))))
     lib = _lib.load()
     addr = rec.buffer_info()[0]
     with _lib.on_device(dev):
@@ -65,7 +72,7 @@ def grad_norm(grads):
     scalar tensor.  Squares are summed in float64."""
     ts, dtypes, _ = _checked(grads, "grads")
     ts = _contiguous(ts)
-    return _run(ts, dtypes, ts, dtypes, 0.0, 0.0, False)
+    return _run(ts, dtypes, ts, dtypes, _sizes(ts), 0.0, 0.0, False)
 
 
 def clip_grad_norm(grads, max_norm: float, *, eps: float = 1e-6, out=None, inplace: bool = False):
@@ -80,6 +87,7 @@ def clip_grad_norm(grads, max_norm: float, *, eps: float = 1e-6, out=None, inpla
     ts, dtypes, device = _checked(grads, "grads")
     if not float(max_norm) >= 0.0 or not float(eps) >= 0.0:
         raise ValueError("max_norm and eps must be non-negative")
+    sizes = _sizes(ts)
     if inplace:
         if out is not None:
             raise ValueError("give either out or inplace=True")
@@ -91,11 +99,11 @@ def clip_grad_norm(grads, max_norm: float, *, eps: float = 1e-6, out=None, inpla
         if out is None:
             outs, out_dtypes = [torch.empty_like(g) for g in ts], dtypes
         else:
-            outs, out_dtypes, out_device = _checked(out, "out") if len(out) else ([], [], device)
+            outs, out_dtypes, out_device = _checked(out, "out") if len(out) else ([], set(), device)
             if len(outs) != len(ts):
                 raise ValueError(f"out has {len(outs)} tensors, grads {len(ts)}")
-            if list(map(_T.numel, outs)) != list(map(_T.numel, ts)) or not all(map(_T.is_contiguous, outs)):
+            if _sizes(outs) != sizes or not all(map(_T.is_contiguous, outs)):
                 raise ValueError("out must hold contiguous tensors of grads' sizes")
             if out_device != device:
                 raise ValueError("out and grads must be on one device")
-    return outs, _run(ts, dtypes, outs, out_dtypes, max_norm, eps, True)
+    return outs, _run(ts, dtypes, outs, out_dtypes, sizes, max_norm, eps, True)
