@@ -44,13 +44,20 @@ __device__ __forceinline__ RowResult warp_row(const float2* stats, int ns, const
     return r;
   }
   const double s = (double)*picked, d = anchor - s;
-  // others / e^s: the odds against the target
-  const double odds = others == 0.0 ? 0.0 : others * exp(d);
+  if (others == 0.0) {     // nothing but the target has mass: p is 1 whatever its logit
+    const bool ok = s > -INFINITY && s < INFINITY;
+    r.loss = r.pm1 = r.inv = ok ? 0.f : NAN;
+    r.lse = ok ? (float)s : NAN;
+    return r;
+  }
+  // others / e^s: the odds against the target; past e^600 they are infinite as far as f32 goes (s may
+  // be -inf, which leaves the others' sum alone)
+  const double odds = others * exp(d);
   const bool far = d > 600.0;
   double loss = far ? log(others) + d : log1p(odds);
   if (!(s < INFINITY)) loss = NAN;   // an infinite or NaN logit, as the formula has it
   r.loss = (float)loss;
-  r.lse = (float)(loss + s);
+  r.lse = (float)(far ? anchor + log(others) : loss + s);
   r.pm1 = (float)(!(s < INFINITY) ? NAN : far ? -1.0 : -odds / (1.0 + odds));
   r.inv = (float)(1.0 / (others + exp(-d)));
   return r;

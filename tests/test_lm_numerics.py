@@ -1,0 +1,96 @@
+"""Numerics of the language-model operators where they can lose digits: rows, words and tokens of very
+different size, confident and hopeless targets, long sums; each against float64, relative to itself.
+
+Inputs are multiples of a power of two and few enough bits long that every logit is exact in float32 (sums
+of integers below 2^24), so that what remains are the errors behind the logits.  u = 2^-24.
+
+Gradients, per element, against the sum A of the magnitudes of its terms (|dl| |W|, or |dl|^T |X|):
+- dl: exp2 (2 ulp: 2^-22), its argument (rounded: u |z|, and log2(e) as a float: u |z| / 2), the row's factor
+  (4 u);
+- two f16 terms per value: at most 2^-22 of it for each operand, and lo * lo: 3 * 2^-22 in all;
+- adds on the tensor cores: 24 in a segment of two K blocks, each cut by up to 2 u of the sum so far; one
+  rounded add per segment of 128 terms;
+- what a value more than 2^16 below the largest of its row or column lacks: 2^-39 of the largest, per term.
+"""
+import math
+
+import pytest
+import torch
+
+from mamba2_b200 import clip_grad_norm, embedding_grad, linear_cross_entropy, linear_cross_entropy_grad
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+DT = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(autouse=True)
+def _need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+
+
+def ints(shape, bits, seed, shift):
+    """Integers of `bits` bits (sign included) times 2^-shift, as float64."""
+    g = torch.Generator().manual_seed(seed)
+    return torch.randint(-2 ** (bits - 1), 2 ** (bits - 1), shape, generator=g).double() * 2.0 ** -shift
+
+
+def reference(x, w, y, coef):
+    """float64: losses, lse, dl (times coef per token)."""
+    s = x @ w.t()
+    lse = torch.logsumexp(s, 1)
+    rows = torch.arange(len(y))
+    dl = torch.exp(s - lse[:, None])
+    # p - 1 of the target from the others' sum, which keeps its digits where p is near 1
+    others = torch.where(torch.nn.functional.one_hot(y, w.shape[0]).bool(), torch.zeros_like(dl), dl).sum(1)
+    dl[rows, y] = -others
+    t = s[rows, y]
+    rest = s.clone()
+    rest[rows, y] = -math.inf
+    loss = torch.log1p(torch.exp(torch.logsumexp(rest, 1) - t))
+    return loss, lse, dl * coef[:, None], s
+
+
+def check_grad(got, dl, m, s):
+    """got against dl @ m, element by element."""
+    k = dl.shape[1]
+    z = float((s - s.max(1, keepdim=True).values).abs().max()) * 1.4427
+    c = 2.0 ** -22 + 1.5 * U * z + 4 * U + 3 * 2.0 ** -22 + 24 * 2 * U + (k / 128 + 1) * U + 4 * U
+    term = dl.abs().max(1, keepdim=True).values * m.abs().max()
+    bound = c * (dl.abs() @ m.abs()) + k * 2.0 ** -38 * term
+    err = (got.double().cpu() - dl @ m).abs()
+    assert (err <= bound).all(), float((err / bound).max())
+
+
+def grads(x, w, y, weights):
+    return linear_cross_entropy_grad(x.float().cuda(), w.float().cuda(), y.cuda(), reduction="none",
+                                     grad_loss=weights.float().cuda(), check_status=True)
+
+
+# ---- nothing but the target, and targets without mass -------------------------------------------
+@pytest.mark.parametrize("t", [1, 3, 40, 200])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("logit", [-1024.0, -3.0, 0.0, 512.0])
+def test_a_vocabulary_of_one_word(t, dtype, logit):
+    x, w = torch.full((t, 64), 4.0, dtype=DT[dtype]).cuda(), torch.full((1, 64), logit / 256, dtype=DT[dtype]).cuda()
+    y = torch.zeros(t, dtype=torch.int64).cuda()
+    loss, lse = linear_cross_entropy(x, w, y, reduction="none", return_lse=True)
+    assert (loss == 0).all() and (lse == logit).all()
+    loss, dx, dw = linear_cross_entropy_grad(x, w, y, reduction="sum")
+    assert float(loss) == 0 and (dx == 0).all() and (dw == 0).all()
+
+
+@pytest.mark.parametrize("t,dtype", [(1, "f32"), (5, "f32"), (1, "bf16"), (4, "bf16"), (40, "bf16"), (200, "bf16")])
+def test_target_logit_minus_infinity(t, dtype):
+    """The target has no mass: its loss is infinite, the log of the sum is that of the others."""
+    x, w = ints((t, 64), 8, 0, 7), ints((30, 64), 8, 1, 7)
+    x[:, 0] = 1.0
+    w[3] = 0.0
+    w[3, 0] = -math.inf
+    y = torch.full((t,), 3)
+    loss, lse = linear_cross_entropy(x.to(DT[dtype]).cuda(), w.to(DT[dtype]).cuda(), y.cuda(), reduction="none",
+                                     return_lse=True)
+    want = torch.logsumexp((x @ w.t())[:, [i for i in range(30) if i != 3]], 1)
+    assert (loss == math.inf).all()
+    assert ((lse.double().cpu() - want).abs() <= 2.0 ** -21 + 8 * U * (1 + want.abs())).all()
