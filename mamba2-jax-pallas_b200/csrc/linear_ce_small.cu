@@ -367,8 +367,14 @@ __global__ void __launch_bounds__(G_THREADS) small_grad_kernel(const __grid_cons
   }
   if (a.gx) {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (r < a.tokens) store4<float, VECTOR>(a.part + ((int64_t)range * a.tokens + r) * a.dim, c, a.dim, step, acc[r]);
+    for (int r = 0; r < R; ++r) {
+      if (r >= a.tokens) continue;
+      if (target_at(a.targets, a.is64, r) == a.ignore) {   // zero times an infinite or NaN weight is not zero
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[r][k] = 0.f;
+      }
+      store4<float, VECTOR>(a.part + ((int64_t)range * a.tokens + r) * a.dim, c, a.dim, step, acc[r]);
+    }
   }
 }
 

@@ -94,3 +94,16 @@ def test_target_logit_minus_infinity(t, dtype):
     want = torch.logsumexp((x @ w.t())[:, [i for i in range(30) if i != 3]], 1)
     assert (loss == math.inf).all()
     assert ((lse.double().cpu() - want).abs() <= 2.0 ** -21 + 8 * U * (1 + want.abs())).all()
+
+
+# ---- ignored rows -------------------------------------------------------------------------------
+@pytest.mark.parametrize("t", [2, 3, 8, 40])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_ignored_rows_have_no_gradient_whatever_the_weight_holds(t, dtype, bad):
+    x, w = ints((t, 64), 8, 0, 7).to(DT[dtype]).cuda(), ints((30, 64), 8, 1, 7).to(DT[dtype]).cuda()
+    w[7, 5] = bad
+    y = torch.arange(t).cuda()
+    y[0] = -100
+    _, dx, _ = linear_cross_entropy_grad(x, w, y)
+    assert (dx[0] == 0).all()
