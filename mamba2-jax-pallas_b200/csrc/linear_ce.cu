@@ -12,9 +12,9 @@
 //              confidence keeps the digits of 1 - p, which a sum with p in it would lose.
 //   gradients  tokens go in chunks whose logits fit a bounded workspace.  The same epilogue also
 //              stores the f32 logits; a row pass forms lse and dl (rounded once, to bf16, for
-//              the tensor pipe; f32 inputs: two f16); two GEMMs follow.  Keeping f32 logits for the chunk costs 10
-//              bytes of HBM per logit; computing them again would cost 2 D operations, more
-//              from D = 512 on.
+//              the tensor pipe; f32 inputs: two f16, in a pass for each product); two GEMMs follow.  Keeping
+//              f32 logits for the chunk costs 10 bytes of HBM per logit; computing them again would cost 2 D
+//              operations, more from D = 512 on.
 // f32 inputs are split into two f16 planes, three products per pair (tc_gemm.cuh).
 //
 // Measured: loss of 4096 x 131072 x 4096, bf16, 2.72 ms (1.62 PFLOP/s); gradients of 16384 x 50000 x 2560,
@@ -57,13 +57,17 @@ size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 // from them the powers of two that bring the planes' largest value to [2^14, 2^15): f16 ends at
 // 65504 below, and two planes keep 22 bits down to 2^-1.
 struct Scales {
-  unsigned x, w, dl;
+  unsigned x, w;
 };
 
 __device__ __forceinline__ float scale_of(unsigned largest) {
   const int e = (int)(largest >> 23);                       // biased exponent; 0 also for subnormals
   return e == 0 ? 1.f : __uint_as_float((unsigned)min(max(127 + 14 + 127 - e, 1), 254) << 23);
 }
+// The exponent of scale_of.
+__device__ __forceinline__ int shift_of(unsigned largest) { return (int)(__float_as_uint(scale_of(largest)) >> 23) - 127; }
+// 2^k; 0 below f32's normal numbers.
+__device__ __forceinline__ float pow2(int k) { return __uint_as_float((unsigned)min(max(k + 127, 0), 254) << 23); }
 __device__ __forceinline__ unsigned finite_bits(float v) {
   const unsigned u = __float_as_uint(v) & 0x7fffffffu;
   return u < 0x7f800000u ? u : 0u;
@@ -86,22 +90,13 @@ struct Selected {
 // then the same again to write.  Latency-bound: 6 us for 2048 tokens, 13 us for 16384.
 __global__ void __launch_bounds__(1024) select_kernel(const void* targets, int is64, int64_t n, int64_t vocab,
                                                       int64_t ignore, int mean, const float* grad_loss,
-                                                      const float* weights, Selected s, float* loss, float* lse) {
+                                                      Selected s, float* loss, float* lse) {
   __shared__ int sh[32];
-  __shared__ unsigned sh_largest;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  if (tid == 0) sh_largest = weights ? 0u : __float_as_uint(1.f);
-  __syncthreads();
   const int64_t per = (n + 1023) / 1024 * 32, lo = min(w * per, n), hi = min(lo + per, n);
   int mine = 0;
-  unsigned largest = 0;
 #pragma unroll 8
-  for (int64_t t = lo + lane; t < hi; t += 32) {
-    const bool counts = target_at(targets, is64, t) != ignore;
-    mine += counts;
-    if (weights && counts) largest = max(largest, finite_bits(weights[t]));
-  }
-  if (weights) atomicMax(&sh_largest, largest);
+  for (int64_t t = lo + lane; t < hi; t += 32) mine += target_at(targets, is64, t) != ignore;
   mine = __reduce_add_sync(0xffffffffu, mine);
   if (lane == 0) sh[w] = mine;
   __syncthreads();
@@ -130,7 +125,6 @@ __global__ void __launch_bounds__(1024) select_kernel(const void* targets, int i
     *s.ticket = 0;
     *s.count = total;
     s.scales->x = s.scales->w = 0;
-    s.scales->dl = sh_largest;
     *s.alpha = (mean ? (float)(1.0 / (double)max(total, 1)) : 1.f) * (grad_loss ? *grad_loss : 1.f);
   }
 }
@@ -379,12 +373,53 @@ struct Reduced {
   int ctas;                // of loss_kernel, over all chunks
 };
 
-// A warp per row that counts: its loss, and with `factors` what the gradients need.  The last CTA
-// of the last chunk reduces the losses, in a fixed order.  Bound by the statistics' bytes: 8192 rows of
+// f32 inputs: what dl is made of.  A row's values may lie anywhere between 1e-38 and the largest
+// grad_loss, and f16 has five bits of exponent, so every factor is kept as a number and a power of two.
+struct SplitRow {
+  float top;               // p of another column than the target's: f 2^(fe + s log2(e) - top)
+  float f, y;              // 1 <= |f| < 2, or zero, or not finite; y 2^ye is dl of the target
+  int fe, ye;
+};
+
+struct SplitOut {
+  SplitRow* rows;          // of the chunk
+  int* row_shift;          // powers of two for dX: a row's largest |dl| 2^shift is in (2^12, 2^14]
+  int* col_top;            // (ld): cleared here (see split_kernel)
+  int64_t vocab;
+};
+
+constexpr int NO_TOP = -(1 << 20);   // of a column in which dl is zero
+
+// Powers of two that split_kernel and the products agree on.
+__device__ __forceinline__ int row_shift_of(int top) { return top == NO_TOP ? 0 : min(max(14 - top, -120), 240); }
+__device__ __forceinline__ int col_shift_of(int top) { return top == NO_TOP ? 0 : min(max(14 - top, -120), 180); }
+
+__device__ __forceinline__ float split2(double v, int* e) {
+  *e = 0;
+  if (v == 0.0 || !isfinite(v)) return (float)v;
+  const double m = frexp(v, e);
+  *e -= 1;
+  return (float)(2.0 * m);   // may round up to 2: the bounds below have room for it
+}
+
+__device__ __forceinline__ void put_split(const SplitOut& o, int64_t row, const RowResult& r, double w) {
+  SplitRow q;
+  q.top = r.top;
+  q.f = split2(w * (double)r.inv, &q.fe);
+  q.y = split2(w * (double)r.pm1, &q.ye);
+  int top = NO_TOP;        // |dl| <= 2^top
+  if (q.f != 0.f) top = q.fe + 1;
+  if (q.y != 0.f) top = max(top, q.ye + 1);
+  o.rows[row] = q;
+  o.row_shift[row] = row_shift_of(top);
+}
+
+// A warp per row that counts: its loss, and with `factors` or `split` what the gradients need.  The last
+// CTA of the last chunk reduces the losses, in a fixed order.  Bound by the statistics' bytes: 8192 rows of
 // 784 statistics 26 us (2 TB/s, from L2), f64 sums included.
 __global__ void __launch_bounds__(256) loss_kernel(const float2* stats, int ns, const float* picked, Selected s, int from,
-                                                   int rows, float* loss, float* lse, const float* weight, int split,
-                                                   RowFactors* factors, const Reduced red) {
+                                                   int rows, float* loss, float* lse, const float* weight,
+                                                   RowFactors* factors, const SplitOut split, const Reduced red) {
   ptx::griddep_wait();
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row < rows && from + row < *s.count) {
@@ -393,12 +428,13 @@ __global__ void __launch_bounds__(256) loss_kernel(const float2* stats, int ns, 
       const int t = s.index[from + row];
       loss[t] = r.loss;
       if (lse) lse[t] = r.lse;
-      if (factors) {
-        const float w = (weight ? weight[t] : 1.f) * (split ? scale_of(s.scales->dl) : 1.f);
-        factors[row] = {r.top, w * r.inv, w * r.pm1};
-      }
+      const float w = weight ? weight[t] : 1.f;
+      if (factors) factors[row] = {r.top, w * r.inv, w * r.pm1};
+      if (split.rows) put_split(split, row, r, (double)w);
     }
   }
+  if (split.rows)
+    for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < split.vocab; v += (int64_t)gridDim.x * 256) split.col_top[v] = NO_TOP;
   if (!red.out) return;
   __shared__ int last;
   __shared__ double sh[8];
@@ -431,15 +467,13 @@ struct RowArgs {
   int from;                // first of the rows that count, of this chunk
   const RowFactors* factors;
   const float* logits;
-  void* dl[2];             // (rows, ld): bf16, or two f16 planes of dl times its scale
+  bf16* dl;                // (rows, ld)
 };
 
 constexpr int ROW_THREADS = 256, ROW_UNROLL = 8, ROW_COLS = ROW_THREADS * 4 * ROW_UNROLL;
 
 // dl from the logits, ROW_COLS columns of a row per CTA, every load issued before the first use.
-// Zero rows up to the next 64.  HBM-bound: 6 bytes per logit (f32 inputs: 8); 8192 x 50000 in 367 us
-// (6.7 TB/s).
-template <bool SPLIT>
+// Zero rows up to the next 64.  HBM-bound: 6 bytes per logit; 8192 x 50000 in 367 us (6.7 TB/s).
 __global__ void __launch_bounds__(ROW_THREADS) row_kernel(const RowArgs a) {
   ptx::griddep_wait();
   const int64_t row = blockIdx.x;
@@ -457,8 +491,7 @@ __global__ void __launch_bounds__(ROW_THREADS) row_kernel(const RowArgs a) {
   const int y = counted ? a.sel.target[a.from + row] : -1;
   RowFactors r = {0.f, 0.f, 0.f};
   if (counted) r = a.factors[row];
-  uint2* hi = reinterpret_cast<uint2*>(static_cast<bf16*>(a.dl[0]) + row * a.ld);
-  uint2* lo = SPLIT ? reinterpret_cast<uint2*>(static_cast<__half*>(a.dl[1]) + row * a.ld) : nullptr;
+  uint2* out = reinterpret_cast<uint2*>(a.dl + row * a.ld);
 #pragma unroll
   for (int u = 0; u < ROW_UNROLL; ++u) {
     const int64_t c = c0 + u * ROW_THREADS * 4;
@@ -473,16 +506,139 @@ __global__ void __launch_bounds__(ROW_THREADS) row_kernel(const RowArgs a) {
       for (int k = 0; k < 4; ++k)
         if (c + k == y) d[k] = r.at_y;
     }
-    if constexpr (SPLIT) {
-      __half2 h[2] = {__floats2half2_rn(d[0], d[1]), __floats2half2_rn(d[2], d[3])};
-      const float2 g0 = __half22float2(h[0]), g1 = __half22float2(h[1]);
-      __half2 l[2] = {__floats2half2_rn(d[0] - g0.x, d[1] - g0.y), __floats2half2_rn(d[2] - g1.x, d[3] - g1.y)};
-      hi[c / 4] = *reinterpret_cast<uint2*>(h);
-      lo[c / 4] = *reinterpret_cast<uint2*>(l);
-    } else {
-      __nv_bfloat162 h[2] = {__floats2bfloat162_rn(d[0], d[1]), __floats2bfloat162_rn(d[2], d[3])};
-      hi[c / 4] = *reinterpret_cast<uint2*>(h);
+    const __nv_bfloat162 h[2] = {__floats2bfloat162_rn(d[0], d[1]), __floats2bfloat162_rn(d[2], d[3])};
+    out[c / 4] = *reinterpret_cast<const uint2*>(h);
+  }
+}
+
+// f32 inputs: dl as two f16 planes, hi + lo, times a power of two that belongs to what the product
+// keeps apart: to a row for dX = dl W, where every token's gradient stands for itself, and to a
+// column for dW = dl^T X, where every word's does.  (One power for all of dl lost the rows of small
+// grad_loss, of confident tokens and of improbable words.)  So the logits are read twice, 16 bytes per logit
+// in all, HBM-bound: 2048 x 50257 in 138 + 131 us (6.1 TB/s).
+//   ROWS      planes for dX; with MAX also each column's largest |dl|, as a power of two
+//   MAX alone the latter, where grad_hidden is not wanted
+//   COLS      planes for dW, over the ones for dX
+// A column's maximum is that of integers, so the order in which CTAs add to it changes nothing.
+struct SplitArgs {
+  int64_t vocab, ld;
+  Selected sel;
+  int from, n, per;        // first of the rows that count; rows of the chunk; rows of a CTA, 64 at most
+  unsigned col_blocks;
+  const SplitRow* rows;
+  const int* row_shift;
+  int* col_top;            // (ld): |dl| <= 2^col_top in this column, NO_TOP where dl is zero
+  const float* logits;
+  __half* hi;
+  __half* lo;
+};
+
+enum Planes { ROWS = 1, MAX = 2, COLS = 4 };
+constexpr int SPLIT_THREADS = 256, SPLIT_COLS = 4 * SPLIT_THREADS, SPLIT_ROWS = 64, SPLIT_AHEAD = 8;
+
+template <int WHAT>
+__global__ void __launch_bounds__(SPLIT_THREADS) split_kernel(const SplitArgs a) {
+  struct Row {
+    float top, f;          // the factor as a number and a power of two, and (ff) as one number
+    int k;
+    float ff, mf;          // mf: what it adds to a column's maximum, as a power of two
+    int target, ky;        // the same of the target's column, if it has one
+    float y, my;
+  };
+  __shared__ Row rows[SPLIT_ROWS];
+  ptx::griddep_wait();
+  const unsigned rb = blockIdx.x / a.col_blocks, cb = blockIdx.x - rb * a.col_blocks;
+  const int live = min(*a.sel.count - a.from, a.n), first = (int)rb * a.per;
+  const int end = min(min(first + a.per, a.n), WHAT == MAX ? live : (live + 63) / 64 * 64);
+  if (live <= 0 || first >= end) return;
+  const int tid = threadIdx.x;
+  if (tid < end - first) {
+    const int row = first + tid;
+    Row q = {0.f, 0.f, 0, 0.f, -INFINITY, -1, 0, 0.f, -INFINITY};   // a row that does not count: zeros
+    if (row < live) {
+      const SplitRow r = a.rows[row];
+      const int shift = (WHAT & ROWS) != 0 ? a.row_shift[row] : 0;
+      q.top = r.top; q.f = r.f; q.y = r.y;
+      q.target = a.sel.target[a.from + row];
+      q.k = r.fe + shift; q.ky = r.ye + shift;
+      q.ff = r.f * pow2(q.k);
+      if (r.f != 0.f) q.mf = (float)(r.fe + 1);
+      if (r.y != 0.f) q.my = (float)(r.ye + 1);
     }
+    rows[tid] = q;
+  }
+  __syncthreads();
+  const int64_t c = (int64_t)cb * SPLIT_COLS + tid * 4;
+  if (c >= a.vocab) return;      // (rows of logits and planes are ld long, a multiple of 64)
+  int shift[4] = {0, 0, 0, 0};
+  if constexpr ((WHAT & COLS) != 0) {
+    const int4 q = *reinterpret_cast<const int4*>(a.col_top + c);
+    shift[0] = col_shift_of(q.x); shift[1] = col_shift_of(q.y); shift[2] = col_shift_of(q.z); shift[3] = col_shift_of(q.w);
+  }
+  // Columns whose largest |dl| is above 2^-86 hold nothing below f32's normal numbers that an f16 of them
+  // could keep: plain products.  For the others the exponential's argument takes 64 of the shift, which
+  // is exact there, z being as far below.
+  const bool plain = max(max(shift[0], shift[1]), max(shift[2], shift[3])) <= 100;
+  const float cs[4] = {pow2(shift[0]), pow2(shift[1]), pow2(shift[2]), pow2(shift[3])};
+  float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  for (int r0 = first; r0 < end; r0 += SPLIT_AHEAD) {
+    float4 x[SPLIT_AHEAD];
+#pragma unroll
+    for (int j = 0; j < SPLIT_AHEAD; ++j)
+      x[j] = r0 + j < min(end, live) ? *reinterpret_cast<const float4*>(a.logits + (int64_t)(r0 + j) * a.ld + c)
+                                     : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < SPLIT_AHEAD; ++j) {
+      if (r0 + j >= end) break;
+      const Row& r = rows[r0 + j - first];
+      const int at_y = r.target - (int)c;
+      float z[4] = {fmaf(x[j].x, LOG2E, -r.top), fmaf(x[j].y, LOG2E, -r.top), fmaf(x[j].z, LOG2E, -r.top), fmaf(x[j].w, LOG2E, -r.top)};
+      float d[4];
+      if constexpr ((WHAT & (ROWS | COLS)) != 0) {
+        if constexpr ((WHAT & ROWS) != 0) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d[i] = r.ff * exp2f(z[i]);
+        } else if (plain) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d[i] = r.ff * exp2f(z[i]) * cs[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = r.k + shift[i];
+            d[i] = k > 100 ? r.f * exp2f(z[i] + 64.f) * pow2(k - 64) : r.f * exp2f(z[i]) * pow2(k);
+          }
+        }
+      }
+      if constexpr ((WHAT & MAX) != 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z[i] += r.mf;
+      }
+      if ((unsigned)at_y < 4u && r.target >= 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i == at_y) {
+            if constexpr ((WHAT & (ROWS | COLS)) != 0) d[i] = r.y * pow2(r.ky + shift[i]);
+            z[i] = r.my;
+          }
+      }
+      if constexpr ((WHAT & MAX) != 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most[i] = fmaxf(most[i], z[i]);
+      }
+      if constexpr ((WHAT & (ROWS | COLS)) != 0) {
+        const int64_t at = (int64_t)(r0 + j) * a.ld + c;
+        const __half2 h[2] = {__floats2half2_rn(d[0], d[1]), __floats2half2_rn(d[2], d[3])};
+        const float2 g0 = __half22float2(h[0]), g1 = __half22float2(h[1]);
+        const __half2 l[2] = {__floats2half2_rn(d[0] - g0.x, d[1] - g0.y), __floats2half2_rn(d[2] - g1.x, d[3] - g1.y)};
+        *reinterpret_cast<uint2*>(a.hi + at) = *reinterpret_cast<const uint2*>(h);
+        *reinterpret_cast<uint2*>(a.lo + at) = *reinterpret_cast<const uint2*>(l);
+      }
+    }
+  }
+  if constexpr ((WHAT & MAX) != 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i < a.vocab && most[i] > -INFINITY) atomicMax(a.col_top + c + i, (int)ceilf(fminf(fmaxf(most[i], -1000.f), 1000.f)));
   }
 }
 
@@ -494,7 +650,11 @@ struct OutArgs {
   const float* alpha;
   float* part;             // f32: parts of a split K range (splits, rows, cols), or the running sum
   int sum, add_part;       // `part` is the running sum over chunks of tokens; add what it holds
-  const unsigned* largest[2];   // f32 inputs: what the operands' scales come from
+  // f32 inputs: the powers of two to take out again.  Of dl for each row of the result: row_shift, or
+  // col_shift_of(col_top); of the other operand: what `largest` gives.
+  const int* row_shift;
+  const int* col_top;
+  const unsigned* largest;
 };
 
 // OUT: tiles go to the output, times alpha.  PART: to f32 parts where the K range is split, or to
@@ -507,9 +667,10 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) grad_gemm_kernel(const __gri
                                                                      const __grid_constant__ OutArgs a) {
   extern __shared__ uint8_t smem[];
   __shared__ gemm::Ctl ctl;
-  float unscale = 1.f, alpha = 1.f;
+  int shift = 0;
+  float alpha = 1.f;
   auto prep = [&]() {
-    if (PLANES == 2) unscale = 1.f / scale_of(*a.largest[0]) / scale_of(*a.largest[1]);
+    if (PLANES == 2) shift = shift_of(*a.largest);
     alpha = *a.alpha;
   };
   gemm::run<CG, PLANES, A_MN, true>(p, smem, &ctl, prep, [&](const gemm::Tile& t, float (&v)[EC], int row0, int n0, int live,
@@ -517,9 +678,18 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) grad_gemm_kernel(const __gri
     const int64_t all = p.limit_k ? a.rows : live;
     const int rows = (int)min((int64_t)32, all - row0), cols = (int)min((int64_t)EC, a.cols - n0);
     if (rows <= 0 || cols <= 0) return;
-    const float f = MODE == OUT ? unscale * alpha : unscale;
+    if constexpr (PLANES == 2) {
+      const int row = row0 + min((int)(threadIdx.x & 31), rows - 1);
+      const int e = shift + (A_MN ? col_shift_of(a.col_top[row]) : a.row_shift[row]);
+      // in two steps: the whole power may lie outside f32
+      const float f0 = pow2(-(e / 2)), f1 = pow2(-(e - e / 2));
 #pragma unroll
-    for (int i = 0; i < EC; ++i) v[i] *= f;
+      for (int i = 0; i < EC; ++i) v[i] = v[i] * f0 * f1;
+    }
+    if constexpr (MODE == OUT) {
+#pragma unroll
+      for (int i = 0; i < EC; ++i) v[i] *= alpha;
+    }
     TO* out = static_cast<TO*>(a.out) + n0;
     auto row_at = [&](int i) { return out + (int64_t)(a.index ? a.index[row0 + i] : row0 + i) * a.cols; };
     bool vec = vec_rows(out, a.cols) && cols % (16 / (int)sizeof(TO)) == 0;
@@ -629,7 +799,7 @@ struct Plan {
   int64_t chunk, nchunks, ns, ld;   // tokens of a chunk; statistics per row; logits' row length
   int64_t part_x, part_w;           // values that the parts of split K ranges may take (0: no split)
   bool pack_w, sum_w;       // sum_w: dW's running sum over chunks needs its own f32 buffer
-  size_t one, index, target, rows, picked, factors, stats, x, w, logits, dl[2], part, wsum, total;
+  size_t one, index, target, rows, picked, factors, row_shift, col_top, stats, x, w, logits, dl[2], part, wsum, total;
 };
 
 Plan plan_of(const ssd_linear_ce_params_t* p) {
@@ -665,7 +835,10 @@ Plan plan_of(const ssd_linear_ce_params_t* p) {
   q.target = take((size_t)p->tokens * 4);
   q.rows = take(p->reduction == SSD_REDUCE_NONE ? 0 : (size_t)p->tokens * 4);
   q.picked = take((size_t)q.chunk * 4);
-  q.factors = take(q.grad ? (size_t)q.chunk * sizeof(RowFactors) : 0);
+  const bool split = q.grad && q.planes == 2;
+  q.factors = take(q.grad ? (size_t)q.chunk * (split ? sizeof(SplitRow) : sizeof(RowFactors)) : 0);
+  q.row_shift = take(split ? (size_t)q.chunk * 4 : 0);
+  q.col_top = take(split ? (size_t)q.ld * 4 : 0);
   q.stats = take((size_t)q.chunk * q.ns * 8);
   q.x = take(planes_bytes(p->tokens, p->dim, p->dtype));
   q.w = take(q.pack_w ? planes_bytes(p->vocab, p->dim, p->dtype) : 0);
@@ -687,6 +860,17 @@ Plan plan_of(const ssd_linear_ce_params_t* p) {
       return e_;                                                  \
     }                                                             \
   } while (0)
+
+// Rows of a CTA: 64, a round of atomics per column, and fewer where that would leave SMs without a CTA.
+template <int WHAT>
+cudaError_t launch_split(SplitArgs a, cudaStream_t st) {
+  a.col_blocks = (unsigned)cdiv(a.vocab, SPLIT_COLS);
+  a.per = SPLIT_ROWS;
+  while (a.per > SPLIT_AHEAD && (int64_t)a.col_blocks * cdiv(a.n, a.per) < 4 * SMS) a.per /= 2;
+  const int64_t ctas = (int64_t)a.col_blocks * cdiv(a.n, a.per);
+  if (ctas >= (int64_t(1) << 31)) return cudaErrorInvalidValue;
+  return launch_dependent(split_kernel<WHAT>, dim3((unsigned)ctas), SPLIT_THREADS, 0, 1, st, a);
+}
 
 template <int CG>
 cudaError_t logits_gemm(const Operand& x, const Operand& w, int planes, LogitArgs a, const int* count, int from,
@@ -774,7 +958,7 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
   const bool bf = p->dtype == SSD_DTYPE_BF16, mean = p->reduction == SSD_REDUCE_MEAN;
   const bool per_row = p->reduction == SSD_REDUCE_NONE && p->grad_loss;
   select_kernel<<<1, 1024, 0, st>>>(p->targets, p->targets_int64, p->tokens, p->vocab, p->ignore_index, mean,
-                                    per_row ? nullptr : p->grad_loss, per_row ? p->grad_loss : nullptr, sel, rows, p->lse);
+                                    per_row ? nullptr : p->grad_loss, sel, rows, p->lse);
   cudaError_t err = cudaGetLastError();
   CE_CHECK(err, "select");
   Operand x{}, w{};
@@ -840,36 +1024,52 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
     // of 200 tokens, in two rows of tiles: 78, by pairs 71)
     if (n > BM) CE_CHECK(logits_gemm<2>(xc, w, q.planes, a, sel.count, from, status, st), "logits");
     else CE_CHECK(logits_gemm<1>(xc, w, q.planes, a, sel.count, from, status, st), "logits");
-    RowFactors* factors = q.grad ? reinterpret_cast<RowFactors*>(ws + q.factors) : nullptr;
+    RowFactors* factors = q.grad && bf ? reinterpret_cast<RowFactors*>(ws + q.factors) : nullptr;
+    SplitOut split{};
+    if (q.grad && !bf) {
+      split.rows = reinterpret_cast<SplitRow*>(ws + q.factors);
+      split.row_shift = reinterpret_cast<int*>(ws + q.row_shift);
+      split.col_top = reinterpret_cast<int*>(ws + q.col_top);
+      split.vocab = p->vocab;
+    }
     err = launch_dependent(loss_kernel, (unsigned)cdiv(n, 8), 256, 0, 1, st, a.stats, a.ns, a.picked, sel, from, (int)n, rows, p->lse,
-                                                     per_row ? p->grad_loss : nullptr, q.planes == 2, factors, red);
+                                                     per_row ? p->grad_loss : nullptr, factors, split, red);
     CE_CHECK(err, "loss");
     if (!q.grad) continue;
-    RowArgs r{};
-    r.vocab = p->vocab; r.ld = q.ld; r.sel = sel; r.from = from; r.factors = factors; r.logits = a.logits;
-    for (int i = 0; i < q.planes; ++i) r.dl[i] = ws + q.dl[i];
-    const dim3 row_grid((unsigned)n, (unsigned)cdiv(p->vocab, ROW_COLS));
-    if (q.planes == 2) err = launch_dependent(row_kernel<true>, row_grid, ROW_THREADS, 0, 1, st, r);
-    else err = launch_dependent(row_kernel<false>, row_grid, ROW_THREADS, 0, 1, st, r);
-    CE_CHECK(err, "rows");
+    SplitArgs sp{};
+    if (bf) {
+      RowArgs r{};
+      r.vocab = p->vocab; r.ld = q.ld; r.sel = sel; r.from = from; r.factors = factors; r.logits = a.logits;
+      r.dl = reinterpret_cast<bf16*>(ws + q.dl[0]);
+      CE_CHECK(launch_dependent(row_kernel, dim3((unsigned)n, (unsigned)cdiv(p->vocab, ROW_COLS)), ROW_THREADS, 0, 1, st, r), "rows");
+    } else {
+      sp.vocab = p->vocab; sp.ld = q.ld; sp.sel = sel; sp.from = from; sp.n = (int)n;
+      sp.rows = split.rows; sp.row_shift = split.row_shift; sp.col_top = split.col_top; sp.logits = a.logits;
+      sp.hi = reinterpret_cast<__half*>(ws + q.dl[0]);
+      sp.lo = reinterpret_cast<__half*>(ws + q.dl[1]);
+      CE_CHECK(p->grad_hidden ? p->grad_weight ? launch_split<ROWS | MAX>(sp, st) : launch_split<ROWS>(sp, st)
+                              : launch_split<MAX>(sp, st), "rows");
+    }
     Operand dl{};
     dl.rows = n; dl.dim = p->vocab; dl.ld = q.ld;
-    for (int i = 0; i < q.planes; ++i) dl.plane[i] = r.dl[i];
+    for (int i = 0; i < q.planes; ++i) dl.plane[i] = ws + q.dl[i];
     OutArgs o{};
     o.alpha = sel.alpha;
-    o.largest[0] = &sel.scales->dl;
+    o.row_shift = split.row_shift;
+    o.col_top = split.col_top;
     o.part = reinterpret_cast<float*>(ws + q.part);
     if (p->grad_hidden) {
       OutArgs ox = o;
       ox.rows = n; ox.cols = p->dim; ox.index = sel.index + t0; ox.out = p->grad_hidden;
-      ox.largest[1] = &sel.scales->w;
+      ox.largest = &sel.scales->w;
       CE_CHECK(grad_gemm_as<false>(n > BM, bf, dl, w, p->vocab, q.planes, q.part_x, ox, sel.count, from, status, st),
                "grad_hidden");
     }
     if (p->grad_weight) {
+      if (!bf) CE_CHECK(launch_split<COLS>(sp, st), "columns");
       OutArgs ow = o;
       ow.rows = p->vocab; ow.cols = p->dim;
-      ow.largest[1] = &sel.scales->x;
+      ow.largest = &sel.scales->x;
       if (q.sum_w) ow.part = reinterpret_cast<float*>(ws + q.wsum);
       ow.sum = q.sum_w;
       ow.add_part = c > 0;

@@ -96,6 +96,51 @@ def test_target_logit_minus_infinity(t, dtype):
     assert ((lse.double().cpu() - want).abs() <= 2.0 ** -21 + 8 * U * (1 + want.abs())).all()
 
 
+# ---- gradients of the logits over many powers of ten --------------------------------------------
+@pytest.mark.parametrize("t", [7, 40, 200, 700])
+@pytest.mark.parametrize("decades", [12, 25])
+def test_token_weights_over_decades(t, decades):
+    x, w = ints((t, 64), 8, 0, 7), ints((513, 64), 8, 1, 7)
+    g = torch.Generator().manual_seed(2)
+    y = torch.randint(0, 513, (t,), generator=g)
+    weights = (10.0 ** (-decades * torch.rand(t, generator=g).double())).float().double()
+    weights[0] = 1.0
+    _, dx, dw = grads(x, w, y, weights)
+    _, _, dl, s = reference(x, w, y, weights)
+    check_grad(dx, dl, w, s)
+    check_grad(dw, dl.t(), x, s)
+
+
+@pytest.mark.parametrize("t", [8, 40, 200])
+def test_confident_rows_keep_their_gradient(t):
+    """1 - p of the target from 0.9 down to 1e-12."""
+    w = ints((300, 64), 8, 1, 8)
+    y = torch.randint(0, 300, (t,), generator=torch.Generator().manual_seed(2))
+    x = w[y] * (1 + torch.arange(t).remainder(8)).double()[:, None]
+    one = torch.ones(t, dtype=torch.float64)
+    loss, dx, _ = grads(x, w, y, one)
+    ref, lse, dl, s = reference(x, w, y, one)
+    assert float(dl.abs().sum(1).min()) < 1e-11
+    check_grad(dx, dl, w, s)
+    e = 2.0 ** -22 + 1.5 * U * float(s.max() - s.min()) * 1.4427 + 8 * U
+    assert ((loss.double().cpu() - ref).abs() <= e * ref).all()
+
+
+@pytest.mark.parametrize("t", [8, 40, 200, 700])
+def test_improbable_words_keep_their_gradient(t):
+    """Words with a probability below 1e-12 for every token: their rows of grad_weight, relative to themselves."""
+    x, w = ints((t, 64), 8, 0, 7), ints((300, 64), 8, 1, 7)
+    x[:, :32] = 127.0 / 128
+    w[:40, :32] = -127.0 / 128
+    y = torch.randint(40, 300, (t,), generator=torch.Generator().manual_seed(2))
+    one = torch.ones(t, dtype=torch.float64)
+    _, dx, dw = grads(x, w, y, one)
+    _, _, dl, s = reference(x, w, y, one)
+    assert float(dl[:, :40].max()) < 1e-12
+    check_grad(dx, dl, w, s)
+    check_grad(dw, dl.t(), x, s)
+
+
 # ---- ignored rows -------------------------------------------------------------------------------
 @pytest.mark.parametrize("t", [2, 3, 8, 40])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
