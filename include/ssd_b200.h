@@ -393,8 +393,11 @@ typedef enum ssd_reduction {
  * [0, vocab) makes its loss NaN (and the gradients it takes part in).
  * bf16 inputs: products on the tensor cores with f32 accumulation; the gradient of the logits
  * is rounded once to bf16 as an operand of the products behind it.  f32 inputs: every operand
- * as two f16 terms of its values times a power of two (22 bits down to 2^-16 of the operand's
- * largest value), three products per pair.  For a few tokens (f32: 32, with gradients 8; bf16: 4
+ * as two f16 terms of its values times a power of two (22 bits down to 2^-16 of the largest value
+ * that shares the power), three products per pair.  A row of hidden or of weight has a power of its
+ * own, and so has a row of either result, so no token and no word takes digits from another; rows
+ * whose largest value is below 2^-98 count as zero, and an infinite value makes the logits that it
+ * takes part in NaN.  For a few tokens (f32: 32, with gradients 8; bf16: 4
  * or 8, with gradients 2) the products run in f32 on the CUDA cores. */
 typedef struct ssd_linear_ce_params {
   int64_t tokens, vocab, dim;

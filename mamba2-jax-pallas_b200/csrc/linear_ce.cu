@@ -53,21 +53,22 @@ size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 // ---------------------------------------------------------------------------
 // the tokens that count
 // ---------------------------------------------------------------------------
-// f32 inputs: the largest finite magnitudes (as the bits of a float, which order like it), and
-// from them the powers of two that bring the planes' largest value to [2^14, 2^15): f16 ends at
-// 65504 below, and two planes keep 22 bits down to 2^-1.
-struct Scales {
-  unsigned x, w;
-};
-
-__device__ __forceinline__ float scale_of(unsigned largest) {
+// f32 inputs: a row of hidden or of the weight has a power of two that brings its largest finite
+// magnitude (as the bits of a float, which order like it) to [2^14, 2^15): f16 ends at 65504, and two
+// planes keep 22 bits down to 2^-1.  Rows have one each, so that a large row takes no digits from the
+// others; the powers come out again in the logits' epilogue, and go into dl where a product runs over
+// the rows.
+__device__ __forceinline__ int shift_of(unsigned largest) {
   const int e = (int)(largest >> 23);                       // biased exponent; 0 also for subnormals
-  return e == 0 ? 1.f : __uint_as_float((unsigned)min(max(127 + 14 + 127 - e, 1), 254) << 23);
+  return e == 0 ? 0 : min(127 + 14 - e, 126);
 }
-// The exponent of scale_of.
-__device__ __forceinline__ int shift_of(unsigned largest) { return (int)(__float_as_uint(scale_of(largest)) >> 23) - 127; }
 // 2^k; 0 below f32's normal numbers.
 __device__ __forceinline__ float pow2(int k) { return __uint_as_float((unsigned)min(max(k + 127, 0), 254) << 23); }
+// Logits of f32 inputs stay times a power of two that belongs to their row until log2(e) multiplies them;
+// 14 of the 28 that the two operands' powers have beyond their values, so that neither part leaves f32
+// (a word or row below 2^-98 throughout counts as zero).
+__device__ __forceinline__ float logit_scale(int x_shift) { return pow2(14 - x_shift); }
+__device__ __forceinline__ float word_scale(int w_shift) { return pow2(-14 - w_shift); }
 __device__ __forceinline__ unsigned finite_bits(float v) {
   const unsigned u = __float_as_uint(v) & 0x7fffffffu;
   return u < 0x7f800000u ? u : 0u;
@@ -83,7 +84,6 @@ struct Selected {
   float* alpha;            // the factor common to all rows: 1 or 1 / count, times a scalar grad_loss
   unsigned* status;        // the workspace's status word
   int* ticket;
-  Scales* scales;
 };
 
 // One CTA; each warp owns a run of tokens and reads 32 at a time: count, one scan over the warps,
@@ -124,7 +124,6 @@ __global__ void __launch_bounds__(1024) select_kernel(const void* targets, int i
     *s.status = 0;
     *s.ticket = 0;
     *s.count = total;
-    s.scales->x = s.scales->w = 0;
     *s.alpha = (mean ? (float)(1.0 / (double)max(total, 1)) : 1.f) * (grad_loss ? *grad_loss : 1.f);
   }
 }
@@ -186,54 +185,59 @@ __device__ __forceinline__ bool vec_rows(const T* p, int64_t stride) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * sizeof(T) % 16 == 0;
 }
 
-// Largest finite magnitude of hidden's rows that count (blockIdx.y = 0) and of the weight (1).
-// Reads both once: 37 us for 50257 x 768 (4.3 TB/s).
-__global__ void __launch_bounds__(256) largest_kernel(const float* x, int64_t x_stride, int64_t tokens, const float* w,
-                                                      int64_t w_stride, int64_t vocab, int64_t dim, const void* targets,
-                                                      int is64, int64_t ignore, Scales* out) {
-  ptx::griddep_wait();
-  const bool of_w = blockIdx.y == 1;
-  const float* src = of_w ? w : x;
-  const int64_t stride = of_w ? w_stride : x_stride, rows = of_w ? vocab : tokens;
+// The lane's share of the largest finite magnitude of a row, for `lanes` lanes of which this is `lane`.
+__device__ __forceinline__ unsigned largest_of(const float* row, int64_t dim, bool vec, int lane, int lanes) {
   unsigned m = 0;
-  const bool vec = vec_rows(src, stride);
-  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
-    if (!of_w && target_at(targets, is64, r) == ignore) continue;
 #pragma unroll 4
-    for (int64_t c = (threadIdx.x & 31) * 8; c < dim; c += 256) {
-      float v[8];
-      load8(src + r * stride, c, dim, vec, v);
+  for (int64_t c = lane * 8; c < dim; c += lanes * 8) {
+    float v[8];
+    load8(row, c, dim, vec, v);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) m = max(m, finite_bits(v[k]));
-    }
+    for (int k = 0; k < 8; ++k) m = max(m, finite_bits(v[k]));
   }
-  m = __reduce_max_sync(0xffffffffu, m);
-  if ((threadIdx.x & 31) == 0 && m) atomicMax(of_w ? &out->w : &out->x, m);
+  return m;
 }
 
-// Planes of a whole matrix (the weight, where the tensor maps cannot read it as it is), a warp
-// per row and 256 columns.  HBM-bound: f32 50257 x 768 46 us (6.7 TB/s).
-template <typename T>
-__global__ void __launch_bounds__(256) planes_kernel(const T* src, int64_t stride, int64_t rows, int64_t dim,
-                                                     int64_t ld, void* hi, void* lo, const unsigned* largest) {
+// The weight where the tensor maps cannot read it as it is.  bf16: the same values, 256 columns of a row a
+// warp at a time.
+__global__ void __launch_bounds__(256) repack_kernel(const bf16* src, int64_t stride, int64_t rows, int64_t dim, int64_t ld,
+                                                     void* out) {
   ptx::griddep_wait();
-  const float scale = scale_of(*largest);
   const bool vec = vec_rows(src, stride);
   const int64_t runs = (ld + 255) / 256, n = rows * runs;
 #pragma unroll 2
   for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < n; u += (int64_t)gridDim.x * 8) {
     const int64_t r = u / runs, c = (u - r * runs) * 256 + (threadIdx.x & 31) * 8;
-    if (c < ld) planes8(src + r * stride, c, dim, vec, scale, hi, lo, r * ld + c);
+    if (c < ld) planes8(src + r * stride, c, dim, vec, 1.f, out, nullptr, r * ld + c);
+  }
+}
+
+// f32: two planes and a power of two per row, a warp per row, whose second reading comes from L1.
+__global__ void __launch_bounds__(256) planes_kernel(const float* src, int64_t stride, int64_t rows, int64_t dim, int64_t ld,
+                                                     void* hi, void* lo, float* shift, float* unscale) {
+  ptx::griddep_wait();
+  const int lane = threadIdx.x & 31;
+  const bool vec = vec_rows(src, stride);
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
+    const float* row = src + r * stride;
+    const int e = shift_of(__reduce_max_sync(0xffffffffu, largest_of(row, dim, vec, lane, 32)));
+    if (lane == 0) {
+      shift[r] = (float)e;
+      unscale[r] = word_scale(e);
+    }
+    const float scale = pow2(e);
+#pragma unroll 4
+    for (int64_t c = lane * 8; c < ld; c += 256) planes8(row, c, dim, vec, scale, hi, lo, r * ld + c);
   }
 }
 
 // Rows of hidden that count, side by side; zero rows up to the next 64 (a K block of the
-// weight's gradient).  blockIdx.y = 1: zero rows of grad_hidden for the ignored tokens.  HBM-bound:
-// bf16 16384 x 2560 35 us (4.8 TB/s).
+// weight's gradient).  f32: a power of two per row.  blockIdx.y = 1: zero rows of grad_hidden for the
+// ignored tokens.  HBM-bound: bf16 16384 x 2560 35 us (4.8 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(128) gather_kernel(const T* src, int64_t stride, int64_t dim, int64_t ld, Selected s,
                                                      const void* targets, int is64, int64_t ignore, void* hi, void* lo,
-                                                     T* grad_hidden) {
+                                                     int* shift, T* grad_hidden) {
   ptx::griddep_wait();
   const int64_t r = blockIdx.x;
   if (blockIdx.y == 1) {
@@ -244,8 +248,17 @@ __global__ void __launch_bounds__(128) gather_kernel(const T* src, int64_t strid
   const int64_t count = *s.count;
   if (r >= (count + 63) / 64 * 64) return;
   const T* x = src + (r < count ? s.index[r] : 0) * stride;
-  const float scale = scale_of(s.scales->x);
   const bool vec = vec_rows(src, stride);
+  float scale = 1.f;
+  if constexpr (sizeof(T) == 4) {
+    __shared__ unsigned sh[4];
+    const unsigned m = __reduce_max_sync(0xffffffffu, largest_of(x, r < count ? dim : 0, vec, threadIdx.x, 128));
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = m;
+    __syncthreads();
+    const int e = shift_of(max(max(sh[0], sh[1]), max(sh[2], sh[3])));
+    if (threadIdx.x == 0) shift[r] = e;
+    scale = pow2(e);
+  }
 #pragma unroll 2
   for (int64_t c = threadIdx.x * 8; c < ld; c += 128 * 8)
     planes8(x, r < count ? c : dim, dim, vec, scale, hi, lo, r * ld + c);
@@ -281,11 +294,24 @@ struct LogitArgs {
   int ns;                  // statistics per row: one for each 64 columns
   float2* stats;           // (rows, ns), target left out: maximum * log2(e), sum of 2^(s log2(e) - that)
   float* picked;           // (rows): the target's logit
-  float* logits;           // (rows, ld) or NULL
+  float* logits;           // (rows, ld) or NULL; f32 inputs: over logit_scale of their row
   int64_t ld;
-  const Scales* scales;
+  // f32 inputs: the rows' and the words' powers of two, the latter as numbers and as word_scale (readable up
+  // to the tile's end), and with `peak` (rows, ns) the largest s log2(e) - w_shift of each 64 columns, the
+  // target left out
+  const int* x_shift;
+  const float* w_shift;
+  const float* w_scale;
+  float* peak;
   CUtensorMap map;         // of the logits, 32 x 32 values a box (pairs)
 };
+
+// Four values from L1.  Volatile: a tile's 64 shifts, kept from one use to the next, would spill.
+__device__ __forceinline__ float4 load_again(const float* p) {
+  float4 q;
+  asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(q.x), "=f"(q.y), "=f"(q.z), "=f"(q.w) : "l"(p));
+  return q;
+}
 
 // Half a warp's 32 x 64 block to global memory: through its 4 KB of shared memory, in the layout
 // of a swizzled box, by one bulk store (f32, 2048 x 50257 x 768: the kernel takes 370 us where
@@ -313,18 +339,20 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) logits_kernel(const __grid_c
                                                                   const __grid_constant__ LogitArgs a) {
   extern __shared__ uint8_t smem[];
   __shared__ gemm::Ctl ctl;
-  float unscale = 1.f;
-  auto prep = [&]() {
-    if (PLANES == 2) unscale = 1.f / scale_of(a.scales->x) / scale_of(a.scales->w);
-  };
-  gemm::run<CG, PLANES, false, false>(p, smem, &ctl, prep, [&](const gemm::Tile& t, float (&v)[EC], int row0, int n0, int live,
+  gemm::run<CG, PLANES, false, false>(p, smem, &ctl, [] {}, [&](const gemm::Tile& t, float (&v)[EC], int row0, int n0, int live,
                                                        int, uint4* stage) {
     const int row = row0 + (threadIdx.x & 31);
     const int y = row < live ? a.target[row] : -1;
-    if (PLANES == 2) {
+    float scale = 1.f;
+    if constexpr (PLANES == 2) {
+      if (row < live) scale = logit_scale(a.x_shift[row]);
 #pragma unroll
-      for (int i = 0; i < EC; ++i) v[i] *= unscale;
+      for (int i = 0; i < EC; i += 4) {
+        const float4 q = load_again(a.w_scale + n0 + i);
+        v[i] *= q.x; v[i + 1] *= q.y; v[i + 2] *= q.z; v[i + 3] *= q.w;
+      }
     }
+    const float to_log2 = PLANES == 2 ? LOG2E * scale : LOG2E;
     // the logits' rows are a multiple of 64 long
     if (CG == 2) {
       if (a.logits && row0 < live && n0 < a.vocab) {
@@ -349,16 +377,28 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) logits_kernel(const __grid_c
         s = y == n0 + i ? v[i] : s;
         v[i] = y == n0 + i ? -INFINITY : v[i];
       }
-      a.picked[row] = s;
+      a.picked[row] = PLANES == 2 ? s * scale : s;
+    }
+    if constexpr (PLANES == 2) {
+      if (a.peak) {
+        float k = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < EC; i += 4) {
+          const float4 q = load_again(a.w_shift + n0 + i);
+          k = fmaxf(fmaxf(k, fmaf(v[i], to_log2, -q.x)), fmaf(v[i + 1], to_log2, -q.y));
+          k = fmaxf(fmaxf(k, fmaf(v[i + 2], to_log2, -q.z)), fmaf(v[i + 3], to_log2, -q.w));
+        }
+        if (row < live) a.peak[(int64_t)row * a.ns + n0 / EC] = k;
+      }
     }
     float m[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
     for (int i = 4; i < EC; ++i) m[i & 3] = fmaxf(m[i & 3], v[i]);
     // the anchor is the rounded product itself, so that what is stored says what was summed
-    const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * LOG2E, at = top == -INFINITY ? 0.f : top;
+    const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * to_log2, at = top == -INFINITY ? 0.f : top;
     float e[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < EC; ++i) e[i & 3] += exp2f(fmaf(v[i], LOG2E, -at));
+    for (int i = 0; i < EC; ++i) e[i & 3] += exp2f(fmaf(v[i], to_log2, -at));
     if (row < live) a.stats[(int64_t)row * a.ns + n0 / (EC)] = make_float2(top, (e[0] + e[1]) + (e[2] + e[3]));
   });
   if (CG == 2) ptx::bulk_wait_all();
@@ -383,15 +423,16 @@ struct SplitRow {
 
 struct SplitOut {
   SplitRow* rows;          // of the chunk
-  int* row_shift;          // powers of two for dX: a row's largest |dl| 2^shift is in (2^12, 2^14]
+  int* row_shift;          // powers of two for dX: a row's largest |dl| 2^(shift - w_shift) is in (2^12, 2^14]
   int* col_top;            // (ld): cleared here (see split_kernel)
+  const float* peak;       // NULL where grad_hidden is not wanted
+  const float* w_shift;
   int64_t vocab;
 };
 
 constexpr int NO_TOP = -(1 << 20);   // of a column in which dl is zero
 
 // Powers of two that split_kernel and the products agree on.
-__device__ __forceinline__ int row_shift_of(int top) { return top == NO_TOP ? 0 : min(max(14 - top, -120), 240); }
 __device__ __forceinline__ int col_shift_of(int top) { return top == NO_TOP ? 0 : min(max(14 - top, -120), 180); }
 
 __device__ __forceinline__ float split2(double v, int* e) {
@@ -402,16 +443,19 @@ __device__ __forceinline__ float split2(double v, int* e) {
   return (float)(2.0 * m);   // may round up to 2: the bounds below have room for it
 }
 
-__device__ __forceinline__ void put_split(const SplitOut& o, int64_t row, const RowResult& r, double w) {
+// `peak`: of the row.
+__device__ __forceinline__ void put_split(const SplitOut& o, int64_t row, const RowResult& r, double w, float peak, int target) {
   SplitRow q;
   q.top = r.top;
   q.f = split2(w * (double)r.inv, &q.fe);
   q.y = split2(w * (double)r.pm1, &q.ye);
-  int top = NO_TOP;        // |dl| <= 2^top
-  if (q.f != 0.f) top = q.fe + 1;
-  if (q.y != 0.f) top = max(top, q.ye + 1);
   o.rows[row] = q;
-  o.row_shift[row] = row_shift_of(top);
+  if (!o.peak) return;
+  int top = NO_TOP;        // |dl| 2^-w_shift <= 2^top
+  if (q.f != 0.f && peak > -INFINITY) top = q.fe + 1 + (int)ceilf(fminf(fmaxf(peak - r.top, -1000.f), 1000.f));
+  if (q.y != 0.f && target >= 0) top = max(top, q.ye + 1 - (int)o.w_shift[target]);
+  // f 2^(fe + shift) has to be a normal number (it would not be where all of the weight is below 1e-33)
+  o.row_shift[row] = top == NO_TOP ? 0 : min(min(max(14 - top, -240), 240), 126 - q.fe);
 }
 
 // A warp per row that counts: its loss, and with `factors` or `split` what the gradients need.  The last
@@ -423,14 +467,21 @@ __global__ void __launch_bounds__(256) loss_kernel(const float2* stats, int ns, 
   ptx::griddep_wait();
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row < rows && from + row < *s.count) {
-    const RowResult r = warp_row(stats + row * ns, ns, picked + row, s.target[from + row]);
+    const int target = s.target[from + row];
+    const RowResult r = warp_row(stats + row * ns, ns, picked + row, target);
+    float peak = -INFINITY;
+    if (split.peak) {
+      for (int i = threadIdx.x & 31; i < ns; i += 32) peak = fmaxf(peak, split.peak[row * ns + i]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+    }
     if ((threadIdx.x & 31) == 0) {
       const int t = s.index[from + row];
       loss[t] = r.loss;
       if (lse) lse[t] = r.lse;
       const float w = weight ? weight[t] : 1.f;
       if (factors) factors[row] = {r.top, w * r.inv, w * r.pm1};
-      if (split.rows) put_split(split, row, r, (double)w);
+      if (split.rows) put_split(split, row, r, (double)w, peak, target);
     }
   }
   if (split.rows)
@@ -514,7 +565,8 @@ __global__ void __launch_bounds__(ROW_THREADS) row_kernel(const RowArgs a) {
 // f32 inputs: dl as two f16 planes, hi + lo, times a power of two that belongs to what the product
 // keeps apart: to a row for dX = dl W, where every token's gradient stands for itself, and to a
 // column for dW = dl^T X, where every word's does.  (One power for all of dl lost the rows of small
-// grad_loss, of confident tokens and of improbable words.)  So the logits are read twice, 16 bytes per logit
+// grad_loss, of confident tokens and of improbable words.)  The other operand's rows have powers of their
+// own (shift_of), which a product over these rows takes from dl.  So the logits are read twice, 16 bytes per logit
 // in all, HBM-bound: 2048 x 50257 in 138 + 131 us (6.1 TB/s).
 //   ROWS      planes for dX; with MAX also each column's largest |dl|, as a power of two
 //   MAX alone the latter, where grad_hidden is not wanted
@@ -527,7 +579,9 @@ struct SplitArgs {
   unsigned col_blocks;
   const SplitRow* rows;
   const int* row_shift;
-  int* col_top;            // (ld): |dl| <= 2^col_top in this column, NO_TOP where dl is zero
+  int* col_top;            // (ld): |dl| 2^-x_shift <= 2^col_top in this column, NO_TOP where dl is zero
+  const int* x_shift;      // of the chunk's rows of hidden
+  const float* w_shift;    // (ld)
   const float* logits;
   __half* hi;
   __half* lo;
@@ -539,7 +593,8 @@ constexpr int SPLIT_THREADS = 256, SPLIT_COLS = 4 * SPLIT_THREADS, SPLIT_ROWS = 
 template <int WHAT>
 __global__ void __launch_bounds__(SPLIT_THREADS) split_kernel(const SplitArgs a) {
   struct Row {
-    float top, f;          // the factor as a number and a power of two, and (ff) as one number
+    float to_log2, top;
+    float f;               // the factor as a number and a power of two, and (ff) as one number
     int k;
     float ff, mf;          // mf: what it adds to a column's maximum, as a power of two
     int target, ky;        // the same of the target's column, if it has one
@@ -554,16 +609,17 @@ __global__ void __launch_bounds__(SPLIT_THREADS) split_kernel(const SplitArgs a)
   const int tid = threadIdx.x;
   if (tid < end - first) {
     const int row = first + tid;
-    Row q = {0.f, 0.f, 0, 0.f, -INFINITY, -1, 0, 0.f, -INFINITY};   // a row that does not count: zeros
+    Row q = {0.f, 0.f, 0.f, 0, 0.f, -INFINITY, -1, 0, 0.f, -INFINITY};   // a row that does not count: zeros
     if (row < live) {
       const SplitRow r = a.rows[row];
-      const int shift = (WHAT & ROWS) != 0 ? a.row_shift[row] : 0;
+      const int x_shift = a.x_shift[row], shift = (WHAT & ROWS) != 0 ? a.row_shift[row] : -x_shift;
+      q.to_log2 = LOG2E * logit_scale(x_shift);
       q.top = r.top; q.f = r.f; q.y = r.y;
       q.target = a.sel.target[a.from + row];
       q.k = r.fe + shift; q.ky = r.ye + shift;
-      q.ff = r.f * pow2(q.k);
-      if (r.f != 0.f) q.mf = (float)(r.fe + 1);
-      if (r.y != 0.f) q.my = (float)(r.ye + 1);
+      q.ff = q.k > 127 ? r.f * INFINITY : r.f * pow2(q.k);
+      if (r.f != 0.f) q.mf = (float)(r.fe + 1 - x_shift);
+      if (r.y != 0.f) q.my = (float)(r.ye + 1 - x_shift);
     }
     rows[tid] = q;
   }
@@ -574,10 +630,13 @@ __global__ void __launch_bounds__(SPLIT_THREADS) split_kernel(const SplitArgs a)
   if constexpr ((WHAT & COLS) != 0) {
     const int4 q = *reinterpret_cast<const int4*>(a.col_top + c);
     shift[0] = col_shift_of(q.x); shift[1] = col_shift_of(q.y); shift[2] = col_shift_of(q.z); shift[3] = col_shift_of(q.w);
+  } else if constexpr ((WHAT & ROWS) != 0) {
+    const float4 q = *reinterpret_cast<const float4*>(a.w_shift + c);
+    shift[0] = -(int)q.x; shift[1] = -(int)q.y; shift[2] = -(int)q.z; shift[3] = -(int)q.w;
   }
-  // Columns whose largest |dl| is above 2^-86 hold nothing below f32's normal numbers that an f16 of them
+  // Columns whose largest |dl| (with the row's power) is above 2^-86 hold nothing below f32's normal numbers that an f16 of them
   // could keep: plain products.  For the others the exponential's argument takes 64 of the shift, which
-  // is exact there, z being as far below.
+  // is exact there, z being as far below; from a shift of 190 on p is below 1e-52.
   const bool plain = max(max(shift[0], shift[1]), max(shift[2], shift[3])) <= 100;
   const float cs[4] = {pow2(shift[0]), pow2(shift[1]), pow2(shift[2]), pow2(shift[3])};
   float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -592,12 +651,13 @@ __global__ void __launch_bounds__(SPLIT_THREADS) split_kernel(const SplitArgs a)
       if (r0 + j >= end) break;
       const Row& r = rows[r0 + j - first];
       const int at_y = r.target - (int)c;
-      float z[4] = {fmaf(x[j].x, LOG2E, -r.top), fmaf(x[j].y, LOG2E, -r.top), fmaf(x[j].z, LOG2E, -r.top), fmaf(x[j].w, LOG2E, -r.top)};
+      float z[4] = {fmaf(x[j].x, r.to_log2, -r.top), fmaf(x[j].y, r.to_log2, -r.top), fmaf(x[j].z, r.to_log2, -r.top),
+                    fmaf(x[j].w, r.to_log2, -r.top)};
       float d[4];
       if constexpr ((WHAT & (ROWS | COLS)) != 0) {
         if constexpr ((WHAT & ROWS) != 0) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) d[i] = r.ff * exp2f(z[i]);
+          for (int i = 0; i < 4; ++i) d[i] = r.ff * exp2f(z[i]) * cs[i];
         } else if (plain) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) d[i] = r.ff * exp2f(z[i]) * cs[i];
@@ -605,7 +665,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS) split_kernel(const SplitArgs a)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int k = r.k + shift[i];
-            d[i] = k > 100 ? r.f * exp2f(z[i] + 64.f) * pow2(k - 64) : r.f * exp2f(z[i]) * pow2(k);
+            d[i] = k > 190 ? 0.f : k > 100 ? r.f * exp2f(z[i] + 64.f) * pow2(k - 64) : r.f * exp2f(z[i]) * pow2(k);
           }
         }
       }
@@ -650,11 +710,10 @@ struct OutArgs {
   const float* alpha;
   float* part;             // f32: parts of a split K range (splits, rows, cols), or the running sum
   int sum, add_part;       // `part` is the running sum over chunks of tokens; add what it holds
-  // f32 inputs: the powers of two to take out again.  Of dl for each row of the result: row_shift, or
-  // col_shift_of(col_top); of the other operand: what `largest` gives.
+  // f32 inputs: the power of two to take out again of each row of the result is row_shift, or
+  // col_shift_of(col_top)
   const int* row_shift;
   const int* col_top;
-  const unsigned* largest;
 };
 
 // OUT: tiles go to the output, times alpha.  PART: to f32 parts where the K range is split, or to
@@ -667,12 +726,8 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) grad_gemm_kernel(const __gri
                                                                      const __grid_constant__ OutArgs a) {
   extern __shared__ uint8_t smem[];
   __shared__ gemm::Ctl ctl;
-  int shift = 0;
   float alpha = 1.f;
-  auto prep = [&]() {
-    if (PLANES == 2) shift = shift_of(*a.largest);
-    alpha = *a.alpha;
-  };
+  auto prep = [&]() { alpha = *a.alpha; };
   gemm::run<CG, PLANES, A_MN, true>(p, smem, &ctl, prep, [&](const gemm::Tile& t, float (&v)[EC], int row0, int n0, int live,
                                                      int splits, uint4* stage) {
     const int64_t all = p.limit_k ? a.rows : live;
@@ -680,7 +735,7 @@ __global__ void __launch_bounds__(gemm::THREADS, 1) grad_gemm_kernel(const __gri
     if (rows <= 0 || cols <= 0) return;
     if constexpr (PLANES == 2) {
       const int row = row0 + min((int)(threadIdx.x & 31), rows - 1);
-      const int e = shift + (A_MN ? col_shift_of(a.col_top[row]) : a.row_shift[row]);
+      const int e = A_MN ? col_shift_of(a.col_top[row]) : a.row_shift[row];
       // in two steps: the whole power may lie outside f32
       const float f0 = pow2(-(e / 2)), f1 = pow2(-(e - e / 2));
 #pragma unroll
@@ -799,7 +854,7 @@ struct Plan {
   int64_t chunk, nchunks, ns, ld;   // tokens of a chunk; statistics per row; logits' row length
   int64_t part_x, part_w;           // values that the parts of split K ranges may take (0: no split)
   bool pack_w, sum_w;       // sum_w: dW's running sum over chunks needs its own f32 buffer
-  size_t one, index, target, rows, picked, factors, row_shift, col_top, stats, x, w, logits, dl[2], part, wsum, total;
+  size_t one, index, target, rows, picked, factors, row_shift, col_top, stats, peak, x, w, x_shift, w_shift, w_scale, logits, dl[2], part, wsum, total;
 };
 
 Plan plan_of(const ssd_linear_ce_params_t* p) {
@@ -840,8 +895,13 @@ Plan plan_of(const ssd_linear_ce_params_t* p) {
   q.row_shift = take(split ? (size_t)q.chunk * 4 : 0);
   q.col_top = take(split ? (size_t)q.ld * 4 : 0);
   q.stats = take((size_t)q.chunk * q.ns * 8);
+  q.peak = take(split && p->grad_hidden ? (size_t)q.chunk * q.ns * 4 : 0);
   q.x = take(planes_bytes(p->tokens, p->dim, p->dtype));
   q.w = take(q.pack_w ? planes_bytes(p->vocab, p->dim, p->dtype) : 0);
+  q.x_shift = take(q.planes == 2 ? (size_t)p->tokens * 4 : 0);
+  const size_t words = q.planes == 2 ? (size_t)cdiv(p->vocab, BN) * BN * 4 : 0;   // whole tiles
+  q.w_shift = take(words);
+  q.w_scale = take(words);
   if (q.grad) {
     q.logits = take((size_t)q.chunk * q.ld * 4);
     for (int i = 0; i < q.planes; ++i) q.dl[i] = take((size_t)q.chunk * q.ld * 2);
@@ -950,7 +1010,6 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
   sel.status = status;
   sel.count = reinterpret_cast<int*>(ws + q.one);
   sel.alpha = reinterpret_cast<float*>(ws + q.one) + 1;
-  sel.scales = reinterpret_cast<Scales*>(ws + q.one + 16);
   sel.ticket = reinterpret_cast<int*>(ws + q.one + 32);
   sel.index = reinterpret_cast<int*>(ws + q.index);
   sel.target = reinterpret_cast<int*>(ws + q.target);
@@ -968,20 +1027,16 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
   void* hi = const_cast<void*>(x.plane[0]);
   void* lo = const_cast<void*>(x.plane[1]);
   const unsigned wide = 148 * 8;
-  if (!bf) {
-    err = launch_dependent(largest_kernel, dim3((unsigned)std::min<int64_t>(cdiv(std::max(p->vocab, p->tokens), 8), wide), 2), 256, 0, 1,
-                           st, static_cast<const float*>(p->hidden), p->hidden_stride_row, p->tokens,
-                           static_cast<const float*>(p->weight), p->weight_stride_row, p->vocab, p->dim, p->targets,
-                           p->targets_int64, p->ignore_index, sel.scales);
-    CE_CHECK(err, "largest");
-  }
+  int* x_shift = reinterpret_cast<int*>(ws + q.x_shift);
+  float* w_shift = reinterpret_cast<float*>(ws + q.w_shift);
+  float* w_scale = reinterpret_cast<float*>(ws + q.w_scale);
   if (bf)
     err = launch_dependent(gather_kernel<bf16>, grid, 128, 0, 1, st, static_cast<const bf16*>(p->hidden), p->hidden_stride_row, p->dim,
-                                              x.ld, sel, p->targets, p->targets_int64, p->ignore_index, hi, lo,
+                                              x.ld, sel, p->targets, p->targets_int64, p->ignore_index, hi, lo, nullptr,
                                               static_cast<bf16*>(p->grad_hidden));
   else
     err = launch_dependent(gather_kernel<float>, grid, 128, 0, 1, st, static_cast<const float*>(p->hidden), p->hidden_stride_row, p->dim,
-                                               x.ld, sel, p->targets, p->targets_int64, p->ignore_index, hi, lo,
+                                               x.ld, sel, p->targets, p->targets_int64, p->ignore_index, hi, lo, x_shift,
                                                static_cast<float*>(p->grad_hidden));
   CE_CHECK(err, "gather");
   w.rows = p->vocab; w.dim = p->dim; w.ld = p->weight_stride_row; w.plane[0] = p->weight;
@@ -991,11 +1046,12 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
     void* wlo = const_cast<void*>(w.plane[1]);
     const unsigned g = (unsigned)std::min<int64_t>((w.rows * ((w.ld + 255) / 256) + 7) / 8, wide * 2);
     if (bf)
-      err = launch_dependent(planes_kernel<bf16>, g, 256, 0, 1, st, static_cast<const bf16*>(p->weight), p->weight_stride_row, p->vocab, p->dim,
-                                             w.ld, whi, wlo, &sel.scales->w);
+      err = launch_dependent(repack_kernel, g, 256, 0, 1, st, static_cast<const bf16*>(p->weight), p->weight_stride_row, p->vocab, p->dim,
+                                            w.ld, whi);
     else
-      err = launch_dependent(planes_kernel<float>, g, 256, 0, 1, st, static_cast<const float*>(p->weight), p->weight_stride_row, p->vocab, p->dim,
-                                              w.ld, whi, wlo, &sel.scales->w);
+      err = launch_dependent(planes_kernel, (unsigned)std::min<int64_t>((w.rows + 7) / 8, wide * 2), 256, 0, 1, st,
+                             static_cast<const float*>(p->weight), p->weight_stride_row, p->vocab, p->dim, w.ld, whi, wlo, w_shift,
+                             w_scale);
     CE_CHECK(err, "weight planes");
   }
   Reduced red{};
@@ -1019,7 +1075,10 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
     a.picked = reinterpret_cast<float*>(ws + q.picked);
     a.logits = q.grad ? reinterpret_cast<float*>(ws + q.logits) : nullptr;
     a.ld = q.ld;
-    a.scales = sel.scales;
+    a.x_shift = x_shift + t0;
+    a.w_shift = w_shift;
+    a.w_scale = w_scale;
+    a.peak = q.planes == 2 && p->grad_hidden ? reinterpret_cast<float*>(ws + q.peak) : nullptr;
     // one SM's tiles where a pair's second half would be empty (loss of 128 x 50000 x 2560: 68 us, by pairs 70;
     // of 200 tokens, in two rows of tiles: 78, by pairs 71)
     if (n > BM) CE_CHECK(logits_gemm<2>(xc, w, q.planes, a, sel.count, from, status, st), "logits");
@@ -1030,6 +1089,8 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
       split.rows = reinterpret_cast<SplitRow*>(ws + q.factors);
       split.row_shift = reinterpret_cast<int*>(ws + q.row_shift);
       split.col_top = reinterpret_cast<int*>(ws + q.col_top);
+      split.peak = a.peak;
+      split.w_shift = w_shift;
       split.vocab = p->vocab;
     }
     err = launch_dependent(loss_kernel, (unsigned)cdiv(n, 8), 256, 0, 1, st, a.stats, a.ns, a.picked, sel, from, (int)n, rows, p->lse,
@@ -1045,6 +1106,7 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
     } else {
       sp.vocab = p->vocab; sp.ld = q.ld; sp.sel = sel; sp.from = from; sp.n = (int)n;
       sp.rows = split.rows; sp.row_shift = split.row_shift; sp.col_top = split.col_top; sp.logits = a.logits;
+      sp.x_shift = a.x_shift; sp.w_shift = w_shift;
       sp.hi = reinterpret_cast<__half*>(ws + q.dl[0]);
       sp.lo = reinterpret_cast<__half*>(ws + q.dl[1]);
       CE_CHECK(p->grad_hidden ? p->grad_weight ? launch_split<ROWS | MAX>(sp, st) : launch_split<ROWS>(sp, st)
@@ -1061,7 +1123,6 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
     if (p->grad_hidden) {
       OutArgs ox = o;
       ox.rows = n; ox.cols = p->dim; ox.index = sel.index + t0; ox.out = p->grad_hidden;
-      ox.largest = &sel.scales->w;
       CE_CHECK(grad_gemm_as<false>(n > BM, bf, dl, w, p->vocab, q.planes, q.part_x, ox, sel.count, from, status, st),
                "grad_hidden");
     }
@@ -1069,7 +1130,6 @@ cudaError_t launch_linear_ce(const ssd_linear_ce_params_t* p, void* workspace, c
       if (!bf) CE_CHECK(launch_split<COLS>(sp, st), "columns");
       OutArgs ow = o;
       ow.rows = p->vocab; ow.cols = p->dim;
-      ow.largest = &sel.scales->x;
       if (q.sum_w) ow.part = reinterpret_cast<float*>(ws + q.wsum);
       ow.sum = q.sum_w;
       ow.add_part = c > 0;

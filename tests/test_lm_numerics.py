@@ -96,6 +96,46 @@ def test_target_logit_minus_infinity(t, dtype):
     assert ((lse.double().cpu() - want).abs() <= 2.0 ** -21 + 8 * U * (1 + want.abs())).all()
 
 
+# ---- one large row or word beside the others ----------------------------------------------------
+@pytest.mark.parametrize("t", [20, 40, 200])
+@pytest.mark.parametrize("large", [2.0 ** 20, 2.0 ** 40, 2.0 ** 90])
+def test_a_large_row_of_hidden_changes_no_other_loss(t, large):
+    x, w = ints((t, 64), 17, 0, 14).float(), ints((300, 64), 17, 1, 18).float()
+    y = torch.randint(0, 300, (t,), generator=torch.Generator().manual_seed(2))
+    want = linear_cross_entropy(x.cuda(), w.cuda(), y.cuda(), reduction="none")
+    x[0] *= large
+    got = linear_cross_entropy(x.cuda(), w.cuda(), y.cuda(), reduction="none")
+    assert torch.equal(got[1:], want[1:])
+
+
+@pytest.mark.parametrize("t", [20, 40, 200])
+@pytest.mark.parametrize("large", [2.0 ** 20, 2.0 ** 40, 2.0 ** 90])
+def test_a_large_word_without_mass_changes_no_loss(t, large):
+    x, w = ints((t, 64), 17, 0, 14).float(), ints((300, 64), 17, 1, 18).float()
+    x[:, 0] = 1.0
+    y = torch.randint(6, 300, (t,), generator=torch.Generator().manual_seed(2))
+    w[5] = 0.0
+    w[5, 0] = -1024.0
+    want = linear_cross_entropy_grad(x.cuda(), w.cuda(), y.cuda(), reduction="none")
+    w[5, 0] = -1024.0 * large
+    got = linear_cross_entropy_grad(x.cuda(), w.cuda(), y.cuda(), reduction="none")
+    assert torch.equal(got[0], want[0])
+    assert all(float((a - b).norm()) <= 1e-5 * float(b.norm()) for a, b in zip(got[1:], want[1:]))
+
+
+@pytest.mark.parametrize("t", [40, 200])
+def test_gradients_beside_a_large_row(t):
+    """hidden's rows over sixty powers of two: every row of grad_hidden relative to itself."""
+    x, w = ints((t, 64), 8, 0, 7), ints((300, 64), 8, 1, 7)
+    x = x * 2.0 ** -torch.arange(t).remainder(60).double()[:, None]
+    y = torch.randint(0, 300, (t,), generator=torch.Generator().manual_seed(2))
+    one = torch.ones(t, dtype=torch.float64)
+    _, dx, dw = grads(x, w, y, one)
+    _, _, dl, s = reference(x, w, y, one)
+    check_grad(dx, dl, w, s)
+    assert float((dw.double().cpu() - dl.t() @ x).norm()) <= 1e-5 * float((dl.t() @ x).norm())
+
+
 # ---- gradients of the logits over many powers of ten --------------------------------------------
 @pytest.mark.parametrize("t", [7, 40, 200, 700])
 @pytest.mark.parametrize("decades", [12, 25])
@@ -137,6 +177,25 @@ def test_improbable_words_keep_their_gradient(t):
     _, dx, dw = grads(x, w, y, one)
     _, _, dl, s = reference(x, w, y, one)
     assert float(dl[:, :40].max()) < 1e-12
+    check_grad(dx, dl, w, s)
+    check_grad(dw, dl.t(), x, s)
+
+
+# ---- both low terms take part -------------------------------------------------------------------
+@pytest.mark.parametrize("t", [40, 200])
+@pytest.mark.parametrize("long", ["hidden", "weight"])
+def test_f32_values_of_17_bits(t, long):
+    x, w = ints((t, 64), 17, 0, 15), ints((300, 64), 2, 1, 1)
+    if long == "weight":
+        x, w = ints((t, 64), 2, 0, 1), ints((300, 64), 17, 1, 15)
+    y = torch.randint(0, 300, (t,), generator=torch.Generator().manual_seed(2))
+    one = torch.ones(t, dtype=torch.float64)
+    loss, dx, dw = grads(x, w, y, one)
+    ref, lse, dl, s = reference(x, w, y, one)
+    got = linear_cross_entropy(x.float().cuda(), w.float().cuda(), y.cuda(), reduction="none", return_lse=True)
+    bound = 2.0 ** -21 + 2 * U * s.abs().max() + 4 * U * (1 + ref.abs() + lse.abs())
+    assert ((got[0].double().cpu() - ref).abs() <= bound).all() and ((got[1].double().cpu() - lse).abs() <= bound).all()
+    assert ((loss.double().cpu() - ref).abs() <= bound).all()
     check_grad(dx, dl, w, s)
     check_grad(dw, dl.t(), x, s)
 
