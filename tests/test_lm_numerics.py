@@ -52,13 +52,17 @@ def reference(x, w, y, coef):
     return loss, lse, dl * coef[:, None], s
 
 
+def grad_constant(k, s):
+    """c of |error| <= c A for a sum of k terms of dl; s are the logits."""
+    z = float((s - s.max(1, keepdim=True).values).abs().max()) * 1.4427
+    return 2.0 ** -22 + 1.5 * U * z + 4 * U + 3 * 2.0 ** -22 + 24 * 2 * U + (k / 128 + 1) * U + 4 * U
+
+
 def check_grad(got, dl, m, s):
     """got against dl @ m, element by element."""
     k = dl.shape[1]
-    z = float((s - s.max(1, keepdim=True).values).abs().max()) * 1.4427
-    c = 2.0 ** -22 + 1.5 * U * z + 4 * U + 3 * 2.0 ** -22 + 24 * 2 * U + (k / 128 + 1) * U + 4 * U
     term = dl.abs().max(1, keepdim=True).values * m.abs().max()
-    bound = c * (dl.abs() @ m.abs()) + k * 2.0 ** -38 * term
+    bound = grad_constant(k, s) * (dl.abs() @ m.abs()) + k * 2.0 ** -38 * term
     err = (got.double().cpu() - dl @ m).abs()
     assert (err <= bound).all(), float((err / bound).max())
 
