@@ -43,7 +43,10 @@ constexpr int EC = gemm::EPI_COLS;
 // one segment 3.3e-6 off in the loss, 16 blocks 7.7e-7, 8 blocks 3.6e-7 at the same speed (4096 x
 // 131072 in 2.67 and 2.69 ms).  f32 operands, with three products a block, take 2: gradients
 // 7.6e-7 off (3 blocks 1.0e-6 and 3 % faster, 1 block 5.8e-7 and 3 % slower).
-constexpr int SEGMENT_BF16 = 8, SEGMENT_F32 = 2;
+// The gradients of bf16 take 32: over 131072 words grad_hidden is 3.5e-6 too small by the adds (whole range 1.07e-4,
+// a fifth of bf16's own rounding and all of one sign; 64 blocks 1.1e-5, 16 blocks 1.1e-6 and 0.6 % slower;
+// 32 as fast as the whole range: 16384 x 50000 x 2560 in 11.7 ms back to back).
+constexpr int SEGMENT_BF16 = 8, SEGMENT_F32 = 2, SEGMENT_GRAD = 32;
 constexpr int64_t LOSS_CHUNK = 16384;              // tokens whose statistics are kept at a time
 // logits and dl of a chunk of tokens (16384 x 50000 x 2560: chunks of 1 GiB 9.6 ms, 3 GiB 9.5, 6 GiB 9.6)
 constexpr int64_t GRAD_BYTES = int64_t(3) << 30;
@@ -973,8 +976,7 @@ cudaError_t grad_gemm(const Operand& a, const Operand& b, int64_t k, int planes,
   g.k_blocks = cdiv(k, gemm::BK);
   g.planes = planes;
   g.m_fastest = 0;
-  // bf16: the operands' own rounding is a hundred times what the adds lose
-  g.segment = planes == 2 ? SEGMENT_F32 : 1 << 20;
+  g.segment = planes == 2 ? SEGMENT_F32 : SEGMENT_GRAD;
   g.status = status;
   static std::atomic<uint64_t> allowed[4] = {};
   const bool out = !o.sum && g.max_splits == 1;

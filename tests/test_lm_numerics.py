@@ -204,6 +204,28 @@ def test_f32_values_of_17_bits(t, long):
     check_grad(dw, dl.t(), x, s)
 
 
+# ---- long sums ----------------------------------------------------------------------------------
+def test_bf16_grad_hidden_has_no_bias_over_a_large_vocabulary():
+    """sum_v p_v w_v over 131072 words, all terms positive: adds that cut lose the more the longer they run.
+    Columns and tokens of many sizes, so that the part of the gradient along the float64 one averages the
+    roundings of dl and of the result (163840 values: 2^-9 / sqrt(3) / 405 = 2.8e-6; five times that).  A
+    segment of 32 K blocks has 128 adds, each cut by up to 2^-23, and 64 rounded ones join the segments."""
+    t, v, d, some = 4096, 131072, 1280, 128
+    g = torch.Generator(device="cuda").manual_seed(0)
+    c = torch.exp2(torch.rand(d, generator=g, device="cuda"))
+    w = ((torch.randn((v, d), generator=g, device="cuda") * 0.05 + 0.25) * c).bfloat16()
+    w[0] = 0.0
+    x = (torch.randn((t, d), generator=g, device="cuda") * 0.4 / c).bfloat16()
+    weight = torch.exp2(torch.rand(t, generator=g, device="cuda"))
+    y = torch.zeros(t, dtype=torch.int64, device="cuda")
+    _, dx, _ = linear_cross_entropy_grad(x, w, y, reduction="none", grad_loss=weight, need_weight_grad=False,
+                                         check_status=True)
+    p = torch.softmax(x[:some].double() @ w.double().t(), 1) * weight[:some, None].double()
+    ref = p @ w.double()
+    bias = float((dx[:some].double() * ref).sum() / (ref * ref).sum()) - 1.0
+    assert abs(bias) <= 128 * 2.0 ** -23 + 64 * U + 5 * 2.8e-6
+
+
 # ---- ignored rows -------------------------------------------------------------------------------
 @pytest.mark.parametrize("t", [2, 3, 8, 40])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
