@@ -1,6 +1,7 @@
 """Global gradient norm over many tensors, and clipping by it."""
 from __future__ import annotations
 
+import math
 import operator
 from array import array
 
@@ -10,7 +11,7 @@ from .. import _lib
 
 _DTYPE = {torch.float32: _lib.SSD_DTYPE_F32, torch.bfloat16: _lib.SSD_DTYPE_BF16}
 _T = torch.Tensor
-_dtype = operator.attrgetter("dtype")
+_dtype, _shape = operator.attrgetter("dtype"), operator.attrgetter("shape")
 
 
 # A model has hundreds of tensors, and the kernels take a few microseconds where they are
@@ -41,6 +42,12 @@ def _contiguous(ts):
 
 def _sizes(ts):
     return array("q", map(_T.numel, ts))
+
+
+def _same_order(out, grads):
+    """Every tensor of out has its gradient's shape, or is a flat piece of as many elements."""
+    a, b = list(map(_shape, out)), list(map(_shape, grads))
+    return a == b or all(x == y or (len(x) == 1 and x[0] == math.prod(y)) for x, y in zip(a, b))
 
 
 def _run(grads, dtypes, outs, out_dtypes, sizes, max_norm, eps, scale):
@@ -81,8 +88,9 @@ def clip_grad_norm(grads, max_norm: float, *, eps: float = 1e-6, out=None, inpla
     Returns ``(clipped, norm)``: ``grads`` times ``min(1, max_norm / (norm + eps))`` and the norm
     before clipping (a float32 scalar tensor on the device; nothing waits for it).  By default
     the clipped gradients are new tensors; ``inplace=True`` scales ``grads`` themselves, ``out``
-    gives contiguous tensors of as many elements to write to, float32 or bfloat16 (bfloat16
-    gradients into the float32 buffers of an optimizer).  A NaN norm makes every gradient NaN.
+    gives contiguous tensors of the same shapes (or flat pieces of as many elements) to write to,
+    float32 or bfloat16 (bfloat16 gradients into the float32 buffers of an optimizer), none of which
+    may overlap another or a gradient that is not its own.  A NaN norm makes every gradient NaN.
     """
     ts, dtypes, device = _checked(grads, "grads")
     if not float(max_norm) >= 0.0 or not float(eps) >= 0.0:
@@ -102,8 +110,8 @@ def clip_grad_norm(grads, max_norm: float, *, eps: float = 1e-6, out=None, inpla
             outs, out_dtypes, out_device = _checked(out, "out") if len(out) else ([], set(), device)
             if len(outs) != len(ts):
                 raise ValueError(f"out has {len(outs)} tensors, grads {len(ts)}")
-            if _sizes(outs) != sizes or not all(map(_T.is_contiguous, outs)):
-                raise ValueError("out must hold contiguous tensors of grads' sizes")
+            if not _same_order(outs, ts) or not all(map(_T.is_contiguous, outs)):
+                raise ValueError("out must hold contiguous tensors of grads' shapes, or flat pieces of their sizes")
             if out_device != device:
                 raise ValueError("out and grads must be on one device")
     return outs, _run(ts, dtypes, outs, out_dtypes, sizes, max_norm, eps, True)

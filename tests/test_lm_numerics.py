@@ -237,3 +237,15 @@ def test_ignored_rows_have_no_gradient_whatever_the_weight_holds(t, dtype, bad):
     y[0] = -100
     _, dx, _ = linear_cross_entropy_grad(x, w, y)
     assert (dx[0] == 0).all()
+
+
+# ---- clipping -----------------------------------------------------------------------------------
+def test_clip_refuses_out_of_another_shape():
+    g = [torch.ones(6, 4).cuda(), torch.ones(5).cuda()]
+    for bad in (torch.empty(4, 6), torch.empty(2, 12), torch.empty(6, 4, 1)):
+        with pytest.raises(ValueError):
+            clip_grad_norm(g, 1.0, out=[bad.cuda(), torch.empty(5).cuda()])
+    # a piece of a flat buffer holds the values in the same order
+    flat = torch.empty(29).cuda()
+    got, _ = clip_grad_norm(g, 1e9, out=[flat[:24], flat[24:]])
+    assert (flat == 1).all() and got[0].shape == (24,)
