@@ -249,3 +249,55 @@ def test_clip_refuses_out_of_another_shape():
     flat = torch.empty(29).cuda()
     got, _ = clip_grad_norm(g, 1e9, out=[flat[:24], flat[24:]])
     assert (flat == 1).all() and got[0].shape == (24,)
+
+
+# ---- the paths around the scaled planes ---------------------------------------------------------
+def test_f32_token_chunks():
+    """More tokens than one chunk of logits holds: every chunk has powers of its own, grad_weight is summed."""
+    t, v, d = 4500, 131072, 64
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w = torch.randn(v, d, generator=g, device="cuda") / 8
+    y = torch.randint(0, v, (t,), generator=g, device="cuda")
+    x = torch.randn(t, d, generator=g, device="cuda") + 4 * w[y]
+    weight = 10.0 ** (-6 * torch.rand(t, generator=g, device="cuda"))
+    weight[t // 2:] *= 1e-6
+    _, dx, dw = linear_cross_entropy_grad(x, w, y, reduction="none", grad_loss=weight, check_status=True)
+    xs, ws = x.double(), w.double()
+    dws, worst = torch.zeros_like(ws), 0.0
+    for lo in range(0, t, 500):
+        p = torch.softmax(xs[lo:lo + 500] @ ws.t(), 1)
+        p[torch.arange(len(p)), y[lo:lo + 500]] -= 1
+        p *= weight[lo:lo + 500, None].double()
+        ref = p @ ws
+        worst = max(worst, float(((dx[lo:lo + 500].double() - ref).norm(dim=1) / ref.norm(dim=1)).max()))
+        dws += p.t() @ xs[lo:lo + 500]
+    # a logit: 6 * 2^-22 |x| |w| / 4 of independent roundings, 24 adds cut by 2^-23 of sums up to 12; twice that
+    # in a row of dl, and the product's own 1e-5
+    tol = 2 * (6 * 2.0 ** -22 * 3 + 24 * 2.0 ** -23 * 12) + 1e-5
+    assert worst <= tol and float((dw.double() - dws).norm() / dws.norm()) <= tol
+
+
+@pytest.mark.parametrize("t", [40, 200])
+def test_f32_rows_without_a_valid_target_or_weight(t):
+    """An invalid target makes its own row of grad_hidden NaN (and grad_weight), and no other row; a token of
+    weight zero has no gradient."""
+    x, w = ints((t, 64), 8, 0, 7), ints((300, 64), 8, 1, 7)
+    y = torch.randint(0, 300, (t,), generator=torch.Generator().manual_seed(2))
+    one = torch.ones(t, dtype=torch.float64)
+    _, _, dl, s = reference(x, w, y, one)
+    bad = y.clone()
+    bad[5], bad[-1] = 300, -1
+    loss, dx, dw = grads(x, w, bad, one)
+    keep = torch.ones(t, dtype=torch.bool)
+    keep[5] = keep[-1] = False
+    assert torch.isnan(loss[~keep]).all() and torch.isnan(dx[~keep]).all() and torch.isnan(dw).all()
+    check_grad(dx[keep], dl[keep], w, s[keep])
+    weight = one.clone()
+    weight[::3] = 0.0
+    _, dx, dw = grads(x, w, y, weight)
+    assert (dx[::3] == 0).all()
+    dl = dl * weight[:, None]
+    check_grad(dx, dl, w, s)
+    check_grad(dw, dl.t(), x, s)
+    _, dx, dw = grads(x, w, y, 0 * one)
+    assert (dx == 0).all() and (dw == 0).all()
