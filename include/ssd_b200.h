@@ -432,7 +432,8 @@ typedef struct ssd_grad_tensor {
 
 /* Norm over all tensors of a list and the clipped gradients:
  *   norm = sqrt(sum of all squares);  out = min(1, max_norm / (norm + eps)) * grad
- * The list is in host memory and read during the call only.  Sums are f64, in a fixed order.
+ * The list is in host memory and read during the call only.  Sums are f64 (of groups of four squares
+ * in f32), in a fixed order.
  * scale = 0: the norm alone.  A NaN norm gives NaN gradients, an infinite one zero (and NaN
  * where the gradient itself is infinite). */
 size_t ssd_clip_grad_norm_workspace_bytes(const ssd_grad_tensor_t* tensors, int64_t count);

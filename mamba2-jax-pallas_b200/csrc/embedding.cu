@@ -729,7 +729,8 @@ cudaError_t launch_embedding_grad(const ssd_embedding_grad_params_t* p, void* wo
   // zero rows reads), half of the zero rows or more come behind the sums, which would else leave their
   // slots empty (us without / with): 5000 ids, 100000 x 1600 f32 132 / 118; 3000 ids, 131072 x 4096 bf16 201 /
   // 185; 4000 ids, 60000 x 1216 f32 (292 MB) 61 / 58; but 777 ids, 50257 x 768 f32 (154 MB) 33 / 37; 32768 ids,
-  // 131072 x 4096 bf16 251 / 263.
+  // 131072 x 4096 bf16 254 / 267.  The two sides meet at 22000 ids for 131072 x 4096 bf16, 15500 for 100000 x
+  // 1600 f32 and 12500 for 50257 x 2560 f32; the rule changes at 28339, 16891 and 13582, at most 5 % off.
   const int64_t sum_ctas = (a.npieces * ((a.dim + SUM_COLS - 1) / SUM_COLS) + SUM_THREADS / 32 - 1) / (SUM_THREADS / 32);
   if (!a.accumulate) {
     a.zero_first = 148 * 4 - (int)std::min<int64_t>(148 * 2, sum_ctas);

@@ -17,9 +17,11 @@
 //              operations, more from D = 512 on.
 // f32 inputs are split into two f16 planes, three products per pair (tc_gemm.cuh).
 //
-// Measured: loss of 4096 x 131072 x 4096, bf16, 2.72 ms (1.62 PFLOP/s); gradients of 16384 x 50000 x 2560,
-// bf16, 9.5 ms of kernels (1.32 PFLOP/s): logits 3.04, dX 2.67, dW 2.81, rows 0.73, parts 0.14, the
-// rest 0.1; gradients of 2048 x 50257 x 768, f32, 1.2 ms (1.2 PFLOP/s of f16 products).
+// Measured, kernels alone: loss of 4096 x 131072 x 4096, bf16, 2.79 ms (1.58 PFLOP/s; calls back to back,
+// under the power limit, 3.10); gradients of 16384 x 50000 x 2560, bf16, 10.4 ms under the power limit (1.21
+// PFLOP/s): logits 3.35, dX 3.00, dW 3.03, rows 0.75, parts 0.15, the rest 0.1 (calls 11.0; in a burst 9.5);
+// gradients of 2048 x 50257 x 768, f32, 1.34 ms (1.06 PFLOP/s of f16 products): logits 0.39, dX 0.29, dW
+// 0.31, the passes over the logits 0.26, planes 0.05, the rest 0.04.
 #include <algorithm>
 
 #include <cuda_fp16.h>
@@ -317,8 +319,8 @@ __device__ __forceinline__ float4 load_again(const float* p) {
 }
 
 // Half a warp's 32 x 64 block to global memory: through its 4 KB of shared memory, in the layout
-// of a swizzled box, by one bulk store (f32, 2048 x 50257 x 768: the kernel takes 370 us where
-// the warp stores values itself, 354 us so and 297 us without any store).
+// of a swizzled box, by one bulk store (f32, 2048 x 50257 x 768, before operands had a power of two per
+// row, which takes 40 us: 370 us where the warp stores values itself, 354 us so, 297 us without any store).
 template <int HALF>
 __device__ __forceinline__ void store_half(const CUtensorMap* map, uint4* stage, const float (&v)[EC], int n0, int row0) {
   const int lane = threadIdx.x & 31;

@@ -69,7 +69,8 @@ def linear_cross_entropy(hidden, weight, targets, *, ignore_index: int = -100, r
     with ``return_lse`` also the log of each row's sum of exponentials (0 where ignored).  A target equal to
     ``ignore_index`` has loss 0 and does not count in the mean (a mean over no tokens is 0); any
     other target outside [0, vocab) has loss NaN.  ``check_status`` waits for the call and
-    raises ``SsdError`` if a bounded wait inside a kernel gave up.
+    raises ``SsdError`` if a bounded wait inside a kernel gave up.  The result carries no autograd
+    history, also where an input requires a gradient: ``linear_cross_entropy_grad`` gives both.
     """
     loss, lse, _, _ = _call(hidden, weight, targets, ignore_index, reduction, None, return_lse, False, False, None,
                             check_status)

@@ -22,7 +22,9 @@ def embedding(tokens, weight, scale: float = 1.0, *, padding_idx=None, out_dtype
 
     tokens (...) int32 or int64; weight (vocab, dim) float32 or bfloat16.  Returns (..., dim)
     in ``out_dtype`` (default: weight's dtype).  A token outside [0, vocab) or equal to
-    ``padding_idx`` gives a zero row.
+    ``padding_idx`` gives a zero row, whatever the table holds there (torch.nn.functional.embedding
+    returns the row and stops only its gradient).  The result carries no autograd history, also
+    where weight requires a gradient: ``embedding_grad`` gives it.
     """
     ids = _lib.index_list(tokens, "tokens")
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
@@ -62,7 +64,8 @@ def embedding_grad(tokens, grad_out, num_embeddings: int, scale: float = 1.0, *,
     tokens (the same bits in every run) and rounded once to ``out_dtype`` (default: grad_out's
     dtype).  With ``accumulate_into`` (a float32 or bfloat16 (num_embeddings, dim) tensor, rows
     contiguous) the sums are added to that tensor, only the named rows are touched, and it is
-    returned: the tied output projection's gradient, or that of an earlier micro-batch.
+    returned: the tied output projection's gradient, or that of an earlier micro-batch.  Autograd
+    does not see that write.
     """
     ids = _lib.index_list(tokens, "tokens")
     vocab = int(num_embeddings)

@@ -76,7 +76,8 @@ def _run(grads, dtypes, outs, out_dtypes, sizes, max_norm, eps, scale):
 
 def grad_norm(grads):
     """2-norm over all tensors of ``grads`` (float32 or bfloat16, any mix and shapes): a float32
-    scalar tensor.  Squares are summed in float64."""
+    scalar tensor.  Squares are added in float32 by fours and those in float64: off by at most
+    2.5 * 2^-24 of itself."""
     ts, dtypes, _ = _checked(grads, "grads")
     ts = _contiguous(ts)
     return _run(ts, dtypes, ts, dtypes, _sizes(ts), 0.0, 0.0, False)
@@ -91,6 +92,7 @@ def clip_grad_norm(grads, max_norm: float, *, eps: float = 1e-6, out=None, inpla
     gives contiguous tensors of the same shapes (or flat pieces of as many elements) to write to,
     float32 or bfloat16 (bfloat16 gradients into the float32 buffers of an optimizer), none of which
     may overlap another or a gradient that is not its own.  A NaN norm makes every gradient NaN.
+    Autograd does not see the writes (tensors' version counters stay).
     """
     ts, dtypes, device = _checked(grads, "grads")
     if not float(max_norm) >= 0.0 or not float(eps) >= 0.0:
