@@ -440,6 +440,67 @@ size_t ssd_clip_grad_norm_workspace_bytes(const ssd_grad_tensor_t* tensors, int6
 int ssd_clip_grad_norm(const ssd_grad_tensor_t* tensors, int64_t count, float max_norm, float eps, int32_t scale,
                        float* norm, void* workspace, size_t workspace_bytes, ssd_stream_t stream);
 
+/* Gated linear recurrence: per channel, with k = scale * softplus(decay),
+ *   a_t = exp(-k sigmoid(decay_gate_t));
+ *   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(input_gate_t) x_t;  y_t = h_t
+ * from initial_state (zero where NULL).  With seq_idx a sequence starts at every t > 0 whose id differs
+ * from that of t - 1: it takes nothing of the state before (initial_state belongs to the first).
+ * x, decay_gate and input_gate are (batch, seqlen, dim), channels contiguous, at any strides of batch and token.
+ * States and arithmetic are f32; y is rounded once.  A value that is not finite makes its channel so up to
+ * the next sequence. */
+#define SSD_GATED_RECURRENCE_CHECKPOINT 32   /* tokens between two checkpoints */
+typedef struct ssd_gated_recurrence_params {
+  int64_t batch, seqlen, dim;
+  int64_t x_stride_b, x_stride_t, decay_gate_stride_b, decay_gate_stride_t;  /* in values */
+  int64_t input_gate_stride_b, input_gate_stride_t;
+  int32_t dtype;              /* ssd_dtype_t of x, the gates, y and their gradients */
+  float scale;                /* not negative, finite */
+  const void* x;
+  const void* decay_gate;
+  const void* input_gate;
+  const float* decay;         /* (dim,) */
+  const float* initial_state; /* (batch, dim), or NULL */
+  const int32_t* seq_idx;     /* (batch, seqlen), or NULL */
+  void* y;                    /* (batch, seqlen, dim) contiguous, or NULL; unused by the gradient */
+  float* final_state;         /* (batch, dim), or NULL; unused by the gradient */
+  float* checkpoints;         /* (batch, ceil(seqlen / 32), dim): the state before each 32 tokens, or NULL.
+                                 Written by the forward pass; read by the gradient, which computes them where NULL */
+} ssd_gated_recurrence_params_t;
+
+int ssd_gated_recurrence(const ssd_gated_recurrence_params_t* p, ssd_stream_t stream);
+
+/* Gradients of sum(grad_y * y) + sum(grad_final_state * final_state). */
+typedef struct ssd_gated_recurrence_grads {
+  int64_t grad_y_stride_b, grad_y_stride_t;
+  const void* grad_y;         /* (batch, seqlen, dim), channels contiguous */
+  const float* grad_final_state; /* (batch, dim), or NULL */
+  void* grad_x;               /* (batch, seqlen, dim) contiguous, as the next two */
+  void* grad_decay_gate;
+  void* grad_input_gate;
+  float* grad_decay;          /* (dim,) */
+  float* grad_initial_state;  /* (batch, dim), or NULL */
+} ssd_gated_recurrence_grads_t;
+
+size_t ssd_gated_recurrence_grad_workspace_bytes(const ssd_gated_recurrence_params_t* p);
+int ssd_gated_recurrence_grad(const ssd_gated_recurrence_params_t* p, const ssd_gated_recurrence_grads_t* g,
+                              void* workspace, size_t workspace_bytes, ssd_stream_t stream);
+
+/* One token of the gated linear recurrence; the state is updated in place. */
+typedef struct ssd_gated_recurrence_update_params {
+  int64_t batch, dim;
+  int64_t x_stride_row, decay_gate_stride_row, input_gate_stride_row; /* in values */
+  int32_t dtype;              /* ssd_dtype_t of x, the gates and y */
+  float scale;
+  const void* x;              /* (batch, dim), as the gates */
+  const void* decay_gate;
+  const void* input_gate;
+  const float* decay;         /* (dim,) */
+  float* state;               /* (batch, dim) contiguous */
+  void* y;                    /* (batch, dim) contiguous */
+} ssd_gated_recurrence_update_params_t;
+
+int ssd_gated_recurrence_update(const ssd_gated_recurrence_update_params_t* p, ssd_stream_t stream);
+
 /* Thread-local description of the last failure on this host thread ("" if none). */
 const char* ssd_last_error(void);
 

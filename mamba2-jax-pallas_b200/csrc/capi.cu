@@ -615,4 +615,61 @@ int ssd_clip_grad_norm(const ssd_grad_tensor_t* tensors, int64_t count, float ma
                      "clip_grad_norm");
 }
 
+namespace {
+int check_gated_recurrence(const ssd_gated_recurrence_params_t* p) {
+  if (!p) return fail(SSD_ERR_INVALID_ARG, "params is NULL");
+  if (p->batch <= 0 || p->seqlen <= 0 || p->dim <= 0) return fail(SSD_ERR_INVALID_ARG, "dims must be positive");
+  if (p->batch > INT32_MAX || p->seqlen > INT32_MAX || p->dim > INT32_MAX)
+    return fail(SSD_ERR_UNSUPPORTED, "dims must be below 2^31");
+  if (!dtype_ok(p->dtype)) return fail(SSD_ERR_INVALID_ARG, "bad dtype enum");
+  if (!(p->scale >= 0.f) || p->scale > 3.4e38f) return fail(SSD_ERR_INVALID_ARG, "scale must be finite and not negative");
+  // CTAs are numbered in 31 bits, clusters of 16 among them
+  if (p->batch * ((p->dim + 31) / 32) >= ((int64_t)1 << 27)) return fail(SSD_ERR_UNSUPPORTED, "batch * dim too large");
+  return SSD_OK;
+}
+}  // namespace
+
+int ssd_gated_recurrence(const ssd_gated_recurrence_params_t* p, ssd_stream_t stream) {
+  g_err[0] = 0;
+  if (int s = check_gated_recurrence(p)) return s;
+  if (!p->x || !p->decay_gate || !p->input_gate || !p->decay)
+    return fail(SSD_ERR_INVALID_ARG, "x, decay_gate, input_gate and decay are required");
+  if (!p->y && !p->final_state && !p->checkpoints) return fail(SSD_ERR_INVALID_ARG, "no output is wanted");
+  return cuda_status(ssd::launch_gated_recurrence(p, (cudaStream_t)stream), "gated_recurrence");
+}
+
+size_t ssd_gated_recurrence_grad_workspace_bytes(const ssd_gated_recurrence_params_t* p) {
+  g_err[0] = 0;
+  if (check_gated_recurrence(p)) return 0;
+  return ssd::gated_recurrence_grad_workspace(p);
+}
+
+int ssd_gated_recurrence_grad(const ssd_gated_recurrence_params_t* p, const ssd_gated_recurrence_grads_t* g,
+                              void* workspace, size_t workspace_bytes, ssd_stream_t stream) {
+  g_err[0] = 0;
+  if (int s = check_gated_recurrence(p)) return s;
+  if (!g) return fail(SSD_ERR_INVALID_ARG, "grads is NULL");
+  if (!p->x || !p->decay_gate || !p->input_gate || !p->decay || !g->grad_y)
+    return fail(SSD_ERR_INVALID_ARG, "x, decay_gate, input_gate, decay and grad_y are required");
+  if (!g->grad_x || !g->grad_decay_gate || !g->grad_input_gate || !g->grad_decay)
+    return fail(SSD_ERR_INVALID_ARG, "grad_x, grad_decay_gate, grad_input_gate and grad_decay are required");
+  const size_t need = ssd::gated_recurrence_grad_workspace(p);
+  if (!workspace || workspace_bytes < need)
+    return fail(SSD_ERR_WORKSPACE, "workspace too small: %zu bytes, need %zu", workspace_bytes, need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(SSD_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
+  return cuda_status(ssd::launch_gated_recurrence_grad(p, g, workspace, (cudaStream_t)stream), "gated_recurrence_grad");
+}
+
+int ssd_gated_recurrence_update(const ssd_gated_recurrence_update_params_t* p, ssd_stream_t stream) {
+  g_err[0] = 0;
+  if (!p) return fail(SSD_ERR_INVALID_ARG, "params is NULL");
+  if (p->batch <= 0 || p->dim <= 0) return fail(SSD_ERR_INVALID_ARG, "dims must be positive");
+  if (p->batch > INT32_MAX || p->dim > INT32_MAX) return fail(SSD_ERR_UNSUPPORTED, "dims must be below 2^31");
+  if (!dtype_ok(p->dtype)) return fail(SSD_ERR_INVALID_ARG, "bad dtype enum");
+  if (!(p->scale >= 0.f) || p->scale > 3.4e38f) return fail(SSD_ERR_INVALID_ARG, "scale must be finite and not negative");
+  if (!p->x || !p->decay_gate || !p->input_gate || !p->decay || !p->state || !p->y)
+    return fail(SSD_ERR_INVALID_ARG, "x, decay_gate, input_gate, decay, state and y are required");
+  return cuda_status(ssd::launch_gated_recurrence_update(p, (cudaStream_t)stream), "gated_recurrence_update");
+}
+
 }  // extern "C"

@@ -52,6 +52,12 @@ int64_t grad_clip_partials(const ssd_grad_tensor_t* list, int64_t count);
 cudaError_t launch_grad_clip(const ssd_grad_tensor_t* list, int64_t count, float max_norm, float eps, bool scale,
                              float* norm, void* workspace, cudaStream_t st);
 
+cudaError_t launch_gated_recurrence(const ssd_gated_recurrence_params_t* p, cudaStream_t st);
+size_t gated_recurrence_grad_workspace(const ssd_gated_recurrence_params_t* p);
+cudaError_t launch_gated_recurrence_grad(const ssd_gated_recurrence_params_t* p, const ssd_gated_recurrence_grads_t* g,
+                                         void* workspace, cudaStream_t st);
+cudaError_t launch_gated_recurrence_update(const ssd_gated_recurrence_update_params_t* p, cudaStream_t st);
+
 // Set the thread-local message ssd_last_error() returns.
 void set_last_error(const char* msg);
 

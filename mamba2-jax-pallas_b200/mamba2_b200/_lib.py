@@ -41,7 +41,9 @@ EXPORTED = ["ssd_combined_workspace_bytes", "ssd_combined_uses_tensor_cores",
             "ssd_last_error", "ssd_abi_version", "ssd_set_fp32_stage_path",
             "ssd_embedding", "ssd_embedding_grad", "ssd_embedding_grad_workspace_bytes",
             "ssd_linear_cross_entropy", "ssd_linear_cross_entropy_workspace_bytes",
-            "ssd_clip_grad_norm", "ssd_clip_grad_norm_workspace_bytes"]
+            "ssd_clip_grad_norm", "ssd_clip_grad_norm_workspace_bytes",
+            "ssd_gated_recurrence", "ssd_gated_recurrence_grad", "ssd_gated_recurrence_grad_workspace_bytes",
+            "ssd_gated_recurrence_update"]
 
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -128,6 +130,26 @@ class GradTensor(ctypes.Structure):
     _fields_ = [("grad", _vp), ("out", _vp), ("numel", _i64), ("grad_dtype", _i32), ("out_dtype", _i32)]
 
 
+class GatedRecurrenceParams(ctypes.Structure):
+    _fields_ = [("batch", _i64), ("seqlen", _i64), ("dim", _i64), ("x_stride_b", _i64), ("x_stride_t", _i64),
+                ("decay_gate_stride_b", _i64), ("decay_gate_stride_t", _i64), ("input_gate_stride_b", _i64),
+                ("input_gate_stride_t", _i64), ("dtype", _i32), ("scale", _f32),
+                ("x", _vp), ("decay_gate", _vp), ("input_gate", _vp), ("decay", _vp), ("initial_state", _vp),
+                ("seq_idx", _vp), ("y", _vp), ("final_state", _vp), ("checkpoints", _vp)]
+
+
+class GatedRecurrenceGrads(ctypes.Structure):
+    _fields_ = [("grad_y_stride_b", _i64), ("grad_y_stride_t", _i64), ("grad_y", _vp), ("grad_final_state", _vp),
+                ("grad_x", _vp), ("grad_decay_gate", _vp), ("grad_input_gate", _vp), ("grad_decay", _vp),
+                ("grad_initial_state", _vp)]
+
+
+class GatedRecurrenceUpdateParams(ctypes.Structure):
+    _fields_ = [("batch", _i64), ("dim", _i64), ("x_stride_row", _i64), ("decay_gate_stride_row", _i64),
+                ("input_gate_stride_row", _i64), ("dtype", _i32), ("scale", _f32),
+                ("x", _vp), ("decay_gate", _vp), ("input_gate", _vp), ("decay", _vp), ("state", _vp), ("y", _vp)]
+
+
 REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
@@ -188,6 +210,10 @@ def load() -> ctypes.CDLL:
     lib.ssd_clip_grad_norm_workspace_bytes.argtypes = [_vp, _i64]
     lib.ssd_embedding_grad_workspace_bytes.argtypes = [P(EmbeddingGradParams)]
     lib.ssd_linear_cross_entropy_workspace_bytes.argtypes = [P(LinearCeParams)]
+    lib.ssd_gated_recurrence.argtypes = [P(GatedRecurrenceParams), _vp]
+    lib.ssd_gated_recurrence_grad_workspace_bytes.argtypes = [P(GatedRecurrenceParams)]
+    lib.ssd_gated_recurrence_grad.argtypes = [P(GatedRecurrenceParams), P(GatedRecurrenceGrads), _vp, ctypes.c_size_t, _vp]
+    lib.ssd_gated_recurrence_update.argtypes = [P(GatedRecurrenceUpdateParams), _vp]
     for name in EXPORTED:
         if name.endswith("_workspace_bytes"):
             getattr(lib, name).restype = ctypes.c_size_t

@@ -1,0 +1,168 @@
+"""A gated linear recurrence per channel, its gradient and its single-token step: a sequence mixer that
+trains, beside the SSD scan (``mamba_chunk_scan_combined_fwd``) and its step (``selective_state_update``)."""
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+
+_TILE = 32   # SSD_GATED_RECURRENCE_CHECKPOINT
+
+
+def _channels_last(t):
+    """A view whose channels are contiguous, else a copy."""
+    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _inputs(x, decay_gate, input_gate, decay, scale, dims):
+    shape = "(batch, seqlen, dim)" if dims == 3 else "(batch, dim)"
+    for t, name in ((x, "x"), (decay_gate, "decay_gate"), (input_gate, "input_gate"), (decay, "decay")):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor (no CPU path)")
+        if t.device != x.device:
+            raise ValueError(f"{name} must be on x's device")
+    if x.dim() != dims or x.shape[-1] == 0:
+        raise ValueError(f"x must be {shape}, with channels")
+    for t, name in ((decay_gate, "decay_gate"), (input_gate, "input_gate")):
+        if t.shape != x.shape:
+            raise ValueError(f"{name} {tuple(t.shape)} must have x's shape {tuple(x.shape)}")
+        if t.dtype != x.dtype:
+            raise TypeError(f"{name} ({t.dtype}) and x ({x.dtype}) must have the same dtype")
+    if tuple(decay.shape) != (x.shape[-1],):
+        raise ValueError("decay must be (dim,)")
+    if not 0 <= scale <= 3.4e38:
+        raise ValueError("scale must be finite and not negative")
+    return (_lib.dtype_code(x), _channels_last(x), _channels_last(decay_gate), _channels_last(input_gate),
+            _lib.dev(decay.detach(), "decay", torch.float32))
+
+
+def _state(t, name, x):
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.device != x.device or tuple(t.shape) != (x.shape[0], x.shape[-1]):
+        raise ValueError(f"{name} must be a (batch, dim) tensor on x's device")
+    return _lib.dev(t.detach(), name, torch.float32)
+
+
+def _ids(seq_idx, x):
+    if seq_idx is None:
+        return None
+    ids = _lib.index_list(seq_idx, "seq_idx")
+    if tuple(ids.shape) != tuple(x.shape[:2]) or ids.device != x.device:
+        raise ValueError("seq_idx must be (batch, seqlen) on x's device")
+    return ids.to(torch.int32)
+
+
+def _checkpoint_shape(x):
+    return (x.shape[0], -(-x.shape[1] // _TILE), x.shape[2])
+
+
+def _params(code, x, decay_gate, input_gate, decay, scale, initial, ids):
+    b, L, d = x.shape
+    return _lib.GatedRecurrenceParams(b, L, d, x.stride(0), x.stride(1), decay_gate.stride(0), decay_gate.stride(1),
+                                      input_gate.stride(0), input_gate.stride(1), code, scale, x.data_ptr(),
+                                      decay_gate.data_ptr(), input_gate.data_ptr(), decay.data_ptr(), _lib.ptr(initial),
+                                      _lib.ptr(ids), None, None, None)
+
+
+def gated_recurrence(x, decay_gate, input_gate, decay, *, scale: float = 8.0, initial_state=None, seq_idx=None,
+                     return_final_state: bool = False, return_checkpoints: bool = False):
+    """``h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(input_gate_t) x_t`` along the sequence, per channel, with
+    ``a_t = exp(-scale softplus(decay) sigmoid(decay_gate_t))``.
+
+    x, decay_gate and input_gate (batch, seqlen, dim) of one dtype, float32 or bfloat16, at any
+    strides with contiguous channels (others are copied); decay (dim,); initial_state (batch, dim) or
+    None for zeros; seq_idx (batch, seqlen) int32 or int64: a packed sequence starts where the id
+    differs from the token before, and takes nothing of what came before (initial_state belongs to the first).
+    Returns h (batch, seqlen, dim) in x's dtype, computed in float32 and rounded once; with
+    ``return_final_state`` also the float32 state after the last token (batch, dim); with
+    ``return_checkpoints`` also the float32 states that ``gated_recurrence_grad`` starts from,
+    (batch, ceil(seqlen / 32), dim), which saves it a pass over the inputs.  A value that is
+    not finite makes its channel so up to the next sequence.  The results carry no autograd history.
+    """
+    code, xs, r, i, lam = _inputs(x, decay_gate, input_gate, decay, scale, 3)
+    h0, ids = _state(initial_state, "initial_state", x), _ids(seq_idx, x)
+    b, L, d = x.shape
+    y = torch.empty((b, L, d), dtype=x.dtype, device=x.device)
+    final = torch.empty((b, d), dtype=torch.float32, device=x.device) if return_final_state else None
+    points = torch.empty(_checkpoint_shape(x), dtype=torch.float32, device=x.device) if return_checkpoints else None
+    if y.numel():
+        p = _params(code, xs, r, i, lam, scale, h0, ids)
+        p.y, p.final_state, p.checkpoints = y.data_ptr(), _lib.ptr(final), _lib.ptr(points)
+        with _lib.on_device(x.device):
+            _lib.check(_lib.load().ssd_gated_recurrence(p, _lib.stream_of(y)))
+    elif final is not None:
+        final.zero_() if h0 is None else final.copy_(h0)
+    if not (return_final_state or return_checkpoints):
+        return y
+    return (y,) + ((final,) if return_final_state else ()) + ((points,) if return_checkpoints else ())
+
+
+def gated_recurrence_grad(x, decay_gate, input_gate, decay, grad_out, *, scale: float = 8.0, initial_state=None,
+                          seq_idx=None, grad_final_state=None, checkpoints=None):
+    """Gradients of ``gated_recurrence``: ``(grad_x, grad_decay_gate, grad_input_gate, grad_decay,
+    grad_initial_state)``.
+
+    grad_out (batch, seqlen, dim) in x's dtype is the gradient that reaches h, grad_final_state
+    (batch, dim) that of the final state (None for none).  The other arguments are those of the
+    forward call; ``checkpoints`` what it returned with ``return_checkpoints`` (None: computed again, by one
+    more pass over x and the gates).  The first three results have x's dtype, rounded once from float32;
+    grad_decay (dim,) is float32, summed in a fixed order, so that equal calls give equal bits;
+    grad_initial_state (batch, dim) is float32, or None where initial_state is.
+    """
+    code, xs, r, i, lam = _inputs(x, decay_gate, input_gate, decay, scale, 3)
+    h0, ids = _state(initial_state, "initial_state", x), _ids(seq_idx, x)
+    gf = _state(grad_final_state, "grad_final_state", x)
+    if not isinstance(grad_out, torch.Tensor) or grad_out.shape != x.shape or grad_out.device != x.device:
+        raise ValueError(f"grad_out must be a {tuple(x.shape)} tensor on x's device")
+    if grad_out.dtype != x.dtype:
+        raise TypeError(f"grad_out ({grad_out.dtype}) and x ({x.dtype}) must have the same dtype")
+    if checkpoints is not None and (not isinstance(checkpoints, torch.Tensor) or checkpoints.dtype != torch.float32 or
+                                    tuple(checkpoints.shape) != _checkpoint_shape(x) or checkpoints.device != x.device):
+        raise ValueError(f"checkpoints must be the float32 {_checkpoint_shape(x)} tensor that gated_recurrence returned")
+    g = _channels_last(grad_out)
+    b, L, d = x.shape
+    gx, gr, gi = (torch.empty((b, L, d), dtype=x.dtype, device=x.device) for _ in range(3))
+    gd = torch.empty(d, dtype=torch.float32, device=x.device)
+    gh = torch.empty((b, d), dtype=torch.float32, device=x.device) if h0 is not None else None
+    if gx.numel() == 0:
+        gd.zero_()
+        if gh is not None:
+            gh.zero_() if gf is None else gh.copy_(gf)
+        return gx, gr, gi, gd, gh
+    p = _params(code, xs, r, i, lam, scale, h0, ids)
+    points = None if checkpoints is None else checkpoints.contiguous()
+    p.checkpoints = _lib.ptr(points)
+    q = _lib.GatedRecurrenceGrads(g.stride(0), g.stride(1), g.data_ptr(), _lib.ptr(gf), gx.data_ptr(), gr.data_ptr(),
+                                  gi.data_ptr(), gd.data_ptr(), _lib.ptr(gh))
+    lib = _lib.load()
+    with _lib.on_device(x.device):
+        ws = torch.empty(lib.ssd_gated_recurrence_grad_workspace_bytes(p), dtype=torch.uint8, device=x.device)
+        _lib.check(lib.ssd_gated_recurrence_grad(p, q, ws.data_ptr(), ws.numel(), _lib.stream_of(gx)))
+    return gx, gr, gi, gd, gh
+
+
+def gated_recurrence_update(state, x, decay_gate, input_gate, decay, *, scale: float = 8.0, inplace: bool = False):
+    """One token of ``gated_recurrence``.  Returns ``(new_state, h)``.
+
+    state (batch, dim) float32; x, decay_gate and input_gate (batch, dim); h has x's dtype.  The given state
+    is copied first; with ``inplace=True`` it is updated itself (it must be contiguous) and returned.
+    """
+    if not isinstance(state, torch.Tensor) or state.dtype != torch.float32:
+        raise TypeError("state must be a float32 tensor")
+    code, xs, r, i, lam = _inputs(x, decay_gate, input_gate, decay, scale, 2)
+    if state.shape != x.shape or state.device != x.device:
+        raise ValueError("state must be (batch, dim) on x's device")
+    if inplace and not state.is_contiguous():
+        raise ValueError("inplace=True needs a contiguous state")
+    st = state if inplace else state.detach().clone(memory_format=torch.contiguous_format)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if y.numel():
+        p = _lib.GatedRecurrenceUpdateParams(x.shape[0], x.shape[1], xs.stride(0), r.stride(0), i.stride(0), code, scale,
+                                             xs.data_ptr(), r.data_ptr(), i.data_ptr(), lam.data_ptr(), st.data_ptr(),
+                                             y.data_ptr())
+        with _lib.on_device(x.device):
+            _lib.check(_lib.load().ssd_gated_recurrence_update(p, _lib.stream_of(y)))
+    return st, y
