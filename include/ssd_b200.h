@@ -501,6 +501,51 @@ typedef struct ssd_gated_recurrence_update_params {
 
 int ssd_gated_recurrence_update(const ssd_gated_recurrence_update_params_t* p, ssd_stream_t stream);
 
+/* Activations of the gated feed-forward block. */
+typedef enum ssd_activation {
+  SSD_ACT_SILU = 0,
+  SSD_ACT_GELU = 1,        /* x times the normal distribution function */
+  SSD_ACT_GELU_TANH = 2,   /* its tanh approximation */
+  SSD_ACT_RELU = 3
+} ssd_activation_t;
+
+/* Gated feed-forward block: h = act(x . w_gate^T) * (x . w_up^T);  y = h . w_down^T.
+ * bf16: products on the tensor cores with f32 accumulation; h (and in the gradients those of the two
+ * projections) is rounded once to bf16, as an operand of the products behind it.  f32: every operand as three
+ * bf16 terms, six products per pair, with the accuracy of f32 (values below 2^-110 lose digits).  For up to 8 tokens the forward products run
+ * in f32 on the CUDA cores. */
+typedef struct ssd_gated_ff_params {
+  int64_t tokens, dim, hidden, dim_out;
+  int64_t x_stride_row, w_gate_stride_row, w_up_stride_row, w_down_stride_row; /* in values, at least a row's length */
+  int32_t dtype;              /* ssd_dtype_t of x, the weights, y, grad_y and grad_x */
+  int32_t activation;         /* ssd_activation_t */
+  const void* x;              /* (tokens, dim) */
+  const void* w_gate;         /* (hidden, dim) */
+  const void* w_up;           /* (hidden, dim) */
+  const void* w_down;         /* (dim_out, hidden) */
+  void* y;                    /* (tokens, dim_out) contiguous; unused by the gradient */
+} ssd_gated_ff_params_t;
+
+/* The workspaces start with the device status word (see ssd_status_copy_async). */
+size_t ssd_gated_ff_workspace_bytes(const ssd_gated_ff_params_t* p);
+int ssd_gated_ff(const ssd_gated_ff_params_t* p, void* workspace, size_t workspace_bytes, ssd_stream_t stream);
+
+/* Gradients of sum(grad_y * y); g and u are computed again from x. */
+typedef struct ssd_gated_ff_grads {
+  int64_t grad_y_stride_row;  /* in values, at least dim_out */
+  const void* grad_y;         /* (tokens, dim_out) */
+  void* grad_x;               /* (tokens, dim) contiguous, or NULL */
+  void* grad_w_gate;          /* (hidden, dim) contiguous, or NULL; grad_w_up with it */
+  void* grad_w_up;
+  void* grad_w_down;          /* (dim_out, hidden) contiguous, or NULL */
+  int32_t grad_weight_dtype;  /* ssd_dtype_t of the three */
+  int32_t reserved;
+} ssd_gated_ff_grads_t;
+
+size_t ssd_gated_ff_grad_workspace_bytes(const ssd_gated_ff_params_t* p, const ssd_gated_ff_grads_t* g);
+int ssd_gated_ff_grad(const ssd_gated_ff_params_t* p, const ssd_gated_ff_grads_t* g, void* workspace,
+                      size_t workspace_bytes, ssd_stream_t stream);
+
 /* Thread-local description of the last failure on this host thread ("" if none). */
 const char* ssd_last_error(void);
 

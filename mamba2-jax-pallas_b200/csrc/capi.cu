@@ -672,4 +672,65 @@ int ssd_gated_recurrence_update(const ssd_gated_recurrence_update_params_t* p, s
   return cuda_status(ssd::launch_gated_recurrence_update(p, (cudaStream_t)stream), "gated_recurrence_update");
 }
 
+namespace {
+int check_gated_ff(const ssd_gated_ff_params_t* p) {
+  if (!p) return fail(SSD_ERR_INVALID_ARG, "params is NULL");
+  if (p->tokens <= 0 || p->dim <= 0 || p->hidden <= 0 || p->dim_out <= 0) return fail(SSD_ERR_INVALID_ARG, "dims must be positive");
+  // tile coordinates are 32-bit, and a tile may reach 256 past the end
+  if (p->tokens > INT32_MAX - 256 || p->dim > INT32_MAX - 256 || p->hidden > INT32_MAX / 2 - 256 || p->dim_out > INT32_MAX - 256)
+    return fail(SSD_ERR_UNSUPPORTED, "dims must be below 2^31 - 256 (hidden: 2^30 - 256)");
+  if (p->x_stride_row < p->dim || p->w_gate_stride_row < p->dim || p->w_up_stride_row < p->dim || p->w_down_stride_row < p->hidden)
+    return fail(SSD_ERR_INVALID_ARG, "row strides must be at least the rows' length");
+  if (!dtype_ok(p->dtype)) return fail(SSD_ERR_INVALID_ARG, "bad dtype enum");
+  if (p->activation < SSD_ACT_SILU || p->activation > SSD_ACT_RELU) return fail(SSD_ERR_INVALID_ARG, "bad activation");
+  if (!p->x || !p->w_gate || !p->w_up || !p->w_down) return fail(SSD_ERR_INVALID_ARG, "x, w_gate, w_up and w_down are required");
+  return SSD_OK;
+}
+
+int check_gated_ff_grads(const ssd_gated_ff_params_t* p, const ssd_gated_ff_grads_t* g) {
+  if (int s = check_gated_ff(p)) return s;
+  if (!g || !g->grad_y) return fail(SSD_ERR_INVALID_ARG, "grad_y is required");
+  if (g->grad_y_stride_row < p->dim_out) return fail(SSD_ERR_INVALID_ARG, "row strides must be at least the rows' length");
+  if (!dtype_ok(g->grad_weight_dtype)) return fail(SSD_ERR_INVALID_ARG, "bad dtype enum");
+  if (!g->grad_w_gate != !g->grad_w_up) return fail(SSD_ERR_INVALID_ARG, "grad_w_gate and grad_w_up come together");
+  return SSD_OK;
+}
+
+int check_workspace(const void* workspace, size_t bytes, size_t need) {
+  if (!workspace || bytes < need) return fail(SSD_ERR_WORKSPACE, "workspace too small: %zu bytes, need %zu", bytes, need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(SSD_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
+  return SSD_OK;
+}
+}  // namespace
+
+size_t ssd_gated_ff_workspace_bytes(const ssd_gated_ff_params_t* p) {
+  g_err[0] = 0;
+  if (check_gated_ff(p)) return 0;
+  return ssd::gated_ff_workspace(p, nullptr);
+}
+
+int ssd_gated_ff(const ssd_gated_ff_params_t* p, void* workspace, size_t workspace_bytes, ssd_stream_t stream) {
+  g_err[0] = 0;
+  if (int s = check_gated_ff(p)) return s;
+  if (!p->y) return fail(SSD_ERR_INVALID_ARG, "y is required");
+  if (int s = check_workspace(workspace, workspace_bytes, ssd::gated_ff_workspace(p, nullptr))) return s;
+  const char* at = "gated_ff";
+  return cuda_status(ssd::launch_gated_ff(p, nullptr, workspace, (cudaStream_t)stream, &at), at);
+}
+
+size_t ssd_gated_ff_grad_workspace_bytes(const ssd_gated_ff_params_t* p, const ssd_gated_ff_grads_t* g) {
+  g_err[0] = 0;
+  if (check_gated_ff_grads(p, g)) return 0;
+  return ssd::gated_ff_workspace(p, g);
+}
+
+int ssd_gated_ff_grad(const ssd_gated_ff_params_t* p, const ssd_gated_ff_grads_t* g, void* workspace,
+                      size_t workspace_bytes, ssd_stream_t stream) {
+  g_err[0] = 0;
+  if (int s = check_gated_ff_grads(p, g)) return s;
+  if (int s = check_workspace(workspace, workspace_bytes, ssd::gated_ff_workspace(p, g))) return s;
+  const char* at = "gated_ff_grad";
+  return cuda_status(ssd::launch_gated_ff(p, g, workspace, (cudaStream_t)stream, &at), at);
+}
+
 }  // extern "C"

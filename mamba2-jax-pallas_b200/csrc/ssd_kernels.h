@@ -58,6 +58,15 @@ cudaError_t launch_gated_recurrence_grad(const ssd_gated_recurrence_params_t* p,
                                          void* workspace, cudaStream_t st);
 cudaError_t launch_gated_recurrence_update(const ssd_gated_recurrence_update_params_t* p, cudaStream_t st);
 
+// `g` NULL: the forward pass.  `at` names the step that failed.
+size_t gated_ff_workspace(const ssd_gated_ff_params_t* p, const ssd_gated_ff_grads_t* g);
+cudaError_t launch_gated_ff(const ssd_gated_ff_params_t* p, const ssd_gated_ff_grads_t* g, void* workspace, cudaStream_t st,
+                            const char** at);
+// The forward pass of a few tokens (gated_ff_few.cu).
+bool gated_ff_is_few(const ssd_gated_ff_params_t* p);
+size_t gated_ff_few_workspace(const ssd_gated_ff_params_t* p);
+cudaError_t launch_gated_ff_few(const ssd_gated_ff_params_t* p, void* workspace, cudaStream_t st, const char** at);
+
 // Set the thread-local message ssd_last_error() returns.
 void set_last_error(const char* msg);
 

@@ -43,7 +43,8 @@ EXPORTED = ["ssd_combined_workspace_bytes", "ssd_combined_uses_tensor_cores",
             "ssd_linear_cross_entropy", "ssd_linear_cross_entropy_workspace_bytes",
             "ssd_clip_grad_norm", "ssd_clip_grad_norm_workspace_bytes",
             "ssd_gated_recurrence", "ssd_gated_recurrence_grad", "ssd_gated_recurrence_grad_workspace_bytes",
-            "ssd_gated_recurrence_update"]
+            "ssd_gated_recurrence_update", "ssd_gated_ff", "ssd_gated_ff_workspace_bytes", "ssd_gated_ff_grad",
+            "ssd_gated_ff_grad_workspace_bytes"]
 
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -150,6 +151,19 @@ class GatedRecurrenceUpdateParams(ctypes.Structure):
                 ("x", _vp), ("decay_gate", _vp), ("input_gate", _vp), ("decay", _vp), ("state", _vp), ("y", _vp)]
 
 
+class GatedFfParams(ctypes.Structure):
+    _fields_ = [("tokens", _i64), ("dim", _i64), ("hidden", _i64), ("dim_out", _i64), ("x_stride_row", _i64),
+                ("w_gate_stride_row", _i64), ("w_up_stride_row", _i64), ("w_down_stride_row", _i64),
+                ("dtype", _i32), ("activation", _i32),
+                ("x", _vp), ("w_gate", _vp), ("w_up", _vp), ("w_down", _vp), ("y", _vp)]
+
+
+class GatedFfGrads(ctypes.Structure):
+    _fields_ = [("grad_y_stride_row", _i64), ("grad_y", _vp), ("grad_x", _vp), ("grad_w_gate", _vp), ("grad_w_up", _vp),
+                ("grad_w_down", _vp), ("grad_weight_dtype", _i32), ("reserved", _i32)]
+
+
+ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
 REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
@@ -214,6 +228,10 @@ def load() -> ctypes.CDLL:
     lib.ssd_gated_recurrence_grad_workspace_bytes.argtypes = [P(GatedRecurrenceParams)]
     lib.ssd_gated_recurrence_grad.argtypes = [P(GatedRecurrenceParams), P(GatedRecurrenceGrads), _vp, ctypes.c_size_t, _vp]
     lib.ssd_gated_recurrence_update.argtypes = [P(GatedRecurrenceUpdateParams), _vp]
+    lib.ssd_gated_ff_workspace_bytes.argtypes = [P(GatedFfParams)]
+    lib.ssd_gated_ff.argtypes = [P(GatedFfParams), _vp, ctypes.c_size_t, _vp]
+    lib.ssd_gated_ff_grad_workspace_bytes.argtypes = [P(GatedFfParams), P(GatedFfGrads)]
+    lib.ssd_gated_ff_grad.argtypes = [P(GatedFfParams), P(GatedFfGrads), _vp, ctypes.c_size_t, _vp]
     for name in EXPORTED:
         if name.endswith("_workspace_bytes"):
             getattr(lib, name).restype = ctypes.c_size_t
