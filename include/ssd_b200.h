@@ -465,6 +465,8 @@ typedef struct ssd_gated_recurrence_params {
   float* final_state;         /* (batch, dim), or NULL; unused by the gradient */
   float* checkpoints;         /* (batch, ceil(seqlen / 32), dim): the state before each 32 tokens, or NULL.
                                  Written by the forward pass; read by the gradient, which computes them where NULL */
+  uint32_t* status;           /* device word that the caller has cleared, or NULL: set as ssd_status_decode reads it if
+                                 a bounded wait in a kernel gave up (the channels concerned are NaN then) */
 } ssd_gated_recurrence_params_t;
 
 int ssd_gated_recurrence(const ssd_gated_recurrence_params_t* p, ssd_stream_t stream);
@@ -485,7 +487,7 @@ size_t ssd_gated_recurrence_grad_workspace_bytes(const ssd_gated_recurrence_para
 int ssd_gated_recurrence_grad(const ssd_gated_recurrence_params_t* p, const ssd_gated_recurrence_grads_t* g,
                               void* workspace, size_t workspace_bytes, ssd_stream_t stream);
 
-/* One token of the gated linear recurrence; the state is updated in place. */
+/* One token of the gated linear recurrence. */
 typedef struct ssd_gated_recurrence_update_params {
   int64_t batch, dim;
   int64_t x_stride_row, decay_gate_stride_row, input_gate_stride_row; /* in values */
@@ -495,7 +497,8 @@ typedef struct ssd_gated_recurrence_update_params {
   const void* decay_gate;
   const void* input_gate;
   const float* decay;         /* (dim,) */
-  float* state;               /* (batch, dim) contiguous */
+  const float* state;         /* (batch, dim) contiguous */
+  float* new_state;           /* (batch, dim) contiguous; == state: in place */
   void* y;                    /* (batch, dim) contiguous */
 } ssd_gated_recurrence_update_params_t;
 

@@ -667,8 +667,8 @@ int ssd_gated_recurrence_update(const ssd_gated_recurrence_update_params_t* p, s
   if (p->batch > INT32_MAX || p->dim > INT32_MAX) return fail(SSD_ERR_UNSUPPORTED, "dims must be below 2^31");
   if (!dtype_ok(p->dtype)) return fail(SSD_ERR_INVALID_ARG, "bad dtype enum");
   if (!(p->scale >= 0.f) || p->scale > 3.4e38f) return fail(SSD_ERR_INVALID_ARG, "scale must be finite and not negative");
-  if (!p->x || !p->decay_gate || !p->input_gate || !p->decay || !p->state || !p->y)
-    return fail(SSD_ERR_INVALID_ARG, "x, decay_gate, input_gate, decay, state and y are required");
+  if (!p->x || !p->decay_gate || !p->input_gate || !p->decay || !p->state || !p->new_state || !p->y)
+    return fail(SSD_ERR_INVALID_ARG, "x, decay_gate, input_gate, decay, state, new_state and y are required");
   return cuda_status(ssd::launch_gated_recurrence_update(p, (cudaStream_t)stream), "gated_recurrence_update");
 }
 

@@ -38,8 +38,10 @@ using gemm::EPI_COLS;
 using gemm::EPI_WARPS;
 using gemm::THREADS;
 
-// K blocks summed in TMEM before they are added in registers (the tensor core's adds truncate, tc_gemm.cuh).
-constexpr int SEGMENT_BF16 = 16, SEGMENT_F32 = 1;
+// K blocks summed in TMEM before they are added in registers (the tensor core's adds truncate, tc_gemm.cuh).  Of bf16
+// operands 64 where the sum is rounded to bf16 behind it: the loss, 1.1e-5 and of one sign, is a two-hundredth of that
+// rounding, and the MMAs wait for an epilogue that takes longer than a segment.  32 for the weights' gradients, which may go to f32: 3.5e-6.
+constexpr int SEGMENT_BF16 = 64, SEGMENT_DW = 32, SEGMENT_F32 = 1;
 
 // ---------------------------------------------------------------------------
 // the products' loop
@@ -53,6 +55,7 @@ struct Product {
   int m_tiles, n_tiles, k_blocks; // over all parts
   int half;                       // k blocks (TWO_K) or m tiles (TWO_M) of a part
   int group;                      // m tiles that are walked together, n by n: what they share stays in L2
+  int full;                       // tiles computed whole; the K range of those behind is split
   int splits, segment;
   int clear;                      // the first launch of a call clears the status word
   unsigned* status;
@@ -62,14 +65,26 @@ struct Tile {
   int m, n, split, k0, k1;
 };
 
-__device__ __forceinline__ Tile tile_at(const Product& p, unsigned u) {
+__device__ __forceinline__ Tile tile_of(const Product& p, unsigned r) {
   Tile t;
-  const unsigned per = (unsigned)p.m_tiles * p.n_tiles, split = p.splits == 1 ? 0 : u / per, r = u - split * per;
   const unsigned span = (unsigned)p.group * p.n_tiles, g = r / span, first = g * p.group, q = r - g * span;
   const unsigned rows = min((unsigned)p.group, (unsigned)p.m_tiles - first);
-  t.split = (int)split;
   t.n = (int)(q / rows);
   t.m = (int)(first + q - (unsigned)t.n * rows);
+  t.split = -1;
+  t.k0 = 0;
+  t.k1 = p.k_blocks;
+  return t;
+}
+__device__ __forceinline__ unsigned units_of(const Product& p) {
+  return (unsigned)p.full + ((unsigned)p.m_tiles * p.n_tiles - p.full) * p.splits;
+}
+// Unit u: a whole tile (split -1), or a part of the K range of one of the last tiles.
+__device__ __forceinline__ Tile tile_at(const Product& p, unsigned u) {
+  if (u < (unsigned)p.full) return tile_of(p, u);
+  const unsigned tail = (unsigned)p.m_tiles * p.n_tiles - p.full, v = u - p.full, split = v / tail;
+  Tile t = tile_of(p, p.full + v - split * tail);
+  t.split = (int)v;                // of the parts: split * tail + tile - full
   t.k0 = (int)((unsigned)p.k_blocks * split / p.splits);
   t.k1 = (int)((unsigned)p.k_blocks * (split + 1) / p.splits);
   return t;
@@ -104,7 +119,7 @@ __device__ __forceinline__ void run(const Product& p, uint8_t* smem_raw, gemm::C
   const uint32_t tmem = c->tmem;
   ptx::griddep_wait();   // all above needs nothing from the launches before
   if (p.clear && blockIdx.x == 0 && threadIdx.x == 0) *p.status = 0;   // (a wait takes seconds to give up)
-  const unsigned unit0 = blockIdx.x / CG, units = (unsigned)p.m_tiles * p.n_tiles * p.splits, step = gridDim.x / CG;
+  const unsigned unit0 = blockIdx.x / CG, units = units_of(p), step = gridDim.x / CG;
   const uint32_t smem0 = ptx::smem_u32(smem);
 
   if (warp == 0) {
@@ -119,7 +134,7 @@ __device__ __forceinline__ void run(const Product& p, uint8_t* smem_raw, gemm::C
         for (int kb = t.k0; ok && kb < t.k1; ++kb) {
           const int ka = PARTS == TWO_K && kb >= p.half, k = (kb - (ka ? p.half : 0)) * BK;
 #pragma unroll
-          for (int pl = 0; pl < PLANES; ++pl, ++it) {
+          for (int pl = PLANES - 1; pl >= 0; --pl, ++it) {   // the lowest terms first
             if (!gemm::wait(c, &c->empty[s], phase, p.status, 1)) {
               ok = false;
               break;
@@ -184,31 +199,36 @@ __device__ __forceinline__ void run(const Product& p, uint8_t* smem_raw, gemm::C
             ptx::tc_fence_after();
             d = tmem + (n & 1) * BN;
           }
-          // plane i lies in the i-th stage from here; its products are those with the planes up to it, as
-          // far as they count
+          // Small products first: what an add cuts off goes by the sum that is there (three planes, products in the order
+          // of the planes: gradients 2.3e-6 off).  The lowest plane's stage is free first, and was loaded first.
           uint32_t at[PLANES];
+          uint64_t* done[PLANES];
 #pragma unroll
-          for (int i = 0; i < PLANES; ++i) {
-            if (!gemm::wait(c, &c->full[s], phase, p.status, 3)) {
-              ok = false;
-              break;
-            }
-            ptx::tc_fence_after();
+          for (int i = PLANES - 1; i >= 0; --i) {
+            if (ok && !gemm::wait(c, &c->full[s], phase, p.status, 3)) ok = false;
             at[i] = smem0 + s * S::STAGE_BYTES;
-#pragma unroll
-            for (int j = 0; j <= i; ++j) {
-              if (i + j >= PLANES) continue;
-              gemm::mma_block<CG, A_MN, B_MN>(d, at[j], at[i] + S::A_BYTES, ID, !(first && i == 0));
-              if (j < i) gemm::mma_block<CG, A_MN, B_MN>(d, at[i], at[j] + S::A_BYTES, ID, true);
-            }
+            done[i] = &c->empty[s];
             if (++s == S::STAGES) {
               s = 0;
               phase ^= 1;
             }
           }
           if (!ok) break;
-#pragma unroll
-          for (int i = 0; i < PLANES; ++i) gemm::commit<CG>(&c->empty[(s + S::STAGES - PLANES + i) % S::STAGES]);
+          ptx::tc_fence_after();
+          auto product = [&](int i, int j, bool add) { gemm::mma_block<CG, A_MN, B_MN>(d, at[i], at[j] + S::A_BYTES, ID, add); };
+          if constexpr (PLANES == 3) {
+            product(1, 1, !first);
+            product(0, 2, true);
+            product(2, 0, true);
+            gemm::commit<CG>(done[2]);
+            product(0, 1, true);
+            product(1, 0, true);
+            gemm::commit<CG>(done[1]);
+            product(0, 0, true);
+          } else {
+            product(0, 0, !first);
+          }
+          gemm::commit<CG>(done[0]);
           if (left == 1) {
             gemm::commit<CG>(&c->acc_full[n & 1]);
             ++n;
@@ -284,35 +304,26 @@ __device__ __forceinline__ void run(const Product& p, uint8_t* smem_raw, gemm::C
 // ---------------------------------------------------------------------------
 // f32 values as three bf16 terms
 // ---------------------------------------------------------------------------
-// v = t[0] + t[1] + t[2] up to 2^-25 of it.  A value that is not finite has no rest, nor has one that rounds up to infinity.
-__device__ __forceinline__ void terms3(float v, float (&t)[3]) {
-  float r = v;
-#pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    float q = __bfloat162float(__float2bfloat16_rn(r));
-    if (isinf(q) && !isinf(v)) q = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
-    t[i] = q;
-    r = isinf(v) ? 0.f : r - q;
-  }
+// Two values as a pair of bf16, and what is left of them.  A finite value that would round to infinity is cut instead.  (What
+// is left of an infinity is NaN: a value that is not finite makes its products so.)
+__device__ __forceinline__ uint32_t term_of(float& a, float& b) {
+  uint32_t w = gemm::pack_bf16(a, b);
+  if ((w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u) w = __float_as_uint(a) >> 16 | (__float_as_uint(b) & 0xffff0000u);
+  a -= __uint_as_float(w << 16);
+  b -= __uint_as_float(w & 0xffff0000u);
+  return w;
 }
 
-// 8 values as planes of 16 bytes each.
+// 8 values as planes of 16 bytes each: v = t[0] + t[1] + t[2] up to 2^-25 of it.
 template <int PLANES>
-__device__ __forceinline__ void planes_of(const float (&v)[8], uint4 (&q)[PLANES]) {
+__device__ __forceinline__ void planes_of(const float (&x)[8], uint4 (&q)[PLANES]) {
   if constexpr (PLANES == 1) {
-    q[0] = make_uint4(gemm::pack_bf16(v[0], v[1]), gemm::pack_bf16(v[2], v[3]), gemm::pack_bf16(v[4], v[5]), gemm::pack_bf16(v[6], v[7]));
+    q[0] = make_uint4(gemm::pack_bf16(x[0], x[1]), gemm::pack_bf16(x[2], x[3]), gemm::pack_bf16(x[4], x[5]), gemm::pack_bf16(x[6], x[7]));
   } else {
-    uint32_t w[3][4];
+    float v[8] = {x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float a[3], b[3];
-      terms3(v[2 * k], a);
-      terms3(v[2 * k + 1], b);
-#pragma unroll
-      for (int i = 0; i < 3; ++i) w[i][k] = gemm::pack_bf16(a[i], b[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < 3; ++i) q[i] = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
+    for (int i = 0; i < PLANES; ++i)
+      q[i] = make_uint4(term_of(v[0], v[1]), term_of(v[2], v[3]), term_of(v[4], v[5]), term_of(v[6], v[7]));
   }
 }
 
@@ -373,18 +384,33 @@ struct HiddenArgs {
   const float* dh;                 // (T, ld)
 };
 
-// 32 rows x 32 columns of bf16 from packed rows, by lines of 64 bytes (neighbouring lanes at neighbouring columns).
-__device__ __forceinline__ void store_block(uint4* stage, const uint4 (&q)[4], uint8_t* out, int64_t ld, int row0, int rows, int64_t f0, int64_t F) {
+// 32 rows x 8 N columns of bf16 from packed rows, by runs of 16 N bytes (neighbouring lanes at neighbouring columns).
+template <int N>
+__device__ __forceinline__ void store_block(uint4* stage, const uint4 (&q)[N], uint8_t* out, int64_t ld, int row0, int rows, int64_t f0, int64_t F) {
+  const int lane = threadIdx.x & 31;
+  auto at = [](int i, int k) { return N == 4 ? gemm::epi_at<1>(i, k) : i * 2 + (k ^ (i >> 2 & 1)); };
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < N; ++i) stage[at(lane, i)] = q[i];
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int i = j * (32 / N) + lane / N, k = lane % N;
+    if (row0 + i < rows && f0 + k * 8 < F) *reinterpret_cast<uint4*>(out + ((int64_t)(row0 + i) * ld + f0 + k * 8) * 2) = stage[at(i, k)];
+  }
+}
+
+// dh of 32 rows and 4 CHUNKS columns on its way into the warp's stage.
+template <int CHUNKS>
+__device__ __forceinline__ void fetch_block(uint4* stage, const HiddenArgs& a, int row0, int64_t f0) {
   const int lane = threadIdx.x & 31;
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) stage[gemm::epi_at<1>(lane, i)] = q[i];
-  __syncwarp();
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int i = j * 8 + lane / 4, k = lane % 4;
-    if (row0 + i < rows && f0 + k * 8 < F)
-      *reinterpret_cast<uint4*>(out + ((int64_t)(row0 + i) * ld + f0 + k * 8) * 2) = stage[gemm::epi_at<1>(i, k)];
+  for (int j = 0; j < CHUNKS; ++j) {
+    const int i = j * (32 / CHUNKS) + lane / CHUNKS, k = lane % CHUNKS;
+    const bool there = row0 + i < a.rows && f0 + k * 4 < a.ld;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(stage + gemm::epi_at<CHUNKS / 4>(i, k))),
+                 "l"(there ? a.dh + (int64_t)(row0 + i) * a.ld + f0 + k * 4 : a.dh), "r"(there ? 16 : 0) : "memory");
   }
 }
 
@@ -392,74 +418,101 @@ template <int CG, int PLANES, int ACT, bool BACKWARD>
 __global__ void __launch_bounds__(THREADS, 1) hidden_kernel(const __grid_constant__ Product p, const __grid_constant__ HiddenArgs a) {
   extern __shared__ uint8_t smem[];
   __shared__ gemm::Ctl ctl;
-  constexpr int CHUNKS = gemm::Shape<CG>::EPI_ROW / 16, HALVES = 8 / CHUNKS;   // 16-byte pieces of dh in a staged row
-  // dh of the warp's block, or of the left half of its columns, on its way while the tile is computed
-  auto fetch = [&](uint4* stage, int row0, int64_t f0) {
-    const int lane = threadIdx.x & 31;
-    __syncwarp();
-#pragma unroll
-    for (int j = 0; j < CHUNKS; ++j) {
-      const int i = j * (32 / CHUNKS) + lane / CHUNKS, k = lane % CHUNKS;
-      const bool there = row0 + i < a.rows && f0 + k * 4 < a.ld;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(stage + gemm::epi_at<CG>(i, k))),
-                   "l"(there ? a.dh + (int64_t)(row0 + i) * a.ld + f0 + k * 4 : a.dh), "r"(there ? 16 : 0) : "memory");
-    }
-  };
+  // columns that are turned into results at a time: the warp's 32, or 16 where shared memory (one SM's tiles) or registers (three
+  // terms a value) are short
+  constexpr int COLS = CG == 2 && PLANES == 1 ? 32 : 16, CHUNKS = COLS / 4;
   run<CG, PLANES, false, false, DUAL>(p, smem, &ctl, [&](const Tile& t, int row0, int group, uint4* stage) {
-    if constexpr (BACKWARD) fetch(stage, row0, (int64_t)t.n * (BN / 2) + group * 32);
+    if constexpr (BACKWARD) fetch_block<CHUNKS>(stage, a, row0, (int64_t)t.n * (BN / 2) + group * 32);   // while the tile is computed
   }, [&](const Tile& t, float (&v)[EPI_COLS], int row0, int group, uint4* stage) {
-    const int lane = threadIdx.x & 31, row = row0 + lane;
-    const int64_t f0 = (int64_t)t.n * (BN / 2) + group * 32;
-    auto put = [&](uint8_t* out, int i, const uint4 (&q)[PLANES]) {   // f32: a lane's own 16 bytes of its row
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-      for (int k = 0; k < PLANES; ++k)
-        if (row < a.rows && f0 + i * 8 < a.F) *reinterpret_cast<uint4*>(out + k * a.plane + ((int64_t)row * a.ld + f0 + i * 8) * 2) = q[k];
-    };
-    uint4 h[4], dg[4], du[4];
-#pragma unroll
-    for (int half = 0; half < (BACKWARD ? HALVES : 1); ++half) {
+    for (int c0 = 0; c0 < 32; c0 += COLS) {
+      const int64_t f0 = (int64_t)t.n * (BN / 2) + group * 32 + c0;
       if constexpr (BACKWARD) {
-        if (half > 0) fetch(stage, row0, f0 + half * CHUNKS * 4);
+        if (c0 > 0) fetch_block<CHUNKS>(stage, a, row0, f0);
         asm volatile("cp.async.wait_all;" ::: "memory");
         __syncwarp();
       }
+      // results over the accumulators: dg over g, du over u (h over g forward)
+      uint4 h[COLS / 8];
+      float hv[8];
 #pragma unroll
-      for (int j = 0; j < 4 / (BACKWARD ? HALVES : 1); ++j) {
-        const int i = half * (4 / HALVES) + j;
-        float hv[8], gv[8], uv[8];
+      for (int i = 0; i < COLS; i += 4) {
+        float4 d = make_float4(0.f, 0.f, 0.f, 0.f);
+        if constexpr (BACKWARD) d = *reinterpret_cast<const float4*>(stage + gemm::epi_at<CHUNKS / 4>(lane, i / 4));
+        const float dv[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float g = v[i * 8 + k], u = v[32 + i * 8 + k];
-          float slope, act;
+        for (int k = 0; k < 4; ++k) {
+          float &g = v[c0 + i + k], &u = v[32 + c0 + i + k], slope;
+          const float act = ff::activate<ACT>(g, BACKWARD ? &slope : nullptr), hk = act * u;
           if constexpr (BACKWARD) {
-            const float d = reinterpret_cast<const float*>(stage + gemm::epi_at<CG>(lane, j * 2 + k / 4))[k % 4];
-            act = ff::activate<ACT>(g, &slope);
-            gv[k] = d * u * slope;
-            uv[k] = d * act;
+            g = dv[k] * u * slope;
+            u = dv[k] * act;
           } else {
-            act = ff::activate<ACT>(g, nullptr);
+            g = hk;
           }
-          hv[k] = act * u;
+          if constexpr (BACKWARD && PLANES == 1) hv[i % 8 + k] = hk;
+          // (three terms: h again from what dg and du are made of would need both; it goes through shared memory)
+          if constexpr (BACKWARD && PLANES == 3) reinterpret_cast<float*>(stage + gemm::epi_at<CHUNKS / 4>(lane, i / 4))[k] = hk;
         }
-        uint4 q[PLANES];
-        planes_of<PLANES>(hv, q);
-        if constexpr (PLANES == 1) h[i] = q[0];
-        else put(a.h, i, q);
-        if constexpr (BACKWARD) {
-          planes_of<PLANES>(gv, q);
-          if constexpr (PLANES == 1) dg[i] = q[0];
-          else put(a.dg, i, q);
-          planes_of<PLANES>(uv, q);
-          if constexpr (PLANES == 1) du[i] = q[0];
-          else put(a.du, i, q);
+        if constexpr (BACKWARD && PLANES == 1) {
+          if (i % 8 == 4) {
+            uint4 q[1];
+            planes_of<1>(hv, q);
+            h[i / 8] = q[0];
+          }
         }
       }
-    }
-    if constexpr (PLANES == 1) {
-      if (a.h) store_block(stage, h, a.h, a.ld, row0, a.rows, f0, a.F);
-      if constexpr (BACKWARD) {
-        store_block(stage, dg, a.dg, a.ld, row0, a.rows, f0, a.F);
-        store_block(stage, du, a.du, a.ld, row0, a.rows, f0, a.F);
+      if constexpr (PLANES == 1) {
+        if constexpr (!BACKWARD) {
+#pragma unroll
+          for (int i = 0; i < COLS / 8; ++i)
+            h[i] = make_uint4(gemm::pack_bf16(v[c0 + 8 * i], v[c0 + 8 * i + 1]), gemm::pack_bf16(v[c0 + 8 * i + 2], v[c0 + 8 * i + 3]),
+                              gemm::pack_bf16(v[c0 + 8 * i + 4], v[c0 + 8 * i + 5]), gemm::pack_bf16(v[c0 + 8 * i + 6], v[c0 + 8 * i + 7]));
+          store_block(stage, h, a.h, a.ld, row0, a.rows, f0, a.F);
+        } else {
+          store_block(stage, h, a.h, a.ld, row0, a.rows, f0, a.F);
+#pragma unroll
+          for (int which = 0; which < 2; ++which) {
+            const float* x = v + 32 * which + c0;
+#pragma unroll
+            for (int i = 0; i < COLS / 8; ++i)
+              h[i] = make_uint4(gemm::pack_bf16(x[8 * i], x[8 * i + 1]), gemm::pack_bf16(x[8 * i + 2], x[8 * i + 3]),
+                                gemm::pack_bf16(x[8 * i + 4], x[8 * i + 5]), gemm::pack_bf16(x[8 * i + 6], x[8 * i + 7]));
+            store_block(stage, h, which ? a.du : a.dg, a.ld, row0, a.rows, f0, a.F);
+          }
+        }
+      } else {
+        // three planes of one result after another
+        auto put = [&](float (&x)[COLS], uint8_t* out) {
+#pragma unroll
+          for (int k = 0; k < PLANES; ++k) {
+#pragma unroll
+            for (int i = 0; i < COLS / 8; ++i)
+              h[i] = make_uint4(term_of(x[8 * i], x[8 * i + 1]), term_of(x[8 * i + 2], x[8 * i + 3]), term_of(x[8 * i + 4], x[8 * i + 5]),
+                                term_of(x[8 * i + 6], x[8 * i + 7]));
+            store_block(stage, h, out + k * a.plane, a.ld, row0, a.rows, f0, a.F);
+          }
+        };
+        float x[COLS];
+        if constexpr (BACKWARD) {
+#pragma unroll
+          for (int i = 0; i < COLS; i += 4) {
+            const float4 d = *reinterpret_cast<const float4*>(stage + gemm::epi_at<CHUNKS / 4>(lane, i / 4));
+            x[i] = d.x; x[i + 1] = d.y; x[i + 2] = d.z; x[i + 3] = d.w;
+          }
+          put(x, a.h);
+#pragma unroll
+          for (int i = 0; i < COLS; ++i) x[i] = v[c0 + i];
+          put(x, a.dg);
+#pragma unroll
+          for (int i = 0; i < COLS; ++i) x[i] = v[32 + c0 + i];
+          put(x, a.du);
+        } else {
+#pragma unroll
+          for (int i = 0; i < COLS; ++i) x[i] = v[c0 + i];
+          put(x, a.h);
+        }
       }
     }
   });
@@ -473,7 +526,7 @@ struct OutArgs {
   void* out[2];                    // of the parts (TWO_M), else the first
   int bf16_out;
   int64_t m_rows;                  // rows of the tiles of a part: m tiles of a part start at row 0
-  float* part;                     // f32 parts of a split K range (splits, parts * rows, cols)
+  float* part;                     // f32 parts of split tiles: (splits, tiles, rows, BN)
 };
 
 template <int CG, int PLANES, bool A_MN, bool B_MN, int PARTS>
@@ -486,7 +539,11 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
     const int64_t row0 = second ? row_of - a.m_rows : row_of, n0 = (int64_t)t.n * BN + group * EPI_COLS;
     const int rows = (int)min((int64_t)32, a.rows - row0), cols = (int)min((int64_t)EPI_COLS, a.cols - n0);
     if (rows <= 0 || cols <= 0) return;
-    if (p.splits == 1 && a.bf16_out) {
+    if (t.split >= 0) {
+      float* o = a.part + ((int64_t)t.split * BM * CG + row_of - t.m * BM * CG) * BN + group * EPI_COLS;
+      gemm::by_rows<CG, float>(stage, v, true, rows, [&](int i, int c, uint4 q) { *reinterpret_cast<uint4*>(o + i * BN + c) = q; },
+                               [](int, int, float) {});
+    } else if (a.bf16_out) {
       bf16* o = static_cast<bf16*>(a.out[second]) + row0 * a.ld + n0;
       const bool wide = reinterpret_cast<uintptr_t>(o) % 16 == 0 && a.ld % 8 == 0 && cols % 8 == 0;
       gemm::by_rows<CG, bf16>(stage, v, wide, rows, [&](int i, int c, uint4 q) {
@@ -495,33 +552,53 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
         if (c < cols) o[i * a.ld + c] = x;
       });
     } else {
-      const int64_t ld = p.splits == 1 ? a.ld : a.cols;
-      float* o = p.splits == 1 ? static_cast<float*>(a.out[second]) + row0 * ld + n0
-                               : a.part + (((int64_t)t.split * (PARTS == TWO_M ? 2 : 1) + second) * a.rows + row0) * ld + n0;
-      const bool wide = reinterpret_cast<uintptr_t>(o) % 16 == 0 && ld % 4 == 0 && cols % 4 == 0;
+      float* o = static_cast<float*>(a.out[second]) + row0 * a.ld + n0;
+      const bool wide = reinterpret_cast<uintptr_t>(o) % 16 == 0 && a.ld % 4 == 0 && cols % 4 == 0;
       gemm::by_rows<CG, float>(stage, v, wide, rows, [&](int i, int c, uint4 q) {
-        if (c < cols) *reinterpret_cast<uint4*>(o + i * ld + c) = q;
+        if (c < cols) *reinterpret_cast<uint4*>(o + i * a.ld + c) = q;
       }, [&](int i, int c, float x) {
-        if (c < cols) o[i * ld + c] = x;
+        if (c < cols) o[i * a.ld + c] = x;
       });
     }
   });
 }
 
-// Sum of the parts of a split K range, in order.  CTAs take rows of the result in turns; bound by L2.
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ OutArgs a, int splits, int parts) {
+// Sum of the parts of split tiles, in order: a warp takes a row of a tile, 4 columns a lane and half.  Bound by L2.
+template <int CG>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Product p, const __grid_constant__ OutArgs a) {
   ptx::griddep_wait();
-  const int64_t rows = parts * a.rows, step = rows * a.cols;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const int second = row >= a.rows;
-    const float* q = a.part + row * a.cols;
-    const int64_t at = (second ? row - a.rows : row) * a.ld;
-    for (int64_t c = threadIdx.x; c < a.cols; c += 256) {
-      float v = 0.f;
+  constexpr int ROWS = BM * CG;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tail = p.m_tiles * p.n_tiles - p.full;
+  const int index = blockIdx.x / (ROWS / 8), r = blockIdx.x % (ROWS / 8) * 8 + warp;
+  const Tile t = tile_of(p, p.full + index);
+  const int second = a.out[1] != nullptr && t.m >= p.half;
+  const int64_t row = (int64_t)t.m * ROWS + r - (second ? a.m_rows : 0);
+  if (row >= a.rows) return;
+  const float* q = a.part + ((int64_t)index * ROWS + r) * BN;
+  const int64_t step = (int64_t)tail * ROWS * BN, n0 = (int64_t)t.n * BN, at = row * a.ld + n0;
+  const bool wide = a.ld % 4 == 0 && reinterpret_cast<uintptr_t>(a.out[second]) % 16 == 0;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int c = half * 128 + lane * 4;
+    if (n0 + c >= a.cols) continue;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-      for (int j = 0; j < splits; ++j) v += q[j * step + c];
-      if (a.bf16_out) st(static_cast<bf16*>(a.out[second]) + at + c, v);
-      else static_cast<float*>(a.out[second])[at + c] = v;
+    for (int j = 0; j < p.splits; ++j) {
+      const float4 x = *reinterpret_cast<const float4*>(q + j * step + c);
+      v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+    }
+    if (wide && n0 + c + 4 <= a.cols) {
+      if (a.bf16_out) *reinterpret_cast<uint2*>(static_cast<bf16*>(a.out[second]) + at + c) = make_uint2(gemm::pack_bf16(v.x, v.y), gemm::pack_bf16(v.z, v.w));
+      else *reinterpret_cast<float4*>(static_cast<float*>(a.out[second]) + at + c) = v;
+    } else {
+      const float w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (n0 + c + k >= a.cols) break;
+        if (a.bf16_out) st(static_cast<bf16*>(a.out[second]) + at + c + k, w[k]);
+        else static_cast<float*>(a.out[second])[at + c + k] = w[k];
+      }
     }
   }
 }
@@ -530,8 +607,8 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ OutAr
 // host side
 // ---------------------------------------------------------------------------
 constexpr int SMS = 148;   // of a B200
-constexpr int MAX_SPLITS = 16;
-constexpr int GROUP = 16;  // m tiles of a walk
+constexpr int MAX_SPLITS = 32;
+constexpr int GROUP = 8;   // m tiles of a walk: the 74 tiles at work are then about as many rows as columns of tiles
 
 size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
@@ -550,30 +627,36 @@ bool maps(CUtensorMap (&m)[3], const Operand& o, int planes, uint32_t box) {
   return true;
 }
 
-// Parts of the K range: enough units of work for all pairs where a result has few tiles.  In K blocks of one
-// wave (a unit's start and epilogue count as 12), and 8 bytes a value and part written and read again (a K block takes 0.37 us, which
-// is 2.2 MB at 6 TB/s).
-int pick_splits(int64_t tiles, int ctas, int64_t blocks, int64_t values) {
-  int best = 1;
-  double least = 1e300;
-  for (int s = 1; s <= MAX_SPLITS && s <= blocks; ++s) {
-    const double waves = (double)((tiles * s + ctas - 1) / ctas);
-    double cost = waves * (double)((blocks + s - 1) / s + 12);
-    if (s > 1) cost += (double)s * (double)values * 3.6e-6 + 8.0;
+// Which tiles are computed whole, and into how many parts the K range of the others goes.  Whole rounds of tiles fill all CTAs;
+// those left over are split so that the last round is short (2560 x 7680 over 16384 tokens, 300 tiles on 74 pairs: 620 -> 525 us under the
+// power limit; 4096 x 4096 over 12288: 335 -> 313).  In K blocks of a unit (its start and epilogue count as 12), and 8 bytes a value and part written and
+// read again (a K block takes 0.37 us, which is 2.2 MB at 6 TB/s).
+void pick_splits(int64_t tiles, int pairs, int64_t blocks, int per, int values, int* full, int* splits) {
+  *full = (int)tiles;
+  *splits = 1;
+  const int64_t tail = tiles % pairs;
+  if (tail == 0) return;
+  double least = (double)(blocks * per + 12);
+  for (int s = 2; s <= MAX_SPLITS && s <= blocks; ++s) {
+    const double rounds = (double)((tail * s + pairs - 1) / pairs);
+    const double cost = rounds * (double)((blocks + s - 1) / s * per + 12) + (double)(tail * s) * values * 3.6e-6 + 8.0;
     if (cost < least) {
       least = cost;
-      best = s;
+      *full = (int)(tiles - tail);
+      *splits = s;
     }
   }
-  return best;
 }
 
 enum Step { Y, DH, DX, DW_IN, DW_OUT, STEPS };
 
 // One product of a call.
 struct Plan {
-  int cg, splits, m_tiles, n_tiles, k_blocks, half, parts;
+  int cg, full, splits, m_tiles, n_tiles, k_blocks, half, parts;
   int64_t rows, cols;              // of a part of the result
+
+  int64_t tail() const { return (int64_t)m_tiles * n_tiles - full; }
+  int64_t part_values() const { return tail() * splits * BM * cg * BN; }
 };
 
 Plan plan_of(int step, const ssd_gated_ff_params_t* p) {
@@ -595,8 +678,7 @@ Plan plan_of(int step, const ssd_gated_ff_params_t* p) {
   q.k_blocks = cdiv(k, BK) * (step == DX ? 2 : 1);
   q.half = step == DX ? q.k_blocks / 2 : q.m_tiles / 2;
   const int per = p->dtype == SSD_DTYPE_F32 ? 6 : 1;   // products a K block
-  q.splits = pick_splits((int64_t)q.m_tiles * q.n_tiles, SMS / q.cg, (int64_t)q.k_blocks * per, q.parts * q.rows * q.cols);
-  q.splits = std::min(q.splits, q.k_blocks);
+  pick_splits((int64_t)q.m_tiles * q.n_tiles, SMS / q.cg, q.k_blocks, per, BM * q.cg * BN, &q.full, &q.splits);
   return q;
 }
 
@@ -649,7 +731,7 @@ Layout layout_of(const ssd_gated_ff_params_t* p, const ssd_gated_ff_grads_t* g) 
   int64_t part = 0;
   auto parts = [&](int step) {
     const Plan s = plan_of(step, p);
-    if (s.splits > 1) part = std::max(part, s.splits * s.parts * s.rows * s.cols);
+    part = std::max(part, s.part_values());
   };
   if (!g) {
     parts(Y);
@@ -682,9 +764,15 @@ cudaError_t launch_tiles(const Product& p, const A& a, cudaStream_t st) {
   constexpr int smem = gemm::Shape<CG>::SMEM;
   const cudaError_t e = allow_smem((const void*)KERNEL, smem, &allowed);
   if (e != cudaSuccess) return e;
-  const int64_t units = (int64_t)p.m_tiles * p.n_tiles * p.splits;
-  if (units >= (int64_t(1) << 31) || (int64_t)p.k_blocks * MAX_SPLITS >= (int64_t(1) << 31)) return cudaErrorInvalidValue;
+  const int64_t units = p.full + ((int64_t)p.m_tiles * p.n_tiles - p.full) * p.splits;
+  if ((int64_t)p.m_tiles * p.n_tiles >= (int64_t(1) << 31) || units >= (int64_t(1) << 31) || (int64_t)p.k_blocks * MAX_SPLITS >= (int64_t(1) << 31)) return cudaErrorInvalidValue;
   return launch_dependent(KERNEL, dim3((unsigned)(CG * std::min<int64_t>(units, SMS / CG))), THREADS, smem, CG, st, p, a);
+}
+
+// Segments of nearly the same length, at most `most`.
+int even_segment(int blocks, int most) {
+  const int n = (blocks + most - 1) / most;
+  return (blocks + n - 1) / n;
 }
 
 template <int CG, int PLANES, bool BACKWARD>
@@ -706,8 +794,9 @@ cudaError_t hidden(const ssd_gated_ff_params_t* p, const Layout& q, const Operan
   g.n_tiles = cdiv(p->hidden, BN / 2);
   g.k_blocks = cdiv(p->dim, BK);
   g.group = GROUP;
+  g.full = g.m_tiles * g.n_tiles;
   g.splits = 1;
-  g.segment = PLANES == 3 ? SEGMENT_F32 : SEGMENT_BF16;
+  g.segment = PLANES == 3 ? SEGMENT_F32 : even_segment(g.k_blocks, SEGMENT_BF16);
   g.clear = clear;
   g.status = status;
   return a.dh ? launch_hidden<CG, PLANES, true>(p->activation, g, a, st) : launch_hidden<CG, PLANES, false>(p->activation, g, a, st);
@@ -727,8 +816,9 @@ cudaError_t product_as(const Plan& s, const Operand (&a)[2], const Operand (&b)[
   g.k_blocks = s.k_blocks;
   g.half = s.half;
   g.group = GROUP;
+  g.full = s.full;
   g.splits = s.splits;
-  g.segment = PLANES == 3 ? SEGMENT_F32 : SEGMENT_BF16;
+  g.segment = PLANES == 3 ? SEGMENT_F32 : even_segment(s.k_blocks, A_MN ? SEGMENT_DW : SEGMENT_BF16);
   g.clear = clear;
   g.status = status;
   OutArgs o{};
@@ -741,8 +831,8 @@ cudaError_t product_as(const Plan& s, const Operand (&a)[2], const Operand (&b)[
   o.m_rows = (int64_t)s.half * BM * CG;
   o.part = part;
   const cudaError_t e = launch_tiles<product_kernel<CG, PLANES, A_MN, B_MN, PARTS>, CG>(g, o, st);
-  if (e != cudaSuccess || s.splits == 1) return e;
-  return launch_dependent(join_kernel, dim3((unsigned)std::min<int64_t>(s.parts * s.rows, SMS * 8)), 256, 0, 1, st, o, s.splits, s.parts);
+  if (e != cudaSuccess || s.tail() == 0) return e;
+  return launch_dependent(join_kernel<CG>, dim3((unsigned)(s.tail() * (BM * CG / 8))), 256, 0, 1, st, g, o);
 }
 
 template <bool A_MN, bool B_MN, int PARTS, typename... Args>

@@ -100,14 +100,16 @@ __global__ void __launch_bounds__(32 * WARPS) few_kernel(const __grid_constant__
   float sum[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) sum[i] = 0.f;
-  constexpr int AHEAD = W * ROWS >= 4 ? 2 : 4;
+  // pieces of the weights on their way, always this many steps ahead
+  constexpr int AHEAD = W * ROWS == 1 ? 8 : W * ROWS == 2 ? 6 : 3;
   Piece<T> w[AHEAD][W * ROWS];
-  auto fetch = [&](int s) {
+  auto fetch = [&](int k, int s) {
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k)
+    for (int i = 0; i < W * ROWS; ++i) w[k][i] = load<T, ALIGNED>(row[i], s < s1 ? (s * 32 + lane) * Piece<T>::N : a.K, a.K);
+  };
+  auto start = [&]() {
 #pragma unroll
-      for (int i = 0; i < W * ROWS; ++i)
-        w[k][i] = load<T, ALIGNED>(row[i], s + k < s1 ? ((s + k) * 32 + lane) * Piece<T>::N : a.K, a.K);
+    for (int k = 0; k < AHEAD; ++k) fetch(k, s0 + k);
   };
   // The first launch waits for whatever ran before it (an optimizer may have written the weights) and lets the second
   // one be set up, which may read its weight at once: the first has waited for that.
@@ -115,9 +117,9 @@ __global__ void __launch_bounds__(32 * WARPS) few_kernel(const __grid_constant__
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
-    fetch(s0);
+    start();
   } else {
-    fetch(s0);
+    start();
     ptx::griddep_wait();
   }
   for (int s = s0; s < s1; s += AHEAD) {
@@ -132,8 +134,8 @@ __global__ void __launch_bounds__(32 * WARPS) few_kernel(const __grid_constant__
 #pragma unroll
           for (int i = 0; i < W * ROWS; ++i) sum[t * W * ROWS + i] = fmaf(v.at(j), w[k][i].at(j), sum[t * W * ROWS + i]);
       }
+      fetch(k, s + k + AHEAD);
     }
-    if (s + AHEAD < s1) fetch(s + AHEAD);
   }
   const float total = warp_sums<N>(sum);
   if (lane < N) sh[warp][lane] = total;

@@ -182,6 +182,14 @@ __device__ __forceinline__ float exp_near(float v) {
   const float p = fmaf(f, fmaf(f, fmaf(f, fmaf(f, fmaf(f, fmaf(f, fmaf(f, 1.f / 5040, 1.f / 720), 1.f / 120), 1.f / 24), 1.f / 6), 0.5f), 1.f), 1.f);
   return p * exp2f(n);
 }
+// 2^v for v <= 0 likewise: what a run of steps leaves of the state multiplies hundreds of times along a sequence (by the approximate
+// instruction gradients of states 2048 tokens back were 1.3e-6 off)
+__device__ __forceinline__ float exp2_near(float v) {
+  constexpr float L = 0.6931471805599453f, L2 = L * L, L3 = L2 * L, L4 = L2 * L2, L5 = L4 * L, L6 = L3 * L3, L7 = L6 * L;
+  const float c = fmaxf(v, -200.f), n = rintf(c), f = c - n;
+  const float p = fmaf(f, fmaf(f, fmaf(f, fmaf(f, fmaf(f, fmaf(f, fmaf(f, L7 / 5040, L6 / 720), L5 / 120), L4 / 24), L3 / 6), L2 / 2), L), 1.f);
+  return p * __int_as_float((max((int)n, -127) + 127) << 23);
+}
 __device__ __forceinline__ float softplus(float v) { return v > 20.f ? v : log1pf(exp_near(v)); }
 
 // 1 / (1 + e^-v); 0 where e^-v is beyond 2^126.  (Two at once by one reciprocal of the product save the special-function unit,
@@ -250,7 +258,8 @@ struct Peers {
   uint64_t* bars;          // [2]
   int cluster, rank;
   int slots;               // of a buffer: the cluster's, and up to the next four that change nothing
-  bool broken;             // a wait gave up
+  unsigned* status;        // or NULL
+  bool broken;             // a wait gave up: the CTA's results are NaN
 
   __device__ __forceinline__ void arm(int par) { ptx::mbar_arrive_expect_tx(&bars[par], (uint32_t)(cluster * 32 * sizeof(Map))); }
   __device__ __forceinline__ void start() {
@@ -275,7 +284,10 @@ struct Peers {
   __device__ __forceinline__ const Map* wait(int64_t turn) {
     const int par = (int)(turn & 1);
     const uint32_t phase = (uint32_t)(turn >> 1) & 1;
-    if (!broken && !ptx::mbar_try_wait(&bars[par], phase) && !wait_long(&bars[par], phase)) broken = true;
+    if (!broken && !ptx::mbar_try_wait(&bars[par], phase) && !wait_long(&bars[par], phase)) {
+      broken = true;
+      if (status) atomicCAS(status, 0u, 0x101u);
+    }
     if (threadIdx.x == 0 && !broken) arm(par);   // of turn + 2, which no peer sends before this CTA's warps have met again
     return maps + par * slots * 32 + (threadIdx.x & 31);
   }
@@ -308,6 +320,7 @@ struct Args {
   void* out[3];                    // y (or NULL); dx, ddecay_gate, dinput_gate: (b, L, D)
   float* state_out;                // (b, D) after the last token, or NULL; grad of state_in, or NULL
   float* part;                     // (b * cluster, D): sums of delta m
+  unsigned* status;                // or NULL: set where a wait gave up
   int64_t L, D, points, groups;
   float scale;
 };
@@ -442,7 +455,7 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) forward_kernel(
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = cluster > 1 ? (int)cluster_rank() : 0;
   const int64_t unit = blockIdx.x / (unsigned)cluster, b = unit / a.groups, c0 = (unit - b * a.groups) * (32 * CH), c = c0 + lane * CH;
-  Peers<T, WARPS> peers{maps + 2 * WARPS * 32, bars, cluster, rank, (cluster + 3) & ~3, false};
+  Peers<T, WARPS> peers{maps + 2 * WARPS * 32, bars, cluster, rank, (cluster + 3) & ~3, a.status, false};
   const int64_t tiles = (a.L + TILE - 1) / TILE, turns = (tiles + cluster - 1) / cluster, ahead = (int64_t)cluster * TILE;
   const int64_t first = (int64_t)rank * TILE + warp * STEPS;
   In in(a, smem, b, c0, first);
@@ -488,7 +501,7 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) forward_kernel(
     if (near) gates(std::true_type());
     else gates(std::false_type());
     Map* const own = maps + (stage * WARPS) * 32 + lane;
-    const V P = PACKED && starts ? all<V>(RESTART) : each(sum, [](float t) { return ex2(t); });
+    const V P = PACKED && starts ? all<V>(RESTART) : each(sum, [](float t) { return exp2_near(t); });
     own[warp * 32] = Lane<T>::map(P, H);
     __syncthreads();
     V h;                   // the state before the CTA's tile, then before the warp's steps
@@ -558,7 +571,7 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) backward_kernel
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = cluster > 1 ? (int)cluster_rank() : 0;
   const int64_t unit = blockIdx.x / (unsigned)cluster, b = unit / a.groups, c0 = (unit - b * a.groups) * (32 * CH), c = c0 + lane * CH;
-  Peers<T, WARPS> peers{maps + 2 * WARPS * 32, bars, cluster, rank, (cluster + 3) & ~3, false};
+  Peers<T, WARPS> peers{maps + 2 * WARPS * 32, bars, cluster, rank, (cluster + 3) & ~3, a.status, false};
   const int64_t tiles = (a.L + TILE - 1) / TILE, turns = (tiles + cluster - 1) / cluster, ahead = -(int64_t)cluster * TILE;
   int64_t t0 = ((turns - 1) * cluster + rank) * TILE + warp * STEPS;
   In in(a, smem, b, c0, t0);
@@ -619,7 +632,7 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) backward_kernel
     }
     Map* const own = maps + (stage * WARPS) * 32 + lane;
     V* const own_end = ends + (stage * WARPS) * 32 + lane;
-    const V P = PACKED && starts ? all<V>(RESTART) : each(sum, [](float t) { return ex2(t); });
+    const V P = PACKED && starts ? all<V>(RESTART) : each(sum, [](float t) { return exp2_near(t); });
     own[warp * 32] = Lane<T>::map(P, R);
     own_end[warp * 32] = H;
     __syncthreads();
@@ -735,7 +748,8 @@ struct StepArgs {
   const void* in[3];
   int64_t stride[3];               // between rows
   const float* decay;
-  float* state;
+  const float* state;
+  float* new_state;                // may be state itself
   void* y;
   int64_t batch, D;
   float scale;
@@ -770,7 +784,7 @@ __global__ void __launch_bounds__(256) step_kernel(const StepArgs a) {
       h.v[i] = fmaf(A, h.v[i], root(b2) * (sigmoid(ld(&pg.v[i])) * ld(&px.v[i])));
       st(&y.v[i], h.v[i]);
     }
-    *reinterpret_cast<State*>(a.state + row * a.D + c) = h;
+    *reinterpret_cast<State*>(a.new_state + row * a.D + c) = h;
     *reinterpret_cast<Pack*>(static_cast<T*>(a.y) + row * a.D + c) = y;
   }
 }
@@ -937,6 +951,7 @@ Args args_of(const ssd_gated_recurrence_params_t* p) {
   a.points = cdiv(p->seqlen, POINT);
   a.groups = cdiv(p->dim, 128 / value_bytes(p->dtype));
   a.scale = p->scale;
+  a.status = p->status;
   return a;
 }
 
@@ -1021,12 +1036,14 @@ cudaError_t launch_gated_recurrence_update(const ssd_gated_recurrence_update_par
   a.stride[0] = p->x_stride_row; a.stride[1] = p->decay_gate_stride_row; a.stride[2] = p->input_gate_stride_row;
   a.decay = p->decay;
   a.state = p->state;
+  a.new_state = p->new_state;
   a.y = p->y;
   a.batch = p->batch;
   a.D = p->dim;
   a.scale = p->scale;
   const int es = value_bytes(p->dtype);
-  bool wide = p->dim % 4 == 0 && reinterpret_cast<uintptr_t>(p->state) % 16 == 0 && reinterpret_cast<uintptr_t>(p->y) % (4 * es) == 0;
+  bool wide = p->dim % 4 == 0 && (reinterpret_cast<uintptr_t>(p->state) | reinterpret_cast<uintptr_t>(p->new_state)) % 16 == 0 &&
+              reinterpret_cast<uintptr_t>(p->y) % (4 * es) == 0;
   for (int i = 0; i < 3; ++i)
     wide = wide && reinterpret_cast<uintptr_t>(a.in[i]) % (4 * es) == 0 && (p->batch == 1 || a.stride[i] % 4 == 0);
   // rows of a thread: as many threads as the GPU holds, where the batch has them

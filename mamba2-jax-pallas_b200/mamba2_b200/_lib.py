@@ -136,7 +136,7 @@ class GatedRecurrenceParams(ctypes.Structure):
                 ("decay_gate_stride_b", _i64), ("decay_gate_stride_t", _i64), ("input_gate_stride_b", _i64),
                 ("input_gate_stride_t", _i64), ("dtype", _i32), ("scale", _f32),
                 ("x", _vp), ("decay_gate", _vp), ("input_gate", _vp), ("decay", _vp), ("initial_state", _vp),
-                ("seq_idx", _vp), ("y", _vp), ("final_state", _vp), ("checkpoints", _vp)]
+                ("seq_idx", _vp), ("y", _vp), ("final_state", _vp), ("checkpoints", _vp), ("status", _vp)]
 
 
 class GatedRecurrenceGrads(ctypes.Structure):
@@ -148,7 +148,8 @@ class GatedRecurrenceGrads(ctypes.Structure):
 class GatedRecurrenceUpdateParams(ctypes.Structure):
     _fields_ = [("batch", _i64), ("dim", _i64), ("x_stride_row", _i64), ("decay_gate_stride_row", _i64),
                 ("input_gate_stride_row", _i64), ("dtype", _i32), ("scale", _f32),
-                ("x", _vp), ("decay_gate", _vp), ("input_gate", _vp), ("decay", _vp), ("state", _vp), ("y", _vp)]
+                ("x", _vp), ("decay_gate", _vp), ("input_gate", _vp), ("decay", _vp), ("state", _vp), ("new_state", _vp),
+                ("y", _vp)]
 
 
 class GatedFfParams(ctypes.Structure):

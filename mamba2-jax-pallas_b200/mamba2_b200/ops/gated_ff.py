@@ -12,26 +12,28 @@ def _prepare(x, w_gate, w_up, w_down, activation):
             raise TypeError(f"{name} must be a torch.Tensor")
         if not t.is_cuda:
             raise ValueError(f"{name} must be a CUDA tensor (no CPU path)")
-        if t.device != x.device:
-            raise ValueError(f"{name} must be on x's device")
         if t.dtype != x.dtype:
             raise TypeError(f"{name} ({t.dtype}) and x ({x.dtype}) must have the same dtype")
-    if activation not in _lib.ACTIVATIONS:
+    if not w_gate.device == w_up.device == w_down.device == x.device:
+        raise ValueError("the weights must be on x's device")
+    act = _lib.ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"activation must be one of {', '.join(_lib.ACTIVATIONS)}")
     if w_gate.dim() != 2 or w_up.shape != w_gate.shape:
         raise ValueError("w_gate and w_up must be (hidden, dim)")
     hidden, dim = w_gate.shape
     if w_down.dim() != 2 or w_down.shape[1] != hidden:
         raise ValueError(f"w_down must be (dim_out, {hidden})")
-    if hidden == 0 or dim == 0 or w_down.shape[0] == 0:
+    out = w_down.shape[0]
+    if hidden == 0 or dim == 0 or out == 0:
         raise ValueError("the weights must not be empty")
     if x.dim() < 1 or x.shape[-1] != dim:
         raise ValueError(f"x {tuple(x.shape)} must end in the weights' {dim} columns")
-    code = _lib.dtype_code(x)
-    rows = [_lib.rows2d(x, dim), _lib.rows2d(w_gate, dim), _lib.rows2d(w_up, dim), _lib.rows2d(w_down, hidden)]
-    p = _lib.GatedFfParams(rows[0].shape[0], dim, hidden, w_down.shape[0], *(_lib.row_stride(t) for t in rows), code,
-                           _lib.ACTIVATIONS[activation], *(t.data_ptr() for t in rows), None)
-    return p, rows
+    xr, g, u, d = _lib.rows2d(x, dim), _lib.rows2d(w_gate, dim), _lib.rows2d(w_up, dim), _lib.rows2d(w_down, hidden)
+    stride = _lib.row_stride
+    p = _lib.GatedFfParams(xr.shape[0], dim, hidden, out, stride(xr), stride(g), stride(u), stride(d), _lib.dtype_code(x), act,
+                           xr.data_ptr(), g.data_ptr(), u.data_ptr(), d.data_ptr(), None)
+    return p, (xr, g, u, d)   # (copies have to live until the call)
 
 
 def gated_feed_forward(x, w_gate, w_up, w_down, *, activation: str = "silu", check_status: bool = False):
@@ -45,13 +47,13 @@ def gated_feed_forward(x, w_gate, w_up, w_down, *, activation: str = "silu", che
     ``gated_feed_forward_grad`` gives the gradients.
     """
     p, rows = _prepare(x, w_gate, w_up, w_down, activation)
-    y = torch.empty((*x.shape[:-1], w_down.shape[0]), dtype=x.dtype, device=x.device)
-    if y.numel() == 0:
+    y = rows[0].new_empty((*x.shape[:-1], p.dim_out))
+    if p.tokens == 0:
         return y
     p.y = y.data_ptr()
     lib = _lib.load()
     with _lib.on_device(x.device):
-        ws = torch.empty(lib.ssd_gated_ff_workspace_bytes(p), dtype=torch.uint8, device=x.device)
+        ws = y.new_empty(lib.ssd_gated_ff_workspace_bytes(p), dtype=torch.uint8)
         _lib.check(lib.ssd_gated_ff(p, ws.data_ptr(), ws.numel(), _lib.stream_of(y)))
         if check_status:
             _lib.check_device_status(ws)

@@ -7,35 +7,36 @@ import torch
 from .. import _lib
 
 _TILE = 32   # SSD_GATED_RECURRENCE_CHECKPOINT
+_F32 = torch.float32
 
 
 def _channels_last(t):
     """A view whose channels are contiguous, else a copy."""
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
 def _inputs(x, decay_gate, input_gate, decay, scale, dims):
-    shape = "(batch, seqlen, dim)" if dims == 3 else "(batch, dim)"
     for t, name in ((x, "x"), (decay_gate, "decay_gate"), (input_gate, "input_gate"), (decay, "decay")):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch.Tensor")
         if not t.is_cuda:
             raise ValueError(f"{name} must be a CUDA tensor (no CPU path)")
-        if t.device != x.device:
-            raise ValueError(f"{name} must be on x's device")
-    if x.dim() != dims or x.shape[-1] == 0:
-        raise ValueError(f"x must be {shape}, with channels")
+    shape, dtype, dev = x.shape, x.dtype, x.device
+    if len(shape) != dims or shape[-1] == 0:
+        raise ValueError(f"x must be {'(batch, seqlen, dim)' if dims == 3 else '(batch, dim)'}, with channels")
     for t, name in ((decay_gate, "decay_gate"), (input_gate, "input_gate")):
-        if t.shape != x.shape:
-            raise ValueError(f"{name} {tuple(t.shape)} must have x's shape {tuple(x.shape)}")
-        if t.dtype != x.dtype:
-            raise TypeError(f"{name} ({t.dtype}) and x ({x.dtype}) must have the same dtype")
-    if tuple(decay.shape) != (x.shape[-1],):
+        if t.shape != shape:
+            raise ValueError(f"{name} {tuple(t.shape)} must have x's shape {tuple(shape)}")
+        if t.dtype != dtype:
+            raise TypeError(f"{name} ({t.dtype}) and x ({dtype}) must have the same dtype")
+    if decay.dim() != 1 or decay.shape[0] != shape[-1]:
         raise ValueError("decay must be (dim,)")
+    if not decay_gate.device == input_gate.device == decay.device == dev:
+        raise ValueError("decay_gate, input_gate and decay must be on x's device")
     if not 0 <= scale <= 3.4e38:
         raise ValueError("scale must be finite and not negative")
     return (_lib.dtype_code(x), _channels_last(x), _channels_last(decay_gate), _channels_last(input_gate),
-            _lib.dev(decay.detach(), "decay", torch.float32))
+            _lib.dev(decay, "decay", _F32))
 
 
 def _state(t, name, x):
@@ -43,14 +44,14 @@ def _state(t, name, x):
         return None
     if not isinstance(t, torch.Tensor) or t.device != x.device or tuple(t.shape) != (x.shape[0], x.shape[-1]):
         raise ValueError(f"{name} must be a (batch, dim) tensor on x's device")
-    return _lib.dev(t.detach(), name, torch.float32)
+    return _lib.dev(t, name, _F32)
 
 
 def _ids(seq_idx, x):
     if seq_idx is None:
         return None
     ids = _lib.index_list(seq_idx, "seq_idx")
-    if tuple(ids.shape) != tuple(x.shape[:2]) or ids.device != x.device:
+    if ids.shape != x.shape[:2] or ids.device != x.device:
         raise ValueError("seq_idx must be (batch, seqlen) on x's device")
     return ids.to(torch.int32)
 
@@ -59,16 +60,16 @@ def _checkpoint_shape(x):
     return (x.shape[0], -(-x.shape[1] // _TILE), x.shape[2])
 
 
-def _params(code, x, decay_gate, input_gate, decay, scale, initial, ids):
+def _params(code, x, decay_gate, input_gate, decay, scale, initial, ids, y, final, points, status):
     b, L, d = x.shape
     return _lib.GatedRecurrenceParams(b, L, d, x.stride(0), x.stride(1), decay_gate.stride(0), decay_gate.stride(1),
                                       input_gate.stride(0), input_gate.stride(1), code, scale, x.data_ptr(),
                                       decay_gate.data_ptr(), input_gate.data_ptr(), decay.data_ptr(), _lib.ptr(initial),
-                                      _lib.ptr(ids), None, None, None)
+                                      _lib.ptr(ids), _lib.ptr(y), _lib.ptr(final), _lib.ptr(points), _lib.ptr(status))
 
 
 def gated_recurrence(x, decay_gate, input_gate, decay, *, scale: float = 8.0, initial_state=None, seq_idx=None,
-                     return_final_state: bool = False, return_checkpoints: bool = False):
+                     return_final_state: bool = False, return_checkpoints: bool = False, check_status: bool = False):
     """``h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(input_gate_t) x_t`` along the sequence, per channel, with
     ``a_t = exp(-scale softplus(decay) sigmoid(decay_gate_t))``.
 
@@ -80,19 +81,23 @@ def gated_recurrence(x, decay_gate, input_gate, decay, *, scale: float = 8.0, in
     ``return_final_state`` also the float32 state after the last token (batch, dim); with
     ``return_checkpoints`` also the float32 states that ``gated_recurrence_grad`` starts from,
     (batch, ceil(seqlen / 32), dim), which saves it a pass over the inputs.  A value that is
-    not finite makes its channel so up to the next sequence.  The results carry no autograd history.
+    not finite makes its channel so up to the next sequence.  ``check_status`` waits for the call and raises
+    ``SsdError`` if a bounded wait inside a kernel gave up (unchecked, the channels concerned are NaN).  The
+    results carry no autograd history.
     """
     code, xs, r, i, lam = _inputs(x, decay_gate, input_gate, decay, scale, 3)
     h0, ids = _state(initial_state, "initial_state", x), _ids(seq_idx, x)
     b, L, d = x.shape
-    y = torch.empty((b, L, d), dtype=x.dtype, device=x.device)
-    final = torch.empty((b, d), dtype=torch.float32, device=x.device) if return_final_state else None
-    points = torch.empty(_checkpoint_shape(x), dtype=torch.float32, device=x.device) if return_checkpoints else None
-    if y.numel():
-        p = _params(code, xs, r, i, lam, scale, h0, ids)
-        p.y, p.final_state, p.checkpoints = y.data_ptr(), _lib.ptr(final), _lib.ptr(points)
+    y = xs.new_empty((b, L, d))
+    final = xs.new_empty((b, d), dtype=_F32) if return_final_state else None
+    points = xs.new_empty(_checkpoint_shape(x), dtype=_F32) if return_checkpoints else None
+    if b and L:
+        status = xs.new_zeros(64, dtype=torch.int32) if check_status else None
+        p = _params(code, xs, r, i, lam, scale, h0, ids, y, final, points, status)
         with _lib.on_device(x.device):
             _lib.check(_lib.load().ssd_gated_recurrence(p, _lib.stream_of(y)))
+            if check_status:
+                _lib.check_device_status(status)
     elif final is not None:
         final.zero_() if h0 is None else final.copy_(h0)
     if not (return_final_state or return_checkpoints):
@@ -101,7 +106,7 @@ def gated_recurrence(x, decay_gate, input_gate, decay, *, scale: float = 8.0, in
 
 
 def gated_recurrence_grad(x, decay_gate, input_gate, decay, grad_out, *, scale: float = 8.0, initial_state=None,
-                          seq_idx=None, grad_final_state=None, checkpoints=None):
+                          seq_idx=None, grad_final_state=None, checkpoints=None, check_status: bool = False):
     """Gradients of ``gated_recurrence``: ``(grad_x, grad_decay_gate, grad_input_gate, grad_decay,
     grad_initial_state)``.
 
@@ -119,28 +124,30 @@ def gated_recurrence_grad(x, decay_gate, input_gate, decay, grad_out, *, scale: 
         raise ValueError(f"grad_out must be a {tuple(x.shape)} tensor on x's device")
     if grad_out.dtype != x.dtype:
         raise TypeError(f"grad_out ({grad_out.dtype}) and x ({x.dtype}) must have the same dtype")
-    if checkpoints is not None and (not isinstance(checkpoints, torch.Tensor) or checkpoints.dtype != torch.float32 or
+    if checkpoints is not None and (not isinstance(checkpoints, torch.Tensor) or checkpoints.dtype != _F32 or
                                     tuple(checkpoints.shape) != _checkpoint_shape(x) or checkpoints.device != x.device):
         raise ValueError(f"checkpoints must be the float32 {_checkpoint_shape(x)} tensor that gated_recurrence returned")
     g = _channels_last(grad_out)
     b, L, d = x.shape
-    gx, gr, gi = (torch.empty((b, L, d), dtype=x.dtype, device=x.device) for _ in range(3))
-    gd = torch.empty(d, dtype=torch.float32, device=x.device)
-    gh = torch.empty((b, d), dtype=torch.float32, device=x.device) if h0 is not None else None
-    if gx.numel() == 0:
+    gx, gr, gi = xs.new_empty((b, L, d)), xs.new_empty((b, L, d)), xs.new_empty((b, L, d))
+    gd = xs.new_empty(d, dtype=_F32)
+    gh = xs.new_empty((b, d), dtype=_F32) if h0 is not None else None
+    if not (b and L):
         gd.zero_()
         if gh is not None:
             gh.zero_() if gf is None else gh.copy_(gf)
         return gx, gr, gi, gd, gh
-    p = _params(code, xs, r, i, lam, scale, h0, ids)
     points = None if checkpoints is None else checkpoints.contiguous()
-    p.checkpoints = _lib.ptr(points)
+    status = xs.new_zeros(64, dtype=torch.int32) if check_status else None
+    p = _params(code, xs, r, i, lam, scale, h0, ids, None, None, points, status)
     q = _lib.GatedRecurrenceGrads(g.stride(0), g.stride(1), g.data_ptr(), _lib.ptr(gf), gx.data_ptr(), gr.data_ptr(),
                                   gi.data_ptr(), gd.data_ptr(), _lib.ptr(gh))
     lib = _lib.load()
     with _lib.on_device(x.device):
-        ws = torch.empty(lib.ssd_gated_recurrence_grad_workspace_bytes(p), dtype=torch.uint8, device=x.device)
+        ws = xs.new_empty(lib.ssd_gated_recurrence_grad_workspace_bytes(p), dtype=torch.uint8)
         _lib.check(lib.ssd_gated_recurrence_grad(p, q, ws.data_ptr(), ws.numel(), _lib.stream_of(gx)))
+        if check_status:
+            _lib.check_device_status(status)
     return gx, gr, gi, gd, gh
 
 
@@ -148,21 +155,23 @@ def gated_recurrence_update(state, x, decay_gate, input_gate, decay, *, scale: f
     """One token of ``gated_recurrence``.  Returns ``(new_state, h)``.
 
     state (batch, dim) float32; x, decay_gate and input_gate (batch, dim); h has x's dtype.  The given state
-    is copied first; with ``inplace=True`` it is updated itself (it must be contiguous) and returned.
+    stays as it is; with ``inplace=True`` it is updated itself (it must be contiguous) and returned.
     """
-    if not isinstance(state, torch.Tensor) or state.dtype != torch.float32:
+    if not isinstance(state, torch.Tensor) or state.dtype != _F32:
         raise TypeError("state must be a float32 tensor")
     code, xs, r, i, lam = _inputs(x, decay_gate, input_gate, decay, scale, 2)
     if state.shape != x.shape or state.device != x.device:
         raise ValueError("state must be (batch, dim) on x's device")
     if inplace and not state.is_contiguous():
         raise ValueError("inplace=True needs a contiguous state")
-    st = state if inplace else state.detach().clone(memory_format=torch.contiguous_format)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if y.numel():
-        p = _lib.GatedRecurrenceUpdateParams(x.shape[0], x.shape[1], xs.stride(0), r.stride(0), i.stride(0), code, scale,
-                                             xs.data_ptr(), r.data_ptr(), i.data_ptr(), lam.data_ptr(), st.data_ptr(),
+    b, d = x.shape
+    old = state.contiguous()
+    new = state if inplace else xs.new_empty((b, d), dtype=_F32)
+    y = xs.new_empty((b, d))
+    if b:
+        p = _lib.GatedRecurrenceUpdateParams(b, d, xs.stride(0), r.stride(0), i.stride(0), code, scale, xs.data_ptr(),
+                                             r.data_ptr(), i.data_ptr(), lam.data_ptr(), old.data_ptr(), new.data_ptr(),
                                              y.data_ptr())
         with _lib.on_device(x.device):
             _lib.check(_lib.load().ssd_gated_recurrence_update(p, _lib.stream_of(y)))
-    return st, y
+    return new, y
