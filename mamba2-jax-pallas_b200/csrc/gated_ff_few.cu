@@ -2,8 +2,10 @@
 // where the weights are read for so few rows that nothing but their bytes counts.
 //
 // The products run in f32 on the CUDA cores, straight from the weights as they lie in memory.  A warp takes
-// some rows of a weight (for g and u the same row of both), or a part of their columns where a weight has few rows, against all tokens' values,
-// which stay in L1.  Two launches, the second set up while the first runs; bound by HBM.
+// some rows of a weight (for g and u the same row of both), or a part of their columns, against all tokens' values, which stay in
+// L1.  One or two CTAs per SM walk over the rows; every lane copies its own 16 bytes of the weights some steps ahead, across the
+// ends of the rows, into slots of shared memory that no other lane reads: 96 KB in flight per SM.  Bound by HBM and the two
+// launches' ends: 1 token of 4096 x 12288 bf16 56.5 us (5.3 TB/s), of 2560 x 7680 f32 41 us (5.8 TB/s), of 768 x 2048 6 us.
 #include <algorithm>
 
 #include "common.cuh"
@@ -15,11 +17,17 @@
 namespace ssd {
 namespace {
 
-constexpr int WARPS = 8;
+constexpr int WARPS = 16;          // of a CTA
+// CTAs of an SM (two where the sums leave room: 1 token of 4096 x 12288 in 56.5 us, with one CTA 60.1), and the ring's places for 16
+// bytes of every lane of a warp (twice as many gained nothing)
+template <int N>
+struct Shape {
+  static constexpr int CTAS = N <= 4 ? 2 : 1, SLOTS = 12 / CTAS;
+};
 constexpr int SMS = 148;   // of a B200
 
 struct FewArgs {
-  const void* x;                   // (tokens, K) values of T
+  const void* x;                   // (tokens, K) values of T; blockIdx.y takes R of the tokens
   const void* w[2];                // rows of the weight, and of the other one
   void* out;                       // (tokens, rows)
   int64_t xs, ws[2], os;           // values between rows
@@ -47,22 +55,6 @@ struct Piece<bf16> {
   }
 };
 
-// The piece from column c of a row of K values; zeros past the end.
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ Piece<T> load(const T* row, int c, int K) {
-  Piece<T> p;
-  p.q = make_uint4(0, 0, 0, 0);
-  if constexpr (ALIGNED) {
-    if (c < K) p.q = __ldg(reinterpret_cast<const uint4*>(row + c));
-  } else {
-    T* v = reinterpret_cast<T*>(&p.q);
-#pragma unroll
-    for (int i = 0; i < Piece<T>::N; ++i)
-      if (c + i < K) v[i] = row[c + i];
-  }
-  return p;
-}
-
 // Values v[0..N) summed over the warp; lane l ends with the sum of value l % N.
 template <int N>
 __device__ __forceinline__ float warp_sums(float (&v)[N]) {
@@ -82,98 +74,206 @@ __device__ __forceinline__ float warp_sums(float (&v)[N]) {
   return s;
 }
 
-// R tokens; a warp's rows: ROWS of each of W weights.  W = 2: out = act(g) u, else the product itself.
-template <typename T, int R, int ROWS, int W, bool ALIGNED>
-__global__ void __launch_bounds__(32 * WARPS) few_kernel(const __grid_constant__ FewArgs a) {
-  constexpr int N = R * ROWS * W;   // sums of a warp, at most 32
-  __shared__ float sh[WARPS][N];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int part = warp % a.parts, units = WARPS / a.parts;   // groups of rows of the CTA
-  const int64_t r0 = ((int64_t)blockIdx.x * units + warp / a.parts) * ROWS;
-  constexpr int STEP = 32 * Piece<T>::N;
-  const int steps = (a.K + STEP - 1) / STEP, s0 = (int)((int64_t)steps * part / a.parts), s1 = (int)((int64_t)steps * (part + 1) / a.parts);
-  const T* row[W * ROWS];
-#pragma unroll
-  for (int i = 0; i < W * ROWS; ++i)   // rows past the end are read as the last one
-    row[i] = static_cast<const T*>(a.w[i % W]) + min(r0 + i / W, a.rows - 1) * a.ws[i % W];
-  const T* x = static_cast<const T*>(a.x);
-  float sum[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) sum[i] = 0.f;
-  // pieces of the weights on their way, always this many steps ahead
-  constexpr int AHEAD = W * ROWS == 1 ? 8 : W * ROWS == 2 ? 6 : 3;
-  Piece<T> w[AHEAD][W * ROWS];
-  auto fetch = [&](int k, int s) {
-#pragma unroll
-    for (int i = 0; i < W * ROWS; ++i) w[k][i] = load<T, ALIGNED>(row[i], s < s1 ? (s * 32 + lane) * Piece<T>::N : a.K, a.K);
-  };
-  auto start = [&]() {
-#pragma unroll
-    for (int k = 0; k < AHEAD; ++k) fetch(k, s0 + k);
-  };
-  // The first launch waits for whatever ran before it (an optimizer may have written the weights) and lets the second
-  // one be set up, which may read its weight at once: the first has waited for that.
-  if constexpr (W == 2) {
-    ptx::griddep_wait();
-    ptx::griddep_launch_dependents();
-    if (blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
-    start();
-  } else {
-    start();
-    ptx::griddep_wait();
-  }
-  for (int s = s0; s < s1; s += AHEAD) {
-#pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      const int c = s + k < s1 ? ((s + k) * 32 + lane) * Piece<T>::N : a.K;
-#pragma unroll
-      for (int t = 0; t < R; ++t) {
-        const Piece<T> v = load<T, ALIGNED>(x + min(t, a.tokens - 1) * a.xs, c, a.K);
-#pragma unroll
-        for (int j = 0; j < Piece<T>::N; ++j)
-#pragma unroll
-          for (int i = 0; i < W * ROWS; ++i) sum[t * W * ROWS + i] = fmaf(v.at(j), w[k][i].at(j), sum[t * W * ROWS + i]);
-      }
-      fetch(k, s + k + AHEAD);
-    }
-  }
-  const float total = warp_sums<N>(sum);
-  if (lane < N) sh[warp][lane] = total;
-  __syncthreads();
-  // a thread per token and row: the parts in order
+// The sums of a CTA's warps, `parts` of them to a group of rows, to the output: a thread per token and row.
+template <typename T, int R, int ROWS, int W>
+__device__ __forceinline__ void finish(const FewArgs& a, const float (*sh)[R * ROWS * W], int groups, int64_t first) {
   constexpr int OUT = R * ROWS;
-  for (int i = threadIdx.x; i < units * OUT; i += 32 * WARPS) {
+  const int t0 = blockIdx.y * R;
+  for (int i = threadIdx.x; i < groups * OUT; i += blockDim.x) {
     const int unit = i / OUT, t = i % OUT / ROWS, r = i % ROWS;
-    const int64_t at = ((int64_t)blockIdx.x * units + unit) * ROWS + r;
-    if (t >= a.tokens || at >= a.rows) continue;
+    const int64_t at = (first + unit) * ROWS + r;
+    if (t0 + t >= a.tokens || at >= a.rows) continue;
     float v[W];
 #pragma unroll
     for (int k = 0; k < W; ++k) {
       v[k] = 0.f;
-      for (int j = 0; j < a.parts; ++j) v[k] += sh[unit * a.parts + j][t * W * ROWS + r * W + k];
+      for (int j = 0; j < a.parts; ++j) v[k] += sh[unit * a.parts + j][t * W * ROWS + r * W + k];   // in order
     }
-    T* o = static_cast<T*>(a.out) + t * a.os + at;
+    T* o = static_cast<T*>(a.out) + (t0 + t) * a.os + at;
     if constexpr (W == 2) st(o, ff::activate(a.act, v[0], nullptr) * v[1]);
     else st(o, v[0]);
   }
 }
 
+template <typename T, int R, int NR>
+__device__ __forceinline__ void accumulate(float (&sum)[R * NR], const Piece<T> (&x)[R], const Piece<T> (&w)[NR]) {
+#pragma unroll
+  for (int j = 0; j < Piece<T>::N; ++j)
+#pragma unroll
+    for (int t = 0; t < R; ++t)
+#pragma unroll
+      for (int i = 0; i < NR; ++i) sum[t * NR + i] = fmaf(x[t].at(j), w[i].at(j), sum[t * NR + i]);
+}
+
+// The first launch (W = 2: out = act(g) u) waits for whatever ran before it (an optimizer may have written the weights) and
+// lets the second one (W = 1: the product itself) be set up, which may read its weight at once: the first has waited for that.
+template <int W>
+__device__ __forceinline__ void before_weights(const FewArgs& a) {
+  if constexpr (W == 2) {
+    ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.status = 0;
+  }
+}
+
+// R tokens; a warp's rows: ROWS of each of W weights.
+template <typename T, int R, int ROWS, int W>
+__global__ void __launch_bounds__(32 * WARPS, Shape<R * ROWS * W>::CTAS) few_kernel(const __grid_constant__ FewArgs a) {
+  constexpr int N = R * ROWS * W, NR = W * ROWS, SLOTS = Shape<N>::SLOTS, STAGES = SLOTS / NR, STEP = 32 * Piece<T>::N;
+  extern __shared__ __align__(16) uint4 ring[];          // [WARPS][SLOTS][32]
+  __shared__ float sh[2][WARPS][N];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = warp % a.parts, groups = WARPS / a.parts;
+  const int steps = (a.K + STEP - 1) / STEP, s0 = steps * part / a.parts, s1 = steps * (part + 1) / a.parts;
+  const int64_t all = (a.rows + ROWS - 1) / ROWS, stride = (int64_t)gridDim.x * groups;
+  uint4* const mine = ring + warp * SLOTS * 32 + lane;
+  before_weights<W>(a);
+  // the next step to copy: of group `next`, step `at`, into slot `to`
+  int64_t next = (int64_t)blockIdx.x * groups + warp / a.parts;
+  int at = s0, to = 0;
+  const T* row[NR];
+  auto rows_of = [&]() {
+#pragma unroll
+    for (int i = 0; i < NR; ++i)   // rows past the end are read as the last one
+      row[i] = static_cast<const T*>(a.w[i % W]) + min(next * ROWS + i / W, a.rows - 1) * a.ws[i % W];
+  };
+  rows_of();
+  auto copy = [&]() {
+    if (next < all) {
+      const int c = (at * 32 + lane) * Piece<T>::N;
+#pragma unroll
+      for (int i = 0; i < NR; ++i)   // columns past the end are zeros
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(mine + (to * NR + i) * 32)), "l"(c < a.K ? row[i] + c : row[i]),
+                     "r"(c < a.K ? 16 : 0) : "memory");
+      if (++at == s1) {
+        at = s0;
+        next += stride;
+        rows_of();
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (++to == STAGES) to = 0;
+  };
+#pragma unroll
+  for (int k = 0; k < STAGES - 1; ++k) copy();
+  if constexpr (W == 1) ptx::griddep_wait();
+  const int tokens = min(R, a.tokens - (int)blockIdx.y * R);
+  const T* x = static_cast<const T*>(a.x) + (int64_t)blockIdx.y * R * a.xs;
+  // one load of each 128 bytes of x, all at once: found missing step by step, they would cost the first rows a trip to L2 each
+  for (int t = 0; t < tokens; ++t)
+    for (int c = threadIdx.x * (128 / (int)sizeof(T)); c < a.K; c += 32 * WARPS * (128 / (int)sizeof(T))) {
+      uint32_t unused;
+      asm volatile("ld.global.ca.b32 %0, [%1];" : "=r"(unused) : "l"(x + t * a.xs + c));
+    }
+  int from = 0, turn = 0;
+  for (int64_t first = (int64_t)blockIdx.x * groups; first < all; first += stride, turn ^= 1) {
+    float sum[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum[i] = 0.f;
+    for (int s = s0; s < s1; ++s) {
+      const int c = (s * 32 + lane) * Piece<T>::N;
+      Piece<T> v[R], w[NR];
+#pragma unroll
+      for (int t = 0; t < R; ++t) {
+        v[t].q = make_uint4(0, 0, 0, 0);
+        if (c < a.K) v[t].q = *reinterpret_cast<const uint4*>(x + min(t, tokens - 1) * a.xs + c);
+      }
+      copy();
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+#pragma unroll
+      for (int i = 0; i < NR; ++i) w[i].q = mine[(from * NR + i) * 32];
+      if (++from == STAGES) from = 0;
+      accumulate<T, R, NR>(sum, v, w);
+    }
+    const float total = warp_sums<N>(sum);
+    if (lane < N) sh[turn][warp][lane] = total;
+    __syncthreads();       // (the buffer of the turn before is read by now only)
+    finish<T, R, ROWS, W>(a, sh[turn], groups, first);
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// The same where rows do not start at 16 bytes: value by value.
+template <typename T, int R, int ROWS, int W>
+__global__ void __launch_bounds__(256) few_odd_kernel(const __grid_constant__ FewArgs a) {
+  constexpr int N = R * ROWS * W, NR = W * ROWS, STEP = 32 * Piece<T>::N;
+  __shared__ float sh[8][N];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = warp % a.parts, groups = 8 / a.parts;
+  const int64_t first = (int64_t)blockIdx.x * groups, r0 = (first + warp / a.parts) * ROWS;
+  const int steps = (a.K + STEP - 1) / STEP, s0 = steps * part / a.parts, s1 = steps * (part + 1) / a.parts;
+  before_weights<W>(a);
+  if constexpr (W == 1) ptx::griddep_wait();
+  const T* row[NR];
+#pragma unroll
+  for (int i = 0; i < NR; ++i) row[i] = static_cast<const T*>(a.w[i % W]) + min(r0 + i / W, a.rows - 1) * a.ws[i % W];
+  const int tokens = min(R, a.tokens - (int)blockIdx.y * R);
+  const T* x = static_cast<const T*>(a.x) + (int64_t)blockIdx.y * R * a.xs;
+  float sum[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) sum[i] = 0.f;
+  for (int s = s0; s < s1; ++s) {   // a lane's values are 32 columns apart
+    float w[Piece<T>::N][NR];
+#pragma unroll
+    for (int j = 0; j < Piece<T>::N; ++j) {
+      const int c = s * STEP + j * 32 + lane;
+#pragma unroll
+      for (int i = 0; i < NR; ++i) w[j][i] = c < a.K ? ld(row[i] + c) : 0.f;
+    }
+#pragma unroll
+    for (int t = 0; t < R; ++t)
+#pragma unroll
+      for (int j = 0; j < Piece<T>::N; ++j) {
+        const int c = s * STEP + j * 32 + lane;
+        const float v = c < a.K ? ld(x + min(t, tokens - 1) * a.xs + c) : 0.f;
+#pragma unroll
+        for (int i = 0; i < NR; ++i) sum[t * NR + i] = fmaf(v, w[j][i], sum[t * NR + i]);
+      }
+  }
+  const float total = warp_sums<N>(sum);
+  if (lane < N) sh[warp][lane] = total;
+  __syncthreads();
+  finish<T, R, ROWS, W>(a, sh, groups, first);
+}
+
 template <typename T, int R, int ROWS, int W>
 cudaError_t launch_rows(FewArgs a, bool aligned, cudaStream_t st) {
-  // warps of a row: as many as fill the GPU
-  a.parts = 1;
-  while (a.parts < WARPS && (a.rows + ROWS - 1) / ROWS * a.parts < SMS * 24 && a.K / (a.parts * 2) >= 32 * Piece<T>::N) a.parts *= 2;
-  const int64_t per = WARPS / a.parts * ROWS, ctas = (a.rows + per - 1) / per;
-  return aligned ? launch_dependent(few_kernel<T, R, ROWS, W, true>, dim3((unsigned)ctas), 32 * WARPS, 0, 1, st, a)
-                 : launch_dependent(few_kernel<T, R, ROWS, W, false>, dim3((unsigned)ctas), 32 * WARPS, 0, 1, st, a);
+  const int64_t groups = (a.rows + ROWS - 1) / ROWS;
+  const unsigned passes = (unsigned)((a.tokens + R - 1) / R);
+  const int steps = (a.K + 32 * Piece<T>::N - 1) / (32 * Piece<T>::N);
+  if (!aligned) {          // parts of a row: as many as fill the GPU
+    a.parts = 1;
+    while (a.parts < 8 && groups * a.parts < SMS * 24 && steps >= a.parts * 2) a.parts *= 2;
+    return launch_dependent(few_odd_kernel<T, R, ROWS, W>, dim3((unsigned)((groups * a.parts + 7) / 8), passes), 256, 0, 1, st, a);
+  }
+  // parts of a row: the fewest steps of a warp; a turn's sums and meeting count as half a step
+  using S = Shape<R * ROWS * W>;
+  const int64_t slots = (int64_t)SMS * S::CTAS * WARPS;
+  int best = 1;
+  double least = 1e300;
+  for (int parts = 1; parts <= WARPS && parts <= steps; parts *= 2) {
+    const int64_t turns = (groups * parts + slots - 1) / slots;
+    const double cost = (double)turns * ((double)((steps + parts - 1) / parts) + 0.5);
+    if (cost < least) {
+      least = cost;
+      best = parts;
+    }
+  }
+  a.parts = best;
+  static std::atomic<uint64_t> allowed{0};
+  constexpr int smem = WARPS * S::SLOTS * 512;
+  const cudaError_t e = allow_smem((const void*)few_kernel<T, R, ROWS, W>, smem, &allowed);
+  if (e != cudaSuccess) return e;
+  const int64_t ctas = std::min<int64_t>(SMS * S::CTAS, (groups * best + WARPS - 1) / WARPS);
+  return launch_dependent(few_kernel<T, R, ROWS, W>, dim3((unsigned)ctas, passes), 32 * WARPS, smem, 1, st, a);
 }
 
 template <typename T, int W>
 cudaError_t launch_tokens(const FewArgs& a, bool aligned, cudaStream_t st) {
   if (a.tokens == 1) return launch_rows<T, 1, 1, W>(a, aligned, st);
-  if (a.tokens == 2) return launch_rows<T, 2, 1, W>(a, aligned, st);
+  if (a.tokens == 2) return launch_rows<T, 2, 2, W>(a, aligned, st);
   if (a.tokens <= 4) return launch_rows<T, 4, 2, W>(a, aligned, st);
-  return launch_rows<T, 8, 2, W>(a, aligned, st);
+  return launch_rows<T, 8, 2, W>(a, aligned, st);   // 8 at a time
 }
 
 size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
@@ -214,7 +314,9 @@ cudaError_t launch_as(const ssd_gated_ff_params_t* p, uint8_t* ws, cudaStream_t 
 
 }  // namespace
 
-bool gated_ff_is_few(const ssd_gated_ff_params_t* p) { return p->tokens <= 8; }
+// bf16: up to 4 tokens (2560 x 7680: 4 tokens 37 us, by the products 42; 8 tokens 63 and 42).  f32: up to 24, 8 at a time (8 tokens 80
+// us, 16 160, by the products 252: their operands have to be split first).
+bool gated_ff_is_few(const ssd_gated_ff_params_t* p) { return p->tokens <= (p->dtype == SSD_DTYPE_BF16 ? 4 : 24); }
 
 size_t gated_ff_few_workspace(const ssd_gated_ff_params_t* p) { return 256 + up256((size_t)p->tokens * ((p->hidden + 7) / 8 * 8) * 4); }
 

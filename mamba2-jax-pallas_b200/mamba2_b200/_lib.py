@@ -349,11 +349,13 @@ def row_stride(t2: torch.Tensor) -> int:
 
 
 _HERE_ALREADY = contextlib.nullcontext()
+# without the public call's check that CUDA is initialised: it is asked only beside a CUDA tensor
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def on_device(dev: torch.device):
     """Context in which ``dev`` is the current device (launches go to the current one)."""
-    return _HERE_ALREADY if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return _HERE_ALREADY if _current_device() == dev.index else torch.cuda.device(dev)
 
 
 # the address of the current stream alone; the public call also builds a Stream object, which

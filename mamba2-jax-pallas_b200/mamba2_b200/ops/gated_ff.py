@@ -7,14 +7,16 @@ from .. import _lib
 
 
 def _prepare(x, w_gate, w_up, w_down, activation):
-    for t, name in ((x, "x"), (w_gate, "w_gate"), (w_up, "w_up"), (w_down, "w_down")):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor")
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor (no CPU path)")
-        if t.dtype != x.dtype:
-            raise TypeError(f"{name} ({t.dtype}) and x ({x.dtype}) must have the same dtype")
-    if not w_gate.device == w_up.device == w_down.device == x.device:
+    if not (isinstance(x, torch.Tensor) and isinstance(w_gate, torch.Tensor) and isinstance(w_up, torch.Tensor) and
+            isinstance(w_down, torch.Tensor)):
+        raise TypeError("x, w_gate, w_up and w_down must be torch.Tensors")
+    if not x.is_cuda:
+        raise ValueError("x must be a CUDA tensor (no CPU path)")
+    dtype, dev = x.dtype, x.device
+    if w_gate.dtype != dtype or w_up.dtype != dtype or w_down.dtype != dtype:
+        raise TypeError(f"w_gate ({w_gate.dtype}), w_up ({w_up.dtype}), w_down ({w_down.dtype}) and x ({dtype}) must have the "
+                        "same dtype")
+    if w_gate.device != dev or w_up.device != dev or w_down.device != dev:
         raise ValueError("the weights must be on x's device")
     act = _lib.ACTIVATIONS.get(activation)
     if act is None:

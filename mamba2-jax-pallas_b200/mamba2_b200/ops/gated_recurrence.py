@@ -16,27 +16,29 @@ def _channels_last(t):
 
 
 def _inputs(x, decay_gate, input_gate, decay, scale, dims):
-    for t, name in ((x, "x"), (decay_gate, "decay_gate"), (input_gate, "input_gate"), (decay, "decay")):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor")
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor (no CPU path)")
+    if not (isinstance(x, torch.Tensor) and isinstance(decay_gate, torch.Tensor) and
+            isinstance(input_gate, torch.Tensor) and isinstance(decay, torch.Tensor)):
+        raise TypeError("x, decay_gate, input_gate and decay must be torch.Tensors")
+    if not x.is_cuda:
+        raise ValueError("x must be a CUDA tensor (no CPU path)")
     shape, dtype, dev = x.shape, x.dtype, x.device
     if len(shape) != dims or shape[-1] == 0:
         raise ValueError(f"x must be {'(batch, seqlen, dim)' if dims == 3 else '(batch, dim)'}, with channels")
-    for t, name in ((decay_gate, "decay_gate"), (input_gate, "input_gate")):
-        if t.shape != shape:
-            raise ValueError(f"{name} {tuple(t.shape)} must have x's shape {tuple(shape)}")
-        if t.dtype != dtype:
-            raise TypeError(f"{name} ({t.dtype}) and x ({dtype}) must have the same dtype")
-    if decay.dim() != 1 or decay.shape[0] != shape[-1]:
+    if decay_gate.shape != shape or input_gate.shape != shape:
+        raise ValueError(f"decay_gate {tuple(decay_gate.shape)} and input_gate {tuple(input_gate.shape)} must have x's "
+                         f"shape {tuple(shape)}")
+    if decay_gate.dtype != dtype or input_gate.dtype != dtype:
+        raise TypeError(f"decay_gate ({decay_gate.dtype}), input_gate ({input_gate.dtype}) and x ({dtype}) must have the "
+                        "same dtype")
+    if decay.shape != shape[-1:]:
         raise ValueError("decay must be (dim,)")
-    if not decay_gate.device == input_gate.device == decay.device == dev:
+    if decay_gate.device != dev or input_gate.device != dev or decay.device != dev:
         raise ValueError("decay_gate, input_gate and decay must be on x's device")
     if not 0 <= scale <= 3.4e38:
         raise ValueError("scale must be finite and not negative")
-    return (_lib.dtype_code(x), _channels_last(x), _channels_last(decay_gate), _channels_last(input_gate),
-            _lib.dev(decay, "decay", _F32))
+    if decay.dtype is not _F32 or not decay.is_contiguous():
+        decay = decay.to(_F32).contiguous()
+    return _lib.dtype_code(x), _channels_last(x), _channels_last(decay_gate), _channels_last(input_gate), decay
 
 
 def _state(t, name, x):
