@@ -11,8 +11,10 @@
 //   dr = delta m (1 - sigmoid(r));  dx = delta b sigmoid(i);  di = delta b w (1 - sigmoid(i))
 //   d decay = sigmoid(decay) / softplus(decay) sum delta m;  dh_0 = c_0
 //
-// Both passes are bound by HBM (8 and 14 bytes per bf16 value), and close behind it by the issue
-// slots of the gates: an SM has to finish 2.9 forward values a cycle.
+// Both passes are bound by HBM (8 and 14 bytes per bf16 value), and close behind it by the issue slots and the special-function
+// unit: 36 and 75 instructions and 4 and 5 special functions a value, the gates' above all.  64 x 512 x 5120 bf16: forward 239 us
+// (5.6 TB/s), gradients 482 us (4.9 TB/s).  With few rows and channels the sequence is the only parallelism left: 1 x 32768 x 5120
+// in clusters of 5 forward 342 us (3.9 TB/s), gradients 678 us; 1 x 65536 x 256 111 and 178 us.
 //
 // A step is the map h -> a h + b; maps compose, so a run of steps is one pair (P, H).  Warps take 16
 // steps (8 backward) of 128 bytes of channels (a lane: one 32-bit word, 2 bf16 or 1 f32 channel), CTAs
@@ -84,6 +86,11 @@ __device__ __forceinline__ float ex2(float v) {
 __device__ __forceinline__ float rcp(float v) {
   float d;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(v));
+  return d;
+}
+__device__ __forceinline__ float rsq(float v) {
+  float d;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(v));
   return d;
 }
 __device__ __forceinline__ float root(float v) {
@@ -182,44 +189,59 @@ __device__ __forceinline__ float exp_near(float v) {
   const float p = fmaf(f, fmaf(f, fmaf(f, fmaf(f, fmaf(f, fmaf(f, fmaf(f, 1.f / 5040, 1.f / 720), 1.f / 120), 1.f / 24), 1.f / 6), 0.5f), 1.f), 1.f);
   return p * exp2f(n);
 }
-// 2^v for v <= 0 likewise: what a run of steps leaves of the state multiplies hundreds of times along a sequence (by the approximate
-// instruction gradients of states 2048 tokens back were 1.3e-6 off)
-__device__ __forceinline__ float exp2_near(float v) {
-  constexpr float L = 0.6931471805599453f, L2 = L * L, L3 = L2 * L, L4 = L2 * L2, L5 = L4 * L, L6 = L3 * L3, L7 = L6 * L;
-  const float c = fmaxf(v, -200.f), n = rintf(c), f = c - n;
-  const float p = fmaf(f, fmaf(f, fmaf(f, fmaf(f, fmaf(f, fmaf(f, fmaf(f, L7 / 5040, L6 / 720), L5 / 120), L4 / 24), L3 / 6), L2 / 2), L), 1.f);
-  return p * __int_as_float((max((int)n, -127) + 127) << 23);
-}
 __device__ __forceinline__ float softplus(float v) { return v > 20.f ? v : log1pf(exp_near(v)); }
 
-// 1 / (1 + e^-v); 0 where e^-v is beyond 2^126.  (Two at once by one reciprocal of the product save the special-function unit,
-// 79 % busy forward, a fifth of its work, but need a second form for large products: 249 -> 273 us by the registers.)
+// 1 / (1 + e^-v); 0 where e^-v is beyond 2^126.  (Two at once by one reciprocal of the product need a second form for large
+// products, whose registers cost more than the special-function unit's share: 249 -> 273 us.)
 template <typename V>
 __device__ __forceinline__ V sigmoid(V v) {
   const V e = each(mul(v, all<V>(-LOG2E)), [](float t) { return ex2(t); });
   return each(add(e, all<V>(1.f)), [](float t) { return rcp(t); });
 }
-// a = 2^v and 1 - a^2 for v <= 0.  Down to 2^-0.36 = e^-1/4 from the series of 1 - e^w up to w^6 (5e-8 of it), so that a is
-// off by its own rounding only and 1 - a^2 keeps its digits.  NEAR: no v is further.
+
+// A channel's rate: the exponent of a is -k sigmoid(decay_gate).
+template <typename V>
+struct Rate {
+  V nk;                    // -k log2(e)
+  V scale;                 // sqrt(2 k)
+};
+
+// What a decay gate makes of a step: sigmoid, exponent l of a = 2^l, a and b = sqrt(1 - a^2).
+// NEAR, l above -0.36 (a above e^-1/4): 1 - a = l M(l) and b = sqrt(-2 l ln 2) G(l), with polynomials for M = (1 - 2^l) / l and
+// G^2 = (1 - 2^2l) / (-2 l ln 2) through Chebyshev points (1.2e-8 and 9.6e-9 off), so that a is off by its own rounding only; and with
+// s = q^2 the root is sqrt(2 k) q, so that one reciprocal square root serves the sigmoid and b (the special-function unit
+// is what binds the forward pass).
 constexpr float NEAR_EXPONENT = -0.25f * LOG2E;
 template <bool NEAR, typename V>
-__device__ __forceinline__ V decay_of(V v, V* rest) {
-  constexpr double L = 0.6931471805599453;   // ln 2
-  V m = fma(v, all<V>((float)(-L * L * L * L * L * L / 720)), all<V>((float)(-L * L * L * L * L / 120)));
-  m = fma(v, m, all<V>((float)(-L * L * L * L / 24)));
-  m = fma(v, m, all<V>((float)(-L * L * L / 6)));
-  m = fma(v, m, all<V>((float)(-L * L / 2)));
-  m = fma(v, m, all<V>((float)-L));
-  m = mul(v, m);
-  V a = fma(m, all<V>(-1.f), all<V>(1.f));
-  if constexpr (!NEAR) {
-    const V far = each(v, [](float t) { return ex2(t); });
-    const V u = each(v, far, [](float t, float f) { return t < NEAR_EXPONENT ? 1.f : 0.f; });
-    m = each(each(u, far, [](float t, float f) { return t != 0.f ? 1.f - f : -1.f; }), m, [](float f, float near) { return f < 0.f ? near : f; });
-    a = each(each(u, far, [](float t, float f) { return t != 0.f ? f : -1.f; }), a, [](float f, float near) { return f < 0.f ? near : f; });
+__device__ __forceinline__ void decay_of(V gate, const Rate<V>& k, V* sig, V* l, V* a, V* b) {
+  const V e = each(mul(gate, all<V>(-LOG2E)), [](float t) { return ex2(t); }), d = add(e, all<V>(1.f));
+  if constexpr (NEAR) {
+    const V q = each(d, [](float t) { return rsq(t); });
+    *sig = mul(q, q);
+    const V v = mul(k.nk, *sig);
+    *l = v;
+    V m = fma(v, all<V>(-0.0012021972797811031f), all<V>(-0.009577498771250248f));
+    V g = fma(v, all<V>(0.00284821935929358f), all<V>(0.020715761929750443f));
+    m = fma(v, m, all<V>(-0.05549892038106918f));
+    g = fma(v, g, all<V>(0.10008183121681213f));
+    m = fma(v, m, all<V>(-0.24022626876831055f));
+    g = fma(v, g, all<V>(0.34657302498817444f));
+    m = fma(v, m, all<V>(-0.6931471824645996f));
+    g = fma(v, g, all<V>(1.f));
+    *a = fma(mul(v, m), all<V>(-1.f), all<V>(1.f));
+    *b = mul(mul(k.scale, q), g);
+  } else {
+    *sig = each(d, [](float t) { return rcp(t); });
+    *l = mul(k.nk, *sig);
+    // 1 - a by the series where the difference would cancel
+    const V m = each(*l, [](float t) {
+      const float w = t * 0.6931471805599453f;
+      const float p = fmaf(w, fmaf(w, fmaf(w, fmaf(w, fmaf(w, 1.f / 720, 1.f / 120), 1.f / 24), 1.f / 6), 0.5f), 1.f) * w;
+      return t < NEAR_EXPONENT ? 1.f - ex2(t) : -p;
+    });
+    *a = each(*l, m, [](float t, float u) { return t < NEAR_EXPONENT ? ex2(t) : 1.f - u; });
+    *b = each(m, [](float u) { return root(u * (2.f - u)); });
   }
-  *rest = mul(m, fma(m, all<V>(-1.f), all<V>(2.f)));
-  return a;
 }
 
 // ---- cluster ---------------------------------------------------------------------------------
@@ -254,20 +276,15 @@ __device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity) {
 template <typename T, int WARPS>
 struct Peers {
   typedef typename Lane<T>::Map Map;
-  Map* maps;               // [2][slots][32]
+  Map* maps;               // [2][cluster][32]
   uint64_t* bars;          // [2]
   int cluster, rank;
-  int slots;               // of a buffer: the cluster's, and up to the next four that change nothing
   unsigned* status;        // or NULL
   bool broken;             // a wait gave up: the CTA's results are NaN
 
   __device__ __forceinline__ void arm(int par) { ptx::mbar_arrive_expect_tx(&bars[par], (uint32_t)(cluster * 32 * sizeof(Map))); }
   __device__ __forceinline__ void start() {
     if (cluster == 1) return;
-    for (int j = cluster + (threadIdx.x >> 5); j < slots; j += WARPS) {
-      const Map none = Lane<T>::map(all<typename Lane<T>::V>(1.f), all<typename Lane<T>::V>(0.f));
-      maps[j * 32 + (threadIdx.x & 31)] = maps[(slots + j) * 32 + (threadIdx.x & 31)] = none;
-    }
     if (threadIdx.x == 0) {
       ptx::mbar_init(&bars[0], 1);
       ptx::mbar_init(&bars[1], 1);
@@ -279,7 +296,7 @@ struct Peers {
   }
   __device__ __forceinline__ void send(int64_t turn, const Map& m) {
     const int par = (int)(turn & 1), lane = threadIdx.x & 31;
-    for (int to = threadIdx.x >> 5; to < cluster; to += WARPS) put_remote(&maps[(par * slots + rank) * 32 + lane], &bars[par], to, m);
+    for (int to = threadIdx.x >> 5; to < cluster; to += WARPS) put_remote(&maps[(par * cluster + rank) * 32 + lane], &bars[par], to, m);
   }
   __device__ __forceinline__ const Map* wait(int64_t turn) {
     const int par = (int)(turn & 1);
@@ -289,7 +306,7 @@ struct Peers {
       if (status) atomicCAS(status, 0u, 0x101u);
     }
     if (threadIdx.x == 0 && !broken) arm(par);   // of turn + 2, which no peer sends before this CTA's warps have met again
-    return maps + par * slots * 32 + (threadIdx.x & 31);
+    return maps + par * cluster * 32 + (threadIdx.x & 31);
   }
   __device__ __forceinline__ void end() {
     // no CTA leaves while another may send to it; nothing is released, so that the outputs' stores need not be waited for
@@ -425,23 +442,25 @@ __device__ __forceinline__ unsigned starts_of(int ids, int live) {
   return __ballot_sync(0xffffffffu, next != ids) & ((1u << live) - 1);
 }
 
-// The channels' -k log2(e); whether no step can take the state further than NEAR_EXPONENT.
+// The channels' rates; whether no step can take the state further than NEAR_EXPONENT.
 template <typename T>
-__device__ __forceinline__ typename Lane<T>::V rates(const Args& a, int64_t c, bool* near) {
-  const typename Lane<T>::V lam = Lane<T>::load(a.decay, c, a.D);
-  const float scale = -a.scale * LOG2E;
-  const typename Lane<T>::V nk = each(lam, [&](float v) { return scale * softplus(v); });
+__device__ __forceinline__ Rate<typename Lane<T>::V> rates(const Args& a, int64_t c, bool* near) {
+  typedef typename Lane<T>::V V;
+  const V lam = Lane<T>::load(a.decay, c, a.D);
+  const V k = each(lam, [&](float v) { return a.scale * softplus(v); });
   bool ok = true;
-  each(nk, [&](float v) { ok = ok && v >= NEAR_EXPONENT; return v; });
+  each(k, [&](float v) { ok = ok && v <= 0.25f; return v; });
   *near = __all_sync(0xffffffffu, ok);
-  return nk;
+  return {mul(k, all<V>(-LOG2E)), each(k, [](float v) { return __fsqrt_rn(2.f * v); })};
 }
 
 // ---- forward -----------------------------------------------------------------------------------
 template <typename T>
-constexpr int maps_bytes(int warps, int cluster) { return 2 * 32 * (int)sizeof(typename Lane<T>::Map) * (warps + (cluster > 1 ? (cluster + 3) & ~3 : 0)); }
+constexpr int peers_bytes(int cluster) { return 2 * 32 * (int)sizeof(typename Lane<T>::Map) * (cluster > 1 ? cluster : 0); }
 template <typename T>
-constexpr int fwd_smem(int warps, int cluster) { return 2 * 3 * warps * FWD_STEPS * 128 + maps_bytes<T>(warps, cluster); }
+constexpr int fwd_smem(int warps, int cluster) {
+  return 2 * 3 * warps * FWD_STEPS * 128 + peers_bytes<T>(cluster) + 2 * warps * 32 * (int)sizeof(typename Lane<T>::Map);
+}
 
 template <typename T, int WARPS, bool ALIGNED, bool PACKED>
 __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) forward_kernel(const __grid_constant__ Args a, const int cluster) {
@@ -451,11 +470,11 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) forward_kernel(
   typedef Rows<T, 3, STEPS, WARPS, ALIGNED> In;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t bars[2];
-  Map* const maps = reinterpret_cast<Map*>(smem + 2 * In::STAGE);   // [2][WARPS][32]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = cluster > 1 ? (int)cluster_rank() : 0;
   const int64_t unit = blockIdx.x / (unsigned)cluster, b = unit / a.groups, c0 = (unit - b * a.groups) * (32 * CH), c = c0 + lane * CH;
-  Peers<T, WARPS> peers{maps + 2 * WARPS * 32, bars, cluster, rank, (cluster + 3) & ~3, a.status, false};
+  Map* const maps = reinterpret_cast<Map*>(smem + 2 * In::STAGE);   // [2][WARPS][32]
+  Peers<T, WARPS> peers{maps + 2 * WARPS * 32, bars, cluster, rank, a.status, false};
   const int64_t tiles = (a.L + TILE - 1) / TILE, turns = (tiles + cluster - 1) / cluster, ahead = (int64_t)cluster * TILE;
   const int64_t first = (int64_t)rank * TILE + warp * STEPS;
   In in(a, smem, b, c0, first);
@@ -464,7 +483,7 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) forward_kernel(
   const int* seq = PACKED ? a.seq_idx + b * a.L : nullptr;
   int ids = PACKED ? load_ids<STEPS>(seq, first, a.L) : 0;
   bool near;
-  const V nk = rates<T>(a, c, &near);
+  const Rate<V> rate = rates<T>(a, c, &near);
   V carry = a.state_in ? Lane<T>::load(a.state_in + b * a.D, c, a.D) : all<V>(0.f);
   T* out = static_cast<T*>(a.out[0]) + (b * a.L + first) * a.D + c;
   peers.start();
@@ -484,27 +503,24 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) forward_kernel(
     __syncwarp();
     if (live < STEPS) in.close(stage, live);
     const uint32_t* words = in.words(stage);
-    V av[STEPS], bw[STEPS], sum = all<V>(0.f), H = all<V>(0.f);
+    V av[STEPS], bw[STEPS], P = all<V>(1.f), H = all<V>(0.f);
     auto gates = [&](auto is_near) {
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
-        V b2;
-        const V l = mul(nk, sigmoid(Lane<T>::get(words[(STEPS + s) * 32])));
-        av[s] = decay_of<decltype(is_near)::value>(l, &b2);
-        const V w = mul(sigmoid(Lane<T>::get(words[(2 * STEPS + s) * 32])), Lane<T>::get(words[s * 32]));
-        bw[s] = mul(each(b2, [](float t) { return root(t); }), w);
-        sum = add(sum, l);
+        V sr, l, b;
+        decay_of<decltype(is_near)::value>(Lane<T>::get(words[(STEPS + s) * 32]), rate, &sr, &l, &av[s], &b);
+        bw[s] = mul(b, mul(sigmoid(Lane<T>::get(words[(2 * STEPS + s) * 32])), Lane<T>::get(words[s * 32])));
+        P = mul(P, av[s]);
         if (PACKED && (starts >> s & 1)) H = all<V>(0.f);
         H = fma(av[s], H, bw[s]);
       }
     };
     if (near) gates(std::true_type());
     else gates(std::false_type());
-    Map* const own = maps + (stage * WARPS) * 32 + lane;
-    const V P = PACKED && starts ? all<V>(RESTART) : each(sum, [](float t) { return exp2_near(t); });
-    own[warp * 32] = Lane<T>::map(P, H);
+    Map* const own = maps + stage * WARPS * 32 + lane;
+    own[warp * 32] = Lane<T>::map(PACKED && starts ? all<V>(RESTART) : P, H);
     __syncthreads();
-    V h;                   // the state before the CTA's tile, then before the warp's steps
+    V h;                   // the state before the warp's steps
     if (cluster > 1) {
       V Pt = all<V>(1.f), Ht = all<V>(0.f);
 #pragma unroll
@@ -513,11 +529,13 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) forward_kernel(
       const Map* q = peers.wait(n);
       h = carry;
       for (int j = 0; j < cluster; j += 4) {   // four loads at a time
-        const Map m[4] = {q[j * 32], q[(j + 1) * 32], q[(j + 2) * 32], q[(j + 3) * 32]};
+        Map m[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m[k] = q[min(j + k, cluster - 1) * 32];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           if (j + k == rank) h = carry;
-          carry = through<PACKED>(m[k], carry);
+          if (j + k < cluster) carry = through<PACKED>(m[k], carry);
         }
       }
       if (peers.broken) h = carry = all<V>(NAN);
@@ -553,7 +571,7 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) forward_kernel(
 // ---- backward ----------------------------------------------------------------------------------
 template <typename T>
 constexpr int bwd_smem(int warps, int cluster) {
-  return 2 * 4 * warps * BWD_STEPS * 128 + maps_bytes<T>(warps, cluster) + 2 * warps * 32 * Lane<T>::CH * 4;
+  return 2 * 4 * warps * BWD_STEPS * 128 + peers_bytes<T>(cluster) + 2 * warps * 32 * ((int)sizeof(typename Lane<T>::Map) + Lane<T>::CH * 4);
 }
 
 // Tiles from the last to the first.  The states before each tile are known, so only the reversed
@@ -567,11 +585,11 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) backward_kernel
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t bars[2];
   Map* const maps = reinterpret_cast<Map*>(smem + 2 * In::STAGE);                       // (P, R) [2][WARPS][32]
-  V* const ends = reinterpret_cast<V*>(maps + 2 * 32 * (WARPS + (cluster > 1 ? (cluster + 3) & ~3 : 0)));   // H [2][WARPS][32]
+  V* const ends = reinterpret_cast<V*>(maps + 2 * 32 * (WARPS + (cluster > 1 ? cluster : 0)));   // H [2][WARPS][32]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = cluster > 1 ? (int)cluster_rank() : 0;
   const int64_t unit = blockIdx.x / (unsigned)cluster, b = unit / a.groups, c0 = (unit - b * a.groups) * (32 * CH), c = c0 + lane * CH;
-  Peers<T, WARPS> peers{maps + 2 * WARPS * 32, bars, cluster, rank, (cluster + 3) & ~3, a.status, false};
+  Peers<T, WARPS> peers{maps + 2 * WARPS * 32, bars, cluster, rank, a.status, false};
   const int64_t tiles = (a.L + TILE - 1) / TILE, turns = (tiles + cluster - 1) / cluster, ahead = -(int64_t)cluster * TILE;
   int64_t t0 = ((turns - 1) * cluster + rank) * TILE + warp * STEPS;
   In in(a, smem, b, c0, t0);
@@ -585,7 +603,7 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) backward_kernel
   };
   V state = state_before(t0);
   bool near;
-  const V nk = rates<T>(a, c, &near);
+  const Rate<V> rate = rates<T>(a, c, &near);
   V carry = a.grad_final ? Lane<T>::load(a.grad_final + b * a.D, c, a.D) : all<V>(0.f);
   V total = all<V>(0.f);
   int64_t at = (b * a.L + t0) * a.D + c;
@@ -608,17 +626,14 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) backward_kernel
     __syncwarp();
     if (live < STEPS) in.close(stage, live);
     const uint32_t* words = in.words(stage);
-    V av[STEPS], bv[STEPS], sr[STEPS], si[STEPS], sum = all<V>(0.f), H = all<V>(0.f), R = all<V>(0.f);
+    V av[STEPS], bv[STEPS], sr[STEPS], si[STEPS], P = all<V>(1.f), H = all<V>(0.f), R = all<V>(0.f);
     auto gates = [&](auto is_near) {
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
-        sr[s] = sigmoid(Lane<T>::get(words[(STEPS + s) * 32]));
+        V l;
+        decay_of<decltype(is_near)::value>(Lane<T>::get(words[(STEPS + s) * 32]), rate, &sr[s], &l, &av[s], &bv[s]);
         si[s] = sigmoid(Lane<T>::get(words[(2 * STEPS + s) * 32]));
-        const V l = mul(nk, sr[s]);
-        V b2;
-        av[s] = decay_of<decltype(is_near)::value>(l, &b2);
-        bv[s] = each(b2, [](float t) { return root(t); });
-        sum = add(sum, l);
+        P = mul(P, av[s]);
         if (PACKED && (starts >> s & 1)) H = all<V>(0.f);
         H = fma(av[s], H, mul(bv[s], mul(si[s], Lane<T>::get(words[s * 32]))));
       }
@@ -632,8 +647,7 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) backward_kernel
     }
     Map* const own = maps + (stage * WARPS) * 32 + lane;
     V* const own_end = ends + (stage * WARPS) * 32 + lane;
-    const V P = PACKED && starts ? all<V>(RESTART) : each(sum, [](float t) { return exp2_near(t); });
-    own[warp * 32] = Lane<T>::map(P, R);
+    own[warp * 32] = Lane<T>::map(PACKED && starts ? all<V>(RESTART) : P, R);
     own_end[warp * 32] = H;
     __syncthreads();
     V after;               // what reaches the CTA's tile from behind, then the warp's steps
@@ -649,29 +663,36 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) backward_kernel
       const int k = warp / BEFORE * BEFORE + j;
       if (k < warp) h = through<PACKED>(Lane<T>::map(map_p(own[k * 32]), own_end[k * 32]), h);
     }
-    // the state before each step, into the words of the gates, which are not needed again
+    // m of each step, from the states before them, into the words of the gates, which are not needed again; what the other
+    // CTAs send is on its way meanwhile
     uint32_t* keep = const_cast<uint32_t*>(words);
+    const V nkl = mul(rate.nk, all<V>(0.6931471805599453f));
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
       if (PACKED && (starts >> s & 1)) h = all<V>(0.f);
+      const V w = mul(si[s], Lane<T>::get(words[s * 32]));
+      const V inverse = each(bv[s], [](float t) { return t == 0.f ? 0.f : -rcp(t); });
+      const V m = mul(mul(mul(sr[s], nkl), av[s]), fma(mul(av[s], inverse), w, h));
       if constexpr (CH == 2) {
-        const float2 u = unpack(h);
+        const float2 u = unpack(m);
         keep[(STEPS + s) * 32] = __float_as_uint(u.x);
         keep[(2 * STEPS + s) * 32] = __float_as_uint(u.y);
       } else {
-        keep[(STEPS + s) * 32] = __float_as_uint(h);
+        keep[(STEPS + s) * 32] = __float_as_uint(m);
       }
-      if (s + 1 < STEPS) h = fma(av[s], h, mul(bv[s], mul(si[s], Lane<T>::get(words[s * 32]))));
+      if (s + 1 < STEPS) h = fma(av[s], h, mul(bv[s], w));
     }
     if (cluster > 1) {
       const Map* q = peers.wait(n);
       after = carry;
-      for (int j = peers.slots - 4; j >= 0; j -= 4) {
-        const Map m[4] = {q[j * 32], q[(j + 1) * 32], q[(j + 2) * 32], q[(j + 3) * 32]};
+      for (int j = cluster - 1; j >= 0; j -= 4) {   // four loads at a time
+        Map m[4];
 #pragma unroll
-        for (int k = 3; k >= 0; --k) {
-          if (j + k == rank) after = carry;
-          carry = through<PACKED>(m[k], carry);
+        for (int k = 0; k < 4; ++k) m[k] = q[max(j - k, 0) * 32];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (j - k == rank) after = carry;
+          if (j - k >= 0) carry = through<PACKED>(m[k], carry);
         }
       }
       if (peers.broken) after = carry = all<V>(NAN);
@@ -690,16 +711,13 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) backward_kernel
 #pragma unroll
     for (int s = STEPS - 1; s >= 0; --s) {
       const V x = Lane<T>::get(words[s * 32]), w = mul(si[s], x);
-      V hp;
-      if constexpr (CH == 2) hp = pack(__uint_as_float(words[(STEPS + s) * 32]), __uint_as_float(words[(2 * STEPS + s) * 32]));
-      else hp = __uint_as_float(words[(STEPS + s) * 32]);
+      V m;
+      if constexpr (CH == 2) m = pack(__uint_as_float(words[(STEPS + s) * 32]), __uint_as_float(words[(2 * STEPS + s) * 32]));
+      else m = __uint_as_float(words[(STEPS + s) * 32]);
       const V d = add(after, Lane<T>::get(words[(3 * STEPS + s) * 32]));
       after = mul(av[s], d);
       if (PACKED && (starts >> s & 1)) after = all<V>(0.f);
-      const V inverse = each(bv[s], [](float t) { return t == 0.f ? 0.f : -rcp(t); });
-      const V la = mul(sr[s], mul(nk, all<V>(0.6931471805599453f)));
-      const V dm = mul(mul(d, mul(la, av[s])), fma(mul(av[s], inverse), w, hp));
-      const V db = mul(d, bv[s]);
+      const V dm = mul(d, m), db = mul(d, bv[s]);
       total = add(total, dm);
       if (s < live) {
         store_word<T, ALIGNED>(static_cast<T*>(a.out[0]) + row, c, a.D, mul(db, si[s]));
@@ -779,9 +797,9 @@ __global__ void __launch_bounds__(256) step_kernel(const StepArgs a) {
     Pack y;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      float b2;
-      const float A = decay_of<false>(nk[i] * sigmoid(ld(&pr.v[i])), &b2);
-      h.v[i] = fmaf(A, h.v[i], root(b2) * (sigmoid(ld(&pg.v[i])) * ld(&px.v[i])));
+      float s, l, A, B;
+      decay_of<false>(ld(&pr.v[i]), Rate<float>{nk[i], 0.f}, &s, &l, &A, &B);
+      h.v[i] = fmaf(A, h.v[i], B * (sigmoid(ld(&pg.v[i])) * ld(&px.v[i])));
       st(&y.v[i], h.v[i]);
     }
     *reinterpret_cast<State*>(a.new_state + row * a.D + c) = h;
@@ -843,31 +861,37 @@ int capacity_of(const Kernel& k, int cluster) {
   return n;
 }
 
-// Microseconds of `units` clusters, from what was measured: a tile takes 1.05 and 0.16 more for each
-// warp that its SM holds (4 warps 1.7, 16 warps 3.6; forward and backward alike), 0.12 for each warp of a CTA above 4
-// (the warps meet), a cluster's exchange 0.35 + 0.04 c, a CTA 2 to start.  Both sides: 64 x 512 x 5120 forward, CTAs of 4
-// warps alone 248 us, of 8 301, pairs of CTAs 342; 1 x 65536 x 256: alone 1711, clusters of 16 CTAs of 4 warps 170, of 16 warps 103.
-double time_of(const Kernel& k, int64_t units, int64_t L, int cluster) {
+// Microseconds of `units` clusters: a turn takes `turn`, and `warp` more for each warp that its SM holds, `wide` for each warp of a CTA
+// above 4 (they meet), and in a cluster `exchange` and `peer` for each CTA; a CTA takes `start`.  Fitted to 26 shapes of both types, of
+// 1 to 64 rows, 300 to 65536 tokens and 128 to 8192 channels, each with 1 to 16 CTAs of 4, 8 and 16 warps: what the rule picks is 1.7 %
+// slower than the best on average (11 and 14 % at worst).  Both sides, forward: 64 x 512 x 5120, CTAs of 4 warps alone 239 us, of 8 281,
+// pairs of CTAs 289; 1 x 65536 x 256: alone 1711, clusters of 16 CTAs of 4 warps 170, of 16 warps 111.
+struct Times {
+  double turn, warp, exchange, peer, start, wide;
+};
+constexpr Times FORWARD = {0.83, 0.167, 0.374, 0.033, 2.8, 0.068}, BACKWARD = {0.65, 0.184, 0.101, 0.141, 1.24, 0.082};
+
+double time_of(const Kernel& k, const Times& t, int64_t units, int64_t L, int cluster) {
   const int cap = capacity_of(k, cluster);
   if (cap <= 0) return 1e30;
   const int64_t turns = cdiv(cdiv(L, k.tile), cluster), full = units / cap, rest = units - full * cap;
-  const double exchange = (cluster > 1 ? 0.35 + 0.04 * cluster : 0.0) + 0.12 * (k.warps - 4);
-  const double turn = 1.05 + 0.16 * MAX_WARPS + exchange;
+  const double alone = t.turn + (cluster > 1 ? t.exchange + t.peer * cluster : 0.0) + t.wide * (k.warps - 4);
   const double warps = std::min<double>(MAX_WARPS, k.warps * (double)cdiv(rest * cluster, SMS));
-  return (double)full * (2.0 + (double)turns * turn) + (rest ? 2.0 + (double)turns * (1.05 + 0.16 * warps + exchange) : 0.0);
+  return (double)full * (t.start + (double)turns * (alone + t.warp * MAX_WARPS)) +
+         (rest ? t.start + (double)turns * (alone + t.warp * warps) : 0.0);
 }
 
 struct Choice {
   int kernel, cluster;
 };
 
-Choice pick(const Kernel* list, int n, int64_t units, int64_t L) {
+Choice pick(const Kernel* list, int n, const Times& times, int64_t units, int64_t L) {
   Choice best = {0, 1};
   double least = 1e300;
   for (int k = 0; k < n; ++k)
     for (int c = 1; c <= MAX_CLUSTER && (c == 1 || (int64_t)(c - 1) * list[k].tile < L); ++c) {
-      const double t = time_of(list[k], units, L, c);
-      if (t < least * 0.98) {
+      const double t = time_of(list[k], times, units, L, c);
+      if (t < least) {
         least = t;
         best = {k, c};
       }
@@ -974,7 +998,7 @@ cudaError_t choose(const ssd_gated_recurrence_params_t* p, const Args& a, bool b
     const cudaError_t e = make_ready(ks->list[i]);
     if (e != cudaSuccess) return e;
   }
-  *c = pick(ks->list, ks->n, p->batch * a.groups, a.L);
+  *c = pick(ks->list, ks->n, backward ? BACKWARD : FORWARD, p->batch * a.groups, a.L);
   return cudaSuccess;
 }
 
