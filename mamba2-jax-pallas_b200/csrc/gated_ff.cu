@@ -304,11 +304,12 @@ __device__ __forceinline__ void run(const Product& p, uint8_t* smem_raw, gemm::C
 // ---------------------------------------------------------------------------
 // f32 values as three bf16 terms
 // ---------------------------------------------------------------------------
-// Two values as a pair of bf16, and what is left of them.  A finite value that would round to infinity is cut instead.  (What
-// is left of an infinity is NaN: a value that is not finite makes its products so.)
+// Two values as a pair of bf16, and what is left of them.  (What is left of an infinity is NaN: a value that is not finite makes its
+// products so.)  CUT: a finite value that would round to infinity is cut instead.
+template <bool CUT>
 __device__ __forceinline__ uint32_t term_of(float& a, float& b) {
   uint32_t w = gemm::pack_bf16(a, b);
-  if ((w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u) w = __float_as_uint(a) >> 16 | (__float_as_uint(b) & 0xffff0000u);
+  if (CUT && ((w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u)) w = __float_as_uint(a) >> 16 | (__float_as_uint(b) & 0xffff0000u);
   a -= __uint_as_float(w << 16);
   b -= __uint_as_float(w & 0xffff0000u);
   return w;
@@ -321,9 +322,10 @@ __device__ __forceinline__ void planes_of(const float (&x)[8], uint4 (&q)[PLANES
     q[0] = make_uint4(gemm::pack_bf16(x[0], x[1]), gemm::pack_bf16(x[2], x[3]), gemm::pack_bf16(x[4], x[5]), gemm::pack_bf16(x[6], x[7]));
   } else {
     float v[8] = {x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]};
+    q[0] = make_uint4(term_of<true>(v[0], v[1]), term_of<true>(v[2], v[3]), term_of<true>(v[4], v[5]), term_of<true>(v[6], v[7]));
 #pragma unroll
-    for (int i = 0; i < PLANES; ++i)
-      q[i] = make_uint4(term_of(v[0], v[1]), term_of(v[2], v[3]), term_of(v[4], v[5]), term_of(v[6], v[7]));
+    for (int i = 1; i < PLANES; ++i)
+      q[i] = make_uint4(term_of<false>(v[0], v[1]), term_of<false>(v[2], v[3]), term_of<false>(v[4], v[5]), term_of<false>(v[6], v[7]));
   }
 }
 
@@ -483,35 +485,29 @@ __global__ void __launch_bounds__(THREADS, 1) hidden_kernel(const __grid_constan
           }
         }
       } else {
-        // three planes of one result after another
-        auto put = [&](float (&x)[COLS], uint8_t* out) {
+        // three planes of one result after another (hidden values above 3.389e38 count as infinite)
+        auto put = [&](float* x, uint8_t* out) {
 #pragma unroll
           for (int k = 0; k < PLANES; ++k) {
 #pragma unroll
             for (int i = 0; i < COLS / 8; ++i)
-              h[i] = make_uint4(term_of(x[8 * i], x[8 * i + 1]), term_of(x[8 * i + 2], x[8 * i + 3]), term_of(x[8 * i + 4], x[8 * i + 5]),
-                                term_of(x[8 * i + 6], x[8 * i + 7]));
+              h[i] = make_uint4(term_of<false>(x[8 * i], x[8 * i + 1]), term_of<false>(x[8 * i + 2], x[8 * i + 3]),
+                                term_of<false>(x[8 * i + 4], x[8 * i + 5]), term_of<false>(x[8 * i + 6], x[8 * i + 7]));
             store_block(stage, h, out + k * a.plane, a.ld, row0, a.rows, f0, a.F);
           }
         };
-        float x[COLS];
         if constexpr (BACKWARD) {
+          float x[COLS];
 #pragma unroll
           for (int i = 0; i < COLS; i += 4) {
             const float4 d = *reinterpret_cast<const float4*>(stage + gemm::epi_at<CHUNKS / 4>(lane, i / 4));
             x[i] = d.x; x[i + 1] = d.y; x[i + 2] = d.z; x[i + 3] = d.w;
           }
           put(x, a.h);
-#pragma unroll
-          for (int i = 0; i < COLS; ++i) x[i] = v[c0 + i];
-          put(x, a.dg);
-#pragma unroll
-          for (int i = 0; i < COLS; ++i) x[i] = v[32 + c0 + i];
-          put(x, a.du);
+          put(v + c0, a.dg);
+          put(v + 32 + c0, a.du);
         } else {
-#pragma unroll
-          for (int i = 0; i < COLS; ++i) x[i] = v[c0 + i];
-          put(x, a.h);
+          put(v + c0, a.h);
         }
       }
     }
