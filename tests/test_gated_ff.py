@@ -417,3 +417,41 @@ def test_refusals():
         with pytest.raises(error):
             call()
             pytest.fail(f"case {k} was not refused")
+
+
+def test_c_refusals_need_no_gpu():
+    """Arguments that the library has to refuse before it touches a device."""
+    from mamba2_b200 import _lib
+    lib = _lib.load()
+
+    def params(**kw):
+        p = _lib.GatedFfParams(50, 64, 96, 32, 64, 64, 64, 96, 1, 0, 256, 256, 256, 256, 256)
+        for k, v in kw.items():
+            setattr(p, k, v)
+        return p
+
+    def grads(**kw):
+        g = _lib.GatedFfGrads(32, 256, 256, 256, 256, 256, 1, 0)
+        for k, v in kw.items():
+            setattr(g, k, v)
+        return g
+
+    bad = [dict(tokens=0), dict(dim=-1), dict(hidden=0), dict(dim_out=0), dict(dtype=2), dict(activation=4),
+           dict(activation=-1), dict(x_stride_row=63), dict(w_gate_stride_row=63), dict(w_up_stride_row=0),
+           dict(w_down_stride_row=95), dict(x=None), dict(w_gate=None), dict(w_up=None), dict(w_down=None)]
+    assert lib.ssd_gated_ff(None, 256, 1 << 30, None) == 1
+    for kw in bad:
+        assert lib.ssd_gated_ff_workspace_bytes(params(**kw)) == 0, kw
+        assert lib.ssd_gated_ff(params(**kw), 256, 1 << 30, None) == 1, kw
+        assert lib.ssd_gated_ff_grad_workspace_bytes(params(**kw), grads()) == 0, kw
+        assert lib.ssd_gated_ff_grad(params(**kw), grads(), 256, 1 << 30, None) == 1, kw
+    assert lib.ssd_gated_ff(params(y=None), 256, 1 << 30, None) == 1
+    assert lib.ssd_gated_ff(params(tokens=1 << 31), 256, 1 << 60, None) == 2
+    for kw in (dict(grad_y=None), dict(grad_y_stride_row=31), dict(grad_weight_dtype=2), dict(grad_w_up=None)):
+        assert lib.ssd_gated_ff_grad(params(), grads(**kw), 256, 1 << 30, None) == 1, kw
+    assert lib.ssd_gated_ff_grad(params(), None, 256, 1 << 30, None) == 1
+    need = lib.ssd_gated_ff_grad_workspace_bytes(params(), grads())
+    assert need > lib.ssd_gated_ff_workspace_bytes(params()) > 256
+    assert lib.ssd_gated_ff_grad(params(), grads(), 256, need - 1, None) == 4
+    assert lib.ssd_gated_ff_grad(params(), grads(), None, need, None) == 4
+    assert lib.ssd_gated_ff_grad(params(), grads(), 264, need, None) == 3

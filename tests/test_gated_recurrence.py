@@ -489,3 +489,41 @@ def test_refusals():
         with pytest.raises(error):
             call()
             pytest.fail(f"case {k} was not refused")
+
+
+def test_c_refusals_need_no_gpu():
+    """Arguments that the library has to refuse before it touches a device."""
+    from mamba2_b200 import _lib
+    lib = _lib.load()
+    P, G, S = _lib.GatedRecurrenceParams, _lib.GatedRecurrenceGrads, _lib.GatedRecurrenceUpdateParams
+
+    def params(**kw):
+        p = P(2, 70, 8, 560, 8, 560, 8, 560, 8, 0, 8.0, 256, 256, 256, 256, None, None, 256, None, None, None)
+        for k, v in kw.items():
+            setattr(p, k, v)
+        return p
+
+    grads = G(560, 8, 256, None, 256, 256, 256, 256, None)
+    assert lib.ssd_gated_recurrence(None, None) == 1
+    bad = [dict(batch=0), dict(seqlen=0), dict(dim=-1), dict(dtype=2), dict(scale=-1.0), dict(scale=float("nan")),
+           dict(scale=float("inf"))]
+    for kw in bad + [dict(x=None), dict(decay=None), dict(y=None)]:
+        assert lib.ssd_gated_recurrence(params(**kw), None) == 1, kw
+        assert lib.ssd_last_error()
+    assert lib.ssd_gated_recurrence(params(seqlen=1 << 31), None) == 2
+    assert lib.ssd_gated_recurrence(params(batch=1 << 30, dim=1 << 20), None) == 2
+    need = lib.ssd_gated_recurrence_grad_workspace_bytes(params())
+    assert need > lib.ssd_gated_recurrence_grad_workspace_bytes(params(checkpoints=256)) > 0
+    for kw in bad:
+        assert lib.ssd_gated_recurrence_grad_workspace_bytes(params(**kw)) == 0, kw
+        assert lib.ssd_gated_recurrence_grad(params(**kw), grads, 256, need, None) == 1, kw
+    assert lib.ssd_gated_recurrence_grad(params(), None, 256, need, None) == 1
+    assert lib.ssd_gated_recurrence_grad(params(), G(560, 8, None, None, 256, 256, 256, 256, None), 256, need, None) == 1
+    assert lib.ssd_gated_recurrence_grad(params(), G(560, 8, 256, None, 256, None, 256, 256, None), 256, need, None) == 1
+    assert lib.ssd_gated_recurrence_grad(params(), grads, 256, need - 1, None) == 4
+    assert lib.ssd_gated_recurrence_grad(params(), grads, None, need, None) == 4
+    assert lib.ssd_gated_recurrence_grad(params(), grads, 264, need, None) == 3
+    good = (2, 8, 8, 8, 8, 0, 8.0, 256, 256, 256, 256, 256, 256, 256)
+    for k, v in ((0, 0), (1, -1), (5, 3), (6, -1.0), (7, None), (10, None), (11, None), (12, None), (13, None)):
+        p = S(*(v if j == k else a for j, a in enumerate(good)))
+        assert lib.ssd_gated_recurrence_update(p, None) == 1, k
