@@ -137,7 +137,9 @@ struct Lane<bf16> {
     const float2 a = unpack(p), b = unpack(h);
     return {a.x, b.x, a.y, b.y};
   }
-  static __device__ __forceinline__ V load(const float* p, int64_t c, int64_t D) { return pack(c < D ? p[c] : 0.f, c + 1 < D ? p[c + 1] : 0.f); }
+  static __device__ __forceinline__ V load(const float* p, int64_t c, int64_t D, float none = 0.f) {
+    return pack(c < D ? p[c] : none, c + 1 < D ? p[c + 1] : none);
+  }
   static __device__ __forceinline__ void store(float* p, int64_t c, int64_t D, V v) {
     const float2 f = unpack(v);
     if (c < D) p[c] = f.x;
@@ -152,7 +154,7 @@ struct Lane<float> {
   static __device__ __forceinline__ V get(uint32_t u) { return __uint_as_float(u); }
   static __device__ __forceinline__ uint32_t put(V v) { return __float_as_uint(v); }
   static __device__ __forceinline__ Map map(V p, V h) { return {p, h}; }
-  static __device__ __forceinline__ V load(const float* p, int64_t c, int64_t D) { return c < D ? p[c] : 0.f; }
+  static __device__ __forceinline__ V load(const float* p, int64_t c, int64_t D, float none = 0.f) { return c < D ? p[c] : none; }
   static __device__ __forceinline__ void store(float* p, int64_t c, int64_t D, V v) {
     if (c < D) p[c] = v;
   }
@@ -446,7 +448,7 @@ __device__ __forceinline__ unsigned starts_of(int ids, int live) {
 template <typename T>
 __device__ __forceinline__ Rate<typename Lane<T>::V> rates(const Args& a, int64_t c, bool* near) {
   typedef typename Lane<T>::V V;
-  const V lam = Lane<T>::load(a.decay, c, a.D);
+  const V lam = Lane<T>::load(a.decay, c, a.D, -1000.f);   // (channels beyond the last decay by nothing)
   const V k = each(lam, [&](float v) { return a.scale * softplus(v); });
   bool ok = true;
   each(k, [&](float v) { ok = ok && v <= 0.25f; return v; });

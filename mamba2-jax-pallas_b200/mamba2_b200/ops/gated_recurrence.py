@@ -55,7 +55,12 @@ def _ids(seq_idx, x):
     ids = _lib.index_list(seq_idx, "seq_idx")
     if ids.shape != x.shape[:2] or ids.device != x.device:
         raise ValueError("seq_idx must be (batch, seqlen) on x's device")
-    return ids.to(torch.int32)
+    if ids.dtype is torch.int32 or not ids.numel():
+        return ids.to(torch.int32)
+    # only where neighbours differ counts, and wider ids need not fit 32 bits
+    seq = ids.new_zeros(ids.shape, dtype=torch.int32)
+    torch.cumsum(ids[:, 1:] != ids[:, :-1], 1, dtype=torch.int32, out=seq[:, 1:])
+    return seq
 
 
 def _checkpoint_shape(x):

@@ -188,6 +188,19 @@ def test_every_token_its_own_sequence():
 
 
 @gpu
+def test_ids_of_64_bits():
+    """Ids that differ by a multiple of 2^32, and negative ones."""
+    x, r, i, lam, *_ = (t.cuda() for t in inputs(2, 90, 32, seed=4))
+    ids = torch.zeros((2, 90), dtype=torch.int64, device="cuda")
+    ids[0, 40:], ids[0, 70:], ids[1, 10:] = 1 << 32, -(1 << 40), -1
+    small = torch.zeros((2, 90), dtype=torch.int32, device="cuda")
+    small[0, 40:], small[0, 70:], small[1, 10:] = 5, -7, 3
+    assert torch.equal(gated_recurrence(x, r, i, lam, seq_idx=ids), gated_recurrence(x, r, i, lam, seq_idx=small))
+    one = torch.zeros((2, 1), dtype=torch.int64, device="cuda")
+    assert torch.equal(gated_recurrence(x[:, :1], r[:, :1], i[:, :1], lam, seq_idx=one), gated_recurrence(x, r, i, lam)[:, :1])
+
+
+@gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_values_do_not_cross_sequences(dtype):
     """NaN and infinities in one packed sequence, in the state before it and in the gradient."""
