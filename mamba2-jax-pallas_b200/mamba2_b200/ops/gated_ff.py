@@ -6,6 +6,14 @@ import torch
 from .. import _lib
 
 
+def _rows(t, width):
+    """Rows of ``width`` contiguous values at one distance, a view where there is one, and that distance."""
+    if t.is_contiguous():
+        return t, width
+    t = _lib.rows2d(t, width)
+    return t, _lib.row_stride(t)
+
+
 def _prepare(x, w_gate, w_up, w_down, activation):
     if not (isinstance(x, torch.Tensor) and isinstance(w_gate, torch.Tensor) and isinstance(w_up, torch.Tensor) and
             isinstance(w_down, torch.Tensor)):
@@ -13,10 +21,10 @@ def _prepare(x, w_gate, w_up, w_down, activation):
     if not x.is_cuda:
         raise ValueError("x must be a CUDA tensor (no CPU path)")
     dtype, dev = x.dtype, x.device
-    if w_gate.dtype != dtype or w_up.dtype != dtype or w_down.dtype != dtype:
+    if w_gate.dtype is not dtype or w_up.dtype is not dtype or w_down.dtype is not dtype:
         raise TypeError(f"w_gate ({w_gate.dtype}), w_up ({w_up.dtype}), w_down ({w_down.dtype}) and x ({dtype}) must have the "
                         "same dtype")
-    if w_gate.device != dev or w_up.device != dev or w_down.device != dev:
+    if not dev == w_gate.device == w_up.device == w_down.device:
         raise ValueError("the weights must be on x's device")
     act = _lib.ACTIVATIONS.get(activation)
     if act is None:
@@ -31,9 +39,8 @@ def _prepare(x, w_gate, w_up, w_down, activation):
         raise ValueError("the weights must not be empty")
     if x.dim() < 1 or x.shape[-1] != dim:
         raise ValueError(f"x {tuple(x.shape)} must end in the weights' {dim} columns")
-    xr, g, u, d = _lib.rows2d(x, dim), _lib.rows2d(w_gate, dim), _lib.rows2d(w_up, dim), _lib.rows2d(w_down, hidden)
-    stride = _lib.row_stride
-    p = _lib.GatedFfParams(xr.shape[0], dim, hidden, out, stride(xr), stride(g), stride(u), stride(d), _lib.dtype_code(x), act,
+    (xr, xs), (g, gs), (u, us), (d, ds) = _rows(x, dim), _rows(w_gate, dim), _rows(w_up, dim), _rows(w_down, hidden)
+    p = _lib.GatedFfParams(xr.numel() // dim, dim, hidden, out, xs, gs, us, ds, _lib.dtype_code(x), act,
                            xr.data_ptr(), g.data_ptr(), u.data_ptr(), d.data_ptr(), None)
     return p, (xr, g, u, d)   # (copies have to live until the call)
 
@@ -49,7 +56,7 @@ def gated_feed_forward(x, w_gate, w_up, w_down, *, activation: str = "silu", che
     ``gated_feed_forward_grad`` gives the gradients.
     """
     p, rows = _prepare(x, w_gate, w_up, w_down, activation)
-    y = rows[0].new_empty((*x.shape[:-1], p.dim_out))
+    y = torch.empty_like(x) if p.dim_out == p.dim and x.is_contiguous() else x.new_empty((*x.shape[:-1], p.dim_out))
     if p.tokens == 0:
         return y
     p.y = y.data_ptr()
@@ -86,8 +93,8 @@ def gated_feed_forward_grad(x, w_gate, w_up, w_down, grad_out, *, activation: st
     gw = [new(w.shape, dtype=wd, device=dev) if need_weight_grad else None for w in (w_gate, w_up, w_down)]
     if p.tokens == 0 or not (need_input_grad or need_weight_grad):
         return gx, *gw
-    dy = _lib.rows2d(grad_out, w_down.shape[0])
-    g = _lib.GatedFfGrads(_lib.row_stride(dy), dy.data_ptr(), _lib.ptr(gx), *(_lib.ptr(t) for t in gw), wd is torch.bfloat16, 0)
+    dy, dys = _rows(grad_out, p.dim_out)
+    g = _lib.GatedFfGrads(dys, dy.data_ptr(), _lib.ptr(gx), *(_lib.ptr(t) for t in gw), wd is torch.bfloat16, 0)
     lib = _lib.load()
     with _lib.on_device(dev):
         ws = torch.empty(lib.ssd_gated_ff_grad_workspace_bytes(p, g), dtype=torch.uint8, device=dev)

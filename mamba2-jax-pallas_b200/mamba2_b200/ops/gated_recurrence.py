@@ -27,12 +27,12 @@ def _inputs(x, decay_gate, input_gate, decay, scale, dims):
     if decay_gate.shape != shape or input_gate.shape != shape:
         raise ValueError(f"decay_gate {tuple(decay_gate.shape)} and input_gate {tuple(input_gate.shape)} must have x's "
                          f"shape {tuple(shape)}")
-    if decay_gate.dtype != dtype or input_gate.dtype != dtype:
+    if decay_gate.dtype is not dtype or input_gate.dtype is not dtype:
         raise TypeError(f"decay_gate ({decay_gate.dtype}), input_gate ({input_gate.dtype}) and x ({dtype}) must have the "
                         "same dtype")
     if decay.shape != shape[-1:]:
         raise ValueError("decay must be (dim,)")
-    if decay_gate.device != dev or input_gate.device != dev or decay.device != dev:
+    if not dev == decay_gate.device == input_gate.device == decay.device:
         raise ValueError("decay_gate, input_gate and decay must be on x's device")
     if not 0 <= scale <= 3.4e38:
         raise ValueError("scale must be finite and not negative")
@@ -41,12 +41,17 @@ def _inputs(x, decay_gate, input_gate, decay, scale, dims):
     return _lib.dtype_code(x), _channels_last(x), _channels_last(decay_gate), _channels_last(input_gate), decay
 
 
+def _like(x):
+    """A new contiguous tensor of x's shape and type."""
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+
+
 def _state(t, name, x):
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or t.device != x.device or tuple(t.shape) != (x.shape[0], x.shape[-1]):
+    if not isinstance(t, torch.Tensor) or t.device != x.device or t.shape != (x.shape[0], x.shape[-1]):
         raise ValueError(f"{name} must be a (batch, dim) tensor on x's device")
-    return _lib.dev(t, name, _F32)
+    return t if t.dtype is _F32 and t.is_contiguous() else t.to(_F32).contiguous()
 
 
 def _ids(seq_idx, x):
@@ -67,12 +72,11 @@ def _checkpoint_shape(x):
     return (x.shape[0], -(-x.shape[1] // _TILE), x.shape[2])
 
 
-def _params(code, x, decay_gate, input_gate, decay, scale, initial, ids, y, final, points, status):
-    b, L, d = x.shape
-    return _lib.GatedRecurrenceParams(b, L, d, x.stride(0), x.stride(1), decay_gate.stride(0), decay_gate.stride(1),
-                                      input_gate.stride(0), input_gate.stride(1), code, scale, x.data_ptr(),
-                                      decay_gate.data_ptr(), input_gate.data_ptr(), decay.data_ptr(), _lib.ptr(initial),
-                                      _lib.ptr(ids), _lib.ptr(y), _lib.ptr(final), _lib.ptr(points), _lib.ptr(status))
+def _params(code, x, decay_gate, input_gate, decay, scale, *optional):
+    ptrs = [None if t is None else t.data_ptr() for t in optional]
+    return _lib.GatedRecurrenceParams(*x.shape, *x.stride()[:2], *decay_gate.stride()[:2], *input_gate.stride()[:2], code,
+                                      scale, x.data_ptr(), decay_gate.data_ptr(), input_gate.data_ptr(), decay.data_ptr(),
+                                      *ptrs)
 
 
 def gated_recurrence(x, decay_gate, input_gate, decay, *, scale: float = 8.0, initial_state=None, seq_idx=None,
@@ -95,7 +99,7 @@ def gated_recurrence(x, decay_gate, input_gate, decay, *, scale: float = 8.0, in
     code, xs, r, i, lam = _inputs(x, decay_gate, input_gate, decay, scale, 3)
     h0, ids = _state(initial_state, "initial_state", x), _ids(seq_idx, x)
     b, L, d = x.shape
-    y = xs.new_empty((b, L, d))
+    y = _like(xs)
     final = xs.new_empty((b, d), dtype=_F32) if return_final_state else None
     points = xs.new_empty(_checkpoint_shape(x), dtype=_F32) if return_checkpoints else None
     if b and L:
@@ -136,7 +140,7 @@ def gated_recurrence_grad(x, decay_gate, input_gate, decay, grad_out, *, scale: 
         raise ValueError(f"checkpoints must be the float32 {_checkpoint_shape(x)} tensor that gated_recurrence returned")
     g = _channels_last(grad_out)
     b, L, d = x.shape
-    gx, gr, gi = xs.new_empty((b, L, d)), xs.new_empty((b, L, d)), xs.new_empty((b, L, d))
+    gx, gr, gi = _like(xs), _like(xs), _like(xs)
     gd = xs.new_empty(d, dtype=_F32)
     gh = xs.new_empty((b, d), dtype=_F32) if h0 is not None else None
     if not (b and L):
@@ -169,12 +173,14 @@ def gated_recurrence_update(state, x, decay_gate, input_gate, decay, *, scale: f
     code, xs, r, i, lam = _inputs(x, decay_gate, input_gate, decay, scale, 2)
     if state.shape != x.shape or state.device != x.device:
         raise ValueError("state must be (batch, dim) on x's device")
-    if inplace and not state.is_contiguous():
-        raise ValueError("inplace=True needs a contiguous state")
     b, d = x.shape
-    old = state.contiguous()
-    new = state if inplace else xs.new_empty((b, d), dtype=_F32)
-    y = xs.new_empty((b, d))
+    old = state
+    if not state.is_contiguous():
+        if inplace:
+            raise ValueError("inplace=True needs a contiguous state")
+        old = state.contiguous()
+    new = state if inplace else torch.empty_like(old)
+    y = _like(xs)
     if b:
         p = _lib.GatedRecurrenceUpdateParams(b, d, xs.stride(0), r.stride(0), i.stride(0), code, scale, xs.data_ptr(),
                                              r.data_ptr(), i.data_ptr(), lam.data_ptr(), old.data_ptr(), new.data_ptr(),
