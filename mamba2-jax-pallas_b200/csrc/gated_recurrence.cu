@@ -182,6 +182,14 @@ __device__ __forceinline__ void compose(const M& m, V& P, V& H) {   // (P, H) th
   }
 }
 
+// The CTA's warps meet; whether a sequence starts in any of their steps.
+template <bool PACKED>
+__device__ __forceinline__ bool meet(bool mine) {
+  if constexpr (PACKED) return __syncthreads_or(mine);
+  __syncthreads();
+  return false;
+}
+
 // ---- per-channel and per-value arithmetic --------------------------------------------------
 // e^v within 2 units, where the approximate instruction's 2^-22 would be one error of all of a channel's steps:
 // v = n ln 2 + f in two parts (Cody and Waite), the series up to f^7 (5e-9)
@@ -513,20 +521,33 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) forward_kernel(
         decay_of<decltype(is_near)::value>(Lane<T>::get(words[(STEPS + s) * 32]), rate, &sr, &l, &av[s], &b);
         bw[s] = mul(b, mul(sigmoid(Lane<T>::get(words[(2 * STEPS + s) * 32])), Lane<T>::get(words[s * 32])));
         P = mul(P, av[s]);
-        if (PACKED && (starts >> s & 1)) H = all<V>(0.f);
         H = fma(av[s], H, bw[s]);
       }
     };
     if (near) gates(std::true_type());
     else gates(std::false_type());
+    if (PACKED && starts) {   // seldom: again, from where the last sequence starts
+      P = all<V>(RESTART);
+      H = all<V>(0.f);
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        if (starts >> s & 1) H = all<V>(0.f);
+        H = fma(av[s], H, bw[s]);
+      }
+    }
     Map* const own = maps + stage * WARPS * 32 + lane;
-    own[warp * 32] = Lane<T>::map(PACKED && starts ? all<V>(RESTART) : P, H);
-    __syncthreads();
+    own[warp * 32] = Lane<T>::map(P, H);
+    const bool restarts = meet<PACKED>(starts != 0);
     V h;                   // the state before the warp's steps
     if (cluster > 1) {
       V Pt = all<V>(1.f), Ht = all<V>(0.f);
+      if (restarts) {
 #pragma unroll
-      for (int j = 0; j < WARPS; ++j) compose<PACKED>(own[j * 32], Pt, Ht);
+        for (int j = 0; j < WARPS; ++j) compose<PACKED>(own[j * 32], Pt, Ht);
+      } else {
+#pragma unroll
+        for (int j = 0; j < WARPS; ++j) compose<false>(own[j * 32], Pt, Ht);
+      }
       peers.send(n, Lane<T>::map(Pt, Ht));
       const Map* q = peers.wait(n);
       h = carry;
@@ -541,28 +562,46 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) forward_kernel(
         }
       }
       if (peers.broken) h = carry = all<V>(NAN);
+      if (restarts) {
 #pragma unroll
-      for (int j = 0; j < WARPS - 1; ++j)
-        if (j < warp) h = through<PACKED>(own[j * 32], h);
+        for (int j = 0; j < WARPS - 1; ++j)
+          if (j < warp) h = through<PACKED>(own[j * 32], h);
+      } else {
+#pragma unroll
+        for (int j = 0; j < WARPS - 1; ++j)
+          if (j < warp) h = through<false>(own[j * 32], h);
+      }
     } else {
       h = carry;
+      if (restarts) {
 #pragma unroll
-      for (int j = 0; j < WARPS; ++j) {
-        if (j == warp) h = carry;
-        carry = through<PACKED>(own[j * 32], carry);
+        for (int j = 0; j < WARPS; ++j) {
+          if (j == warp) h = carry;
+          carry = through<PACKED>(own[j * 32], carry);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < WARPS; ++j) {
+          if (j == warp) h = carry;
+          carry = through<false>(own[j * 32], carry);
+        }
       }
     }
     if (a.states && (warp * STEPS) % POINT == 0 && t0 < a.L)
       Lane<T>::store(a.states + (b * a.points + t0 / POINT) * a.D, c, a.D, h);
     if (a.out[0]) {
       T* o = out;
+      auto run = [&](auto restarts) {
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        if (PACKED && (starts >> s & 1)) h = all<V>(0.f);
-        h = fma(av[s], h, bw[s]);
-        if (s < live) store_word<T, ALIGNED>(o, c, a.D, h);
-        o += a.D;
-      }
+        for (int s = 0; s < STEPS; ++s) {
+          if (decltype(restarts)::value && (starts >> s & 1)) h = all<V>(0.f);
+          h = fma(av[s], h, bw[s]);
+          if (s < live) store_word<T, ALIGNED>(o, c, a.D, h);
+          o += a.D;
+        }
+      };
+      if (PACKED && starts) run(std::true_type());
+      else run(std::false_type());
       out += ahead * a.D;
     }
   }
