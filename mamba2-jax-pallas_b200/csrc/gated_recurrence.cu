@@ -427,16 +427,17 @@ struct Rows {
   }
 };
 
+// `channels`: of the lane's, that there are.
 template <typename T, bool ALIGNED>
-__device__ __forceinline__ void store_word(T* o, int64_t c, int64_t D, typename Lane<T>::V v) {
+__device__ __forceinline__ void store_word(T* o, int channels, typename Lane<T>::V v) {
   const uint32_t u = Lane<T>::put(v);
   if constexpr (ALIGNED) {
-    if (c < D) *reinterpret_cast<uint32_t*>(o) = u;
+    if (channels) *reinterpret_cast<uint32_t*>(o) = u;
   } else {
     const T* w = reinterpret_cast<const T*>(&u);
 #pragma unroll
     for (int k = 0; k < Lane<T>::CH; ++k)
-      if (c + k < D) o[k] = w[k];
+      if (k < channels) o[k] = w[k];
   }
 }
 
@@ -496,6 +497,7 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) forward_kernel(
   const Rate<V> rate = rates<T>(a, c, &near);
   V carry = a.state_in ? Lane<T>::load(a.state_in + b * a.D, c, a.D) : all<V>(0.f);
   T* out = static_cast<T*>(a.out[0]) + (b * a.L + first) * a.D + c;
+  const int channels = (int)max((int64_t)0, min((int64_t)CH, a.D - c));
   peers.start();
 
   int64_t t0 = first;
@@ -591,16 +593,17 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) forward_kernel(
       Lane<T>::store(a.states + (b * a.points + t0 / POINT) * a.D, c, a.D, h);
     if (a.out[0]) {
       T* o = out;
-      auto run = [&](auto restarts) {
+      auto run = [&](auto plain) {
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
-          if (decltype(restarts)::value && (starts >> s & 1)) h = all<V>(0.f);
+          if (!decltype(plain)::value && PACKED && (starts >> s & 1)) h = all<V>(0.f);
           h = fma(av[s], h, bw[s]);
-          if (s < live) store_word<T, ALIGNED>(o, c, a.D, h);
+          if (decltype(plain)::value || s < live) store_word<T, ALIGNED>(o, channels, h);
           o += a.D;
         }
       };
-      if (PACKED && starts) run(std::true_type());
+      // the checks of every step (and of c against D beside them) were 9 of its 60 instructions
+      if (live == STEPS && !(PACKED && starts)) run(std::true_type());
       else run(std::false_type());
       out += ahead * a.D;
     }
@@ -648,6 +651,7 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) backward_kernel
   V carry = a.grad_final ? Lane<T>::load(a.grad_final + b * a.D, c, a.D) : all<V>(0.f);
   V total = all<V>(0.f);
   int64_t at = (b * a.L + t0) * a.D + c;
+  const int channels = (int)max((int64_t)0, min((int64_t)CH, a.D - c));
   peers.start();
 
   for (int64_t n = 0; n < turns; ++n, t0 += ahead) {
@@ -748,25 +752,29 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) backward_kernel
         carry = through<PACKED>(own[j * 32], carry);
       }
     }
-    int64_t row = at + (STEPS - 1) * a.D;
+    auto finish = [&](auto whole) {
+      int64_t row = at + (STEPS - 1) * a.D;
 #pragma unroll
-    for (int s = STEPS - 1; s >= 0; --s) {
-      const V x = Lane<T>::get(words[s * 32]), w = mul(si[s], x);
-      V m;
-      if constexpr (CH == 2) m = pack(__uint_as_float(words[(STEPS + s) * 32]), __uint_as_float(words[(2 * STEPS + s) * 32]));
-      else m = __uint_as_float(words[(STEPS + s) * 32]);
-      const V d = add(after, Lane<T>::get(words[(3 * STEPS + s) * 32]));
-      after = mul(av[s], d);
-      if (PACKED && (starts >> s & 1)) after = all<V>(0.f);
-      const V dm = mul(d, m), db = mul(d, bv[s]);
-      total = add(total, dm);
-      if (s < live) {
-        store_word<T, ALIGNED>(static_cast<T*>(a.out[0]) + row, c, a.D, mul(db, si[s]));
-        store_word<T, ALIGNED>(static_cast<T*>(a.out[1]) + row, c, a.D, mul(dm, fma(sr[s], all<V>(-1.f), all<V>(1.f))));
-        store_word<T, ALIGNED>(static_cast<T*>(a.out[2]) + row, c, a.D, mul(mul(db, w), fma(si[s], all<V>(-1.f), all<V>(1.f))));
+      for (int s = STEPS - 1; s >= 0; --s) {
+        const V x = Lane<T>::get(words[s * 32]), w = mul(si[s], x);
+        V m;
+        if constexpr (CH == 2) m = pack(__uint_as_float(words[(STEPS + s) * 32]), __uint_as_float(words[(2 * STEPS + s) * 32]));
+        else m = __uint_as_float(words[(STEPS + s) * 32]);
+        const V d = add(after, Lane<T>::get(words[(3 * STEPS + s) * 32]));
+        after = mul(av[s], d);
+        if (PACKED && (starts >> s & 1)) after = all<V>(0.f);
+        const V dm = mul(d, m), db = mul(d, bv[s]);
+        total = add(total, dm);
+        if (decltype(whole)::value || s < live) {
+          store_word<T, ALIGNED>(static_cast<T*>(a.out[0]) + row, channels, mul(db, si[s]));
+          store_word<T, ALIGNED>(static_cast<T*>(a.out[1]) + row, channels, mul(dm, fma(sr[s], all<V>(-1.f), all<V>(1.f))));
+          store_word<T, ALIGNED>(static_cast<T*>(a.out[2]) + row, channels, mul(mul(db, w), fma(si[s], all<V>(-1.f), all<V>(1.f))));
+        }
+        row -= a.D;
       }
-      row -= a.D;
-    }
+    };
+    if (live == STEPS) finish(std::true_type());
+    else finish(std::false_type());
     at += ahead * a.D;
   }
   // the CTA's sum for the decay, warps in order
