@@ -12,9 +12,9 @@
 //   d decay = sigmoid(decay) / softplus(decay) sum delta m;  dh_0 = c_0
 //
 // Both passes are bound by HBM (8 and 14 bytes per bf16 value), and close behind it by the issue slots and the special-function
-// unit: 36 and 75 instructions and 4 and 5 special functions a value, the gates' above all.  64 x 512 x 5120 bf16: forward 239 us
-// (5.6 TB/s), gradients 482 us (4.9 TB/s).  With few rows and channels the sequence is the only parallelism left: 1 x 32768 x 5120
-// in clusters of 5 forward 342 us (3.9 TB/s), gradients 678 us; 1 x 65536 x 256 111 and 178 us.
+// unit: 32 and 68 instructions and 4 and 5 special functions a value, the gates' above all.  64 x 512 x 5120 bf16: forward 229 us
+// (5.9 TB/s), gradients 454 us (5.2 TB/s).  With few rows and channels the sequence is the only parallelism left: 1 x 32768 x 5120
+// in clusters of 5 forward 325 us (4.1 TB/s), gradients 637 us; 1 x 65536 x 256 111 and 178 us.
 //
 // A step is the map h -> a h + b; maps compose, so a run of steps is one pair (P, H).  Warps take 16
 // steps (8 backward) of 128 bytes of channels (a lane: one 32-bit word, 2 bf16 or 1 f32 channel), CTAs
