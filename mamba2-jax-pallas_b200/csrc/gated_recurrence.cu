@@ -14,7 +14,7 @@
 // Both passes are bound by HBM (8 and 14 bytes per bf16 value), and close behind it by the issue slots and the special-function
 // unit: 32 and 68 instructions and 4 and 5 special functions a value, the gates' above all.  64 x 512 x 5120 bf16: forward 229 us
 // (5.9 TB/s), gradients 454 us (5.2 TB/s).  With few rows and channels the sequence is the only parallelism left: 1 x 32768 x 5120
-// in clusters of 5 forward 325 us (4.1 TB/s), gradients 637 us; 1 x 65536 x 256 111 and 178 us.
+// in clusters of 5 forward 325 us (4.1 TB/s), gradients 636 us; 1 x 65536 x 256 102 and 170 us.
 //
 // A step is the map h -> a h + b; maps compose, so a run of steps is one pair (P, H).  Warps take 16
 // steps (8 backward) of 128 bytes of channels (a lane: one 32-bit word, 2 bf16 or 1 f32 channel), CTAs
@@ -912,9 +912,9 @@ int capacity_of(const Kernel& k, int cluster) {
 
 // Microseconds of `units` clusters: a turn takes `turn`, and `warp` more for each warp that its SM holds, `wide` for each warp of a CTA
 // above 4 (they meet), and in a cluster `exchange` and `peer` for each CTA; a CTA takes `start`.  Fitted to 26 shapes of both types, of
-// 1 to 64 rows, 300 to 65536 tokens and 128 to 8192 channels, each with 1 to 16 CTAs of 4, 8 and 16 warps: what the rule picks is 1.7 %
-// slower than the best on average (11 and 14 % at worst).  Both sides, forward: 64 x 512 x 5120, CTAs of 4 warps alone 239 us, of 8 281,
-// pairs of CTAs 289; 1 x 65536 x 256: alone 1711, clusters of 16 CTAs of 4 warps 170, of 16 warps 111.
+// 1 to 64 rows, 300 to 65536 tokens and 128 to 8192 channels, each with 1 to 16 CTAs of 4, 8 and 16 warps: what the rule picks is 3 %
+// slower than the best on average (14 and 17 % at worst).  Both sides, forward: 64 x 512 x 5120, CTAs of 4 warps alone 228 us, of 8 266,
+// pairs of CTAs 286; 1 x 65536 x 256: alone 1295, clusters of 16 CTAs of 4 warps 135, of 16 warps 102.
 struct Times {
   double turn, warp, exchange, peer, start, wide;
 };
