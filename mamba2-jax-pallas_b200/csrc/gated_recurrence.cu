@@ -352,36 +352,63 @@ struct Args {
   float scale;
 };
 
+// Lanes that hold channels.  Rows that start anywhere are copied from the 16-byte boundary in front of them, so that 128 bytes
+// hold 28 words at any of them (value by value, 1 x 64078 x 7927 took 4235 us in place of 1487).
+constexpr int lanes_of(bool aligned) { return aligned ? 32 : 28; }
+
 // A warp's rows of N tensors, 128 bytes each, into its part of a stage; zeros beyond the sequence and beyond the channels.
 template <typename T, int N, int STEPS, int WARPS, bool ALIGNED>
 struct Rows {
-  static constexpr int WARP_BYTES = N * STEPS * 128, STAGE = WARPS * WARP_BYTES;
-  const uint8_t* at[N];            // the lane's first row and 16 bytes of the next turn
+  static constexpr int WARP_BYTES = N * STEPS * 128, STAGE = WARPS * WARP_BYTES, LANES = ALIGNED ? 32 : 28;
+  const uint8_t* at[N];            // the lane's first row of the next turn, and where ALIGNED its 16 bytes there
   uint8_t* smem;                   // the warp's part of stage 0
-  int bytes;                       // 16, or 0 beyond the channels
+  int bytes;                       // ALIGNED: 16, or 0 beyond the channels; else of the group's channels
   int64_t t0;                      // of the next turn
+  uint32_t low[N], step[N];        // not ALIGNED: addresses of the present turn's first row and from row to row, of which four bits count
 
   __device__ __forceinline__ Rows(const Args& a, uint8_t* stages, int64_t b, int64_t c0, int64_t first) {
     const int lane = threadIdx.x & 31;
     smem = stages + (threadIdx.x >> 5) * WARP_BYTES;
     t0 = first;
-    const int64_t c = c0 + lane % 8 * (16 / (int)sizeof(T));
-    bytes = ALIGNED && c < a.D ? 16 : 0;
+    const int64_t c = ALIGNED ? c0 + lane % 8 * (16 / (int)sizeof(T)) : c0;
+    if constexpr (ALIGNED) bytes = c < a.D ? 16 : 0;
+    else bytes = (int)(min((int64_t)(LANES * Lane<T>::CH), a.D - c0) * (int)sizeof(T));
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const T* p = static_cast<const T*>(a.in[i].p) + b * a.in[i].stride_b;
-      if (ALIGNED) p += (first + lane / 8) * a.in[i].stride_t + (bytes ? c : 0);
+      const T* p = static_cast<const T*>(a.in[i].p) + b * a.in[i].stride_b + (first + lane / 8) * a.in[i].stride_t + (bytes ? c : 0);
       at[i] = reinterpret_cast<const uint8_t*>(p);
+      if constexpr (!ALIGNED) {
+        step[i] = (uint32_t)(a.in[i].stride_t * (int64_t)sizeof(T));
+        low[i] = (uint32_t)reinterpret_cast<uintptr_t>(p) - (uint32_t)(lane / 8) * step[i];
+      }
     }
   }
   __device__ __forceinline__ uint8_t* row(int stage, int i, int s) { return smem + stage * STAGE + (i * STEPS + s) * 128; }
   __device__ __forceinline__ const uint32_t* words(int stage) { return reinterpret_cast<const uint32_t*>(smem + stage * STAGE) + (threadIdx.x & 31); }
+  // The lane's channels of tensor i in step s; `words` is of this turn's stage.
+  __device__ __forceinline__ uint32_t word(const uint32_t* words, int i, int s) const {
+    if constexpr (ALIGNED) {
+      return words[(i * STEPS + s) * 32];
+    } else {
+      const int lane = threadIdx.x & 31;
+      const uint32_t shift = low[i] + (uint32_t)s * step[i];
+      const uint32_t* w = words + (i * STEPS + s) * 32 + ((int)(shift >> 2 & 3) + min(lane, LANES - 1) - lane);
+      return sizeof(T) == 2 ? __funnelshift_r(w[0], w[1], shift << 3 & 16) : w[0];
+    }
+  }
+  // The turn is over: `ahead` tokens on.
+  __device__ __forceinline__ void turn(int64_t ahead) {
+    if constexpr (!ALIGNED) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) low[i] += (uint32_t)ahead * step[i];
+    }
+  }
 
   // `ahead`: tokens from this turn to the next
-  __device__ __forceinline__ void load(const Args& a, int stage, int64_t c0, int64_t ahead) {
+  __device__ __forceinline__ void load(const Args& a, int stage, int64_t ahead) {
     const int lane = threadIdx.x & 31;
+    const uint32_t dst = ptx::smem_u32(row(stage, 0, lane / 8)) + lane % 8 * 16;
     if constexpr (ALIGNED) {
-      const uint32_t dst = ptx::smem_u32(row(stage, 0, lane / 8)) + lane % 8 * 16;
       if (t0 + STEPS <= a.L) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -401,21 +428,20 @@ struct Rows {
           at[i] += ahead * a.in[i].stride_t * (int64_t)sizeof(T);
         }
       }
-    } else {   // rows that do not start at 16 bytes: value by value
-      constexpr int CH = Lane<T>::CH;
-      const int64_t c = c0 + lane * CH;
+    } else {
+      // Nothing is read behind the row's channels.  In front of them up to 14 bytes are, which lie in the same 16 bytes as the
+      // first channel and so in its allocation.
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const T* p = reinterpret_cast<const T*>(at[i]);
-        T v[STEPS][CH];
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-          for (int k = 0; k < CH; ++k) v[s][k] = t0 + s < a.L && c + k < a.D ? p[(t0 + s) * a.in[i].stride_t + c + k] : T(0.f);
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-          for (int k = 0; k < CH; ++k) reinterpret_cast<T*>(row(stage, i, s))[lane * CH + k] = v[s][k];
+        for (int j = 0; j < STEPS / 4; ++j) {
+          const uint8_t* p = at[i] + j * (4 * (int64_t)sizeof(T)) * a.in[i].stride_t;
+          const int in = (int)(reinterpret_cast<uintptr_t>(p) & 15), left = in + bytes - lane % 8 * 16;
+          const bool there = t0 + lane / 8 + 4 * j < a.L && left > 0;
+          cp16(dst + (i * STEPS + 4 * j) * 128, there ? p - in + lane % 8 * 16 : reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(a.in[i].p) & ~uintptr_t(15)),
+               there ? min(left, 16) : 0);
+        }
+        at[i] += ahead * a.in[i].stride_t * (int64_t)sizeof(T);
       }
     }
     t0 += ahead;
@@ -424,6 +450,7 @@ struct Rows {
   __device__ __forceinline__ void close(int stage, int live) {
     const uint32_t shut = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
     for (int s = live; s < STEPS; ++s) reinterpret_cast<uint32_t*>(row(stage, 1, s))[threadIdx.x & 31] = shut;
+    if (!ALIGNED) __syncwarp();
   }
 };
 
@@ -483,13 +510,14 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) forward_kernel(
   __shared__ uint64_t bars[2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = cluster > 1 ? (int)cluster_rank() : 0;
-  const int64_t unit = blockIdx.x / (unsigned)cluster, b = unit / a.groups, c0 = (unit - b * a.groups) * (32 * CH), c = c0 + lane * CH;
+  const int64_t unit = blockIdx.x / (unsigned)cluster, b = unit / a.groups, c0 = (unit - b * a.groups) * (In::LANES * CH);
+  const int64_t c = lane < In::LANES ? c0 + lane * CH : a.D;
   Map* const maps = reinterpret_cast<Map*>(smem + 2 * In::STAGE);   // [2][WARPS][32]
   Peers<T, WARPS> peers{maps + 2 * WARPS * 32, bars, cluster, rank, a.status, false};
   const int64_t tiles = (a.L + TILE - 1) / TILE, turns = (tiles + cluster - 1) / cluster, ahead = (int64_t)cluster * TILE;
   const int64_t first = (int64_t)rank * TILE + warp * STEPS;
   In in(a, smem, b, c0, first);
-  in.load(a, 0, c0, ahead);
+  in.load(a, 0, ahead);
   cp_commit();
   const int* seq = PACKED ? a.seq_idx + b * a.L : nullptr;
   int ids = PACKED ? load_ids<STEPS>(seq, first, a.L) : 0;
@@ -504,7 +532,7 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) forward_kernel(
   for (int64_t n = 0; n < turns; ++n, t0 += ahead) {
     const int stage = (int)(n & 1);
     const int live = (int)max((int64_t)0, min((int64_t)STEPS, a.L - t0));
-    if (n + 1 < turns) in.load(a, stage ^ 1, c0, ahead);
+    if (n + 1 < turns) in.load(a, stage ^ 1, ahead);
     cp_commit();
     unsigned starts = 0;
     if constexpr (PACKED) {
@@ -520,8 +548,8 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) forward_kernel(
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
         V sr, l, b;
-        decay_of<decltype(is_near)::value>(Lane<T>::get(words[(STEPS + s) * 32]), rate, &sr, &l, &av[s], &b);
-        bw[s] = mul(b, mul(sigmoid(Lane<T>::get(words[(2 * STEPS + s) * 32])), Lane<T>::get(words[s * 32])));
+        decay_of<decltype(is_near)::value>(Lane<T>::get(in.word(words, 1, s)), rate, &sr, &l, &av[s], &b);
+        bw[s] = mul(b, mul(sigmoid(Lane<T>::get(in.word(words, 2, s))), Lane<T>::get(in.word(words, 0, s))));
         P = mul(P, av[s]);
         H = fma(av[s], H, bw[s]);
       }
@@ -607,6 +635,7 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) forward_kernel(
       else run(std::false_type());
       out += ahead * a.D;
     }
+    in.turn(ahead);
   }
   if (a.state_out && rank == 0 && warp == 0) Lane<T>::store(a.state_out + b * a.D, c, a.D, carry);
   peers.end();
@@ -632,12 +661,13 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) backward_kernel
   V* const ends = reinterpret_cast<V*>(maps + 2 * 32 * (WARPS + (cluster > 1 ? cluster : 0)));   // H [2][WARPS][32]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = cluster > 1 ? (int)cluster_rank() : 0;
-  const int64_t unit = blockIdx.x / (unsigned)cluster, b = unit / a.groups, c0 = (unit - b * a.groups) * (32 * CH), c = c0 + lane * CH;
+  const int64_t unit = blockIdx.x / (unsigned)cluster, b = unit / a.groups, c0 = (unit - b * a.groups) * (In::LANES * CH);
+  const int64_t c = lane < In::LANES ? c0 + lane * CH : a.D;
   Peers<T, WARPS> peers{maps + 2 * WARPS * 32, bars, cluster, rank, a.status, false};
   const int64_t tiles = (a.L + TILE - 1) / TILE, turns = (tiles + cluster - 1) / cluster, ahead = -(int64_t)cluster * TILE;
   int64_t t0 = ((turns - 1) * cluster + rank) * TILE + warp * STEPS;
   In in(a, smem, b, c0, t0);
-  in.load(a, 0, c0, ahead);
+  in.load(a, 0, ahead);
   cp_commit();
   const int* seq = PACKED ? a.seq_idx + b * a.L : nullptr;
   int ids = PACKED ? load_ids<STEPS>(seq, t0, a.L) : 0;
@@ -658,7 +688,7 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) backward_kernel
     const int stage = (int)(n & 1);
     const int live = (int)max((int64_t)0, min((int64_t)STEPS, a.L - t0));
     __syncwarp();          // the other lanes have read the stage that is loaded next
-    if (n + 1 < turns) in.load(a, stage ^ 1, c0, ahead);
+    if (n + 1 < turns) in.load(a, stage ^ 1, ahead);
     cp_commit();
     V h = state;
     state = state_before(t0 + ahead);
@@ -676,18 +706,18 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) backward_kernel
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
         V l;
-        decay_of<decltype(is_near)::value>(Lane<T>::get(words[(STEPS + s) * 32]), rate, &sr[s], &l, &av[s], &bv[s]);
-        si[s] = sigmoid(Lane<T>::get(words[(2 * STEPS + s) * 32]));
+        decay_of<decltype(is_near)::value>(Lane<T>::get(in.word(words, 1, s)), rate, &sr[s], &l, &av[s], &bv[s]);
+        si[s] = sigmoid(Lane<T>::get(in.word(words, 2, s)));
         P = mul(P, av[s]);
         if (PACKED && (starts >> s & 1)) H = all<V>(0.f);
-        H = fma(av[s], H, mul(bv[s], mul(si[s], Lane<T>::get(words[s * 32]))));
+        H = fma(av[s], H, mul(bv[s], mul(si[s], Lane<T>::get(in.word(words, 0, s)))));
       }
     };
     if (near) gates(std::true_type());
     else gates(std::false_type());
 #pragma unroll
     for (int s = STEPS - 1; s >= 0; --s) {
-      R = mul(av[s], add(R, Lane<T>::get(words[(3 * STEPS + s) * 32])));
+      R = mul(av[s], add(R, Lane<T>::get(in.word(words, 3, s))));
       if (PACKED && (starts >> s & 1)) R = all<V>(0.f);
     }
     Map* const own = maps + (stage * WARPS) * 32 + lane;
@@ -715,7 +745,7 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) backward_kernel
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
       if (PACKED && (starts >> s & 1)) h = all<V>(0.f);
-      const V w = mul(si[s], Lane<T>::get(words[s * 32]));
+      const V w = mul(si[s], Lane<T>::get(in.word(words, 0, s)));
       const V inverse = each(bv[s], [](float t) { return t == 0.f ? 0.f : -rcp(t); });
       const V m = mul(mul(mul(sr[s], nkl), av[s]), fma(mul(av[s], inverse), w, h));
       if constexpr (CH == 2) {
@@ -756,11 +786,11 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) backward_kernel
       int64_t row = at + (STEPS - 1) * a.D;
 #pragma unroll
       for (int s = STEPS - 1; s >= 0; --s) {
-        const V x = Lane<T>::get(words[s * 32]), w = mul(si[s], x);
+        const V x = Lane<T>::get(in.word(words, 0, s)), w = mul(si[s], x);
         V m;
         if constexpr (CH == 2) m = pack(__uint_as_float(words[(STEPS + s) * 32]), __uint_as_float(words[(2 * STEPS + s) * 32]));
         else m = __uint_as_float(words[(STEPS + s) * 32]);
-        const V d = add(after, Lane<T>::get(words[(3 * STEPS + s) * 32]));
+        const V d = add(after, Lane<T>::get(in.word(words, 3, s)));
         after = mul(av[s], d);
         if (PACKED && (starts >> s & 1)) after = all<V>(0.f);
         const V dm = mul(d, m), db = mul(d, bv[s]);
@@ -776,6 +806,7 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) backward_kernel
     if (live == STEPS) finish(std::true_type());
     else finish(std::false_type());
     at += ahead * a.D;
+    in.turn(ahead);
   }
   // the CTA's sum for the decay, warps in order
   __syncthreads();
@@ -1022,7 +1053,6 @@ Args args_of(const ssd_gated_recurrence_params_t* p) {
   a.L = p->seqlen;
   a.D = p->dim;
   a.points = cdiv(p->seqlen, POINT);
-  a.groups = cdiv(p->dim, 128 / value_bytes(p->dtype));
   a.scale = p->scale;
   a.status = p->status;
   return a;
@@ -1038,8 +1068,9 @@ bool all_aligned(const ssd_gated_recurrence_params_t* p, const Args& a, int inpu
 
 size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 
-// The kernels of a call, on the current device, and which of them.
-cudaError_t choose(const ssd_gated_recurrence_params_t* p, const Args& a, bool backward, bool aligned, Kernels* ks, Choice* c) {
+// The kernels of a call, on the current device, and which of them; the groups that its channels make.
+cudaError_t choose(const ssd_gated_recurrence_params_t* p, Args& a, bool backward, bool aligned, Kernels* ks, Choice* c) {
+  a.groups = cdiv(p->dim, 4 / value_bytes(p->dtype) * lanes_of(aligned));
   const bool bf = p->dtype == SSD_DTYPE_BF16, packed = a.seq_idx != nullptr;
   if (backward) *ks = bf ? backward_kernels<bf16>(aligned, packed) : backward_kernels<float>(aligned, packed);
   else *ks = bf ? forward_kernels<bf16>(aligned, packed) : forward_kernels<float>(aligned, packed);

@@ -277,6 +277,39 @@ def test_strides_and_broadcasts(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("packed", [False, True])
+def test_rows_that_start_anywhere(dtype, packed):
+    """Views of buffers that hold NaN around them, every start of a row within 16 bytes, one and several groups of channels."""
+    b, L = 2, 83
+    for d in (1, 27, 57, 113):
+        x, r, i, lam, h0, dy, df = inputs(b, L, d, seed=d)
+        seq = torch.tensor([0] * 5 + [1] + [2] * 30 + [3] * 47, dtype=torch.int32).expand(b, L).contiguous() if packed else None
+        data = [t.to(DT[dtype]) for t in (x, r, i, dy)]
+        n = 22 * E + lives(lam) * U
+        close(gated_recurrence(*cuda(*data[:3], lam), initial_state=h0.cuda(), seq_idx=cuda(seq)[0]),
+              loop(*data[:3], lam, h0, seq)[0], n * magnitude(*data[:3], lam, h0, seq, 8.0)[0], dtype)
+        kw = dict(initial_state=h0.cuda(), seq_idx=cuda(seq)[0])
+        whole = cuda(*data)
+        y, final, points = gated_recurrence(*whole[:3], lam.cuda(), return_final_state=True, return_checkpoints=True, **kw)
+        grads = gated_recurrence_grad(*whole[:3], lam.cuda(), whole[3], grad_final_state=df.cuda(), checkpoints=points, **kw)
+        refs, sizes = loop_grad(*data[:3], lam, h0, data[3], df, seq)
+        for k, q in enumerate(grads):
+            close(q, refs[k], 8 * n * sizes[k], dtype if k < 3 else "f32", norm=k < 3)
+        for at in range(9):
+            views = []
+            for k, t in enumerate(whole):
+                wide = torch.full((b, L, d + 16 + k), float("nan"), dtype=DT[dtype], device="cuda")
+                view = wide[..., (at + 3 * k) % 9:][..., :d]
+                view.copy_(t)
+                views.append(view)
+            for p, q in zip(gated_recurrence(*views[:3], lam.cuda(), return_final_state=True, return_checkpoints=True, **kw), (y, final, points)):
+                assert torch.equal(p, q), (d, at)
+            for p, q in zip(gated_recurrence_grad(*views[:3], lam.cuda(), views[3], grad_final_state=df.cuda(), checkpoints=points, **kw), grads):
+                assert torch.equal(p, q), (d, at)
+
+
+@gpu
 @pytest.mark.parametrize("b,L,d", [(1, 777, 64), (64, 70, 64), (1, 4000, 2048), (7, 300, 5000)])
 def test_cluster_sizes_agree_with_halves(b, L, d):
     """A sequence in two calls, the state carried between them: other clusters, other tiles."""
