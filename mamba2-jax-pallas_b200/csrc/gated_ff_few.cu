@@ -6,6 +6,7 @@
 // L1.  One or two CTAs per SM walk over the rows; every lane copies its own 16 bytes of the weights some steps ahead, across the
 // ends of the rows, into slots of shared memory that no other lane reads: 96 KB in flight per SM.  Bound by HBM and the two
 // launches' ends: 1 token of 4096 x 12288 bf16 56.5 us (5.3 TB/s), of 2560 x 7680 f32 41 us (5.8 TB/s), of 768 x 2048 6 us.
+// Rows that start at no 16-byte boundary: 1 token of 4095 x 12287 bf16 89 us, 4 tokens 147 (value by value 144 and 284).
 #include <algorithm>
 
 #include "common.cuh"
@@ -116,10 +117,27 @@ __device__ __forceinline__ void before_weights(const FewArgs& a) {
   }
 }
 
+// 16 bytes that start `shift` bytes into `own`, behind which `next` lies.  (The shift is the same for the warp.)
+__device__ __forceinline__ uint4 window(const uint4& own, const uint4& next, unsigned shift) {
+  uint32_t w[8] = {own.x, own.y, own.z, own.w, next.x, next.y, next.z, next.w};
+#pragma unroll
+  for (int k = 0; k < 7; ++k) w[k] = shift & 4 ? w[k + 1] : w[k];
+#pragma unroll
+  for (int k = 0; k < 5; ++k) w[k] = shift & 8 ? w[k + 2] : w[k];
+  const unsigned half = shift << 3 & 16;
+  return make_uint4(__funnelshift_r(w[0], w[1], half), __funnelshift_r(w[1], w[2], half), __funnelshift_r(w[2], w[3], half),
+                    __funnelshift_r(w[3], w[4], half));
+}
+
+// Columns of a warp's step: every lane's 16 bytes.  Rows that do not start at 16 bytes are copied from the boundary in front, and a lane's
+// columns lie in its own piece and the next lane's, so that the last lane has none.
+template <typename T>
+constexpr int step_columns(bool aligned) { return (aligned ? 32 : 31) * Piece<T>::N; }
+
 // R tokens; a warp's rows: ROWS of each of W weights.
-template <typename T, int R, int ROWS, int W>
+template <typename T, int R, int ROWS, int W, bool ALIGNED>
 __global__ void __launch_bounds__(32 * WARPS, Shape<R * ROWS * W>::CTAS) few_kernel(const __grid_constant__ FewArgs a) {
-  constexpr int N = R * ROWS * W, NR = W * ROWS, SLOTS = Shape<N>::SLOTS, STAGES = SLOTS / NR, STEP = 32 * Piece<T>::N;
+  constexpr int N = R * ROWS * W, NR = W * ROWS, SLOTS = Shape<N>::SLOTS, STAGES = SLOTS / NR, STEP = (ALIGNED ? 32 : 31) * Piece<T>::N;
   extern __shared__ __align__(16) uint4 ring[];          // [WARPS][SLOTS][32]
   __shared__ float sh[2][WARPS][N];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -140,11 +158,19 @@ __global__ void __launch_bounds__(32 * WARPS, Shape<R * ROWS * W>::CTAS) few_ker
   rows_of();
   auto copy = [&]() {
     if (next < all) {
-      const int c = (at * 32 + lane) * Piece<T>::N;
+      const int c = at * STEP + lane * Piece<T>::N;
 #pragma unroll
-      for (int i = 0; i < NR; ++i)   // columns past the end are zeros
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(mine + (to * NR + i) * 32)), "l"(c < a.K ? row[i] + c : row[i]),
-                     "r"(c < a.K ? 16 : 0) : "memory");
+      for (int i = 0; i < NR; ++i) {   // columns past the end are zeros
+        const uint8_t* p = reinterpret_cast<const uint8_t*>(row[i]);
+        int left = min(a.K - c, 32) * (int)sizeof(T);
+        if constexpr (!ALIGNED) {      // (what lies in front of the row in its first 16 bytes is in its allocation)
+          const int in = (int)(reinterpret_cast<uintptr_t>(p) & 15);
+          p -= in;
+          left += in;
+        }
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(mine + (to * NR + i) * 32)),
+                     "l"(left > 0 ? p + (int64_t)c * sizeof(T) : p), "r"(max(0, min(left, 16))) : "memory");
+      }
       if (++at == s1) {
         at = s0;
         next += stride;
@@ -162,28 +188,57 @@ __global__ void __launch_bounds__(32 * WARPS, Shape<R * ROWS * W>::CTAS) few_ker
   // one load of each 128 bytes of x, all at once: found missing step by step, they would cost the first rows a trip to L2 each
   for (int t = 0; t < tokens; ++t)
     for (int c = threadIdx.x * (128 / (int)sizeof(T)); c < a.K; c += 32 * WARPS * (128 / (int)sizeof(T))) {
-      uint32_t unused;
-      asm volatile("ld.global.ca.b32 %0, [%1];" : "=r"(unused) : "l"(x + t * a.xs + c));
+      if constexpr (ALIGNED) {
+        uint32_t unused;
+        asm volatile("ld.global.ca.b32 %0, [%1];" : "=r"(unused) : "l"(x + t * a.xs + c));
+      } else {
+        unsigned short unused;
+        asm volatile("ld.global.ca.b16 %0, [%1];" : "=h"(unused) : "l"(x + t * a.xs + c));
+      }
     }
   int from = 0, turn = 0;
   for (int64_t first = (int64_t)blockIdx.x * groups; first < all; first += stride, turn ^= 1) {
     float sum[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) sum[i] = 0.f;
+    unsigned shift[NR];    // not ALIGNED: of the rows' starts
+    if constexpr (!ALIGNED) {
+#pragma unroll
+      for (int i = 0; i < NR; ++i)
+        shift[i] = (unsigned)reinterpret_cast<uintptr_t>(static_cast<const T*>(a.w[i % W]) + min((first + warp / a.parts) * ROWS + i / W, a.rows - 1) * a.ws[i % W]) & 15;
+    }
     for (int s = s0; s < s1; ++s) {
-      const int c = (s * 32 + lane) * Piece<T>::N;
+      const int c = s * STEP + lane * Piece<T>::N;
       Piece<T> v[R], w[NR];
 #pragma unroll
       for (int t = 0; t < R; ++t) {
         v[t].q = make_uint4(0, 0, 0, 0);
-        if (c < a.K) v[t].q = *reinterpret_cast<const uint4*>(x + min(t, tokens - 1) * a.xs + c);
+        const T* xt = x + min(t, tokens - 1) * a.xs + c;
+        if constexpr (ALIGNED) {
+          if (c < a.K) v[t].q = *reinterpret_cast<const uint4*>(xt);
+        } else if (c + 2 * Piece<T>::N <= a.K) {   // by the 16 bytes that hold them, which end within the row
+          const unsigned in = (unsigned)reinterpret_cast<uintptr_t>(xt) & 15;
+          const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(xt) - in);
+          const uint4 own = q[0];
+          v[t].q = in ? window(own, q[1], in) : own;
+        } else if (lane < 31) {
+          alignas(16) T u[Piece<T>::N];
+#pragma unroll
+          for (int k = 0; k < Piece<T>::N; ++k) u[k] = c + k < a.K ? xt[k] : T(0.f);
+          v[t].q = *reinterpret_cast<const uint4*>(u);
+        }
       }
+      if constexpr (!ALIGNED) __syncwarp();   // the lane in front has read what is copied over
       copy();
       asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+      if constexpr (!ALIGNED) __syncwarp();
 #pragma unroll
-      for (int i = 0; i < NR; ++i) w[i].q = mine[(from * NR + i) * 32];
+      for (int i = 0; i < NR; ++i) {
+        w[i].q = mine[(from * NR + i) * 32];
+        if constexpr (!ALIGNED) w[i].q = window(w[i].q, mine[(from * NR + i) * 32 + (lane < 31)], shift[i]);
+      }
       if (++from == STAGES) from = 0;
-      accumulate<T, R, NR>(sum, v, w);
+      if (ALIGNED || lane < 31) accumulate<T, R, NR>(sum, v, w);
     }
     const float total = warp_sums<N>(sum);
     if (lane < N) sh[turn][warp][lane] = total;
@@ -193,59 +248,11 @@ __global__ void __launch_bounds__(32 * WARPS, Shape<R * ROWS * W>::CTAS) few_ker
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// The same where rows do not start at 16 bytes: value by value.
-template <typename T, int R, int ROWS, int W>
-__global__ void __launch_bounds__(256) few_odd_kernel(const __grid_constant__ FewArgs a) {
-  constexpr int N = R * ROWS * W, NR = W * ROWS, STEP = 32 * Piece<T>::N;
-  __shared__ float sh[8][N];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int part = warp % a.parts, groups = 8 / a.parts;
-  const int64_t first = (int64_t)blockIdx.x * groups, r0 = (first + warp / a.parts) * ROWS;
-  const int steps = (a.K + STEP - 1) / STEP, s0 = steps * part / a.parts, s1 = steps * (part + 1) / a.parts;
-  before_weights<W>(a);
-  if constexpr (W == 1) ptx::griddep_wait();
-  const T* row[NR];
-#pragma unroll
-  for (int i = 0; i < NR; ++i) row[i] = static_cast<const T*>(a.w[i % W]) + min(r0 + i / W, a.rows - 1) * a.ws[i % W];
-  const int tokens = min(R, a.tokens - (int)blockIdx.y * R);
-  const T* x = static_cast<const T*>(a.x) + (int64_t)blockIdx.y * R * a.xs;
-  float sum[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) sum[i] = 0.f;
-  for (int s = s0; s < s1; ++s) {   // a lane's values are 32 columns apart
-    float w[Piece<T>::N][NR];
-#pragma unroll
-    for (int j = 0; j < Piece<T>::N; ++j) {
-      const int c = s * STEP + j * 32 + lane;
-#pragma unroll
-      for (int i = 0; i < NR; ++i) w[j][i] = c < a.K ? ld(row[i] + c) : 0.f;
-    }
-#pragma unroll
-    for (int t = 0; t < R; ++t)
-#pragma unroll
-      for (int j = 0; j < Piece<T>::N; ++j) {
-        const int c = s * STEP + j * 32 + lane;
-        const float v = c < a.K ? ld(x + min(t, tokens - 1) * a.xs + c) : 0.f;
-#pragma unroll
-        for (int i = 0; i < NR; ++i) sum[t * NR + i] = fmaf(v, w[j][i], sum[t * NR + i]);
-      }
-  }
-  const float total = warp_sums<N>(sum);
-  if (lane < N) sh[warp][lane] = total;
-  __syncthreads();
-  finish<T, R, ROWS, W>(a, sh, groups, first);
-}
-
-template <typename T, int R, int ROWS, int W>
-cudaError_t launch_rows(FewArgs a, bool aligned, cudaStream_t st) {
+template <typename T, int R, int ROWS, int W, bool ALIGNED>
+cudaError_t launch_rows(FewArgs a, cudaStream_t st) {
   const int64_t groups = (a.rows + ROWS - 1) / ROWS;
   const unsigned passes = (unsigned)((a.tokens + R - 1) / R);
-  const int steps = (a.K + 32 * Piece<T>::N - 1) / (32 * Piece<T>::N);
-  if (!aligned) {          // parts of a row: as many as fill the GPU
-    a.parts = 1;
-    while (a.parts < 8 && groups * a.parts < SMS * 24 && steps >= a.parts * 2) a.parts *= 2;
-    return launch_dependent(few_odd_kernel<T, R, ROWS, W>, dim3((unsigned)((groups * a.parts + 7) / 8), passes), 256, 0, 1, st, a);
-  }
+  const int steps = (a.K + step_columns<T>(ALIGNED) - 1) / step_columns<T>(ALIGNED);
   // parts of a row: the fewest steps of a warp; a turn's sums and meeting count as half a step
   using S = Shape<R * ROWS * W>;
   const int64_t slots = (int64_t)SMS * S::CTAS * WARPS;
@@ -262,18 +269,22 @@ cudaError_t launch_rows(FewArgs a, bool aligned, cudaStream_t st) {
   a.parts = best;
   static std::atomic<uint64_t> allowed{0};
   constexpr int smem = WARPS * S::SLOTS * 512;
-  const cudaError_t e = allow_smem((const void*)few_kernel<T, R, ROWS, W>, smem, &allowed);
+  const cudaError_t e = allow_smem((const void*)few_kernel<T, R, ROWS, W, ALIGNED>, smem, &allowed);
   if (e != cudaSuccess) return e;
   const int64_t ctas = std::min<int64_t>(SMS * S::CTAS, (groups * best + WARPS - 1) / WARPS);
-  return launch_dependent(few_kernel<T, R, ROWS, W>, dim3((unsigned)ctas, passes), 32 * WARPS, smem, 1, st, a);
+  return launch_dependent(few_kernel<T, R, ROWS, W, ALIGNED>, dim3((unsigned)ctas, passes), 32 * WARPS, smem, 1, st, a);
 }
 
+template <typename T, int W, bool ALIGNED>
+cudaError_t launch_tokens(const FewArgs& a, cudaStream_t st) {
+  if (a.tokens == 1) return launch_rows<T, 1, 1, W, ALIGNED>(a, st);
+  if (a.tokens == 2) return launch_rows<T, 2, 2, W, ALIGNED>(a, st);
+  if (a.tokens <= 4) return launch_rows<T, 4, 2, W, ALIGNED>(a, st);
+  return launch_rows<T, 8, 2, W, ALIGNED>(a, st);   // 8 at a time
+}
 template <typename T, int W>
 cudaError_t launch_tokens(const FewArgs& a, bool aligned, cudaStream_t st) {
-  if (a.tokens == 1) return launch_rows<T, 1, 1, W>(a, aligned, st);
-  if (a.tokens == 2) return launch_rows<T, 2, 2, W>(a, aligned, st);
-  if (a.tokens <= 4) return launch_rows<T, 4, 2, W>(a, aligned, st);
-  return launch_rows<T, 8, 2, W>(a, aligned, st);   // 8 at a time
+  return aligned ? launch_tokens<T, W, true>(a, st) : launch_tokens<T, W, false>(a, st);
 }
 
 size_t up256(size_t v) { return (v + 255) & ~size_t(255); }

@@ -205,6 +205,24 @@ def test_strides(t, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("t", [1, 3, 9])
+def test_rows_that_start_anywhere(t, dtype):
+    """Few tokens: views of buffers that hold NaN around them, at every start of a row within 16 bytes; rows of several steps of a warp."""
+    d, f, o = 777, 251, 21
+    ins = inputs(t, d, f, o, dtype, 3)
+    refs, _ = reference(*ins, "silu", dtype)
+    for at in range(9):
+        views = []
+        for k, a in enumerate(ins[:4]):
+            wide = torch.full((a.shape[0], a.shape[1] + 16 + k), float("nan"), dtype=DT[dtype], device="cuda")
+            view = wide[:, (at + 3 * k) % 9:][:, :a.shape[1]]
+            view.copy_(a)
+            views.append(view)
+        close(gated_feed_forward(*views), *refs[0], dtype)
+
+
+@gpu
 @pytest.mark.parametrize("t,d,f,o", [(300, 4096, 64, 64), (64, 64, 4096, 64), (1000, 64, 64, 64), (16, 8, 2000, 8), (5000, 24, 16, 8)])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_long_reductions(t, d, f, o, dtype):
