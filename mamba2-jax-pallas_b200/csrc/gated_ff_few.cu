@@ -326,8 +326,12 @@ cudaError_t launch_as(const ssd_gated_ff_params_t* p, uint8_t* ws, cudaStream_t 
 }  // namespace
 
 // bf16: up to 4 tokens (2560 x 7680: 4 tokens 37 us, by the products 42; 8 tokens 63 and 42).  f32: up to 24, 8 at a time (8 tokens 80
-// us, 16 160, by the products 252: their operands have to be split first).
-bool gated_ff_is_few(const ssd_gated_ff_params_t* p) { return p->tokens <= (p->dtype == SSD_DTYPE_BF16 ? 4 : 24); }
+// us, 16 143, 24 207, by the products 252: their operands have to be split first); where rows start off 16 bytes, and the shifting of
+// every pass costs more than the weights' bytes, up to 8 (2559 x 7681: 16 tokens 323, by the products 259).
+bool gated_ff_is_few(const ssd_gated_ff_params_t* p) {
+  if (p->dtype == SSD_DTYPE_BF16) return p->tokens <= 4;
+  return p->tokens <= (p->w_gate_stride_row % 4 || p->w_up_stride_row % 4 || p->w_down_stride_row % 4 ? 8 : 24);
+}
 
 size_t gated_ff_few_workspace(const ssd_gated_ff_params_t* p) { return 256 + up256((size_t)p->tokens * ((p->hidden + 7) / 8 * 8) * 4); }
 
