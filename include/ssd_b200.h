@@ -516,7 +516,7 @@ typedef enum ssd_activation {
  * bf16: products on the tensor cores with f32 accumulation; h (and in the gradients those of the two
  * projections) is rounded once to bf16, as an operand of the products behind it.  f32: every operand as three
  * bf16 terms, six products per pair, with the accuracy of f32 (values below 2^-110 lose digits).  For a few tokens (bf16: 4, f32: 24) the
- * forward products run in f32 on the CUDA cores. */
+ * forward products run in f32 on the CUDA cores, and h stays f32. */
 typedef struct ssd_gated_ff_params {
   int64_t tokens, dim, hidden, dim_out;
   int64_t x_stride_row, w_gate_stride_row, w_up_stride_row, w_down_stride_row; /* in values, at least a row's length */

@@ -3,10 +3,12 @@
 //
 // The products run in f32 on the CUDA cores, straight from the weights as they lie in memory.  A warp takes
 // some rows of a weight (for g and u the same row of both), or a part of their columns, against all tokens' values, which stay in
-// L1.  One or two CTAs per SM walk over the rows; every lane copies its own 16 bytes of the weights some steps ahead, across the
-// ends of the rows, into slots of shared memory that no other lane reads: 96 KB in flight per SM.  Bound by HBM and the two
-// launches' ends: 1 token of 4096 x 12288 bf16 56.5 us (5.3 TB/s), of 2560 x 7680 f32 41 us (5.8 TB/s), of 768 x 2048 6 us.
-// Rows that start at no 16-byte boundary: 1 token of 4095 x 12287 bf16 89 us, 4 tokens 147 (value by value 144 and 284).
+// L1.  The hidden values between the two launches stay f32: nothing here needs bf16 operands (rounded to bf16 they would double the
+// square of the result's error, 0.0024 against 0.0017).  One or two CTAs per SM walk over the rows; every lane copies its own 16
+// bytes of the weights some steps ahead, across the ends of the rows, into slots of shared memory that no other lane reads: 96 KB in
+// flight per SM.  Bound by HBM and the two launches' ends: 1 token of 4096 x 12288 bf16 59.5 us (5.1 TB/s), 4 tokens 72, 1 token of
+// 2560 x 7680 f32 43.6 us (5.4 TB/s), of 768 x 2048 bf16 6.1 us.  Rows that start at no 16-byte boundary: 1 token of 4095 x 12287
+// bf16 95 us, 4 tokens 134 (value by value 144 and 284).
 #include <algorithm>
 
 #include "common.cuh"
@@ -28,9 +30,9 @@ struct Shape {
 constexpr int SMS = 148;   // of a B200
 
 struct FewArgs {
-  const void* x;                   // (tokens, K) values of T; blockIdx.y takes R of the tokens
+  const void* x;                   // (tokens, K) values, of T for g and u, else f32; blockIdx.y takes R of the tokens
   const void* w[2];                // rows of the weight, and of the other one
-  void* out;                       // (tokens, rows)
+  void* out;                       // (tokens, rows): f32 hidden values, or the results in T
   int64_t xs, ws[2], os;           // values between rows
   int64_t rows;
   int K, tokens, act, parts;       // parts: warps that share rows, a power of two
@@ -55,6 +57,45 @@ struct Piece<bf16> {
     return __uint_as_float(i & 1 ? u & 0xffff0000u : u << 16);
   }
 };
+
+// As many f32 values as a piece of T holds.  In memory a row is N / 4 runs of a fraction of its length each: the first four values of
+// every piece, then the next four, so that neighbouring lanes read neighbouring 16 bytes.
+template <int N>
+struct Hidden {
+  float4 q[N / 4];
+  static __device__ __forceinline__ int64_t place(int64_t c, int64_t length) {
+    return N == 4 ? c : (c >> 2 & 1) * (length / 2) + (c >> 3) * 4 + (c & 3);
+  }
+  __device__ __forceinline__ float at(int i) const {
+    const float4& p = q[i / 4];
+    return i % 4 == 0 ? p.x : i % 4 == 1 ? p.y : i % 4 == 2 ? p.z : p.w;
+  }
+};
+
+// Those whose first four lie at p and the next `run` behind; zeros where there are none.
+template <int N>
+__device__ __forceinline__ Hidden<N> hidden_at(const float* p, int run, bool there) {
+  Hidden<N> h = {};
+  if (there) {
+#pragma unroll
+    for (int k = 0; k < N / 4; ++k) h.q[k] = *reinterpret_cast<const float4*>(p + k * run);
+  }
+  return h;
+}
+// All but the first `left` become zeros: rows hold whole pieces, and what lies behind their last value was not written.
+template <int R, int N>
+__device__ __forceinline__ void cut(Hidden<N> (&h)[R], int left) {
+#pragma unroll
+  for (int t = 0; t < R; ++t)
+#pragma unroll
+    for (int k = 0; k < N / 4; ++k) {
+      float4& q = h[t].q[k];
+      if (left < 4 * k + 1) q.x = 0.f;
+      if (left < 4 * k + 2) q.y = 0.f;
+      if (left < 4 * k + 3) q.z = 0.f;
+      if (left < 4 * k + 4) q.w = 0.f;
+    }
+}
 
 // Values v[0..N) summed over the warp; lane l ends with the sum of value l % N.
 template <int N>
@@ -90,14 +131,15 @@ __device__ __forceinline__ void finish(const FewArgs& a, const float (*sh)[R * R
       v[k] = 0.f;
       for (int j = 0; j < a.parts; ++j) v[k] += sh[unit * a.parts + j][t * W * ROWS + r * W + k];   // in order
     }
-    T* o = static_cast<T*>(a.out) + (t0 + t) * a.os + at;
-    if constexpr (W == 2) st(o, ff::activate(a.act, v[0], nullptr) * v[1]);
-    else st(o, v[0]);
+    if constexpr (W == 2)
+      static_cast<float*>(a.out)[(t0 + t) * a.os + Hidden<Piece<T>::N>::place(at, a.os)] = ff::activate(a.act, v[0], nullptr) * v[1];
+    else
+      st(static_cast<T*>(a.out) + (t0 + t) * a.os + at, v[0]);
   }
 }
 
-template <typename T, int R, int NR>
-__device__ __forceinline__ void accumulate(float (&sum)[R * NR], const Piece<T> (&x)[R], const Piece<T> (&w)[NR]) {
+template <typename T, int R, int NR, typename X>
+__device__ __forceinline__ void accumulate(float (&sum)[R * NR], const X (&x)[R], const Piece<T> (&w)[NR]) {
 #pragma unroll
   for (int j = 0; j < Piece<T>::N; ++j)
 #pragma unroll
@@ -184,11 +226,13 @@ __global__ void __launch_bounds__(32 * WARPS, Shape<R * ROWS * W>::CTAS) few_ker
   for (int k = 0; k < STAGES - 1; ++k) copy();
   if constexpr (W == 1) ptx::griddep_wait();
   const int tokens = min(R, a.tokens - (int)blockIdx.y * R);
-  const T* x = static_cast<const T*>(a.x) + (int64_t)blockIdx.y * R * a.xs;
+  typedef std::conditional_t<W == 2, T, float> X;
+  const X* x = static_cast<const X*>(a.x) + (int64_t)blockIdx.y * R * a.xs;
   // one load of each 128 bytes of x, all at once: found missing step by step, they would cost the first rows a trip to L2 each
+  const int length = W == 1 ? (int)a.xs : a.K;
   for (int t = 0; t < tokens; ++t)
-    for (int c = threadIdx.x * (128 / (int)sizeof(T)); c < a.K; c += 32 * WARPS * (128 / (int)sizeof(T))) {
-      if constexpr (ALIGNED) {
+    for (int c = threadIdx.x * (128 / (int)sizeof(X)); c < length; c += 32 * WARPS * (128 / (int)sizeof(X))) {
+      if constexpr (ALIGNED || W == 1) {
         uint32_t unused;
         asm volatile("ld.global.ca.b32 %0, [%1];" : "=r"(unused) : "l"(x + t * a.xs + c));
       } else {
@@ -209,12 +253,15 @@ __global__ void __launch_bounds__(32 * WARPS, Shape<R * ROWS * W>::CTAS) few_ker
     }
     for (int s = s0; s < s1; ++s) {
       const int c = s * STEP + lane * Piece<T>::N;
-      Piece<T> v[R], w[NR];
+      std::conditional_t<W == 2, Piece<T>, Hidden<Piece<T>::N>> v[R];
+      Piece<T> w[NR];
 #pragma unroll
       for (int t = 0; t < R; ++t) {
-        v[t].q = make_uint4(0, 0, 0, 0);
-        const T* xt = x + min(t, tokens - 1) * a.xs + c;
-        if constexpr (ALIGNED) {
+        const X* xt = x + min(t, tokens - 1) * a.xs + (W == 1 ? c / (Piece<T>::N / 4) : c);
+        v[t] = {};
+        if constexpr (W == 1) {
+          v[t] = hidden_at<Piece<T>::N>(xt, (int)a.xs / 2, c < a.K);
+        } else if constexpr (ALIGNED) {
           if (c < a.K) v[t].q = *reinterpret_cast<const uint4*>(xt);
         } else if (c + 2 * Piece<T>::N <= a.K) {   // by the 16 bytes that hold them, which end within the row
           const unsigned in = (unsigned)reinterpret_cast<uintptr_t>(xt) & 15;
@@ -227,6 +274,9 @@ __global__ void __launch_bounds__(32 * WARPS, Shape<R * ROWS * W>::CTAS) few_ker
           for (int k = 0; k < Piece<T>::N; ++k) u[k] = c + k < a.K ? xt[k] : T(0.f);
           v[t].q = *reinterpret_cast<const uint4*>(u);
         }
+      }
+      if constexpr (W == 1 && !ALIGNED) {
+        if (a.K - c < Piece<T>::N) cut(v, a.K - c);
       }
       if constexpr (!ALIGNED) __syncwarp();   // the lane in front has read what is copied over
       copy();
@@ -275,11 +325,13 @@ cudaError_t launch_rows(FewArgs a, cudaStream_t st) {
   return launch_dependent(few_kernel<T, R, ROWS, W, ALIGNED>, dim3((unsigned)ctas, passes), 32 * WARPS, smem, 1, st, a);
 }
 
+// Of 3 or 4 tokens' f32 hidden values a warp reads as many bytes as of 4 rows of bf16: 2 rows of the weight against them take 84 us
+// (4096 x 12288), 4 rows 72.
 template <typename T, int W, bool ALIGNED>
 cudaError_t launch_tokens(const FewArgs& a, cudaStream_t st) {
   if (a.tokens == 1) return launch_rows<T, 1, 1, W, ALIGNED>(a, st);
   if (a.tokens == 2) return launch_rows<T, 2, 2, W, ALIGNED>(a, st);
-  if (a.tokens <= 4) return launch_rows<T, 4, 2, W, ALIGNED>(a, st);
+  if (a.tokens <= 4) return launch_rows<T, 4, W == 1 && sizeof(T) == 2 ? 4 : 2, W, ALIGNED>(a, st);
   return launch_rows<T, 8, 2, W, ALIGNED>(a, st);   // 8 at a time
 }
 template <typename T, int W>
