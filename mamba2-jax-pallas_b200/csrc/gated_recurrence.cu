@@ -191,10 +191,12 @@ __device__ __forceinline__ bool meet(bool mine) {
 }
 
 // ---- per-channel and per-value arithmetic --------------------------------------------------
-// e^v within 2 units, where the approximate instruction's 2^-22 would be one error of all of a channel's steps:
-// v = n ln 2 + f in two parts (Cody and Waite), the series up to f^7 (5e-9)
+// e^v of v up to 80, within 2 units, where the approximate instruction's 2^-22 would be one error of all of a channel's steps:
+// v = n ln 2 + f in two parts (Cody and Waite), the series up to f^7 (5e-9).  0 where e^v is below 2^-126, however far: the series
+// holds for what v is reduced to, so v is cut off before that.  NaN stays.
 __device__ __forceinline__ float exp_near(float v) {
-  const float n = rintf(fminf(fmaxf(v, -100.f), 100.f) * LOG2E);
+  v = v < -100.f ? -100.f : v;
+  const float n = rintf(v * LOG2E);
   const float f = fmaf(n, -3.1946183e-5f, fmaf(n, -0.693115234375f, v));   // n times the first is exact
   const float p = fmaf(f, fmaf(f, fmaf(f, fmaf(f, fmaf(f, fmaf(f, fmaf(f, 1.f / 5040, 1.f / 720), 1.f / 120), 1.f / 24), 1.f / 6), 0.5f), 1.f), 1.f);
   return p * exp2f(n);

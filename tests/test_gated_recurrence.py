@@ -247,6 +247,40 @@ def test_saturated_gates():
         assert e <= 1e-5 * float(refs[1][..., c].norm()) + 1e-30, c
 
 
+FAR = [-104.0, -1e3, -1.2e6, -1e7, -1e9, torch.finfo(torch.float32).min, -math.inf]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_decays_that_keep_everything(dtype):
+    """softplus(decay) below float32's smallest number: a is 1 and b is 0 (the formula's b is below 1e-21), whatever the gates."""
+    n, b, L = len(FAR), 2, 70
+    x, r, i, _, h0, dy, df = inputs(b, L, 3 * n, dtype, seed=21)
+    r[0, 10:20], r[1, 30:40] = 200.0, -200.0
+    lam = torch.tensor([v for f in FAR for v in (f, -5.0, f)])     # beside channels that decay, alike in both lanes of a pair
+    ref = loop(x, r, i, lam, h0)[0]
+    bound = (22 * E + lives(torch.tensor([-5.0])) * U) * magnitude(x, r, i, lam, h0, None, 8.0)[0]
+    y, final = gated_recurrence(*cuda(x, r, i, lam), initial_state=h0.cuda(), return_final_state=True)
+    close(y, ref, bound + 1e-18, dtype)
+    close(final, ref[:, -1], bound[:, -1] + 1e-18, "f32")
+    new, one = gated_recurrence_update(h0.cuda(), *cuda(x[:, 0], r[:, 0], i[:, 0], lam))
+    close(new, ref[:, 0], 24 * E * magnitude(x, r, i, lam, h0, None, 8.0)[0][:, 0] + 1e-18, "f32")
+    close(one, ref[:, 0], 24 * E * magnitude(x, r, i, lam, h0, None, 8.0)[0][:, 0] + 1e-18, dtype)
+    got = gated_recurrence_grad(*cuda(x, r, i, lam, dy), initial_state=h0.cuda(), grad_final_state=df.cuda())
+    keep = torch.tensor([v != -5.0 for v in lam.tolist()])
+    assert torch.equal(final.cpu()[:, keep], h0[:, keep]) and torch.equal(new.cpu()[:, keep], h0[:, keep])
+    for k in range(3):
+        assert float(got[k][..., keep].abs().max()) <= 1e-18
+    assert float(got[3][keep].abs().max()) <= 1e-18
+    want = dy.double().sum(1) + df.double()
+    close(got[4].cpu()[:, keep], want[:, keep], (L + 1) * U * (dy.double().abs().sum(1) + df.double().abs())[:, keep], "f32", norm=False)
+    short = [g.cpu()[..., ~keep] for g in got[:3]]
+    refs, sizes = loop_grad(x[..., ~keep], r[..., ~keep], i[..., ~keep], lam[~keep], h0[:, ~keep], dy[..., ~keep], df[:, ~keep])
+    for k in range(3):
+        # (2^-126: the closed gate's sigmoid(-200) = 1e-87 and its root 1e-44, and with them their gradients, are below float32's range)
+        close(short[k], refs[k], 8 * (22 * E + lives(lam[~keep]) * U) * sizes[k] + 2.0 ** -126, dtype, norm=False)
+
+
 @gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_strides_and_broadcasts(dtype):
