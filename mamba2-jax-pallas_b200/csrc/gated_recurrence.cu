@@ -202,6 +202,12 @@ __device__ __forceinline__ float exp_near(float v) {
   return p * exp2f(n);
 }
 __device__ __forceinline__ float softplus(float v) { return v > 20.f ? v : log1pf(exp_near(v)); }
+// A channel's k.  Beyond float32 it is 2^127, not infinite: a closed gate's sigmoid is 0, and 0 times it has to be 0 (the steps behind
+// the last token are closed gates, and so are gates below -88).  NaN stays.
+__device__ __forceinline__ float rate_of(float scale, float decay) {
+  const float k = scale * softplus(decay);
+  return k > 0x1p127f ? 0x1p127f : k;
+}
 
 // 1 / (1 + e^-v); 0 where e^-v is beyond 2^126.  (Two at once by one reciprocal of the product need a second form for large
 // products, whose registers cost more than the special-function unit's share: 249 -> 273 us.)
@@ -487,7 +493,7 @@ template <typename T>
 __device__ __forceinline__ Rate<typename Lane<T>::V> rates(const Args& a, int64_t c, bool* near) {
   typedef typename Lane<T>::V V;
   const V lam = Lane<T>::load(a.decay, c, a.D, -1000.f);   // (channels beyond the last decay by nothing)
-  const V k = each(lam, [&](float v) { return a.scale * softplus(v); });
+  const V k = each(lam, [&](float v) { return rate_of(a.scale, v); });
   bool ok = true;
   each(k, [&](float v) { ok = ok && v <= 0.25f; return v; });
   *near = __all_sync(0xffffffffu, ok);
@@ -863,7 +869,7 @@ __global__ void __launch_bounds__(256) step_kernel(const StepArgs a) {
   if (c >= a.D) return;
   float nk[VEC];
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) nk[i] = -a.scale * LOG2E * softplus(a.decay[c + i]);
+  for (int i = 0; i < VEC; ++i) nk[i] = -LOG2E * rate_of(a.scale, a.decay[c + i]);
   const int64_t r1 = min(r0 + a.rows, a.batch);
   const T* x = static_cast<const T*>(a.in[0]) + c;
   const T* r = static_cast<const T*>(a.in[1]) + c;

@@ -283,6 +283,49 @@ def test_decays_that_keep_everything(dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("packed", [False, True])
+def test_decays_that_keep_nothing(dtype, packed):
+    """scale * softplus(decay) beyond float32: a is 0 and b is 1, so that a token gives w = sigmoid(i) x, and every gradient is
+    that token's own.  (70 tokens end inside a tile.)"""
+    b, L = 2, 70
+    most = torch.finfo(torch.float32).max
+    lam = torch.tensor([most, 1e38, math.inf, 5e37] * 3 + [most])
+    x, r, i, _, h0, dy, df = inputs(b, L, lam.numel(), dtype, seed=22)
+    seq = torch.zeros((b, L), dtype=torch.int32)
+    seq[0, 33:] = 1
+    kw = dict(initial_state=h0.cuda(), seq_idx=seq.cuda() if packed else None)
+    si = torch.sigmoid(i.double())
+    w = si * x.double()
+    y, final = gated_recurrence(*cuda(x, r, i, lam), return_final_state=True, **kw)
+    close(y, w, E * w.abs(), dtype)
+    close(final, w[:, -1], E * w[:, -1].abs(), "f32")
+    for t in (0, L - 1):
+        new, one = gated_recurrence_update(h0.cuda(), *cuda(x[:, t], r[:, t], i[:, t], lam))
+        close(new, w[:, t], E * w[:, t].abs(), "f32")
+        close(one, w[:, t], E * w[:, t].abs(), dtype)
+    got = gated_recurrence_grad(*cuda(x, r, i, lam, dy), grad_final_state=df.cuda(), **kw)
+    delta = dy.double().clone()
+    delta[:, -1] += df.double()
+    close(got[0], delta * si, E * (delta * si).abs() + 2 * U * delta.abs(), dtype)
+    close(got[2], delta * w * (1 - si), 4 * E * (delta * w).abs(), dtype)
+    for k in (1, 3, 4):
+        assert float(got[k].abs().max()) == 0
+
+
+@gpu
+def test_decays_that_keep_nothing_behind_a_closed_gate():
+    """A gate whose sigmoid is zero in float32 keeps the state, whatever the decay."""
+    x, r, i, _, h0, *_ = inputs(1, 40, 4, seed=23)
+    lam = torch.full((4,), torch.finfo(torch.float32).max)
+    r[:, 5:] = -math.inf
+    y, final = gated_recurrence(*cuda(x, r, i, lam), initial_state=h0.cuda(), return_final_state=True)
+    assert torch.isfinite(y).all() and torch.equal(final, y[:, 4]) and torch.equal(y[:, 5:], y[:, 4:5].expand(1, 35, 4))
+    state, _ = gated_recurrence_update(h0.cuda(), *cuda(x[:, 5], r[:, 5], i[:, 5], lam))
+    assert torch.equal(state.cpu(), h0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_strides_and_broadcasts(dtype):
     """Slices of one fused projection, odd starts, transposed tokens, one row for all tokens."""
     b, L, d = 2, 150, 40
