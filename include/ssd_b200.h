@@ -515,8 +515,9 @@ typedef enum ssd_activation {
 /* Gated feed-forward block: h = act(x . w_gate^T) * (x . w_up^T);  y = h . w_down^T.
  * bf16: products on the tensor cores with f32 accumulation; h (and in the gradients those of the two
  * projections) is rounded once to bf16, as an operand of the products behind it.  f32: every operand as three
- * bf16 terms, six products per pair, with the accuracy of f32 (values below 2^-110 lose digits).  For a few tokens (bf16: 4, f32: 24) the
- * forward products run in f32 on the CUDA cores, and h stays f32. */
+ * bf16 terms, six products per pair, with the accuracy of f32 (values below 2^-110 lose digits).  For a few tokens (bf16: 4; f32: 24, but
+ * of large weights 16 or 8 where rows of the operands start off 16 bytes) the forward products run in f32 on the CUDA cores, and h
+ * stays f32. */
 typedef struct ssd_gated_ff_params {
   int64_t tokens, dim, hidden, dim_out;
   int64_t x_stride_row, w_gate_stride_row, w_up_stride_row, w_down_stride_row; /* in values, at least a row's length */
@@ -529,7 +530,8 @@ typedef struct ssd_gated_ff_params {
   void* y;                    /* (tokens, dim_out) contiguous; unused by the gradient */
 } ssd_gated_ff_params_t;
 
-/* The workspaces start with the device status word (see ssd_status_copy_async). */
+/* The workspaces start with the device status word (see ssd_status_copy_async).  Their sizes go by the sizes, strides and
+ * 16-byte alignment of the operands: ask with the pointers of the call. */
 size_t ssd_gated_ff_workspace_bytes(const ssd_gated_ff_params_t* p);
 int ssd_gated_ff(const ssd_gated_ff_params_t* p, void* workspace, size_t workspace_bytes, ssd_stream_t stream);
 

@@ -332,7 +332,8 @@ cudaError_t launch_tokens(const FewArgs& a, cudaStream_t st) {
   if (a.tokens == 1) return launch_rows<T, 1, 1, W, ALIGNED>(a, st);
   if (a.tokens == 2) return launch_rows<T, 2, 2, W, ALIGNED>(a, st);
   if (a.tokens <= 4) return launch_rows<T, 4, W == 1 && sizeof(T) == 2 ? 4 : 2, W, ALIGNED>(a, st);
-  return launch_rows<T, 8, 2, W, ALIGNED>(a, st);   // 8 at a time
+  if constexpr (sizeof(T) == 4) return launch_rows<T, 8, 2, W, ALIGNED>(a, st);   // 8 at a time
+  return cudaErrorInvalidValue;
 }
 template <typename T, int W>
 cudaError_t launch_tokens(const FewArgs& a, bool aligned, cudaStream_t st) {
@@ -344,6 +345,18 @@ size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 template <typename T>
 bool aligned16(const void* p, int64_t stride, int64_t rows) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows == 1 || stride * sizeof(T) % 16 == 0);
+}
+
+// Whether x, the rows of w_gate and w_up, and those of w_down start at 16 bytes, the weights' rows in whole pieces.
+struct Starts {
+  bool x, in, down;
+};
+template <typename T>
+Starts starts_of(const ssd_gated_ff_params_t* p) {
+  constexpr int N = Piece<T>::N;
+  return {aligned16<T>(p->x, p->x_stride_row, p->tokens),
+          p->dim % N == 0 && aligned16<T>(p->w_gate, p->w_gate_stride_row, p->hidden) && aligned16<T>(p->w_up, p->w_up_stride_row, p->hidden),
+          p->hidden % N == 0 && aligned16<T>(p->w_down, p->w_down_stride_row, p->dim_out)};
 }
 
 template <typename T>
@@ -359,9 +372,8 @@ cudaError_t launch_as(const ssd_gated_ff_params_t* p, uint8_t* ws, cudaStream_t 
   a.tokens = (int)p->tokens;
   a.act = p->activation;
   a.status = reinterpret_cast<unsigned*>(ws);
-  constexpr int N = Piece<T>::N;
-  cudaError_t e = launch_tokens<T, 2>(a, p->dim % N == 0 && aligned16<T>(p->x, a.xs, p->tokens) && aligned16<T>(p->w_gate, a.ws[0], a.rows) &&
-                                            aligned16<T>(p->w_up, a.ws[1], a.rows), st);
+  const Starts s = starts_of<T>(p);
+  cudaError_t e = launch_tokens<T, 2>(a, s.x && s.in, st);
   *at = "gate and up";
   if (e != cudaSuccess) return e;
   a.x = ws + 256; a.xs = ldh;
@@ -372,17 +384,23 @@ cudaError_t launch_as(const ssd_gated_ff_params_t* p, uint8_t* ws, cudaStream_t 
   a.K = (int)p->hidden;
   a.status = nullptr;
   *at = "down";
-  return launch_tokens<T, 1>(a, p->hidden % N == 0 && aligned16<T>(p->w_down, a.ws[0], a.rows), st);
+  return launch_tokens<T, 1>(a, s.down, st);
 }
 
 }  // namespace
 
-// bf16: up to 4 tokens (2560 x 7680: 4 tokens 37 us, by the products 42; 8 tokens 63 and 42).  f32: up to 24, 8 at a time (8 tokens 80
-// us, 16 143, 24 207, by the products 252: their operands have to be split first); where rows start off 16 bytes, and the shifting of
-// every pass costs more than the weights' bytes, up to 8 (2559 x 7681: 16 tokens 323, by the products 259).
+// bf16: up to 4 tokens (2560 x 7680: 4 tokens 36 us, by the products 42; 8 tokens 63 and 42).  f32: up to 24, 8 to a pass, where the
+// passes take less than the products, whose operands have to be split first.  Both in us, fitted to 768 x 2048, 4096 x 4096, 2560 x 7680 and
+// 4096 x 12288 of 8 to 25 tokens.  Rows that start off 16 bytes are shifted into place in every pass, those of x once more for every row of a
+// weight.  2560 x 7680, 8, 16 and 24 tokens: 79, 145, 209, by the products 252; w_down off 16 bytes 87, 164, 236; w_gate and w_up 111, 208,
+// 273; x 185, 340, 492.
 bool gated_ff_is_few(const ssd_gated_ff_params_t* p) {
   if (p->dtype == SSD_DTYPE_BF16) return p->tokens <= 4;
-  return p->tokens <= (p->w_gate_stride_row % 4 || p->w_up_stride_row % 4 || p->w_down_stride_row % 4 ? 8 : 24);
+  if (p->tokens > 24) return false;
+  const Starts s = starts_of<float>(p);
+  const double size = (2e-6 / 3 * (double)p->dim + 1e-6 / 3 * (double)p->dim_out) * (double)p->hidden;   // millions of values of a weight
+  const double pass = (3.3 + (s.down ? 0 : 0.6) + (!s.x ? 4.3 : !s.in ? 1.3 : 0)) * size + (s.x ? 6 : 9);
+  return (double)((p->tokens + 7) / 8) * pass <= 45 + 10.4 * size;
 }
 
 size_t gated_ff_few_workspace(const ssd_gated_ff_params_t* p) { return 256 + up256((size_t)p->tokens * ((p->hidden + 7) / 8 * 8) * 4); }

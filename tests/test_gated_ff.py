@@ -223,6 +223,53 @@ def test_rows_that_start_anywhere(t, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("t", [5, 8, 9, 16, 17, 24, 25])
+def test_float32_slices_of_wider_rows(t):
+    """Rows of a few tokens and of weights at one distance, a multiple of 16 bytes, whose first starts off 16 bytes: passes of 8 tokens, whole
+    and cut off, and what takes over behind them.  NaN lies around the views."""
+    d, f, o = 777, 251, 21
+    ins = inputs(t, d, f, o, "f32", 19)
+    refs, _ = reference(*ins, "silu", "f32")
+    for at in ((0, 0, 0, 0), (1, 0, 0, 0), (0, 1, 2, 0), (0, 2, 0, 3), (0, 0, 0, 1), (3, 2, 1, 2)):
+        views = []
+        for a, start in zip(ins[:4], at):
+            wide = torch.full((a.shape[0], (a.shape[1] + 7) // 4 * 4), float("nan"), device="cuda")
+            view = wide[:, start:start + a.shape[1]]
+            view.copy_(a)
+            views.append(view)
+        close(gated_feed_forward(*views), *refs[0], "f32")
+
+
+def test_which_form_takes_few_tokens():
+    """The limits go by sizes and by where rows start, base addresses among it; seen by the workspace, which then holds the hidden values alone."""
+    from mamba2_b200 import _lib
+    lib = _lib.load()
+
+    def few(tokens, dtype=0, dim=2560, hidden=7680, **kw):
+        p = _lib.GatedFfParams(tokens, dim, hidden, dim, dim, dim, dim, hidden, dtype, 0, 256, 256, 256, 256, 256)
+        for k, v in kw.items():
+            setattr(p, k, v)
+        size = lib.ssd_gated_ff_workspace_bytes(p)
+        only = 256 + (tokens * ((hidden + 7) // 8 * 8) * 4 + 255) // 256 * 256
+        assert size >= only
+        return size == only
+
+    def limit(**kw):
+        most = max(t for t in range(1, 40) if few(t, **kw))
+        assert all(few(t, **kw) == (t <= most) for t in range(1, 40))
+        return most
+
+    assert limit(dtype=1) == 4 and limit(dtype=1, x=258) == 4
+    assert limit() == 24 and limit(w_down=260) == 24 and limit(w_down_stride_row=7681) == 24
+    assert limit(w_gate=260) == 16 and limit(w_up=264) == 16 and limit(w_up_stride_row=2561) == 16
+    assert limit(x=260) == 8 and limit(x_stride_row=2562) == 8 and limit(x=260, w_gate=260) == 8
+    assert limit(dim=2559, x_stride_row=2560, w_gate_stride_row=2560, w_up_stride_row=2560) == 16
+    assert limit(hidden=7681, w_down_stride_row=7684) == 24
+    small, large = dict(dim=768, hidden=2048), dict(dim=4096, hidden=12288)
+    assert limit(**small, w_up=260) == 24 and limit(**small, x=260) == 16 and limit(**large) == 24 and limit(**large, w_down=260) == 16
+
+
+@gpu
 @pytest.mark.parametrize("act", ["silu", "relu"])
 @pytest.mark.parametrize("t,d,f,o", [(1, 40, 7, 64), (2, 24, 9, 130), (3, 40, 16, 65), (4, 33, 24, 128), (4, 8, 5, 200)])
 def test_few_tokens_round_once(t, d, f, o, act):
