@@ -687,7 +687,7 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) backward_kernel
   bool near;
   const Rate<V> rate = rates<T>(a, c, &near);
   V carry = a.grad_final ? Lane<T>::load(a.grad_final + b * a.D, c, a.D) : all<V>(0.f);
-  V total = all<V>(0.f);
+  V sum = all<V>(0.f), total = all<V>(0.f);   // of delta m: over the turns, and of a turn with what the sum has lost so far
   int64_t at = (b * a.L + t0) * a.D + c;
   const int channels = (int)max((int64_t)0, min((int64_t)CH, a.D - c));
   peers.start();
@@ -813,16 +813,21 @@ __global__ void __launch_bounds__(32 * WARPS, MAX_WARPS / WARPS) backward_kernel
     };
     if (live == STEPS) finish(std::true_type());
     else finish(std::false_type());
+    // What the addition loses stays in total (Kahan): where summands are alike a plain sum rounds the same way each time, and 4096
+    // tokens of a warp were 6e-5 off
+    const V now = add(sum, total);
+    total = fma(fma(sum, all<V>(-1.f), now), all<V>(-1.f), total);
+    sum = now;
     at += ahead * a.D;
     in.turn(ahead);
   }
   // the CTA's sum for the decay, warps in order
   __syncthreads();
-  ends[warp * 32 + lane] = total;
+  ends[warp * 32 + lane] = sum;
   __syncthreads();
   if (warp == 0) {
-    for (int j = 1; j < WARPS; ++j) total = add(total, ends[j * 32 + lane]);
-    Lane<T>::store(a.part + (b * cluster + rank) * a.D, c, a.D, total);
+    for (int j = 1; j < WARPS; ++j) sum = add(sum, ends[j * 32 + lane]);
+    Lane<T>::store(a.part + (b * cluster + rank) * a.D, c, a.D, sum);
     if (a.state_out && rank == 0) Lane<T>::store(a.state_out + b * a.D, c, a.D, carry);
   }
   peers.end();

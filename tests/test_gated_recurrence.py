@@ -325,6 +325,47 @@ def test_decays_that_keep_nothing_behind_a_closed_gate():
 
 
 @gpu
+def test_gradient_of_the_decay_channel_by_channel():
+    """Far negative, moderate and large decays, gates that are all but closed or open: each channel on its own size."""
+    b, L, d = 2, 200, 8
+    x, r, i, lam, h0, dy, df = inputs(b, L, d, seed=24)
+    r[0, 10:40], r[0, 60:90], i[0, 100:120], i[0, 130:150] = -200.0, 200.0, -200.0, 200.0
+    lam = torch.tensor([-80.0, -40.0, -10.0, -3.0, 0.0, 5.0, 30.0, 100.0])
+    refs, sizes = loop_grad(x, r, i, lam, h0, dy, df)
+    got = gated_recurrence_grad(*cuda(x, r, i, lam, dy), initial_state=h0.cuda(), grad_final_state=df.cuda())[3].double().cpu()
+    for c in range(d):
+        # (no state lives through more than the 200 tokens)
+        assert abs(float(got[c] - refs[3][c])) <= 8 * (22 * E + L * U) * float(sizes[3][c]) + 1e-30, c
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_gradient_of_the_decay_over_many_tokens(dtype):
+    """Summands that are all alike, where every addition to a running sum rounds the same way.  Against the same summands of a short
+    row, so that nothing but the sums differs.  8 summands of a turn are added up in float32 (8 u at most, in both), the turns by a compensated
+    sum (2 u), and warps and CTAs join by 16 additions at most (16 u in both); a state or a gradient that another order of steps rounds
+    otherwise moves a summand by 8 u: 96 u takes that in.  (One running sum of 4096 would be off by up to 2000 u.)"""
+    L, d = 16384, 18944 if dtype == "f32" else 37888
+    g = torch.Generator(device="cuda").manual_seed(25)
+
+    def row(lo, hi):
+        return (lo + (hi - lo) * torch.rand((1, 1, d), generator=g, device="cuda")).to(DT[dtype])
+
+    x, r, i, dy = row(0.5, 1.5), row(-1, 1), row(-1, 1), row(0.5, 1.5)
+    lam = torch.linspace(-1.5, 0.0, d, device="cuda")    # a between 0.1 and 0.6 of the state is kept
+
+    def rows(n):
+        return [t.expand(1, n, d) for t in (x, r, i)] + [lam]
+
+    # the state, and the gradient that reaches it, where neither moves any more
+    h = gated_recurrence(*rows(256), return_final_state=True)[1]
+    c = gated_recurrence_grad(*rows(256), dy.expand(1, 256, d), initial_state=h)[4]
+    sums = [gated_recurrence_grad(*rows(n), dy.expand(1, n, d), initial_state=h, grad_final_state=c)[3].double() / n for n in (64, L)]
+    assert float(sums[0].abs().min()) > 1e-3
+    assert float(((sums[1] - sums[0]) / sums[0]).abs().max()) <= 96 * U
+
+
+@gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_strides_and_broadcasts(dtype):
     """Slices of one fused projection, odd starts, transposed tokens, one row for all tokens."""
