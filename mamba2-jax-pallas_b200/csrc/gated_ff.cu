@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackA
 struct HiddenArgs {
   int rows;                        // T
   int64_t F, ld;                   // rows of h, dg, du and dh are ld values long, a multiple of 64
-  uint8_t* h;                      // planes of (T, ld) bf16, `plane` bytes apart
+  uint8_t* h;                      // planes of (T, ld) bf16, `plane` bytes apart; backward NULL where no product reads it
   uint8_t* dg;
   uint8_t* du;
   int64_t plane;
@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(THREADS, 1) hidden_kernel(const __grid_constan
                               gemm::pack_bf16(v[c0 + 8 * i + 4], v[c0 + 8 * i + 5]), gemm::pack_bf16(v[c0 + 8 * i + 6], v[c0 + 8 * i + 7]));
           store_block(stage, h, a.h, a.ld, row0, a.rows, f0, a.F);
         } else {
-          store_block(stage, h, a.h, a.ld, row0, a.rows, f0, a.F);
+          if (a.h) store_block(stage, h, a.h, a.ld, row0, a.rows, f0, a.F);
 #pragma unroll
           for (int which = 0; which < 2; ++which) {
             const float* x = v + 32 * which + c0;
@@ -497,13 +497,15 @@ __global__ void __launch_bounds__(THREADS, 1) hidden_kernel(const __grid_constan
           }
         };
         if constexpr (BACKWARD) {
-          float x[COLS];
+          if (a.h) {
+            float x[COLS];
 #pragma unroll
-          for (int i = 0; i < COLS; i += 4) {
-            const float4 d = *reinterpret_cast<const float4*>(stage + gemm::epi_at<CHUNKS / 4>(lane, i / 4));
-            x[i] = d.x; x[i + 1] = d.y; x[i + 2] = d.z; x[i + 3] = d.w;
+            for (int i = 0; i < COLS; i += 4) {
+              const float4 d = *reinterpret_cast<const float4*>(stage + gemm::epi_at<CHUNKS / 4>(lane, i / 4));
+              x[i] = d.x; x[i + 1] = d.y; x[i + 2] = d.z; x[i + 3] = d.w;
+            }
+            put(x, a.h);
           }
-          put(x, a.h);
           put(v + c0, a.dg);
           put(v + 32 + c0, a.du);
         } else {
@@ -696,9 +698,12 @@ struct Inputs {
   int n;
 };
 
+// Whether a call needs dg and du, so dh as well; the gradient of w_down alone needs h, as the forward pass makes it.
+bool goes_back(const ssd_gated_ff_grads_t* g) { return g && (g->grad_x || g->grad_w_gate); }
+
 Inputs inputs_of(const ssd_gated_ff_params_t* p, const ssd_gated_ff_grads_t* g) {
   Inputs in{};
-  const void* ptr[5] = {p->x, p->w_gate, p->w_up, p->w_down, g ? g->grad_y : nullptr};
+  const void* ptr[5] = {p->x, p->w_gate, p->w_up, g && !goes_back(g) ? nullptr : p->w_down, g ? g->grad_y : nullptr};   // NULL: not read
   const int64_t stride[5] = {p->x_stride_row, p->w_gate_stride_row, p->w_up_stride_row, p->w_down_stride_row, g ? g->grad_y_stride_row : 0};
   const int64_t rows[5] = {p->tokens, p->hidden, p->hidden, p->dim_out, p->tokens};
   const int64_t dim[5] = {p->dim, p->dim, p->dim, p->hidden, p->dim_out};
@@ -722,8 +727,8 @@ Layout layout_of(const ssd_gated_ff_params_t* p, const ssd_gated_ff_grads_t* g) 
   };
   const Inputs in = inputs_of(p, g);
   for (int i = 0; i < in.n; ++i)
-    if (!direct(in.p[i], in.stride[i], p->dtype)) q.in[i] = take((size_t)q.planes * up256((size_t)in.rows[i] * ((in.dim[i] + 7) / 8 * 8) * 2));
-  q.h = take(q.planes * q.plane_h);
+    if (in.p[i] && !direct(in.p[i], in.stride[i], p->dtype)) q.in[i] = take((size_t)q.planes * up256((size_t)in.rows[i] * ((in.dim[i] + 7) / 8 * 8) * 2));
+  if (!g || g->grad_w_down) q.h = take(q.planes * q.plane_h);
   int64_t part = 0;
   auto parts = [&](int step) {
     const Plan s = plan_of(step, p);
@@ -732,10 +737,12 @@ Layout layout_of(const ssd_gated_ff_params_t* p, const ssd_gated_ff_grads_t* g) 
   if (!g) {
     parts(Y);
   } else {
-    q.dg = take(q.planes * q.plane_h);
-    q.du = take(q.planes * q.plane_h);
-    q.dh = take((size_t)p->tokens * q.ldf * 4);
-    parts(DH);
+    if (goes_back(g)) {
+      q.dg = take(q.planes * q.plane_h);
+      q.du = take(q.planes * q.plane_h);
+      q.dh = take((size_t)p->tokens * q.ldf * 4);
+      parts(DH);
+    }
     if (g->grad_x) parts(DX);
     if (g->grad_w_gate) parts(DW_IN);
     if (g->grad_w_down) parts(DW_OUT);
@@ -859,14 +866,18 @@ cudaError_t launch_gated_ff(const ssd_gated_ff_params_t* p, const ssd_gated_ff_g
   const Layout q = layout_of(p, g);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   unsigned* status = reinterpret_cast<unsigned*>(ws);
+  if (g && !goes_back(g) && !g->grad_w_down) {   // nothing is wanted
+    FF_CHECK(cudaMemsetAsync(status, 0, sizeof(*status), st), "status");
+    return cudaSuccess;
+  }
   const bool bf = p->dtype == SSD_DTYPE_BF16;
   const Inputs in = inputs_of(p, g);
-  Operand op[5];
+  Operand op[5] = {};
   PackArgs pack{};
   pack.status = status;
   for (int i = 0; i < in.n; ++i) {
     op[i] = {static_cast<const uint8_t*>(in.p[i]), in.rows[i], in.dim[i], in.stride[i], 0};
-    if (direct(in.p[i], in.stride[i], p->dtype)) continue;
+    if (!in.p[i] || direct(in.p[i], in.stride[i], p->dtype)) continue;
     Pack& m = pack.m[pack.n++];
     m.src = in.p[i]; m.stride = in.stride[i]; m.rows = in.rows[i]; m.dim = in.dim[i];
     m.ld = (in.dim[i] + 7) / 8 * 8;
@@ -894,7 +905,7 @@ cudaError_t launch_gated_ff(const ssd_gated_ff_params_t* p, const ssd_gated_ff_g
   ha.rows = (int)p->tokens;
   ha.F = p->hidden;
   ha.ld = q.ldf;
-  ha.h = ws + q.h;
+  ha.h = q.h ? ws + q.h : nullptr;
   ha.plane = (int64_t)q.plane_h;
   const Operand none{};
   if (!g) {
@@ -905,14 +916,15 @@ cudaError_t launch_gated_ff(const ssd_gated_ff_params_t* p, const ssd_gated_ff_g
   }
   const Operand& dy = op[4];
   const Operand dg = middle(q.dg), du = middle(q.du);
-  {
+  if (goes_back(g)) {
     const Operand a[2] = {dy, none}, b[2] = {wd, none};
     FF_CHECK((product<false, true, ONE>(q.planes, plan_of(DH, p), a, b, ws + q.dh, (void*)nullptr, false, q.ldf, part, clear, status, st)), "grad_hidden");
+    clear = false;
+    ha.dg = ws + q.dg;
+    ha.du = ws + q.du;
+    ha.dh = reinterpret_cast<const float*>(ws + q.dh);
   }
-  ha.dg = ws + q.dg;
-  ha.du = ws + q.du;
-  ha.dh = reinterpret_cast<const float*>(ws + q.dh);
-  FF_CHECK(hidden_as(q.planes, p->tokens, p, q, x, wg, wu, ha, false, status, st), "gate and up");
+  FF_CHECK(hidden_as(q.planes, p->tokens, p, q, x, wg, wu, ha, clear, status, st), "gate and up");
   if (g->grad_x) {
     const Operand a[2] = {dg, du}, b[2] = {wg, wu};
     FF_CHECK((product<false, true, TWO_K>(q.planes, plan_of(DX, p), a, b, g->grad_x, (void*)nullptr, bf, p->dim, part, false, status, st)), "grad_x");

@@ -181,6 +181,55 @@ def test_what_is_not_needed_is_none():
     assert gated_feed_forward_grad(*c, need_input_grad=False, need_weight_grad=False) == (None,) * 4
 
 
+def grad_params(c, **kw):
+    """The C call's structs for x, w_gate, w_up, w_down, grad_y and the gradients' tensors that are wanted."""
+    from mamba2_b200 import _lib
+    x, wg, wu, wd, dy = c
+    (t, d), (f, _), o = x.shape, wg.shape, wd.shape[0]
+    code = int(x.dtype == torch.bfloat16)
+    p = _lib.GatedFfParams(t, d, f, o, d, d, d, f, code, 0, *(a.data_ptr() for a in (x, wg, wu, wd)), None)
+    ptr = [None if kw.get(n) is None else kw[n].data_ptr() for n in ("grad_x", "grad_w_gate", "grad_w_up", "grad_w_down")]
+    return p, _lib.GatedFfGrads(o, dy.data_ptr(), *ptr, code, 0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_what_is_not_needed_takes_no_workspace(dtype):
+    """h is there for w_down's gradient alone, dg, du and dh are for the others."""
+    from mamba2_b200 import _lib
+    size = _lib.load().ssd_gated_ff_grad_workspace_bytes
+    c = [torch.empty(s, dtype=DT[dtype]) for s in ((1000, 64), (128, 64), (128, 64), (64, 128), (1000, 64))]
+    g = dict(zip(("grad_x", "grad_w_gate", "grad_w_up", "grad_w_down"), c))
+    plane = 1000 * 128 * 2 * (3 if dtype == "f32" else 1)
+    need = {k: size(*grad_params(c, **{n: g[n] for n in names})) for k, names in dict(
+        all=list(g), x=["grad_x"], in_=["grad_w_gate", "grad_w_up"], down=["grad_w_down"]).items()}
+    assert need["all"] - need["x"] >= plane and need["all"] - need["in_"] >= plane
+    assert need["all"] - need["down"] >= 2 * plane + 1000 * 128 * 4
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("t,d,f,o", [(3, 40, 24, 16), (140, 96, 72, 64), (300, 65, 130, 9)])
+def test_each_gradient_alone(t, d, f, o, dtype):
+    """Through the C entry point, which takes any of them; workspaces full of NaN; the status word is cleared in any case."""
+    from mamba2_b200 import _lib
+    lib = _lib.load()
+    ins, refs = separated(t, d, f, o, dtype, "silu", 20)
+    c = [a.cuda() for a in ins]
+    names = ("grad_x", "grad_w_gate", "grad_w_up", "grad_w_down")
+    full = dict(zip(names, gated_feed_forward_grad(*c)))
+    ref = dict(zip(names, refs[1:]))
+    for wanted in (("grad_x",), ("grad_w_gate", "grad_w_up"), ("grad_w_down",), ("grad_x", "grad_w_down"), ()):
+        out = {n: torch.full_like(full[n], float("nan")) for n in wanted}
+        p, g = grad_params(c, **out)
+        ws = torch.full((max(lib.ssd_gated_ff_grad_workspace_bytes(p, g), 256),), 255, dtype=torch.uint8, device="cuda")
+        _lib.check(lib.ssd_gated_ff_grad(p, g, ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream))
+        _lib.check_device_status(ws)
+        for n in wanted:
+            close(out[n], *ref[n], dtype)
+            if n != "grad_w_down":
+                assert torch.equal(out[n], full[n]), n
+
+
 @gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("t", [2, 7, 40, 150])
