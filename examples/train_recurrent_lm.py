@@ -14,7 +14,8 @@ and back, with the projections' gradients as plain products:
 
 Rows hold several documents, packed (seq_idx): no state crosses from one to the next.  The gradients go through
 clip_grad_norm into float32 buffers for an Adam step on float32 master weights.  Decoding keeps one state per layer:
-gated_recurrence's final state after the prompt, then gated_recurrence_update token by token.
+gated_recurrence's final state after the prompt, then gated_recurrence_update token by token.  A prompt that is cut
+out of packed rows takes their seq_idx along, so that each row is continued from its last document alone.
 
 The data are synthetic: a random first-order chain over the vocabulary.
 
@@ -115,6 +116,17 @@ class Model:
         return h
 
 
+def generate(model, prompt, count, seq_idx=None):
+    """``count`` ids that continue each row of the prompt, the likeliest first."""
+    states, out = [], []
+    h = model.forward(prompt, seq_idx, states=states)[:, -1]
+    for _ in range(count):
+        last = (h @ model.p["head"].t()).argmax(dim=-1)
+        out.append(last)
+        h = model.step(last, states)
+    return torch.stack(out, 1)
+
+
 def documents(vocab, rows, length, gen):
     """Packed rows of a chain in which each id is followed by one of four: ids, targets, seq_idx."""
     follow = torch.randint(0, vocab, (vocab, 4), generator=gen, device="cuda")
@@ -155,14 +167,7 @@ def main(steps=30, vocab=4099, dim=512, layers=2, rows=4, length=256, lr=3e-3, v
     model = Model(masters)
     ids, targets, seq = draw()
     held_out = model.loss(ids, targets, seq)
-    # continue a prompt: its final states, then single tokens
-    states, out = [], []
-    h = model.forward(ids[:, :64].contiguous(), states=states)[:, -1]
-    for _ in range(8):
-        last = (h @ model.p["head"].t()).argmax(dim=-1)
-        out.append(last)
-        h = model.step(last, states)
-    out = torch.stack(out, 1)
+    out = generate(model, ids[:, :64].contiguous(), 8, seq[:, :64].contiguous())
     if verbose:
         print(f"held-out loss {float(held_out):.4f}; continuation of row 0: {out[0].tolist()}")
     return torch.stack(losses), held_out, out

@@ -13,6 +13,8 @@ import sys
 import pytest
 import torch
 
+from mamba2_b200 import gated_recurrence
+
 pytestmark = pytest.mark.gpu
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
 
@@ -98,3 +100,40 @@ def test_steps_continue_the_forward_pass():
     for t in range(30, 40):
         h = model.step(ids[:, t].contiguous(), states)
         assert float((h - whole[:, t]).norm() / whole[:, t].norm()) <= 4e-5
+
+
+def test_no_call_of_the_example_drops_its_sequences(monkeypatch):
+    """Training, the held-out loss and the prompt all work on packed rows: every call names their sequences."""
+    import train_recurrent_lm as example
+    calls = []
+
+    def recurrence(v, *args, **kw):
+        seq = kw.get("seq_idx")
+        calls.append(seq is not None and tuple(seq.shape) == tuple(v.shape[:2]))
+        return gated_recurrence(v, *args, **kw)
+
+    monkeypatch.setattr(example, "gated_recurrence", recurrence)
+    example.main(steps=2, vocab=67, dim=64, layers=2, rows=2, length=100, verbose=False)
+    assert len(calls) == 2 * (2 + 1 + 1) and all(calls)
+
+
+def test_packed_prompt_continues_its_last_document():
+    """The states after a packed prompt, and what follows from them, are those of each row's last document alone.  (float32;
+    the same steps in other tiles: each layer's states are within 4e-5, as in the test above.)"""
+    import train_recurrent_lm as example
+    model = example.Model(example.init(61, 32, 2, hidden=48, seed=7), torch.float32)
+    ids = torch.randint(0, 61, (3, 50), generator=torch.Generator().manual_seed(8)).cuda()
+    seq = torch.zeros((3, 50), dtype=torch.int32, device="cuda")
+    last = (20, 0, 49)                    # where each row's last document starts
+    seq[0, 7:], seq[0, 20:], seq[2, 49:] = 1, 2, 1
+    packed_states = []
+    h = model.forward(ids, seq, states=packed_states)
+    follow = example.generate(model, ids, 6, seq)
+    for row, start in enumerate(last):
+        alone = ids[row:row + 1, start:].contiguous()
+        states = []
+        end = model.forward(alone, states=states)[0, -1]
+        assert float((h[row, -1] - end).norm() / end.norm()) <= 4e-5
+        for p, q in zip(packed_states, states):
+            assert float((p[row] - q[0]).norm() / q[0].norm()) <= 4e-5
+        assert torch.equal(follow[row], example.generate(model, alone, 6)[0])
