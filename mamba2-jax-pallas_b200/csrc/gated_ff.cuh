@@ -18,7 +18,7 @@ __device__ __forceinline__ float activate(float g, float* slope) {
     if (slope) *slope = fmaf(g * exp2f(g * g * -0.72134752044448170f), 0.39894228040143268f, p);
     return g * p;
   } else if constexpr (ACT == SSD_ACT_GELU_TANH) {   // (1 + tanh z) / 2 = sigmoid(2 z)
-    const float k = 1.5957691216057308f, q = g * g;   // 2 sqrt(2 / pi)
+    const float k = 1.5957691216057308f, q = fminf(g * g, 1e30f);   // 2 sqrt(2 / pi); beyond 1e15 p is 0 or 1, and 0 times q has to be 0
     const float p = sigmoid(k * g * fmaf(0.044715f, q, 1.f));
     if (slope) *slope = fmaf(g * p * (1.f - p), k * fmaf(3.f * 0.044715f, q, 1.f), p);
     return g * p;

@@ -155,6 +155,27 @@ def test_activations(t, act, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("t", [2, 200])
+def test_gates_of_any_size(t, act, dtype):
+    """g from 2^3 to 2^100 (its square is beyond float32) either way, u = 1: act(g) is g or 0 and its slope 1 or 0, up to
+    (1 + |g|) e^-|g| (silu; the others are nearer)."""
+    size = torch.tensor([2.0 ** 70, 2.0 ** 100]) if t == 2 else 2.0 ** torch.arange(3, 101).repeat(3)[:t].float()
+    tail = ((1 + size.double()) * torch.exp(-size.double()) * 1.001 + 1e-30)[:, None]
+    for sign in (1.0, -1.0):
+        x = torch.stack([sign * size, torch.ones(t)], 1).to(DT[dtype]).cuda()
+        wg, wu, wd = (torch.tensor([row], device="cuda").to(DT[dtype]) for row in ([1.0, 0.0], [0.0, 1.0], [1.0]))
+        dy = torch.ones((t, 1), dtype=DT[dtype], device="cuda")
+        y = gated_feed_forward(x, wg, wu, wd, activation=act).double().cpu()
+        dx = gated_feed_forward_grad(x, wg, wu, wd, dy, activation=act)[0].double().cpu()
+        on = 1.0 if sign > 0 else 0.0
+        for got, want in ((y, on * size.double()[:, None]), (dx, on * torch.stack([torch.ones(t), size], 1).double())):
+            assert torch.isfinite(got).all()
+            assert float(((got - want).abs() - (V * want + tail)).max()) <= 0
+
+
+@gpu
 @pytest.mark.parametrize("dtype,wd", [("bf16", torch.float32), ("f32", torch.bfloat16)])
 def test_weight_grad_dtype(dtype, wd):
     ins, refs = separated(140, 96, 72, 64, dtype, "silu", 3)
