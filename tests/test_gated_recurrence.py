@@ -179,6 +179,31 @@ def test_packed_sequences(ends, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("near", [True, False])
+@pytest.mark.parametrize("b,L,d", [(1, 2000, 64), (1, 4000, 64), (2, 2049, 64), (3, 1500, 256), (16, 300, 1024)])
+def test_packed_sequences_of_few_channels(b, L, d, near, dtype):
+    """Few rows and channels take CTAs of 8 and 16 warps in clusters of up to 16, where no pass has more than one turn or a few; sequences
+    start on both sides of their tiles' ends and anywhere between.  Decays that leave a near 1, and larger ones."""
+    x, r, i, lam, h0, dy, df = inputs(b, L, d, dtype, seed=L + b)
+    if not near:
+        lam = torch.linspace(-3.0, 1.0, d)
+    g = torch.Generator().manual_seed(26)
+    ends = torch.rand((b, L), generator=g) < 0.004
+    ends[0, ::256], ends[-1, 127::256], ends[0, 129::512], ends[:, 0] = True, True, True, False
+    seq = torch.cumsum(ends, 1).to(torch.int32)
+    n = 22 * E + lives(lam) * U
+    y, final = gated_recurrence(*cuda(x, r, i, lam), initial_state=h0.cuda(), seq_idx=seq.cuda(), return_final_state=True, check_status=True)
+    ref, bound = loop(x, r, i, lam, h0, seq)[0], n * magnitude(x, r, i, lam, h0, seq, 8.0)[0]
+    close(y, ref, bound, dtype)
+    close(final, ref[:, -1], bound[:, -1], "f32")
+    refs, sizes = loop_grad(x, r, i, lam, h0, dy, df, seq)
+    got = gated_recurrence_grad(*cuda(x, r, i, lam, dy), initial_state=h0.cuda(), seq_idx=seq.cuda(), grad_final_state=df.cuda(), check_status=True)
+    for k in range(5):
+        close(got[k], refs[k], 8 * n * sizes[k], dtype if k < 3 else "f32", norm=k < 3)
+
+
+@gpu
 def test_every_token_its_own_sequence():
     x, r, i, lam, h0, dy, _ = inputs(1, 130, 32, seed=5)
     seq = torch.arange(130, dtype=torch.int64)[None]
