@@ -515,7 +515,8 @@ typedef enum ssd_activation {
 /* Gated feed-forward block: h = act(x . w_gate^T) * (x . w_up^T);  y = h . w_down^T.
  * bf16: products on the tensor cores with f32 accumulation; h (and in the gradients those of the two
  * projections) is rounded once to bf16, as an operand of the products behind it.  f32: every operand as three
- * bf16 terms, six products per pair, with the accuracy of f32 (values below 2^-110 lose digits).  For a few tokens (bf16: 4; f32: 24, but
+ * bf16 terms, six products per pair, with the accuracy of f32 (values below 2^-110 lose digits; an infinity, or an h above
+ * 3.396e38, becomes NaN wherever it is read: what is left of it for the second term is).  For a few tokens (bf16: 4; f32: 24, but
  * of large weights 16 or 8 where rows of the operands start off 16 bytes) the forward products run in f32 on the CUDA cores, and h
  * stays f32. */
 typedef struct ssd_gated_ff_params {

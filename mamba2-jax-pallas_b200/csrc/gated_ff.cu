@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(THREADS, 1) hidden_kernel(const __grid_constan
           }
         }
       } else {
-        // three planes of one result after another (hidden values above 3.389e38 count as infinite)
+        // three planes of one result after another (hidden values above 3.396e38 count as infinite)
         auto put = [&](float* x, uint8_t* out) {
 #pragma unroll
           for (int k = 0; k < PLANES; ++k) {

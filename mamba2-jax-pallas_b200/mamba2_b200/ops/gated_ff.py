@@ -51,7 +51,10 @@ def gated_feed_forward(x, w_gate, w_up, w_down, *, activation: str = "silu", che
     x (..., dim), w_gate and w_up (hidden, dim) and w_down (dim_out, hidden) of one dtype, float32 or
     bfloat16; the weights may be row slices of a larger one.  ``activation`` is "silu", "gelu", "gelu_tanh" or "relu".
     Returns (..., dim_out) in x's dtype: products summed in float32, the hidden values rounded once to x's
-    dtype (float32: not below its own accuracy; bfloat16, up to 4 tokens: kept in float32), the result once.  ``check_status`` waits for the call and raises
+    dtype (float32: not below its own accuracy; bfloat16, up to 4 tokens: kept in float32), the result once.  A
+    value that is not finite makes its row's results so where the formula has them so; in float32 of more than 24
+    tokens (and in its gradients) an infinity, or a hidden value above 3.396e38, gives NaN where the formula keeps an infinity or
+    drops it.  ``check_status`` waits for the call and raises
     ``SsdError`` if a bounded wait inside a kernel gave up.  The result carries no autograd history:
     ``gated_feed_forward_grad`` gives the gradients.
     """

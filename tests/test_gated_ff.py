@@ -405,6 +405,20 @@ def test_values_that_are_not_finite_stay_in_their_rows():
 
 
 @gpu
+@pytest.mark.parametrize("dtype,t", [("f32", 6), ("bf16", 3), ("bf16", 150), ("f32", 150)])
+def test_what_becomes_of_an_infinity(dtype, t):
+    """Where the formula keeps one (nothing negative meets it) it stays one, but for float32 operands in three terms: what is left of it for
+    the second is NaN."""
+    x, w = torch.ones((t, 64)), torch.full((64, 64), 0.125)
+    x[2, 5] = math.inf
+    x, w = x.to(DT[dtype]).cuda(), w.to(DT[dtype]).cuda()
+    y = gated_feed_forward(x, w, w, w)
+    assert (torch.isnan(y[2]) if (dtype, t) == ("f32", 150) else torch.isposinf(y[2])).all()
+    keep = torch.arange(t, device="cuda") != 2
+    assert torch.isfinite(y[keep]).all()
+
+
+@gpu
 def test_large_tiles_against_float64():
     """Several tiles each way, ragged, on the GPU's own float64."""
     for dtype, (t, d, f, o) in (("bf16", (1500, 1024, 1400, 900)), ("f32", (700, 500, 600, 300))):
