@@ -13,8 +13,8 @@
 //
 // Both passes are bound by HBM (8 and 14 bytes per bf16 value), and close behind it by the issue slots and the special-function
 // unit: 32 and 68 instructions and 4 and 5 special functions a value, the gates' above all.  64 x 512 x 5120 bf16: forward 229 us
-// (5.9 TB/s), gradients 454 us (5.2 TB/s).  With few rows and channels the sequence is the only parallelism left: 1 x 32768 x 5120
-// in clusters of 5 forward 325 us (4.1 TB/s), gradients 636 us; 1 x 65536 x 256 102 and 170 us.
+// (5.9 TB/s), gradients 456 us (5.2 TB/s).  With few rows and channels the sequence is the only parallelism left: 1 x 32768 x 5120
+// in clusters of 5 forward 325 us (4.1 TB/s), gradients 642 us; 1 x 65536 x 256 102 and 175 us.  Packed, 16 sequences: 349 and 772.
 //
 // A step is the map h -> a h + b; maps compose, so a run of steps is one pair (P, H).  Warps take 16
 // steps (8 backward) of 128 bytes of channels (a lane: one 32-bit word, 2 bf16 or 1 f32 channel), CTAs
@@ -228,7 +228,9 @@ struct Rate {
 // NEAR, l above -0.36 (a above e^-1/4): 1 - a = l M(l) and b = sqrt(-2 l ln 2) G(l), with polynomials for M = (1 - 2^l) / l and
 // G^2 = (1 - 2^2l) / (-2 l ln 2) through Chebyshev points (1.2e-8 and 9.6e-9 off), so that a is off by its own rounding only; and with
 // s = q^2 the root is sqrt(2 k) q, so that one reciprocal square root serves the sigmoid and b (the special-function unit
-// is what binds the forward pass).
+// is what binds the forward pass).  A warp takes this form where k is at most 1/4 in all its channels, so that no gate leads out of it.
+// 64 x 512 x 5120 bf16: forward 229 us, gradients 456; with k of 5.5 in every channel, by the other form, 332 and 535; with one such channel
+// in every warp's 64, 347 and 562 (f32 x 2560: 208 and 379; 206 and 382; 220 and 395).
 constexpr float NEAR_EXPONENT = -0.25f * LOG2E;
 template <bool NEAR, typename V>
 __device__ __forceinline__ void decay_of(V gate, const Rate<V>& k, V* sig, V* l, V* a, V* b) {
